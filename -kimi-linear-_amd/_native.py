@@ -14,11 +14,12 @@ from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "libkda_hip.so"
 HOST_PATH = Path(__file__).resolve().parent / "_kda_host.so"     # csrc/host_binding.cpp
-ABI_VERSION = 15
+ABI_VERSION = 16
 
 DTYPE_F32 = 0
 DTYPE_F16 = 1
 DTYPE_BF16 = 2
+DTYPE_E4M3 = 3
 
 STATUS_OK = 0
 STATUS_BAD_SHAPE = 2
@@ -146,6 +147,67 @@ class KdaOutputBwdArgs(ctypes.Structure):
     ]
 
 
+class KdaMlaExpandedArgs(ctypes.Structure):
+    """Mirror of ``struct kda_mla_expanded_args`` (include/kda_hip.h)."""
+
+    _fields_ = [
+        ("B", ctypes.c_int64), ("T", ctypes.c_int64), ("S", ctypes.c_int64), ("H", ctypes.c_int64),
+        ("N", ctypes.c_int64), ("P", ctypes.c_int64), ("V", ctypes.c_int64),
+        ("q", ctypes.c_void_p), ("q_stride", _i64x3), ("k", ctypes.c_void_p), ("k_stride", _i64x3),
+        ("k_pe", ctypes.c_void_p), ("k_pe_stride", ctypes.c_int64 * 2), ("v", ctypes.c_void_p), ("v_stride", _i64x3),
+        ("lengths", ctypes.c_void_p), ("starts", ctypes.c_void_p),
+        ("o", ctypes.c_void_p), ("lse", ctypes.c_void_p), ("scale", ctypes.c_float), ("dtype", ctypes.c_int32),
+    ]
+
+
+class KdaMlaExpandedBwdArgs(ctypes.Structure):
+    """Mirror of ``struct kda_mla_expanded_bwd_args`` (include/kda_hip.h)."""
+
+    _fields_ = [
+        ("fwd", KdaMlaExpandedArgs), ("d_o", ctypes.c_void_p), ("d_o_stride", _i64x3),
+        ("dq", ctypes.c_void_p), ("dk", ctypes.c_void_p), ("dk_pe", ctypes.c_void_p), ("dv", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p),
+    ]
+
+
+class KdaMlaAbsorbedArgs(ctypes.Structure):
+    """Mirror of ``struct kda_mla_absorbed_args`` (include/kda_hip.h)."""
+
+    _fields_ = [
+        ("B", ctypes.c_int64), ("T", ctypes.c_int64), ("H", ctypes.c_int64), ("S", ctypes.c_int64),
+        ("R", ctypes.c_int64), ("P", ctypes.c_int64), ("q", ctypes.c_void_p), ("q_stride", _i64x3),
+        ("cache", ctypes.c_void_p), ("cache_stride", ctypes.c_int64 * 2),
+        ("cache_scale", ctypes.c_void_p), ("scale_stride", ctypes.c_int64 * 2),
+        ("lengths", ctypes.c_void_p), ("o", ctypes.c_void_p),
+        ("scale", ctypes.c_float), ("dtype", ctypes.c_int32), ("cache_dtype", ctypes.c_int32),
+        ("workspace", ctypes.c_void_p),
+    ]
+
+
+class KdaMlaAppendArgs(ctypes.Structure):
+    """Mirror of ``struct kda_mla_append_args`` (include/kda_hip.h)."""
+
+    _fields_ = [
+        ("B", ctypes.c_int64), ("T", ctypes.c_int64), ("S", ctypes.c_int64), ("R", ctypes.c_int64),
+        ("P", ctypes.c_int64), ("x", ctypes.c_void_p), ("x_stride", ctypes.c_int64 * 2),
+        ("cache", ctypes.c_void_p), ("cache_stride", ctypes.c_int64 * 2),
+        ("cache_scale", ctypes.c_void_p), ("scale_stride", ctypes.c_int64 * 2),
+        ("lengths", ctypes.c_void_p), ("counts", ctypes.c_void_p), ("norm_weight", ctypes.c_void_p),
+        ("eps", ctypes.c_float), ("x_dtype", ctypes.c_int32), ("cache_dtype", ctypes.c_int32),
+    ]
+
+
+class KdaMlaReadArgs(ctypes.Structure):
+    """Mirror of ``struct kda_mla_read_args`` (include/kda_hip.h)."""
+
+    _fields_ = [
+        ("B", ctypes.c_int64), ("S", ctypes.c_int64), ("R", ctypes.c_int64), ("P", ctypes.c_int64),
+        ("cache", ctypes.c_void_p), ("cache_stride", ctypes.c_int64 * 2),
+        ("cache_scale", ctypes.c_void_p), ("scale_stride", ctypes.c_int64 * 2),
+        ("lengths", ctypes.c_void_p), ("out", ctypes.c_void_p), ("out_dtype", ctypes.c_int32),
+    ]
+
+
 EXPORTED_SYMBOLS = ("kda_chunkwise_fwd", "kda_recurrent_fwd", "kda_chunkwise_fwd_ckpt",
                     "kda_chunkwise_gated_fwd", "kda_recurrent_gated_fwd", "kda_chunkwise_fused_fwd",
                     "kda_chunkwise_long_fwd", "kda_chunkwise_long_workspace_size",
@@ -154,7 +216,9 @@ EXPORTED_SYMBOLS = ("kda_chunkwise_fwd", "kda_recurrent_fwd", "kda_chunkwise_fwd
                     "kda_chunkwise_split_fwd", "kda_chunkwise_split_workspace_size",
                     "kda_prep_fwd", "kda_output_fwd", "kda_linear_fwd", "kda_linear_wgrad",
                     "kda_linear_wgrad_workspace_size", "kda_prep_bwd", "kda_prep_bwd_workspace_size",
-                    "kda_output_bwd", "kda_output_bwd_workspace_size", "kda_status_str", "kda_abi_version")
+                    "kda_output_bwd", "kda_output_bwd_workspace_size", "kda_mla_expanded_fwd", "kda_mla_expanded_bwd",
+                    "kda_mla_expanded_bwd_workspace_size", "kda_mla_absorbed_fwd", "kda_mla_absorbed_workspace_size",
+                    "kda_mla_cache_append", "kda_mla_cache_read", "kda_status_str", "kda_abi_version")
 
 _lib = None
 _host = None
@@ -227,6 +291,14 @@ def load() -> ctypes.CDLL:
         lib.kda_output_bwd.restype = ctypes.c_int
         lib.kda_output_bwd_workspace_size.argtypes = [ctypes.c_int64] * 4
         lib.kda_output_bwd_workspace_size.restype = ctypes.c_size_t
+        for name, args in (("expanded_fwd", KdaMlaExpandedArgs), ("expanded_bwd", KdaMlaExpandedBwdArgs),
+                           ("absorbed_fwd", KdaMlaAbsorbedArgs), ("cache_append", KdaMlaAppendArgs),
+                           ("cache_read", KdaMlaReadArgs)):
+            getattr(lib, f"kda_mla_{name}").argtypes = [ctypes.POINTER(args), ctypes.c_void_p]
+            getattr(lib, f"kda_mla_{name}").restype = ctypes.c_int
+        for name in ("expanded_bwd", "absorbed"):
+            getattr(lib, f"kda_mla_{name}_workspace_size").argtypes = [ctypes.c_int64] * 5
+            getattr(lib, f"kda_mla_{name}_workspace_size").restype = ctypes.c_size_t
         lib.kda_status_str.argtypes = [ctypes.c_int]
         lib.kda_status_str.restype = ctypes.c_char_p
         lib.kda_abi_version.argtypes = []

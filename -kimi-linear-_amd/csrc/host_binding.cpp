@@ -50,6 +50,13 @@ struct Fns {
     decltype(&kda_linear_fwd) linear = nullptr;
     decltype(&kda_linear_wgrad) wgrad = nullptr;
     decltype(&kda_linear_wgrad_workspace_size) wgrad_ws = nullptr;
+    decltype(&kda_mla_expanded_fwd) mla_expanded = nullptr;
+    decltype(&kda_mla_expanded_bwd) mla_expanded_bwd = nullptr;
+    decltype(&kda_mla_expanded_bwd_workspace_size) mla_expanded_bwd_ws = nullptr;
+    decltype(&kda_mla_absorbed_fwd) mla_absorbed = nullptr;
+    decltype(&kda_mla_absorbed_workspace_size) mla_absorbed_ws = nullptr;
+    decltype(&kda_mla_cache_append) mla_append = nullptr;
+    decltype(&kda_mla_cache_read) mla_read = nullptr;
     decltype(&kda_status_str) status_str = nullptr;
 };
 Fns fn;
@@ -80,6 +87,13 @@ void bind(const py::dict& addr, const py::object& stream_fn, const py::object& e
     take(fn.linear, addr, "kda_linear_fwd");
     take(fn.wgrad, addr, "kda_linear_wgrad");
     take(fn.wgrad_ws, addr, "kda_linear_wgrad_workspace_size");
+    take(fn.mla_expanded, addr, "kda_mla_expanded_fwd");
+    take(fn.mla_expanded_bwd, addr, "kda_mla_expanded_bwd");
+    take(fn.mla_expanded_bwd_ws, addr, "kda_mla_expanded_bwd_workspace_size");
+    take(fn.mla_absorbed, addr, "kda_mla_absorbed_fwd");
+    take(fn.mla_absorbed_ws, addr, "kda_mla_absorbed_workspace_size");
+    take(fn.mla_append, addr, "kda_mla_cache_append");
+    take(fn.mla_read, addr, "kda_mla_cache_read");
     take(fn.status_str, addr, "kda_status_str");
     device_type = at::Device(device).type();
     raw_stream = stream_fn.inc_ref().ptr();
@@ -534,6 +548,229 @@ py::object linear_wgrad(const Tensor& dy, const Tensor& x) {
     return py::cast(dw);
 }
 
+// ---- latent attention -------------------------------------------------------
+// Rows of 16-byte pieces: contiguous channels, aligned base and strides.
+bool wide_rows(const Tensor& t) {
+    const int64_t last = t.dim() - 1, n = 16 / t.element_size();
+    if (t.size(last) > 1 && t.stride(last) != 1) return false;
+    if (reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 != 0) return false;
+    for (int64_t i = 0; i < last; ++i)
+        if (t.size(i) > 1 && t.stride(i) % n != 0) return false;
+    return true;
+}
+// The strides of the dimensions before the channels; one of a single entry may be anything, and counts as 0.
+template <size_t M>
+void row_strides(int64_t (&out)[M], const Tensor& t) {
+    for (size_t i = 0; i < M; ++i) out[i] = t.size(i) > 1 ? t.stride(i) : 0;
+}
+bool half_type(const Tensor& t) { return t.scalar_type() == at::kHalf || t.scalar_type() == at::kBFloat16; }
+bool counts_ok(const OptTensor& t, int64_t B) {
+    return !t || (t->scalar_type() == at::kInt && t->dim() == 1 && t->size(0) == B && t->is_contiguous());
+}
+const int32_t* counts_ptr(const OptTensor& t) { return t ? static_cast<const int32_t*>(t->data_ptr()) : nullptr; }
+
+bool expanded_ok(const Plain& plain, const Tensor& q, const Tensor& k, const OptTensor& k_pe, const Tensor& v,
+                 const OptTensor& lengths, const OptTensor& starts) {
+    if (!plain.ok || q.dim() != 4 || k.dim() != 4 || v.dim() != 4 || !half_type(q)) return false;
+    const int64_t B = q.size(0), H = q.size(2), S = k.size(1), N = k.size(3), P = k_pe ? k_pe->size(-1) : 0;
+    if (!sized(k, {B, S, H, N}) || !sized(v, {B, S, H, N}) || q.size(3) != N + P) return false;
+    if (k_pe && (!sized(*k_pe, {B, S, P}) || k_pe->scalar_type() != q.scalar_type() || !wide_rows(*k_pe))) return false;
+    return k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type() && wide_rows(q) && wide_rows(k) &&
+           wide_rows(v) && counts_ok(lengths, B) && counts_ok(starts, B);
+}
+
+kda_mla_expanded_args expanded_args(const Tensor& q, const Tensor& k, const OptTensor& k_pe, const Tensor& v,
+                                    const OptTensor& lengths, const OptTensor& starts, double scale, const Tensor& o,
+                                    const OptTensor& lse) {
+    kda_mla_expanded_args a{};
+    a.B = q.size(0); a.T = q.size(1); a.S = k.size(1); a.H = q.size(2);
+    a.N = k.size(3); a.P = q.size(3) - a.N; a.V = v.size(3);
+    a.q = q.data_ptr(); a.k = k.data_ptr(); a.v = v.data_ptr();
+    row_strides(a.q_stride, q);
+    row_strides(a.k_stride, k);
+    row_strides(a.v_stride, v);
+    if (a.P > 0) {
+        a.k_pe = k_pe->data_ptr();
+        row_strides(a.k_pe_stride, *k_pe);
+    }
+    a.lengths = counts_ptr(lengths);
+    a.starts = counts_ptr(starts);
+    a.o = o.data_ptr();
+    a.lse = lse ? static_cast<float*>(lse->data_ptr()) : nullptr;
+    a.scale = static_cast<float>(scale);
+    a.dtype = code(q);
+    return a;
+}
+
+// mla_expanded: o, with want_lse (o, lse), or None.
+py::object mla_expanded(const Tensor& q, const Tensor& k, const OptTensor& k_pe, const Tensor& v,
+                        const OptTensor& lengths, const OptTensor& starts, double scale, bool want_lse) {
+    Plain plain(q);
+    plain.add(k).add(k_pe).add(v).add(lengths).add(starts);
+    if (!expanded_ok(plain, q, k, k_pe, v, lengths, starts)) return py::none();
+    Tensor o;
+    OptTensor lse;
+    const int status = run(plain.dev, [&](void* stream) -> int {
+        const auto opt = q.options().requires_grad(false);
+        o = at::empty({q.size(0), q.size(1), q.size(2), v.size(3)}, opt);
+        if (want_lse) lse = at::empty({q.size(0), q.size(2), q.size(1)}, opt.dtype(at::kFloat));
+        const auto a = expanded_args(q, k, k_pe, v, lengths, starts, scale, o, lse);
+        return fn.mla_expanded(&a, stream);
+    });
+    if (refused(status, "kda_mla_expanded_fwd")) return py::none();
+    return want_lse ? py::object(py::make_tuple(o, *lse)) : py::cast(o);
+}
+
+// Its gradients: (dq, dk, dk_pe or None, dv) or None.
+py::object mla_expanded_bwd(const Tensor& d_o, const Tensor& q, const Tensor& k, const OptTensor& k_pe, const Tensor& v,
+                            const OptTensor& lengths, const OptTensor& starts, double scale, const Tensor& o,
+                            const Tensor& lse) {
+    Plain plain(q);
+    plain.add(k).add(k_pe).add(v).add(lengths).add(starts).add(d_o).add(o).add(lse);
+    if (!expanded_ok(plain, q, k, k_pe, v, lengths, starts) || !d_o.sizes().equals(o.sizes()) ||
+        d_o.scalar_type() != q.scalar_type() || !wide_rows(d_o) || !o.is_contiguous() || !lse.is_contiguous() ||
+        lse.scalar_type() != at::kFloat)
+        return py::none();
+    Tensor dq, dk, dv;
+    OptTensor dpe;
+    const int status = run(plain.dev, [&](void* stream) -> int {
+        const auto opt = q.options().requires_grad(false);
+        dq = at::empty(q.sizes(), opt);
+        dk = at::empty(k.sizes(), opt);
+        dv = at::empty(v.sizes(), opt);
+        if (k_pe) dpe = at::empty(k_pe->sizes(), opt);
+        kda_mla_expanded_bwd_args g{};
+        g.fwd = expanded_args(q, k, k_pe, v, lengths, starts, scale, o, lse);
+        const size_t bytes = fn.mla_expanded_bwd_ws(g.fwd.B, g.fwd.T, g.fwd.S, g.fwd.H, g.fwd.P);
+        const Tensor ws = at::empty({static_cast<int64_t>(bytes)}, opt.dtype(at::kByte));
+        g.d_o = d_o.data_ptr();
+        row_strides(g.d_o_stride, d_o);
+        g.dq = dq.data_ptr();
+        g.dk = dk.data_ptr();
+        g.dk_pe = g.fwd.P > 0 ? dpe->data_ptr() : nullptr;
+        g.dv = dv.data_ptr();
+        g.workspace = ws.data_ptr();
+        return fn.mla_expanded_bwd(&g, stream);
+    });
+    if (refused(status, "kda_mla_expanded_bwd")) return py::none();
+    return py::make_tuple(dq, dk, dpe ? py::cast(*dpe) : py::object(py::none()), dv);
+}
+
+// A cache [B, S, rank + P] in 16 or 8 bits, in 8 with its scales [B, S, 2].
+bool cache_ok(const Tensor& cache, const OptTensor& scale, int64_t B, at::ScalarType act) {
+    if (cache.dim() != 3 || cache.size(0) != B || !wide_rows(cache)) return false;
+    if (cache.scalar_type() == act) return !scale;
+    return cache.scalar_type() == at::kFloat8_e4m3fn && scale && scale->scalar_type() == at::kFloat &&
+           sized(*scale, {B, cache.size(1), 2}) && scale->stride(2) == 1 &&
+           (scale->size(0) <= 1 || scale->stride(0) % 2 == 0) && (scale->size(1) <= 1 || scale->stride(1) % 2 == 0) &&
+           reinterpret_cast<uintptr_t>(scale->data_ptr()) % 8 == 0;
+}
+int cache_code(const Tensor& cache) {
+    return cache.scalar_type() == at::kFloat8_e4m3fn ? static_cast<int>(KDA_DTYPE_E4M3) : code(cache);
+}
+
+// mla_absorbed: o [B, T, H, rank] or None.
+py::object mla_absorbed(const Tensor& q, const Tensor& cache, const Tensor& lengths, int64_t rank, double scale,
+                        const OptTensor& cache_scale) {
+    Plain plain(q);
+    plain.add(cache).add(lengths).add(cache_scale);
+    if (!plain.ok || q.dim() != 4 || !half_type(q) || !wide_rows(q) || !counts_ok(lengths, q.size(0)) ||
+        !cache_ok(cache, cache_scale, q.size(0), q.scalar_type()) || cache.size(2) != q.size(3))
+        return py::none();
+    Tensor o;
+    const int status = run(plain.dev, [&](void* stream) -> int {
+        const auto opt = q.options().requires_grad(false);
+        kda_mla_absorbed_args a{};
+        a.B = q.size(0); a.T = q.size(1); a.H = q.size(2); a.S = cache.size(1); a.R = rank; a.P = q.size(3) - rank;
+        if (rank < 0 || a.P < 0) return KDA_ERR_BAD_SHAPE;
+        o = at::empty({a.B, a.T, a.H, rank}, opt);
+        a.q = q.data_ptr();
+        row_strides(a.q_stride, q);
+        a.cache = cache.data_ptr();
+        row_strides(a.cache_stride, cache);
+        if (cache_scale) {
+            a.cache_scale = static_cast<const float*>(cache_scale->data_ptr());
+            row_strides(a.scale_stride, *cache_scale);
+        }
+        a.lengths = static_cast<const int32_t*>(lengths.data_ptr());
+        a.o = o.data_ptr();
+        a.scale = static_cast<float>(scale);
+        a.dtype = code(q);
+        a.cache_dtype = cache_code(cache);
+        const size_t bytes = fn.mla_absorbed_ws(a.B, a.T, a.H, a.S, a.R);
+        Tensor ws;
+        if (bytes > 0) {
+            ws = at::empty({static_cast<int64_t>(bytes)}, opt.dtype(at::kByte));
+            a.workspace = ws.data_ptr();
+        }
+        return fn.mla_absorbed(&a, stream);
+    });
+    if (refused(status, "kda_mla_absorbed_fwd")) return py::none();
+    return py::cast(o);
+}
+
+// mla_cache_append: whether it was done.
+bool mla_append(const Tensor& x, const Tensor& cache, const Tensor& lengths, int64_t rank, const OptTensor& cache_scale,
+                const OptTensor& counts, const OptTensor& weight, double eps) {
+    Plain plain(x);
+    plain.add(cache).add(lengths).add(cache_scale).add(counts).add(weight);
+    if (!plain.ok || x.dim() != 3 || !half_type(x) || !wide_rows(x) || !counts_ok(lengths, x.size(0)) ||
+        !counts_ok(counts, x.size(0)) || !cache_ok(cache, cache_scale, x.size(0), x.scalar_type()) ||
+        cache.size(2) != x.size(2) || overlaps(cache, x) || (cache_scale && overlaps(*cache_scale, x)))
+        return false;
+    if (weight && (weight->scalar_type() != x.scalar_type() || !sized(*weight, {rank}) || !wide_rows(*weight)))
+        return false;
+    kda_mla_append_args a{};
+    a.B = x.size(0); a.T = x.size(1); a.S = cache.size(1); a.R = rank; a.P = x.size(2) - rank;
+    a.x = x.data_ptr();
+    row_strides(a.x_stride, x);
+    a.cache = cache.data_ptr();
+    row_strides(a.cache_stride, cache);
+    if (cache_scale) {
+        a.cache_scale = static_cast<float*>(cache_scale->data_ptr());
+        row_strides(a.scale_stride, *cache_scale);
+    }
+    a.lengths = static_cast<const int32_t*>(lengths.data_ptr());
+    a.counts = counts_ptr(counts);
+    a.norm_weight = weight ? weight->data_ptr() : nullptr;
+    a.eps = static_cast<float>(eps);
+    a.x_dtype = code(x);
+    a.cache_dtype = cache_code(cache);
+    const int status = run(plain.dev, [&](void* stream) -> int { return fn.mla_append(&a, stream); });
+    if (refused(status, "kda_mla_cache_append")) return false;
+    // written in place, unseen by autograd: its version counters say so
+    if (!cache.is_inference()) cache.unsafeGetTensorImpl()->bump_version();
+    if (cache_scale && !cache_scale->is_inference()) cache_scale->unsafeGetTensorImpl()->bump_version();
+    return true;
+}
+
+// mla_cache_read: [B, tokens, rank + P] or None.
+py::object mla_read(const Tensor& cache, const Tensor& cache_scale, int64_t rank, at::ScalarType dtype, int64_t count,
+                    const OptTensor& lengths) {
+    Plain plain(cache);
+    plain.add(cache_scale).add(lengths);
+    if (!plain.ok || cache.dim() != 3 || (dtype != at::kHalf && dtype != at::kBFloat16) ||
+        !cache_ok(cache, cache_scale, cache.size(0), dtype) || cache.scalar_type() == dtype ||
+        !counts_ok(lengths, cache.size(0)) || count < 0 || count > cache.size(1))
+        return py::none();
+    Tensor out;
+    const int status = run(plain.dev, [&](void* stream) -> int {
+        out = at::empty({cache.size(0), count, cache.size(2)}, cache.options().dtype(dtype).requires_grad(false));
+        kda_mla_read_args a{};
+        a.B = cache.size(0); a.S = count; a.R = rank; a.P = cache.size(2) - rank;
+        a.cache = cache.data_ptr();
+        row_strides(a.cache_stride, cache);
+        a.cache_scale = static_cast<const float*>(cache_scale.data_ptr());
+        row_strides(a.scale_stride, cache_scale);
+        a.lengths = counts_ptr(lengths);
+        a.out = out.data_ptr();
+        a.out_dtype = code(out);
+        return fn.mla_read(&a, stream);
+    });
+    if (refused(status, "kda_mla_cache_read")) return py::none();
+    return py::cast(out);
+}
+
 // What decides whether a copy made of these parameters is still theirs:
 // storage address, version, type and device of each.
 py::bytes params_key(const std::vector<Tensor>& params) {
@@ -569,5 +806,10 @@ PYBIND11_MODULE(_kda_host, m) {
     m.def("linear", &linear);
     m.def("linear2", &linear2);
     m.def("linear_wgrad", &linear_wgrad);
+    m.def("mla_expanded", &mla_expanded);
+    m.def("mla_expanded_bwd", &mla_expanded_bwd);
+    m.def("mla_absorbed", &mla_absorbed);
+    m.def("mla_append", &mla_append);
+    m.def("mla_read", &mla_read);
     m.def("params_key", &params_key);
 }

@@ -77,4 +77,15 @@ bool linear_wgrad_supported(int64_t M, int64_t N, int64_t K);
 int64_t linear_wgrad_workspace_bytes(int64_t M, int64_t N, int64_t K);
 int linear_wgrad_launch(const kda_linear_wgrad_args& a, hipStream_t stream);
 
+
+// Latent attention (kda_mla_*.hip); arguments checked by the caller, no work
+// of size zero.
+int mla_expanded_launch(const kda_mla_expanded_args& a, hipStream_t stream);
+int64_t mla_expanded_bwd_workspace_bytes(int64_t B, int64_t T, int64_t S, int64_t H, int64_t P);
+int mla_expanded_bwd_launch(const kda_mla_expanded_bwd_args& a, hipStream_t stream);
+int64_t mla_absorbed_workspace_bytes(int64_t B, int64_t T, int64_t H, int64_t S, int64_t R);
+int mla_absorbed_launch(const kda_mla_absorbed_args& a, hipStream_t stream);
+int mla_append_launch(const kda_mla_append_args& a, hipStream_t stream);
+int mla_read_launch(const kda_mla_read_args& a, hipStream_t stream);
+
 }  // namespace kda

@@ -1,0 +1,191 @@
+// Latent attention in its expanded form, forward: causal attention whose keys
+// are a head's own N channels and P position channels that all heads share.
+//
+//   s_tj = scale q_t . [k_j | k_pe_j],  o_t = sum_j 2^(s'_tj - M_t) v_j / sum_j 2^(s'_tj - M_t),
+//   s' = s log2(e),  M a running maximum.
+//
+// Bound by the matrix cores: 2 (N + P + V) flops a visible pair.  A wave has 32
+// query rows; a workgroup's waves share 64-key tiles of K, K_pe and V in LDS,
+// two buffers, the next tile's loads in flight through the current one's
+// products.  The scores are formed transposed (keys x rows, 32x32x16), so a
+// lane has 32 scores of one row: the row's maximum and sum are its own
+// registers and one exchange with the other half of the wave, and the scores,
+// rounded, are the second operand of the value product O^T = V^T P^T as they
+// lie, in an order of the keys that the transposed reads of V follow.  O^T's
+// columns are rows again, so a new maximum rescales a lane's own registers;
+// it does so only when the maximum has grown by more than 2^8 (P stays below
+// 2^8, exact range for both types), the sums are exact either way.
+//
+// LDS rows are padded so that sixteen rows' 16-byte pieces (K) and the four
+// rows of a transposed read (V) fall into different banks.
+#include <hip/hip_runtime.h>
+
+#include "kda_launch.h"
+#include "kda_mla.h"
+#include "kda_mla_tile.h"
+
+namespace kda {
+namespace {
+
+using namespace mla;
+
+constexpr float kLazy = 8.f;          // log2 of how far a maximum may lag
+
+// Grid: (query tiles, longest first) x (batch, head) with the latter inner, so
+// that a head's tiles share an XCD's L2 where B H is a multiple of eight.
+template <typename T, int N, int P, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : 1) void expanded_kernel(kda_mla_expanded_args a, int qtiles) {
+    using F = KvTile<T, N, P, 64 * WAVES, 32>;
+    constexpr int D = F::D, V = F::V, kRows = 32 * WAVES;
+    __shared__ __align__(16) T smem[2 * F::kBuf];
+    const int64_t bhs = a.B * a.H;
+    const int64_t bh = blockIdx.x % bhs, b = bh / a.H, h = bh - b * a.H;
+    const int t0 = (qtiles - 1 - static_cast<int>(blockIdx.x / bhs)) * kRows;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lq = lane & 31, half = lane >> 5;
+    const int len = tokens(a.lengths, b, a.S), nq = static_cast<int>(a.T);
+    const int start = first_position(a.starts, b, a.S, a.T);
+    const int exist = max(0, min(nq, len - start));              // queries that exist
+    const int t = t0 + 32 * wave + lq;
+    const bool live = t < exist;
+    const int limit = live ? start + t : -1;                      // last key this lane's row sees
+    const int w0 = t0 + 32 * wave;                                // the wave's rows: all, some or none exist
+    const int wlast = w0 < exist ? start + min(w0 + 31, exist - 1) : -1;
+    const int wall = w0 + 32 <= exist ? start + w0 : -1;          // keys up to this one every row sees
+    const int keys = t0 < exist ? start + min(t0 + kRows, exist) : 0;
+    const float c = a.scale * kLog2E;
+
+    uint4 q[D / 16];
+    f16v o[V / 32];
+#pragma unroll
+    for (int i = 0; i < V / 32; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[i][e] = 0.f;
+    float top = kNoMax, sum = 0.f;
+
+    if (keys > 0) {
+        const T* qr = static_cast<const T*>(a.q) + b * a.q_stride[0] + min(t, exist - 1) * a.q_stride[1] +
+                      h * a.q_stride[2] + 8 * half;
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) q[k] = *reinterpret_cast<const uint4*>(qr + 16 * k);
+        const T* kp = static_cast<const T*>(a.k) + b * a.k_stride[0] + h * a.k_stride[2];
+        const T* pe = static_cast<const T*>(a.k_pe) + b * a.k_pe_stride[0];
+        const T* vp = static_cast<const T*>(a.v) + b * a.v_stride[0] + h * a.v_stride[2];
+        uint4 r[F::kPer];
+        F::fetch(a, kp, pe, vp, 0, keys, r);
+        F::put(smem, r);
+        __syncthreads();
+        int cur = 0;
+        for (int j0 = 0; j0 < keys; j0 += kTile, cur ^= 1) {
+            const bool more = j0 + kTile < keys;
+            if (more) F::fetch(a, kp, pe, vp, j0 + kTile, keys, r);
+            if (j0 <= wlast) {
+                const T* kt = smem + cur * F::kBuf + lq * F::kK + 8 * half;
+                f16v s[2];
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) s[u][e] = 0.f;
+#pragma unroll
+                    for (int k = 0; k < D / 16; ++k)
+                        s[u] = Act<T>::mma32(*reinterpret_cast<const uint4*>(kt + 32 * u * F::kK + 16 * k), q[k], s[u]);
+                }
+                if (j0 + kTile - 1 > wall) {
+#pragma unroll
+                    for (int u = 0; u < 2; ++u)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e)
+                            if (j0 + 32 * u + 8 * (e / 4) + 4 * half + e % 4 > limit) s[u][e] = -INFINITY;
+                }
+                float mx = s[0][0];
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[u][e]);
+                mx = half_max(mx) * c;
+                if (__any(mx > top + kLazy)) {
+                    const float now = fmaxf(top, mx), alpha = __builtin_amdgcn_exp2f(top - now);
+                    top = now;
+                    sum *= alpha;
+#pragma unroll
+                    for (int i = 0; i < V / 32; ++i)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) o[i][e] *= alpha;
+                }
+                uint4 p[4];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float x = __builtin_amdgcn_exp2f(fmaf(s[u / 2][8 * (u % 2) + 2 * e], c, -top));
+                        const float y = __builtin_amdgcn_exp2f(fmaf(s[u / 2][8 * (u % 2) + 2 * e + 1], c, -top));
+                        sum += x;
+                        sum += y;
+                        w[e] = Act<T>::pair(x, y);
+                    }
+                    p[u] = uint4{w[0], w[1], w[2], w[3]};
+                }
+                const T* vt = smem + cur * F::kBuf + kTile * F::kK + (4 * half + ((lane & 15) >> 2)) * F::kV +
+                              16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+#pragma unroll
+                    for (int i = 0; i < V / 32; ++i) {
+                        const uint2 v0 = read_tr(vt + 16 * u * F::kV + 32 * i);
+                        const uint2 v1 = read_tr(vt + (16 * u + 8) * F::kV + 32 * i);
+                        o[i] = Act<T>::mma32(uint4{v0.x, v0.y, v1.x, v1.y}, p[u], o[i]);
+                    }
+            }
+            if (more) F::put(smem + (cur ^ 1) * F::kBuf, r);
+            __syncthreads();
+        }
+    }
+    if (t >= nq) return;
+    sum = half_sum(sum);
+    const float norm = sum == 0.f ? 0.f : 1.f / sum;
+    T* out = static_cast<T*>(a.o) + ((b * a.T + t) * a.H + h) * V + 4 * half;
+#pragma unroll
+    for (int i = 0; i < V / 32; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            *reinterpret_cast<uint2*>(out + 32 * i + 8 * e) =
+                uint2{Act<T>::pair(o[i][4 * e] * norm, o[i][4 * e + 1] * norm),
+                      Act<T>::pair(o[i][4 * e + 2] * norm, o[i][4 * e + 3] * norm)};
+    if (a.lse && half == 0)
+        a.lse[(b * a.H + h) * a.T + t] = sum == 0.f ? INFINITY : top + __builtin_amdgcn_logf(sum);
+}
+
+template <typename T, int N, int P, int WAVES>
+int launch_waves(const kda_mla_expanded_args& a, hipStream_t stream) {
+    const int64_t qtiles = (a.T + 32 * WAVES - 1) / (32 * WAVES);
+    expanded_kernel<T, N, P, WAVES><<<static_cast<unsigned>(qtiles * a.B * a.H), 64 * WAVES, 0, stream>>>(
+        a, static_cast<int>(qtiles));
+    return hipGetLastError() == hipSuccess ? KDA_OK : KDA_ERR_LAUNCH;
+}
+
+template <typename T, int N, int P>
+int launch(const kda_mla_expanded_args& a, hipStream_t stream) {
+    // as many rows a workgroup as leave every CU one
+    if (a.B * a.H * ((a.T + 255) / 256) >= 256) return launch_waves<T, N, P, 8>(a, stream);
+    if (a.B * a.H * ((a.T + 127) / 128) >= 256) return launch_waves<T, N, P, 4>(a, stream);
+    return launch_waves<T, N, P, 2>(a, stream);
+}
+
+template <typename T>
+int launch_dims(const kda_mla_expanded_args& a, hipStream_t stream) {
+    switch (a.N + a.P) {
+        case 192: return launch<T, 128, 64>(a, stream);
+        case 160: return launch<T, 128, 32>(a, stream);
+        case 128: return a.N == 128 ? launch<T, 128, 0>(a, stream) : launch<T, 64, 64>(a, stream);
+        case 96: return launch<T, 64, 32>(a, stream);
+        default: return launch<T, 64, 0>(a, stream);
+    }
+}
+
+}  // namespace
+
+int mla_expanded_launch(const kda_mla_expanded_args& a, hipStream_t stream) {
+    return a.dtype == KDA_DTYPE_F16 ? launch_dims<_Float16>(a, stream) : launch_dims<bf16_t>(a, stream);
+}
+
+}  // namespace kda

@@ -1,0 +1,461 @@
+// Latent attention in its expanded form, backward.  With the forward's lse,
+//
+//   p_tj = 2^(s'_tj - lse_t),  dp_tj = do_t . v_j,  delta_t = do_t . o_t,
+//   ds_tj = p_tj (dp_tj - delta_t),
+//   dv_j = sum_t p_tj do_t,  dq_t = scale sum_j ds_tj [k_j | k_pe_j],
+//   dk_j = scale sum_t ds_tj q_t  (its last P channels summed over the heads too).
+//
+// Two kernels that each form s and dp anew, one with a wave's 32 query rows
+// standing and the keys passing (dq, and delta for the other), one with a
+// wave's 32 keys standing and the queries passing (dk, dv): seven products
+// instead of the five that adding dq's parts in memory would take, and no
+// atomics, so the sums have one order.  Bound by the matrix cores.
+//
+// In both, the scores are formed with the standing index in the lanes, so p
+// and ds, rounded to the activation type, are operands of the accumulating
+// products as they lie in their registers; those products' other operand is
+// the passing tile read transposed from LDS.  The position part's gradient is
+// left per head in fp32 and summed over the heads by a third kernel.
+//
+// fp16: p is formed times 2^12 and ds times a power of two that follows its
+// magnitude (per row in dq, per wave in dk), so neither long contexts nor
+// small gradients fall below fp16's range; bf16 needs neither.
+#include <hip/hip_runtime.h>
+
+#include "kda_launch.h"
+#include "kda_mla.h"
+#include "kda_mla_tile.h"
+
+namespace kda {
+namespace {
+
+using namespace mla;
+
+constexpr int kQTile = 32;            // queries a tile of the dk, dv kernel
+constexpr int kWaves = 4;
+constexpr int kThreads = 64 * kWaves;
+
+template <typename T> constexpr bool kHalf = Elem<T>::code == KDA_DTYPE_F16;
+template <typename T> constexpr float kPShift = kHalf<T> ? 12.f : 0.f;
+
+// Where a sequence's queries and keys are.
+struct Place {
+    int64_t b, h;
+    int len, start, exist;            // tokens; position of query 0; queries that exist
+    __device__ __forceinline__ Place(const kda_mla_expanded_args& a, int64_t bh) {
+        b = bh / a.H;
+        h = bh - b * a.H;
+        len = tokens(a.lengths, b, a.S);
+        start = first_position(a.starts, b, a.S, a.T);
+        exist = max(0, min(static_cast<int>(a.T), len - start));
+    }
+};
+
+// A power of two for values up to m, so that their products with it stay
+// within 2^14: the one in use, or where that is too large one that leaves 2^6
+// of room.
+__device__ __forceinline__ float follow(float f, float m) {
+    return m * f > 0x1p14f ? __builtin_amdgcn_ldexpf(1.f, 8 - __builtin_amdgcn_frexp_expf(m)) : f;
+}
+constexpr float kFirst = 0x1p60f;     // before any value
+
+__device__ __forceinline__ float dot8(uint4 x, uint4 y, float acc, _Float16) {
+    const h8 a = __builtin_bit_cast(h8, x), b = __builtin_bit_cast(h8, y);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) acc = fmaf(static_cast<float>(a[i]), static_cast<float>(b[i]), acc);
+    return acc;
+}
+__device__ __forceinline__ float dot8(uint4 x, uint4 y, float acc, bf16_t) {
+    const uint32_t a[4] = {x.x, x.y, x.z, x.w}, b[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        acc = fmaf(__uint_as_float(a[i] << 16), __uint_as_float(b[i] << 16), acc);
+        acc = fmaf(__uint_as_float(a[i] & 0xffff0000u), __uint_as_float(b[i] & 0xffff0000u), acc);
+    }
+    return acc;
+}
+
+// dq of 32 rows a wave, and delta.  Grid as the forward's.
+template <typename T, int N, int P>
+__global__ __launch_bounds__(kThreads, 1) void dq_kernel(kda_mla_expanded_bwd_args g, float* delta, int qtiles) {
+    const kda_mla_expanded_args& a = g.fwd;
+    using F = KvTile<T, N, P, kThreads, 8>;
+    constexpr int D = F::D, V = F::V, kRows = 32 * kWaves;
+    __shared__ __align__(16) T smem[2 * F::kBuf];
+    const int64_t bhs = a.B * a.H, bh = blockIdx.x % bhs;
+    const Place at(a, bh);
+    const int t0 = (qtiles - 1 - static_cast<int>(blockIdx.x / bhs)) * kRows;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lq = lane & 31, half = lane >> 5;
+    const int t = t0 + 32 * wave + lq, nq = static_cast<int>(a.T);
+    const bool live = t < at.exist;
+    const int limit = live ? at.start + t : -1;
+    const int w0 = t0 + 32 * wave;
+    const int wlast = w0 < at.exist ? at.start + min(w0 + 31, at.exist - 1) : -1;
+    const int wall = w0 + 32 <= at.exist ? at.start + w0 : -1;
+    const int keys = t0 < at.exist ? at.start + min(t0 + kRows, at.exist) : 0;
+    const float c = a.scale * kLog2E;
+
+    f16v dq[D / 32];
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) dq[i][e] = 0.f;
+    float f = kHalf<T> ? kFirst : 1.f;
+
+    if (keys > 0) {
+        const int tc = min(t, at.exist - 1);
+        const T* qr = static_cast<const T*>(a.q) + at.b * a.q_stride[0] + tc * a.q_stride[1] + at.h * a.q_stride[2] +
+                      8 * half;
+        const T* dor = static_cast<const T*>(g.d_o) + at.b * g.d_o_stride[0] + tc * g.d_o_stride[1] +
+                       at.h * g.d_o_stride[2] + 8 * half;
+        const T* orow = static_cast<const T*>(a.o) + ((at.b * a.T + tc) * a.H + at.h) * V + 8 * half;
+        uint4 q[D / 16], d_o[V / 16];
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) q[k] = *reinterpret_cast<const uint4*>(qr + 16 * k);
+        float dl = 0.f;
+#pragma unroll
+        for (int k = 0; k < V / 16; ++k) {
+            d_o[k] = *reinterpret_cast<const uint4*>(dor + 16 * k);
+            dl = dot8(d_o[k], *reinterpret_cast<const uint4*>(orow + 16 * k), dl, T{});
+        }
+        dl = half_sum(dl);
+        if (live && half == 0) delta[bh * a.T + t] = dl;
+        const float lse = (live ? a.lse[bh * a.T + t] : INFINITY) - kPShift<T>;
+
+        const T* kp = static_cast<const T*>(a.k) + at.b * a.k_stride[0] + at.h * a.k_stride[2];
+        const T* pe = static_cast<const T*>(a.k_pe) + at.b * a.k_pe_stride[0];
+        const T* vp = static_cast<const T*>(a.v) + at.b * a.v_stride[0] + at.h * a.v_stride[2];
+        uint4 r[F::kPer];
+        F::fetch(a, kp, pe, vp, 0, keys, r);
+        F::put(smem, r);
+        __syncthreads();
+        int cur = 0;
+        for (int j0 = 0; j0 < keys; j0 += kTile, cur ^= 1) {
+            const bool more = j0 + kTile < keys;
+            if (more) F::fetch(a, kp, pe, vp, j0 + kTile, keys, r);
+#pragma unroll 1
+            for (int u = 0; u < kTile && j0 + u <= wlast; u += 32) {
+                const T* kt = smem + cur * F::kBuf + (u + lq) * F::kK + 8 * half;
+                const T* vt = smem + cur * F::kBuf + kTile * F::kK + (u + lq) * F::kV + 8 * half;
+                f16v s, dp;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) s[e] = dp[e] = 0.f;
+#pragma unroll
+                for (int k = 0; k < D / 16; ++k) s = Act<T>::mma32(*reinterpret_cast<const uint4*>(kt + 16 * k), q[k], s);
+#pragma unroll
+                for (int k = 0; k < V / 16; ++k)
+                    dp = Act<T>::mma32(*reinterpret_cast<const uint4*>(vt + 16 * k), d_o[k], dp);
+                if (j0 + u + 31 > wall) {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                        if (j0 + u + 8 * (e / 4) + 4 * half + e % 4 > limit) s[e] = -INFINITY;
+                }
+                float m = 0.f;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    dp[e] = __builtin_amdgcn_exp2f(fmaf(s[e], c, -lse)) * (dp[e] - dl);
+                    if constexpr (kHalf<T>) m = fmaxf(m, fabsf(dp[e]));
+                }
+                if constexpr (kHalf<T>) {
+                    m = half_max(m);
+                    if (__any(m * f > 0x1p14f)) {
+                        const float now = follow(f, m), ratio = now / f;
+                        f = now;
+#pragma unroll
+                        for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) dq[i][e] *= ratio;
+                    }
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) dp[e] *= f;
+                }
+                const T* tr = smem + cur * F::kBuf + (u + 4 * half + ((lane & 15) >> 2)) * F::kK +
+                              16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const uint4 ds{Act<T>::pair(dp[8 * k], dp[8 * k + 1]), Act<T>::pair(dp[8 * k + 2], dp[8 * k + 3]),
+                                   Act<T>::pair(dp[8 * k + 4], dp[8 * k + 5]), Act<T>::pair(dp[8 * k + 6], dp[8 * k + 7])};
+#pragma unroll
+                    for (int i = 0; i < D / 32; ++i) {
+                        const uint2 x = read_tr(tr + 16 * k * F::kK + 32 * i);
+                        const uint2 y = read_tr(tr + (16 * k + 8) * F::kK + 32 * i);
+                        dq[i] = Act<T>::mma32(uint4{x.x, x.y, y.x, y.y}, ds, dq[i]);
+                    }
+                }
+            }
+            if (more) F::put(smem + (cur ^ 1) * F::kBuf, r);
+            __syncthreads();
+        }
+    }
+    if (t >= nq) return;
+    const float norm = a.scale * __builtin_amdgcn_exp2f(-kPShift<T>) / f;
+    T* out = static_cast<T*>(g.dq) + ((at.b * a.T + t) * a.H + at.h) * D + 4 * half;
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            *reinterpret_cast<uint2*>(out + 32 * i + 8 * e) =
+                uint2{Act<T>::pair(dq[i][4 * e] * norm, dq[i][4 * e + 1] * norm),
+                      Act<T>::pair(dq[i][4 * e + 2] * norm, dq[i][4 * e + 3] * norm)};
+}
+
+// A tile of queries and their output gradients, as KvTile: [kQTile][D + 8] and
+// [kQTile][V + 8], then lse and delta of each.
+template <typename T, int D, int V>
+struct QTile {
+    static constexpr int kQ = D + 8, kO = V + 8;
+    static constexpr int kRow = kQTile * (kQ + kO);               // elements before lse
+    static constexpr int kBuf = kRow + 4 * kQTile;                // a float is two elements
+    static constexpr int kChunks = kQTile * (D + V) / 8;
+    static constexpr int kPer = (kChunks + kThreads - 1) / kThreads;
+
+    static __device__ __forceinline__ void fetch(const kda_mla_expanded_bwd_args& g, const T* q, const T* d_o,
+                                                 const float* lse, const float* delta, int t0, int exist,
+                                                 uint4 (&r)[kPer], float& x) {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            const int c = threadIdx.x + i * kThreads;
+            if (kChunks % kThreads != 0 && c >= kChunks) break;
+            // rows past the last that exists repeat it; their lse makes p zero
+            if (c < kQTile * D / 8) {
+                const int row = min(t0 + c / (D / 8), exist - 1);
+                r[i] = *reinterpret_cast<const uint4*>(q + row * g.fwd.q_stride[1] + c % (D / 8) * 8);
+            } else {
+                const int d = c - kQTile * D / 8, row = min(t0 + d / (V / 8), exist - 1);
+                r[i] = *reinterpret_cast<const uint4*>(d_o + row * g.d_o_stride[1] + d % (V / 8) * 8);
+            }
+        }
+        if (threadIdx.x < 2 * kQTile) {
+            const int t = t0 + (threadIdx.x & (kQTile - 1));
+            const bool second = threadIdx.x >= kQTile;
+            x = second ? 0.f : INFINITY;
+            if (t < exist) x = second ? delta[t] : lse[t] - kPShift<T>;
+        }
+    }
+    static __device__ __forceinline__ void put(T* buf, const uint4 (&r)[kPer], float x) {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            const int c = threadIdx.x + i * kThreads;
+            if (kChunks % kThreads != 0 && c >= kChunks) break;
+            int at;
+            if (c < kQTile * D / 8) {
+                at = c / (D / 8) * kQ + c % (D / 8) * 8;
+            } else {
+                const int d = c - kQTile * D / 8;
+                at = kQTile * kQ + d / (V / 8) * kO + d % (V / 8) * 8;
+            }
+            *reinterpret_cast<uint4*>(buf + at) = r[i];
+        }
+        if (threadIdx.x < 2 * kQTile) reinterpret_cast<float*>(buf + kRow)[threadIdx.x] = x;
+    }
+};
+
+// dk and dv of 32 keys a wave.  Grid: (key tiles, the first have the most
+// queries) x (batch, head), the latter inner.
+template <typename T, int N, int P>
+__global__ __launch_bounds__(kThreads, 1) void dkv_kernel(kda_mla_expanded_bwd_args g, const float* delta, float* dpe) {
+    const kda_mla_expanded_args& a = g.fwd;
+    constexpr int D = N + P, V = N, kKeys = 32 * kWaves;
+    using F = QTile<T, D, V>;
+    __shared__ __align__(16) T smem[2 * F::kBuf];
+    const int64_t bhs = a.B * a.H, bh = blockIdx.x % bhs;
+    const Place at(a, bh);
+    const int j0 = static_cast<int>(blockIdx.x / bhs) * kKeys;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lk = lane & 31, half = lane >> 5;
+    const int w0 = j0 + 32 * wave, j = w0 + lk;
+    const float c = a.scale * kLog2E;
+
+    f16v dk[D / 32], dv[V / 32];
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) dk[i][e] = 0.f;
+#pragma unroll
+    for (int i = 0; i < V / 32; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) dv[i][e] = 0.f;
+    float f = kHalf<T> ? kFirst : 1.f;
+
+    const int first = max(0, j0 - at.start) / kQTile * kQTile;       // the first queries that see a key of these
+    if (j0 < at.len && first < at.exist) {
+        const int jc = min(j, at.len - 1);
+        const T* kr = static_cast<const T*>(a.k) + at.b * a.k_stride[0] + jc * a.k_stride[1] + at.h * a.k_stride[2] +
+                      8 * half;
+        const T* pr = static_cast<const T*>(a.k_pe) + at.b * a.k_pe_stride[0] + jc * a.k_pe_stride[1] + 8 * half;
+        const T* vr = static_cast<const T*>(a.v) + at.b * a.v_stride[0] + jc * a.v_stride[1] + at.h * a.v_stride[2] +
+                      8 * half;
+        uint4 k[D / 16], v[V / 16];
+#pragma unroll
+        for (int i = 0; i < N / 16; ++i) k[i] = *reinterpret_cast<const uint4*>(kr + 16 * i);
+#pragma unroll
+        for (int i = 0; i < P / 16; ++i) k[N / 16 + i] = *reinterpret_cast<const uint4*>(pr + 16 * i);
+#pragma unroll
+        for (int i = 0; i < V / 16; ++i) v[i] = *reinterpret_cast<const uint4*>(vr + 16 * i);
+        const T* qp = static_cast<const T*>(a.q) + at.b * a.q_stride[0] + at.h * a.q_stride[2];
+        const T* dop = static_cast<const T*>(g.d_o) + at.b * g.d_o_stride[0] + at.h * g.d_o_stride[2];
+        const float *lse = a.lse + bh * a.T, *del = delta + bh * a.T;
+        uint4 r[F::kPer];
+        float x;
+        F::fetch(g, qp, dop, lse, del, first, at.exist, r, x);
+        F::put(smem, r, x);
+        __syncthreads();
+        int cur = 0;
+        for (int t0 = first; t0 < at.exist; t0 += kQTile, cur ^= 1) {
+            const bool more = t0 + kQTile < at.exist;
+            if (more) F::fetch(g, qp, dop, lse, del, t0 + kQTile, at.exist, r, x);
+            if (at.start + t0 + kQTile - 1 >= w0 && w0 < at.len) {
+                const T* buf = smem + cur * F::kBuf;
+                const T* qt = buf + lk * F::kQ + 8 * half;
+                const T* ot = buf + kQTile * F::kQ + lk * F::kO + 8 * half;
+                const float* st = reinterpret_cast<const float*>(buf + F::kRow) + 4 * half;
+                f16v s, dp;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) s[e] = dp[e] = 0.f;
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i) s = Act<T>::mma32(*reinterpret_cast<const uint4*>(qt + 16 * i), k[i], s);
+#pragma unroll
+                for (int i = 0; i < V / 16; ++i)
+                    dp = Act<T>::mma32(*reinterpret_cast<const uint4*>(ot + 16 * i), v[i], dp);
+                if (at.start + t0 < w0 + 31 || w0 + 32 > at.len) {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                        if (at.start + t0 + 8 * (e / 4) + 4 * half + e % 4 < j || j >= at.len) s[e] = -INFINITY;
+                }
+                float m = 0.f;
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const f4 l = *reinterpret_cast<const f4*>(st + 8 * u), d = *reinterpret_cast<const f4*>(st + kQTile + 8 * u);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float p = __builtin_amdgcn_exp2f(fmaf(s[4 * u + e], c, -l[e]));
+                        s[4 * u + e] = p;
+                        dp[4 * u + e] = p * (dp[4 * u + e] - d[e]);
+                        if constexpr (kHalf<T>) m = fmaxf(m, fabsf(dp[4 * u + e]));
+                    }
+                }
+                if constexpr (kHalf<T>) {
+                    m = wave_max(m);
+                    if (m * f > 0x1p14f) {
+                        const float now = follow(f, m), ratio = now / f;
+                        f = now;
+#pragma unroll
+                        for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) dk[i][e] *= ratio;
+                    }
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) dp[e] *= f;
+                }
+                const int trow = 4 * half + ((lane & 15) >> 2), tcol = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+                const T* qtr = buf + trow * F::kQ + tcol;
+                const T* otr = buf + kQTile * F::kQ + trow * F::kO + tcol;
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const uint4 pf{Act<T>::pair(s[8 * u], s[8 * u + 1]), Act<T>::pair(s[8 * u + 2], s[8 * u + 3]),
+                                   Act<T>::pair(s[8 * u + 4], s[8 * u + 5]), Act<T>::pair(s[8 * u + 6], s[8 * u + 7])};
+                    const uint4 df{Act<T>::pair(dp[8 * u], dp[8 * u + 1]), Act<T>::pair(dp[8 * u + 2], dp[8 * u + 3]),
+                                   Act<T>::pair(dp[8 * u + 4], dp[8 * u + 5]), Act<T>::pair(dp[8 * u + 6], dp[8 * u + 7])};
+#pragma unroll
+                    for (int i = 0; i < V / 32; ++i) {
+                        const uint2 y = read_tr(otr + 16 * u * F::kO + 32 * i), z = read_tr(otr + (16 * u + 8) * F::kO + 32 * i);
+                        dv[i] = Act<T>::mma32(uint4{y.x, y.y, z.x, z.y}, pf, dv[i]);
+                    }
+#pragma unroll
+                    for (int i = 0; i < D / 32; ++i) {
+                        const uint2 y = read_tr(qtr + 16 * u * F::kQ + 32 * i), z = read_tr(qtr + (16 * u + 8) * F::kQ + 32 * i);
+                        dk[i] = Act<T>::mma32(uint4{y.x, y.y, z.x, z.y}, df, dk[i]);
+                    }
+                }
+            }
+            if (more) F::put(smem + (cur ^ 1) * F::kBuf, r, x);
+            __syncthreads();
+        }
+    }
+    if (j >= a.S) return;
+    const float pn = __builtin_amdgcn_exp2f(-kPShift<T>), norm = a.scale * pn / f;
+    const int64_t row = (at.b * a.S + j) * a.H + at.h;
+    T* kout = static_cast<T*>(g.dk) + row * N + 4 * half;
+    T* vout = static_cast<T*>(g.dv) + row * V + 4 * half;
+#pragma unroll
+    for (int i = 0; i < N / 32; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            *reinterpret_cast<uint2*>(kout + 32 * i + 8 * e) =
+                uint2{Act<T>::pair(dk[i][4 * e] * norm, dk[i][4 * e + 1] * norm),
+                      Act<T>::pair(dk[i][4 * e + 2] * norm, dk[i][4 * e + 3] * norm)};
+            *reinterpret_cast<uint2*>(vout + 32 * i + 8 * e) =
+                uint2{Act<T>::pair(dv[i][4 * e] * pn, dv[i][4 * e + 1] * pn),
+                      Act<T>::pair(dv[i][4 * e + 2] * pn, dv[i][4 * e + 3] * pn)};
+        }
+    if constexpr (P > 0) {
+        float* out = dpe + (bh * a.S + j) * P + 4 * half;
+#pragma unroll
+        for (int i = 0; i < P / 32; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const f16v& x = dk[N / 32 + i];
+                *reinterpret_cast<f4*>(out + 32 * i + 8 * e) = f4{x[4 * e] * norm, x[4 * e + 1] * norm,
+                                                                  x[4 * e + 2] * norm, x[4 * e + 3] * norm};
+            }
+    }
+}
+
+// The heads' position gradients summed in order: four channels a thread.
+template <typename T>
+__global__ __launch_bounds__(256) void dpe_kernel(const float* dpe, T* out, int64_t B, int64_t H, int64_t n) {
+    const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;     // of B n, n = S P / 4
+    if (i >= B * n) return;
+    const int64_t b = i / n;
+    const f4* from = reinterpret_cast<const f4*>(dpe) + (b * H) * n + (i - b * n);
+    f4 sum = from[0];
+    for (int64_t h = 1; h < H; ++h) {
+        const f4 x = from[h * n];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum[e] += x[e];
+    }
+    reinterpret_cast<uint2*>(out)[i] = uint2{Act<T>::pair(sum[0], sum[1]), Act<T>::pair(sum[2], sum[3])};
+}
+
+int64_t delta_bytes(int64_t B, int64_t T, int64_t H) { return (B * T * H * 4 + 15) / 16 * 16; }
+
+template <typename T, int N, int P>
+int launch(const kda_mla_expanded_bwd_args& g, hipStream_t stream) {
+    const kda_mla_expanded_args& a = g.fwd;
+    float* delta = static_cast<float*>(g.workspace);
+    float* dpe = reinterpret_cast<float*>(static_cast<char*>(g.workspace) + delta_bytes(a.B, a.T, a.H));
+    const int64_t qtiles = (a.T + 32 * kWaves - 1) / (32 * kWaves), ktiles = (a.S + 32 * kWaves - 1) / (32 * kWaves);
+    if (qtiles > 0)
+        dq_kernel<T, N, P><<<static_cast<unsigned>(qtiles * a.B * a.H), kThreads, 0, stream>>>(
+            g, delta, static_cast<int>(qtiles));
+    if (ktiles == 0) return hipGetLastError() == hipSuccess ? KDA_OK : KDA_ERR_LAUNCH;
+    dkv_kernel<T, N, P><<<static_cast<unsigned>(ktiles * a.B * a.H), kThreads, 0, stream>>>(g, delta, dpe);
+    if constexpr (P > 0) {
+        const int64_t n = a.S * P / 4;
+        dpe_kernel<T><<<static_cast<unsigned>((a.B * n + 255) / 256), 256, 0, stream>>>(dpe, static_cast<T*>(g.dk_pe),
+                                                                                       a.B, a.H, n);
+    }
+    return hipGetLastError() == hipSuccess ? KDA_OK : KDA_ERR_LAUNCH;
+}
+
+template <typename T>
+int launch_dims(const kda_mla_expanded_bwd_args& g, hipStream_t stream) {
+    switch (g.fwd.N + g.fwd.P) {
+        case 192: return launch<T, 128, 64>(g, stream);
+        case 160: return launch<T, 128, 32>(g, stream);
+        case 128: return g.fwd.N == 128 ? launch<T, 128, 0>(g, stream) : launch<T, 64, 64>(g, stream);
+        case 96: return launch<T, 64, 32>(g, stream);
+        default: return launch<T, 64, 0>(g, stream);
+    }
+}
+
+}  // namespace
+
+int64_t mla_expanded_bwd_workspace_bytes(int64_t B, int64_t T, int64_t S, int64_t H, int64_t P) {
+    return delta_bytes(B, T, H) + B * S * H * P * 4;
+}
+
+int mla_expanded_bwd_launch(const kda_mla_expanded_bwd_args& g, hipStream_t stream) {
+    return g.fwd.dtype == KDA_DTYPE_F16 ? launch_dims<_Float16>(g, stream) : launch_dims<bf16_t>(g, stream);
+}
+
+}  // namespace kda

@@ -39,13 +39,14 @@
 extern "C" {
 #endif
 
-#define KDA_ABI_VERSION 15
+#define KDA_ABI_VERSION 16
 
 /* Element types accepted at the boundary. */
 typedef enum kda_dtype {
     KDA_DTYPE_F32 = 0,
     KDA_DTYPE_F16 = 1,
-    KDA_DTYPE_BF16 = 2
+    KDA_DTYPE_BF16 = 2,
+    KDA_DTYPE_E4M3 = 3             /* 8 bits, of a latent cache only (kda_mla_*) */
 } kda_dtype;
 
 typedef enum kda_status {
@@ -481,6 +482,133 @@ typedef struct kda_output_bwd_args {
 
 size_t kda_output_bwd_workspace_size(int64_t B, int64_t T, int64_t H, int64_t V);
 int kda_output_bwd(const kda_output_bwd_args* args, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Latent attention: the full-attention mixer that stands between the KDA
+ * layers of the architecture (kimi_linear/mla.py).  A token's keys and values
+ * come from one latent vector of R channels, which a head's up-projections
+ * expand to N key and V value channels, and from P position channels that all
+ * heads share.  A cache holds a token as one row [latent R | position P].
+ *
+ * All four entry points: pointers on the current device, last dimensions
+ * contiguous, strides in elements; rows 16-byte aligned (base and strides);
+ * outputs overlap no input; asynchronous on `stream`, nothing allocated,
+ * nothing read back, capturable.  Workspaces are the caller's, 16-byte
+ * aligned; calls that may overlap in time need one each.  lengths, starts and
+ * counts are int32 device arrays read by the kernels (out-of-range values are
+ * clamped).
+ *
+ * Expanded form, for prompts and training:
+ *   s_tj = scale (q_t[0:N] . k_j + q_t[N:N+P] . k_pe_j)
+ *   o_t  = sum_j softmax_j(s_tj) v_j   over j < lengths[b], j <= starts[b] + t
+ * A query at or past position lengths[b] does not exist: its output is zero,
+ * as is that of a row with no key.  Rows of k, k_pe and v at or past
+ * lengths[b] are never read.  lengths NULL: S; starts NULL: S - T.
+ * Products in the activation type with fp32 sums, softmax in fp32. */
+typedef struct kda_mla_expanded_args {
+    int64_t B, T, S, H, N, P, V;   /* N = V in {64, 128}; P in {0, 32, 64} */
+    const void* q;                 /* [B, T, H, N+P] */
+    int64_t q_stride[3];           /* (batch, token, head) */
+    const void* k;                 /* [B, S, H, N] */
+    int64_t k_stride[3];
+    const void* k_pe;              /* [B, S, P]; NULL if P = 0 */
+    int64_t k_pe_stride[2];        /* (batch, token) */
+    const void* v;                 /* [B, S, H, V] */
+    int64_t v_stride[3];
+    const int32_t* lengths;        /* [B] or NULL */
+    const int32_t* starts;         /* [B], >= 0, or NULL */
+    void* o;                       /* [B, T, H, V] contiguous */
+    float* lse;                    /* [B, H, T] or NULL: log2 of the row's sum of exp(s), +inf for a row without keys;
+                                    * what the backward needs */
+    float scale;
+    int32_t dtype;                 /* KDA_DTYPE_F16 or KDA_DTYPE_BF16, of all activations */
+} kda_mla_expanded_args;
+
+int kda_mla_expanded_fwd(const kda_mla_expanded_args* args, void* stream);
+
+/* Its gradients, from d_o and the forward's arguments, o and lse.  Every sum
+ * in fp32 in a fixed order (the position part's over the heads too), rounded
+ * once to the activation type.  d_o of queries that do not exist is not read. */
+typedef struct kda_mla_expanded_bwd_args {
+    kda_mla_expanded_args fwd;     /* o and lse as kda_mla_expanded_fwd left them */
+    const void* d_o;               /* [B, T, H, V] */
+    int64_t d_o_stride[3];
+    void* dq;                      /* [B, T, H, N+P] contiguous */
+    void* dk;                      /* [B, S, H, N] contiguous */
+    void* dk_pe;                   /* [B, S, P] contiguous; NULL if P = 0 */
+    void* dv;                      /* [B, S, H, V] contiguous */
+    void* workspace;               /* kda_mla_expanded_bwd_workspace_size() bytes */
+} kda_mla_expanded_bwd_args;
+
+size_t kda_mla_expanded_bwd_workspace_size(int64_t B, int64_t T, int64_t S, int64_t H, int64_t P);
+int kda_mla_expanded_bwd(const kda_mla_expanded_bwd_args* args, void* stream);
+
+/* Absorbed form, for decoding: attention in the latent space over the cache
+ * itself, with q [B, T, H, R+P] whose first R channels have been taken through
+ * the head's key up-projection:
+ *   s_tj = scale (q_t . c_j),  o_t = sum_j softmax_j(s_tj) c_j[0:R]
+ * over j <= lengths[b] - T + t: the T queries are the last of the sequence's
+ * lengths[b] tokens.  A row without keys is zero.  Cache rows at or past
+ * lengths[b] are never read.  A KDA_DTYPE_E4M3 cache stands for
+ * cache[j] * cache_scale[j][0 (latent) or 1 (position)], scales at least 2^-60. */
+typedef struct kda_mla_absorbed_args {
+    int64_t B, T, H, S, R, P;      /* R in {128, 256, 512}; P in {0, 32, 64} */
+    const void* q;                 /* [B, T, H, R+P] */
+    int64_t q_stride[3];
+    const void* cache;             /* [B, S, R+P] */
+    int64_t cache_stride[2];       /* (batch, token) */
+    const float* cache_scale;      /* [B, S, 2], 8-bit caches only */
+    int64_t scale_stride[2];       /* (batch, token), even */
+    const int32_t* lengths;        /* [B] */
+    void* o;                       /* [B, T, H, R] contiguous */
+    float scale;
+    int32_t dtype;                 /* of q and o: KDA_DTYPE_F16 or KDA_DTYPE_BF16 */
+    int32_t cache_dtype;           /* dtype, or KDA_DTYPE_E4M3 */
+    void* workspace;               /* kda_mla_absorbed_workspace_size() bytes */
+} kda_mla_absorbed_args;
+
+size_t kda_mla_absorbed_workspace_size(int64_t B, int64_t T, int64_t H, int64_t S, int64_t R);
+int kda_mla_absorbed_fwd(const kda_mla_absorbed_args* args, void* stream);
+
+/* New rows behind the cached ones: x[b, t] goes to cache row lengths[b] + t for
+ * t < counts[b] (NULL: T); rows at or past S are dropped, all others left as
+ * they are.  With norm_weight the latent part is RMS-normalised first
+ * (x rsqrt(mean x^2 + eps) weight, in fp32).  Rounded once to the cache's type;
+ * in 8 bits x / scale to the nearest e4m3 value, with scale = max|x| / 448 (at
+ * least 2^-60) of the row's latent part and, separately, of its position part
+ * (1 if P = 0).  A row with a value that is not finite gets scales that are not. */
+typedef struct kda_mla_append_args {
+    int64_t B, T, S, R, P;
+    const void* x;                 /* [B, T, R+P] */
+    int64_t x_stride[2];           /* (batch, token) */
+    void* cache;                   /* [B, S, R+P] */
+    int64_t cache_stride[2];
+    float* cache_scale;            /* [B, S, 2], 8-bit caches only */
+    int64_t scale_stride[2];
+    const int32_t* lengths;        /* [B] rows held before the call */
+    const int32_t* counts;         /* [B] or NULL */
+    const void* norm_weight;       /* [R] contiguous, x dtype, or NULL */
+    float eps;
+    int32_t x_dtype;               /* KDA_DTYPE_F16 or KDA_DTYPE_BF16 */
+    int32_t cache_dtype;           /* x_dtype or KDA_DTYPE_E4M3 */
+} kda_mla_append_args;
+
+int kda_mla_cache_append(const kda_mla_append_args* args, void* stream);
+
+/* An 8-bit cache's first S rows back in 16 bits: out = value * scale rounded
+ * once; zeros in rows at or past lengths[b] (NULL: S). */
+typedef struct kda_mla_read_args {
+    int64_t B, S, R, P;
+    const void* cache;             /* [B, >= S, R+P] e4m3 */
+    int64_t cache_stride[2];
+    const float* cache_scale;      /* [B, >= S, 2] */
+    int64_t scale_stride[2];
+    const int32_t* lengths;        /* [B] or NULL */
+    void* out;                     /* [B, S, R+P] contiguous */
+    int32_t out_dtype;             /* KDA_DTYPE_F16 or KDA_DTYPE_BF16 */
+} kda_mla_read_args;
+
+int kda_mla_cache_read(const kda_mla_read_args* args, void* stream);
 
 /* Human-readable name of a kda_status code (static storage). */
 const char* kda_status_str(int status);

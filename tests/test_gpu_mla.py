@@ -1,0 +1,562 @@
+"""Latent attention and its cache against their formulas in float64.
+
+Bounds are per element, from the roundings the kernels make: u is half a step
+of the activation type (``finfo.eps / 2``), E the relative error of a softmax
+weight from fp32 scores and exponentials.  A score's sum of D products in fp32
+is off by at most D 2^-24 times the sum of their magnitudes; at these tests'
+D <= 576 and magnitudes (below 60 after scaling) that is 2e-3 in the worst
+case and 2^-24 sqrt(D) 60 = 9e-5 where roundings are independent; the
+exponential adds 2^-22.  E = 4e-4.
+
+* forward: weights rounded to the type (u), sums in fp32, output rounded (u):
+  |o - o'| <= (u + E) sum p |v| + u |o|
+* dv: the same with |do|.  ds = p (dp - delta): rounded (u), delta from the
+  rounded o (u sum |do o|), dp's fp32 sum (2^-20 sum |do v| covers 128 terms):
+  |dds| <= (u + 2E) |ds| + p (u sum |do o| + 2^-20 sum |do v|), and dq and dk
+  are sums of it against |k| and |q|, rounded once (u).
+"""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda:0"
+E = 4e-4
+F8 = torch.float8_e4m3fn
+BF16, F16 = torch.bfloat16, torch.float16
+
+
+def half_step(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def rand(*shape, seed, dtype=torch.float64, std=1.0):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    return (torch.randn(*shape, device=DEV, generator=g, dtype=torch.float64) * std).to(dtype)
+
+
+def i32(values):
+    return torch.tensor(values, dtype=torch.int32, device=DEV)
+
+
+def close(name, got, want, bound):
+    """Every element within its bound (plus the smallest step of a 16-bit type)."""
+    assert got.shape == want.shape, (name, got.shape, want.shape)
+    assert torch.isfinite(got.double()).all(), f"{name} is not finite"
+    off = (got.double() - want).abs() - bound - 2.0 ** -24
+    worst = off.max().item() if off.numel() else -1.0
+    assert worst <= 0, f"{name}: {worst:.3e} over its bound, {int((off > 0).sum())} of {off.numel()} elements"
+
+
+# ---- the formulas -----------------------------------------------------------
+
+def mask_of(T, S, lengths, starts):
+    n = torch.tensor(lengths, device=DEV).clamp(0, S)[:, None]
+    pos = torch.tensor(starts, device=DEV)[:, None] + torch.arange(T, device=DEV)
+    return (torch.arange(S, device=DEV) <= pos[..., None]) & (torch.arange(S, device=DEV) < n[..., None]) & (
+        pos < n)[..., None]                                                      # [B, T, S]
+
+
+def weights(s, mask):
+    s = s.masked_fill(~mask, -torch.inf)
+    e = torch.exp(s - s.amax(-1, keepdim=True).nan_to_num(neginf=0.0))
+    return e / e.sum(-1, keepdim=True).clamp_min(1e-300)
+
+
+def expanded_ref(q, kn, pe, v, lengths, starts, scale, d_o=None):
+    """(o, its bound) and, with d_o, {gradient: (value, bound)}; all [B, tokens, ...] in float64."""
+    u = half_step(q.dtype)
+    B, T, H, _ = q.shape
+    S, N = kn.shape[1], kn.shape[3]
+    mask = mask_of(T, S, lengths, starts)[:, None]
+    keep = (torch.arange(S, device=DEV) < torch.tensor(lengths, device=DEV)[:, None])[:, :, None, None]
+    Q = q.double().transpose(1, 2)
+    K = torch.where(keep, kn.double(), 0).transpose(1, 2)
+    V = torch.where(keep, v.double(), 0).transpose(1, 2)
+    if pe is not None:
+        Pe = torch.where(keep[..., 0], pe.double(), 0)
+        K = torch.cat([K, Pe[:, None].expand(B, H, S, pe.shape[-1])], -1)
+    p = weights(Q @ K.transpose(2, 3) * scale, mask)
+    o = p @ V
+    bound = (u + E) * (p @ V.abs()) + u * o.abs()
+    if d_o is None:
+        return o.transpose(1, 2), bound.transpose(1, 2)
+    dO = torch.where(mask.any(-1)[..., None], d_o.double().transpose(1, 2), 0)
+    dp = dO @ V.transpose(2, 3)
+    ds = p * (dp - (dO * o).sum(-1, keepdim=True))
+    e_ds = (u + 2 * E) * ds.abs() + p * (u * (dO * o).abs().sum(-1, keepdim=True)
+                                         + 2.0 ** -20 * (dO.abs() @ V.abs().transpose(2, 3)))
+    e_ds = e_ds + 2.0 ** -30 * ds.abs().amax((-1, -2), keepdim=True)     # fp16: ds far below the largest of its wave
+    dv, e_dv = p.transpose(2, 3) @ dO, (u + E) * (p.transpose(2, 3) @ dO.abs())
+    dq, e_dq = scale * ds @ K, scale * e_ds @ K.abs()
+    dk, e_dk = scale * ds.transpose(2, 3) @ Q, scale * e_ds.transpose(2, 3) @ Q.abs()
+
+    def out(x, e):
+        return x.transpose(1, 2), (e + u * x.abs()).transpose(1, 2)
+
+    grads = {"q": out(dq, e_dq), "k_nope": out(dk[..., :N], e_dk[..., :N]), "v": out(dv, e_dv)}
+    if pe is not None:
+        x, e = dk[..., N:].sum(1), e_dk[..., N:].sum(1)
+        grads["k_pe"] = (x, e + u * x.abs())
+    return o.transpose(1, 2), bound.transpose(1, 2), grads
+
+
+def absorbed_ref(q, rows, lengths, rank, scale):
+    u = half_step(q.dtype)
+    B, T, H, D = q.shape
+    S = rows.shape[1]
+    mask = mask_of(T, S, lengths, [n - T for n in lengths])
+    rows = torch.where((torch.arange(S, device=DEV) < torch.tensor(lengths, device=DEV)[:, None])[..., None],
+                       rows.double(), 0)
+    p = weights(torch.einsum("bthd,bsd->bhts", q.double(), rows) * scale, mask[:, None])
+    o = (p @ rows[:, None, :, :rank]).transpose(1, 2)
+    return o, (u + E) * (p @ rows[:, None, :, :rank].abs()).transpose(1, 2) + u * o.abs()
+
+
+def quantised(x, rank):
+    """x [B, S, D] float as the 8-bit cache holds it."""
+    scale = torch.stack([x[..., :rank].float().abs().amax(-1),
+                         x[..., rank:].float().abs().amax(-1) if x.shape[-1] > rank else
+                         torch.full(x.shape[:2], 448.0, device=DEV)], -1).clamp_min(448 * 2.0 ** -60)
+    scale = scale / torch.full_like(scale, 448.0)        # (by a Python number torch multiplies with its rounded inverse)
+    each = torch.cat([scale[..., :1].expand(*x.shape[:2], rank), scale[..., 1:].expand(*x.shape[:2], x.shape[-1] - rank)], -1)
+    return (x.float() / each).clamp(-448, 448).to(F8), scale
+
+
+def dequantised(data, scale, rank):
+    return torch.cat([data[..., :rank].double() * scale[..., :1].double(),
+                      data[..., rank:].double() * scale[..., 1:].double()], -1)
+
+
+# ---- expanded ---------------------------------------------------------------
+
+def inputs(B, T, S, H, N, P, dtype, seed=0):
+    return (rand(B, T, H, N + P, seed=seed, dtype=dtype), rand(B, S, H, N, seed=seed + 1, dtype=dtype),
+            rand(B, S, P, seed=seed + 2, dtype=dtype) if P else None, rand(B, S, H, N, seed=seed + 3, dtype=dtype))
+
+
+EXPANDED = [
+    # B, T, S, H, N, P, dtype, lengths, starts
+    (1, 1, 1, 1, 128, 64, BF16, None, None),
+    (2, 1, 300, 3, 128, 64, F16, [300, 77], [299, 76]),          # one new token each, of two lengths
+    (1, 65, 65, 2, 64, 32, BF16, None, None),
+    (2, 200, 200, 3, 128, 64, F16, [200, 131], None),            # a padded batch
+    (3, 70, 190, 2, 64, 64, BF16, [190, 0, 130], [120, 0, 60]),  # pieces of prompts and an empty slot
+    (1, 33, 500, 1, 128, 0, F16, None, None),
+    (1, 300, 300, 2, 64, 0, BF16, None, None),
+    (1, 129, 257, 5, 128, 32, BF16, None, [100]),                # queries end before the keys do
+    (2, 40, 16, 2, 64, 64, F16, None, None),                     # more queries than keys: the first see none
+    (1, 600, 600, 16, 128, 64, BF16, None, None),
+    (4, 700, 700, 24, 64, 32, F16, None, None),                  # enough rows for the widest workgroups
+]
+
+
+@pytest.mark.parametrize("case", EXPANDED, ids=lambda c: "-".join(map(str, c[:6])) + "-" + str(c[6])[6:])
+def test_expanded_forward_and_gradients(kda_pkg, case):
+    B, T, S, H, N, P, dtype, lengths, starts = case
+    q, kn, pe, v = inputs(B, T, S, H, N, P, dtype)
+    n, st = lengths or [S] * B, starts or [S - T] * B
+    for b in range(B):                       # what the kernels must not read
+        for x in (kn, v, pe):
+            if x is not None:
+                x[b, n[b]:] = float("nan")
+    d_o = rand(B, T, H, N, seed=9, dtype=dtype)
+    leaves = [x.requires_grad_() for x in (q, kn, pe, v) if x is not None]
+    kw = dict(lengths=None if lengths is None else i32(lengths), starts=None if starts is None else i32(starts))
+    o = kda_pkg.mla_expanded(q, kn, pe, v, **kw)
+    grads = torch.autograd.grad(o, leaves, d_o)
+    with torch.no_grad():
+        assert torch.equal(o, kda_pkg.mla_expanded(q, kn, pe, v, **kw))
+        want, bound, ref = expanded_ref(q, kn, pe, v, n, st, (N + P) ** -0.5, d_o)
+    close("o", o, want, bound)
+    names = [m for m, x in (("q", q), ("k_nope", kn), ("k_pe", pe), ("v", v)) if x is not None]
+    for m, g in zip(names, grads):
+        close("d" + m, g, *ref[m])
+
+
+def test_expanded_gradients_against_differences(kda_pkg):
+    """The directional derivative of sum(o w) in each input, by central differences of the float64 formula."""
+    B, T, S, H, N, P = 1, 40, 56, 2, 64, 32
+    q, kn, pe, v = inputs(B, T, S, H, N, P, BF16, seed=20)
+    w = rand(B, T, H, N, seed=30, dtype=BF16)
+    leaves = [x.requires_grad_() for x in (q, kn, pe, v)]
+    grads = torch.autograd.grad(kda_pkg.mla_expanded(q, kn, pe, v), leaves, w)
+    base = [x.detach().double() for x in (q, kn, pe, v)]
+
+    def value(xs):
+        K = torch.cat([xs[1], xs[2][:, :, None].expand(B, S, H, P)], -1).transpose(1, 2)
+        p = weights(xs[0].transpose(1, 2) @ K.transpose(2, 3) * (N + P) ** -0.5, mask_of(T, S, [S], [S - T])[:, None])
+        return ((p @ xs[3].transpose(1, 2)).transpose(1, 2) * w.double()).sum()
+
+    _, _, ref = expanded_ref(*(x.detach() for x in (q, kn, pe, v)), [S], [S - T], (N + P) ** -0.5, w)
+    for i, m in enumerate(("q", "k_nope", "k_pe", "v")):
+        d = rand(*base[i].shape, seed=40 + i)
+        up, down = list(base), list(base)
+        up[i], down[i] = base[i] + 1e-5 * d, base[i] - 1e-5 * d
+        slope = (value(up) - value(down)).item() / 2e-5
+        got = (grads[i].double() * d).sum().item()
+        # each element's bound against |d|, and the differences' own error (third derivatives, 1e-10, and roundings, 1e-9)
+        assert abs(got - slope) <= (ref[m][1] * d.abs()).sum().item() + 1e-6, m
+
+
+def test_expanded_small_fp16_gradients(kda_pkg):
+    """Gradients a loss scale has left near fp16's smallest: ds is 2^-24 and below, its sums are not."""
+    q, kn, pe, v = inputs(1, 256, 256, 2, 64, 32, F16, seed=50)
+    d_o = rand(1, 256, 2, 64, seed=51, dtype=F16, std=2.0 ** -9)
+    leaves = [x.requires_grad_() for x in (q, kn, pe, v)]
+    grads = torch.autograd.grad(kda_pkg.mla_expanded(q, kn, pe, v), leaves, d_o)
+    _, _, ref = expanded_ref(*(x.detach() for x in leaves), [256], [0], 96 ** -0.5, d_o)
+    for m, g in zip(("q", "k_nope", "k_pe", "v"), grads):
+        close("d" + m, g, *ref[m])
+
+
+def test_expanded_views_streams_and_types(kda_pkg):
+    B, T, H, N, P = 2, 90, 3, 128, 64
+    kv = rand(B, T, H, 2 * N, seed=60, dtype=BF16)
+    wide = rand(B, T, 700, seed=61, dtype=BF16)
+    q = rand(B, H, T, N + P, seed=62, dtype=BF16).transpose(1, 2)
+    kn, v, pe = kv[..., :N], kv[..., N:], wide[..., 512:512 + P]
+    want = kda_pkg.mla_expanded(q.contiguous(), kn.contiguous(), pe.contiguous(), v.contiguous())
+    assert torch.equal(kda_pkg.mla_expanded(q, kn, pe, v), want)
+    # unaligned rows and reversed channels are copied first; 64-bit lengths are taken too
+    odd = rand(B, T, P + 1, seed=61, dtype=BF16)
+    odd[..., 1:] = pe
+    assert torch.equal(kda_pkg.mla_expanded(q, kn, odd[..., 1:], v, lengths=torch.full((B,), T, device=DEV)), want)
+    # one sequence for all: batch stride 0
+    one = kda_pkg.mla_expanded(q, kn[:1].expand(B, T, H, N), pe[:1].expand(B, T, P), v[:1].expand(B, T, H, N))
+    assert torch.equal(one[0], want[0])
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        other = kda_pkg.mla_expanded(q, kn, pe, v)
+    torch.cuda.current_stream().wait_stream(s)
+    assert torch.equal(other, want)
+    # fp32 keys are taken in q's type, as under mixed precision; their gradient comes back in fp32
+    k32 = kn.float().contiguous().requires_grad_()
+    o = kda_pkg.mla_expanded(q, k32, pe, v)
+    assert torch.equal(o, want)
+    assert torch.autograd.grad(o.float().sum(), k32)[0].dtype == torch.float32
+
+
+def test_expanded_empty(kda_pkg):
+    q, kn, pe, v = inputs(2, 0, 5, 2, 64, 32, BF16)
+    leaves = [x.requires_grad_() for x in (q, kn, pe, v)]
+    o = kda_pkg.mla_expanded(q, kn, pe, v)
+    assert o.shape == (2, 0, 2, 64)
+    for g in torch.autograd.grad(o.sum(), leaves):
+        assert (g == 0).all()
+    q, kn, pe, v = inputs(2, 7, 0, 2, 64, 32, BF16)
+    assert (kda_pkg.mla_expanded(q, kn, pe, v) == 0).all()
+
+
+def test_expanded_far_offsets(kda_pkg):
+    """A batch stride past 2^32 bytes."""
+    H, N, T, far = 1, 64, 20, 2 ** 31 + 2 ** 20
+    store = torch.empty(far + T * H * N, dtype=BF16, device=DEV)
+    kn = store.as_strided((2, T, H, N), (far, H * N, N, 1))
+    src = rand(2, T, H, N, seed=70, dtype=BF16)
+    kn.copy_(src)
+    q, v = rand(2, T, H, N, seed=71, dtype=BF16), rand(2, T, H, N, seed=72, dtype=BF16)
+    assert torch.equal(kda_pkg.mla_expanded(q, kn, None, v), kda_pkg.mla_expanded(q, src, None, v))
+
+
+def test_expanded_captured(kda_pkg):
+    """Forward and backward in a graph whose lengths change between replays, beside eager work."""
+    B, T, H, N, P = 2, 150, 2, 64, 32
+    q, kn, pe, v = inputs(B, T, T, H, N, P, BF16, seed=80)
+    d_o = rand(B, T, H, N, seed=84, dtype=BF16)
+    leaves = [x.requires_grad_() for x in (q, kn, pe, v)]
+    lengths = i32([T, T])
+
+    def step():
+        o = kda_pkg.mla_expanded(q, kn, pe, v, lengths=lengths)
+        return [o.detach(), *torch.autograd.grad(o, leaves, d_o)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for n in ([150, 150], [1, 100], [0, 64], [150, 149]):
+        lengths.copy_(i32(n))
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(got, step()):
+            assert torch.equal(a, b), n
+
+
+# ---- absorbed ---------------------------------------------------------------
+
+ABSORBED = [
+    # B, T, H, S, R, P, dtype, lengths
+    (1, 1, 16, 1, 512, 64, BF16, [1]),
+    (1, 1, 16, 200, 512, 64, F16, [199]),
+    (3, 1, 16, 70, 512, 64, BF16, [70, 0, 33]),
+    (5, 1, 7, 1000, 256, 32, F16, [1000, 1, 999, 0, 517]),        # shared among workgroups, an idle slot
+    (2, 3, 5, 2000, 128, 0, BF16, [2000, 2]),                     # several tokens; the second has fewer than T
+    (2, 6, 20, 777, 512, 64, F16, [777, 500]),
+    (70, 1, 16, 600, 128, 64, BF16, [(37 * b) % 601 for b in range(70)]),
+    (1100, 1, 4, 520, 128, 32, F16, [(211 * b) % 521 for b in range(1100)]),   # one workgroup a sequence
+    (1, 1, 64, 5000, 512, 64, BF16, [4999]),                      # four row tiles
+    (1, 2, 16, 9000, 256, 64, BF16, [8999]),
+    (2, 1, 16, 30000, 512, 0, F16, [30000, 12345]),
+]
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+@pytest.mark.parametrize("case", ABSORBED, ids=lambda c: "-".join(map(str, c[:6])) + "-" + str(c[6])[6:])
+def test_absorbed(kda_pkg, case, bits):
+    B, T, H, S, R, P, dtype, lengths = case
+    q = rand(B, T, H, R + P, seed=1, dtype=dtype, std=R ** -0.5 * 12)
+    rows = rand(B, S, R + P, seed=2, dtype=torch.float32)
+    rows[..., R:] *= 3
+    cache, scale = (rows.to(dtype), None) if bits == 16 else quantised(rows, R)
+    held = cache.double() if bits == 16 else dequantised(cache, scale, R)
+    for b in range(B):                       # unwritten memory
+        if bits == 16:
+            cache[b, lengths[b]:] = float("nan")
+        else:
+            cache.view(torch.uint8)[b, lengths[b]:] = 0x7f
+            scale[b, lengths[b]:] = float("nan")
+    got = kda_pkg.mla_absorbed(q, cache, i32(lengths), R, (128 + P) ** -0.5, cache_scale=scale)
+    want, bound = absorbed_ref(q, held, lengths, R, (128 + P) ** -0.5)
+    close("o", got, want, bound)
+    assert torch.equal(got, kda_pkg.mla_absorbed(q, cache, i32(lengths), R, (128 + P) ** -0.5, cache_scale=scale))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_absorbed_8bit_scales_of_any_size(kda_pkg, dtype):
+    """Scales from 2^-60 (rows of zeros) over six orders of magnitude: weights keep their precision."""
+    S, R, P = 300, 128, 32
+    rows = rand(1, S, R + P, seed=5, dtype=torch.float32) * torch.logspace(-5, 1, S, device=DEV)[None, :, None]
+    rows[:, ::7] = 0
+    cache, scale = quantised(rows, R)
+    q = rand(1, 1, 16, R + P, seed=6, dtype=dtype, std=0.5)
+    got = kda_pkg.mla_absorbed(q, cache, i32([S]), R, 0.1, cache_scale=scale)
+    want, bound = absorbed_ref(q, dequantised(cache, scale, R), [S], R, 0.1)
+    close("o", got, want, bound)
+    tiny = rows * 1e-4                       # every value is small: so is the output, at the same relative error
+    cache, scale = quantised(tiny, R)
+    got = kda_pkg.mla_absorbed(q, cache, i32([S]), R, 0.1, cache_scale=scale)
+    want, bound = absorbed_ref(q, dequantised(cache, scale, R), [S], R, 0.1)
+    close("o", got, want, bound)
+
+
+def test_absorbed_far_rows(kda_pkg):
+    """A cache past 2^32 bytes: rows of zeros but for some, so the softmax has a closed form."""
+    R, P = 512, 64
+    S = 2 ** 32 // ((R + P) * 2) + 5000
+    cache = torch.zeros(1, S, R + P, dtype=BF16, device=DEV)
+    at = torch.tensor([0, 1000, S // 2, S - 3001, S - 1], device=DEV)
+    some = rand(5, R + P, seed=7, dtype=BF16)
+    cache[0, at] = some
+    q = rand(1, 1, 4, R + P, seed=8, dtype=BF16, std=0.7)
+    got = kda_pkg.mla_absorbed(q, cache, i32([S]), R, 1.0)[0, 0]
+    s = q[0, 0].double() @ some.double().T
+    w = torch.exp(s)
+    den = w.sum(1, keepdim=True) + (S - 5)
+    p = w / den
+    want, u = p @ some[:, :R].double(), half_step(BF16)
+    close("o", got, want, (u + E) * (p @ some[:, :R].double().abs()) + u * want.abs())
+
+
+def test_absorbed_views_streams_and_graph(kda_pkg):
+    B, H, S, R, P = 4, 16, 900, 128, 64
+    store = rand(B + 1, S + 30, R + P + 64, seed=11, dtype=BF16)
+    cache = store[1:, 10:S + 10, :R + P]
+    q = rand(B, H, 1, R + P, seed=12, dtype=BF16).transpose(1, 2)
+    n = [900, 0, 451, 32]
+    want = kda_pkg.mla_absorbed(q.contiguous(), cache.contiguous(), i32(n), R, 0.05)
+    lengths = i32(n)
+    assert torch.equal(kda_pkg.mla_absorbed(q, cache, lengths, R, 0.05), want)
+    assert torch.equal(kda_pkg.mla_absorbed(q, cache, lengths.long(), R, 0.05), want)
+    # lengths out of range count as S and 0
+    assert torch.equal(kda_pkg.mla_absorbed(q, cache, i32([5000, -7, 451, 32]), R, 0.05), want)
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    got = []
+    for s in streams:                        # calls at once, each with a workspace of its own
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            got.append(kda_pkg.mla_absorbed(q, cache, lengths, R, 0.05))
+    for s in streams:
+        torch.cuda.current_stream().wait_stream(s)
+    assert all(torch.equal(g, want) for g in got)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        kda_pkg.mla_absorbed(q, cache, lengths, R, 0.05)
+    torch.cuda.current_stream().wait_stream(side)
+    graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
+    outs = []
+    for g in graphs:
+        with torch.cuda.graph(g):
+            outs.append(kda_pkg.mla_absorbed(q, cache, lengths, R, 0.05))
+    for n in ([900, 0, 451, 32], [1, 900, 0, 700], [0, 0, 0, 0], [33, 64, 65, 899]):
+        lengths.copy_(i32(n))
+        for g in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        want = kda_pkg.mla_absorbed(q, cache, lengths, R, 0.05)
+        assert all(torch.equal(o, want) for o in outs), n
+
+
+def test_absorbed_is_the_expanded_form(kda_pkg):
+    """The two forms of one attention: up-projections applied to the latents, or to q and o."""
+    B, S, H, N, P, R = 2, 130, 8, 128, 64, 256
+    cache = rand(B, S, R + P, seed=13, dtype=F16)
+    wk, wv = rand(H, N, R, seed=14, dtype=F16, std=R ** -0.5), rand(H, N, R, seed=15, dtype=F16, std=R ** -0.5)
+    q = rand(B, 1, H, N + P, seed=16, dtype=F16)
+    lat = cache[..., :R].double()
+    kn = torch.einsum("bsr,hnr->bshn", lat, wk.double()).to(F16)
+    v = torch.einsum("bsr,hnr->bshn", lat, wv.double()).to(F16)
+    full = kda_pkg.mla_expanded(q, kn, cache[..., R:].contiguous(), v)
+    qa = torch.cat([torch.einsum("bthn,hnr->bthr", q[..., :N].double(), wk.double()).to(F16), q[..., N:]], -1)
+    o = kda_pkg.mla_absorbed(qa, cache, i32([S, S]), R, (N + P) ** -0.5)
+    absorbed = torch.einsum("bthr,hnr->bthn", o.double(), wv.double())
+    # intermediate roundings of keys, values, queries and outputs (2^-11 each) move scores of size <= 6 and values of size <= 5
+    assert (full.double() - absorbed).abs().max().item() <= 2.0 ** -11 * (6 * 4 * 2 + 4) * 2
+
+
+# ---- the cache --------------------------------------------------------------
+
+CACHE = [
+    # B, T, S, R, P, dtype, lengths, counts
+    (1, 1, 1, 512, 64, BF16, [0], None),
+    (64, 1, 100, 512, 64, F16, [b % 101 for b in range(64)], None),          # some at the end: dropped
+    (3, 50, 120, 256, 32, BF16, [0, 100, 70], [50, 50, 13]),
+    (2, 37, 64, 128, 0, F16, [5, 27], [0, 37]),
+    (2, 9, 30, 512, 0, BF16, [-4, 2 ** 31 - 5], None),                       # held rows that cannot be
+]
+
+
+@pytest.mark.parametrize("norm", [False, True])
+@pytest.mark.parametrize("bits", [16, 8])
+@pytest.mark.parametrize("case", CACHE, ids=lambda c: "-".join(map(str, c[:5])) + "-" + str(c[5])[6:])
+def test_append(kda_pkg, case, bits, norm):
+    B, T, S, R, P, dtype, lengths, counts = case
+    x = rand(B, T, R + P, seed=21, dtype=dtype, std=2.0)
+    x[:, -1, R // 2:] = 0
+    x[0, 0] = 0
+    w = rand(R, seed=22, dtype=dtype) if norm else None
+    before = rand(B, S, R + P, seed=23, dtype=torch.float32)
+    cache, scale = (before.to(dtype), None) if bits == 16 else quantised(before, R)
+    raw = torch.int16 if bits == 16 else torch.uint8
+    old, old_scale = cache.clone(), None if scale is None else scale.clone()
+    out = kda_pkg.mla_cache_append(x, cache, i32(lengths), R, cache_scale=scale,
+                                   counts=None if counts is None else i32(counts), norm_weight=w, eps=1e-5)
+    assert out is None
+    y = x.double()
+    if norm:
+        y[..., :R] = y[..., :R] * torch.rsqrt(y[..., :R].square().mean(-1, keepdim=True) + 1e-5) * w.double()
+    touched = torch.zeros(B, S, dtype=torch.bool, device=DEV)
+    for b in range(B):
+        for t in range(T if counts is None else counts[b]):
+            at = lengths[b] + t
+            if not (0 <= lengths[b] and at < S):
+                continue
+            touched[b, at] = True
+            if bits == 16:
+                if norm:                                # fp32 arithmetic (2^-21), rounded once
+                    close("row", cache[b, at], y[b, t], (half_step(dtype) + 2.0 ** -21) * y[b, t].abs())
+                else:
+                    assert torch.equal(cache[b, at], x[b, t])
+            else:
+                want, s = quantised(y[b, t][None, None], R)
+                if not norm:                            # the same divisions: the same bits
+                    assert torch.equal(scale[b, at], s[0, 0])
+                    assert torch.equal(cache.view(torch.uint8)[b, at], want.view(torch.uint8)[0, 0])
+                else:                                   # half a step of e4m3, 2^-4, of 2^-9 below its normal range
+                    assert ((scale[b, at] - s[0, 0]).abs() <= 2.0 ** -21 * s[0, 0]).all()
+                    got = dequantised(cache[b:b + 1, at:at + 1], scale[b:b + 1, at:at + 1], R)[0, 0]
+                    step = torch.cat([s[0, 0, :1].expand(R), s[0, 0, 1:].expand(P)]).double() * 2.0 ** -10
+                    close("row", got, y[b, t], (2.0 ** -4 + 2.0 ** -20) * y[b, t].abs() + step)
+    keep = ~touched
+    assert torch.equal(cache.view(raw)[keep], old.view(raw)[keep])
+    if scale is not None:
+        assert torch.equal(scale[keep], old_scale[keep])
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("B,S,R,P,n", [(1, 1, 128, 0, None), (3, 77, 512, 64, [77, 0, 13]), (2, 300, 256, 32, None)])
+def test_read(kda_pkg, B, S, R, P, n, dtype):
+    cache, scale = quantised(rand(B, S, R + P, seed=31, dtype=torch.float32), R)
+    want = dequantised(cache, scale, R).to(torch.float32).to(dtype)     # the product of an e4m3 value and a scale, in fp32
+    if n is not None:
+        for b in range(B):
+            want[b, n[b]:] = 0
+            cache.view(torch.uint8)[b, n[b]:] = 0x7f
+    got = kda_pkg.mla_cache_read(cache, scale, R, dtype=dtype, lengths=None if n is None else i32(n))
+    assert torch.equal(got, want)
+    assert torch.equal(kda_pkg.mla_cache_read(cache, scale, R, dtype=dtype, tokens=S // 2,
+                                              lengths=None if n is None else i32(n)), want[:, :S // 2])
+
+
+def test_not_finite_rows(kda_pkg):
+    """A row with an infinity or a NaN reads back as not finite; its neighbours do not notice."""
+    R, P = 128, 32
+    x = rand(1, 4, R + P, seed=32, dtype=BF16)
+    x[0, 1, 3], x[0, 2, R + 1] = float("inf"), float("nan")
+    cache, scale = torch.zeros(1, 4, R + P, dtype=F8, device=DEV), torch.ones(1, 4, 2, device=DEV)
+    kda_pkg.mla_cache_append(x, cache, i32([0]), R, cache_scale=scale)
+    got = torch.isfinite(kda_pkg.mla_cache_read(cache, scale, R).float())
+    assert got[0, 0].all() and got[0, 3].all()
+    assert not got[0, 1, :R].any() and got[0, 1, R:].all() and got[0, 2, :R].all() and not got[0, 2, R:].any()
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+def test_run_together(kda_pkg, bits):
+    """A prompt in two pieces through the expanded form, then tokens through the absorbed one, captured; every
+    step against the formula over what the cache holds."""
+    B, H, N, P, R, S, dtype = 2, 4, 128, 64, 256, 96, BF16
+    scale = (N + P) ** -0.5
+    wk, wv = rand(H, N, R, seed=41, dtype=dtype, std=R ** -0.5), rand(H, N, R, seed=42, dtype=dtype, std=R ** -0.5)
+    w = rand(R, seed=43, dtype=dtype, std=0.1) + 1
+    cache = torch.full((B, S, R + P), 0x7f if bits == 8 else -1, device=DEV, dtype=torch.uint8 if bits == 8 else torch.int16)
+    cache = cache.view(F8 if bits == 8 else dtype)
+    scales = torch.full((B, S, 2), float("nan"), device=DEV) if bits == 8 else None
+    lengths = torch.zeros(B, dtype=torch.int32, device=DEV)
+
+    def held():
+        return cache.double() if bits == 16 else dequantised(cache, scales, R)
+
+    for piece, T in enumerate((40, 23)):
+        x = rand(B, T, R + P, seed=50 + piece, dtype=dtype, std=1.5)
+        q = rand(B, T, H, N + P, seed=60 + piece, dtype=dtype)
+        kda_pkg.mla_cache_append(x, cache, lengths, R, cache_scale=scales, norm_weight=w)
+        starts = lengths.clone()
+        lengths += T
+        n = int(lengths[0])
+        rows = cache[:, :n] if bits == 16 else kda_pkg.mla_cache_read(cache, scales, R, dtype=dtype, tokens=n, lengths=lengths)
+        kn = torch.einsum("bsr,hnr->bshn", rows[..., :R].float(), wk.float()).to(dtype)
+        v = torch.einsum("bsr,hnr->bshn", rows[..., :R].float(), wv.float()).to(dtype)
+        o = kda_pkg.mla_expanded(q, kn, rows[..., R:], v, lengths=lengths, starts=starts)
+        close("piece", o, *expanded_ref(q, kn, rows[..., R:], v, [n] * B, [n - T] * B, scale))
+    x_in, q_in = torch.zeros(B, 1, R + P, dtype=dtype, device=DEV), torch.zeros(B, 1, H, R + P, dtype=dtype, device=DEV)
+
+    def step():
+        kda_pkg.mla_cache_append(x_in, cache, lengths, R, cache_scale=scales, norm_weight=w)
+        lengths.add_(1)
+        return kda_pkg.mla_absorbed(q_in, cache, lengths, R, scale, cache_scale=scales)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    lengths.sub_(1)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for t in range(5):
+        x_in.copy_(rand(B, 1, R + P, seed=70 + t, dtype=dtype))
+        q_in.copy_(rand(B, 1, H, R + P, seed=80 + t, dtype=dtype, std=0.7))
+        graph.replay()
+        n = int(lengths[0])
+        assert n == 64 + t
+        close("token", out, *absorbed_ref(q_in, held(), [n] * B, R, scale))
