@@ -325,33 +325,52 @@ __global__ __launch_bounds__(64 * kWaves, 1) void absorbed_shared_kernel(kda_mla
     }
 }
 
-// The parts of one row's sequence joined, in order: grid (row tiles, 16), R / 4 threads.
-template <typename T, int R>
-__global__ __launch_bounds__(R / 4) void join_kernel(kda_mla_absorbed_args a, int rts, int groups) {
+// The parts of one row's sequence joined: grid (row tiles, 16, R / 64), sixteen
+// lanes on 64 channels and sixteen groups of them on every sixteenth part, whose
+// sums meet in LDS, in an order that the lengths alone decide.
+constexpr int kJoinGroups = 16;
+template <typename T>
+__global__ __launch_bounds__(16 * kJoinGroups) void join_kernel(kda_mla_absorbed_args a, int rts, int groups) {
     const int64_t v = blockIdx.x, b = v / rts, nv = a.B * rts;
     const int rows = static_cast<int>(a.T * a.H), m = static_cast<int>(v - b * rts) * kRowTile + blockIdx.y;
     if (m >= rows) return;
-    T* out = static_cast<T*>(a.o) + (b * rows + m) * R + 4 * threadIdx.x;
+    const int c = 64 * blockIdx.z + 4 * (threadIdx.x & 15), group = threadIdx.x >> 4;
+    const Workspace ws = carve(a.workspace, slots(groups, nv), a.R);
+    const int2 span = tokens(a.lengths, b, a.S) > 0 ? ws.span[v] : int2{0, -1};
+    if (span.x == span.y) return;                // one workgroup had it all, and wrote the result
+    const float2* ml = ws.ml + v * kRowTile + blockIdx.y;
+    const float* o = ws.o + (v * kRowTile + blockIdx.y) * a.R + c;
+    float top = kNoMax, den = 0.f;
     f4 r{};
-    float norm = 0.f;
-    if (tokens(a.lengths, b, a.S) > 0) {
-        const Workspace ws = carve(a.workspace, slots(groups, nv), R);
-        const int2 span = ws.span[v];
-        if (span.x == span.y) return;            // one workgroup had it all, and wrote the result
-        float top = kNoMax, den = 0.f;
-        for (int g = span.x; g <= span.y; ++g) top = fmaxf(top, ws.ml[(g + v) * kRowTile + blockIdx.y].x);
-        for (int g = span.x; g <= span.y; ++g) {
-            const float2 ml = ws.ml[(g + v) * kRowTile + blockIdx.y];
-            if (ml.y == 0.f) continue;
-            const float w = __builtin_amdgcn_exp2f(ml.x - top);
-            den = fmaf(w, ml.y, den);
-            const f4 x = *reinterpret_cast<const f4*>(ws.o + ((g + v) * kRowTile + blockIdx.y) * R + 4 * threadIdx.x);
+    for (int g = span.x + group; g <= span.y; g += kJoinGroups) {
+        const float2 x = ml[g * kRowTile];
+        const f4 y = *reinterpret_cast<const f4*>(o + static_cast<int64_t>(g) * kRowTile * a.R);
+        const float now = fmaxf(top, x.x), f0 = __builtin_amdgcn_exp2f(top - now);
+        const float f1 = x.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(x.x - now);
+        top = now;
+        den = den * f0 + x.y * f1;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) r[e] = fmaf(w, x[e], r[e]);
-        }
-        norm = den == 0.f ? 0.f : 1.f / den;
+        for (int e = 0; e < 4; ++e) r[e] = r[e] * f0 + y[e] * f1;
     }
-    *reinterpret_cast<uint2*>(out) =
+    __shared__ f4 sums[kJoinGroups][16];
+    __shared__ float2 stats[kJoinGroups];
+    sums[group][threadIdx.x & 15] = r;
+    if ((threadIdx.x & 15) == 0) stats[group] = float2{top, den};
+    __syncthreads();
+    if (group != 0) return;
+    const int n = min(kJoinGroups, span.y - span.x + 1);
+    for (int g = 0; g < n; ++g) top = fmaxf(top, stats[g].x);
+    den = 0.f;
+    r = f4{};
+    for (int g = 0; g < n; ++g) {
+        const float w = __builtin_amdgcn_exp2f(stats[g].x - top);
+        den = fmaf(w, stats[g].y, den);
+        const f4 y = sums[g][threadIdx.x];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) r[e] = fmaf(w, y[e], r[e]);
+    }
+    const float norm = den == 0.f ? 0.f : 1.f / den;
+    *reinterpret_cast<uint2*>(static_cast<T*>(a.o) + (b * rows + m) * a.R + c) =
         uint2{Act<T>::pair(r[0] * norm, r[1] * norm), Act<T>::pair(r[2] * norm, r[3] * norm)};
 }
 
@@ -370,8 +389,8 @@ int launch(const kda_mla_absorbed_args& a, hipStream_t stream) {
         absorbed_kernel<T, F8, R, P><<<static_cast<unsigned>(nv), 64 * kWaves, 0, stream>>>(a, rts);
     } else {
         absorbed_shared_kernel<T, F8, R, P><<<kGroups, 64 * kWaves, 0, stream>>>(a, rts);
-        join_kernel<T, R><<<dim3(static_cast<unsigned>(nv), kRowTile), R / 4, 0, stream>>>(a, rts,
-                                                                                           static_cast<int>(kGroups));
+        join_kernel<T><<<dim3(static_cast<unsigned>(nv), kRowTile, R / 64), 16 * kJoinGroups, 0, stream>>>(
+            a, rts, static_cast<int>(kGroups));
     }
     return hipGetLastError() == hipSuccess ? KDA_OK : KDA_ERR_LAUNCH;
 }

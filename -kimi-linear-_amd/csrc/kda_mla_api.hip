@@ -25,6 +25,9 @@ bool rows_ok(const void* p, const int64_t* stride, int n, int64_t bytes) {
     return true;
 }
 
+// Token strides whose tiles of up to 128 rows a 32-bit offset reaches.
+bool near(int64_t stride) { return stride < (int64_t{1} << 23); }
+
 bool scale_ok(float s) { return std::isfinite(s) && s > 0.f; }
 bool pos_ok(int64_t P) { return P == 0 || P == 32 || P == 64; }
 
@@ -47,7 +50,8 @@ int expanded_check(const kda_mla_expanded_args& a) {
     if (a.T > 0 && (!a.q || !a.o)) return KDA_ERR_NULL_POINTER;
     if (a.S > 0 && (!a.k || !a.v || (a.P > 0 && !a.k_pe))) return KDA_ERR_NULL_POINTER;
     if (!rows_ok(a.q, a.q_stride, 3, 2) || !rows_ok(a.k, a.k_stride, 3, 2) || !rows_ok(a.v, a.v_stride, 3, 2) ||
-        (a.P > 0 && !rows_ok(a.k_pe, a.k_pe_stride, 2, 2)) || !at16(a.o))
+        (a.P > 0 && !rows_ok(a.k_pe, a.k_pe_stride, 2, 2)) || !at16(a.o) ||
+        !near(a.q_stride[1]) || !near(a.k_stride[1]) || !near(a.v_stride[1]) || (a.P > 0 && !near(a.k_pe_stride[1])))
         return KDA_ERR_UNSUPPORTED;
     return KDA_OK;
 }
@@ -76,7 +80,7 @@ int kda_mla_expanded_bwd(const kda_mla_expanded_bwd_args* g, void* stream) {
     if (a.T > 0 && (!a.lse || !g->d_o || !g->dq)) return KDA_ERR_NULL_POINTER;
     if (a.S > 0 && (!g->dk || !g->dv || (a.P > 0 && !g->dk_pe))) return KDA_ERR_NULL_POINTER;
     if (!g->workspace && kda::mla_expanded_bwd_workspace_bytes(a.B, a.T, a.S, a.H, a.P) > 0) return KDA_ERR_NULL_POINTER;
-    if (!rows_ok(g->d_o, g->d_o_stride, 3, 2) || !at16(g->dq) || !at16(g->dk) || !at16(g->dk_pe) || !at16(g->dv) ||
+    if (!rows_ok(g->d_o, g->d_o_stride, 3, 2) || !near(g->d_o_stride[1]) || !at16(g->dq) || !at16(g->dk) || !at16(g->dk_pe) || !at16(g->dv) ||
         !at16(g->workspace))
         return KDA_ERR_UNSUPPORTED;
     return kda::mla_expanded_bwd_launch(*g, static_cast<hipStream_t>(stream));

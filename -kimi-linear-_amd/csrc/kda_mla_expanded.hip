@@ -31,30 +31,37 @@ using namespace mla;
 
 constexpr float kLazy = 8.f;          // log2 of how far a maximum may lag
 
+// A workgroup: RW waves of 32 query rows, times KW waves that share the keys
+// of each: of a step's KW KEYS keys, wave group g takes the g-th KEYS.  BUFS
+// buffers of a step's tiles.
 // Grid: (query tiles, longest first) x (batch, head) with the latter inner, so
 // that a head's tiles share an XCD's L2 where B H is a multiple of eight.
-template <typename T, int N, int P, int WAVES>
-__global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : 1) void expanded_kernel(kda_mla_expanded_args a, int qtiles) {
-    using F = KvTile<T, N, P, 64 * WAVES, 32>;
-    constexpr int D = F::D, V = F::V, kRows = 32 * WAVES;
-    __shared__ __align__(16) T smem[2 * F::kBuf];
+template <typename T, int N, int P, int RW, int KW, int KEYS, int BUFS>
+__global__ __launch_bounds__(64 * RW * KW, RW * KW == 8 ? 2 : 1) void expanded_kernel(kda_mla_expanded_args a,
+                                                                                     int qtiles) {
+    constexpr int kStep = KW * KEYS, kRows = 32 * RW, kU = KEYS / 32;
+    using F = KvTile<T, N, P, 64 * RW * KW, kStep, 32>;
+    constexpr int D = F::D, V = F::V;
+    constexpr int kJoin = KW == 1 ? 0 : RW * (KW / 2) * (32 * V + 64) * 4;        // bytes
+    constexpr int kBytes = BUFS * F::kBuf * 2 > kJoin ? BUFS * F::kBuf * 2 : kJoin;
+    __shared__ __align__(16) char raw[kBytes];
+    T* smem = reinterpret_cast<T*>(raw);
     const int64_t bhs = a.B * a.H;
     const int64_t bh = blockIdx.x % bhs, b = bh / a.H, h = bh - b * a.H;
     const int t0 = (qtiles - 1 - static_cast<int>(blockIdx.x / bhs)) * kRows;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lq = lane & 31, half = lane >> 5;
+    const int lane = threadIdx.x & 63, lq = lane & 31, half = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), row = wave % RW, group = wave / RW;
     const int len = tokens(a.lengths, b, a.S), nq = static_cast<int>(a.T);
     const int start = first_position(a.starts, b, a.S, a.T);
     const int exist = max(0, min(nq, len - start));              // queries that exist
-    const int t = t0 + 32 * wave + lq;
+    const int w0 = t0 + 32 * row, t = w0 + lq;
     const bool live = t < exist;
     const int limit = live ? start + t : -1;                      // last key this lane's row sees
-    const int w0 = t0 + 32 * wave;                                // the wave's rows: all, some or none exist
-    const int wlast = w0 < exist ? start + min(w0 + 31, exist - 1) : -1;
+    const int wlast = w0 < exist ? start + min(w0 + 31, exist - 1) : -1;       // and the last of the wave's
     const int wall = w0 + 32 <= exist ? start + w0 : -1;          // keys up to this one every row sees
     const int keys = t0 < exist ? start + min(t0 + kRows, exist) : 0;
     const float c = a.scale * kLog2E;
 
-    uint4 q[D / 16];
     f16v o[V / 32];
 #pragma unroll
     for (int i = 0; i < V / 32; ++i)
@@ -63,42 +70,41 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : 1) void expanded_kerne
     float top = kNoMax, sum = 0.f;
 
     if (keys > 0) {
+        uint4 q[D / 16];
         const T* qr = static_cast<const T*>(a.q) + b * a.q_stride[0] + min(t, exist - 1) * a.q_stride[1] +
                       h * a.q_stride[2] + 8 * half;
+        F tile(a, b, h);
+        tile.fetch(a, 0, keys);
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) q[k] = *reinterpret_cast<const uint4*>(qr + 16 * k);
-        const T* kp = static_cast<const T*>(a.k) + b * a.k_stride[0] + h * a.k_stride[2];
-        const T* pe = static_cast<const T*>(a.k_pe) + b * a.k_pe_stride[0];
-        const T* vp = static_cast<const T*>(a.v) + b * a.v_stride[0] + h * a.v_stride[2];
-        uint4 r[F::kPer];
-        F::fetch(a, kp, pe, vp, 0, keys, r);
-        F::put(smem, r);
+        tile.put(smem);
         __syncthreads();
         int cur = 0;
-        for (int j0 = 0; j0 < keys; j0 += kTile, cur ^= 1) {
-            const bool more = j0 + kTile < keys;
-            if (more) F::fetch(a, kp, pe, vp, j0 + kTile, keys, r);
-            if (j0 <= wlast) {
-                const T* kt = smem + cur * F::kBuf + lq * F::kK + 8 * half;
-                f16v s[2];
+        for (int j0 = 0; j0 < keys; j0 += kStep) {
+            tile.fetch(a, j0 + kStep, keys);
+            const T* buf = smem + cur * F::kBuf;
+            const int jw = j0 + KEYS * group;                     // the wave's first key
+            if (jw <= wlast) {
+                const T* kt = buf + (KEYS * group + lq) * F::kK + 8 * half;
+                f16v s[kU];
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
+                for (int u = 0; u < kU; ++u) {
 #pragma unroll
                     for (int e = 0; e < 16; ++e) s[u][e] = 0.f;
 #pragma unroll
                     for (int k = 0; k < D / 16; ++k)
                         s[u] = Act<T>::mma32(*reinterpret_cast<const uint4*>(kt + 32 * u * F::kK + 16 * k), q[k], s[u]);
                 }
-                if (j0 + kTile - 1 > wall) {
+                if (jw + KEYS - 1 > wall) {
 #pragma unroll
-                    for (int u = 0; u < 2; ++u)
+                    for (int u = 0; u < kU; ++u)
 #pragma unroll
                         for (int e = 0; e < 16; ++e)
-                            if (j0 + 32 * u + 8 * (e / 4) + 4 * half + e % 4 > limit) s[u][e] = -INFINITY;
+                            if (jw + 32 * u + 8 * (e / 4) + 4 * half + e % 4 > limit) s[u][e] = -INFINITY;
                 }
                 float mx = s[0][0];
 #pragma unroll
-                for (int u = 0; u < 2; ++u)
+                for (int u = 0; u < kU; ++u)
 #pragma unroll
                     for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[u][e]);
                 mx = half_max(mx) * c;
@@ -111,9 +117,9 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : 1) void expanded_kerne
 #pragma unroll
                         for (int e = 0; e < 16; ++e) o[i][e] *= alpha;
                 }
-                uint4 p[4];
+                uint4 p[2 * kU];
 #pragma unroll
-                for (int u = 0; u < 4; ++u) {
+                for (int u = 0; u < 2 * kU; ++u) {
                     uint32_t w[4];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
@@ -125,10 +131,10 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : 1) void expanded_kerne
                     }
                     p[u] = uint4{w[0], w[1], w[2], w[3]};
                 }
-                const T* vt = smem + cur * F::kBuf + kTile * F::kK + (4 * half + ((lane & 15) >> 2)) * F::kV +
+                const T* vt = buf + kStep * F::kK + (KEYS * group + 4 * half + ((lane & 15) >> 2)) * F::kV +
                               16 * ((lane >> 4) & 1) + 4 * (lane & 3);
 #pragma unroll
-                for (int u = 0; u < 4; ++u)
+                for (int u = 0; u < 2 * kU; ++u)
 #pragma unroll
                     for (int i = 0; i < V / 32; ++i) {
                         const uint2 v0 = read_tr(vt + 16 * u * F::kV + 32 * i);
@@ -136,11 +142,50 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : 1) void expanded_kerne
                         o[i] = Act<T>::mma32(uint4{v0.x, v0.y, v1.x, v1.y}, p[u], o[i]);
                     }
             }
-            if (more) F::put(smem + (cur ^ 1) * F::kBuf, r);
-            __syncthreads();
+            if constexpr (BUFS == 2) {
+                cur ^= 1;
+                tile.put(smem + cur * F::kBuf);
+                __syncthreads();
+            } else {
+                __syncthreads();
+                tile.put(smem);
+                __syncthreads();
+            }
         }
     }
-    if (t >= nq) return;
+    // the key groups' sums, half of them onto the other half at a time
+#pragma unroll
+    for (int n = KW / 2; n > 0; n /= 2) {
+        f4* part = reinterpret_cast<f4*>(raw);
+        const int slot = (group % n) * RW + row;                  // of n RW
+        f4* mine = part + slot * (V / 32) * 4 * 64 + lane;
+        float2* stat = reinterpret_cast<float2*>(part + n * RW * (V / 32) * 4 * 64) + slot * 64 + lane;
+        if (group >= n && group < 2 * n) {
+#pragma unroll
+            for (int i = 0; i < V / 32; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    mine[(4 * i + e) * 64] = f4{o[i][4 * e], o[i][4 * e + 1], o[i][4 * e + 2], o[i][4 * e + 3]};
+            *stat = float2{top, sum};
+        }
+        __syncthreads();
+        if (group < n) {
+            const float2 x = *stat;
+            const float now = fmaxf(top, x.x), f0 = __builtin_amdgcn_exp2f(top - now), f1 = __builtin_amdgcn_exp2f(x.x - now);
+            top = now;
+            sum = sum * f0 + x.y * f1;
+#pragma unroll
+            for (int i = 0; i < V / 32; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const f4 y = mine[(4 * i + e) * 64];
+#pragma unroll
+                    for (int d = 0; d < 4; ++d) o[i][4 * e + d] = o[i][4 * e + d] * f0 + y[d] * f1;
+                }
+        }
+        __syncthreads();
+    }
+    if (group != 0 || t >= nq) return;
     sum = half_sum(sum);
     const float norm = sum == 0.f ? 0.f : 1.f / sum;
     T* out = static_cast<T*>(a.o) + ((b * a.T + t) * a.H + h) * V + 4 * half;
@@ -155,20 +200,20 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : 1) void expanded_kerne
         a.lse[(b * a.H + h) * a.T + t] = sum == 0.f ? INFINITY : top + __builtin_amdgcn_logf(sum);
 }
 
-template <typename T, int N, int P, int WAVES>
-int launch_waves(const kda_mla_expanded_args& a, hipStream_t stream) {
-    const int64_t qtiles = (a.T + 32 * WAVES - 1) / (32 * WAVES);
-    expanded_kernel<T, N, P, WAVES><<<static_cast<unsigned>(qtiles * a.B * a.H), 64 * WAVES, 0, stream>>>(
+template <typename T, int N, int P, int RW, int KW, int KEYS, int BUFS>
+int launch_as(const kda_mla_expanded_args& a, hipStream_t stream) {
+    const int64_t qtiles = (a.T + 32 * RW - 1) / (32 * RW);
+    expanded_kernel<T, N, P, RW, KW, KEYS, BUFS><<<static_cast<unsigned>(qtiles * a.B * a.H), 64 * RW * KW, 0, stream>>>(
         a, static_cast<int>(qtiles));
     return hipGetLastError() == hipSuccess ? KDA_OK : KDA_ERR_LAUNCH;
 }
 
 template <typename T, int N, int P>
 int launch(const kda_mla_expanded_args& a, hipStream_t stream) {
-    // as many rows a workgroup as leave every CU one
-    if (a.B * a.H * ((a.T + 255) / 256) >= 256) return launch_waves<T, N, P, 8>(a, stream);
-    if (a.B * a.H * ((a.T + 127) / 128) >= 256) return launch_waves<T, N, P, 4>(a, stream);
-    return launch_waves<T, N, P, 2>(a, stream);
+    // eight waves a workgroup, as many of them on rows of their own as leave every CU a workgroup
+    if (a.B * a.H * ((a.T + 255) / 256) >= 256) return launch_as<T, N, P, 8, 1, 64, 2>(a, stream);
+    if (a.B * a.H * ((a.T + 127) / 128) >= 256) return launch_as<T, N, P, 4, 2, 32, 2>(a, stream);
+    return launch_as<T, N, P, 2, 4, 32, 1>(a, stream);
 }
 
 template <typename T>

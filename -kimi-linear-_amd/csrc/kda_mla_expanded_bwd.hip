@@ -31,6 +31,7 @@ namespace {
 
 using namespace mla;
 
+constexpr int kTile = 64;             // keys a tile of the dq kernel
 constexpr int kQTile = 32;            // queries a tile of the dk, dv kernel
 constexpr int kWaves = 4;
 constexpr int kThreads = 64 * kWaves;
@@ -79,7 +80,7 @@ __device__ __forceinline__ float dot8(uint4 x, uint4 y, float acc, bf16_t) {
 template <typename T, int N, int P>
 __global__ __launch_bounds__(kThreads, 1) void dq_kernel(kda_mla_expanded_bwd_args g, float* delta, int qtiles) {
     const kda_mla_expanded_args& a = g.fwd;
-    using F = KvTile<T, N, P, kThreads, 8>;
+    using F = KvTile<T, N, P, kThreads, kTile, 8>;
     constexpr int D = F::D, V = F::V, kRows = 32 * kWaves;
     __shared__ __align__(16) T smem[2 * F::kBuf];
     const int64_t bhs = a.B * a.H, bh = blockIdx.x % bhs;
@@ -122,17 +123,13 @@ __global__ __launch_bounds__(kThreads, 1) void dq_kernel(kda_mla_expanded_bwd_ar
         if (live && half == 0) delta[bh * a.T + t] = dl;
         const float lse = (live ? a.lse[bh * a.T + t] : INFINITY) - kPShift<T>;
 
-        const T* kp = static_cast<const T*>(a.k) + at.b * a.k_stride[0] + at.h * a.k_stride[2];
-        const T* pe = static_cast<const T*>(a.k_pe) + at.b * a.k_pe_stride[0];
-        const T* vp = static_cast<const T*>(a.v) + at.b * a.v_stride[0] + at.h * a.v_stride[2];
-        uint4 r[F::kPer];
-        F::fetch(a, kp, pe, vp, 0, keys, r);
-        F::put(smem, r);
+        F tile(a, at.b, at.h);
+        tile.fetch(a, 0, keys);
+        tile.put(smem);
         __syncthreads();
         int cur = 0;
-        for (int j0 = 0; j0 < keys; j0 += kTile, cur ^= 1) {
-            const bool more = j0 + kTile < keys;
-            if (more) F::fetch(a, kp, pe, vp, j0 + kTile, keys, r);
+        for (int j0 = 0; j0 < keys; j0 += kTile) {
+            tile.fetch(a, j0 + kTile, keys);
 #pragma unroll 1
             for (int u = 0; u < kTile && j0 + u <= wlast; u += 32) {
                 const T* kt = smem + cur * F::kBuf + (u + lq) * F::kK + 8 * half;
@@ -183,7 +180,8 @@ __global__ __launch_bounds__(kThreads, 1) void dq_kernel(kda_mla_expanded_bwd_ar
                     }
                 }
             }
-            if (more) F::put(smem + (cur ^ 1) * F::kBuf, r);
+            cur ^= 1;
+            tile.put(smem + cur * F::kBuf);
             __syncthreads();
         }
     }
@@ -199,54 +197,45 @@ __global__ __launch_bounds__(kThreads, 1) void dq_kernel(kda_mla_expanded_bwd_ar
                       Act<T>::pair(dq[i][4 * e + 2] * norm, dq[i][4 * e + 3] * norm)};
 }
 
-// A tile of queries and their output gradients, as KvTile: [kQTile][D + 8] and
+// A tile of queries and their output gradients: [kQTile][D + 8] and
 // [kQTile][V + 8], then lse and delta of each.
 template <typename T, int D, int V>
 struct QTile {
     static constexpr int kQ = D + 8, kO = V + 8;
     static constexpr int kRow = kQTile * (kQ + kO);               // elements before lse
     static constexpr int kBuf = kRow + 4 * kQTile;                // a float is two elements
-    static constexpr int kChunks = kQTile * (D + V) / 8;
-    static constexpr int kPer = (kChunks + kThreads - 1) / kThreads;
+    // the position channels apart, so that each part is whole rounds of the threads
+    static constexpr int kP = D % 64 == 0 ? 0 : 32;
+    Rows<T, kQTile, D - kP, kThreads, kQ> q;
+    Rows<T, kQTile, kP, kThreads, kQ> qp;
+    Rows<T, kQTile, V, kThreads, kO> d_o;
+    float x;
 
-    static __device__ __forceinline__ void fetch(const kda_mla_expanded_bwd_args& g, const T* q, const T* d_o,
-                                                 const float* lse, const float* delta, int t0, int exist,
-                                                 uint4 (&r)[kPer], float& x) {
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-            const int c = threadIdx.x + i * kThreads;
-            if (kChunks % kThreads != 0 && c >= kChunks) break;
-            // rows past the last that exists repeat it; their lse makes p zero
-            if (c < kQTile * D / 8) {
-                const int row = min(t0 + c / (D / 8), exist - 1);
-                r[i] = *reinterpret_cast<const uint4*>(q + row * g.fwd.q_stride[1] + c % (D / 8) * 8);
-            } else {
-                const int d = c - kQTile * D / 8, row = min(t0 + d / (V / 8), exist - 1);
-                r[i] = *reinterpret_cast<const uint4*>(d_o + row * g.d_o_stride[1] + d % (V / 8) * 8);
-            }
-        }
-        if (threadIdx.x < 2 * kQTile) {
-            const int t = t0 + (threadIdx.x & (kQTile - 1));
-            const bool second = threadIdx.x >= kQTile;
-            x = second ? 0.f : INFINITY;
-            if (t < exist) x = second ? delta[t] : lse[t] - kPShift<T>;
-        }
+    __device__ __forceinline__ QTile(const kda_mla_expanded_bwd_args& g) {
+        q.start(g.fwd.q_stride[1]);
+        qp.start(g.fwd.q_stride[1]);
+        d_o.start(g.d_o_stride[1]);
     }
-    static __device__ __forceinline__ void put(T* buf, const uint4 (&r)[kPer], float x) {
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-            const int c = threadIdx.x + i * kThreads;
-            if (kChunks % kThreads != 0 && c >= kChunks) break;
-            int at;
-            if (c < kQTile * D / 8) {
-                at = c / (D / 8) * kQ + c % (D / 8) * 8;
-            } else {
-                const int d = c - kQTile * D / 8;
-                at = kQTile * kQ + d / (V / 8) * kO + d % (V / 8) * 8;
-            }
-            *reinterpret_cast<uint4*>(buf + at) = r[i];
+    // Rows past the last that exists are zeros, and their lse makes p zero.
+    __device__ __forceinline__ void fetch(const kda_mla_expanded_bwd_args& g, const T* qb, const T* ob, const float* lse,
+                                          const float* delta, int t0, int exist) {
+        q.fetch(qb, g.fwd.q_stride[1], t0, exist);
+        qp.fetch(qb + D - kP, g.fwd.q_stride[1], t0, exist);
+        d_o.fetch(ob, g.d_o_stride[1], t0, exist);
+        const int t = t0 + (threadIdx.x & (kQTile - 1));
+        const float* from = threadIdx.x & kQTile ? delta : lse;
+        x = from[min(t, exist - 1)];
+        issued();
+    }
+    __device__ __forceinline__ void put(T* buf, int t0, int exist) const {
+        q.put(buf);
+        qp.put(buf + D - kP);
+        d_o.put(buf + kQTile * kQ);
+        if (threadIdx.x < 2 * kQTile) {
+            const bool there = t0 + static_cast<int>(threadIdx.x & (kQTile - 1)) < exist;
+            const float y = threadIdx.x & kQTile ? (there ? x : 0.f) : (there ? x - kPShift<T> : INFINITY);
+            reinterpret_cast<float*>(buf + kRow)[threadIdx.x] = y;
         }
-        if (threadIdx.x < 2 * kQTile) reinterpret_cast<float*>(buf + kRow)[threadIdx.x] = x;
     }
 };
 
@@ -294,15 +283,13 @@ __global__ __launch_bounds__(kThreads, 1) void dkv_kernel(kda_mla_expanded_bwd_a
         const T* qp = static_cast<const T*>(a.q) + at.b * a.q_stride[0] + at.h * a.q_stride[2];
         const T* dop = static_cast<const T*>(g.d_o) + at.b * g.d_o_stride[0] + at.h * g.d_o_stride[2];
         const float *lse = a.lse + bh * a.T, *del = delta + bh * a.T;
-        uint4 r[F::kPer];
-        float x;
-        F::fetch(g, qp, dop, lse, del, first, at.exist, r, x);
-        F::put(smem, r, x);
+        F tile(g);
+        tile.fetch(g, qp, dop, lse, del, first, at.exist);
+        tile.put(smem, first, at.exist);
         __syncthreads();
         int cur = 0;
-        for (int t0 = first; t0 < at.exist; t0 += kQTile, cur ^= 1) {
-            const bool more = t0 + kQTile < at.exist;
-            if (more) F::fetch(g, qp, dop, lse, del, t0 + kQTile, at.exist, r, x);
+        for (int t0 = first; t0 < at.exist; t0 += kQTile) {
+            tile.fetch(g, qp, dop, lse, del, t0 + kQTile, at.exist);
             if (at.start + t0 + kQTile - 1 >= w0 && w0 < at.len) {
                 const T* buf = smem + cur * F::kBuf;
                 const T* qt = buf + lk * F::kQ + 8 * half;
@@ -367,7 +354,8 @@ __global__ __launch_bounds__(kThreads, 1) void dkv_kernel(kda_mla_expanded_bwd_a
                     }
                 }
             }
-            if (more) F::put(smem + (cur ^ 1) * F::kBuf, r, x);
+            cur ^= 1;
+            tile.put(smem + cur * F::kBuf, t0 + kQTile, at.exist);
             __syncthreads();
         }
     }

@@ -1,4 +1,4 @@
-// The key and value tiles of the expanded latent attention's kernels.
+// Tiles of rows moved from memory to LDS for the expanded latent attention.
 #pragma once
 
 #include "kda_mla.h"
@@ -6,56 +6,86 @@
 namespace kda {
 namespace mla {
 
-constexpr int kTile = 64;             // keys a tile
+// ROWS rows of C channels (16 bits each) moved by NT threads, 16 bytes each, to
+// LDS rows of PITCH elements.  The loads go through a buffer descriptor that
+// ends with the last row there is: rows past it read as zeros, without a
+// branch or a clamp, so that the loads of a tile stay in flight together.
+template <typename T, int ROWS, int C, int NT, int PITCH>
+struct Rows {
+    static constexpr int kPieces = ROWS * C / 8;
+    static constexpr int kPer = (kPieces + NT - 1) / NT;
+    static_assert(kPieces % NT == 0 || kPieces < NT, "whole rounds, or less than one");
+    uint32_t from[kPer];
+    uint4 r[kPer];
 
-// A tile of keys and values moved from memory to LDS by a workgroup of NT
-// threads: [kTile][D + 8] keys, the head's channels and the position channels
-// side by side, then [kTile][V + VPAD] values.
-template <typename T, int N, int P, int NT, int VPAD>
+    // Threads past a round that is less than whole move its first pieces once more.
+    static __device__ __forceinline__ int piece(int i) { return (threadIdx.x + i * NT) % kPieces; }
+
+    __device__ __forceinline__ void start(int64_t stride) {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            const int c = piece(i);
+            from[i] = static_cast<uint32_t>(c / (C / 8)) * static_cast<uint32_t>(stride * 2) + c % (C / 8) * 16;
+        }
+    }
+    // Rows first.. of base, of which there are `rows` in all.
+    __device__ __forceinline__ void fetch(const T* base, int64_t stride, int first, int rows) {
+        const int n = min(rows - first, ROWS);
+        const uint32_t bytes = n > 0 ? static_cast<uint32_t>(n - 1) * static_cast<uint32_t>(stride * 2) + 2 * C : 0u;
+        const auto rsrc = make_rsrc_uniform(base + static_cast<int64_t>(first) * stride, bytes);
+#pragma unroll
+        for (int i = 0; i < kPer; ++i)
+            r[i] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, static_cast<int>(from[i]), 0, 0));
+    }
+    __device__ __forceinline__ void put(T* lds) const {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            const int c = piece(i);
+            *reinterpret_cast<uint4*>(lds + c / (C / 8) * PITCH + c % (C / 8) * 8) = r[i];
+        }
+    }
+};
+template <typename T, int ROWS, int NT, int PITCH>
+struct Rows<T, ROWS, 0, NT, PITCH> {
+    __device__ __forceinline__ void start(int64_t) {}
+    __device__ __forceinline__ void fetch(const T*, int64_t, int, int) {}
+    __device__ __forceinline__ void put(T*) const {}
+};
+
+// Loads issued before this stay before it: the compiler otherwise sinks a
+// prefetch past the products it is to overlap, down to its first use.
+__device__ __forceinline__ void issued() { asm volatile("" ::: "memory"); }
+
+// A tile of keys and values: [KEYS][D + 8] keys, the head's channels and the
+// position channels side by side, then [KEYS][V + VPAD] values.
+template <typename T, int N, int P, int NT, int KEYS, int VPAD>
 struct KvTile {
     static constexpr int D = N + P, V = N;
     static constexpr int kK = D + 8, kV = V + VPAD;               // LDS rows, elements
-    static constexpr int kBuf = kTile * (kK + kV);                // elements of one buffer
-    static constexpr int kChunks = kTile * (D + V) / 8;           // 16-byte pieces of a tile
-    static constexpr int kPer = (kChunks + NT - 1) / NT;
+    static constexpr int kBuf = KEYS * (kK + kV);                 // elements of one buffer
+    Rows<T, KEYS, N, NT, kK> k;
+    Rows<T, KEYS, P, NT, kK> pe;
+    Rows<T, KEYS, V, NT, kV> v;
+    const T *kp, *pp, *vp;
 
-    // Piece c of a tile: first the head's keys, then the position parts, then the values.
-    static __device__ __forceinline__ void fetch(const kda_mla_expanded_args& a, const T* k, const T* pe, const T* v,
-                                                 int j0, int keys, uint4 (&r)[kPer]) {
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-            const int c = threadIdx.x + i * NT;
-            if (kChunks % NT != 0 && c >= kChunks) break;
-            // rows past the last repeat it: their scores are masked
-            if (c < kTile * N / 8) {
-                const int row = min(c / (N / 8), keys - 1 - j0);
-                r[i] = *reinterpret_cast<const uint4*>(k + (j0 + row) * a.k_stride[1] + c % (N / 8) * 8);
-            } else if (P > 0 && c < kTile * D / 8) {
-                const int d = c - kTile * N / 8, row = min(d / (P > 0 ? P / 8 : 1), keys - 1 - j0);
-                r[i] = *reinterpret_cast<const uint4*>(pe + (j0 + row) * a.k_pe_stride[1] + d % (P > 0 ? P / 8 : 1) * 8);
-            } else {
-                const int d = c - kTile * D / 8, row = min(d / (V / 8), keys - 1 - j0);
-                r[i] = *reinterpret_cast<const uint4*>(v + (j0 + row) * a.v_stride[1] + d % (V / 8) * 8);
-            }
-        }
+    __device__ __forceinline__ KvTile(const kda_mla_expanded_args& a, int64_t b, int64_t h) {
+        kp = static_cast<const T*>(a.k) + b * a.k_stride[0] + h * a.k_stride[2];
+        pp = static_cast<const T*>(a.k_pe) + b * a.k_pe_stride[0];
+        vp = static_cast<const T*>(a.v) + b * a.v_stride[0] + h * a.v_stride[2];
+        k.start(a.k_stride[1]);
+        pe.start(a.k_pe_stride[1]);
+        v.start(a.v_stride[1]);
     }
-    static __device__ __forceinline__ void put(T* buf, const uint4 (&r)[kPer]) {
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-            const int c = threadIdx.x + i * NT;
-            if (kChunks % NT != 0 && c >= kChunks) break;
-            int at;
-            if (c < kTile * N / 8) {
-                at = c / (N / 8) * kK + c % (N / 8) * 8;
-            } else if (P > 0 && c < kTile * D / 8) {
-                const int d = c - kTile * N / 8;
-                at = d / (P > 0 ? P / 8 : 1) * kK + N + d % (P > 0 ? P / 8 : 1) * 8;
-            } else {
-                const int d = c - kTile * D / 8;
-                at = kTile * kK + d / (V / 8) * kV + d % (V / 8) * 8;
-            }
-            *reinterpret_cast<uint4*>(buf + at) = r[i];
-        }
+    __device__ __forceinline__ void fetch(const kda_mla_expanded_args& a, int j0, int keys) {
+        k.fetch(kp, a.k_stride[1], j0, keys);
+        pe.fetch(pp, a.k_pe_stride[1], j0, keys);
+        v.fetch(vp, a.v_stride[1], j0, keys);
+        issued();
+    }
+    __device__ __forceinline__ void put(T* buf) const {
+        k.put(buf);
+        pe.put(buf + N);
+        v.put(buf + KEYS * kK);
     }
 };
 
