@@ -17,6 +17,8 @@
 #include <ATen/autocast_mode.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/utils/pybind.h>
 #include <torch/extension.h>
 
@@ -602,58 +604,106 @@ kda_mla_expanded_args expanded_args(const Tensor& q, const Tensor& k, const OptT
     return a;
 }
 
-// mla_expanded: o, with want_lse (o, lse), or None.
-py::object mla_expanded(const Tensor& q, const Tensor& k, const OptTensor& k_pe, const Tensor& v,
-                        const OptTensor& lengths, const OptTensor& starts, double scale, bool want_lse) {
-    Plain plain(q);
-    plain.add(k).add(k_pe).add(v).add(lengths).add(starts);
-    if (!expanded_ok(plain, q, k, k_pe, v, lengths, starts)) return py::none();
-    Tensor o;
-    OptTensor lse;
-    const int status = run(plain.dev, [&](void* stream) -> int {
+// The forward, with its lse if wanted: whether the library took it.
+bool expanded_forward(const Tensor& q, const Tensor& k, const OptTensor& k_pe, const Tensor& v, const OptTensor& lengths,
+                      const OptTensor& starts, double scale, Tensor& o, OptTensor* lse) {
+    const int status = run(q.device(), [&](void* stream) -> int {
         const auto opt = q.options().requires_grad(false);
         o = at::empty({q.size(0), q.size(1), q.size(2), v.size(3)}, opt);
-        if (want_lse) lse = at::empty({q.size(0), q.size(2), q.size(1)}, opt.dtype(at::kFloat));
-        const auto a = expanded_args(q, k, k_pe, v, lengths, starts, scale, o, lse);
+        if (lse) *lse = at::empty({q.size(0), q.size(2), q.size(1)}, opt.dtype(at::kFloat));
+        const auto a = expanded_args(q, k, k_pe, v, lengths, starts, scale, o, lse ? *lse : OptTensor());
         return fn.mla_expanded(&a, stream);
     });
-    if (refused(status, "kda_mla_expanded_fwd")) return py::none();
-    return want_lse ? py::object(py::make_tuple(o, *lse)) : py::cast(o);
+    return !refused(status, "kda_mla_expanded_fwd");
 }
 
-// Its gradients: (dq, dk, dk_pe or None, dv) or None.
-py::object mla_expanded_bwd(const Tensor& d_o, const Tensor& q, const Tensor& k, const OptTensor& k_pe, const Tensor& v,
-                            const OptTensor& lengths, const OptTensor& starts, double scale, const Tensor& o,
-                            const Tensor& lse) {
-    Plain plain(q);
-    plain.add(k).add(k_pe).add(v).add(lengths).add(starts).add(d_o).add(o).add(lse);
-    if (!expanded_ok(plain, q, k, k_pe, v, lengths, starts) || !d_o.sizes().equals(o.sizes()) ||
-        d_o.scalar_type() != q.scalar_type() || !wide_rows(d_o) || !o.is_contiguous() || !lse.is_contiguous() ||
-        lse.scalar_type() != at::kFloat)
-        return py::none();
-    Tensor dq, dk, dv;
-    OptTensor dpe;
-    const int status = run(plain.dev, [&](void* stream) -> int {
-        const auto opt = q.options().requires_grad(false);
-        dq = at::empty(q.sizes(), opt);
-        dk = at::empty(k.sizes(), opt);
-        dv = at::empty(v.sizes(), opt);
-        if (k_pe) dpe = at::empty(k_pe->sizes(), opt);
-        kda_mla_expanded_bwd_args g{};
-        g.fwd = expanded_args(q, k, k_pe, v, lengths, starts, scale, o, lse);
-        const size_t bytes = fn.mla_expanded_bwd_ws(g.fwd.B, g.fwd.T, g.fwd.S, g.fwd.H, g.fwd.P);
-        const Tensor ws = at::empty({static_cast<int64_t>(bytes)}, opt.dtype(at::kByte));
-        g.d_o = d_o.data_ptr();
-        row_strides(g.d_o_stride, d_o);
-        g.dq = dq.data_ptr();
-        g.dk = dk.data_ptr();
-        g.dk_pe = g.fwd.P > 0 ? dpe->data_ptr() : nullptr;
-        g.dv = dv.data_ptr();
-        g.workspace = ws.data_ptr();
-        return fn.mla_expanded_bwd(&g, stream);
-    });
-    if (refused(status, "kda_mla_expanded_bwd")) return py::none();
-    return py::make_tuple(dq, dk, dpe ? py::cast(*dpe) : py::object(py::none()), dv);
+OptTensor maybe(const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); }
+Tensor or_none(const OptTensor& t) { return t ? *t : Tensor(); }
+
+// Its node in the autograd graph: in native code, as its Python form took
+// 80 us of a small training step's 160.
+struct ExpandedFn : torch::autograd::Function<ExpandedFn> {
+    static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& q, const Tensor& k, const OptTensor& k_pe,
+                          const Tensor& v, const OptTensor& lengths, const OptTensor& starts, double scale) {
+        Tensor o;
+        OptTensor lse;
+        if (!expanded_forward(q, k, k_pe, v, lengths, starts, scale, o, &lse)) return Tensor();
+        ctx->save_for_backward({q, k, or_none(k_pe), v, or_none(lengths), or_none(starts), o, *lse});
+        ctx->saved_data["scale"] = scale;
+        return o;
+    }
+
+    // In the engine's thread, which does not hold the interpreter lock.
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                   const torch::autograd::variable_list& grads) {
+        const auto s = ctx->get_saved_variables();
+        const Tensor &q = s[0], &k = s[1], &k_pe = s[2], &v = s[3], &o = s[6], &lse = s[7];
+        const bool again = at::GradMode::is_enabled();
+        Tensor d_o = grads[0].detach();
+        if (d_o.scalar_type() != q.scalar_type()) d_o = d_o.to(q.scalar_type());
+        if (!wide_rows(d_o)) d_o = d_o.clone(at::MemoryFormat::Contiguous);
+        Tensor dq, dk, dpe, dv;
+        {
+            const at::AutoGradMode off(false);
+            const py::gil_scoped_acquire gil;
+            const int status = run(q.device(), [&](void* stream) -> int {
+                const auto opt = q.options().requires_grad(false);
+                dq = at::empty(q.sizes(), opt);
+                dk = at::empty(k.sizes(), opt);
+                dv = at::empty(v.sizes(), opt);
+                if (k_pe.defined()) dpe = at::empty(k_pe.sizes(), opt);
+                kda_mla_expanded_bwd_args g{};
+                g.fwd = expanded_args(q, k, maybe(k_pe), v, maybe(s[4]), maybe(s[5]), ctx->saved_data["scale"].toDouble(),
+                                      o, lse);
+                const size_t bytes = fn.mla_expanded_bwd_ws(g.fwd.B, g.fwd.T, g.fwd.S, g.fwd.H, g.fwd.P);
+                const Tensor ws = at::empty({static_cast<int64_t>(bytes)}, opt.dtype(at::kByte));
+                g.d_o = d_o.data_ptr();
+                row_strides(g.d_o_stride, d_o);
+                g.dq = dq.data_ptr();
+                g.dk = dk.data_ptr();
+                g.dk_pe = g.fwd.P > 0 ? dpe.data_ptr() : nullptr;
+                g.dv = dv.data_ptr();
+                g.workspace = ws.data_ptr();
+                return fn.mla_expanded_bwd(&g, stream);
+            });
+            if (status != KDA_OK) {
+                PyErr_Format(error, "kda_mla_expanded_bwd failed: %s", fn.status_str(status));
+                throw py::error_already_set();
+            }
+        }
+        torch::autograd::variable_list out{dq, dk, dpe, dv, Tensor(), Tensor(), Tensor()};
+        if (again) {                                 // create_graph: differentiable once, an error the second time
+            torch::autograd::variable_list made{dq, dk, dv};
+            if (dpe.defined()) made.push_back(dpe);
+            for (Tensor& t : made) t.requires_grad_(true);
+            const auto stop = std::make_shared<torch::autograd::DelayedError>(
+                "mla_expanded can be differentiated only once", static_cast<int64_t>(made.size()));
+            made = (*stop)(std::move(made));
+            out[0] = made[0];
+            out[1] = made[1];
+            out[3] = made[2];
+            if (dpe.defined()) out[2] = made[3];
+        }
+        return out;
+    }
+};
+
+// mla_expanded: o, differentiable where an input is, or None.
+py::object mla_expanded(const Tensor& q, const Tensor& k, const OptTensor& k_pe, const Tensor& v,
+                        const OptTensor& lengths, const OptTensor& starts, double scale) {
+    bool grad = false;
+    {
+        const at::AutoGradMode off(false);           // inputs that require grad are plain here
+        Plain plain(q);
+        plain.add(k).add(k_pe).add(v).add(lengths).add(starts);
+        if (!expanded_ok(plain, q, k, k_pe, v, lengths, starts)) return py::none();
+    }
+    if (at::GradMode::is_enabled())
+        grad = q.requires_grad() || k.requires_grad() || v.requires_grad() || (k_pe && k_pe->requires_grad());
+    Tensor o;
+    if (grad) o = ExpandedFn::apply(q, k, k_pe, v, lengths, starts, scale);
+    else if (!expanded_forward(q, k, k_pe, v, lengths, starts, scale, o, nullptr)) return py::none();
+    return o.defined() ? py::cast(o) : py::object(py::none());
 }
 
 // A cache [B, S, rank + P] in 16 or 8 bits, in 8 with its scales [B, S, 2].
@@ -807,7 +857,6 @@ PYBIND11_MODULE(_kda_host, m) {
     m.def("linear2", &linear2);
     m.def("linear_wgrad", &linear_wgrad);
     m.def("mla_expanded", &mla_expanded);
-    m.def("mla_expanded_bwd", &mla_expanded_bwd);
     m.def("mla_absorbed", &mla_absorbed);
     m.def("mla_append", &mla_append);
     m.def("mla_read", &mla_read);

@@ -30,7 +30,6 @@ from __future__ import annotations
 import math
 
 import torch
-from torch.autograd.function import once_differentiable
 from torch.utils._python_dispatch import _disable_current_modes
 
 from . import _native
@@ -91,7 +90,7 @@ def _no_grad(what, *tensors):
 
 def _native_call(name, *args):
     """The native call on arguments already checked and laid out."""
-    with _disable_current_modes(), torch.no_grad():
+    with _disable_current_modes():
         got = getattr(_native.host(), name)(*args)
     if got is None or got is False:
         raise KdaError(f"{name}: no kernel for these arguments (sizes beyond the kernels' limits, an output that "
@@ -120,15 +119,12 @@ def mla_expanded(q, k_nope, k_pe, v, lengths=None, starts=None, scale=None):
 
     Differentiable in q, k_nope, k_pe and v (once); gradients have the inputs'
     types, are the same from run to run, and zero in rows past ``lengths``."""
-    if not (torch.is_grad_enabled() and any(isinstance(x, torch.Tensor) and x.requires_grad
-                                            for x in (q, k_nope, k_pe, v))):
-        try:
-            o = _native.host().mla_expanded(q, k_nope, k_pe, v, lengths, starts,
-                                            q.shape[-1] ** -0.5 if scale is None else scale, False)
-        except (TypeError, AttributeError):      # an argument of no type a common call has
-            o = None
-        if o is not None:
-            return o
+    try:
+        o = _native.host().mla_expanded(q, k_nope, k_pe, v, lengths, starts, q.shape[-1] ** -0.5 if scale is None else scale)
+    except (TypeError, AttributeError, ZeroDivisionError):      # an argument of no type a common call has
+        o = None
+    if o is not None:
+        return o
     _activations("q", q)
     _check_tensor("k_nope", k_nope)
     _check_tensor("v", v)
@@ -157,28 +153,7 @@ def mla_expanded(q, k_nope, k_pe, v, lengths=None, starts=None, scale=None):
     q = _rows(q)
     k_nope, v = _rows(k_nope.to(q.dtype)), _rows(v.to(q.dtype))
     k_pe = None if k_pe is None else _rows(k_pe.to(q.dtype))
-    if torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in (q, k_nope, k_pe, v)):
-        return _ExpandedFn.apply(q, k_nope, k_pe, v, lengths, starts, scale)
-    return _native_call("mla_expanded", q, k_nope, k_pe, v, lengths, starts, scale, False)
-
-
-class _ExpandedFn(torch.autograd.Function):
-    """:func:`mla_expanded` on checked arguments, with the native backward."""
-
-    @staticmethod
-    def forward(ctx, q, k_nope, k_pe, v, lengths, starts, scale):
-        o, lse = _native_call("mla_expanded", q, k_nope, k_pe, v, lengths, starts, scale, True)
-        ctx.save_for_backward(q, k_nope, k_pe, v, lengths, starts, o, lse)
-        ctx.scale = scale
-        return o
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, d_o):
-        q, k_nope, k_pe, v, lengths, starts, o, lse = ctx.saved_tensors
-        d_o = _rows(d_o.to(q.dtype))
-        dq, dk, dpe, dv = _native_call("mla_expanded_bwd", d_o, q, k_nope, k_pe, v, lengths, starts, ctx.scale, o, lse)
-        return dq, dk, dpe, dv, None, None, None
+    return _native_call("mla_expanded", q, k_nope, k_pe, v, lengths, starts, scale)
 
 
 # ---- the cache --------------------------------------------------------------

@@ -241,6 +241,27 @@ def test_expanded_views_streams_and_types(kda_pkg):
     assert torch.autograd.grad(o.float().sum(), k32)[0].dtype == torch.float32
 
 
+def test_expanded_is_differentiated_once(kda_pkg):
+    q, kn, pe, v = (x.requires_grad_() for x in inputs(1, 20, 20, 2, 64, 32, BF16, seed=90))
+    o = kda_pkg.mla_expanded(q, kn, pe, v)
+    first = torch.autograd.grad(o.float().square().sum(), (q, kn, pe, v), create_graph=True)
+    with pytest.raises(RuntimeError):            # torch's own word for it: v is not in first's graph
+        torch.autograd.grad(first[0].float().sum(), v)
+    with pytest.raises(RuntimeError, match="once"):
+        first[0].float().sum().backward()
+    # an input changed after the forward is noticed
+    leaf = v.detach().clone()
+    o = kda_pkg.mla_expanded(q, kn, pe, leaf)
+    leaf.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        o.float().sum().backward()
+    # a gradient of another layout or shared by broadcasting
+    o = kda_pkg.mla_expanded(q, kn, pe, v)
+    a = torch.autograd.grad(o, v, torch.ones_like(o), retain_graph=True)[0]
+    b = torch.autograd.grad(o, v, torch.ones(1, 1, 1, 1, dtype=BF16, device=DEV).expand_as(o))[0]
+    assert torch.equal(a, b)
+
+
 def test_expanded_empty(kda_pkg):
     q, kn, pe, v = inputs(2, 0, 5, 2, 64, 32, BF16)
     leaves = [x.requires_grad_() for x in (q, kn, pe, v)]
