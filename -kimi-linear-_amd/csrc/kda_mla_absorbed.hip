@@ -6,20 +6,23 @@
 //
 // Bound by reading the cache: 16 heads of one token make 2 (2R + P) 16 flops of
 // each row's 2 (R + P) bytes, 30 a byte.  So each row is read from memory once,
-// straight into the registers that the score product takes it from (lane: one
-// key, eight neighbouring channels), and from there written to LDS, from where
-// the value product reads it transposed.  The scores come as keys x rows, whose
-// accumulator layout is the value product's operand layout up to an order of
-// the keys, which the transposed reads follow: P never leaves its registers.
+// whole rows at a time (the score product's operand layout, a lane a row, would
+// ask for 16 cache lines an instruction: a window's loads took 6.8 k cycles to
+// issue that way, 2 k this way), and goes to LDS, from where the score product
+// reads it by rows and the value product transposed.
 //
-// The four waves of a workgroup each take 32-key tiles of their own, with a
-// softmax of their own: nothing in the loop waits for another wave.  They meet
-// in LDS once a sequence, in a fixed order.
+// A workgroup's waves each take 16 keys of a window and leave their scores
+// in LDS beside the rows; then every wave forms all of the window's weights
+// for itself (a few exponentials a lane) and the value product for its own
+// R / WAVES channels.  So the rows' sums are never spread over waves: there is
+// nothing to merge at the end of a sequence, and a wave holds few of them,
+// which leaves registers for the next window's rows, in flight while this one
+// is worked on, and room for a second workgroup on the CU.
 //
-// The tiles of all sequences are one list that the workgroups share evenly,
-// whatever the lengths (a decode batch's differ): a workgroup's share may
-// begin and end inside a sequence, and what it has of one that others share
-// goes to the workspace, to be joined by a second kernel.
+// The keys of all sequences are one list that the workgroups share evenly in
+// units of 16, whatever the lengths (a decode batch's differ): a workgroup's
+// share may begin and end inside a sequence, and what it has of one that
+// others share goes to the workspace, to be joined by a second kernel.
 //
 // In 8 bits a value is widened to the activation type exactly; a key's scale
 // multiplies its score, and enters the value product through the exponent,
@@ -36,13 +39,13 @@ namespace {
 
 using namespace mla;
 
-constexpr int kTile = 32;         // keys of a wave's tile
-constexpr int kWaves = 4;
-constexpr int kRowTile = 16;      // query rows of a workgroup
+constexpr int kUnit = 16;         // keys of a wave's part of a window
+constexpr int kRows = 16;         // query rows of a workgroup
+constexpr int WAVES = 4, kThreads = 64 * WAVES;
 
 // Workspace: for every slot (a workgroup's part of a row tile's sequence) the
-// rows' sums, [16][R] fp32, and their (maximum, denominator); for every row tile
-// the first and last workgroup that has a part of it.
+// rows' sums, [16][R] fp32, and their (maximum, denominator); for every row
+// tile the first and last workgroup that has a part of it.
 struct Workspace {
     float* o;
     float2* ml;
@@ -52,221 +55,247 @@ __host__ __device__ inline int64_t slots(int64_t groups, int64_t tiles) { return
 __host__ __device__ inline Workspace carve(void* p, int64_t n_slots, int64_t R) {
     Workspace w;
     w.o = static_cast<float*>(p);
-    w.ml = reinterpret_cast<float2*>(w.o + n_slots * kRowTile * R);
-    w.span = reinterpret_cast<int2*>(w.ml + n_slots * kRowTile);
+    w.ml = reinterpret_cast<float2*>(w.o + n_slots * kRows * R);
+    w.span = reinterpret_cast<int2*>(w.ml + n_slots * kRows);
     return w;
 }
 
 template <typename T, bool F8, int R, int P>
 struct Kernel {
     static constexpr int D = R + P;
-    static constexpr int kLat = R / 32, kPos = P / 32;          // depth steps of the score product
-    static constexpr int kStride = R + 16;                      // LDS row, elements
-    static constexpr int kArea = kTile * kStride * 2;           // bytes of a wave's tile
-    static constexpr int kOTiles = R / 16;
-    static_assert(kArea >= kOTiles * 64 * 16, "a wave's sums fit its tile's place");
+    static constexpr int kWindow = kUnit * WAVES;
+    static constexpr int kSteps = D / 32;                       // depth steps of the score product
+    static constexpr int kStride = D + 8;                       // LDS row, elements
+    static constexpr int kScore = kWindow + 4;                  // and floats
+    static constexpr int kTiles = R / 16 / WAVES;               // 16-channel tiles of a wave
+    static constexpr int kLane = F8 ? 16 : 8;                   // channels a lane loads
+    // Rows of a load of the latent and of the position part, and the loads a unit takes.
+    static constexpr int kLatRows = 64 * kLane / R, kLat = kUnit / kLatRows;
+    static constexpr int kPosRows = P == 0 ? kUnit : (64 * kLane / P < kUnit ? 64 * kLane / P : kUnit);
+    static constexpr int kPos = P == 0 ? 0 : kUnit / kPosRows;
 
-    // A tile's rows as loaded: lane (ln, lg) has row 16 s + ln.  16 bits: step k
-    // is channels 32 k + 8 lg on.  8 bits: 16 channels 64 k + 16 lg on serve two
-    // steps of the latent part, and the position part comes in 8-byte pieces.
-    struct Rows {
-        uint4 lat[2][F8 ? kLat / 2 : kLat];
-        uint4 pos[2][F8 || kPos == 0 ? 1 : kPos];
-        uint2 pos8[2][F8 && kPos ? kPos : 1];
-        float2 scale[2][4];
+    struct Shared {
+        T c[kWindow][kStride];           // the window's rows; at first, the queries
+        float s[kRows][kScore];
+        float inv[F8 ? kWindow : 4];
     };
 
-    static __device__ __forceinline__ void load(const kda_mla_absorbed_args& a, int64_t b, int tile, int len, int ln,
-                                                int lg, Rows& r) {
-        const int es = F8 ? 1 : 2;
-        const char* base = static_cast<const char*>(a.cache) + b * a.cache_stride[0] * es;
+    // A unit's rows as loaded, whole rows at a time (a lane's piece by lane and
+    // load); rows past the end come as zeros from the descriptor's range check.
+    struct Rows {
+        uint4 lat[kLat], pos[kPos ? kPos : 1];
+        float2 scale[4];
+    };
+    static __device__ __forceinline__ void load(const kda_mla_absorbed_args& a, int64_t b, int j, int hi, int lane,
+                                                Rows& r) {
+        constexpr int es = F8 ? 1 : 2;
+        const int stride = static_cast<int>(a.cache_stride[1]) * es, n = min(hi - j, kUnit);
+        const auto rsrc = make_rsrc_uniform(
+            static_cast<const char*>(a.cache) + b * a.cache_stride[0] * es + static_cast<int64_t>(j) * stride,
+            n > 0 ? static_cast<uint32_t>(n - 1) * stride + D * es : 0u);
+        const int lat = lane / (64 / kLatRows) * stride + lane % (64 / kLatRows) * 16;
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            // rows past the last repeat it: their scores are masked
-            const int j = min(tile * kTile + 16 * s + ln, len - 1);
-            const char* row = base + j * a.cache_stride[1] * es + 16 * lg;
+        for (int i = 0; i < kLat; ++i)
+            r.lat[i] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, lat, i * kLatRows * stride, 0));
+        if constexpr (P > 0) {
+            constexpr int per = P / kLane;                       // lanes a row
+            const int pos = lane / per % kPosRows * stride + R * es + lane % per * 16;
 #pragma unroll
-            for (int k = 0; k < (F8 ? kLat / 2 : kLat); ++k) r.lat[s][k] = *reinterpret_cast<const uint4*>(row + 64 * k);
-            if constexpr (kPos > 0 && !F8) {
+            for (int i = 0; i < kPos; ++i)
+                r.pos[i] = __builtin_bit_cast(uint4,
+                                              __builtin_amdgcn_raw_buffer_load_b128(rsrc, pos, i * kPosRows * stride, 0));
+        }
+        if constexpr (F8) {
+            const float* sc = a.cache_scale + b * a.scale_stride[0];
 #pragma unroll
-                for (int k = 0; k < kPos; ++k) r.pos[s][k] = *reinterpret_cast<const uint4*>(row + 2 * R + 64 * k);
-            }
-            if constexpr (F8) {
-                if constexpr (kPos > 0) {
+            for (int i = 0; i < 4; ++i)
+                r.scale[i] = *reinterpret_cast<const float2*>(sc + min(j + 4 * (lane >> 4) + i, hi - 1) * a.scale_stride[1]);
+        }
+    }
+    static __device__ __forceinline__ void put8(T* to, uint4 w) {
+        if constexpr (F8) {
+            reinterpret_cast<uint4*>(to)[0] = widen8<T>(w.x, w.y);
+            reinterpret_cast<uint4*>(to)[1] = widen8<T>(w.z, w.w);
+        } else {
+            *reinterpret_cast<uint4*>(to) = w;
+        }
+    }
+    static __device__ __forceinline__ void put(T* rows, int lane, const Rows& r) {
+        T* lat = rows + lane / (64 / kLatRows) * kStride + lane % (64 / kLatRows) * kLane;
 #pragma unroll
-                    for (int k = 0; k < kPos; ++k)
-                        r.pos8[s][k] = *reinterpret_cast<const uint2*>(row + R - 8 * lg + 32 * k);
-                }
-                const float* sc = a.cache_scale + b * a.scale_stride[0];
+        for (int i = 0; i < kLat; ++i) put8(lat + i * kLatRows * kStride, r.lat[i]);
+        if constexpr (P > 0) {
+            constexpr int per = P / kLane;
+            T* pos = rows + lane / per % kPosRows * kStride + R + lane % per * kLane;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int key = min(tile * kTile + 16 * s + 4 * lg + i, len - 1);
-                    r.scale[s][i] = *reinterpret_cast<const float2*>(sc + key * a.scale_stride[1]);
-                }
-            }
+            for (int i = 0; i < kPos; ++i) put8(pos + i * kPosRows * kStride, r.pos[i]);
         }
     }
 
-    // The rows' q, as the score product's second operand in the same order of channels.
-    static __device__ __forceinline__ void load_q(const T* q, int lg, uint4 (&f)[kLat + kPos]) {
-#pragma unroll
-        for (int k = 0; k < kLat; ++k) {
-            const int c = F8 ? 64 * (k / 2) + 16 * lg + 8 * (k % 2) : 32 * k + 8 * lg;
-            f[k] = *reinterpret_cast<const uint4*>(q + c);
+    // Query rows m0.. as (token, head): row m0 + r, past the last repeating it.
+    struct Queries {
+        int H, t0, h0, last;
+        float inv;
+        __device__ __forceinline__ Queries(const kda_mla_absorbed_args& a, int m0) {
+            H = static_cast<int>(a.H);
+            t0 = m0 / H;
+            h0 = m0 - t0 * H;
+            last = static_cast<int>(a.T) * H - 1 - m0;
+            inv = __builtin_amdgcn_rcpf(static_cast<float>(H));
         }
-#pragma unroll
-        for (int k = 0; k < kPos; ++k) f[kLat + k] = *reinterpret_cast<const uint4*>(q + R + 32 * k + 8 * lg);
-    }
-
-    // Scores of a tile (keys 16 s + 4 lg + i of row ln), times scale log2(e), plus
-    // log2 of the key's scale in 8 bits; the latent part goes to LDS on the way.
-    static __device__ __forceinline__ void scores(const Rows& r, const uint4 (&q)[kLat + kPos], float c, T* lds, int ln,
-                                                  int lg, f4 (&s)[2], float (&inv)[2][4]) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            f4 acc{}, pos{};
-            T* row = lds + (16 * h + ln) * kStride;
-            if constexpr (F8) {
-#pragma unroll
-                for (int k = 0; k < kLat / 2; ++k) {
-                    const uint4 w = r.lat[h][k];
-                    const uint4 lo = widen8<T>(w.x, w.y), hi = widen8<T>(w.z, w.w);
-                    acc = Act<T>::mma16(lo, q[2 * k], acc);
-                    acc = Act<T>::mma16(hi, q[2 * k + 1], acc);
-                    uint4* to = reinterpret_cast<uint4*>(row + 64 * k + 16 * lg);
-                    to[0] = lo;
-                    to[1] = hi;
-                }
-#pragma unroll
-                for (int k = 0; k < kPos; ++k)
-                    pos = Act<T>::mma16(widen8<T>(r.pos8[h][k].x, r.pos8[h][k].y), q[kLat + k], pos);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float2 sc = r.scale[h][i];
-                    s[h][i] = fmaf(acc[i] * sc.x + pos[i] * sc.y, c, __builtin_amdgcn_logf(sc.x));
-                    inv[h][i] = __builtin_amdgcn_rcpf(sc.x);
-                }
-            } else {
-#pragma unroll
-                for (int k = 0; k < kLat; ++k) {
-                    acc = Act<T>::mma16(r.lat[h][k], q[k], acc);
-                    *reinterpret_cast<uint4*>(row + 32 * k + 8 * lg) = r.lat[h][k];
-                }
-#pragma unroll
-                for (int k = 0; k < kPos; ++k) acc = Act<T>::mma16(r.pos[h][k], q[kLat + k], acc);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) s[h][i] = acc[i] * c;
-            }
+        // h0 + r < H + 16: with 16 heads or more it passes H once at most, with
+        // fewer it is below 32, which the reciprocal divides exactly
+        __device__ __forceinline__ int token(int r) const {
+            const int x = h0 + min(r, last);
+            return t0 + (H >= kRows ? (x >= H ? 1 : 0) : static_cast<int>((static_cast<float>(x) + 0.5f) * inv));
         }
-    }
+        __device__ __forceinline__ int head(int r, int t) const { return h0 + min(r, last) - (t - t0) * H; }
+    };
 
-    // One row tile's part of tiles [lo, hi) of sequence b; the whole of it if
+    // One row tile's part, keys [lo, hi), of sequence b; the whole of it if
     // `whole`, else into the workspace's slot.
-    static __device__ __forceinline__ void segment(const kda_mla_absorbed_args& a, char* smem, int64_t b, int rt, int len,
+    static __device__ __forceinline__ void segment(const kda_mla_absorbed_args& a, Shared& sh, int64_t b, int rt, int len,
                                                    int lo, int hi, bool whole, const Workspace& ws, int64_t slot) {
-        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, ln = lane & 15, lg = lane >> 4;
-        const int rows = static_cast<int>(a.T * a.H), H = static_cast<int>(a.H);
-        const int m = rt * kRowTile + ln, mc = min(m, rows - 1), t = mc / H, h = mc - t * H;
-        const int limit = len - static_cast<int>(a.T) + t;       // last key this lane's row sees
+        const int lane = threadIdx.x & 63, ln = lane & 15, lg = lane >> 4;
+        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        const int rows = static_cast<int>(a.T * a.H), m0 = rt * kRows;
         const float c = a.scale * kLog2E;
-        T* lds = reinterpret_cast<T*>(smem + wave * kArea);
 
         Rows cur;
-        int tile = lo + wave;
-        if (tile < hi) load(a, b, tile, len, ln, lg, cur);
-        uint4 q[kLat + kPos];
-        load_q(static_cast<const T*>(a.q) + b * a.q_stride[0] + t * a.q_stride[1] + h * a.q_stride[2], lg, q);
-
-        f4 o[kOTiles];
+        load(a, b, lo + kUnit * wave, hi, lane, cur);
+        // the queries through LDS: each piece is read from memory once
+        const Queries rq(a, m0);
+        constexpr int kPieces = kRows * (D / 8), kPer = (kPieces + kThreads - 1) / kThreads;
+        typedef uint32_t u4 __attribute__((ext_vector_type(4)));      // (an array of uint4 stays in scratch memory here)
+        u4 qr[kPer];
+        const T* qb = static_cast<const T*>(a.q) + b * a.q_stride[0];
 #pragma unroll
-        for (int i = 0; i < kOTiles; ++i) o[i] = f4{0.f, 0.f, 0.f, 0.f};
+        for (int n = 0; n < kPer; ++n) {
+            const int i = min(static_cast<int>(threadIdx.x) + n * kThreads, kPieces - 1), r = i / (D / 8);
+            const int t = rq.token(r);
+            qr[n] = *reinterpret_cast<const u4*>(qb + t * a.q_stride[1] + rq.head(r, t) * a.q_stride[2] +
+                                                    i % (D / 8) * 8);
+        }
+        const int limit = min(hi - 1, len - static_cast<int>(a.T) + rq.token(ln));    // last key that the lane's row sees
+        __syncthreads();                 // an earlier segment's readers are done
+        T* qs = &sh.c[0][0];
+#pragma unroll
+        for (int n = 0; n < kPer; ++n) {
+            const int i = min(static_cast<int>(threadIdx.x) + n * kThreads, kPieces - 1);
+            *reinterpret_cast<u4*>(qs + i / (D / 8) * kStride + i % (D / 8) * 8) = qr[n];
+        }
+        __syncthreads();
+        uint4 q[kSteps];
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k) q[k] = *reinterpret_cast<const uint4*>(qs + ln * kStride + 32 * k + 8 * lg);
+
+        f4 o[kTiles];
+#pragma unroll
+        for (int i = 0; i < kTiles; ++i) o[i] = f4{0.f, 0.f, 0.f, 0.f};
         float top = kNoMax, sum = 0.f;
-        const int tr_row = 4 * lg + (ln >> 2), tr_col = 4 * (ln & 3);
 
-        for (; tile < hi; tile += kWaves) {
-            f4 s[2];
-            float inv[2][4];
-            scores(cur, q, c, lds, ln, lg, s, inv);
-            if (tile + kWaves < hi) load(a, b, tile + kWaves, len, ln, lg, cur);
-            const int j0 = tile * kTile + 4 * lg;
-            if (tile * kTile + kTile > len - static_cast<int>(a.T)) {
+        for (int j0 = lo; j0 < hi; j0 += kWindow) {
+            __syncthreads();             // the last window's readers are done
+            T* mine = &sh.c[kUnit * wave][0];
+            put(mine, lane, cur);
+            float2 scale[4];
+            if constexpr (F8) {
 #pragma unroll
-                for (int g = 0; g < 2; ++g)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (j0 + 16 * g + i > limit) s[g][i] = -INFINITY;
+                for (int i = 0; i < 4; ++i) scale[i] = cur.scale[i];
+                if (ln == 0)
+                    *reinterpret_cast<f4*>(&sh.inv[kUnit * wave + 4 * lg]) =
+                        f4{__builtin_amdgcn_rcpf(scale[0].x), __builtin_amdgcn_rcpf(scale[1].x),
+                           __builtin_amdgcn_rcpf(scale[2].x), __builtin_amdgcn_rcpf(scale[3].x)};
             }
-            float mx = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
-                             fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
-            mx = fmaxf(top, lanegroup4_max(mx));
+            load(a, b, min(j0 + kWindow + kUnit * wave, hi), hi, lane, cur);
+            // scores of the wave's unit: keys 4 lg + i of row ln
+            const int key = j0 + kUnit * wave + 4 * lg;
+            const T* row = mine + ln * kStride + 8 * lg;
+            f4 acc{}, odd{};             // two chains; in 8 bits the latent and the position part
+#pragma unroll
+            for (int k = 0; k < kSteps; ++k) {
+                const uint4 x = *reinterpret_cast<const uint4*>(row + 32 * k);
+                if (F8 ? k < R / 32 : k % 2 == 0) acc = Act<T>::mma16(x, q[k], acc);
+                else odd = Act<T>::mma16(x, q[k], odd);
+            }
+            f4 s;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if constexpr (F8)
+                    s[i] = fmaf(acc[i] * scale[i].x + odd[i] * scale[i].y, c, __builtin_amdgcn_logf(scale[i].x));
+                else
+                    s[i] = (acc[i] + odd[i]) * c;
+                if (key + i > limit) s[i] = -INFINITY;
+            }
+            *reinterpret_cast<f4*>(&sh.s[ln][kUnit * wave + 4 * lg]) = s;
+            __syncthreads();
+
+            uint4 p[kWindow / 32];
+            float x[kWindow / 32][8], mx = top;
+#pragma unroll
+            for (int k = 0; k < kWindow / 32; ++k) {
+                const f4* from = reinterpret_cast<const f4*>(&sh.s[ln][32 * k + 8 * lg]);
+                const f4 lo4 = from[0], hi4 = from[1];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    x[k][e] = lo4[e];
+                    x[k][4 + e] = hi4[e];
+                    mx = fmaxf(mx, fmaxf(lo4[e], hi4[e]));
+                }
+            }
+            mx = lanegroup4_max(mx);
             const float alpha = __builtin_amdgcn_exp2f(top - mx);
             top = mx;
-            float p[2][4], part = 0.f;
+            float part = 0.f;
 #pragma unroll
-            for (int g = 0; g < 2; ++g)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    p[g][i] = __builtin_amdgcn_exp2f(s[g][i] - mx);
-                    part = F8 ? fmaf(p[g][i], inv[g][i], part) : part + p[g][i];
+            for (int k = 0; k < kWindow / 32; ++k) {
+                f4 inv[2];
+                if constexpr (F8) {
+                    inv[0] = *reinterpret_cast<const f4*>(&sh.inv[32 * k + 8 * lg]);
+                    inv[1] = *reinterpret_cast<const f4*>(&sh.inv[32 * k + 8 * lg + 4]);
                 }
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    x[k][e] = __builtin_amdgcn_exp2f(x[k][e] - mx);
+                    part = F8 ? fmaf(x[k][e], inv[e / 4][e % 4], part) : part + x[k][e];
+                }
+                p[k] = uint4{Act<T>::pair(x[k][0], x[k][1]), Act<T>::pair(x[k][2], x[k][3]),
+                             Act<T>::pair(x[k][4], x[k][5]), Act<T>::pair(x[k][6], x[k][7])};
+            }
             sum = fmaf(sum, alpha, part);
-            const uint4 pf{Act<T>::pair(p[0][0], p[0][1]), Act<T>::pair(p[0][2], p[0][3]),
-                           Act<T>::pair(p[1][0], p[1][1]), Act<T>::pair(p[1][2], p[1][3])};
-            if (__any(alpha != 1.f)) {
 #pragma unroll
-                for (int i = 0; i < kOTiles; ++i)
+            for (int i = 0; i < kTiles; ++i)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) o[i][e] *= alpha;
-            }
-            const T* v = lds + tr_row * kStride + tr_col;
+                for (int e = 0; e < 4; ++e) o[i][e] *= alpha;
+            const T* v = &sh.c[8 * lg + (ln >> 2)][16 * kTiles * wave + 4 * (ln & 3)];
 #pragma unroll
-            for (int i = 0; i < kOTiles; ++i) {
-                const uint2 v0 = read_tr(v + 16 * i), v1 = read_tr(v + 16 * kStride + 16 * i);
-                o[i] = Act<T>::mma16(uint4{v0.x, v0.y, v1.x, v1.y}, pf, o[i]);
-            }
+            for (int k = 0; k < kWindow / 32; ++k)
+#pragma unroll
+                for (int i = 0; i < kTiles; ++i) {
+                    const uint2 v0 = read_tr(v + 32 * k * kStride + 16 * i);
+                    const uint2 v1 = read_tr(v + (32 * k + 4) * kStride + 16 * i);
+                    o[i] = Act<T>::mma16(uint4{v0.x, v0.y, v1.x, v1.y}, p[k], o[i]);
+                }
         }
-        sum = lanegroup4_sum(sum);
-
-        // the four waves' sums, on the largest maximum of each row
-        __shared__ float2 ml[kWaves][kRowTile];
-        __syncthreads();             // an earlier segment's readers are done
-        if (lg == 0) ml[wave][ln] = float2{top, sum};
-        __syncthreads();
-        float big = ml[0][ln].x, den = 0.f;
+        const float den = lanegroup4_sum(sum), norm = den == 0.f ? 0.f : 1.f / den;
+        const int ch = 16 * kTiles * wave + 4 * lg;
+        if (whole) {
+            if (m0 + ln >= rows) return;
+            T* out = static_cast<T*>(a.o) + (b * rows + m0 + ln) * R + ch;
 #pragma unroll
-        for (int w = 1; w < kWaves; ++w) big = fmaxf(big, ml[w][ln].x);
+            for (int i = 0; i < kTiles; ++i)
+                *reinterpret_cast<uint2*>(out + 16 * i) = uint2{Act<T>::pair(o[i][0] * norm, o[i][1] * norm),
+                                                                Act<T>::pair(o[i][2] * norm, o[i][3] * norm)};
+        } else {
+            float* out = ws.o + (slot * kRows + ln) * R + ch;
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) den += ml[w][ln].y * __builtin_amdgcn_exp2f(ml[w][ln].x - big);
-        const float mine = __builtin_amdgcn_exp2f(top - big);
-        f4* area = reinterpret_cast<f4*>(smem + wave * kArea);
-#pragma unroll
-        for (int i = 0; i < kOTiles; ++i) area[i * 64 + lane] = f4{o[i][0] * mine, o[i][1] * mine, o[i][2] * mine,
-                                                                    o[i][3] * mine};
-        __syncthreads();
-        const float norm = den == 0.f ? 0.f : 1.f / den;
-        for (int i = wave; i < kOTiles; i += kWaves) {
-            f4 r = reinterpret_cast<const f4*>(smem)[i * 64 + lane];
-#pragma unroll
-            for (int w = 1; w < kWaves; ++w) {
-                const f4 x = reinterpret_cast<const f4*>(smem + w * kArea)[i * 64 + lane];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) r[e] += x[e];
-            }
-            if (whole) {
-                if (m < rows)
-                    *reinterpret_cast<uint2*>(static_cast<T*>(a.o) + (b * rows + m) * R + 16 * i + 4 * lg) =
-                        uint2{Act<T>::pair(r[0] * norm, r[1] * norm), Act<T>::pair(r[2] * norm, r[3] * norm)};
-            } else {
-                *reinterpret_cast<f4*>(ws.o + (slot * kRowTile + ln) * R + 16 * i + 4 * lg) = r;
-            }
+            for (int i = 0; i < kTiles; ++i) *reinterpret_cast<f4*>(out + 16 * i) = o[i];
+            if (wave == 0 && lg == 0) ws.ml[slot * kRows + ln] = float2{top, den};
         }
-        if (!whole && wave == 0 && lg == 0) ws.ml[slot * kRowTile + ln] = float2{big, den};
     }
 };
 
-__device__ __forceinline__ int tiles_of(const kda_mla_absorbed_args& a, int64_t v, int64_t nv, int rts) {
-    return v < nv ? (tokens(a.lengths, v / rts, a.S) + kTile - 1) / kTile : 0;
-}
+__device__ __forceinline__ int units(int len) { return (len + kUnit - 1) / kUnit; }
 __device__ __forceinline__ int wave_scan(int x, int lane) {
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) {
@@ -276,86 +305,121 @@ __device__ __forceinline__ int wave_scan(int x, int lane) {
     return x;
 }
 
-// Grid: one workgroup for each row tile of each sequence.
+// Grid: a workgroup for each row tile of each sequence (`alone`), or any number
+// of workgroups, each with its share of all units, at least kLeast.
+constexpr int kLeast = 8;
 template <typename T, bool F8, int R, int P>
-__global__ __launch_bounds__(64 * kWaves, 1) void absorbed_kernel(kda_mla_absorbed_args a, int rts) {
+__global__ __launch_bounds__(kThreads, 2) void absorbed_kernel(kda_mla_absorbed_args a, int rts, bool alone) {
     using K = Kernel<T, F8, R, P>;
-    __shared__ __align__(16) char smem[kWaves * K::kArea];
-    const int64_t b = blockIdx.x / rts;
-    const int len = tokens(a.lengths, b, a.S);
-    K::segment(a, smem, b, static_cast<int>(blockIdx.x - b * rts), len, 0, (len + kTile - 1) / kTile, true, Workspace{},
-               0);
-}
-
-// Grid: any number of workgroups, each with its share of all tiles.
-template <typename T, bool F8, int R, int P>
-__global__ __launch_bounds__(64 * kWaves, 1) void absorbed_shared_kernel(kda_mla_absorbed_args a, int rts) {
-    using K = Kernel<T, F8, R, P>;
-    __shared__ __align__(16) char smem[kWaves * K::kArea];
-    const int lane = threadIdx.x & 63;
-    const int64_t nv = a.B * rts;
+    __shared__ __align__(16) typename K::Shared sh;
+    const int lane = threadIdx.x & 63, nv = static_cast<int>(a.B) * rts, group = static_cast<int>(blockIdx.x);
+    if (alone) {
+        const int b = group / rts, rt = group - b * rts, len = tokens(a.lengths, b, a.S);
+        if (len > 0) {
+            K::segment(a, sh, b, rt, len, 0, len, true, Workspace{}, 0);
+        } else {
+            const int rows = static_cast<int>(a.T * a.H), m0 = rt * kRows, n = min(rows - m0, kRows) * (R / 8);
+            uint4* out = reinterpret_cast<uint4*>(static_cast<T*>(a.o) + (static_cast<int64_t>(b) * rows + m0) * R);
+            for (int i = threadIdx.x; i < n; i += kThreads) out[i] = uint4{0, 0, 0, 0};
+        }
+        return;
+    }
     const Workspace ws = carve(a.workspace, slots(gridDim.x, nv), R);
+    // 64 row tiles at a time, one a lane: their tokens, and where their units end in the list
+    int len = 0, end = 0;
+    const auto look = [&](int v0) {
+        len = v0 + lane < nv ? tokens(a.lengths, (v0 + lane) / rts, a.S) : 0;
+        end = wave_scan(units(len), lane);
+        return __builtin_amdgcn_readlane(end, 63);
+    };
     int64_t total = 0;
-    for (int64_t v = 0; v < nv; v += 64) total += __shfl(wave_scan(tiles_of(a, v + lane, nv, rts), lane), 63);
-    const int64_t share = (total + gridDim.x - 1) / gridDim.x;
-    const int64_t from = blockIdx.x * share, to = min(from + share, total);
-    if (from >= to) return;
-    int64_t before = 0;              // tiles of the row tiles before this chunk's
-    for (int64_t v0 = 0; v0 < nv && before < to; v0 += 64) {
-        const int n = tiles_of(a, v0 + lane, nv, rts);
-        const int end = wave_scan(n, lane);
-        const int chunk = __shfl(end, 63);
-        const int64_t mine = before + end - n;       // this lane's first tile in the list
-        uint64_t todo = __ballot(n > 0 && mine < to && mine + n > from);
+    for (int v0 = (nv - 1) / 64 * 64; v0 >= 0; v0 -= 64) total += look(v0);       // ends with the first 64
+    if (total == 0) return;
+    // A part is not worth its place in the workspace below kLeast units; short
+    // sequences have a workgroup each.
+    int64_t share;
+    if (total < INT32_MAX / 2) {     // (a 64-bit division takes ten times as long)
+        const int all = static_cast<int>(total), groups = static_cast<int>(gridDim.x);
+        share = max((all + groups - 1) / groups, min(kLeast, (all + nv - 1) / nv));
+    } else {
+        share = (total + gridDim.x - 1) / gridDim.x;
+    }
+    const int64_t from = group * share, to = min(from + share, total);
+    int64_t before = 0;              // units of the row tiles before these 64
+    for (int v0 = 0; v0 < nv && before < to; v0 += 64) {
+        if (v0 > 0) look(v0);
+        const int n = units(len);
+        const int64_t first = before + end - n;      // this lane's first unit in the list
+        uint64_t todo = __ballot(n > 0 && first < to && first + n > from);
         while (todo) {
             const int i = __builtin_ctzll(todo);
             todo &= todo - 1;
-            const int tiles = __builtin_amdgcn_readlane(n, i);
-            const int64_t first = before + __builtin_amdgcn_readlane(end, i) - tiles, v = v0 + i, b = v / rts;
-            const int lo = static_cast<int>(max(from - first, static_cast<int64_t>(0)));
-            const int hi = static_cast<int>(min(to - first, static_cast<int64_t>(tiles)));
-            K::segment(a, smem, b, static_cast<int>(v - b * rts), tokens(a.lengths, b, a.S), lo, hi,
-                       lo == 0 && hi == tiles, ws, blockIdx.x + v);
+            const int v = v0 + i, b = v / rts, size = __builtin_amdgcn_readlane(len, i), n = units(size);
+            const int64_t at = before + __builtin_amdgcn_readlane(end, i) - n;
+            const int lo = static_cast<int>(max(from - at, static_cast<int64_t>(0)));
+            const int hi = static_cast<int>(min(to - at, static_cast<int64_t>(n)));
+            K::segment(a, sh, b, v - b * rts, size, kUnit * lo, min(kUnit * hi, size), lo == 0 && hi == n, ws,
+                       static_cast<int64_t>(group) + v);
             if (threadIdx.x == 0) {
-                if (lo == 0) ws.span[v].x = static_cast<int>(blockIdx.x);
-                if (hi == tiles) ws.span[v].y = static_cast<int>(blockIdx.x);
+                if (lo == 0) ws.span[v].x = group;
+                if (hi == n) ws.span[v].y = group;
             }
         }
-        before += chunk;
+        before += __builtin_amdgcn_readlane(end, 63);
     }
 }
 
-// The parts of one row's sequence joined: grid (row tiles, 16, R / 64), sixteen
-// lanes on 64 channels and sixteen groups of them on every sixteenth part, whose
-// sums meet in LDS, in an order that the lengths alone decide.
-constexpr int kJoinGroups = 16;
-template <typename T>
-__global__ __launch_bounds__(16 * kJoinGroups) void join_kernel(kda_mla_absorbed_args a, int rts, int groups) {
+// The parts of one row's sequence joined: grid (row tiles, their rows, R / 4 /
+// LANES), LANES lanes on 4 channels each and 256 / LANES groups of them on every
+// so-manieth part, whose sums meet in LDS, in an order that the lengths alone decide.
+template <typename T, int LANES>
+__global__ __launch_bounds__(256) void join_kernel(kda_mla_absorbed_args a, int rts, int groups) {
     const int64_t v = blockIdx.x, b = v / rts, nv = a.B * rts;
-    const int rows = static_cast<int>(a.T * a.H), m = static_cast<int>(v - b * rts) * kRowTile + blockIdx.y;
+    const int rows = static_cast<int>(a.T * a.H), m = static_cast<int>(v - b * rts) * kRows + blockIdx.y;
     if (m >= rows) return;
-    const int c = 64 * blockIdx.z + 4 * (threadIdx.x & 15), group = threadIdx.x >> 4;
+    constexpr int kJoinGroups = 256 / LANES;
+    const int at = threadIdx.x % LANES, c = 4 * LANES * blockIdx.z + 4 * at, group = threadIdx.x / LANES;
     const Workspace ws = carve(a.workspace, slots(groups, nv), a.R);
     const int2 span = tokens(a.lengths, b, a.S) > 0 ? ws.span[v] : int2{0, -1};
     if (span.x == span.y) return;                // one workgroup had it all, and wrote the result
-    const float2* ml = ws.ml + v * kRowTile + blockIdx.y;
-    const float* o = ws.o + (v * kRowTile + blockIdx.y) * a.R + c;
+    const float2* ml = ws.ml + v * kRows + blockIdx.y;
+    const float* o = ws.o + (v * kRows + blockIdx.y) * a.R + c;
     float top = kNoMax, den = 0.f;
     f4 r{};
-    for (int g = span.x + group; g <= span.y; g += kJoinGroups) {
-        const float2 x = ml[g * kRowTile];
-        const f4 y = *reinterpret_cast<const f4*>(o + static_cast<int64_t>(g) * kRowTile * a.R);
-        const float now = fmaxf(top, x.x), f0 = __builtin_amdgcn_exp2f(top - now);
-        const float f1 = x.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(x.x - now);
-        top = now;
-        den = den * f0 + x.y * f1;
+    // four parts' loads in flight together; one past the last counts as empty
+    constexpr int kAhead = 4;
+    for (int g = span.x + group; g <= span.y; g += kAhead * kJoinGroups) {
+        float2 x[kAhead];
+        f4 y[kAhead];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) r[e] = r[e] * f0 + y[e] * f1;
+        for (int i = 0; i < kAhead; ++i) {
+            const int at_g = min(g + i * kJoinGroups, span.y);
+            x[i] = ml[at_g * kRows];
+            y[i] = *reinterpret_cast<const f4*>(o + static_cast<int64_t>(at_g) * kRows * a.R);
+        }
+        float now = top;
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            if (g + i * kJoinGroups > span.y) x[i] = float2{kNoMax, 0.f};
+            now = fmaxf(now, x[i].x);
+        }
+        const float f0 = __builtin_amdgcn_exp2f(top - now);
+        top = now;
+        den *= f0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) r[e] *= f0;
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            const float f = x[i].y == 0.f ? 0.f : __builtin_amdgcn_exp2f(x[i].x - now);
+            den = fmaf(f, x[i].y, den);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) r[e] = fmaf(f, y[i][e], r[e]);
+        }
     }
-    __shared__ f4 sums[kJoinGroups][16];
+    __shared__ f4 sums[kJoinGroups][LANES];
     __shared__ float2 stats[kJoinGroups];
-    sums[group][threadIdx.x & 15] = r;
-    if ((threadIdx.x & 15) == 0) stats[group] = float2{top, den};
+    sums[group][at] = r;
+    if (at == 0) stats[group] = float2{top, den};
     __syncthreads();
     if (group != 0) return;
     const int n = min(kJoinGroups, span.y - span.x + 1);
@@ -365,7 +429,7 @@ __global__ __launch_bounds__(16 * kJoinGroups) void join_kernel(kda_mla_absorbed
     for (int g = 0; g < n; ++g) {
         const float w = __builtin_amdgcn_exp2f(stats[g].x - top);
         den = fmaf(w, stats[g].y, den);
-        const f4 y = sums[g][threadIdx.x];
+        const f4 y = sums[g][at];
 #pragma unroll
         for (int e = 0; e < 4; ++e) r[e] = fmaf(w, y[e], r[e]);
     }
@@ -374,23 +438,27 @@ __global__ __launch_bounds__(16 * kJoinGroups) void join_kernel(kda_mla_absorbed
         uint2{Act<T>::pair(r[0] * norm, r[1] * norm), Act<T>::pair(r[2] * norm, r[3] * norm)};
 }
 
-int row_tiles(int64_t T, int64_t H) { return static_cast<int>((T * H + kRowTile - 1) / kRowTile); }
+int row_tiles(int64_t T, int64_t H) { return static_cast<int>((T * H + kRows - 1) / kRows); }
 
-constexpr int64_t kGroups = 256;      // workgroups of the shared form: one a CU
-// Whether the tiles are shared among the workgroups: where one workgroup a row
+constexpr int64_t kGroups = 512;      // workgroups of the shared form: two a CU
+// Whether the units are shared among the workgroups: where one workgroup a row
 // tile would leave CUs idle or wait for the longest sequence.
-bool shared_form(int64_t nv, int64_t S) { return nv < 4 * kGroups && S > 16 * kTile; }
+bool shared_form(int64_t nv, int64_t S) { return nv < 4 * kGroups && S > 512; }
 
 template <typename T, bool F8, int R, int P>
 int launch(const kda_mla_absorbed_args& a, hipStream_t stream) {
     const int rts = row_tiles(a.T, a.H);
     const int64_t nv = a.B * rts;
     if (!shared_form(nv, a.S)) {
-        absorbed_kernel<T, F8, R, P><<<static_cast<unsigned>(nv), 64 * kWaves, 0, stream>>>(a, rts);
+        absorbed_kernel<T, F8, R, P><<<static_cast<unsigned>(nv), kThreads, 0, stream>>>(a, rts, true);
     } else {
-        absorbed_shared_kernel<T, F8, R, P><<<kGroups, 64 * kWaves, 0, stream>>>(a, rts);
-        join_kernel<T><<<dim3(static_cast<unsigned>(nv), kRowTile, R / 64), 16 * kJoinGroups, 0, stream>>>(
-            a, rts, static_cast<int>(kGroups));
+        absorbed_kernel<T, F8, R, P><<<kGroups, kThreads, 0, stream>>>(a, rts, false);
+        // many rows have few parts each, and few rows may have many
+        const dim3 grid(static_cast<unsigned>(nv), kRows);
+        if (nv >= 32)
+            join_kernel<T, R / 4><<<grid, 256, 0, stream>>>(a, rts, static_cast<int>(kGroups));
+        else
+            join_kernel<T, 16><<<dim3(grid.x, grid.y, R / 64), 256, 0, stream>>>(a, rts, static_cast<int>(kGroups));
     }
     return hipGetLastError() == hipSuccess ? KDA_OK : KDA_ERR_LAUNCH;
 }
@@ -417,7 +485,7 @@ int launch_rank(const kda_mla_absorbed_args& a, hipStream_t stream) {
 int64_t mla_absorbed_workspace_bytes(int64_t B, int64_t T, int64_t H, int64_t S, int64_t R) {
     const int64_t nv = B * row_tiles(T, H);
     if (nv == 0 || !shared_form(nv, S)) return 0;
-    return slots(kGroups, nv) * kRowTile * (R * 4 + 8) + nv * 8;
+    return slots(kGroups, nv) * kRows * (R * 4 + 8) + nv * 8;
 }
 
 int mla_absorbed_launch(const kda_mla_absorbed_args& a, hipStream_t stream) {

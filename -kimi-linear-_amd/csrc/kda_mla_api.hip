@@ -104,7 +104,7 @@ int kda_mla_absorbed_fwd(const kda_mla_absorbed_args* a, void* stream) {
     if (a->S > 0 && (!a->cache || (f8 && !a->cache_scale))) return KDA_ERR_NULL_POINTER;
     if (!a->workspace && kda::mla_absorbed_workspace_bytes(a->B, a->T, a->H, a->S, a->R) > 0) return KDA_ERR_NULL_POINTER;
     if (!rows_ok(a->q, a->q_stride, 3, 2) || !rows_ok(a->cache, a->cache_stride, 2, f8 ? 1 : 2) || !at16(a->o) ||
-        !at16(a->workspace))
+        !at16(a->workspace) || !near(a->cache_stride[1]))
         return KDA_ERR_UNSUPPORTED;
     if (f8 && (reinterpret_cast<uintptr_t>(a->cache_scale) % 8 != 0 || a->scale_stride[0] % 2 != 0 ||
                a->scale_stride[1] % 2 != 0))
