@@ -31,10 +31,9 @@ namespace {
 
 using namespace mla;
 
-constexpr int kTile = 64;             // keys a tile of the dq kernel
-constexpr int kQTile = 32;            // queries a tile of the dk, dv kernel
-constexpr int kWaves = 4;
-constexpr int kThreads = 64 * kWaves;
+constexpr int kKeys = 32;             // keys a tile of the dq kernel
+constexpr int kStand = 128;           // keys a workgroup of the dk, dv kernel
+constexpr int kPass = 64;             // and queries a step
 
 template <typename T> constexpr bool kHalf = Elem<T>::code == KDA_DTYPE_F16;
 template <typename T> constexpr float kPShift = kHalf<T> ? 12.f : 0.f;
@@ -77,11 +76,11 @@ __device__ __forceinline__ float dot8(uint4 x, uint4 y, float acc, bf16_t) {
 }
 
 // dq of 32 rows a wave, and delta.  Grid as the forward's.
-template <typename T, int N, int P>
-__global__ __launch_bounds__(kThreads, 1) void dq_kernel(kda_mla_expanded_bwd_args g, float* delta, int qtiles) {
+template <typename T, int N, int P, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, 2) void dq_kernel(kda_mla_expanded_bwd_args g, float* delta, int qtiles) {
     const kda_mla_expanded_args& a = g.fwd;
-    using F = KvTile<T, N, P, kThreads, kTile, 8>;
-    constexpr int D = F::D, V = F::V, kRows = 32 * kWaves;
+    using F = KvTile<T, N, P, 64 * WAVES, kKeys, 8>;
+    constexpr int D = F::D, V = F::V, kRows = 32 * WAVES;
     __shared__ __align__(16) T smem[2 * F::kBuf];
     const int64_t bhs = a.B * a.H, bh = blockIdx.x % bhs;
     const Place at(a, bh);
@@ -128,12 +127,11 @@ __global__ __launch_bounds__(kThreads, 1) void dq_kernel(kda_mla_expanded_bwd_ar
         tile.put(smem);
         __syncthreads();
         int cur = 0;
-        for (int j0 = 0; j0 < keys; j0 += kTile) {
-            tile.fetch(a, j0 + kTile, keys);
-#pragma unroll 1
-            for (int u = 0; u < kTile && j0 + u <= wlast; u += 32) {
-                const T* kt = smem + cur * F::kBuf + (u + lq) * F::kK + 8 * half;
-                const T* vt = smem + cur * F::kBuf + kTile * F::kK + (u + lq) * F::kV + 8 * half;
+        for (int j0 = 0; j0 < keys; j0 += kKeys) {
+            tile.fetch(a, j0 + kKeys, keys);
+            if (j0 <= wlast) {
+                const T* kt = smem + cur * F::kBuf + lq * F::kK + 8 * half;
+                const T* vt = smem + cur * F::kBuf + kKeys * F::kK + lq * F::kV + 8 * half;
                 f16v s, dp;
 #pragma unroll
                 for (int e = 0; e < 16; ++e) s[e] = dp[e] = 0.f;
@@ -142,10 +140,10 @@ __global__ __launch_bounds__(kThreads, 1) void dq_kernel(kda_mla_expanded_bwd_ar
 #pragma unroll
                 for (int k = 0; k < V / 16; ++k)
                     dp = Act<T>::mma32(*reinterpret_cast<const uint4*>(vt + 16 * k), d_o[k], dp);
-                if (j0 + u + 31 > wall) {
+                if (j0 + kKeys - 1 > wall) {
 #pragma unroll
                     for (int e = 0; e < 16; ++e)
-                        if (j0 + u + 8 * (e / 4) + 4 * half + e % 4 > limit) s[e] = -INFINITY;
+                        if (j0 + 8 * (e / 4) + 4 * half + e % 4 > limit) s[e] = -INFINITY;
                 }
                 float m = 0.f;
 #pragma unroll
@@ -166,7 +164,7 @@ __global__ __launch_bounds__(kThreads, 1) void dq_kernel(kda_mla_expanded_bwd_ar
 #pragma unroll
                     for (int e = 0; e < 16; ++e) dp[e] *= f;
                 }
-                const T* tr = smem + cur * F::kBuf + (u + 4 * half + ((lane & 15) >> 2)) * F::kK +
+                const T* tr = smem + cur * F::kBuf + (4 * half + ((lane & 15) >> 2)) * F::kK +
                               16 * ((lane >> 4) & 1) + 4 * (lane & 3);
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
@@ -197,61 +195,40 @@ __global__ __launch_bounds__(kThreads, 1) void dq_kernel(kda_mla_expanded_bwd_ar
                       Act<T>::pair(dq[i][4 * e + 2] * norm, dq[i][4 * e + 3] * norm)};
 }
 
-// A tile of queries and their output gradients: [kQTile][D + 8] and
-// [kQTile][V + 8], then lse and delta of each.
-template <typename T, int D, int V>
-struct QTile {
-    static constexpr int kQ = D + 8, kO = V + 8;
-    static constexpr int kRow = kQTile * (kQ + kO);               // elements before lse
-    static constexpr int kBuf = kRow + 4 * kQTile;                // a float is two elements
-    // the position channels apart, so that each part is whole rounds of the threads
-    static constexpr int kP = D % 64 == 0 ? 0 : 32;
-    Rows<T, kQTile, D - kP, kThreads, kQ> q;
-    Rows<T, kQTile, kP, kThreads, kQ> qp;
-    Rows<T, kQTile, V, kThreads, kO> d_o;
-    float x;
-
-    __device__ __forceinline__ QTile(const kda_mla_expanded_bwd_args& g) {
-        q.start(g.fwd.q_stride[1]);
-        qp.start(g.fwd.q_stride[1]);
-        d_o.start(g.d_o_stride[1]);
-    }
-    // Rows past the last that exists are zeros, and their lse makes p zero.
-    __device__ __forceinline__ void fetch(const kda_mla_expanded_bwd_args& g, const T* qb, const T* ob, const float* lse,
-                                          const float* delta, int t0, int exist) {
-        q.fetch(qb, g.fwd.q_stride[1], t0, exist);
-        qp.fetch(qb + D - kP, g.fwd.q_stride[1], t0, exist);
-        d_o.fetch(ob, g.d_o_stride[1], t0, exist);
-        const int t = t0 + (threadIdx.x & (kQTile - 1));
-        const float* from = threadIdx.x & kQTile ? delta : lse;
-        x = from[min(t, exist - 1)];
-        issued();
-    }
-    __device__ __forceinline__ void put(T* buf, int t0, int exist) const {
-        q.put(buf);
-        qp.put(buf + D - kP);
-        d_o.put(buf + kQTile * kQ);
-        if (threadIdx.x < 2 * kQTile) {
-            const bool there = t0 + static_cast<int>(threadIdx.x & (kQTile - 1)) < exist;
-            const float y = threadIdx.x & kQTile ? (there ? x : 0.f) : (there ? x - kPShift<T> : INFINITY);
-            reinterpret_cast<float*>(buf + kRow)[threadIdx.x] = y;
-        }
-    }
+// dk and dv.  A workgroup has kStand keys, whose rows of K and V stay in LDS,
+// and takes kPass queries a step: eight waves, each 32 of the keys and 32 of a
+// step's queries, so that a SIMD has two waves and each holds one half of the
+// sums of its keys, joined at the end.  (Four waves with K and V in registers
+// need more than 256 of them, and moving values between the two halves of the
+// register file took most of the time: 403 us at B=4 T=2048 H=16.)
+// Grid: (key tiles, the first have the most queries) x (batch, head), the latter inner.
+template <typename T, int N, int P>
+struct Dkv {
+    static constexpr int D = N + P, V = N, NT = 512;
+    static constexpr int kK = D + 8, kV = V + 8;                  // LDS rows, elements
+    static constexpr int kStanding = kStand * (kK + kV), kPassing = kPass * (kK + kV);
+    static constexpr int kJoin = 4 * 64 * (D / 32) * 16 * 4;      // bytes: one half's dk
+    static constexpr int kTiles = (kStanding + kPassing) * 2;
+    static constexpr int kBytes = (kTiles > kJoin ? kTiles : kJoin);
 };
 
-// dk and dv of 32 keys a wave.  Grid: (key tiles, the first have the most
-// queries) x (batch, head), the latter inner.
 template <typename T, int N, int P>
-__global__ __launch_bounds__(kThreads, 1) void dkv_kernel(kda_mla_expanded_bwd_args g, const float* delta, float* dpe) {
+__global__ __launch_bounds__(512, 2) void dkv_kernel(kda_mla_expanded_bwd_args g, const float* delta, float* dpe) {
     const kda_mla_expanded_args& a = g.fwd;
-    constexpr int D = N + P, V = N, kKeys = 32 * kWaves;
-    using F = QTile<T, D, V>;
-    __shared__ __align__(16) T smem[2 * F::kBuf];
+    using F = Dkv<T, N, P>;
+    constexpr int D = F::D, V = F::V, kK = F::kK, kV = F::kV;
+    __shared__ __align__(16) char raw[F::kBytes];
+    __shared__ __align__(16) float stats[2][kPass];               // lse and delta of a step's queries
+    T* ks = reinterpret_cast<T*>(raw);
+    T* vs = ks + kStand * kK;
+    T* qs = vs + kStand * kV;
+    T* os = qs + kPass * kK;
     const int64_t bhs = a.B * a.H, bh = blockIdx.x % bhs;
     const Place at(a, bh);
-    const int j0 = static_cast<int>(blockIdx.x / bhs) * kKeys;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lk = lane & 31, half = lane >> 5;
-    const int w0 = j0 + 32 * wave, j = w0 + lk;
+    const int j0 = static_cast<int>(blockIdx.x / bhs) * kStand;
+    const int lane = threadIdx.x & 63, lk = lane & 31, half = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), mine = wave & 3, side = wave >> 2;
+    const int w0 = j0 + 32 * mine, j = w0 + lk;
     const float c = a.scale * kLog2E;
 
     f16v dk[D / 32], dv[V / 32];
@@ -265,53 +242,82 @@ __global__ __launch_bounds__(kThreads, 1) void dkv_kernel(kda_mla_expanded_bwd_a
         for (int e = 0; e < 16; ++e) dv[i][e] = 0.f;
     float f = kHalf<T> ? kFirst : 1.f;
 
-    const int first = max(0, j0 - at.start) / kQTile * kQTile;       // the first queries that see a key of these
+    const int first = max(0, j0 - at.start) / kPass * kPass;         // the first queries that see a key of these
     if (j0 < at.len && first < at.exist) {
-        const int jc = min(j, at.len - 1);
-        const T* kr = static_cast<const T*>(a.k) + at.b * a.k_stride[0] + jc * a.k_stride[1] + at.h * a.k_stride[2] +
-                      8 * half;
-        const T* pr = static_cast<const T*>(a.k_pe) + at.b * a.k_pe_stride[0] + jc * a.k_pe_stride[1] + 8 * half;
-        const T* vr = static_cast<const T*>(a.v) + at.b * a.v_stride[0] + jc * a.v_stride[1] + at.h * a.v_stride[2] +
-                      8 * half;
-        uint4 k[D / 16], v[V / 16];
-#pragma unroll
-        for (int i = 0; i < N / 16; ++i) k[i] = *reinterpret_cast<const uint4*>(kr + 16 * i);
-#pragma unroll
-        for (int i = 0; i < P / 16; ++i) k[N / 16 + i] = *reinterpret_cast<const uint4*>(pr + 16 * i);
-#pragma unroll
-        for (int i = 0; i < V / 16; ++i) v[i] = *reinterpret_cast<const uint4*>(vr + 16 * i);
-        const T* qp = static_cast<const T*>(a.q) + at.b * a.q_stride[0] + at.h * a.q_stride[2];
-        const T* dop = static_cast<const T*>(g.d_o) + at.b * g.d_o_stride[0] + at.h * g.d_o_stride[2];
-        const float *lse = a.lse + bh * a.T, *del = delta + bh * a.T;
-        F tile(g);
-        tile.fetch(g, qp, dop, lse, del, first, at.exist);
-        tile.put(smem, first, at.exist);
+        const T* qb = static_cast<const T*>(a.q) + at.b * a.q_stride[0] + at.h * a.q_stride[2];
+        const T* ob = static_cast<const T*>(g.d_o) + at.b * g.d_o_stride[0] + at.h * g.d_o_stride[2];
+        const float* sb = (threadIdx.x & kPass ? delta : a.lse) + bh * a.T;
+        constexpr int kP = D % 64 == 0 ? 0 : 32;                     // so that each part is whole rounds of the threads
+        Rows<T, kPass, D - kP, F::NT, kK> q;
+        Rows<T, kPass, kP, F::NT, kK> qp;
+        Rows<T, kPass, V, F::NT, kV> d_o;
+        q.start(a.q_stride[1]);
+        qp.start(a.q_stride[1]);
+        d_o.start(g.d_o_stride[1]);
+        float x;
+        // rows past the last query that exists are zeros, and their lse makes p zero
+        const auto fetch = [&](int t0) {
+            q.fetch(qb, a.q_stride[1], t0, at.exist);
+            qp.fetch(qb + D - kP, a.q_stride[1], t0, at.exist);
+            d_o.fetch(ob, g.d_o_stride[1], t0, at.exist);
+            x = sb[min(t0 + static_cast<int>(threadIdx.x & (kPass - 1)), at.exist - 1)];
+            issued();
+        };
+        const auto put = [&](int t0) {
+            q.put(qs);
+            qp.put(qs + D - kP);
+            d_o.put(os);
+            if (threadIdx.x < 2 * kPass) {
+                const bool there = t0 + static_cast<int>(threadIdx.x & (kPass - 1)) < at.exist;
+                (&stats[0][0])[threadIdx.x] = threadIdx.x & kPass ? (there ? x : 0.f) : (there ? x - kPShift<T> : INFINITY);
+            }
+        };
+        fetch(first);
+        {
+            Rows<T, kStand, N, F::NT, kK> k;
+            Rows<T, kStand, P, F::NT, kK> pe;
+            Rows<T, kStand, V, F::NT, kV> v;
+            k.start(a.k_stride[1]);
+            pe.start(a.k_pe_stride[1]);
+            v.start(a.v_stride[1]);
+            k.fetch(static_cast<const T*>(a.k) + at.b * a.k_stride[0] + at.h * a.k_stride[2], a.k_stride[1], j0, at.len);
+            pe.fetch(static_cast<const T*>(a.k_pe) + at.b * a.k_pe_stride[0], a.k_pe_stride[1], j0, at.len);
+            v.fetch(static_cast<const T*>(a.v) + at.b * a.v_stride[0] + at.h * a.v_stride[2], a.v_stride[1], j0, at.len);
+            k.put(ks);
+            pe.put(ks + N);
+            v.put(vs);
+        }
+        put(first);
         __syncthreads();
-        int cur = 0;
-        for (int t0 = first; t0 < at.exist; t0 += kQTile) {
-            tile.fetch(g, qp, dop, lse, del, t0 + kQTile, at.exist);
-            if (at.start + t0 + kQTile - 1 >= w0 && w0 < at.len) {
-                const T* buf = smem + cur * F::kBuf;
-                const T* qt = buf + lk * F::kQ + 8 * half;
-                const T* ot = buf + kQTile * F::kQ + lk * F::kO + 8 * half;
-                const float* st = reinterpret_cast<const float*>(buf + F::kRow) + 4 * half;
+        for (int t0 = first; t0 < at.exist; t0 += kPass) {
+            fetch(t0 + kPass);
+            const int tw = t0 + 32 * side;                            // the wave's queries
+            if (tw < at.exist && at.start + tw + 31 >= w0 && w0 < at.len) {
+                const T* qt = qs + (32 * side + lk) * kK + 8 * half;
+                const T* ot = os + (32 * side + lk) * kV + 8 * half;
+                const T* kt = ks + (32 * mine + lk) * kK + 8 * half;
+                const T* vt = vs + (32 * mine + lk) * kV + 8 * half;
                 f16v s, dp;
 #pragma unroll
                 for (int e = 0; e < 16; ++e) s[e] = dp[e] = 0.f;
 #pragma unroll
-                for (int i = 0; i < D / 16; ++i) s = Act<T>::mma32(*reinterpret_cast<const uint4*>(qt + 16 * i), k[i], s);
+                for (int i = 0; i < D / 16; ++i)
+                    s = Act<T>::mma32(*reinterpret_cast<const uint4*>(qt + 16 * i),
+                                      *reinterpret_cast<const uint4*>(kt + 16 * i), s);
 #pragma unroll
                 for (int i = 0; i < V / 16; ++i)
-                    dp = Act<T>::mma32(*reinterpret_cast<const uint4*>(ot + 16 * i), v[i], dp);
-                if (at.start + t0 < w0 + 31 || w0 + 32 > at.len) {
+                    dp = Act<T>::mma32(*reinterpret_cast<const uint4*>(ot + 16 * i),
+                                       *reinterpret_cast<const uint4*>(vt + 16 * i), dp);
+                if (at.start + tw < w0 + 31 || w0 + 32 > at.len) {
 #pragma unroll
                     for (int e = 0; e < 16; ++e)
-                        if (at.start + t0 + 8 * (e / 4) + 4 * half + e % 4 < j || j >= at.len) s[e] = -INFINITY;
+                        if (at.start + tw + 8 * (e / 4) + 4 * half + e % 4 < j || j >= at.len) s[e] = -INFINITY;
                 }
                 float m = 0.f;
+                const float* st = &stats[0][32 * side + 4 * half];
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {
-                    const f4 l = *reinterpret_cast<const f4*>(st + 8 * u), d = *reinterpret_cast<const f4*>(st + kQTile + 8 * u);
+                    const f4 l = *reinterpret_cast<const f4*>(st + 8 * u), d = *reinterpret_cast<const f4*>(st + kPass + 8 * u);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const float p = __builtin_amdgcn_exp2f(fmaf(s[4 * u + e], c, -l[e]));
@@ -333,9 +339,9 @@ __global__ __launch_bounds__(kThreads, 1) void dkv_kernel(kda_mla_expanded_bwd_a
 #pragma unroll
                     for (int e = 0; e < 16; ++e) dp[e] *= f;
                 }
-                const int trow = 4 * half + ((lane & 15) >> 2), tcol = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
-                const T* qtr = buf + trow * F::kQ + tcol;
-                const T* otr = buf + kQTile * F::kQ + trow * F::kO + tcol;
+                const int trow = 32 * side + 4 * half + ((lane & 15) >> 2), tcol = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+                const T* qtr = qs + trow * kK + tcol;
+                const T* otr = os + trow * kV + tcol;
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
                     const uint4 pf{Act<T>::pair(s[8 * u], s[8 * u + 1]), Act<T>::pair(s[8 * u + 2], s[8 * u + 3]),
@@ -344,23 +350,52 @@ __global__ __launch_bounds__(kThreads, 1) void dkv_kernel(kda_mla_expanded_bwd_a
                                    Act<T>::pair(dp[8 * u + 4], dp[8 * u + 5]), Act<T>::pair(dp[8 * u + 6], dp[8 * u + 7])};
 #pragma unroll
                     for (int i = 0; i < V / 32; ++i) {
-                        const uint2 y = read_tr(otr + 16 * u * F::kO + 32 * i), z = read_tr(otr + (16 * u + 8) * F::kO + 32 * i);
+                        const uint2 y = read_tr(otr + 16 * u * kV + 32 * i), z = read_tr(otr + (16 * u + 8) * kV + 32 * i);
                         dv[i] = Act<T>::mma32(uint4{y.x, y.y, z.x, z.y}, pf, dv[i]);
                     }
 #pragma unroll
                     for (int i = 0; i < D / 32; ++i) {
-                        const uint2 y = read_tr(qtr + 16 * u * F::kQ + 32 * i), z = read_tr(qtr + (16 * u + 8) * F::kQ + 32 * i);
+                        const uint2 y = read_tr(qtr + 16 * u * kK + 32 * i), z = read_tr(qtr + (16 * u + 8) * kK + 32 * i);
                         dk[i] = Act<T>::mma32(uint4{y.x, y.y, z.x, z.y}, df, dk[i]);
                     }
                 }
             }
-            cur ^= 1;
-            tile.put(smem + cur * F::kBuf, t0 + kQTile, at.exist);
+            __syncthreads();
+            put(t0 + kPass);
             __syncthreads();
         }
     }
-    if (j >= a.S) return;
+    // the two sides' sums, the second's onto the first's
     const float pn = __builtin_amdgcn_exp2f(-kPShift<T>), norm = a.scale * pn / f;
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) dk[i][e] *= norm;
+    f4* half_sums = reinterpret_cast<f4*>(raw) + mine * (D / 32) * 4 * 64 + lane;
+    const auto join = [&](auto& x, int n) {
+        if (side == 1) {
+#pragma unroll
+            for (int i = 0; i < n; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    half_sums[(4 * i + e) * 64] = f4{x[i][4 * e], x[i][4 * e + 1], x[i][4 * e + 2], x[i][4 * e + 3]};
+        }
+        __syncthreads();
+        if (side == 0) {
+#pragma unroll
+            for (int i = 0; i < n; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const f4 y = half_sums[(4 * i + e) * 64];
+#pragma unroll
+                    for (int d = 0; d < 4; ++d) x[i][4 * e + d] += y[d];
+                }
+        }
+        __syncthreads();
+    };
+    join(dk, D / 32);
+    join(dv, V / 32);
+    if (side == 1 || j >= a.S) return;
     const int64_t row = (at.b * a.S + j) * a.H + at.h;
     T* kout = static_cast<T*>(g.dk) + row * N + 4 * half;
     T* vout = static_cast<T*>(g.dv) + row * V + 4 * half;
@@ -368,9 +403,8 @@ __global__ __launch_bounds__(kThreads, 1) void dkv_kernel(kda_mla_expanded_bwd_a
     for (int i = 0; i < N / 32; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            *reinterpret_cast<uint2*>(kout + 32 * i + 8 * e) =
-                uint2{Act<T>::pair(dk[i][4 * e] * norm, dk[i][4 * e + 1] * norm),
-                      Act<T>::pair(dk[i][4 * e + 2] * norm, dk[i][4 * e + 3] * norm)};
+            *reinterpret_cast<uint2*>(kout + 32 * i + 8 * e) = uint2{Act<T>::pair(dk[i][4 * e], dk[i][4 * e + 1]),
+                                                                     Act<T>::pair(dk[i][4 * e + 2], dk[i][4 * e + 3])};
             *reinterpret_cast<uint2*>(vout + 32 * i + 8 * e) =
                 uint2{Act<T>::pair(dv[i][4 * e] * pn, dv[i][4 * e + 1] * pn),
                       Act<T>::pair(dv[i][4 * e + 2] * pn, dv[i][4 * e + 3] * pn)};
@@ -382,8 +416,7 @@ __global__ __launch_bounds__(kThreads, 1) void dkv_kernel(kda_mla_expanded_bwd_a
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const f16v& x = dk[N / 32 + i];
-                *reinterpret_cast<f4*>(out + 32 * i + 8 * e) = f4{x[4 * e] * norm, x[4 * e + 1] * norm,
-                                                                  x[4 * e + 2] * norm, x[4 * e + 3] * norm};
+                *reinterpret_cast<f4*>(out + 32 * i + 8 * e) = f4{x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3]};
             }
     }
 }
@@ -411,12 +444,15 @@ int launch(const kda_mla_expanded_bwd_args& g, hipStream_t stream) {
     const kda_mla_expanded_args& a = g.fwd;
     float* delta = static_cast<float*>(g.workspace);
     float* dpe = reinterpret_cast<float*>(static_cast<char*>(g.workspace) + delta_bytes(a.B, a.T, a.H));
-    const int64_t qtiles = (a.T + 32 * kWaves - 1) / (32 * kWaves), ktiles = (a.S + 32 * kWaves - 1) / (32 * kWaves);
-    if (qtiles > 0)
-        dq_kernel<T, N, P><<<static_cast<unsigned>(qtiles * a.B * a.H), kThreads, 0, stream>>>(
-            g, delta, static_cast<int>(qtiles));
+    const int64_t bhs = a.B * a.H, ktiles = (a.S + kStand - 1) / kStand;
+    // eight waves a workgroup where that leaves every CU one
+    const int64_t wide = (a.T + 255) / 256, narrow = (a.T + 127) / 128;
+    if (wide * bhs >= 256)
+        dq_kernel<T, N, P, 8><<<static_cast<unsigned>(wide * bhs), 512, 0, stream>>>(g, delta, static_cast<int>(wide));
+    else if (narrow > 0)
+        dq_kernel<T, N, P, 4><<<static_cast<unsigned>(narrow * bhs), 256, 0, stream>>>(g, delta, static_cast<int>(narrow));
     if (ktiles == 0) return hipGetLastError() == hipSuccess ? KDA_OK : KDA_ERR_LAUNCH;
-    dkv_kernel<T, N, P><<<static_cast<unsigned>(ktiles * a.B * a.H), kThreads, 0, stream>>>(g, delta, dpe);
+    dkv_kernel<T, N, P><<<static_cast<unsigned>(ktiles * bhs), 512, 0, stream>>>(g, delta, dpe);
     if constexpr (P > 0) {
         const int64_t n = a.S * P / 4;
         dpe_kernel<T><<<static_cast<unsigned>((a.B * n + 255) / 256), 256, 0, stream>>>(dpe, static_cast<T*>(g.dk_pe),
