@@ -1,4 +1,5 @@
-"""hipGraph-captured decoding over a stack of KDA layers.
+"""hipGraph-captured decoding over a stack of KDA layers, latent-attention
+layers (:class:`kimi_linear_amd.LatentAttention`) or both.
 
 The capture recipe of the reference's ``GraphedDecoder``
 (``kimi_linear/graph_decode.py:241-289``), for the KDA part of the model:
@@ -20,9 +21,14 @@ place (``KimiDeltaAttention.decode_step_``), so a replay touches each state
 element exactly once for reading and once for writing; only the small conv
 windows are shifted by copy.
 
+A latent layer's state is its cache, a buffer for ``max_tokens`` tokens that a
+step appends to in place; the tokens held are counted on the device, where the
+captured kernels read them, and on the host, where :meth:`step` refuses a full
+cache.  Rows past the count are never read, so a snapshot is the count alone.
+
 The stack is ``h <- h + layer(h)`` per layer (``residual=True``) or
-``h <- layer(h)``; the model's other blocks (MLA, FFN, norms, LM head) are not
-part of the KDA path.
+``h <- layer(h)``; the model's other blocks (FFN, norms, LM head) are not
+part of it.
 """
 
 from __future__ import annotations
@@ -32,11 +38,13 @@ from typing import Sequence
 import torch
 import torch.nn as nn
 
+from .kda import KdaError
 from .layer import KimiDeltaAttention
+from .mla_layer import LatentAttention
 
 
 class KdaGraphedDecoder:
-    """Graph-replayed incremental decoding of a stack of KDA layers.
+    """Graph-replayed incremental decoding of a stack of KDA and latent-attention layers.
 
     Usage::
 
@@ -58,7 +66,7 @@ class KdaGraphedDecoder:
     ``step`` calls of one generation, call :meth:`refresh_weights`.
     """
 
-    def __init__(self, layers: Sequence[KimiDeltaAttention], residual: bool = True, warmup_iters: int = 3):
+    def __init__(self, layers: Sequence[KimiDeltaAttention | LatentAttention], residual: bool = True, warmup_iters: int = 3):
         self.layers = nn.ModuleList(layers)
         if len(self.layers) == 0:
             raise ValueError("KdaGraphedDecoder needs at least one layer")
@@ -73,6 +81,9 @@ class KdaGraphedDecoder:
     def _weight_buffers(self):
         bufs = []
         for layer in self.layers:
+            if isinstance(layer, LatentAttention):
+                bufs.append(tuple(layer._weight_buffers()))
+                continue
             w, b = layer._input_weight()
             a_log, dt_bias = layer._gate_params()
             bufs.append((w.data_ptr(), b.data_ptr() if b is not None else 0, a_log.data_ptr(), dt_bias.data_ptr()))
@@ -109,28 +120,55 @@ class KdaGraphedDecoder:
                 # the residual add belongs to the output projection, which writes the result in place
                 h = layer._decode(h, st, h, result if i + 1 == len(self.layers) else None)
                 continue
-            out = layer.decode_step_(h, st)
+            out = layer._step(h, st) if isinstance(layer, LatentAttention) else layer.decode_step_(h, st)
             h = h + out if self.residual else out
         if h is not result:
             self.output_static.copy_(h[:, -1, :])
 
     # ------------------------------------------------------------ state plumbing
     def _snapshot(self):
-        return [{"conv": {n: t.clone() for n, t in st["conv"].items()}, "recurrent": st["recurrent"].clone()}
+        return [{"lengths": st["lengths"].clone()} if "latent" in st else
+                {"conv": {n: t.clone() for n, t in st["conv"].items()}, "recurrent": st["recurrent"].clone()}
                 for st in self.static_states]
 
     def _restore(self, snap):
         for st, sn in zip(self.static_states, snap):
+            if "latent" in st:
+                st["lengths"].copy_(sn["lengths"])
+                continue
             for n in st["conv"]:
                 st["conv"][n].copy_(sn["conv"][n])
             st["recurrent"].copy_(sn["recurrent"])
 
     def _fill_static(self, states):
-        if self.static_states is None:
-            self.static_states = [{"conv": {n: t.clone() for n, t in st["conv"].items()},
+        if self.static_states is None:          # a prompt's own cache becomes the static one
+            self.static_states = [st if "latent" in st else
+                                  {"conv": {n: t.clone() for n, t in st["conv"].items()},
                                    "recurrent": st["recurrent"].clone()} for st in states]
-        else:
-            self._restore(states)
+            return
+        for st, new in zip(self.static_states, states):
+            if "latent" in st:
+                n = st["tokens"] = new["tokens"]
+                st["latent"][:, :n].copy_(new["latent"][:, :n])
+                if st["scale"] is not None:
+                    st["scale"][:, :n].copy_(new["scale"][:, :n])
+        self._restore(states)
+
+    @staticmethod
+    def _alike(st, new):
+        """Whether a captured step over the state st serves the state new."""
+        if "latent" in st:
+            return st["latent"].shape == new["latent"].shape and st["latent"].dtype == new["latent"].dtype
+        return st["recurrent"].dtype == new["recurrent"].dtype
+
+    def _advance(self, n=0):
+        """Refuse a step that a latent cache has no room for, or count n tokens."""
+        for st in self.static_states:
+            if "latent" not in st:
+                continue
+            if n == 0 and st["tokens"] >= st["latent"].shape[1]:
+                raise KdaError(f"a latent cache is full ({st['tokens']} tokens): prefill again, or raise max_tokens")
+            st["tokens"] += n
 
     @torch.no_grad()
     def _capture(self):
@@ -166,7 +204,7 @@ class KdaGraphedDecoder:
             self.graph = None
             self.static_states = None
         if self.static_states is not None and any(
-                st["recurrent"].dtype != new["recurrent"].dtype for st, new in zip(self.static_states, states)):
+                not self._alike(st, new) for st, new in zip(self.static_states, states)):
             self.graph = None
             self.static_states = None
         if self.graph is not None and self._weight_buffers() != self._wbufs:
@@ -185,13 +223,17 @@ class KdaGraphedDecoder:
             raise RuntimeError("call prefill() before step()")
         if tuple(x.shape) != tuple(self.input_static.shape):
             raise ValueError(f"step takes x of shape {tuple(self.input_static.shape)}, got {tuple(x.shape)}")
+        self._advance()
         self.input_static.copy_(x)
         self.graph.replay()
+        self._advance(1)
         return self.output_static
 
     @torch.no_grad()
     def step_eager(self, x: torch.Tensor) -> torch.Tensor:
         """The same step without the graph, on the same static state."""
+        self._advance()
         self.input_static.copy_(x)
         self._step()
+        self._advance(1)
         return self.output_static

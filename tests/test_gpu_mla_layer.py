@@ -1,0 +1,176 @@
+"""The latent-attention layer: against its float64 restatement, its gradients, its cached calls, and a
+captured stack that mixes it with KDA layers.
+
+Tolerances are relative L2 norms.  A rounding to a type is off by at most u = finfo.eps / 2 of the value,
+rms u / sqrt(3); the layer's forward rounds eight times in a row (projections, norm, weights, output), and
+their errors added up without cancelling are 8 u / sqrt(3): 1.8e-2 in bf16, 2.3e-3 in fp16.  A gradient
+passes twice as many.  An 8-bit cache adds e4m3's rounding of keys and values, rms 2^-4 / sqrt(3) = 3.6e-2
+each, at scores of size one."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda:0"
+TOL = {torch.bfloat16: 1.8e-2, torch.float16: 2.3e-3}
+
+
+def rel(a, b):
+    a, b = a.detach().double(), b.detach().double()
+    return ((a - b).norm() / b.norm()).item()
+
+
+def make(kda_pkg, dtype, seed=0, **kw):
+    torch.manual_seed(seed)
+    cfg = kda_pkg.latent_attn_config(**{**dict(hidden_size=256, num_heads=4, head_dim=64, position_dim=32, rank=128,
+                                               max_tokens=96), **kw})
+    layer = kda_pkg.LatentAttention(cfg)
+    with torch.no_grad():
+        layer.kv_norm.add_(0.1 * torch.randn_like(layer.kv_norm))
+    return layer.to(DEV, dtype)
+
+
+def reference(layer, x):
+    """The layer in float64, differentiable in its parameters' copies: (output, parameters)."""
+    p = {n: t.detach().double().requires_grad_() for n, t in layer.named_parameters()}
+    B, T, _ = x.shape
+    H, N, P, R = layer.num_heads, layer.head_dim, layer.position_dim, layer.rank
+    q = (x @ p["q_proj.weight"].T).view(B, T, H, N + P).transpose(1, 2)
+    c = x @ p["kv_down.weight"].T
+    lat = c[..., :R] * torch.rsqrt(c[..., :R].square().mean(-1, keepdim=True) + layer.eps) * p["kv_norm"]
+    kv = (lat @ p["kv_up.weight"].T).view(B, T, H, 2 * N).transpose(1, 2)
+    k = torch.cat([kv[..., :N], c[:, None, :, R:].expand(B, H, T, P)], -1)
+    s = (q @ k.transpose(2, 3) * layer.scale).masked_fill(torch.ones(T, T, device=DEV, dtype=torch.bool).triu(1), -torch.inf)
+    o = (torch.softmax(s, -1) @ kv[..., N:]).transpose(1, 2).reshape(B, T, H * N)
+    return o @ p["o_proj.weight"].T, p
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("T,kw", [(77, {}), (1, {}), (150, dict(head_dim=128, position_dim=64, rank=256)),
+                                  (40, dict(position_dim=0))])
+def test_forward_and_gradients(kda_pkg, dtype, T, kw):
+    layer = make(kda_pkg, dtype, **kw)
+    x = torch.randn(2, T, 256, device=DEV).to(dtype).requires_grad_()
+    w = torch.randn(2, T, 256, device=DEV).to(dtype)
+    out = layer(x)
+    out.backward(w)
+    xd = x.detach().double().requires_grad_()
+    want, p = reference(layer, xd)
+    want.backward(w.double())
+    assert rel(out, want) <= TOL[dtype]
+    assert rel(x.grad, xd.grad) <= 2 * TOL[dtype]
+    for n, t in layer.named_parameters():
+        if T == 1 and n in ("q_proj.weight",):       # one key: its weight is 1 whatever q is
+            # dp - delta is the difference of two fp32 sums of N <= 128 products, each off by at most
+            # N 2^-24 sum |do v|; through scale k x (|k| <= |W_k c|, bounded here by the largest) and two sequences
+            with torch.no_grad():
+                H, N = layer.num_heads, layer.head_dim
+                do = (w.double() @ p["o_proj.weight"]).view(2, H, N)
+                c = x.double()[:, 0] @ p["kv_down.weight"].T
+                lat = c[:, :layer.rank]
+                lat = lat * torch.rsqrt(lat.square().mean(-1, keepdim=True) + layer.eps) * p["kv_norm"]
+                kv = (lat @ p["kv_up.weight"].T).view(2, H, 2 * N)
+                k = max(kv[..., :N].abs().max().item(), c.abs().max().item())
+                ds = 2 * N * 2.0 ** -24 * (do * kv[..., N:]).abs().sum(-1).max().item()
+                assert t.grad.abs().max().item() <= 2 * 1.1 * layer.scale * ds * k * x.abs().max().item()
+            continue
+        if T == 1 and n == "kv_down.weight":
+            assert rel(t.grad[:layer.rank], p[n].grad[:layer.rank]) <= 2 * TOL[dtype]
+            continue
+        assert rel(t.grad, p[n].grad) <= 2 * TOL[dtype], n
+    with torch.no_grad():
+        assert rel(layer(x), want) <= TOL[dtype]
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+def test_cached_calls(kda_pkg, bits):
+    """A prompt in two pieces and tokens one by one give what the whole sequence gives."""
+    dtype = torch.bfloat16
+    layer = make(kda_pkg, dtype, cache_bits=bits)
+    x = torch.randn(2, 96, 256, device=DEV).to(dtype)
+    with torch.no_grad():
+        want, _ = reference(layer, x.double())
+        out, state = layer(x[:, :50], use_cache=True)
+        got = [out]
+        out, state = layer(x[:, 50:83], state=state, use_cache=True)
+        got.append(out)
+        for t in range(83, 96):
+            out, state = layer(x[:, t:t + 1], state=state, use_cache=True)
+            got.append(out)
+        assert state["tokens"] == 96 and state["lengths"].tolist() == [96, 96]
+        # the absorbed form rounds q and o once more each
+        assert rel(torch.cat(got, 1), want) <= TOL[dtype] * 10 / 8 + (0 if bits == 16 else 2 * 3.6e-2)
+        before = state["latent"].view(torch.uint8).clone()
+        for call in (lambda: layer(x[:, :1], state=state, use_cache=True), lambda: layer.decode_step_(x[:, :1], state),
+                     lambda: layer(x[:, :5], state=state, use_cache=True)):
+            with pytest.raises(kda_pkg.KdaError, match="96"):
+                call()
+        assert torch.equal(state["latent"].view(torch.uint8), before) and state["lengths"].tolist() == [96, 96]
+        with pytest.raises(kda_pkg.KdaError):
+            layer(x[:, :1], state=state)
+    with pytest.raises(kda_pkg.KdaError):
+        layer(x, use_cache=True)                     # under grad mode
+    with pytest.raises(kda_pkg.KdaError):
+        make(kda_pkg, dtype, cache_bits=4)
+
+
+def test_weights_change(kda_pkg):
+    layer = make(kda_pkg, torch.float16)
+    x = torch.randn(1, 9, 256, device=DEV).half()
+    with torch.no_grad():
+        _, state = layer(x[:, :8], use_cache=True)
+        layer._up_weights()
+        layer.kv_up.weight.mul_(0.5)                 # half the values and, nearly, half the output
+        _, state = layer(x[:, :8], use_cache=True)
+        got, _ = layer(x[:, 8:], state=state, use_cache=True)
+        assert rel(got, reference(layer, x.double())[0][:, 8:]) <= TOL[torch.float16] * 10 / 8
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+def test_mixed_stack_captured(kda_pkg, bits):
+    from kimi_linear_amd.graph_decode import KdaGraphedDecoder
+    dtype = torch.float16
+    torch.manual_seed(3)
+    cfg = kda_pkg.linear_attn_config(hidden_size=256, num_heads=2, gate_low_rank=32, output_gate_low_rank=32)
+    layers = [kda_pkg.KimiDeltaAttention(cfg).to(DEV, dtype).eval(), make(kda_pkg, dtype, seed=4, cache_bits=bits).eval(),
+              kda_pkg.KimiDeltaAttention(cfg).to(DEV, dtype).eval()]
+    x = torch.randn(2, 90, 256, device=DEV).to(dtype)
+    with torch.no_grad():
+        dec = KdaGraphedDecoder(layers)
+        for n, steps in ((40, 12), (61, 20), (5, 3)):        # the second and third prompt reuse the capture
+            h = dec.prefill(x[:, :n])
+            captured = dec.graph
+            states, y = [None] * 3, x[:, :n]
+            for i, layer in enumerate(layers):
+                out, states[i] = layer(y, use_cache=True)
+                y = y + out
+            assert torch.equal(h, y[:, -1])
+            for t in range(n, n + steps):
+                got = dec.step(x[:, t:t + 1]).clone()
+                y = x[:, t:t + 1]
+                for i, layer in enumerate(layers):
+                    out, states[i] = layer(y, state=states[i], use_cache=True)
+                    y = y + out
+                torch.cuda.synchronize()
+                assert torch.equal(got, y[:, 0]), (n, t)
+            assert dec.graph is captured
+        # a full cache is refused on the host, before the replay
+        dec.prefill(x[:, :90].repeat(1, 2, 1)[:, :94])
+        dec.step(x[:, :1])
+        dec.step(x[:, :1])
+        with pytest.raises(kda_pkg.KdaError, match="full"):
+            dec.step(x[:, :1])
+        assert dec.static_states[1]["lengths"].tolist() == [96, 96]
+        # new weights are seen by the captured step
+        dec.prefill(x[:, :30])
+        a = dec.step(x[:, 30:31]).clone()
+        layers[1].kv_up.weight.mul_(1.5)
+        dec.prefill(x[:, :30])
+        b = dec.step(x[:, 30:31]).clone()
+        assert not torch.equal(a, b)
+        c = KdaGraphedDecoder(layers)
+        c.prefill(x[:, :30])
+        assert torch.equal(c.step_eager(x[:, 30:31]), b)
