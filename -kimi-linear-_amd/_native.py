@@ -157,6 +157,7 @@ class KdaMlaExpandedArgs(ctypes.Structure):
         ("k_pe", ctypes.c_void_p), ("k_pe_stride", ctypes.c_int64 * 2), ("v", ctypes.c_void_p), ("v_stride", _i64x3),
         ("lengths", ctypes.c_void_p), ("starts", ctypes.c_void_p),
         ("o", ctypes.c_void_p), ("lse", ctypes.c_void_p), ("scale", ctypes.c_float), ("dtype", ctypes.c_int32),
+        ("workspace", ctypes.c_void_p),
     ]
 
 
@@ -217,6 +218,7 @@ EXPORTED_SYMBOLS = ("kda_chunkwise_fwd", "kda_recurrent_fwd", "kda_chunkwise_fwd
                     "kda_prep_fwd", "kda_output_fwd", "kda_linear_fwd", "kda_linear_wgrad",
                     "kda_linear_wgrad_workspace_size", "kda_prep_bwd", "kda_prep_bwd_workspace_size",
                     "kda_output_bwd", "kda_output_bwd_workspace_size", "kda_mla_expanded_fwd", "kda_mla_expanded_bwd",
+                    "kda_mla_expanded_workspace_size",
                     "kda_mla_expanded_bwd_workspace_size", "kda_mla_absorbed_fwd", "kda_mla_absorbed_workspace_size",
                     "kda_mla_cache_append", "kda_mla_cache_read", "kda_status_str", "kda_abi_version")
 
@@ -296,7 +298,7 @@ def load() -> ctypes.CDLL:
                            ("cache_read", KdaMlaReadArgs)):
             getattr(lib, f"kda_mla_{name}").argtypes = [ctypes.POINTER(args), ctypes.c_void_p]
             getattr(lib, f"kda_mla_{name}").restype = ctypes.c_int
-        for name in ("expanded_bwd", "absorbed"):
+        for name in ("expanded", "expanded_bwd", "absorbed"):
             getattr(lib, f"kda_mla_{name}_workspace_size").argtypes = [ctypes.c_int64] * 5
             getattr(lib, f"kda_mla_{name}_workspace_size").restype = ctypes.c_size_t
         lib.kda_status_str.argtypes = [ctypes.c_int]

@@ -53,6 +53,7 @@ struct Fns {
     decltype(&kda_linear_wgrad) wgrad = nullptr;
     decltype(&kda_linear_wgrad_workspace_size) wgrad_ws = nullptr;
     decltype(&kda_mla_expanded_fwd) mla_expanded = nullptr;
+    decltype(&kda_mla_expanded_workspace_size) mla_expanded_ws = nullptr;
     decltype(&kda_mla_expanded_bwd) mla_expanded_bwd = nullptr;
     decltype(&kda_mla_expanded_bwd_workspace_size) mla_expanded_bwd_ws = nullptr;
     decltype(&kda_mla_absorbed_fwd) mla_absorbed = nullptr;
@@ -90,6 +91,7 @@ void bind(const py::dict& addr, const py::object& stream_fn, const py::object& e
     take(fn.wgrad, addr, "kda_linear_wgrad");
     take(fn.wgrad_ws, addr, "kda_linear_wgrad_workspace_size");
     take(fn.mla_expanded, addr, "kda_mla_expanded_fwd");
+    take(fn.mla_expanded_ws, addr, "kda_mla_expanded_workspace_size");
     take(fn.mla_expanded_bwd, addr, "kda_mla_expanded_bwd");
     take(fn.mla_expanded_bwd_ws, addr, "kda_mla_expanded_bwd_workspace_size");
     take(fn.mla_absorbed, addr, "kda_mla_absorbed_fwd");
@@ -611,7 +613,13 @@ bool expanded_forward(const Tensor& q, const Tensor& k, const OptTensor& k_pe, c
         const auto opt = q.options().requires_grad(false);
         o = at::empty({q.size(0), q.size(1), q.size(2), v.size(3)}, opt);
         if (lse) *lse = at::empty({q.size(0), q.size(2), q.size(1)}, opt.dtype(at::kFloat));
-        const auto a = expanded_args(q, k, k_pe, v, lengths, starts, scale, o, lse ? *lse : OptTensor());
+        auto a = expanded_args(q, k, k_pe, v, lengths, starts, scale, o, lse ? *lse : OptTensor());
+        const size_t bytes = fn.mla_expanded_ws(a.B, a.T, a.S, a.H, a.V);
+        Tensor ws;
+        if (bytes > 0) {
+            ws = at::empty({static_cast<int64_t>(bytes)}, opt.dtype(at::kByte));
+            a.workspace = ws.data_ptr();
+        }
         return fn.mla_expanded(&a, stream);
     });
     return !refused(status, "kda_mla_expanded_fwd");

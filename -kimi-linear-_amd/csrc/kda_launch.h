@@ -80,6 +80,7 @@ int linear_wgrad_launch(const kda_linear_wgrad_args& a, hipStream_t stream);
 
 // Latent attention (kda_mla_*.hip); arguments checked by the caller, no work
 // of size zero.
+int64_t mla_expanded_workspace_bytes(int64_t B, int64_t T, int64_t S, int64_t H, int64_t V);
 int mla_expanded_launch(const kda_mla_expanded_args& a, hipStream_t stream);
 int64_t mla_expanded_bwd_workspace_bytes(int64_t B, int64_t T, int64_t S, int64_t H, int64_t P);
 int mla_expanded_bwd_launch(const kda_mla_expanded_bwd_args& a, hipStream_t stream);

@@ -440,10 +440,15 @@ __global__ __launch_bounds__(256) void join_kernel(kda_mla_absorbed_args a, int 
 
 int row_tiles(int64_t T, int64_t H) { return static_cast<int>((T * H + kRows - 1) / kRows); }
 
-constexpr int64_t kGroups = 512;      // workgroups of the shared form: two a CU
+// Workgroups of the shared form: one a CU in 16 bits, two in 8 bits, where a
+// window has half the bytes and its conversions to hide.  us, 256 / 512: B=64
+// of 2048 tokens 33.1 / 36.7, of 8192 116 / 124, of 64 to 4096 38.3 / 40.0; in 8
+// bits of 128 to 8192 54.6 / 46.1.
+constexpr int64_t kMostGroups = 512;
+constexpr int64_t groups_of(bool f8) { return f8 ? 512 : 256; }
 // Whether the units are shared among the workgroups: where one workgroup a row
 // tile would leave CUs idle or wait for the longest sequence.
-bool shared_form(int64_t nv, int64_t S) { return nv < 4 * kGroups && S > 512; }
+bool shared_form(int64_t nv, int64_t S) { return nv < 1024 && S > 512; }
 
 template <typename T, bool F8, int R, int P>
 int launch(const kda_mla_absorbed_args& a, hipStream_t stream) {
@@ -452,13 +457,14 @@ int launch(const kda_mla_absorbed_args& a, hipStream_t stream) {
     if (!shared_form(nv, a.S)) {
         absorbed_kernel<T, F8, R, P><<<static_cast<unsigned>(nv), kThreads, 0, stream>>>(a, rts, true);
     } else {
-        absorbed_kernel<T, F8, R, P><<<kGroups, kThreads, 0, stream>>>(a, rts, false);
+        constexpr int groups = static_cast<int>(groups_of(F8));
+        absorbed_kernel<T, F8, R, P><<<groups, kThreads, 0, stream>>>(a, rts, false);
         // many rows have few parts each, and few rows may have many
         const dim3 grid(static_cast<unsigned>(nv), kRows);
         if (nv >= 32)
-            join_kernel<T, R / 4><<<grid, 256, 0, stream>>>(a, rts, static_cast<int>(kGroups));
+            join_kernel<T, R / 4><<<grid, 256, 0, stream>>>(a, rts, groups);
         else
-            join_kernel<T, 16><<<dim3(grid.x, grid.y, R / 64), 256, 0, stream>>>(a, rts, static_cast<int>(kGroups));
+            join_kernel<T, 16><<<dim3(grid.x, grid.y, R / 64), 256, 0, stream>>>(a, rts, groups);
     }
     return hipGetLastError() == hipSuccess ? KDA_OK : KDA_ERR_LAUNCH;
 }
@@ -485,7 +491,7 @@ int launch_rank(const kda_mla_absorbed_args& a, hipStream_t stream) {
 int64_t mla_absorbed_workspace_bytes(int64_t B, int64_t T, int64_t H, int64_t S, int64_t R) {
     const int64_t nv = B * row_tiles(T, H);
     if (nv == 0 || !shared_form(nv, S)) return 0;
-    return slots(kGroups, nv) * kRows * (R * 4 + 8) + nv * 8;
+    return slots(kMostGroups, nv) * kRows * (R * 4 + 8) + nv * 8;
 }
 
 int mla_absorbed_launch(const kda_mla_absorbed_args& a, hipStream_t stream) {

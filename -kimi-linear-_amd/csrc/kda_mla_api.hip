@@ -60,10 +60,17 @@ int expanded_check(const kda_mla_expanded_args& a) {
 
 extern "C" {
 
+size_t kda_mla_expanded_workspace_size(int64_t B, int64_t T, int64_t S, int64_t H, int64_t V) {
+    if (!sizes_ok(B, T, S, H) || (V != 64 && V != 128)) return 0;
+    return static_cast<size_t>(kda::mla_expanded_workspace_bytes(B, T, S, H, V));
+}
+
 int kda_mla_expanded_fwd(const kda_mla_expanded_args* a, void* stream) {
     if (a == nullptr) return KDA_ERR_NULL_POINTER;
     if (const int st = expanded_check(*a); st != KDA_OK) return st;
     if (a->B == 0 || a->H == 0 || a->T == 0) return KDA_OK;
+    if (!a->workspace && kda::mla_expanded_workspace_bytes(a->B, a->T, a->S, a->H, a->V) > 0) return KDA_ERR_NULL_POINTER;
+    if (!at16(a->workspace)) return KDA_ERR_UNSUPPORTED;
     return kda::mla_expanded_launch(*a, static_cast<hipStream_t>(stream));
 }
 

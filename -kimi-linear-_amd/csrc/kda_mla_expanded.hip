@@ -16,6 +16,9 @@
 // it does so only when the maximum has grown by more than 2^8 (P stays below
 // 2^8, exact range for both types), the sums are exact either way.
 //
+// Few rows over many keys: several workgroups share the keys of a query tile,
+// each leaves its sums in the workspace, and a second kernel joins them.
+//
 // LDS rows are padded so that sixteen rows' 16-byte pieces (K) and the four
 // rows of a transposed read (V) fall into different banks.
 #include <hip/hip_runtime.h>
@@ -31,14 +34,24 @@ using namespace mla;
 
 constexpr float kLazy = 8.f;          // log2 of how far a maximum may lag
 
+// The workspace of shared keys: every row's parts, [rows][splits][V] sums and
+// their (maximum, denominator).
+struct Parts {
+    float* o;
+    float2* stat;
+    __host__ __device__ Parts(void* p, int64_t rows, int splits, int64_t V)
+        : o(static_cast<float*>(p)), stat(reinterpret_cast<float2*>(o + rows * splits * V)) {}
+};
+
 // A workgroup: RW waves of 32 query rows, times KW waves that share the keys
 // of each: of a step's KW KEYS keys, wave group g takes the g-th KEYS.  BUFS
 // buffers of a step's tiles.
 // Grid: (query tiles, longest first) x (batch, head) with the latter inner, so
 // that a head's tiles share an XCD's L2 where B H is a multiple of eight.
-template <typename T, int N, int P, int RW, int KW, int KEYS, int BUFS>
+// SPLIT: `splits` workgroups a query tile, its steps shared out evenly.
+template <typename T, int N, int P, int RW, int KW, int KEYS, int BUFS, bool SPLIT>
 __global__ __launch_bounds__(64 * RW * KW, RW * KW == 8 ? 2 : 1) void expanded_kernel(kda_mla_expanded_args a,
-                                                                                     int qtiles) {
+                                                                                     int qtiles, int splits) {
     constexpr int kStep = KW * KEYS, kRows = 32 * RW, kU = KEYS / 32;
     using F = KvTile<T, N, P, 64 * RW * KW, kStep, 32>;
     constexpr int D = F::D, V = F::V;
@@ -46,9 +59,10 @@ __global__ __launch_bounds__(64 * RW * KW, RW * KW == 8 ? 2 : 1) void expanded_k
     constexpr int kBytes = BUFS * F::kBuf * 2 > kJoin ? BUFS * F::kBuf * 2 : kJoin;
     __shared__ __align__(16) char raw[kBytes];
     T* smem = reinterpret_cast<T*>(raw);
-    const int64_t bhs = a.B * a.H;
-    const int64_t bh = blockIdx.x % bhs, b = bh / a.H, h = bh - b * a.H;
-    const int t0 = (qtiles - 1 - static_cast<int>(blockIdx.x / bhs)) * kRows;
+    const int64_t bhs = a.B * a.H, unit = SPLIT ? blockIdx.x / splits : blockIdx.x;
+    const int part = SPLIT ? static_cast<int>(blockIdx.x - unit * splits) : 0;
+    const int64_t bh = unit % bhs, b = bh / a.H, h = bh - b * a.H;
+    const int tile_at = qtiles - 1 - static_cast<int>(unit / bhs), t0 = tile_at * kRows;
     const int lane = threadIdx.x & 63, lq = lane & 31, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), row = wave % RW, group = wave / RW;
     const int len = tokens(a.lengths, b, a.S), nq = static_cast<int>(a.T);
@@ -59,7 +73,13 @@ __global__ __launch_bounds__(64 * RW * KW, RW * KW == 8 ? 2 : 1) void expanded_k
     const int limit = live ? start + t : -1;                      // last key this lane's row sees
     const int wlast = w0 < exist ? start + min(w0 + 31, exist - 1) : -1;       // and the last of the wave's
     const int wall = w0 + 32 <= exist ? start + w0 : -1;          // keys up to this one every row sees
-    const int keys = t0 < exist ? start + min(t0 + kRows, exist) : 0;
+    const int seen = t0 < exist ? start + min(t0 + kRows, exist) : 0;           // keys that the tile's rows see
+    int first = 0, keys = seen;                                   // and the workgroup's
+    if constexpr (SPLIT) {
+        const int steps = (seen + kStep - 1) / kStep;
+        first = static_cast<int>(static_cast<int64_t>(part) * steps / splits) * kStep;
+        keys = min(static_cast<int>(static_cast<int64_t>(part + 1) * steps / splits) * kStep, seen);
+    }
     const float c = a.scale * kLog2E;
 
     f16v o[V / 32];
@@ -69,18 +89,18 @@ __global__ __launch_bounds__(64 * RW * KW, RW * KW == 8 ? 2 : 1) void expanded_k
         for (int e = 0; e < 16; ++e) o[i][e] = 0.f;
     float top = kNoMax, sum = 0.f;
 
-    if (keys > 0) {
+    if (keys > first) {
         uint4 q[D / 16];
         const T* qr = static_cast<const T*>(a.q) + b * a.q_stride[0] + min(t, exist - 1) * a.q_stride[1] +
                       h * a.q_stride[2] + 8 * half;
         F tile(a, b, h);
-        tile.fetch(a, 0, keys);
+        tile.fetch(a, first, keys);
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) q[k] = *reinterpret_cast<const uint4*>(qr + 16 * k);
         tile.put(smem);
         __syncthreads();
         int cur = 0;
-        for (int j0 = 0; j0 < keys; j0 += kStep) {
+        for (int j0 = first; j0 < keys; j0 += kStep) {
             tile.fetch(a, j0 + kStep, keys);
             const T* buf = smem + cur * F::kBuf;
             const int jw = j0 + KEYS * group;                     // the wave's first key
@@ -187,6 +207,20 @@ __global__ __launch_bounds__(64 * RW * KW, RW * KW == 8 ? 2 : 1) void expanded_k
     }
     if (group != 0 || t >= nq) return;
     sum = half_sum(sum);
+    if constexpr (SPLIT) {
+        const Parts parts(a.workspace, bhs * a.T, splits, V);
+        const int64_t at = (bh * a.T + t) * splits + part;
+        if (half == 0) parts.stat[at] = float2{top, sum};
+        if (sum != 0.f) {            // (or not a number); a part without keys is not read
+#pragma unroll
+            for (int i = 0; i < V / 32; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    *reinterpret_cast<f4*>(parts.o + at * V + 32 * i + 8 * e + 4 * half) =
+                        f4{o[i][4 * e], o[i][4 * e + 1], o[i][4 * e + 2], o[i][4 * e + 3]};
+        }
+        return;
+    }
     const float norm = sum == 0.f ? 0.f : 1.f / sum;
     T* out = static_cast<T*>(a.o) + ((b * a.T + t) * a.H + h) * V + 4 * half;
 #pragma unroll
@@ -200,11 +234,53 @@ __global__ __launch_bounds__(64 * RW * KW, RW * KW == 8 ? 2 : 1) void expanded_k
         a.lse[(b * a.H + h) * a.T + t] = sum == 0.f ? INFINITY : top + __builtin_amdgcn_logf(sum);
 }
 
-template <typename T, int N, int P, int RW, int KW, int KEYS, int BUFS>
-int launch_as(const kda_mla_expanded_args& a, hipStream_t stream) {
+// The parts of a row joined in order: V / 4 lanes a row.
+template <typename T, int V>
+__global__ __launch_bounds__(256) void join_kernel(kda_mla_expanded_args a, int splits) {
+    constexpr int kLanes = V / 4;
+    const int64_t rows = a.B * a.H * a.T, row = static_cast<int64_t>(blockIdx.x) * (256 / kLanes) + threadIdx.x / kLanes;
+    if (row >= rows) return;
+    const int ch = 4 * (threadIdx.x % kLanes);
+    const Parts parts(a.workspace, rows, splits, V);
+    const float2* stat = parts.stat + row * splits;
+    const float* from = parts.o + row * splits * V + ch;
+    float top = kNoMax, sum = 0.f;
+    for (int i = 0; i < splits; ++i) top = fmaxf(top, stat[i].x);
+    f4 r{};
+    for (int i = 0; i < splits; ++i) {
+        const float2 x = stat[i];
+        if (x.y == 0.f) continue;
+        const float w = __builtin_amdgcn_exp2f(x.x - top);
+        const f4 y = *reinterpret_cast<const f4*>(from + static_cast<int64_t>(i) * V);
+        sum = fmaf(w, x.y, sum);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) r[e] = fmaf(w, y[e], r[e]);
+    }
+    const float norm = sum == 0.f ? 0.f : 1.f / sum;
+    const int64_t bh = row / a.T, t = row - bh * a.T, b = bh / a.H, h = bh - b * a.H;
+    *reinterpret_cast<uint2*>(static_cast<T*>(a.o) + ((b * a.T + t) * a.H + h) * V + ch) =
+        uint2{Act<T>::pair(r[0] * norm, r[1] * norm), Act<T>::pair(r[2] * norm, r[3] * norm)};
+    if (a.lse && ch == 0) a.lse[row] = sum == 0.f ? INFINITY : top + __builtin_amdgcn_logf(sum);
+}
+
+// Workgroups that share the keys of a query tile of 64 rows: where there are too
+// few tiles for the CUs, as many as fill them with at least 512 keys each.
+int splits_of(int64_t B, int64_t T, int64_t S, int64_t H) {
+    const int64_t tiles = B * H * ((T + 63) / 64);
+    if (tiles == 0 || tiles > 128 || S < 1024) return 1;
+    const int64_t most = S / 512, fill = 256 / tiles;
+    return static_cast<int>(most < fill ? most : fill);
+}
+
+template <typename T, int N, int P, int RW, int KW, int KEYS, int BUFS, bool SPLIT = false>
+int launch_as(const kda_mla_expanded_args& a, hipStream_t stream, int splits = 1) {
     const int64_t qtiles = (a.T + 32 * RW - 1) / (32 * RW);
-    expanded_kernel<T, N, P, RW, KW, KEYS, BUFS><<<static_cast<unsigned>(qtiles * a.B * a.H), 64 * RW * KW, 0, stream>>>(
-        a, static_cast<int>(qtiles));
+    expanded_kernel<T, N, P, RW, KW, KEYS, BUFS, SPLIT>
+        <<<static_cast<unsigned>(qtiles * a.B * a.H * splits), 64 * RW * KW, 0, stream>>>(a, static_cast<int>(qtiles), splits);
+    if constexpr (SPLIT) {
+        constexpr int rows = 256 / (N / 4);
+        join_kernel<T, N><<<static_cast<unsigned>((a.B * a.H * a.T + rows - 1) / rows), 256, 0, stream>>>(a, splits);
+    }
     return hipGetLastError() == hipSuccess ? KDA_OK : KDA_ERR_LAUNCH;
 }
 
@@ -213,6 +289,8 @@ int launch(const kda_mla_expanded_args& a, hipStream_t stream) {
     // eight waves a workgroup, as many of them on rows of their own as leave every CU a workgroup
     if (a.B * a.H * ((a.T + 255) / 256) >= 256) return launch_as<T, N, P, 8, 1, 64, 2>(a, stream);
     if (a.B * a.H * ((a.T + 127) / 128) >= 256) return launch_as<T, N, P, 4, 2, 32, 2>(a, stream);
+    const int splits = splits_of(a.B, a.T, a.S, a.H);
+    if (splits > 1) return launch_as<T, N, P, 2, 4, 32, 1, true>(a, stream, splits);
     return launch_as<T, N, P, 2, 4, 32, 1>(a, stream);
 }
 
@@ -228,6 +306,11 @@ int launch_dims(const kda_mla_expanded_args& a, hipStream_t stream) {
 }
 
 }  // namespace
+
+int64_t mla_expanded_workspace_bytes(int64_t B, int64_t T, int64_t S, int64_t H, int64_t V) {
+    const int splits = splits_of(B, T, S, H);
+    return splits > 1 ? B * H * T * splits * (V * 4 + 8) : 0;
+}
 
 int mla_expanded_launch(const kda_mla_expanded_args& a, hipStream_t stream) {
     return a.dtype == KDA_DTYPE_F16 ? launch_dims<_Float16>(a, stream) : launch_dims<bf16_t>(a, stream);

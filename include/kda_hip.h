@@ -522,8 +522,10 @@ typedef struct kda_mla_expanded_args {
                                     * what the backward needs */
     float scale;
     int32_t dtype;                 /* KDA_DTYPE_F16 or KDA_DTYPE_BF16, of all activations */
+    void* workspace;               /* forward: kda_mla_expanded_workspace_size() bytes (0 for most shapes) */
 } kda_mla_expanded_args;
 
+size_t kda_mla_expanded_workspace_size(int64_t B, int64_t T, int64_t S, int64_t H, int64_t V);
 int kda_mla_expanded_fwd(const kda_mla_expanded_args* args, void* stream);
 
 /* Its gradients, from d_o and the forward's arguments, o and lse.  Every sum

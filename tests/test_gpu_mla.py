@@ -150,6 +150,9 @@ EXPANDED = [
     (1, 129, 257, 5, 128, 32, BF16, None, [100]),                # queries end before the keys do
     (2, 40, 16, 2, 64, 64, F16, None, None),                     # more queries than keys: the first see none
     (1, 600, 600, 16, 128, 64, BF16, None, None),
+    (1, 1, 5000, 2, 128, 64, BF16, None, None),                  # few rows over many keys: shared among workgroups
+    (2, 70, 2100, 3, 64, 32, F16, [2100, 40], [2030, 0]),
+    (3, 9, 1300, 2, 128, 0, BF16, [0, 600, 1300], [0, 591, 1291]),
     (4, 700, 700, 24, 64, 32, F16, None, None),                  # enough rows for the widest workgroups
 ]
 

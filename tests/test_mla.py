@@ -75,6 +75,9 @@ def test_expanded_codes(native):
     assert rc(q=None) == 1 and rc(k=None) == 1 and rc(k_pe=None) == 1 and rc(v=None) == 1 and rc(o=None) == 1
     assert rc(q=FAKE + 2) == 4 and rc(k_stride=(0, 4, 0)) == 4 and rc(v_stride=(0, -8, 0)) == 4
     assert rc(B=0) == 0 and rc(H=0) == 0 and rc(T=0) == 0
+    size = native.load().kda_mla_expanded_workspace_size
+    assert size(1, 8, 8, 2, 64) == 0 and size(4, 2048, 2048, 16, 128) == 0 and size(1, 8, 4096, 2, 100) == 0
+    assert size(1, 8, 4096, 2, 64) > 0 and rc(S=4096) == 1 and rc(S=4096, workspace=FAKE + 4) == 4
 
 
 def test_expanded_bwd_codes(native):
