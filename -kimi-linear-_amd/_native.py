@@ -156,7 +156,7 @@ class KdaMlaExpandedArgs(ctypes.Structure):
         ("q", ctypes.c_void_p), ("q_stride", _i64x3), ("k", ctypes.c_void_p), ("k_stride", _i64x3),
         ("k_pe", ctypes.c_void_p), ("k_pe_stride", ctypes.c_int64 * 2), ("v", ctypes.c_void_p), ("v_stride", _i64x3),
         ("lengths", ctypes.c_void_p), ("starts", ctypes.c_void_p),
-        ("o", ctypes.c_void_p), ("lse", ctypes.c_void_p), ("scale", ctypes.c_float), ("dtype", ctypes.c_int32),
+        ("o", ctypes.c_void_p), ("lse", ctypes.c_void_p), ("o_low", ctypes.c_void_p), ("scale", ctypes.c_float), ("dtype", ctypes.c_int32),
         ("workspace", ctypes.c_void_p),
     ]
 

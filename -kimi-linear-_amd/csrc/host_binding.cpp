@@ -585,7 +585,7 @@ bool expanded_ok(const Plain& plain, const Tensor& q, const Tensor& k, const Opt
 
 kda_mla_expanded_args expanded_args(const Tensor& q, const Tensor& k, const OptTensor& k_pe, const Tensor& v,
                                     const OptTensor& lengths, const OptTensor& starts, double scale, const Tensor& o,
-                                    const OptTensor& lse) {
+                                    const Tensor* lse, const Tensor* low) {
     kda_mla_expanded_args a{};
     a.B = q.size(0); a.T = q.size(1); a.S = k.size(1); a.H = q.size(2);
     a.N = k.size(3); a.P = q.size(3) - a.N; a.V = v.size(3);
@@ -601,6 +601,7 @@ kda_mla_expanded_args expanded_args(const Tensor& q, const Tensor& k, const OptT
     a.starts = counts_ptr(starts);
     a.o = o.data_ptr();
     a.lse = lse ? static_cast<float*>(lse->data_ptr()) : nullptr;
+    a.o_low = low ? low->data_ptr() : nullptr;
     a.scale = static_cast<float>(scale);
     a.dtype = code(q);
     return a;
@@ -608,12 +609,13 @@ kda_mla_expanded_args expanded_args(const Tensor& q, const Tensor& k, const OptT
 
 // The forward, with its lse if wanted: whether the library took it.
 bool expanded_forward(const Tensor& q, const Tensor& k, const OptTensor& k_pe, const Tensor& v, const OptTensor& lengths,
-                      const OptTensor& starts, double scale, Tensor& o, OptTensor* lse) {
+                      const OptTensor& starts, double scale, Tensor& o, Tensor* lse = nullptr, Tensor* low = nullptr) {
     const int status = run(q.device(), [&](void* stream) -> int {
         const auto opt = q.options().requires_grad(false);
         o = at::empty({q.size(0), q.size(1), q.size(2), v.size(3)}, opt);
         if (lse) *lse = at::empty({q.size(0), q.size(2), q.size(1)}, opt.dtype(at::kFloat));
-        auto a = expanded_args(q, k, k_pe, v, lengths, starts, scale, o, lse ? *lse : OptTensor());
+        if (low) *low = at::empty(o.sizes(), opt);
+        auto a = expanded_args(q, k, k_pe, v, lengths, starts, scale, o, lse, low);
         const size_t bytes = fn.mla_expanded_ws(a.B, a.T, a.S, a.H, a.V);
         Tensor ws;
         if (bytes > 0) {
@@ -633,10 +635,9 @@ Tensor or_none(const OptTensor& t) { return t ? *t : Tensor(); }
 struct ExpandedFn : torch::autograd::Function<ExpandedFn> {
     static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& q, const Tensor& k, const OptTensor& k_pe,
                           const Tensor& v, const OptTensor& lengths, const OptTensor& starts, double scale) {
-        Tensor o;
-        OptTensor lse;
-        if (!expanded_forward(q, k, k_pe, v, lengths, starts, scale, o, &lse)) return Tensor();
-        ctx->save_for_backward({q, k, or_none(k_pe), v, or_none(lengths), or_none(starts), o, *lse});
+        Tensor o, lse, low;
+        if (!expanded_forward(q, k, k_pe, v, lengths, starts, scale, o, &lse, &low)) return Tensor();
+        ctx->save_for_backward({q, k, or_none(k_pe), v, or_none(lengths), or_none(starts), o, lse, low});
         ctx->saved_data["scale"] = scale;
         return o;
     }
@@ -662,7 +663,7 @@ struct ExpandedFn : torch::autograd::Function<ExpandedFn> {
                 if (k_pe.defined()) dpe = at::empty(k_pe.sizes(), opt);
                 kda_mla_expanded_bwd_args g{};
                 g.fwd = expanded_args(q, k, maybe(k_pe), v, maybe(s[4]), maybe(s[5]), ctx->saved_data["scale"].toDouble(),
-                                      o, lse);
+                                      o, &lse, &s[8]);
                 const size_t bytes = fn.mla_expanded_bwd_ws(g.fwd.B, g.fwd.T, g.fwd.S, g.fwd.H, g.fwd.P);
                 const Tensor ws = at::empty({static_cast<int64_t>(bytes)}, opt.dtype(at::kByte));
                 g.d_o = d_o.data_ptr();
@@ -710,7 +711,7 @@ py::object mla_expanded(const Tensor& q, const Tensor& k, const OptTensor& k_pe,
         grad = q.requires_grad() || k.requires_grad() || v.requires_grad() || (k_pe && k_pe->requires_grad());
     Tensor o;
     if (grad) o = ExpandedFn::apply(q, k, k_pe, v, lengths, starts, scale);
-    else if (!expanded_forward(q, k, k_pe, v, lengths, starts, scale, o, nullptr)) return py::none();
+    else if (!expanded_forward(q, k, k_pe, v, lengths, starts, scale, o)) return py::none();
     return o.defined() ? py::cast(o) : py::object(py::none());
 }
 

@@ -74,6 +74,19 @@ __device__ __forceinline__ uint2 read_tr(const void* p) {
                                          (lds_s4)(reinterpret_cast<const s4*>(p))));
 }
 
+// Four neighbouring outputs, and where `low` is there what rounding took from each.
+template <typename T>
+__device__ __forceinline__ void store_out(T* out, T* low, f4 x) {
+    const uint2 r{Act<T>::pair(x[0], x[1]), Act<T>::pair(x[2], x[3])};
+    *reinterpret_cast<uint2*>(out) = r;
+    if (low) {
+        T e[4];
+        __builtin_memcpy(e, &r, 8);
+        *reinterpret_cast<uint2*>(low) = uint2{Act<T>::pair(x[0] - Elem<T>::ld(&e[0]), x[1] - Elem<T>::ld(&e[1])),
+                                               Act<T>::pair(x[2] - Elem<T>::ld(&e[2]), x[3] - Elem<T>::ld(&e[3]))};
+    }
+}
+
 // Largest x over the four lanes that share l & 15.
 __device__ __forceinline__ float lanegroup4_max(float x) {
     {

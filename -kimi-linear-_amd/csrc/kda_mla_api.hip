@@ -51,7 +51,7 @@ int expanded_check(const kda_mla_expanded_args& a) {
     if (a.S > 0 && (!a.k || !a.v || (a.P > 0 && !a.k_pe))) return KDA_ERR_NULL_POINTER;
     if (!rows_ok(a.q, a.q_stride, 3, 2) || !rows_ok(a.k, a.k_stride, 3, 2) || !rows_ok(a.v, a.v_stride, 3, 2) ||
         (a.P > 0 && !rows_ok(a.k_pe, a.k_pe_stride, 2, 2)) || !at16(a.o) ||
-        !near(a.q_stride[1]) || !near(a.k_stride[1]) || !near(a.v_stride[1]) || (a.P > 0 && !near(a.k_pe_stride[1])))
+        !at16(a.o_low) || !near(a.q_stride[1]) || !near(a.k_stride[1]) || !near(a.v_stride[1]) || (a.P > 0 && !near(a.k_pe_stride[1])))
         return KDA_ERR_UNSUPPORTED;
     return KDA_OK;
 }
@@ -84,7 +84,7 @@ int kda_mla_expanded_bwd(const kda_mla_expanded_bwd_args* g, void* stream) {
     const kda_mla_expanded_args& a = g->fwd;
     if (const int st = expanded_check(a); st != KDA_OK) return st;
     if (a.B == 0 || a.H == 0) return KDA_OK;
-    if (a.T > 0 && (!a.lse || !g->d_o || !g->dq)) return KDA_ERR_NULL_POINTER;
+    if (a.T > 0 && (!a.lse || !a.o_low || !g->d_o || !g->dq)) return KDA_ERR_NULL_POINTER;
     if (a.S > 0 && (!g->dk || !g->dv || (a.P > 0 && !g->dk_pe))) return KDA_ERR_NULL_POINTER;
     if (!g->workspace && kda::mla_expanded_bwd_workspace_bytes(a.B, a.T, a.S, a.H, a.P) > 0) return KDA_ERR_NULL_POINTER;
     if (!rows_ok(g->d_o, g->d_o_stride, 3, 2) || !near(g->d_o_stride[1]) || !at16(g->dq) || !at16(g->dk) || !at16(g->dk_pe) || !at16(g->dv) ||
@@ -121,7 +121,7 @@ int kda_mla_absorbed_fwd(const kda_mla_absorbed_args* a, void* stream) {
 
 int kda_mla_cache_append(const kda_mla_append_args* a, void* stream) {
     if (a == nullptr) return KDA_ERR_NULL_POINTER;
-    if (!sizes_ok(a->B, a->T, a->S, 1) || a->B * (a->T / 4 + 1) > kMaxGrid) return KDA_ERR_BAD_SHAPE;
+    if (!sizes_ok(a->B, a->T, a->S, 1) || (a->T > 0 && a->B > kMaxGrid / a->T)) return KDA_ERR_BAD_SHAPE;
     if (!act(a->x_dtype) || (a->cache_dtype != a->x_dtype && a->cache_dtype != KDA_DTYPE_E4M3)) return KDA_ERR_BAD_DTYPE;
     if ((a->R != 128 && a->R != 256 && a->R != 512) || !pos_ok(a->P)) return KDA_ERR_UNSUPPORTED;
     if (a->B == 0 || a->T == 0 || a->S == 0) return KDA_OK;

@@ -222,14 +222,15 @@ __global__ __launch_bounds__(64 * RW * KW, RW * KW == 8 ? 2 : 1) void expanded_k
         return;
     }
     const float norm = sum == 0.f ? 0.f : 1.f / sum;
-    T* out = static_cast<T*>(a.o) + ((b * a.T + t) * a.H + h) * V + 4 * half;
+    const int64_t to = ((b * a.T + t) * a.H + h) * V + 4 * half;
+    T* out = static_cast<T*>(a.o) + to;
+    T* low = a.o_low ? static_cast<T*>(a.o_low) + to : nullptr;
 #pragma unroll
     for (int i = 0; i < V / 32; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-            *reinterpret_cast<uint2*>(out + 32 * i + 8 * e) =
-                uint2{Act<T>::pair(o[i][4 * e] * norm, o[i][4 * e + 1] * norm),
-                      Act<T>::pair(o[i][4 * e + 2] * norm, o[i][4 * e + 3] * norm)};
+            store_out(out + 32 * i + 8 * e, low ? low + 32 * i + 8 * e : nullptr,
+                      f4{o[i][4 * e] * norm, o[i][4 * e + 1] * norm, o[i][4 * e + 2] * norm, o[i][4 * e + 3] * norm});
     if (a.lse && half == 0)
         a.lse[(b * a.H + h) * a.T + t] = sum == 0.f ? INFINITY : top + __builtin_amdgcn_logf(sum);
 }
@@ -258,17 +259,20 @@ __global__ __launch_bounds__(256) void join_kernel(kda_mla_expanded_args a, int 
     }
     const float norm = sum == 0.f ? 0.f : 1.f / sum;
     const int64_t bh = row / a.T, t = row - bh * a.T, b = bh / a.H, h = bh - b * a.H;
-    *reinterpret_cast<uint2*>(static_cast<T*>(a.o) + ((b * a.T + t) * a.H + h) * V + ch) =
-        uint2{Act<T>::pair(r[0] * norm, r[1] * norm), Act<T>::pair(r[2] * norm, r[3] * norm)};
+    const int64_t to = ((b * a.T + t) * a.H + h) * V + ch;
+    store_out(static_cast<T*>(a.o) + to, a.o_low ? static_cast<T*>(a.o_low) + to : nullptr,
+              f4{r[0] * norm, r[1] * norm, r[2] * norm, r[3] * norm});
     if (a.lse && ch == 0) a.lse[row] = sum == 0.f ? INFINITY : top + __builtin_amdgcn_logf(sum);
 }
 
 // Workgroups that share the keys of a query tile of 64 rows: where there are too
-// few tiles for the CUs, as many as fill them with at least 512 keys each.
+// few tiles for the CUs, as many as fill them with at least 512 keys each, or 256
+// in up to four.  us at T=64 H=16, parts of 512 / 256: S=1024 17.4 / 15.9, S=4096
+// 23.5 / 27.1.
 int splits_of(int64_t B, int64_t T, int64_t S, int64_t H) {
     const int64_t tiles = B * H * ((T + 63) / 64);
     if (tiles == 0 || tiles > 128 || S < 1024) return 1;
-    const int64_t most = S / 512, fill = 256 / tiles;
+    const int64_t most = S >= 2048 ? S / 512 : S / 256, fill = 256 / tiles;
     return static_cast<int>(most < fill ? most : fill);
 }
 
@@ -286,9 +290,13 @@ int launch_as(const kda_mla_expanded_args& a, hipStream_t stream, int splits = 1
 
 template <typename T, int N, int P>
 int launch(const kda_mla_expanded_args& a, hipStream_t stream) {
-    // eight waves a workgroup, as many of them on rows of their own as leave every CU a workgroup
-    if (a.B * a.H * ((a.T + 255) / 256) >= 256) return launch_as<T, N, P, 8, 1, 64, 2>(a, stream);
-    if (a.B * a.H * ((a.T + 127) / 128) >= 256) return launch_as<T, N, P, 4, 2, 32, 2>(a, stream);
+    // Eight waves a workgroup, as many of them on rows of their own as leave every
+    // CU a workgroup, or two where the tiles differ (few keys before the first
+    // query), so that long and short ones share a CU.  us, 256 / 128 rows: B=1
+    // T=4096 H=16 132 / 105; 128 / 64 rows: T=2048 46.5 / 45.1.
+    const int64_t heads = a.B * a.H, least = a.S >= 2 * a.T ? 256 : 512;
+    if (heads * ((a.T + 255) / 256) >= least) return launch_as<T, N, P, 8, 1, 64, 2>(a, stream);
+    if (heads * ((a.T + 127) / 128) >= least) return launch_as<T, N, P, 4, 2, 32, 2>(a, stream);
     const int splits = splits_of(a.B, a.T, a.S, a.H);
     if (splits > 1) return launch_as<T, N, P, 2, 4, 32, 1, true>(a, stream, splits);
     return launch_as<T, N, P, 2, 4, 32, 1>(a, stream);

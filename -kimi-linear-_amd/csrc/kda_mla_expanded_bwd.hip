@@ -108,7 +108,11 @@ __global__ __launch_bounds__(64 * WAVES, 2) void dq_kernel(kda_mla_expanded_bwd_
                       8 * half;
         const T* dor = static_cast<const T*>(g.d_o) + at.b * g.d_o_stride[0] + tc * g.d_o_stride[1] +
                        at.h * g.d_o_stride[2] + 8 * half;
-        const T* orow = static_cast<const T*>(a.o) + ((at.b * a.T + tc) * a.H + at.h) * V + 8 * half;
+        // delta from o as it was before rounding: its rounding is one value for the row and would
+        // move every ds of it (fp16, T=203: dq off by 3.2e-4 with it, 3.0e-4 without)
+        const int64_t from = ((at.b * a.T + tc) * a.H + at.h) * V + 8 * half;
+        const T* orow = static_cast<const T*>(a.o) + from;
+        const T* lrow = static_cast<const T*>(a.o_low) + from;
         uint4 q[D / 16], d_o[V / 16];
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) q[k] = *reinterpret_cast<const uint4*>(qr + 16 * k);
@@ -117,6 +121,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void dq_kernel(kda_mla_expanded_bwd_
         for (int k = 0; k < V / 16; ++k) {
             d_o[k] = *reinterpret_cast<const uint4*>(dor + 16 * k);
             dl = dot8(d_o[k], *reinterpret_cast<const uint4*>(orow + 16 * k), dl, T{});
+            dl = dot8(d_o[k], *reinterpret_cast<const uint4*>(lrow + 16 * k), dl, T{});
         }
         dl = half_sum(dl);
         if (live && half == 0) delta[bh * a.T + t] = dl;

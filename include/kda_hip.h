@@ -518,8 +518,9 @@ typedef struct kda_mla_expanded_args {
     const int32_t* lengths;        /* [B] or NULL */
     const int32_t* starts;         /* [B], >= 0, or NULL */
     void* o;                       /* [B, T, H, V] contiguous */
-    float* lse;                    /* [B, H, T] or NULL: log2 of the row's sum of exp(s), +inf for a row without keys;
-                                    * what the backward needs */
+    float* lse;                    /* [B, H, T] or NULL: log2 of the row's sum of exp(s), +inf for a row without keys */
+    void* o_low;                   /* [B, T, H, V] contiguous, or NULL: what rounding took from o, rounded itself;
+                                    * the backward needs both of these */
     float scale;
     int32_t dtype;                 /* KDA_DTYPE_F16 or KDA_DTYPE_BF16, of all activations */
     void* workspace;               /* forward: kda_mla_expanded_workspace_size() bytes (0 for most shapes) */
@@ -528,11 +529,11 @@ typedef struct kda_mla_expanded_args {
 size_t kda_mla_expanded_workspace_size(int64_t B, int64_t T, int64_t S, int64_t H, int64_t V);
 int kda_mla_expanded_fwd(const kda_mla_expanded_args* args, void* stream);
 
-/* Its gradients, from d_o and the forward's arguments, o and lse.  Every sum
+/* Its gradients, from d_o and the forward's arguments, o, lse and o_low.  Every sum
  * in fp32 in a fixed order (the position part's over the heads too), rounded
  * once to the activation type.  d_o of queries that do not exist is not read. */
 typedef struct kda_mla_expanded_bwd_args {
-    kda_mla_expanded_args fwd;     /* o and lse as kda_mla_expanded_fwd left them */
+    kda_mla_expanded_args fwd;     /* o, lse and o_low as kda_mla_expanded_fwd left them */
     const void* d_o;               /* [B, T, H, V] */
     int64_t d_o_stride[3];
     void* dq;                      /* [B, T, H, N+P] contiguous */

@@ -85,13 +85,13 @@ def test_expanded_bwd_codes(native):
 
     def rc(fwd=None, **kw):
         g = native.KdaMlaExpandedBwdArgs()
-        g.fwd = expanded(native, **{"lse": FAKE, **(fwd or {})})
+        g.fwd = expanded(native, **{"lse": FAKE, "o_low": FAKE, **(fwd or {})})
         for f in ("d_o", "dq", "dk", "dk_pe", "dv", "workspace"):
             setattr(g, f, FAKE)
         return lib.kda_mla_expanded_bwd(ctypes.byref(fill(g, kw)), None)
 
     assert lib.kda_mla_expanded_bwd(None, None) == 1
-    assert rc(fwd={"N": 96}) == 4 and rc(fwd={"lse": None}) == 1
+    assert rc(fwd={"N": 96}) == 4 and rc(fwd={"lse": None}) == 1 and rc(fwd={"o_low": None}) == 1
     for name in ("d_o", "dq", "dk", "dk_pe", "dv", "workspace"):
         assert rc(**{name: None}) == 1, name
         assert rc(**{name: FAKE + 8}) == 4, name
