@@ -31,6 +31,8 @@
 // denominator are divided by the scale again.
 #include <hip/hip_runtime.h>
 
+#include <type_traits>
+
 #include "kda_launch.h"
 #include "kda_mla.h"
 
@@ -59,6 +61,243 @@ __host__ __device__ inline Workspace carve(void* p, int64_t n_slots, int64_t R) 
     w.span = reinterpret_cast<int2*>(w.ml + n_slots * kRows);
     return w;
 }
+
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));      // (arrays of uint4 may stay in scratch memory)
+
+// Query rows m0.. as (token, head): row m0 + r, past the last repeating it.
+struct Queries {
+    int H, t0, h0, last;
+    float inv;
+    __device__ __forceinline__ Queries(const kda_mla_absorbed_args& a, int m0) {
+        H = static_cast<int>(a.H);
+        t0 = m0 / H;
+        h0 = m0 - t0 * H;
+        last = static_cast<int>(a.T) * H - 1 - m0;
+        inv = __builtin_amdgcn_rcpf(static_cast<float>(H));
+    }
+    // h0 + r < H + 16: with 16 heads or more it passes H once at most, with
+    // fewer it is below 32, which the reciprocal divides exactly
+    __device__ __forceinline__ int token(int r) const {
+        const int x = h0 + min(r, last);
+        return t0 + (H >= kRows ? (x >= H ? 1 : 0) : static_cast<int>((static_cast<float>(x) + 0.5f) * inv));
+    }
+    __device__ __forceinline__ int head(int r, int t) const { return h0 + min(r, last) - (t - t0) * H; }
+};
+
+// 16 bits.  Rows go straight to LDS, asynchronously: two buffers, the next
+// window's rows under way while this one is worked on, none in registers.  LDS
+// rows have no padding (a load fills 1 KB on end); instead the 16-byte piece c of
+// row r lies at c ^ turn(r), low four bits, which puts sixteen rows' pieces (the
+// score product's reads) and four rows' neighbouring two (the value product's)
+// into different banks.
+// Reads issued before this stay before it.
+__device__ __forceinline__ void stay() { asm volatile("" ::: "memory"); }
+// A barrier for what the waves leave each other in LDS, that does not wait for loads under way as __syncthreads does.
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+__device__ __forceinline__ int turn(int r) { return ((r << 1) & 14) | ((r >> 3) & 1); }
+
+template <typename T, int R, int P>
+struct Kernel16 {
+    static constexpr int D = R + P, kWindow = kUnit * WAVES, kSteps = D / 32, kScore = kWindow + 4;
+    static constexpr int kTiles = R / 16 / WAVES;
+    static constexpr int kBuffer = kWindow * D;                 // elements: [kWindow][R] latent, [kWindow][P] position
+    static constexpr int kLatRows = 512 / R, kLat = kUnit / kLatRows;            // rows a load, loads a unit
+    static constexpr int kPosRows = P == 0 ? kUnit : 512 / P, kPos = P == 0 ? 0 : kUnit / kPosRows;
+    static_assert(kBuffer >= kRows * (D + 8), "the queries pass through a buffer");
+
+    // Where piece c of row r's position part lies: 16 rows' pieces in different banks.
+    static __device__ __forceinline__ int pos_piece(int r, int c) { return c ^ (P == 64 ? (r >> 1) & 7 : (r >> 2) & 3); }
+
+    // 64 lanes' 16 bytes each, from base + offset, on end to LDS; waited for by the
+    // reader (landed() below).  In assembly for the compiler not to wait: it takes
+    // a transposed LDS read for one that may be of any load's place.
+    static __device__ __forceinline__ void to_lds(const T* base, int offset, T* lds) {
+        const uint32_t at = static_cast<uint32_t>(
+            reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) void*)(lds)));
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+                     :
+                     : "s"(at), "v"(2 * offset), "s"(base)
+                     : "memory");          // (m0 is reserved: the compiler keeps nothing in it)
+    }
+    // This wave's loads into LDS are there.
+    static __device__ __forceinline__ void landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+    // A unit's rows, keys j.. of which those past hi - 1 repeat it, into their place in a buffer.
+    static __device__ __forceinline__ void load(const kda_mla_absorbed_args& a, int64_t b, int j, int hi, int wave, int lane,
+                                                T* buf) {
+        const int base = min(j, hi - 1), last = hi - 1 - base, stride = static_cast<int>(a.cache_stride[1]);
+        const T* rows = static_cast<const T*>(a.cache) + b * a.cache_stride[0] + base * a.cache_stride[1];
+        constexpr int per = R / 8;                               // pieces of a row, lanes of a row
+        const int x = lane / per, c = lane % per;
+#pragma unroll
+        for (int i = 0; i < kLat; ++i)
+            to_lds(rows, min(kLatRows * i + x, last) * stride + 8 * (c ^ turn(kLatRows * i) ^ (x << 1)),
+                   buf + (kUnit * wave + kLatRows * i) * R);
+        if constexpr (P > 0) {
+            constexpr int pp = P / 8;
+            T* pos = buf + kWindow * R + kUnit * wave * P;
+#pragma unroll
+            for (int i = 0; i < kPos; ++i) {
+                const int r = kPosRows * i + lane / pp;
+                to_lds(rows, min(r, last) * stride + R + 8 * pos_piece(r, lane % pp), pos + kPosRows * i * P);
+            }
+        }
+    }
+
+    // A window at keys j0..; its rows are in `buf`, the next window's are asked for into `next`.
+    struct State {
+        uint4 q[kSteps];
+        f4 o[kTiles];
+        float top, sum;
+    };
+    static __device__ __forceinline__ void window(const kda_mla_absorbed_args& a, int64_t b, int j0, int hi, int limit,
+                                                  float c, int wave, int lane, const T* buf, T* next,
+                                                  float (*sh)[kScore], State& st) {
+        const int ln = lane & 15, lg = lane >> 4;
+        if (j0 + kWindow < hi) load(a, b, j0 + kWindow + kUnit * wave, hi, wave, lane, next);
+        // scores of the wave's unit: keys 4 lg + i of row ln, in two chains
+        f4 acc{}, odd{};
+        const T* row = buf + (kUnit * wave + ln) * R;
+        const int f = turn(ln);
+        const T* pos = buf + kWindow * R + (kUnit * wave + ln) * P;
+        u4 piece[kSteps];                // all asked for before the first product: nothing else hides their latency
+#pragma unroll
+        for (int k = 0; k < R / 32; ++k)
+            piece[k] = *reinterpret_cast<const u4*>(row + 128 * (k / 4) + 8 * ((4 * (k % 4) + lg) ^ f));
+#pragma unroll
+        for (int k = 0; k < P / 32; ++k)
+            piece[R / 32 + k] = *reinterpret_cast<const u4*>(pos + 8 * pos_piece(ln, 4 * k + lg));
+        stay();
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k) {
+            const uint4 x = __builtin_bit_cast(uint4, piece[k]);
+            if (k % 2 == 0) acc = Act<T>::mma16(x, st.q[k], acc);
+            else odd = Act<T>::mma16(x, st.q[k], odd);
+        }
+        const int key = j0 + kUnit * wave + 4 * lg;
+        f4 s;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[i] = key + i > limit ? -INFINITY : (acc[i] + odd[i]) * c;
+        *reinterpret_cast<f4*>(&sh[ln][kUnit * wave + 4 * lg]) = s;
+        lds_barrier();
+
+        uint4 p[kWindow / 32];
+        float x[kWindow / 32][8], mx = st.top;
+#pragma unroll
+        for (int k = 0; k < kWindow / 32; ++k) {
+            const f4* from = reinterpret_cast<const f4*>(&sh[ln][32 * k + 8 * lg]);
+            const f4 lo4 = from[0], hi4 = from[1];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                x[k][e] = lo4[e];
+                x[k][4 + e] = hi4[e];
+                mx = fmaxf(mx, fmaxf(lo4[e], hi4[e]));
+            }
+        }
+        mx = lanegroup4_max(mx);
+        const float alpha = __builtin_amdgcn_exp2f(st.top - mx);
+        st.top = mx;
+        float part = 0.f;
+#pragma unroll
+        for (int k = 0; k < kWindow / 32; ++k) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                x[k][e] = __builtin_amdgcn_exp2f(x[k][e] - mx);
+                part += x[k][e];
+            }
+            p[k] = uint4{Act<T>::pair(x[k][0], x[k][1]), Act<T>::pair(x[k][2], x[k][3]), Act<T>::pair(x[k][4], x[k][5]),
+                         Act<T>::pair(x[k][6], x[k][7])};
+        }
+        st.sum = fmaf(st.sum, alpha, part);
+#pragma unroll
+        for (int i = 0; i < kTiles; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) st.o[i][e] *= alpha;
+        const int r = 8 * lg + (ln >> 2), f0 = turn(r & 15), f1 = turn((r + 4) & 15);
+        constexpr int kAtOnce = kTiles < 4 ? kTiles : 4;
+#pragma unroll
+        for (int i0 = 0; i0 < kTiles; i0 += kAtOnce) {
+            uint2 y[kAtOnce][kWindow / 32][2];
+#pragma unroll
+            for (int i = 0; i < kAtOnce; ++i) {
+                const int at = 2 * kTiles * wave + 2 * (i0 + i) + ((ln >> 1) & 1);
+                const T* v0 = buf + r * R + 8 * (at & ~15) + 8 * ((at & 15) ^ f0) + 4 * (ln & 1);
+                const T* v1 = buf + (r + 4) * R + 8 * (at & ~15) + 8 * ((at & 15) ^ f1) + 4 * (ln & 1);
+#pragma unroll
+                for (int k = 0; k < kWindow / 32; ++k) {
+                    y[i][k][0] = read_tr(v0 + 32 * k * R);
+                    y[i][k][1] = read_tr(v1 + 32 * k * R);
+                }
+            }
+            stay();
+#pragma unroll
+            for (int i = 0; i < kAtOnce; ++i)
+#pragma unroll
+                for (int k = 0; k < kWindow / 32; ++k)
+                    st.o[i0 + i] = Act<T>::mma16(uint4{y[i][k][0].x, y[i][k][0].y, y[i][k][1].x, y[i][k][1].y}, p[k],
+                                                 st.o[i0 + i]);
+        }
+        landed();                        // the next window's
+        lds_barrier();
+    }
+
+    static __device__ __forceinline__ void segment(const kda_mla_absorbed_args& a, T* buf0, T* buf1, float (*sh)[kScore],
+                                                   int64_t b, int rt, int len, int lo, int hi, bool whole,
+                                                   const Workspace& ws, int64_t slot) {
+        const int lane = threadIdx.x & 63, ln = lane & 15, lg = lane >> 4;
+        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        const int rows = static_cast<int>(a.T * a.H), m0 = rt * kRows;
+        const float c = a.scale * kLog2E;
+        load(a, b, lo + kUnit * wave, hi, wave, lane, buf0);
+        // the queries through the other buffer: each piece is read from memory once
+        const Queries rq(a, m0);
+        constexpr int kQStride = D + 8, kPieces = kRows * (D / 8), kPer = (kPieces + kThreads - 1) / kThreads;
+        u4 qr[kPer];
+        const T* qb = static_cast<const T*>(a.q) + b * a.q_stride[0];
+#pragma unroll
+        for (int n = 0; n < kPer; ++n) {
+            const int i = min(static_cast<int>(threadIdx.x) + n * kThreads, kPieces - 1), r = i / (D / 8);
+            const int t = rq.token(r);
+            qr[n] = *reinterpret_cast<const u4*>(qb + t * a.q_stride[1] + rq.head(r, t) * a.q_stride[2] + i % (D / 8) * 8);
+        }
+        const int limit = min(hi - 1, len - static_cast<int>(a.T) + rq.token(ln));    // last key that the lane's row sees
+#pragma unroll
+        for (int n = 0; n < kPer; ++n) {
+            const int i = min(static_cast<int>(threadIdx.x) + n * kThreads, kPieces - 1);
+            *reinterpret_cast<u4*>(buf1 + i / (D / 8) * kQStride + i % (D / 8) * 8) = qr[n];
+        }
+        __syncthreads();
+        State st;
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k)
+            st.q[k] = *reinterpret_cast<const uint4*>(buf1 + ln * kQStride + 32 * k + 8 * lg);
+#pragma unroll
+        for (int i = 0; i < kTiles; ++i) st.o[i] = f4{0.f, 0.f, 0.f, 0.f};
+        st.top = kNoMax;
+        st.sum = 0.f;
+        landed();
+        lds_barrier();
+        for (int j0 = lo; j0 < hi; j0 += 2 * kWindow) {
+            window(a, b, j0, hi, limit, c, wave, lane, buf0, buf1, sh, st);
+            if (j0 + kWindow < hi) window(a, b, j0 + kWindow, hi, limit, c, wave, lane, buf1, buf0, sh, st);
+        }
+        const float den = lanegroup4_sum(st.sum), norm = den == 0.f ? 0.f : 1.f / den;
+        const int ch = 16 * kTiles * wave + 4 * lg;
+        if (whole) {
+            if (m0 + ln >= rows) return;
+            T* out = static_cast<T*>(a.o) + (b * rows + m0 + ln) * R + ch;
+#pragma unroll
+            for (int i = 0; i < kTiles; ++i)
+                *reinterpret_cast<uint2*>(out + 16 * i) = uint2{Act<T>::pair(st.o[i][0] * norm, st.o[i][1] * norm),
+                                                                Act<T>::pair(st.o[i][2] * norm, st.o[i][3] * norm)};
+        } else {
+            float* out = ws.o + (slot * kRows + ln) * R + ch;
+#pragma unroll
+            for (int i = 0; i < kTiles; ++i) *reinterpret_cast<f4*>(out + 16 * i) = st.o[i];
+            if (wave == 0 && lg == 0) ws.ml[slot * kRows + ln] = float2{st.top, den};
+        }
+    }
+};
 
 template <typename T, bool F8, int R, int P>
 struct Kernel {
@@ -132,26 +371,6 @@ struct Kernel {
         }
     }
 
-    // Query rows m0.. as (token, head): row m0 + r, past the last repeating it.
-    struct Queries {
-        int H, t0, h0, last;
-        float inv;
-        __device__ __forceinline__ Queries(const kda_mla_absorbed_args& a, int m0) {
-            H = static_cast<int>(a.H);
-            t0 = m0 / H;
-            h0 = m0 - t0 * H;
-            last = static_cast<int>(a.T) * H - 1 - m0;
-            inv = __builtin_amdgcn_rcpf(static_cast<float>(H));
-        }
-        // h0 + r < H + 16: with 16 heads or more it passes H once at most, with
-        // fewer it is below 32, which the reciprocal divides exactly
-        __device__ __forceinline__ int token(int r) const {
-            const int x = h0 + min(r, last);
-            return t0 + (H >= kRows ? (x >= H ? 1 : 0) : static_cast<int>((static_cast<float>(x) + 0.5f) * inv));
-        }
-        __device__ __forceinline__ int head(int r, int t) const { return h0 + min(r, last) - (t - t0) * H; }
-    };
-
     // One row tile's part, keys [lo, hi), of sequence b; the whole of it if
     // `whole`, else into the workspace's slot.
     static __device__ __forceinline__ void segment(const kda_mla_absorbed_args& a, Shared& sh, int64_t b, int rt, int len,
@@ -166,7 +385,6 @@ struct Kernel {
         // the queries through LDS: each piece is read from memory once
         const Queries rq(a, m0);
         constexpr int kPieces = kRows * (D / 8), kPer = (kPieces + kThreads - 1) / kThreads;
-        typedef uint32_t u4 __attribute__((ext_vector_type(4)));      // (an array of uint4 stays in scratch memory here)
         u4 qr[kPer];
         const T* qb = static_cast<const T*>(a.q) + b * a.q_stride[0];
 #pragma unroll
@@ -309,14 +527,22 @@ __device__ __forceinline__ int wave_scan(int x, int lane) {
 // of workgroups, each with its share of all units, at least kLeast.
 constexpr int kLeast = 8;
 template <typename T, bool F8, int R, int P>
-__global__ __launch_bounds__(kThreads, 2) void absorbed_kernel(kda_mla_absorbed_args a, int rts, bool alone) {
+__global__ __launch_bounds__(kThreads, F8 ? 2 : 1) void absorbed_kernel(kda_mla_absorbed_args a, int rts, bool alone) {
     using K = Kernel<T, F8, R, P>;
-    __shared__ __align__(16) typename K::Shared sh;
+    using K16 = Kernel16<T, R, P>;
+    __shared__ __align__(16) typename std::conditional<F8, typename K::Shared, int>::type sh;
+    __shared__ __align__(16) T buf0[F8 ? 1 : K16::kBuffer], buf1[F8 ? 1 : K16::kBuffer];
+    __shared__ __align__(16) float scores[F8 ? 1 : kRows][K16::kScore];
+    const auto segment = [&](int64_t b, int rt, int len, int lo, int hi, bool whole, const Workspace& ws,
+                             int64_t slot) __attribute__((always_inline)) {
+        if constexpr (F8) K::segment(a, sh, b, rt, len, lo, hi, whole, ws, slot);
+        else K16::segment(a, buf0, buf1, scores, b, rt, len, lo, hi, whole, ws, slot);
+    };
     const int lane = threadIdx.x & 63, nv = static_cast<int>(a.B) * rts, group = static_cast<int>(blockIdx.x);
     if (alone) {
         const int b = group / rts, rt = group - b * rts, len = tokens(a.lengths, b, a.S);
         if (len > 0) {
-            K::segment(a, sh, b, rt, len, 0, len, true, Workspace{}, 0);
+            segment(b, rt, len, 0, len, true, Workspace{}, 0);
         } else {
             const int rows = static_cast<int>(a.T * a.H), m0 = rt * kRows, n = min(rows - m0, kRows) * (R / 8);
             uint4* out = reinterpret_cast<uint4*>(static_cast<T*>(a.o) + (static_cast<int64_t>(b) * rows + m0) * R);
@@ -358,8 +584,8 @@ __global__ __launch_bounds__(kThreads, 2) void absorbed_kernel(kda_mla_absorbed_
             const int64_t at = before + __builtin_amdgcn_readlane(end, i) - n;
             const int lo = static_cast<int>(max(from - at, static_cast<int64_t>(0)));
             const int hi = static_cast<int>(min(to - at, static_cast<int64_t>(n)));
-            K::segment(a, sh, b, v - b * rts, size, kUnit * lo, min(kUnit * hi, size), lo == 0 && hi == n, ws,
-                       static_cast<int64_t>(group) + v);
+            segment(b, v - b * rts, size, kUnit * lo, min(kUnit * hi, size), lo == 0 && hi == n, ws,
+                    static_cast<int64_t>(group) + v);
             if (threadIdx.x == 0) {
                 if (lo == 0) ws.span[v].x = group;
                 if (hi == n) ws.span[v].y = group;
