@@ -74,6 +74,14 @@ __device__ __forceinline__ uint2 read_tr(const void* p) {
                                          (lds_s4)(reinterpret_cast<const s4*>(p))));
 }
 
+// Eight 8-bit values of one column: within 16 lanes, lane i gets rows 0..7 of
+// column i where lane 2 r + c points at row r, columns 8 c on.
+__device__ __forceinline__ uint2 read_tr8(const void* p) {
+    typedef int i2 __attribute__((ext_vector_type(2)));
+    typedef __attribute__((address_space(3))) i2* lds_i2;
+    return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i2)(reinterpret_cast<const i2*>(p))));
+}
+
 // Four neighbouring outputs, and where `low` is there what rounding took from each.
 template <typename T>
 __device__ __forceinline__ void store_out(T* out, T* low, f4 x) {

@@ -114,7 +114,7 @@ int kda_mla_absorbed_fwd(const kda_mla_absorbed_args* a, void* stream) {
         !at16(a->workspace) || !near(a->cache_stride[1]))
         return KDA_ERR_UNSUPPORTED;
     if (f8 && (reinterpret_cast<uintptr_t>(a->cache_scale) % 8 != 0 || a->scale_stride[0] % 2 != 0 ||
-               a->scale_stride[1] % 2 != 0))
+               a->scale_stride[1] % 2 != 0 || !near(a->scale_stride[1])))
         return KDA_ERR_UNSUPPORTED;
     return kda::mla_absorbed_launch(*a, static_cast<hipStream_t>(stream));
 }

@@ -115,7 +115,7 @@ def mla_expanded(q, k_nope, k_pe, v, lengths=None, starts=None, scale=None):
     of query 0.  A query whose position is ``lengths[b]`` or more does not
     exist, and one below 0 or of an empty sequence sees no key: both give zeros
     (and zero gradients).  A key or value that is not finite may reach the
-    queries of up to 64 positions before its own.
+    queries of up to 127 positions before its own.
 
     Differentiable in q, k_nope, k_pe and v (once); gradients have the inputs'
     types, are the same from run to run, and zero in rows past ``lengths``."""
