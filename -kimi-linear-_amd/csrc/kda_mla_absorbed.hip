@@ -543,12 +543,11 @@ __global__ __launch_bounds__(256) void join_kernel(kda_mla_absorbed_args a, int 
 
 int row_tiles(int64_t T, int64_t H) { return static_cast<int>((T * H + kRows - 1) / kRows); }
 
-// Workgroups of the shared form: one a CU in 16 bits, two in 8 bits, where a
-// window has half the bytes and its conversions to hide.  us, 256 / 512: B=64
-// of 2048 tokens 33.1 / 36.7, of 8192 116 / 124, of 64 to 4096 38.3 / 40.0; in 8
-// bits of 128 to 8192 54.6 / 46.1.
-constexpr int64_t kMostGroups = 512;
-constexpr int64_t groups_of(bool f8) { return f8 ? 512 : 256; }
+// Workgroups of the shared form: one a CU.  Two leave twice the parts to join
+// and are no faster in between; us at 16 heads, 256 / 512 workgroups: B=64 of 64
+// to 4096 tokens 36.8 / 44.4, in 8 bits 29.7 / 29.6; B=16 of 8192 34.1 / 40.2, in 8
+// bits 23.9 / 25.8.
+constexpr int64_t kGroups = 256;
 // Whether the units are shared among the workgroups: where one workgroup a row
 // tile would leave CUs idle or wait for the longest sequence.  us, shared /
 // one a row tile, lengths spread evenly: 300 sequences up to 4096 tokens 158 /
@@ -562,7 +561,7 @@ int launch(const kda_mla_absorbed_args& a, hipStream_t stream) {
     if (!shared_form(nv, a.S)) {
         absorbed_kernel<T, F8, R, P><<<static_cast<unsigned>(nv), kThreads, 0, stream>>>(a, rts, true);
     } else {
-        constexpr int groups = static_cast<int>(groups_of(F8));
+        constexpr int groups = static_cast<int>(kGroups);
         absorbed_kernel<T, F8, R, P><<<groups, kThreads, 0, stream>>>(a, rts, false);
         // many rows have few parts each, and few rows may have many
         const dim3 grid(static_cast<unsigned>(nv), kRows);
@@ -596,7 +595,7 @@ int launch_rank(const kda_mla_absorbed_args& a, hipStream_t stream) {
 int64_t mla_absorbed_workspace_bytes(int64_t B, int64_t T, int64_t H, int64_t S, int64_t R) {
     const int64_t nv = B * row_tiles(T, H);
     if (nv == 0 || !shared_form(nv, S)) return 0;
-    return slots(kMostGroups, nv) * kRows * (R * 4 + 8) + nv * 8;
+    return slots(kGroups, nv) * kRows * (R * 4 + 8) + nv * 8;
 }
 
 int mla_absorbed_launch(const kda_mla_absorbed_args& a, hipStream_t stream) {
