@@ -4,7 +4,10 @@
 //   s_tj = scale q_t . [k_j | k_pe_j],  o_t = sum_j 2^(s'_tj - M_t) v_j / sum_j 2^(s'_tj - M_t),
 //   s' = s log2(e),  M a running maximum.
 //
-// Bound by the matrix cores: 2 (N + P + V) flops a visible pair.  A wave has 32
+// Bound by the matrix cores: 2 (N + P + V) flops a visible pair.  At 128 + 64
+// channels, bf16, H=16: 1110 TFLOP/s at T=16384, 930 for T=2048 over 16384 keys,
+// 810 at B=4 T=2048 (a large product reaches 1200); one prompt of 1000 tokens
+// takes 22 us, the longest tile's eight steps in a row.  A wave has 32
 // query rows; a workgroup's waves share 64-key tiles of K, K_pe and V in LDS,
 // two buffers, the next tile's loads in flight through the current one's
 // products.  The scores are formed transposed (keys x rows, 32x32x16), so a

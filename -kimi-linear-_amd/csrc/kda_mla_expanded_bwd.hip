@@ -9,7 +9,9 @@
 // standing and the keys passing (dq, and delta for the other), one with a
 // wave's 32 keys standing and the queries passing (dk, dv): seven products
 // instead of the five that adding dq's parts in memory would take, and no
-// atomics, so the sums have one order.  Bound by the matrix cores.
+// atomics, so the sums have one order.  Bound by the matrix cores, which are
+// busy 40 % (dq) and 35 % (dk, dv) of the time: two waves a SIMD hide the steps
+// between a wave's products from each other in part only.
 //
 // In both, the scores are formed with the standing index in the lanes, so p
 // and ds, rounded to the activation type, are operands of the accumulating
@@ -75,7 +77,8 @@ __device__ __forceinline__ float dot8(uint4 x, uint4 y, float acc, bf16_t) {
     return acc;
 }
 
-// dq of 32 rows a wave, and delta.  Grid as the forward's.
+// dq of 32 rows a wave, and delta.  196 us at B=4 T=2048 H=16, 128 + 64 channels,
+// bf16: 700 TFLOP/s.  Grid as the forward's.
 template <typename T, int N, int P, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, 2) void dq_kernel(kda_mla_expanded_bwd_args g, float* delta, int qtiles) {
     const kda_mla_expanded_args& a = g.fwd;
@@ -205,12 +208,15 @@ __global__ __launch_bounds__(64 * WAVES, 2) void dq_kernel(kda_mla_expanded_bwd_
 // step's queries, so that a SIMD has two waves and each holds one half of the
 // sums of its keys, joined at the end.  (Four waves with K and V in registers
 // need more than 256 of them, and moving values between the two halves of the
-// register file took most of the time: 403 us at B=4 T=2048 H=16.)
+// register file took most of the time: 403 us at B=4 T=2048 H=16 with 128 + 64
+// channels, 268 this way, 640 TFLOP/s.)
 // Grid: (key tiles, the first have the most queries) x (batch, head), the latter inner.
 template <typename T, int N, int P>
 struct Dkv {
     static constexpr int D = N + P, V = N, NT = 512;
-    static constexpr int kK = D + 8, kV = V + 8;                  // LDS rows, elements
+    // LDS rows, elements: sixteen rows' pieces and, nearly, four rows of a transposed
+    // read in different banks (V + 8, which is right for the former alone: 274 us, V + 24 268)
+    static constexpr int kK = D + 8, kV = V + 24;
     static constexpr int kStanding = kStand * (kK + kV), kPassing = kPass * (kK + kV);
     static constexpr int kJoin = 4 * 64 * (D / 32) * 16 * 4;      // bytes: one half's dk
     static constexpr int kTiles = (kStanding + kPassing) * 2;
