@@ -14,10 +14,8 @@
 // A workgroup's waves each take 16 keys of a window and leave their scores
 // in LDS beside the rows; then every wave forms all of the window's weights
 // for itself (a few exponentials a lane) and the value product for its own
-// R / WAVES channels.  So the rows' sums are never spread over waves: there is
-// nothing to merge at the end of a sequence, and a wave holds few of them,
-// which leaves registers for the next window's rows, in flight while this one
-// is worked on, and room for a second workgroup on the CU.
+// R / WAVES channels.  So the rows' sums are never spread over waves, and there
+// is nothing to merge at the end of a sequence.
 //
 // The keys of all sequences are one list that the workgroups share evenly in
 // units of 16, whatever the lengths (a decode batch's differ): a workgroup's

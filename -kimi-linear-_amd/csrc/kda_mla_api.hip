@@ -35,6 +35,13 @@ bool sizes_ok(int64_t B, int64_t T, int64_t S, int64_t H) {
     return B >= 0 && T >= 0 && S >= 0 && H >= 0 && T <= kMaxTokens && S <= kMaxTokens && B <= kMaxGrid && H <= kMaxGrid;
 }
 
+// [n0, n1] rows of `width` elements of which no two share any, by strides that nest.
+bool distinct(const int64_t (&stride)[2], int64_t n0, int64_t n1, int64_t width) {
+    const int64_t s0 = n0 > 1 ? stride[0] : 0, s1 = n1 > 1 ? stride[1] : 0;
+    const bool rows = (n0 <= 1 || s0 >= width) && (n1 <= 1 || s1 >= width);
+    return rows && (n0 <= 1 || n1 <= 1 || s0 - width >= (n1 - 1) * s1 || s1 - width >= (n0 - 1) * s0);
+}
+
 // [p, p + bytes) of two arrays.
 bool apart(const void* a, int64_t na, const void* b, int64_t nb) {
     const auto a0 = reinterpret_cast<uintptr_t>(a), b0 = reinterpret_cast<uintptr_t>(b);
@@ -45,6 +52,7 @@ int expanded_check(const kda_mla_expanded_args& a) {
     if (!sizes_ok(a.B, a.T, a.S, a.H)) return KDA_ERR_BAD_SHAPE;
     if (!act(a.dtype)) return KDA_ERR_BAD_DTYPE;
     if ((a.N != 64 && a.N != 128) || a.V != a.N || !pos_ok(a.P) || !scale_ok(a.scale)) return KDA_ERR_UNSUPPORTED;
+    if (a.B * a.H > kMaxGrid) return KDA_ERR_BAD_SHAPE;
     if (a.B * a.H * ((a.T > a.S ? a.T : a.S) / 64 + 1) > kMaxGrid) return KDA_ERR_BAD_SHAPE;
     if (a.B == 0 || a.H == 0) return KDA_OK;
     if (a.T > 0 && (!a.q || !a.o)) return KDA_ERR_NULL_POINTER;
@@ -129,11 +137,10 @@ int kda_mla_cache_append(const kda_mla_append_args* a, void* stream) {
     if (!a->x || !a->cache || !a->lengths || (f8 && !a->cache_scale)) return KDA_ERR_NULL_POINTER;
     if (!rows_ok(a->x, a->x_stride, 2, 2) || !rows_ok(a->cache, a->cache_stride, 2, f8 ? 1 : 2) || !at16(a->norm_weight))
         return KDA_ERR_UNSUPPORTED;
-    // distinct rows of the cache, so that no two workgroups write one
-    const int64_t D = a->R + a->P;
-    if ((a->S > 1 && a->cache_stride[1] < D) || (a->B > 1 && a->cache_stride[0] < D)) return KDA_ERR_UNSUPPORTED;
+    // distinct rows of the cache, so that no two waves write one
+    if (!distinct(a->cache_stride, a->B, a->S, a->R + a->P)) return KDA_ERR_UNSUPPORTED;
     if (f8 && (reinterpret_cast<uintptr_t>(a->cache_scale) % 8 != 0 || a->scale_stride[0] % 2 != 0 ||
-               a->scale_stride[1] % 2 != 0 || (a->S > 1 && a->scale_stride[1] < 2) || (a->B > 1 && a->scale_stride[0] < 2)))
+               a->scale_stride[1] % 2 != 0 || !distinct(a->scale_stride, a->B, a->S, 2)))
         return KDA_ERR_UNSUPPORTED;
     return kda::mla_append_launch(*a, static_cast<hipStream_t>(stream));
 }

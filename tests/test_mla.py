@@ -159,6 +159,26 @@ def test_cache_codes(native):
     assert read(B=0) == 0 and read(S=0) == 0
 
 
+def test_append_wants_distinct_rows(native):
+    """Rows of different sequences may not share memory, in either order of the strides; sizes whose product
+    passes 64 bits are refused."""
+    lib = native.load()
+
+    def append(cache, scales=None):
+        a = native.KdaMlaAppendArgs(B=3, T=2, S=8, R=128, P=32, x_dtype=native.DTYPE_BF16,
+                                    cache_dtype=native.DTYPE_BF16 if scales is None else native.DTYPE_E4M3)
+        for f in ("x", "cache", "lengths") + (() if scales is None else ("cache_scale",)):
+            setattr(a, f, FAKE)
+        fill(a, {"x_stride": (320, 160), "cache_stride": cache, "scale_stride": scales or (0, 0)})
+        return lib.kda_mla_cache_append(ctypes.byref(a), None)
+
+    assert append((160, 160)) == 4 and append((1272, 160)) == 4 and append((160, 472)) == 4
+    assert append((1280, 160), (2, 2)) == 4 and append((1280, 160), (14, 2)) == 4 and append((1280, 160), (2, 4)) == 4
+    a = native.KdaMlaExpandedArgs(B=2 ** 31 - 1, T=2 ** 30, S=2 ** 30, H=2 ** 31 - 1, N=64, V=64, scale=1.0,
+                                  dtype=native.DTYPE_F16)
+    assert lib.kda_mla_expanded_fwd(ctypes.byref(a), None) == 2
+
+
 def test_wrapper_refuses_cpu_tensors(kda_pkg):
     q, k, pe = torch.zeros(1, 2, 2, 96, dtype=torch.bfloat16), torch.zeros(1, 2, 2, 64, dtype=torch.bfloat16), \
         torch.zeros(1, 2, 32, dtype=torch.bfloat16)
