@@ -630,6 +630,31 @@ bool expanded_forward(const Tensor& q, const Tensor& k, const OptTensor& k_pe, c
 OptTensor maybe(const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); }
 Tensor or_none(const OptTensor& t) { return t ? *t : Tensor(); }
 
+// While a backward pass is captured into a graph, the engine makes the stream of
+// each node that a gradient goes to wait for the captured one.  A leaf's node
+// lives as long as any graph of it: one made eagerly belongs to the default
+// stream, which no capture may touch, and the process would end there.
+void check_capture(const at::Device& dev) {
+    const auto node = torch::autograd::get_current_node();
+    if (!node || stream_of(dev) == nullptr) return;          // the default stream captures nothing
+    const c10::DeviceGuard guard(dev);
+    static PyObject* const capturing =
+        py::object(py::module_::import("torch.cuda").attr("is_current_stream_capturing")).release().ptr();
+    const py::object is = py::reinterpret_steal<py::object>(PyObject_CallNoArgs(capturing));
+    if (!is) throw py::error_already_set();
+    if (!is.cast<bool>()) return;
+    for (size_t i = 0; i < node->num_outputs(); ++i) {
+        if (!node->task_should_compute_output(i)) continue;
+        const auto stream = node->next_edge(i).function->stream();
+        if (stream && stream->id() == 0) {
+            PyErr_SetString(error, "mla_expanded: this captured backward pass goes on to a node of the default stream; "
+                                   "delete the eager outputs of the same tensors (or run them on another stream) before "
+                                   "the capture");
+            throw py::error_already_set();
+        }
+    }
+}
+
 // Its node in the autograd graph: in native code, as its Python form took
 // 80 us of a small training step's 160.
 struct ExpandedFn : torch::autograd::Function<ExpandedFn> {
@@ -655,6 +680,7 @@ struct ExpandedFn : torch::autograd::Function<ExpandedFn> {
         {
             const at::AutoGradMode off(false);
             const py::gil_scoped_acquire gil;
+            check_capture(q.device());
             const int status = run(q.device(), [&](void* stream) -> int {
                 const auto opt = q.options().requires_grad(false);
                 dq = at::empty(q.sizes(), opt);

@@ -118,7 +118,9 @@ def mla_expanded(q, k_nope, k_pe, v, lengths=None, starts=None, scale=None):
     queries of up to 127 positions before its own.
 
     Differentiable in q, k_nope, k_pe and v (once); gradients have the inputs'
-    types, are the same from run to run, and zero in rows past ``lengths``."""
+    types, are the same from run to run, and zero in rows past ``lengths``.  In a
+    captured backward pass the inputs must have no eager graph alive on the
+    default stream (its outputs deleted, or made on another stream): refused."""
     try:
         o = _native.host().mla_expanded(q, k_nope, k_pe, v, lengths, starts, q.shape[-1] ** -0.5 if scale is None else scale)
     except (TypeError, AttributeError, ZeroDivisionError):      # an argument of no type a common call has
@@ -197,8 +199,9 @@ def mla_absorbed(q, cache, lengths, rank, scale, cache_scale=None):
     ``lengths [B]`` counts a sequence's tokens with the T new ones, which are
     its last (append them first); cache rows from there on are never read.  A
     row that sees no key (an idle slot, or ``lengths[b] < T``) gives zeros.
-    ``scale`` is that of the expanded form, ``(N + P) ** -0.5``.  Ranks 128,
-    256, 512, P 0, 32, 64.  Forward only."""
+    ``scale`` is that of the expanded form, ``(N + P) ** -0.5``; ``cache_scale``
+    of the tokens as :func:`mla_cache_append` writes it (positive, from 2^-60).
+    Ranks 128, 256, 512, P 0, 32, 64.  Forward only."""
     try:
         o = _native.host().mla_absorbed(q, cache, lengths, rank, scale, cache_scale)
     except TypeError:
@@ -230,7 +233,8 @@ def mla_cache_append(x, cache, lengths, rank, cache_scale=None, counts=None, nor
     latent part and its position part each get the scale max|x| / 448 (at
     least 2^-60, written to ``cache_scale``; 1 where P = 0) and x / scale is
     rounded to the nearest e4m3 value.  A row with a value that is not finite
-    reads back as not finite.  x must not overlap the cache.  Forward only."""
+    reads back as not finite.  x must not overlap the cache, nor rows of the
+    cache each other.  Forward only."""
     try:
         if _native.host().mla_append(x, cache, lengths, rank, cache_scale, counts, norm_weight, eps):
             return

@@ -315,6 +315,38 @@ def test_expanded_captured(kda_pkg):
             assert torch.equal(a, b), n
 
 
+def test_expanded_capture_beside_an_eager_graph(kda_pkg):
+    """An eager graph of the same leaves, on the default stream, that lives when a backward pass is captured:
+    refused, as the engine would end the process; with it deleted, or of other leaves, the capture is fine."""
+    q, kn, pe, v = inputs(1, 70, 70, 2, 64, 32, F16, seed=85)
+    d_o = rand(1, 70, 2, 64, seed=89, dtype=F16)
+    leaves = [x.requires_grad_() for x in (q, kn, pe, v)]
+
+    def grads(xs):
+        return torch.autograd.grad(kda_pkg.mla_expanded(*xs), xs, d_o)
+
+    want = grads(leaves)
+    others = [x.detach().clone().requires_grad_() for x in leaves]
+    kept = kda_pkg.mla_expanded(*leaves)
+    torch.cuda.synchronize()
+    with pytest.raises(kda_pkg.KdaError, match="default stream"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            grads(leaves)
+    for xs in (others, leaves):
+        if xs is leaves:
+            assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(kept, leaves, d_o), want))
+            del kept
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = grads(xs)
+        for _ in range(3):
+            for g in got:
+                g.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 # ---- absorbed ---------------------------------------------------------------
 
 ABSORBED = [
