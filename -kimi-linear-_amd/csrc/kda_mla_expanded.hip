@@ -6,8 +6,8 @@
 //
 // Bound by the matrix cores: 2 (N + P + V) flops a visible pair.  At 128 + 64
 // channels, bf16, H=16: 1110 TFLOP/s at T=16384, 930 for T=2048 over 16384 keys,
-// 810 at B=4 T=2048 (a large product reaches 1200); one prompt of 1000 tokens
-// takes 22 us, the longest tile's eight steps in a row.  A wave has 32
+// 850 at B=4 T=2048 (a large product reaches 1200); one prompt of 1000 tokens
+// takes 21 us, the longest tile's eight steps in a row.  A wave has 32
 // query rows; a workgroup's waves share 64-key tiles of K, K_pe and V in LDS,
 // two buffers, the next tile's loads in flight through the current one's
 // products.  The scores are formed transposed (keys x rows, 32x32x16), so a
@@ -48,7 +48,9 @@ struct Parts {
 
 // A workgroup: RW waves of 32 query rows, times KW waves that share the keys
 // of each: of a step's KW KEYS keys, wave group g takes the g-th KEYS.  BUFS
-// buffers of a step's tiles.
+// buffers of a step's tiles; with one, the next step's keys are put where this
+// one's were while its values are still in use, and the values during the next
+// scores (T=1000 H=16 22.2 -> 21.5 us against both at the step's end).
 // Grid: (query tiles, longest first) x (batch, head) with the latter inner, so
 // that a head's tiles share an XCD's L2 where B H is a multiple of eight.
 // SPLIT: `splits` workgroups a query tile, its steps shared out evenly.
@@ -100,16 +102,18 @@ __global__ __launch_bounds__(64 * RW * KW, RW * KW == 8 ? 2 : 1) void expanded_k
         tile.fetch(a, first, keys);
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) q[k] = *reinterpret_cast<const uint4*>(qr + 16 * k);
-        tile.put(smem);
+        if constexpr (BUFS == 2) tile.put(smem);
+        else tile.put_keys(smem);
         __syncthreads();
         int cur = 0;
         for (int j0 = first; j0 < keys; j0 += kStep) {
+            if constexpr (BUFS == 1) tile.put_values(smem);
             tile.fetch(a, j0 + kStep, keys);
             const T* buf = smem + cur * F::kBuf;
             const int jw = j0 + KEYS * group;                     // the wave's first key
+            f16v s[kU];
             if (jw <= wlast) {
                 const T* kt = buf + (KEYS * group + lq) * F::kK + 8 * half;
-                f16v s[kU];
 #pragma unroll
                 for (int u = 0; u < kU; ++u) {
 #pragma unroll
@@ -118,6 +122,9 @@ __global__ __launch_bounds__(64 * RW * KW, RW * KW == 8 ? 2 : 1) void expanded_k
                     for (int k = 0; k < D / 16; ++k)
                         s[u] = Act<T>::mma32(*reinterpret_cast<const uint4*>(kt + 32 * u * F::kK + 16 * k), q[k], s[u]);
                 }
+            }
+            if constexpr (BUFS == 1) __syncthreads();     // the values are there, and the keys read
+            if (jw <= wlast) {
                 if (jw + KEYS - 1 > wall) {
 #pragma unroll
                     for (int u = 0; u < kU; ++u)
@@ -170,8 +177,7 @@ __global__ __launch_bounds__(64 * RW * KW, RW * KW == 8 ? 2 : 1) void expanded_k
                 tile.put(smem + cur * F::kBuf);
                 __syncthreads();
             } else {
-                __syncthreads();
-                tile.put(smem);
+                tile.put_keys(smem);
                 __syncthreads();
             }
         }
@@ -294,12 +300,14 @@ int launch_as(const kda_mla_expanded_args& a, hipStream_t stream, int splits = 1
 template <typename T, int N, int P>
 int launch(const kda_mla_expanded_args& a, hipStream_t stream) {
     // Eight waves a workgroup, as many of them on rows of their own as leave every
-    // CU a workgroup, or two where the tiles differ (few keys before the first
-    // query), so that long and short ones share a CU.  us, 256 / 128 rows: B=1
-    // T=4096 H=16 132 / 105; 128 / 64 rows: T=2048 46.5 / 45.1.
+    // CU a workgroup; of 256 rows two where the tiles differ (few keys before the
+    // first query), so that a long one is not alone at the end: us, 256 / 128 rows,
+    // B=1 T=4096 H=16 132 / 105.  128 / 64 rows, at 128 channels: T=2048 46 / 44, T=3000
+    // 66 / 88, B=2 T=1200 31 / 44, B=4 T=512 18 / 23.  At 64 channels two workgroups
+    // of either fit a CU, and 64 rows share it better: T=2800 48 / 39.
     const int64_t heads = a.B * a.H, least = a.S >= 2 * a.T ? 256 : 512;
     if (heads * ((a.T + 255) / 256) >= least) return launch_as<T, N, P, 8, 1, 64, 2>(a, stream);
-    if (heads * ((a.T + 127) / 128) >= least) return launch_as<T, N, P, 4, 2, 32, 2>(a, stream);
+    if (heads * ((a.T + 127) / 128) >= (N == 128 ? 256 : least)) return launch_as<T, N, P, 4, 2, 32, 2>(a, stream);
     const int splits = splits_of(a.B, a.T, a.S, a.H);
     if (splits > 1) return launch_as<T, N, P, 2, 4, 32, 1, true>(a, stream, splits);
     return launch_as<T, N, P, 2, 4, 32, 1>(a, stream);

@@ -82,10 +82,14 @@ struct KvTile {
         v.fetch(vp, a.v_stride[1], j0, keys);
         issued();
     }
-    __device__ __forceinline__ void put(T* buf) const {
+    __device__ __forceinline__ void put_keys(T* buf) const {
         k.put(buf);
         pe.put(buf + N);
-        v.put(buf + KEYS * kK);
+    }
+    __device__ __forceinline__ void put_values(T* buf) const { v.put(buf + KEYS * kK); }
+    __device__ __forceinline__ void put(T* buf) const {
+        put_keys(buf);
+        put_values(buf);
     }
 };
 
