@@ -34,8 +34,6 @@ namespace {
 using namespace mla;
 
 constexpr int kKeys = 32;             // keys a tile of the dq kernel
-constexpr int kStand = 128;           // keys a workgroup of the dk, dv kernel
-constexpr int kPass = 64;             // and queries a step
 
 template <typename T> constexpr bool kHalf = Elem<T>::code == KDA_DTYPE_F16;
 template <typename T> constexpr float kPShift = kHalf<T> ? 12.f : 0.f;
@@ -78,21 +76,31 @@ __device__ __forceinline__ float dot8(uint4 x, uint4 y, float acc, bf16_t) {
 }
 
 // dq of 32 rows a wave, and delta.  196 us at B=4 T=2048 H=16, 128 + 64 channels,
-// bf16: 700 TFLOP/s.  Grid as the forward's.
-template <typename T, int N, int P, int WAVES>
-__global__ __launch_bounds__(64 * WAVES, 2) void dq_kernel(kda_mla_expanded_bwd_args g, float* delta, int qtiles) {
+// bf16: 700 TFLOP/s.  RW waves of rows times KW that share the keys of each (of
+// a step's KW kKeys keys, wave group g takes the g-th kKeys), joined at the end.
+// Four groups' tiles of 128 + 64 channels fit LDS once, and the registers do not
+// hold the next ones beside the sums: those are loaded after the products.
+// Grid as the forward's.
+template <typename T, int N, int P, int RW, int KW>
+__global__ __launch_bounds__(64 * RW * KW, 2) void dq_kernel(kda_mla_expanded_bwd_args g, float* delta, int qtiles) {
     const kda_mla_expanded_args& a = g.fwd;
-    using F = KvTile<T, N, P, 64 * WAVES, kKeys, 8>;
-    constexpr int D = F::D, V = F::V, kRows = 32 * WAVES;
-    __shared__ __align__(16) T smem[2 * F::kBuf];
+    constexpr int kStep = KW * kKeys, kRows = 32 * RW;
+    using F = KvTile<T, N, P, 64 * RW * KW, kStep, 8>;
+    constexpr int D = F::D, V = F::V;
+    constexpr int kBufs = N == 128 && KW == 4 ? 1 : 2;
+    constexpr int kJoin = KW / 2 * RW * (D / 32) * 16 * 64 * 4, kTiles = kBufs * F::kBuf * 2;
+    constexpr int kBytes = kTiles > kJoin ? kTiles : kJoin;
+    __shared__ __align__(16) char raw[kBytes];
+    T* smem = reinterpret_cast<T*>(raw);
     const int64_t bhs = a.B * a.H, bh = blockIdx.x % bhs;
     const Place at(a, bh);
     const int t0 = (qtiles - 1 - static_cast<int>(blockIdx.x / bhs)) * kRows;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lq = lane & 31, half = lane >> 5;
-    const int t = t0 + 32 * wave + lq, nq = static_cast<int>(a.T);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lq = lane & 31;
+    const int half = lane >> 5, row = wave % RW, group = wave / RW;
+    const int t = t0 + 32 * row + lq, nq = static_cast<int>(a.T);
     const bool live = t < at.exist;
     const int limit = live ? at.start + t : -1;
-    const int w0 = t0 + 32 * wave;
+    const int w0 = t0 + 32 * row;
     const int wlast = w0 < at.exist ? at.start + min(w0 + 31, at.exist - 1) : -1;
     const int wall = w0 + 32 <= at.exist ? at.start + w0 : -1;
     const int keys = t0 < at.exist ? at.start + min(t0 + kRows, at.exist) : 0;
@@ -127,7 +135,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void dq_kernel(kda_mla_expanded_bwd_
             dl = dot8(d_o[k], *reinterpret_cast<const uint4*>(lrow + 16 * k), dl, T{});
         }
         dl = half_sum(dl);
-        if (live && half == 0) delta[bh * a.T + t] = dl;
+        if (live && half == 0 && group == 0) delta[bh * a.T + t] = dl;
         const float lse = (live ? a.lse[bh * a.T + t] : INFINITY) - kPShift<T>;
 
         F tile(a, at.b, at.h);
@@ -135,11 +143,12 @@ __global__ __launch_bounds__(64 * WAVES, 2) void dq_kernel(kda_mla_expanded_bwd_
         tile.put(smem);
         __syncthreads();
         int cur = 0;
-        for (int j0 = 0; j0 < keys; j0 += kKeys) {
-            tile.fetch(a, j0 + kKeys, keys);
-            if (j0 <= wlast) {
-                const T* kt = smem + cur * F::kBuf + lq * F::kK + 8 * half;
-                const T* vt = smem + cur * F::kBuf + kKeys * F::kK + lq * F::kV + 8 * half;
+        for (int j0 = 0; j0 < keys; j0 += kStep) {
+            if constexpr (kBufs == 2) tile.fetch(a, j0 + kStep, keys);
+            const int jw = j0 + kKeys * group;                    // the wave's first key
+            if (jw <= wlast) {
+                const T* kt = smem + cur * F::kBuf + (kKeys * group + lq) * F::kK + 8 * half;
+                const T* vt = smem + cur * F::kBuf + kStep * F::kK + (kKeys * group + lq) * F::kV + 8 * half;
                 f16v s, dp;
 #pragma unroll
                 for (int e = 0; e < 16; ++e) s[e] = dp[e] = 0.f;
@@ -148,10 +157,10 @@ __global__ __launch_bounds__(64 * WAVES, 2) void dq_kernel(kda_mla_expanded_bwd_
 #pragma unroll
                 for (int k = 0; k < V / 16; ++k)
                     dp = Act<T>::mma32(*reinterpret_cast<const uint4*>(vt + 16 * k), d_o[k], dp);
-                if (j0 + kKeys - 1 > wall) {
+                if (jw + kKeys - 1 > wall) {
 #pragma unroll
                     for (int e = 0; e < 16; ++e)
-                        if (j0 + 8 * (e / 4) + 4 * half + e % 4 > limit) s[e] = -INFINITY;
+                        if (jw + 8 * (e / 4) + 4 * half + e % 4 > limit) s[e] = -INFINITY;
                 }
                 float m = 0.f;
 #pragma unroll
@@ -172,7 +181,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void dq_kernel(kda_mla_expanded_bwd_
 #pragma unroll
                     for (int e = 0; e < 16; ++e) dp[e] *= f;
                 }
-                const T* tr = smem + cur * F::kBuf + (4 * half + ((lane & 15) >> 2)) * F::kK +
+                const T* tr = smem + cur * F::kBuf + (kKeys * group + 4 * half + ((lane & 15) >> 2)) * F::kK +
                               16 * ((lane >> 4) & 1) + 4 * (lane & 3);
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
@@ -186,34 +195,66 @@ __global__ __launch_bounds__(64 * WAVES, 2) void dq_kernel(kda_mla_expanded_bwd_
                     }
                 }
             }
-            cur ^= 1;
+            if constexpr (kBufs == 2) {
+                cur ^= 1;
+            } else {
+                __syncthreads();
+                tile.fetch(a, j0 + kStep, keys);
+            }
             tile.put(smem + cur * F::kBuf);
             __syncthreads();
         }
     }
-    if (t >= nq) return;
     const float norm = a.scale * __builtin_amdgcn_exp2f(-kPShift<T>) / f;
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) dq[i][e] *= norm;
+    // the key groups' sums, half of them onto the other half at a time
+#pragma unroll
+    for (int n = KW / 2; n > 0; n /= 2) {
+        f4* sums = reinterpret_cast<f4*>(raw) + (group % n * RW + row) * (D / 32) * 4 * 64 + lane;
+        if (group >= n && group < 2 * n) {
+#pragma unroll
+            for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    sums[(4 * i + e) * 64] = f4{dq[i][4 * e], dq[i][4 * e + 1], dq[i][4 * e + 2], dq[i][4 * e + 3]};
+        }
+        __syncthreads();
+        if (group < n) {
+#pragma unroll
+            for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const f4 y = sums[(4 * i + e) * 64];
+#pragma unroll
+                    for (int d = 0; d < 4; ++d) dq[i][4 * e + d] += y[d];
+                }
+        }
+        __syncthreads();
+    }
+    if (group != 0 || t >= nq) return;
     T* out = static_cast<T*>(g.dq) + ((at.b * a.T + t) * a.H + at.h) * D + 4 * half;
 #pragma unroll
     for (int i = 0; i < D / 32; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
             *reinterpret_cast<uint2*>(out + 32 * i + 8 * e) =
-                uint2{Act<T>::pair(dq[i][4 * e] * norm, dq[i][4 * e + 1] * norm),
-                      Act<T>::pair(dq[i][4 * e + 2] * norm, dq[i][4 * e + 3] * norm)};
+                uint2{Act<T>::pair(dq[i][4 * e], dq[i][4 * e + 1]), Act<T>::pair(dq[i][4 * e + 2], dq[i][4 * e + 3])};
 }
 
-// dk and dv.  A workgroup has kStand keys, whose rows of K and V stay in LDS,
-// and takes kPass queries a step: eight waves, each 32 of the keys and 32 of a
-// step's queries, so that a SIMD has two waves and each holds one half of the
+// dk and dv.  A workgroup has 32 KG keys, whose rows of K and V stay in LDS, and
+// takes 32 (8 / KG) queries a step: eight waves, each 32 of the keys and 32 of a
+// step's queries, so that a SIMD has two waves and each holds a part of the
 // sums of its keys, joined at the end.  (Four waves with K and V in registers
 // need more than 256 of them, and moving values between the two halves of the
 // register file took most of the time: 403 us at B=4 T=2048 H=16 with 128 + 64
 // channels, 268 this way, 640 TFLOP/s.)
 // Grid: (key tiles, the first have the most queries) x (batch, head), the latter inner.
-template <typename T, int N, int P>
+template <typename T, int N, int P, int KG>
 struct Dkv {
-    static constexpr int D = N + P, V = N, NT = 512;
+    static constexpr int D = N + P, V = N, NT = 512, kSides = 8 / KG, kStand = 32 * KG, kPass = 32 * kSides;
     // LDS rows, elements: sixteen rows' pieces and, nearly, four rows of a transposed
     // read in different banks (V + 8, which is right for the former alone: 274 us, V + 24 268)
     static constexpr int kK = D + 8, kV = V + 24;
@@ -223,11 +264,14 @@ struct Dkv {
     static constexpr int kBytes = (kTiles > kJoin ? kTiles : kJoin);
 };
 
-template <typename T, int N, int P>
+template <typename T, int N, int P, int KG>
 __global__ __launch_bounds__(512, 2) void dkv_kernel(kda_mla_expanded_bwd_args g, const float* delta, float* dpe) {
     const kda_mla_expanded_args& a = g.fwd;
-    using F = Dkv<T, N, P>;
-    constexpr int D = F::D, V = F::V, kK = F::kK, kV = F::kV;
+    using F = Dkv<T, N, P, KG>;
+    constexpr int D = F::D, V = F::V, kK = F::kK, kV = F::kV, kStand = F::kStand, kPass = F::kPass;
+    // the next step's queries in flight through the products where registers hold them
+    // (128 queries of 128 + 64 channels took 46 registers to scratch memory: T=1000 48 us, 32 without)
+    constexpr bool kEarly = KG == 4 || N == 64;
     __shared__ __align__(16) char raw[F::kBytes];
     __shared__ __align__(16) float stats[2][kPass];               // lse and delta of a step's queries
     T* ks = reinterpret_cast<T*>(raw);
@@ -238,7 +282,7 @@ __global__ __launch_bounds__(512, 2) void dkv_kernel(kda_mla_expanded_bwd_args g
     const Place at(a, bh);
     const int j0 = static_cast<int>(blockIdx.x / bhs) * kStand;
     const int lane = threadIdx.x & 63, lk = lane & 31, half = lane >> 5;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), mine = wave & 3, side = wave >> 2;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), mine = wave % KG, side = wave / KG;
     const int w0 = j0 + 32 * mine, j = w0 + lk;
     const float c = a.scale * kLog2E;
 
@@ -301,7 +345,7 @@ __global__ __launch_bounds__(512, 2) void dkv_kernel(kda_mla_expanded_bwd_args g
         put(first);
         __syncthreads();
         for (int t0 = first; t0 < at.exist; t0 += kPass) {
-            fetch(t0 + kPass);
+            if constexpr (kEarly) fetch(t0 + kPass);
             const int tw = t0 + 32 * side;                            // the wave's queries
             if (tw < at.exist && at.start + tw + 31 >= w0 && w0 < at.len) {
                 const T* qt = qs + (32 * side + lk) * kK + 8 * half;
@@ -372,41 +416,45 @@ __global__ __launch_bounds__(512, 2) void dkv_kernel(kda_mla_expanded_bwd_args g
                 }
             }
             __syncthreads();
+            if constexpr (!kEarly) fetch(t0 + kPass);
             put(t0 + kPass);
             __syncthreads();
         }
     }
-    // the two sides' sums, the second's onto the first's
+    // the sides' sums, half of them onto the other half at a time
     const float pn = __builtin_amdgcn_exp2f(-kPShift<T>), norm = a.scale * pn / f;
 #pragma unroll
     for (int i = 0; i < D / 32; ++i)
 #pragma unroll
         for (int e = 0; e < 16; ++e) dk[i][e] *= norm;
-    f4* half_sums = reinterpret_cast<f4*>(raw) + mine * (D / 32) * 4 * 64 + lane;
-    const auto join = [&](auto& x, int n) {
-        if (side == 1) {
+    const auto join = [&](auto& x, int tiles, int n) {
+        f4* sums = reinterpret_cast<f4*>(raw) + (side % n * KG + mine) * tiles * 4 * 64 + lane;
+        if (side >= n && side < 2 * n) {
 #pragma unroll
-            for (int i = 0; i < n; ++i)
+            for (int i = 0; i < tiles; ++i)
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    half_sums[(4 * i + e) * 64] = f4{x[i][4 * e], x[i][4 * e + 1], x[i][4 * e + 2], x[i][4 * e + 3]};
+                    sums[(4 * i + e) * 64] = f4{x[i][4 * e], x[i][4 * e + 1], x[i][4 * e + 2], x[i][4 * e + 3]};
         }
         __syncthreads();
-        if (side == 0) {
+        if (side < n) {
 #pragma unroll
-            for (int i = 0; i < n; ++i)
+            for (int i = 0; i < tiles; ++i)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const f4 y = half_sums[(4 * i + e) * 64];
+                    const f4 y = sums[(4 * i + e) * 64];
 #pragma unroll
                     for (int d = 0; d < 4; ++d) x[i][4 * e + d] += y[d];
                 }
         }
         __syncthreads();
     };
-    join(dk, D / 32);
-    join(dv, V / 32);
-    if (side == 1 || j >= a.S) return;
+#pragma unroll
+    for (int n = F::kSides / 2; n > 0; n /= 2) {
+        join(dk, D / 32, n);
+        join(dv, V / 32, n);
+    }
+    if (side != 0 || j >= a.S) return;
     const int64_t row = (at.b * a.S + j) * a.H + at.h;
     T* kout = static_cast<T*>(g.dk) + row * N + 4 * half;
     T* vout = static_cast<T*>(g.dv) + row * V + 4 * half;
@@ -450,20 +498,40 @@ __global__ __launch_bounds__(256) void dpe_kernel(const float* dpe, T* out, int6
 
 int64_t delta_bytes(int64_t B, int64_t T, int64_t H) { return (B * T * H * 4 + 15) / 16 * 16; }
 
+template <typename T, int N, int P, int RW, int KW>
+void launch_dq(const kda_mla_expanded_bwd_args& g, float* delta, hipStream_t stream) {
+    const int64_t qtiles = (g.fwd.T + 32 * RW - 1) / (32 * RW);
+    dq_kernel<T, N, P, RW, KW><<<static_cast<unsigned>(qtiles * g.fwd.B * g.fwd.H), 64 * RW * KW, 0, stream>>>(
+        g, delta, static_cast<int>(qtiles));
+}
+
 template <typename T, int N, int P>
 int launch(const kda_mla_expanded_bwd_args& g, hipStream_t stream) {
     const kda_mla_expanded_args& a = g.fwd;
     float* delta = static_cast<float*>(g.workspace);
     float* dpe = reinterpret_cast<float*>(static_cast<char*>(g.workspace) + delta_bytes(a.B, a.T, a.H));
-    const int64_t bhs = a.B * a.H, ktiles = (a.S + kStand - 1) / kStand;
-    // eight waves a workgroup where that leaves every CU one
-    const int64_t wide = (a.T + 255) / 256, narrow = (a.T + 127) / 128;
-    if (wide * bhs >= 256)
-        dq_kernel<T, N, P, 8><<<static_cast<unsigned>(wide * bhs), 512, 0, stream>>>(g, delta, static_cast<int>(wide));
-    else if (narrow > 0)
-        dq_kernel<T, N, P, 4><<<static_cast<unsigned>(narrow * bhs), 256, 0, stream>>>(g, delta, static_cast<int>(narrow));
+    const int64_t bhs = a.B * a.H, ktiles = (a.S + 127) / 128;
+    // Tiles of 256 query rows where that leaves every CU one; of 64, whose waves share
+    // the keys four ways, where those of 128 leave CUs idle and these have one each or
+    // are long; else of 128, the keys shared two ways unless they are few (a wave
+    // group's start costs more than it saves).  us, 128 rows alone / shared / 64
+    // rows, B=1 H=16, 128 + 64 channels: T=203 19 / 20 / 20, T=500 34 / 32 / 24, T=1000
+    // 60 / 48 / 33, T=3000 159 / 112; 64 + 32: T=500 H=8 21 / - / 14, T=3000 100 / 66.
+    if (a.T > 0) {
+        const int64_t wide = (a.T + 255) / 256, narrow = (a.T + 127) / 128, least = (a.T + 63) / 64;
+        if (wide * bhs >= 256) launch_dq<T, N, P, 8, 1>(g, delta, stream);
+        else if (narrow * bhs < 256 && (least * bhs <= 256 || a.S >= 1024) && (N == 64 || a.S > 256))
+            launch_dq<T, N, P, 2, 4>(g, delta, stream);
+        else if (a.S < (N == 128 ? 512 : 1024)) launch_dq<T, N, P, 4, 1>(g, delta, stream);
+        else launch_dq<T, N, P, 4, 2>(g, delta, stream);
+    }
     if (ktiles == 0) return hipGetLastError() == hipSuccess ? KDA_OK : KDA_ERR_LAUNCH;
-    dkv_kernel<T, N, P><<<static_cast<unsigned>(ktiles * bhs), 512, 0, stream>>>(g, delta, dpe);
+    // Likewise 64 keys a workgroup instead of 128: B=1 H=16, 128 + 64 channels T=203 20 /
+    // 15 us, T=1000 48 / 32, T=1500 67 / 46, B=4 T=300 (two rounds of short ones) 24 / 27.
+    if (ktiles * bhs >= 256 || ((a.S + 63) / 64 * bhs > 256 && a.S < 1024))
+        dkv_kernel<T, N, P, 4><<<static_cast<unsigned>(ktiles * bhs), 512, 0, stream>>>(g, delta, dpe);
+    else
+        dkv_kernel<T, N, P, 2><<<static_cast<unsigned>((a.S + 63) / 64 * bhs), 512, 0, stream>>>(g, delta, dpe);
     if constexpr (P > 0) {
         const int64_t n = a.S * P / 4;
         dpe_kernel<T><<<static_cast<unsigned>((a.B * n + 255) / 256), 256, 0, stream>>>(dpe, static_cast<T*>(g.dk_pe),

@@ -180,6 +180,24 @@ def test_expanded_forward_and_gradients(kda_pkg, case):
         close("d" + m, g, *ref[m])
 
 
+# Each of the backward's tilings (rows or keys a workgroup, how the waves share them), at lengths that end inside one.
+TILINGS = [
+    (1, 300, 300, 2, 128, 64, F16, [299], None),                 # 64 rows and keys
+    (2, 333, 700, 3, 128, 32, BF16, [700, 411], [367, 78]),
+    (1, 1100, 1100, 5, 128, 64, BF16, None, None),
+    (1, 270, 270, 1, 128, 0, F16, None, None),
+    (4, 520, 520, 16, 128, 64, BF16, [520, 519, 1, 300], None),  # 128 rows, their keys shared
+    (4, 520, 520, 16, 64, 32, F16, [520, 0, 129, 384], None),    # 128 rows
+    (2, 1030, 1030, 16, 64, 64, BF16, None, None),
+    (8, 300, 300, 16, 128, 64, F16, [300, 1, 0, 257, 256, 255, 299, 33], None),   # 256 rows
+]
+
+
+@pytest.mark.parametrize("case", TILINGS, ids=lambda c: "-".join(map(str, c[:6])) + "-" + str(c[6])[6:])
+def test_expanded_tilings(kda_pkg, case):
+    test_expanded_forward_and_gradients(kda_pkg, case)
+
+
 def test_expanded_gradients_against_differences(kda_pkg):
     """The directional derivative of sum(o w) in each input, by central differences of the float64 formula."""
     B, T, S, H, N, P = 1, 40, 56, 2, 64, 32
