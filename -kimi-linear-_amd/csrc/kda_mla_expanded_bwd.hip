@@ -511,24 +511,27 @@ int launch(const kda_mla_expanded_bwd_args& g, hipStream_t stream) {
     float* delta = static_cast<float*>(g.workspace);
     float* dpe = reinterpret_cast<float*>(static_cast<char*>(g.workspace) + delta_bytes(a.B, a.T, a.H));
     const int64_t bhs = a.B * a.H, ktiles = (a.S + 127) / 128;
-    // Tiles of 256 query rows where that leaves every CU one; of 64, whose waves share
-    // the keys four ways, where those of 128 leave CUs idle and these have one each or
-    // are long; else of 128, the keys shared two ways unless they are few (a wave
-    // group's start costs more than it saves).  us, 128 rows alone / shared / 64
+    // Tiles of 256 query rows where that leaves every CU two (a long one alone at the
+    // end takes as long as all the others); of 64, whose waves share the keys four ways,
+    // where those of 128 are no more than the CUs and these no more either or long;
+    // else of 128, the keys shared two ways unless they are few (a wave group's start
+    // costs more than it saves).  us, 128 rows alone / shared / 64
     // rows, B=1 H=16, 128 + 64 channels: T=203 19 / 20 / 20, T=500 34 / 32 / 24, T=1000
-    // 60 / 48 / 33, T=3000 159 / 112; 64 + 32: T=500 H=8 21 / - / 14, T=3000 100 / 66.
+    // 60 / 48 / 33, T=2048 109 / 86 / 73, T=2200 - / 84 / 92, T=3000 159 / 112 / 132; 64 + 32:
+    // T=500 H=8 21 / - / 14, T=3000 100 / 66 / 71.  256 rows / 128 shared, T=4096: 201 / 175.
     if (a.T > 0) {
         const int64_t wide = (a.T + 255) / 256, narrow = (a.T + 127) / 128, least = (a.T + 63) / 64;
-        if (wide * bhs >= 256) launch_dq<T, N, P, 8, 1>(g, delta, stream);
-        else if (narrow * bhs < 256 && (least * bhs <= 256 || a.S >= 1024) && (N == 64 || a.S > 256))
+        if (wide * bhs >= 512) launch_dq<T, N, P, 8, 1>(g, delta, stream);
+        else if (narrow * bhs <= 256 && (least * bhs <= 256 || a.S >= 1024) && (N == 64 || a.S > 256))
             launch_dq<T, N, P, 2, 4>(g, delta, stream);
         else if (a.S < (N == 128 ? 512 : 1024)) launch_dq<T, N, P, 4, 1>(g, delta, stream);
         else launch_dq<T, N, P, 4, 2>(g, delta, stream);
     }
     if (ktiles == 0) return hipGetLastError() == hipSuccess ? KDA_OK : KDA_ERR_LAUNCH;
     // Likewise 64 keys a workgroup instead of 128: B=1 H=16, 128 + 64 channels T=203 20 /
-    // 15 us, T=1000 48 / 32, T=1500 67 / 46, B=4 T=300 (two rounds of short ones) 24 / 27.
-    if (ktiles * bhs >= 256 || ((a.S + 63) / 64 * bhs > 256 && a.S < 1024))
+    // 15 us, T=1000 48 / 32, T=2048 89 / 69, T=2500 107 / 104, T=3000 125 / 133, B=4 T=300 (two
+    // rounds of short ones) 24 / 27.
+    if (ktiles * bhs > 320 || ((a.S + 63) / 64 * bhs > 256 && a.S < 1024))
         dkv_kernel<T, N, P, 4><<<static_cast<unsigned>(ktiles * bhs), 512, 0, stream>>>(g, delta, dpe);
     else
         dkv_kernel<T, N, P, 2><<<static_cast<unsigned>((a.S + 63) / 64 * bhs), 512, 0, stream>>>(g, delta, dpe);

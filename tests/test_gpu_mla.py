@@ -189,7 +189,8 @@ TILINGS = [
     (4, 520, 520, 16, 128, 64, BF16, [520, 519, 1, 300], None),  # 128 rows, their keys shared
     (4, 520, 520, 16, 64, 32, F16, [520, 0, 129, 384], None),    # 128 rows
     (2, 1030, 1030, 16, 64, 64, BF16, None, None),
-    (8, 300, 300, 16, 128, 64, F16, [300, 1, 0, 257, 256, 255, 299, 33], None),   # 256 rows
+    (8, 300, 300, 16, 128, 64, F16, [300, 1, 0, 257, 256, 255, 299, 33], None),
+    (16, 300, 300, 16, 128, 64, BF16, [300, 1, 0, 257, 256, 255, 299, 33] * 2, None),   # 256 rows
 ]
 
 
