@@ -17,10 +17,9 @@
 // R / WAVES channels.  So the rows' sums are never spread over waves, and there
 // is nothing to merge at the end of a sequence.
 //
-// The keys of all sequences are one list that the workgroups share evenly in
-// units of 16, whatever the lengths (a decode batch's differ): a workgroup's
-// share may begin and end inside a sequence, and what it has of one that
-// others share goes to the workspace, to be joined by a second kernel.
+// The keys of all sequences are shared among the workgroups in units of 16 by
+// what the lengths are (a decode batch's differ), and what a workgroup has of a
+// sequence that others share goes to the workspace, to be joined by a second kernel.
 //
 // In 8 bits a value is widened to the activation type exactly; a key's scale
 // multiplies its score, and enters the value product through the exponent,
@@ -28,9 +27,9 @@
 // scale.  M is then the largest of the sums, and the terms of the softmax's
 // denominator are divided by the scale again.
 //
-// At 16 heads, R=512 P=64 (a copy reaches 4.8 TB/s): B=64 of 8192 tokens 117 us
-// (5.2 TB/s), of 64 to 4096 tokens 45 us from HBM, in 8 bits 64 to 8192 47 us, with
-// 7 us of them the join; one sequence of 32768 18 us; of 200, in one workgroup,
+// At 16 heads, R=512 P=64 (a copy reaches 4.8 TB/s): B=64 of 8192 tokens 115 us
+// (5.2 TB/s), of 64 to 4096 tokens 41 us from HBM, in 8 bits 64 to 8192 44 us, with
+// 5 us of them the join; one sequence of 32768 18 us; of 200, in one workgroup,
 // 10 us: a window is 1.5 us and the way to the first one 3.
 #include <hip/hip_runtime.h>
 
@@ -410,9 +409,16 @@ __device__ __forceinline__ int wave_scan(int x, int lane) {
     return x;
 }
 
-// Grid: a workgroup for each row tile of each sequence (`alone`), or any number
-// of workgroups, each with its share of all units, at least kLeast.
-constexpr int kLeast = 8;
+// Grid: a workgroup for each row tile of each sequence (`alone`), or more than
+// kCut workgroups, each with its share of all units, at least kLeast.
+//
+// Up to kCut row tiles are cut each for itself into even parts, one a workgroup;
+// of more, the shares run on from one row tile into the next, which evens them out
+// but gives most workgroups two parts to start (1.3 us each) and more parts to join.
+// us at 16 heads, R=512 P=64, run on / cut: 64 sequences of 64 to 4096 tokens 36.6 /
+// 32.6, of 1 to 1000 23.7 / 16.8, 16 of 1900 with 4 tokens each 31 / 25, 37 of 8192
+// 74 / 73; in 8 bits 64 of 64 to 4096 29 / 24, but 52 of 8192 52 / 57.
+constexpr int kLeast = 8, kCut = 64;
 template <typename T, bool F8, int R, int P>
 __global__ __launch_bounds__(kThreads, F8 ? 2 : 1) void absorbed_kernel(kda_mla_absorbed_args a, int rts, bool alone) {
     using K = Kernel<T, F8, R, P>;
@@ -440,6 +446,32 @@ __global__ __launch_bounds__(kThreads, F8 ? 2 : 1) void absorbed_kernel(kda_mla_
     int64_t total = 0;
     for (int v0 = (nv - 1) / 64 * 64; v0 >= 0; v0 -= 64) total += look(v0);       // ends with the first 64
     if (total == 0) return;
+    if (nv <= kCut && total < INT32_MAX / 2) {       // cut by row tile; every workgroup returns in here
+        // The share: whole windows, so that the parts, each row tile's even, are no
+        // more than the workgroups.  Rounding up adds less than one part a row tile,
+        // so leaving nv workgroups out of the division always suffices; half as many
+        // mostly do.
+        const int n = units(len), all = static_cast<int>(total), groups = static_cast<int>(gridDim.x);
+        int k = 0;
+        for (int spare = nv / 2;; spare = nv) {
+            const int share = max((all / (groups - spare) + WAVES) / WAVES * WAVES, kLeast);
+            k = (n + share - 1) / share;
+            end = wave_scan(k, lane);
+            if (spare == nv || __builtin_amdgcn_readlane(end, 63) <= groups) break;
+        }
+        const uint64_t mine = __ballot(end - k <= group && group < end);
+        if (mine == 0) return;
+        const int v = __builtin_ctzll(mine), b = v / rts, size = __builtin_amdgcn_readlane(len, v);
+        const int parts = __builtin_amdgcn_readlane(k, v), at = group - (__builtin_amdgcn_readlane(end, v) - parts);
+        const int per = (units(size) + parts - 1) / parts, lo = at * per;
+        K::segment(a, sh, b, v - b * rts, size, kUnit * lo, min(kUnit * (lo + per), size), parts == 1, ws,
+                   static_cast<int64_t>(group) + v);
+        if (threadIdx.x == 0) {
+            if (at == 0) ws.span[v].x = group;
+            if (at == parts - 1) ws.span[v].y = group;
+        }
+        return;
+    }
     // A part is not worth its place in the workspace below kLeast units; short
     // sequences have a workgroup each.
     int64_t share;
@@ -551,6 +583,7 @@ int row_tiles(int64_t T, int64_t H) { return static_cast<int>((T * H + kRows - 1
 // to 4096 tokens 36.8 / 44.4, in 8 bits 29.7 / 29.6; B=16 of 8192 34.1 / 40.2, in 8
 // bits 23.9 / 25.8.
 constexpr int64_t kGroups = 256;
+static_assert(kGroups > kCut);
 // Whether the units are shared among the workgroups: where one workgroup a row
 // tile would leave CUs idle or wait for the longest sequence.  us, shared /
 // one a row tile, lengths spread evenly: 300 sequences up to 4096 tokens 158 /

@@ -405,6 +405,22 @@ def test_absorbed(kda_pkg, case, bits):
     assert torch.equal(got, kda_pkg.mla_absorbed(q, cache, i32(lengths), R, (128 + P) ** -0.5, cache_scale=scale))
 
 
+# Row tiles cut one by one, the most of them, and one more.
+SHARED = [
+    (64, 1, 16, 600, 128, 64, BF16, [600] + [1] * 63),
+    (64, 1, 16, 4096, 256, 32, F16, [(997 * b) % 4097 for b in range(64)]),
+    (65, 1, 16, 4096, 256, 32, F16, [(997 * b) % 4097 for b in range(65)]),
+    (9, 5, 20, 900, 128, 0, BF16, [900, 899, 0, 5, 3, 128, 129, 640, 17]),       # 63 row tiles
+    (60, 1, 16, 2048, 128, 64, BF16, 60 * [2048]),
+]
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+@pytest.mark.parametrize("case", SHARED, ids=lambda c: "-".join(map(str, c[:6])) + "-" + str(c[6])[6:])
+def test_absorbed_shared(kda_pkg, case, bits):
+    test_absorbed(kda_pkg, case, bits)
+
+
 @pytest.mark.parametrize("dtype", [BF16, F16])
 def test_absorbed_8bit_scales_of_any_size(kda_pkg, dtype):
     """Scales from 2^-60 (rows of zeros) over six orders of magnitude: weights keep their precision."""
