@@ -54,7 +54,8 @@ struct Parts {
 // Grid: (query tiles, longest first) x (batch, head) with the latter inner, so
 // that a head's tiles share an XCD's L2 where B H is a multiple of eight.
 // SPLIT: `splits` workgroups a query tile, its steps shared out evenly.
-template <typename T, int N, int P, int RW, int KW, int KEYS, int BUFS, bool SPLIT>
+// FEW: p goes into the value product with what its rounding leaves.
+template <typename T, int N, int P, int RW, int KW, int KEYS, int BUFS, bool SPLIT, bool FEW>
 __global__ __launch_bounds__(64 * RW * KW, RW * KW == 8 ? 2 : 1) void expanded_kernel(kda_mla_expanded_args a,
                                                                                      int qtiles, int splits) {
     constexpr int kStep = KW * KEYS, kRows = 32 * RW, kU = KEYS / 32;
@@ -147,10 +148,10 @@ __global__ __launch_bounds__(64 * RW * KW, RW * KW == 8 ? 2 : 1) void expanded_k
 #pragma unroll
                         for (int e = 0; e < 16; ++e) o[i][e] *= alpha;
                 }
-                uint4 p[2 * kU];
+                uint4 p[2 * kU], left[FEW ? 2 * kU : 1];
 #pragma unroll
                 for (int u = 0; u < 2 * kU; ++u) {
-                    uint32_t w[4];
+                    uint32_t w[4], l[4];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const float x = __builtin_amdgcn_exp2f(fmaf(s[u / 2][8 * (u % 2) + 2 * e], c, -top));
@@ -158,7 +159,9 @@ __global__ __launch_bounds__(64 * RW * KW, RW * KW == 8 ? 2 : 1) void expanded_k
                         sum += x;
                         sum += y;
                         w[e] = Act<T>::pair(x, y);
+                        if constexpr (FEW) l[e] = rest(x, y, T{});
                     }
+                    if constexpr (FEW) left[u] = uint4{l[0], l[1], l[2], l[3]};
                     p[u] = uint4{w[0], w[1], w[2], w[3]};
                 }
                 const T* vt = buf + kStep * F::kK + (KEYS * group + 4 * half + ((lane & 15) >> 2)) * F::kV +
@@ -170,6 +173,7 @@ __global__ __launch_bounds__(64 * RW * KW, RW * KW == 8 ? 2 : 1) void expanded_k
                         const uint2 v0 = read_tr(vt + 16 * u * F::kV + 32 * i);
                         const uint2 v1 = read_tr(vt + (16 * u + 8) * F::kV + 32 * i);
                         o[i] = Act<T>::mma32(uint4{v0.x, v0.y, v1.x, v1.y}, p[u], o[i]);
+                        if constexpr (FEW) o[i] = Act<T>::mma32(uint4{v0.x, v0.y, v1.x, v1.y}, left[u], o[i]);
                     }
             }
             if constexpr (BUFS == 2) {
@@ -285,10 +289,10 @@ int splits_of(int64_t B, int64_t T, int64_t S, int64_t H) {
     return static_cast<int>(most < fill ? most : fill);
 }
 
-template <typename T, int N, int P, int RW, int KW, int KEYS, int BUFS, bool SPLIT = false>
+template <typename T, int N, int P, int RW, int KW, int KEYS, int BUFS, bool SPLIT = false, bool FEW = false>
 int launch_as(const kda_mla_expanded_args& a, hipStream_t stream, int splits = 1) {
     const int64_t qtiles = (a.T + 32 * RW - 1) / (32 * RW);
-    expanded_kernel<T, N, P, RW, KW, KEYS, BUFS, SPLIT>
+    expanded_kernel<T, N, P, RW, KW, KEYS, BUFS, SPLIT, FEW>
         <<<static_cast<unsigned>(qtiles * a.B * a.H * splits), 64 * RW * KW, 0, stream>>>(a, static_cast<int>(qtiles), splits);
     if constexpr (SPLIT) {
         constexpr int rows = 256 / (N / 4);
@@ -305,6 +309,7 @@ int launch(const kda_mla_expanded_args& a, hipStream_t stream) {
     // B=1 T=4096 H=16 132 / 105.  128 / 64 rows, at 128 channels: T=2048 46 / 44, T=3000
     // 66 / 88, B=2 T=1200 31 / 44, B=4 T=512 18 / 23.  At 64 channels two workgroups
     // of either fit a CU, and 64 rows share it better: T=2800 48 / 39.
+    if (few(a)) return launch_as<T, N, P, 2, 4, 32, 1, false, true>(a, stream);
     const int64_t heads = a.B * a.H, least = a.S >= 2 * a.T ? 256 : 512;
     if (heads * ((a.T + 255) / 256) >= least) return launch_as<T, N, P, 8, 1, 64, 2>(a, stream);
     if (heads * ((a.T + 127) / 128) >= (N == 128 ? 256 : least)) return launch_as<T, N, P, 4, 2, 32, 2>(a, stream);

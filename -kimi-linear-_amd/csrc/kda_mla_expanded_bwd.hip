@@ -75,13 +75,20 @@ __device__ __forceinline__ float dot8(uint4 x, uint4 y, float acc, bf16_t) {
     return acc;
 }
 
+template <typename T>
+__device__ __forceinline__ uint4 rest8(const f16v& x, int at) {
+    return uint4{rest(x[at], x[at + 1], T{}), rest(x[at + 2], x[at + 3], T{}), rest(x[at + 4], x[at + 5], T{}),
+                 rest(x[at + 6], x[at + 7], T{})};
+}
+// FEW: p and ds go into the products with what their rounding leaves.  In variants of
+// their own: the others' registers are full (dk and dv 247 -> 277 us at 4 x 2048).
 // dq of 32 rows a wave, and delta.  196 us at B=4 T=2048 H=16, 128 + 64 channels,
 // bf16: 700 TFLOP/s.  RW waves of rows times KW that share the keys of each (of
 // a step's KW kKeys keys, wave group g takes the g-th kKeys), joined at the end.
 // Four groups' tiles of 128 + 64 channels fit LDS once, and the registers do not
 // hold the next ones beside the sums: those are loaded after the products.
 // Grid as the forward's.
-template <typename T, int N, int P, int RW, int KW>
+template <typename T, int N, int P, int RW, int KW, bool FEW>
 __global__ __launch_bounds__(64 * RW * KW, 2) void dq_kernel(kda_mla_expanded_bwd_args g, float* delta, int qtiles) {
     const kda_mla_expanded_args& a = g.fwd;
     constexpr int kStep = KW * kKeys, kRows = 32 * RW;
@@ -183,6 +190,18 @@ __global__ __launch_bounds__(64 * RW * KW, 2) void dq_kernel(kda_mla_expanded_bw
                 }
                 const T* tr = smem + cur * F::kBuf + (kKeys * group + 4 * half + ((lane & 15) >> 2)) * F::kK +
                               16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+                if constexpr (FEW) {
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        const uint4 ds = rest8<T>(dp, 8 * k);
+#pragma unroll
+                        for (int i = 0; i < D / 32; ++i) {
+                            const uint2 x = read_tr(tr + 16 * k * F::kK + 32 * i);
+                            const uint2 y = read_tr(tr + (16 * k + 8) * F::kK + 32 * i);
+                            dq[i] = Act<T>::mma32(uint4{x.x, x.y, y.x, y.y}, ds, dq[i]);
+                        }
+                    }
+                }
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
                     const uint4 ds{Act<T>::pair(dp[8 * k], dp[8 * k + 1]), Act<T>::pair(dp[8 * k + 2], dp[8 * k + 3]),
@@ -264,7 +283,7 @@ struct Dkv {
     static constexpr int kBytes = (kTiles > kJoin ? kTiles : kJoin);
 };
 
-template <typename T, int N, int P, int KG>
+template <typename T, int N, int P, int KG, bool FEW>
 __global__ __launch_bounds__(512, 2) void dkv_kernel(kda_mla_expanded_bwd_args g, const float* delta, float* dpe) {
     const kda_mla_expanded_args& a = g.fwd;
     using F = Dkv<T, N, P, KG>;
@@ -397,6 +416,22 @@ __global__ __launch_bounds__(512, 2) void dkv_kernel(kda_mla_expanded_bwd_args g
                 const int trow = 32 * side + 4 * half + ((lane & 15) >> 2), tcol = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
                 const T* qtr = qs + trow * kK + tcol;
                 const T* otr = os + trow * kV + tcol;
+                if constexpr (FEW) {
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        const uint4 pf = rest8<T>(s, 8 * u), df = rest8<T>(dp, 8 * u);
+#pragma unroll
+                        for (int i = 0; i < V / 32; ++i) {
+                            const uint2 y = read_tr(otr + 16 * u * kV + 32 * i), z = read_tr(otr + (16 * u + 8) * kV + 32 * i);
+                            dv[i] = Act<T>::mma32(uint4{y.x, y.y, z.x, z.y}, pf, dv[i]);
+                        }
+#pragma unroll
+                        for (int i = 0; i < D / 32; ++i) {
+                            const uint2 y = read_tr(qtr + 16 * u * kK + 32 * i), z = read_tr(qtr + (16 * u + 8) * kK + 32 * i);
+                            dk[i] = Act<T>::mma32(uint4{y.x, y.y, z.x, z.y}, df, dk[i]);
+                        }
+                    }
+                }
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
                     const uint4 pf{Act<T>::pair(s[8 * u], s[8 * u + 1]), Act<T>::pair(s[8 * u + 2], s[8 * u + 3]),
@@ -498,10 +533,10 @@ __global__ __launch_bounds__(256) void dpe_kernel(const float* dpe, T* out, int6
 
 int64_t delta_bytes(int64_t B, int64_t T, int64_t H) { return (B * T * H * 4 + 15) / 16 * 16; }
 
-template <typename T, int N, int P, int RW, int KW>
+template <typename T, int N, int P, int RW, int KW, bool FEW = false>
 void launch_dq(const kda_mla_expanded_bwd_args& g, float* delta, hipStream_t stream) {
     const int64_t qtiles = (g.fwd.T + 32 * RW - 1) / (32 * RW);
-    dq_kernel<T, N, P, RW, KW><<<static_cast<unsigned>(qtiles * g.fwd.B * g.fwd.H), 64 * RW * KW, 0, stream>>>(
+    dq_kernel<T, N, P, RW, KW, FEW><<<static_cast<unsigned>(qtiles * g.fwd.B * g.fwd.H), 64 * RW * KW, 0, stream>>>(
         g, delta, static_cast<int>(qtiles));
 }
 
@@ -521,7 +556,8 @@ int launch(const kda_mla_expanded_bwd_args& g, hipStream_t stream) {
     // T=500 H=8 21 / - / 14, T=3000 100 / 66 / 71.  256 rows / 128 shared, T=4096: 201 / 175.
     if (a.T > 0) {
         const int64_t wide = (a.T + 255) / 256, narrow = (a.T + 127) / 128, least = (a.T + 63) / 64;
-        if (wide * bhs >= 512) launch_dq<T, N, P, 8, 1>(g, delta, stream);
+        if (few(a)) launch_dq<T, N, P, 4, 1, true>(g, delta, stream);
+        else if (wide * bhs >= 512) launch_dq<T, N, P, 8, 1>(g, delta, stream);
         else if (narrow * bhs <= 256 && (least * bhs <= 256 || a.S >= 1024) && (N == 64 || a.S > 256))
             launch_dq<T, N, P, 2, 4>(g, delta, stream);
         else if (a.S < (N == 128 ? 512 : 1024)) launch_dq<T, N, P, 4, 1>(g, delta, stream);
@@ -531,10 +567,12 @@ int launch(const kda_mla_expanded_bwd_args& g, hipStream_t stream) {
     // Likewise 64 keys a workgroup instead of 128: B=1 H=16, 128 + 64 channels T=203 20 /
     // 15 us, T=1000 48 / 32, T=2048 89 / 69, T=2500 107 / 104, T=3000 125 / 133, B=4 T=300 (two
     // rounds of short ones) 24 / 27.
-    if (ktiles * bhs > 320 || ((a.S + 63) / 64 * bhs > 256 && a.S < 1024))
-        dkv_kernel<T, N, P, 4><<<static_cast<unsigned>(ktiles * bhs), 512, 0, stream>>>(g, delta, dpe);
+    if (few(a))
+        dkv_kernel<T, N, P, 2, true><<<static_cast<unsigned>((a.S + 63) / 64 * bhs), 512, 0, stream>>>(g, delta, dpe);
+    else if (ktiles * bhs > 320 || ((a.S + 63) / 64 * bhs > 256 && a.S < 1024))
+        dkv_kernel<T, N, P, 4, false><<<static_cast<unsigned>(ktiles * bhs), 512, 0, stream>>>(g, delta, dpe);
     else
-        dkv_kernel<T, N, P, 2><<<static_cast<unsigned>((a.S + 63) / 64 * bhs), 512, 0, stream>>>(g, delta, dpe);
+        dkv_kernel<T, N, P, 2, false><<<static_cast<unsigned>((a.S + 63) / 64 * bhs), 512, 0, stream>>>(g, delta, dpe);
     if constexpr (P > 0) {
         const int64_t n = a.S * P / 4;
         dpe_kernel<T><<<static_cast<unsigned>((a.B * n + 255) / 256), 256, 0, stream>>>(dpe, static_cast<T*>(g.dk_pe),

@@ -52,6 +52,22 @@ struct Rows<T, ROWS, 0, NT, PITCH> {
     __device__ __forceinline__ void put(T*) const {}
 };
 
+// What rounding two values to the activation type leaves of them, rounded.
+__device__ __forceinline__ uint32_t rest(float x, float y, _Float16) {
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+    const h2 r = __builtin_bit_cast(h2, Act<_Float16>::pair(x, y));
+    return Act<_Float16>::pair(x - static_cast<float>(r[0]), y - static_cast<float>(r[1]));
+}
+__device__ __forceinline__ uint32_t rest(float x, float y, bf16_t) {
+    const uint32_t r = Act<bf16_t>::pair(x, y);
+    return Act<bf16_t>::pair(x - __uint_as_float(r << 16), y - __uint_as_float(r & 0xffff0000u));
+}
+// Whether the expanded form's p and ds go into the products with what their rounding
+// leaves: of few values one rounding may be most of an output's error, and there is
+// time for it (bf16: two tokens dk 2.9e-3 off, 33 tokens 2.6e-3, by its own rounding 1.6e-3
+// and 1.7e-3, which it comes down to).  Of many the roundings average out to 2.4e-3.
+inline bool few(const kda_mla_expanded_args& a) { return a.S <= 32 || (a.S <= 128 && a.B * a.H <= 64); }
+
 // Loads issued before this stay before it: the compiler otherwise sinks a
 // prefetch past the products it is to overlap, down to its first use.
 __device__ __forceinline__ void issued() { asm volatile("" ::: "memory"); }

@@ -235,6 +235,26 @@ def test_expanded_small_fp16_gradients(kda_pkg):
         close("d" + m, g, *ref[m])
 
 
+@pytest.mark.parametrize("B,T,H,N,P,dtype", [(1, 2, 3, 128, 0, BF16), (1, 33, 3, 64, 64, BF16), (2, 128, 2, 128, 64, F16)])
+def test_expanded_few_tokens(kda_pkg, B, T, H, N, P, dtype):
+    """Of few values no single rounding may dominate: the weights and ds keep 16 bits or more, so what is left of
+    an output's error is its own rounding (relative, in the 2-norm) and less than 2^-12 in bf16 (a weight kept to
+    2^-17, o and its rounding to 2^-17, a sum's cancellation below 2^5), 2^-14 in fp16 (E, as above, is 2^-11)."""
+    q, kn, pe, v = inputs(B, T, T, H, N, P, dtype, seed=60)
+    d_o = rand(B, T, H, N, seed=64, dtype=dtype)
+    leaves = [x.requires_grad_() for x in (q, kn, pe, v) if x is not None]
+    o = kda_pkg.mla_expanded(q, kn, pe, v)
+    grads = torch.autograd.grad(o, leaves, d_o)
+    with torch.no_grad():
+        want, _, ref = expanded_ref(q, kn, pe, v, [T] * B, [0] * B, (N + P) ** -0.5, d_o)
+    ref = {"o": (want, None), **ref}
+    names = ["o"] + [m for m, x in (("q", q), ("k_nope", kn), ("k_pe", pe), ("v", v)) if x is not None]
+    for m, got in zip(names, (o, *grads)):
+        r = ref[m][0]
+        off, own = (((x.double() - r).norm() / r.norm()).item() for x in (got, r.to(dtype)))
+        assert off <= own + (2.0 ** -12 if dtype is BF16 else 2.0 ** -14), (m, off, own)
+
+
 def test_expanded_views_streams_and_types(kda_pkg):
     B, T, H, N, P = 2, 90, 3, 128, 64
     kv = rand(B, T, H, 2 * N, seed=60, dtype=BF16)
