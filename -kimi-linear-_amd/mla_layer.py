@@ -20,7 +20,10 @@ protocol of ``KimiDeltaAttention``, so the two mix in one stack and in
   the device and, as all sequences grow together, on the host;
 * ``layer(x, state=state, use_cache=True)``: continues it, in place: one token
   through the absorbed form (the key and value up-projections applied to q and
-  to the output), several through the expanded form over the cached latents;
+  to the output), several through the expanded form over the cached latents.
+  The absorbed form takes ``kv_up`` for the product with its weight: where the
+  module does more (an adapter, a hook, a bias, a forward of its own) one token
+  goes through the expanded form too, which calls the module;
 * ``layer.decode_step_(x, state)``: one token.
 
 A cache that would overflow raises :class:`KdaError` before anything is written.
@@ -35,6 +38,7 @@ import torch.nn as nn
 
 from . import _native
 from .kda import KdaError
+from .layer import _plain_weight
 from .mla import mla_absorbed, mla_cache_append, mla_cache_read, mla_expanded
 
 
@@ -95,10 +99,16 @@ class LatentAttention(nn.Module):
         """Make the absorbed form's copies again."""
         if self._up is not None:
             self._up = (None, self._up[1], self._up[2])
-        self._up_weights()
+        if self._absorbs():
+            self._up_weights()
+
+    def _absorbs(self, x=None):
+        """Whether ``kv_up`` is just the product with its weight, which the absorbed form splits."""
+        return _plain_weight(self.kv_up, *(() if x is None else (x,))) is not None
 
     def _weight_buffers(self):
-        return [w.data_ptr() for w in self._up_weights()]
+        """What a captured step reads of ``kv_up``."""
+        return [w.data_ptr() for w in (self._up_weights() if self._absorbs() else self.kv_up.parameters())]
 
     # ------------------------------------------------------------ the cache
     def new_state(self, B: int, device, dtype) -> dict:
@@ -120,13 +130,14 @@ class LatentAttention(nn.Module):
         state["lengths"].add_(x.shape[1])
 
     # ------------------------------------------------------------ the two forms
-    def _expanded(self, x, rows, starts=None):
+    def _expanded(self, x, rows, lengths=None, starts=None):
         """Attention of x's queries over latent rows [B, S, rank + P], normalised already."""
         B, T, _ = x.shape
         H, N, R = self.num_heads, self.head_dim, self.rank
         kv = self.kv_up(rows[..., :R]).view(B, rows.shape[1], H, 2 * N)
         o = mla_expanded(self.q_proj(x).view(B, T, H, N + self.position_dim), kv[..., :N],
-                         rows[..., R:] if self.position_dim else None, kv[..., N:], starts=starts, scale=self.scale)
+                         rows[..., R:] if self.position_dim else None, kv[..., N:], lengths=lengths, starts=starts,
+                         scale=self.scale)
         return self.o_proj(o.reshape(B, T, H * N))
 
     def _norm(self, c):
@@ -163,25 +174,34 @@ class LatentAttention(nn.Module):
             return self.decode_step_(x, state), state
         self._append(x, state)
         state["tokens"] += T
-        n = state["tokens"]
-        rows = state["latent"][:, :n]
-        if self.cache_bits == 8:
-            rows = mla_cache_read(state["latent"], state["scale"], self.rank, dtype=x.dtype, tokens=n)
-        return self._expanded(x, rows), state
+        return self._expanded(x, self._held(x, state, state["tokens"])), state
 
     def _whole(self, x):
         c = self.kv_down(x)
         return self._expanded(x, torch.cat([self._norm(c[..., :self.rank]), c[..., self.rank:]], -1))
 
-    def _step(self, x, state):
-        """One token, unchecked: the captured part of a decode step."""
+    def _held(self, x, state, n):
+        """The cache's first n rows in x's type."""
+        if self.cache_bits == 8:
+            return mla_cache_read(state["latent"], state["scale"], self.rank, dtype=x.dtype, tokens=n)
+        return state["latent"][:, :n]
+
+    def _step(self, x, state, n=None):
+        """One token, unchecked: the captured part of a decode step.  ``n``: the tokens held with it, by which the
+        expanded form is cut to the rows that there are; a captured step, whose count moves, expands all of the
+        cache and takes the count from the device."""
         self._append(x, state)
-        return self._absorbed(x, state)
+        if self._absorbs(x):
+            return self._absorbed(x, state)
+        if n is not None:
+            return self._expanded(x, self._held(x, state, n))
+        rows = self._held(x, state, state["latent"].shape[1])
+        return self._expanded(x, rows, lengths=state["lengths"], starts=state["lengths"] - 1)
 
     @torch.no_grad()
     def decode_step_(self, x, state):
         """One token x ``[B, 1, d]`` -> ``[B, 1, d]``; the state is updated in place."""
         self._room(state, 1)
-        out = self._step(x, state)
+        out = self._step(x, state, state["tokens"] + 1)
         state["tokens"] += 1
         return out

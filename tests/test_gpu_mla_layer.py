@@ -9,8 +9,11 @@ each, at scores of size one."""
 
 from __future__ import annotations
 
+import copy
+
 import pytest
 import torch
+import torch.nn as nn
 
 pytestmark = pytest.mark.gpu
 
@@ -174,3 +177,62 @@ def test_mixed_stack_captured(kda_pkg, bits):
         c = KdaGraphedDecoder(layers)
         c.prefill(x[:, :30])
         assert torch.equal(c.step_eager(x[:, 30:31]), b)
+
+
+class Adapter(nn.Module):
+    """A linear layer with a low-rank part beside it, whose ``weight`` is the base's."""
+
+    def __init__(self, base, seed):
+        super().__init__()
+        g = torch.Generator(device=DEV).manual_seed(seed)
+        self.base = base
+        w = base.weight
+        self.down = nn.Parameter(torch.randn(8, w.shape[1], device=DEV, generator=g).to(w.dtype) * w.shape[1] ** -0.5)
+        self.up = nn.Parameter(torch.randn(w.shape[0], 8, device=DEV, generator=g).to(w.dtype) * 0.3)
+
+    @property
+    def weight(self):
+        return self.base.weight
+
+    def forward(self, x):
+        return self.base(x) + (x @ self.down.T) @ self.up.T
+
+
+def wrapped(kda_pkg, kind, **kw):
+    """A layer whose kv_up does more than the product with its weight, and a plain layer that computes the same."""
+    layer = make(kda_pkg, torch.bfloat16, **kw).eval()
+    same = copy.deepcopy(layer)
+    w = layer.kv_up.weight.detach().double()
+    if kind == "adapter":
+        layer.kv_up = Adapter(layer.kv_up, 7)
+        w = w + layer.kv_up.up.detach().double() @ layer.kv_up.down.detach().double()
+    elif kind == "hook":
+        layer.kv_up.register_forward_hook(lambda mod, args, out: 0.5 * out)
+        w = 0.5 * w
+    else:
+        layer.kv_up.forward = lambda x: 2 * nn.functional.linear(x, layer.kv_up.weight)
+        w = 2 * w
+    same.kv_up.weight = nn.Parameter(w)
+    return layer, same
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+@pytest.mark.parametrize("kind", ["adapter", "hook", "forward"])
+def test_decode_follows_what_wraps_kv_up(kda_pkg, kind, bits):
+    """Single tokens, eager and captured, see what the module adds to its weight, as prompts do."""
+    from kimi_linear_amd.graph_decode import KdaGraphedDecoder
+    layer, same = wrapped(kda_pkg, kind, cache_bits=bits)
+    x = torch.randn(2, 60, 256, device=DEV).bfloat16()
+    # two roundings more than the layer's ten (the low-rank part's products)
+    tol = TOL[torch.bfloat16] * 12 / 8 + (0 if bits == 16 else 2 * 3.6e-2)
+    with torch.no_grad():
+        want, _ = reference(same, x.double())
+        got, state = layer(x[:, :50], use_cache=True)
+        dec = KdaGraphedDecoder([layer], residual=False)
+        dec.prefill(x[:, :50])
+        assert rel(got, want[:, :50]) <= tol
+        for t in range(50, 60):
+            out, state = layer(x[:, t:t + 1], state=state, use_cache=True)
+            assert rel(out, want[:, t:t + 1]) <= tol, t
+            assert rel(dec.step(x[:, t:t + 1]), want[:, t]) <= tol, t
+        assert state["tokens"] == 60 and dec.static_states[0]["lengths"].tolist() == [60, 60]
