@@ -25,6 +25,9 @@ A latent layer's state is its cache, a buffer for ``max_tokens`` tokens that a
 step appends to in place; the tokens held are counted on the device, where the
 captured kernels read them, and on the host, where :meth:`step` refuses a full
 cache.  Rows past the count are never read, so a snapshot is the count alone.
+A ``decode_step_`` of a subclass or an instance is the one that is captured; a
+position it needs has to come from ``state["lengths"]``, as ``state["tokens"]``
+is a number that the capture would keep.
 
 The stack is ``h <- h + layer(h)`` per layer (``residual=True``) or
 ``h <- layer(h)``; the model's other blocks (FFN, norms, LM head) are not
@@ -120,7 +123,13 @@ class KdaGraphedDecoder:
                 # the residual add belongs to the output projection, which writes the result in place
                 h = layer._decode(h, st, h, result if i + 1 == len(self.layers) else None)
                 continue
-            out = layer._step(h, st) if isinstance(layer, LatentAttention) else layer.decode_step_(h, st)
+            if isinstance(layer, LatentAttention) and layer._unmodified("decode_step_"):
+                out = layer._step(h, st)
+            else:
+                held = st.get("tokens")
+                out = layer.decode_step_(h, st)
+                if held is not None:
+                    st["tokens"] = held         # counted by step(): a replay counts nothing on the host
             h = h + out if self.residual else out
         if h is not result:
             self.output_static.copy_(h[:, -1, :])
@@ -172,6 +181,18 @@ class KdaGraphedDecoder:
 
     @torch.no_grad()
     def _capture(self):
+        held = [st.get("tokens") for st in self.static_states]
+        try:
+            for st, n in zip(self.static_states, held):
+                if n is not None:               # a full cache is captured too: what it has no room for is dropped
+                    st["tokens"] = min(n, st["latent"].shape[1] - 1)
+            self._record()
+        finally:
+            for st, n in zip(self.static_states, held):
+                if n is not None:
+                    st["tokens"] = n
+
+    def _record(self):
         torch.cuda.synchronize()
         snap = self._snapshot()
         side = torch.cuda.Stream()

@@ -7,8 +7,7 @@
     [k | v] = W_up c               per head, N channels each
     out = W_o attention(q, [k | p], v)
 
-The position channels carry no rotation (a caller that wants one applies it in
-``q_proj`` and ``kv_down``'s outputs by subclassing).  The layer has the call
+The position channels carry no rotation.  The layer has the call
 protocol of ``KimiDeltaAttention``, so the two mix in one stack and in
 ``KdaGraphedDecoder``:
 
@@ -101,6 +100,10 @@ class LatentAttention(nn.Module):
             self._up = (None, self._up[1], self._up[2])
         if self._absorbs():
             self._up_weights()
+
+    def _unmodified(self, method):
+        """Whether the method is the one written here, not a subclass's, the instance's or a later replacement."""
+        return getattr(type(self), method) is _METHODS[method] and method not in self.__dict__
 
     def _absorbs(self, x=None):
         """Whether ``kv_up`` is just the product with its weight, which the absorbed form splits."""
@@ -205,3 +208,6 @@ class LatentAttention(nn.Module):
         out = self._step(x, state, state["tokens"] + 1)
         state["tokens"] += 1
         return out
+
+
+_METHODS = {n: getattr(LatentAttention, n) for n in ("decode_step_",)}

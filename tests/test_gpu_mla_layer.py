@@ -236,3 +236,33 @@ def test_decode_follows_what_wraps_kv_up(kda_pkg, kind, bits):
             assert rel(out, want[:, t:t + 1]) <= tol, t
             assert rel(dec.step(x[:, t:t + 1]), want[:, t]) <= tol, t
         assert state["tokens"] == 60 and dec.static_states[0]["lengths"].tolist() == [60, 60]
+
+
+@pytest.mark.parametrize("how", ["subclass", "instance"])
+def test_decoder_takes_an_overridden_decode_step(kda_pkg, how):
+    """Captured and eager steps of the decoder are the layer's own decode_step_; the host's count moves once a step,
+    and a prompt that fills the cache is still captured."""
+    from kimi_linear_amd.graph_decode import KdaGraphedDecoder
+    plain = kda_pkg.LatentAttention.decode_step_
+    layer = make(kda_pkg, torch.float16).eval()
+    if how == "subclass":
+        layer.__class__ = type("Doubled", (kda_pkg.LatentAttention,), {"decode_step_": lambda self, x, st: 2 * plain(self, x, st)})
+    else:
+        layer.decode_step_ = lambda x, st: 2 * plain(layer, x, st)
+    x = torch.randn(2, 50, 256, device=DEV).half()
+    with torch.no_grad():
+        _, state = layer(x[:, :40], use_cache=True)
+        dec = KdaGraphedDecoder([layer], residual=False)
+        dec.prefill(x[:, :40])
+        assert dec.static_states[0]["tokens"] == 40
+        for t in range(40, 50):
+            want, state = layer(x[:, t:t + 1], state=state, use_cache=True)
+            got = dec.step(x[:, t:t + 1]) if t < 47 else dec.step_eager(x[:, t:t + 1])
+            assert torch.equal(got, want[:, 0]), t
+            assert dec.static_states[0]["tokens"] == state["tokens"] == t + 1
+        assert dec.static_states[0]["lengths"].tolist() == [50, 50]
+        full = KdaGraphedDecoder([layer], residual=False)
+        full.prefill(x.repeat(1, 2, 1)[:, :96])
+        assert full.static_states[0]["tokens"] == 96 and full.static_states[0]["lengths"].tolist() == [96, 96]
+        with pytest.raises(kda_pkg.KdaError, match="full"):
+            full.step(x[:, :1])
