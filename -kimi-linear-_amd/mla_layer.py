@@ -204,6 +204,8 @@ class LatentAttention(nn.Module):
     @torch.no_grad()
     def decode_step_(self, x, state):
         """One token x ``[B, 1, d]`` -> ``[B, 1, d]``; the state is updated in place."""
+        if x.dim() != 3 or x.shape[1] != 1:
+            raise KdaError(f"decode_step_ takes one token, got x of shape {tuple(x.shape)}")
         self._room(state, 1)
         out = self._step(x, state, state["tokens"] + 1)
         state["tokens"] += 1

@@ -266,3 +266,17 @@ def test_decoder_takes_an_overridden_decode_step(kda_pkg, how):
         assert full.static_states[0]["tokens"] == 96 and full.static_states[0]["lengths"].tolist() == [96, 96]
         with pytest.raises(kda_pkg.KdaError, match="full"):
             full.step(x[:, :1])
+
+
+def test_decode_step_takes_one_token(kda_pkg):
+    """Anything but one token is refused before the cache or its count has changed."""
+    layer = make(kda_pkg, torch.bfloat16)
+    x = torch.randn(2, 30, 256, device=DEV).bfloat16()
+    with torch.no_grad():
+        _, state = layer(x, use_cache=True)
+        before = state["latent"].view(torch.int16).clone()
+        for bad in (x[:, :2], x[:, :0], x[:, 0]):
+            with pytest.raises(kda_pkg.KdaError, match="one token"):
+                layer.decode_step_(bad, state)
+        assert state["tokens"] == 30 and state["lengths"].tolist() == [30, 30]
+        assert torch.equal(state["latent"].view(torch.int16), before)
