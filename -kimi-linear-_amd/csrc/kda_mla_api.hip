@@ -28,6 +28,13 @@ bool rows_ok(const void* p, const int64_t* stride, int n, int64_t bytes) {
 // Token strides whose tiles of up to 128 rows a 32-bit offset reaches.
 bool near(int64_t stride) { return stride < (int64_t{1} << 23); }
 
+// Rows of scale pairs, read and written 8 bytes at a time.  (The kernels' offsets
+// from a row are unsigned.)
+bool scale_rows_ok(const void* p, const int64_t (&stride)[2]) {
+    return reinterpret_cast<uintptr_t>(p) % 8 == 0 && stride[0] >= 0 && stride[1] >= 0 && stride[0] % 2 == 0 &&
+           stride[1] % 2 == 0;
+}
+
 bool scale_ok(float s) { return std::isfinite(s) && s > 0.f; }
 bool pos_ok(int64_t P) { return P == 0 || P == 32 || P == 64; }
 
@@ -121,8 +128,7 @@ int kda_mla_absorbed_fwd(const kda_mla_absorbed_args* a, void* stream) {
     if (!rows_ok(a->q, a->q_stride, 3, 2) || !rows_ok(a->cache, a->cache_stride, 2, f8 ? 1 : 2) || !at16(a->o) ||
         !at16(a->workspace) || !near(a->cache_stride[1]))
         return KDA_ERR_UNSUPPORTED;
-    if (f8 && (reinterpret_cast<uintptr_t>(a->cache_scale) % 8 != 0 || a->scale_stride[0] % 2 != 0 ||
-               a->scale_stride[1] % 2 != 0 || !near(a->scale_stride[1])))
+    if (f8 && (!scale_rows_ok(a->cache_scale, a->scale_stride) || !near(a->scale_stride[1])))
         return KDA_ERR_UNSUPPORTED;
     return kda::mla_absorbed_launch(*a, static_cast<hipStream_t>(stream));
 }
@@ -139,8 +145,7 @@ int kda_mla_cache_append(const kda_mla_append_args* a, void* stream) {
         return KDA_ERR_UNSUPPORTED;
     // distinct rows of the cache, so that no two waves write one
     if (!distinct(a->cache_stride, a->B, a->S, a->R + a->P)) return KDA_ERR_UNSUPPORTED;
-    if (f8 && (reinterpret_cast<uintptr_t>(a->cache_scale) % 8 != 0 || a->scale_stride[0] % 2 != 0 ||
-               a->scale_stride[1] % 2 != 0 || !distinct(a->scale_stride, a->B, a->S, 2)))
+    if (f8 && (!scale_rows_ok(a->cache_scale, a->scale_stride) || !distinct(a->scale_stride, a->B, a->S, 2)))
         return KDA_ERR_UNSUPPORTED;
     return kda::mla_append_launch(*a, static_cast<hipStream_t>(stream));
 }
@@ -152,8 +157,7 @@ int kda_mla_cache_read(const kda_mla_read_args* a, void* stream) {
     if ((a->R != 128 && a->R != 256 && a->R != 512) || !pos_ok(a->P)) return KDA_ERR_UNSUPPORTED;
     if (a->B == 0 || a->S == 0) return KDA_OK;
     if (!a->cache || !a->cache_scale || !a->out) return KDA_ERR_NULL_POINTER;
-    if (!rows_ok(a->cache, a->cache_stride, 2, 1) || !at16(a->out) ||
-        reinterpret_cast<uintptr_t>(a->cache_scale) % 8 != 0 || a->scale_stride[0] % 2 != 0 || a->scale_stride[1] % 2 != 0)
+    if (!rows_ok(a->cache, a->cache_stride, 2, 1) || !at16(a->out) || !scale_rows_ok(a->cache_scale, a->scale_stride))
         return KDA_ERR_UNSUPPORTED;
     const int64_t D = a->R + a->P;
     if (!apart(a->out, a->B * a->S * D * 2, a->cache, (a->B - 1) * a->cache_stride[0] + (a->S - 1) * a->cache_stride[1] + D))

@@ -491,7 +491,7 @@ int kda_output_bwd(const kda_output_bwd_args* args, void* stream);
  * heads share.  A cache holds a token as one row [latent R | position P].
  *
  * All four entry points: pointers on the current device, last dimensions
- * contiguous, strides in elements; rows 16-byte aligned (base and strides);
+ * contiguous, strides in elements, none negative; rows 16-byte aligned (base and strides);
  * outputs overlap no input; asynchronous on `stream`, nothing allocated,
  * nothing read back, capturable.  Workspaces are the caller's, 16-byte
  * aligned; calls that may overlap in time need one each.  lengths, starts and

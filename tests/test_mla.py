@@ -179,6 +179,27 @@ def test_append_wants_distinct_rows(native):
     assert lib.kda_mla_expanded_fwd(ctypes.byref(a), None) == 2
 
 
+def test_negative_scale_strides(native):
+    """Strides of the scales may not be negative: the kernels form unsigned offsets from them."""
+    lib = native.load()
+    for stride in ((16, -2), (-16, 2)):
+        a = native.KdaMlaAbsorbedArgs(B=2, T=1, H=2, S=8, R=128, P=32, scale=0.1, dtype=native.DTYPE_F16,
+                                      cache_dtype=native.DTYPE_E4M3)
+        for f in ("q", "cache", "cache_scale", "lengths", "o", "workspace"):
+            setattr(a, f, FAKE)
+        fill(a, {"q_stride": (320, 320, 160), "cache_stride": (1280, 160), "scale_stride": stride})
+        assert lib.kda_mla_absorbed_fwd(ctypes.byref(a), None) == 4
+        r = native.KdaMlaReadArgs(B=2, S=8, R=128, P=32, out_dtype=native.DTYPE_BF16, cache=FAKE, cache_scale=FAKE,
+                                  out=FAKE * 4)
+        fill(r, {"cache_stride": (1280, 160), "scale_stride": stride})
+        assert lib.kda_mla_cache_read(ctypes.byref(r), None) == 4
+        w = native.KdaMlaAppendArgs(B=2, T=1, S=8, R=128, P=32, x_dtype=native.DTYPE_BF16, cache_dtype=native.DTYPE_E4M3)
+        for f in ("x", "cache", "cache_scale", "lengths"):
+            setattr(w, f, FAKE)
+        fill(w, {"x_stride": (160, 160), "cache_stride": (1280, 160), "scale_stride": stride})
+        assert lib.kda_mla_cache_append(ctypes.byref(w), None) == 4
+
+
 def test_wrapper_refuses_cpu_tensors(kda_pkg):
     q, k, pe = torch.zeros(1, 2, 2, 96, dtype=torch.bfloat16), torch.zeros(1, 2, 2, 64, dtype=torch.bfloat16), \
         torch.zeros(1, 2, 32, dtype=torch.bfloat16)
