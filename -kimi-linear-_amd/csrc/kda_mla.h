@@ -19,6 +19,19 @@ constexpr float kLog2E = 1.4426950408889634f;
 // and not a NaN.
 constexpr float kNoMax = -1e30f;
 
+// A row's weights are formed as 2^(s' - reference), s' its scores times log2(e), and go into
+// the value product in the activation type.  In bf16 the reference is the largest score.  In
+// fp16, whose values end at 2^-14 (2^-24 with fewer and fewer bits), it is 2^15 below it: a
+// weight keeps its 11 bits down to 2^-29 of the largest and something of itself down to 2^-39.
+// Without that room a token that takes nearly all of a row's weight and has zeros in its
+// values takes the others' share with it (18 nats above 4096 others: 95 % of the output lost).
+// Beyond 2^20, where the difference of 15 is rounded, there is none.
+template <typename T>
+__device__ __forceinline__ float reference(float largest) {
+    if constexpr (Elem<T>::code == KDA_DTYPE_F16) return fabsf(largest) < 0x1p20f ? largest - 15.f : largest;
+    else return largest;
+}
+
 template <typename T> struct Act;
 template <> struct Act<_Float16> {
     // 16x16 tile, depth 32: lane l has row/column l % 16 and the k slots 8 (l / 16) on;

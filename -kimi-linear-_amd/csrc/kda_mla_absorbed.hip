@@ -2,7 +2,7 @@
 // the cache itself, whose rows are keys and (their first R channels) values.
 //
 //   s_mj = scale q_m . c_j,   o_m = sum_j 2^(s'_mj - M_m) c_j[0:R] / sum_j 2^(s'_mj - M_m),
-//   s' = s log2(e),  M a running maximum.
+//   s' = s log2(e),  M a running maximum (in fp16 less 15).
 //
 // Bound by reading the cache: 16 heads of one token make 2 (2R + P) 16 flops of
 // each row's 2 (R + P) bytes, 30 a byte.  So each row is read from memory once,
@@ -23,9 +23,10 @@
 //
 // In 8 bits a value is widened to the activation type exactly; a key's scale
 // multiplies its score, and enters the value product through the exponent,
-// 2^(s' + log2 scale - M), so that P keeps its full precision in 16 bits at any
-// scale.  M is then the largest of the sums, and the terms of the softmax's
-// denominator are divided by the scale again.
+// 2^(s' + log2 scale - M), so that P keeps its full precision in 16 bits whatever
+// the scales' size (in fp16 down to 2^-29 of the largest: reference).  M is then the
+// largest of the sums, and the terms of the softmax's denominator are divided by the
+// scale again.
 //
 // At 16 heads, R=512 P=64 (a copy reaches 4.8 TB/s): B=64 of 8192 tokens 115 us
 // (5.2 TB/s), of 64 to 4096 tokens 41 us from HBM, in 8 bits 64 to 8192 44 us, with
@@ -258,7 +259,7 @@ struct Kernel {
         lds_barrier();
 
         uint4 p[kWindow / 32];
-        float x[kWindow / 32][8], mx = st.top;
+        float x[kWindow / 32][8], mx = kNoMax;
 #pragma unroll
         for (int k = 0; k < kWindow / 32; ++k) {
             const f4* from = reinterpret_cast<const f4*>(&sh.s[ln][32 * k + 8 * lg]);
@@ -270,7 +271,7 @@ struct Kernel {
                 mx = fmaxf(mx, fmaxf(lo4[e], hi4[e]));
             }
         }
-        mx = lanegroup4_max(mx);
+        mx = fmaxf(st.top, reference<T>(lanegroup4_max(mx)));
         const float alpha = __builtin_amdgcn_exp2f(st.top - mx);
         st.top = mx;
         float part = 0.f;

@@ -2,7 +2,7 @@
 // are a head's own N channels and P position channels that all heads share.
 //
 //   s_tj = scale q_t . [k_j | k_pe_j],  o_t = sum_j 2^(s'_tj - M_t) v_j / sum_j 2^(s'_tj - M_t),
-//   s' = s log2(e),  M a running maximum.
+//   s' = s log2(e),  M a running maximum (in fp16 less 15).
 //
 // Bound by the matrix cores: 2 (N + P + V) flops a visible pair.  At 128 + 64
 // channels, bf16, H=16: 1110 TFLOP/s at T=16384, 930 for T=2048 over 16384 keys,
@@ -16,8 +16,8 @@
 // rounded, are the second operand of the value product O^T = V^T P^T as they
 // lie, in an order of the keys that the transposed reads of V follow.  O^T's
 // columns are rows again, so a new maximum rescales a lane's own registers;
-// it does so only when the maximum has grown by more than 2^8 (P stays below
-// 2^8, exact range for both types), the sums are exact either way.
+// in bf16 it does so only when the maximum has grown by more than 2^8 (P stays
+// below 2^8); fp16 has its room below the maximum (reference) and 2^0.75 above.
 //
 // Few rows over many keys: several workgroups share the keys of a query tile,
 // each leaves its sums in the workspace, and a second kernel joins them.
@@ -35,7 +35,8 @@ namespace {
 
 using namespace mla;
 
-constexpr float kLazy = 8.f;          // log2 of how far a maximum may lag
+// log2 of how far a maximum may lag: in fp16 what there is between 2^15 and its largest value
+template <typename T> constexpr float kLazy = Elem<T>::code == KDA_DTYPE_F16 ? 0.75f : 8.f;
 
 // The workspace of shared keys: every row's parts, [rows][splits][V] sums and
 // their (maximum, denominator).
@@ -138,8 +139,8 @@ __global__ __launch_bounds__(64 * RW * KW, RW * KW == 8 ? 2 : 1) void expanded_k
                 for (int u = 0; u < kU; ++u)
 #pragma unroll
                     for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[u][e]);
-                mx = half_max(mx) * c;
-                if (__any(mx > top + kLazy)) {
+                mx = reference<T>(half_max(mx) * c);
+                if (__any(mx > top + kLazy<T>)) {
                     const float now = fmaxf(top, mx), alpha = __builtin_amdgcn_exp2f(top - now);
                     top = now;
                     sum *= alpha;

@@ -671,3 +671,44 @@ def test_run_together(kda_pkg, bits):
         n = int(lengths[0])
         assert n == 64 + t
         close("token", out, *absorbed_ref(q_in, held(), [n] * B, R, scale))
+
+
+# ---- a token that takes nearly all of the weight ----------------------------
+
+@pytest.mark.parametrize("gap", [16.0, 20.0])
+@pytest.mark.parametrize("B,T,S,at", [(1, 1, 4097, 0), (1, 70, 4097, 1000), (2, 300, 300, 0), (1, 20, 20, 0), (4, 520, 520, 3)])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_expanded_sink(kda_pkg, dtype, B, T, S, at, gap):
+    """One key scores `gap` nats above all others and its values are zero in half of the channels: what the others
+    leave there, each with a weight of 2^-23 to 2^-29, is kept to the types' precision."""
+    H, N, P, scale = 2, 64, 32, 0.1
+    q, kn, pe, v = inputs(B, T, S, H, N, P, dtype, seed=70)
+    q, kn, pe, v = 0.3 * q, 0.3 * kn, 0.3 * pe, 30 * v.abs() + 30
+    q[..., 0], kn[..., 0], kn[:, at, :, 0] = 8.0, 0.0, gap / (8 * scale)
+    v[:, at, :, ::2] = 0
+    d_o = rand(B, T, H, N, seed=75, dtype=dtype)
+    leaves = [x.requires_grad_() for x in (q, kn, pe, v)]
+    o = kda_pkg.mla_expanded(q, kn, pe, v, scale=scale)
+    grads = torch.autograd.grad(o, leaves, d_o)
+    with torch.no_grad():
+        want, bound, ref = expanded_ref(q, kn, pe, v, [S] * B, [S - T] * B, scale, d_o)
+    close("o", o, want, bound)
+    for m, g in zip(("q", "k_nope", "k_pe", "v"), grads):
+        close("d" + m, g, *ref[m])
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+@pytest.mark.parametrize("gap", [16.0, 20.0])
+@pytest.mark.parametrize("B,T,H,S,at", [(1, 1, 16, 4097, 0), (3, 2, 4, 400, 130), (70, 1, 16, 1000, 7)])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_absorbed_sink(kda_pkg, dtype, B, T, H, S, at, gap, bits):
+    R, P, scale = 128, 32, 0.1
+    q = rand(B, T, H, R + P, seed=76, dtype=dtype, std=0.01)
+    rows = rand(B, S, R + P, seed=77, dtype=torch.float32)
+    rows[..., :R] = 30 * rows[..., :R].abs() + 30
+    q[..., R], rows[..., R], rows[:, at, R] = 8.0, 0.0, gap / (8 * scale)
+    rows[:, at, :R:2] = 0
+    cache, sc = (rows.to(dtype), None) if bits == 16 else quantised(rows, R)
+    held = cache.double() if bits == 16 else dequantised(cache, sc, R)
+    got = kda_pkg.mla_absorbed(q, cache, i32([S] * B), R, scale, cache_scale=sc)
+    close("o", got, *absorbed_ref(q, held, [S] * B, R, scale))
