@@ -14,7 +14,7 @@ from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "libkda_hip.so"
 HOST_PATH = Path(__file__).resolve().parent / "_kda_host.so"     # csrc/host_binding.cpp
-ABI_VERSION = 16
+ABI_VERSION = 17
 
 DTYPE_F32 = 0
 DTYPE_F16 = 1
@@ -157,7 +157,7 @@ class KdaMlaExpandedArgs(ctypes.Structure):
         ("k_pe", ctypes.c_void_p), ("k_pe_stride", ctypes.c_int64 * 2), ("v", ctypes.c_void_p), ("v_stride", _i64x3),
         ("lengths", ctypes.c_void_p), ("starts", ctypes.c_void_p),
         ("o", ctypes.c_void_p), ("lse", ctypes.c_void_p), ("o_low", ctypes.c_void_p), ("scale", ctypes.c_float), ("dtype", ctypes.c_int32),
-        ("workspace", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p), ("lse_low", ctypes.c_void_p),
     ]
 
 

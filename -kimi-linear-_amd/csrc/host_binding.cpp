@@ -600,7 +600,10 @@ kda_mla_expanded_args expanded_args(const Tensor& q, const Tensor& k, const OptT
     a.lengths = counts_ptr(lengths);
     a.starts = counts_ptr(starts);
     a.o = o.data_ptr();
-    a.lse = lse ? static_cast<float*>(lse->data_ptr()) : nullptr;
+    if (lse) {                                       // [2, B, H, T]: lse and what its rounding took
+        a.lse = static_cast<float*>(lse->data_ptr());
+        a.lse_low = a.lse + a.B * a.H * a.T;
+    }
     a.o_low = low ? low->data_ptr() : nullptr;
     a.scale = static_cast<float>(scale);
     a.dtype = code(q);
@@ -613,7 +616,7 @@ bool expanded_forward(const Tensor& q, const Tensor& k, const OptTensor& k_pe, c
     const int status = run(q.device(), [&](void* stream) -> int {
         const auto opt = q.options().requires_grad(false);
         o = at::empty({q.size(0), q.size(1), q.size(2), v.size(3)}, opt);
-        if (lse) *lse = at::empty({q.size(0), q.size(2), q.size(1)}, opt.dtype(at::kFloat));
+        if (lse) *lse = at::empty({2, q.size(0), q.size(2), q.size(1)}, opt.dtype(at::kFloat));
         if (low) *low = at::empty(o.sizes(), opt);
         auto a = expanded_args(q, k, k_pe, v, lengths, starts, scale, o, lse, low);
         const size_t bytes = fn.mla_expanded_ws(a.B, a.T, a.S, a.H, a.V);

@@ -14,10 +14,17 @@ typedef float f16v __attribute__((ext_vector_type(16)));
 typedef short s4 __attribute__((ext_vector_type(4)));
 
 constexpr float kLog2E = 1.4426950408889634f;
-// A maximum that no score has been compared with yet: finite, so that a row
-// whose keys are all masked (scores of -inf) has exp2(-inf - max) = 0 terms
-// and not a NaN.
-constexpr float kNoMax = -1e30f;
+// A maximum that no score has been compared with yet: no score is below it, and it is
+// finite, so that a row whose keys are all masked (scores of -inf) has
+// exp2(-inf - max) = 0 terms and not a NaN.
+constexpr float kNoMax = -0x1.fffffep127f;
+// A fused s c - reference keeps what rounding took from the reference itself, up to
+// 2^-24 of it; for references past this (the rest is 2^-8 here) the product is rounded
+// first, as the reference was, so that the largest score's weight is 1 at any magnitude.
+constexpr float kFar = 0x1p16f;
+__device__ __forceinline__ bool far_from_zero(float reference) {
+    return fabsf(reference) > kFar && fabsf(reference) < -kNoMax;
+}
 
 // A row's weights are formed as 2^(s' - reference), s' its scores times log2(e), and go into
 // the value product in the activation type.  In bf16 the reference is the largest score.  In
@@ -106,6 +113,14 @@ __device__ __forceinline__ void store_out(T* out, T* low, f4 x) {
         *reinterpret_cast<uint2*>(low) = uint2{Act<T>::pair(x[0] - Elem<T>::ld(&e[0]), x[1] - Elem<T>::ld(&e[1])),
                                                Act<T>::pair(x[2] - Elem<T>::ld(&e[2]), x[3] - Elem<T>::ld(&e[3]))};
     }
+}
+
+// log2 of a row's sum of exp(s) from its reference and the sum against it, with what rounding takes
+// from it (+inf for a row without keys).
+__device__ __forceinline__ void store_lse(float* lse, float* low, int64_t row, float top, float sum) {
+    const float rest = __builtin_amdgcn_logf(sum), x = sum == 0.f ? INFINITY : top + rest;
+    lse[row] = x;
+    if (low) low[row] = sum == 0.f ? 0.f : fabsf(top) > fabsf(rest) ? (top - x) + rest : (rest - x) + top;
 }
 
 // Largest x over the four lanes that share l & 15.

@@ -95,6 +95,7 @@ __global__ __launch_bounds__(64 * RW * KW, RW * KW == 8 ? 2 : 1) void expanded_k
 #pragma unroll
         for (int e = 0; e < 16; ++e) o[i][e] = 0.f;
     float top = kNoMax, sum = 0.f;
+    bool far = false;                                             // some row's top is far from zero
 
     if (keys > first) {
         uint4 q[D / 16];
@@ -143,11 +144,20 @@ __global__ __launch_bounds__(64 * RW * KW, RW * KW == 8 ? 2 : 1) void expanded_k
                 if (__any(mx > top + kLazy<T>)) {
                     const float now = fmaxf(top, mx), alpha = __builtin_amdgcn_exp2f(top - now);
                     top = now;
+                    far = __any(far_from_zero(top));
                     sum *= alpha;
 #pragma unroll
                     for (int i = 0; i < V / 32; ++i)
 #pragma unroll
                         for (int e = 0; e < 16; ++e) o[i][e] *= alpha;
+                }
+                float m = c;
+                if (far) {
+#pragma unroll
+                    for (int u = 0; u < kU; ++u)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) s[u][e] *= c;
+                    m = 1.f;
                 }
                 uint4 p[2 * kU], left[FEW ? 2 * kU : 1];
 #pragma unroll
@@ -155,8 +165,8 @@ __global__ __launch_bounds__(64 * RW * KW, RW * KW == 8 ? 2 : 1) void expanded_k
                     uint32_t w[4], l[4];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const float x = __builtin_amdgcn_exp2f(fmaf(s[u / 2][8 * (u % 2) + 2 * e], c, -top));
-                        const float y = __builtin_amdgcn_exp2f(fmaf(s[u / 2][8 * (u % 2) + 2 * e + 1], c, -top));
+                        const float x = __builtin_amdgcn_exp2f(fmaf(s[u / 2][8 * (u % 2) + 2 * e], m, -top));
+                        const float y = __builtin_amdgcn_exp2f(fmaf(s[u / 2][8 * (u % 2) + 2 * e + 1], m, -top));
                         sum += x;
                         sum += y;
                         w[e] = Act<T>::pair(x, y);
@@ -245,8 +255,7 @@ __global__ __launch_bounds__(64 * RW * KW, RW * KW == 8 ? 2 : 1) void expanded_k
         for (int e = 0; e < 4; ++e)
             store_out(out + 32 * i + 8 * e, low ? low + 32 * i + 8 * e : nullptr,
                       f4{o[i][4 * e] * norm, o[i][4 * e + 1] * norm, o[i][4 * e + 2] * norm, o[i][4 * e + 3] * norm});
-    if (a.lse && half == 0)
-        a.lse[(b * a.H + h) * a.T + t] = sum == 0.f ? INFINITY : top + __builtin_amdgcn_logf(sum);
+    if (a.lse && half == 0) store_lse(a.lse, a.lse_low, (b * a.H + h) * a.T + t, top, sum);
 }
 
 // The parts of a row joined in order: V / 4 lanes a row.
@@ -276,7 +285,7 @@ __global__ __launch_bounds__(256) void join_kernel(kda_mla_expanded_args a, int 
     const int64_t to = ((b * a.T + t) * a.H + h) * V + ch;
     store_out(static_cast<T*>(a.o) + to, a.o_low ? static_cast<T*>(a.o_low) + to : nullptr,
               f4{r[0] * norm, r[1] * norm, r[2] * norm, r[3] * norm});
-    if (a.lse && ch == 0) a.lse[row] = sum == 0.f ? INFINITY : top + __builtin_amdgcn_logf(sum);
+    if (a.lse && ch == 0) store_lse(a.lse, a.lse_low, row, top, sum);
 }
 
 // Workgroups that share the keys of a query tile of 64 rows: where there are too

@@ -22,6 +22,10 @@
 // fp16: p is formed times 2^12 and ds times a power of two that follows its
 // magnitude (per row in dq, per wave in dk), so neither long contexts nor
 // small gradients fall below fp16's range; bf16 needs neither.
+//
+// Where lse is past 2^16 the scaled score is rounded first here too (kFar), and what
+// lse's own rounding took is subtracted as well: keys that share a row's weight at
+// such scores would have all of it each otherwise.
 #include <hip/hip_runtime.h>
 
 #include "kda_launch.h"
@@ -143,7 +147,9 @@ __global__ __launch_bounds__(64 * RW * KW, 2) void dq_kernel(kda_mla_expanded_bw
         }
         dl = half_sum(dl);
         if (live && half == 0 && group == 0) delta[bh * a.T + t] = dl;
-        const float lse = (live ? a.lse[bh * a.T + t] : INFINITY) - kPShift<T>;
+        float lse = live ? a.lse[bh * a.T + t] : INFINITY;
+        const bool far = __any(far_from_zero(lse));
+        if (!far) lse -= kPShift<T>;
 
         F tile(a, at.b, at.h);
         tile.fetch(a, 0, keys);
@@ -169,10 +175,20 @@ __global__ __launch_bounds__(64 * RW * KW, 2) void dq_kernel(kda_mla_expanded_bw
                     for (int e = 0; e < 16; ++e)
                         if (jw + 8 * (e / 4) + 4 * half + e % 4 > limit) s[e] = -INFINITY;
                 }
-                float m = 0.f;
+                float m = 0.f, by = c, less = lse;
+                if (far) {
+#pragma clang fp contract(off)
+                    int r = static_cast<int>(__lane_id()) & 31;
+                    asm volatile("" : "+v"(r));                   // read here, for no register to be kept for it
+                    const float low = a.lse_low ? a.lse_low[bh * a.T + min(w0 + r, at.exist - 1)] : 0.f;
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) s[e] = s[e] * c - lse - low;
+                    by = 1.f;
+                    less = -kPShift<T>;
+                }
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
-                    dp[e] = __builtin_amdgcn_exp2f(fmaf(s[e], c, -lse)) * (dp[e] - dl);
+                    dp[e] = __builtin_amdgcn_exp2f(fmaf(s[e], by, -less)) * (dp[e] - dl);
                     if constexpr (kHalf<T>) m = fmaxf(m, fabsf(dp[e]));
                 }
                 if constexpr (kHalf<T>) {
@@ -292,7 +308,10 @@ __global__ __launch_bounds__(512, 2) void dkv_kernel(kda_mla_expanded_bwd_args g
     // (128 queries of 128 + 64 channels took 46 registers to scratch memory: T=1000 48 us, 32 without)
     constexpr bool kEarly = KG == 4 || N == 64;
     __shared__ __align__(16) char raw[F::kBytes];
-    __shared__ __align__(16) float stats[2][kPass];               // lse and delta of a step's queries
+    // lse, delta and lse's rest of a step's queries; where one of 64 has an lse far from zero, zeros are in
+    // its place and it is the last
+    __shared__ __align__(16) float stats[4][kPass];
+    __shared__ int fars[kPass / 64];
     T* ks = reinterpret_cast<T*>(raw);
     T* vs = ks + kStand * kK;
     T* qs = vs + kStand * kV;
@@ -320,7 +339,9 @@ __global__ __launch_bounds__(512, 2) void dkv_kernel(kda_mla_expanded_bwd_args g
     if (j0 < at.len && first < at.exist) {
         const T* qb = static_cast<const T*>(a.q) + at.b * a.q_stride[0] + at.h * a.q_stride[2];
         const T* ob = static_cast<const T*>(g.d_o) + at.b * g.d_o_stride[0] + at.h * g.d_o_stride[2];
-        const float* sb = (threadIdx.x & kPass ? delta : a.lse) + bh * a.T;
+        // kPass threads on each of lse, delta and lse's rest (the others repeat them)
+        const int what = wave / (kPass / 64);
+        const float* sb = (what & 1 ? delta : what == 2 && a.lse_low ? a.lse_low : a.lse) + bh * a.T;
         constexpr int kP = D % 64 == 0 ? 0 : 32;                     // so that each part is whole rounds of the threads
         Rows<T, kPass, D - kP, F::NT, kK> q;
         Rows<T, kPass, kP, F::NT, kK> qp;
@@ -341,9 +362,17 @@ __global__ __launch_bounds__(512, 2) void dkv_kernel(kda_mla_expanded_bwd_args g
             q.put(qs);
             qp.put(qs + D - kP);
             d_o.put(os);
-            if (threadIdx.x < 2 * kPass) {
-                const bool there = t0 + static_cast<int>(threadIdx.x & (kPass - 1)) < at.exist;
-                (&stats[0][0])[threadIdx.x] = threadIdx.x & kPass ? (there ? x : 0.f) : (there ? x - kPShift<T> : INFINITY);
+            if (what < 3) {
+                const int i = threadIdx.x & (kPass - 1);
+                const bool there = t0 + i < at.exist;
+                float y = there ? x : 0.f;
+                if (what == 0) {
+                    const bool far = __any(there && far_from_zero(x));
+                    if (far) stats[3][i] = there ? x : INFINITY;
+                    if (lane == 0) fars[wave] = far;
+                    y = there ? (far ? 0.f : x) - kPShift<T> : INFINITY;
+                }
+                stats[what][i] = what == 2 && !a.lse_low ? 0.f : y;
             }
         };
         fetch(first);
@@ -389,6 +418,18 @@ __global__ __launch_bounds__(512, 2) void dkv_kernel(kda_mla_expanded_bwd_args g
                 }
                 float m = 0.f;
                 const float* st = &stats[0][32 * side + 4 * half];
+                if (__builtin_amdgcn_readfirstlane(fars[32 * side / 64])) {
+#pragma clang fp contract(off)
+                    // in place, for the product with c below: the common path stays as it is
+                    float opaque = c;
+                    asm volatile("" : "+v"(opaque));      // (and forms nothing of this ahead, in registers)
+                    const float back = __builtin_amdgcn_rcpf(opaque);
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const float* far = st + 2 * kPass + 8 * (e / 4) + e % 4;
+                        s[e] = (s[e] * opaque - far[kPass] - far[0]) * back;
+                    }
+                }
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {
                     const f4 l = *reinterpret_cast<const f4*>(st + 8 * u), d = *reinterpret_cast<const f4*>(st + kPass + 8 * u);

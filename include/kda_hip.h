@@ -39,7 +39,7 @@
 extern "C" {
 #endif
 
-#define KDA_ABI_VERSION 16
+#define KDA_ABI_VERSION 17
 
 /* Element types accepted at the boundary. */
 typedef enum kda_dtype {
@@ -504,7 +504,8 @@ int kda_output_bwd(const kda_output_bwd_args* args, void* stream);
  * A query at or past position lengths[b] does not exist: its output is zero,
  * as is that of a row with no key.  Rows of k, k_pe and v at or past
  * lengths[b] are never read.  lengths NULL: S; starts NULL: S - T.
- * Products in the activation type with fp32 sums, softmax in fp32. */
+ * Products in the activation type with fp32 sums, softmax in fp32 (scores of
+ * any finite size; a weight is as exact as its score, to 2^-24 of that). */
 typedef struct kda_mla_expanded_args {
     int64_t B, T, S, H, N, P, V;   /* N = V in {64, 128}; P in {0, 32, 64} */
     const void* q;                 /* [B, T, H, N+P] */
@@ -524,6 +525,8 @@ typedef struct kda_mla_expanded_args {
     float scale;
     int32_t dtype;                 /* KDA_DTYPE_F16 or KDA_DTYPE_BF16, of all activations */
     void* workspace;               /* forward: kda_mla_expanded_workspace_size() bytes (0 for most shapes) */
+    float* lse_low;                /* [B, H, T] or NULL: what rounding took from lse.  The backward uses it where
+                                    * |lse| > 2^16 (NULL: zeros) */
 } kda_mla_expanded_args;
 
 size_t kda_mla_expanded_workspace_size(int64_t B, int64_t T, int64_t S, int64_t H, int64_t V);

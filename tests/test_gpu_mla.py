@@ -712,3 +712,61 @@ def test_absorbed_sink(kda_pkg, dtype, B, T, H, S, at, gap, bits):
     held = cache.double() if bits == 16 else dequantised(cache, sc, R)
     got = kda_pkg.mla_absorbed(q, cache, i32([S] * B), R, scale, cache_scale=sc)
     close("o", got, *absorbed_ref(q, held, [S] * B, R, scale))
+
+
+# ---- scores far from zero ---------------------------------------------------
+
+def steps(shape, at):
+    """1, 1 + 2^-7 .. 2 - 2^-7 along dimension `at`, in a shuffled order: what a bf16 mantissa holds."""
+    n = shape[at]
+    m = 1 + (torch.arange(n, device=DEV, dtype=torch.float64) * 37 % 128) / 128
+    return m.view([-1 if d == at else 1 for d in range(len(shape))]).expand(shape)
+
+
+FAR = [(BF16, -60, 43), (BF16, 60, 43), (BF16, -60, 66), (BF16, 60, 66), (F16, 15, 14), (F16, -15, 14), (F16, -12, 10),
+       (BF16, 17, 0), (BF16, -17, 0)]
+
+
+@pytest.mark.parametrize("dtype,a,b", FAR, ids=lambda x: str(x)[6:] if isinstance(x, torch.dtype) else str(x))
+@pytest.mark.parametrize("B,T,S,H", [(1, 20, 20, 2), (2, 300, 300, 3), (1, 70, 2100, 2), (2, 150, 400, 1), (8, 520, 520, 16)])
+def test_expanded_far_scores(kda_pkg, B, T, S, H, dtype, a, b):
+    """Scores of one sign and up to 2^126 in size, all far from zero: finite, so a row's largest takes the weight,
+    shared evenly by the keys that have it.  The products are exact, and weights other than these below 2^-700."""
+    if B == 8 and b not in (43, 14):
+        pytest.skip("one magnitude a type for the widest workgroups")
+    N, P = 64, 32
+    q, kn, pe, v = inputs(B, T, S, H, N, P, dtype, seed=90)
+    q.zero_()
+    q[..., 0] = float((1 if a > 0 else -1) * 2.0 ** abs(a))
+    kn[..., 0] = (steps((B, S, H), 1) * 2.0 ** b).to(dtype)
+    d_o = rand(B, T, H, N, seed=95, dtype=dtype)
+    leaves = [x.requires_grad_() for x in (q, kn, pe, v)]
+    o = kda_pkg.mla_expanded(q, kn, pe, v, scale=1.0)
+    grads = torch.autograd.grad(o, leaves, d_o)
+    with torch.no_grad():
+        want, bound, ref = expanded_ref(q, kn, pe, v, [S] * B, [S - T] * B, 1.0, d_o)
+    close("o", o, want, bound)
+    for m, g in zip(("q", "k_nope", "k_pe", "v"), grads):
+        r, e = ref[m]
+        if torch.finfo(dtype).max < 1e5:                 # fp16: a bound past its largest value allows any
+            inside = (r.abs() + e) < torch.finfo(dtype).max
+            g, r, e = torch.where(inside, g.double(), 0), torch.where(inside, r, 0), torch.where(inside, e, 0)
+        close("d" + m, g, r, e)
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+@pytest.mark.parametrize("dtype,a,b", FAR, ids=lambda x: str(x)[6:] if isinstance(x, torch.dtype) else str(x))
+@pytest.mark.parametrize("B,T,H,S", [(1, 1, 16, 100), (2, 3, 4, 1000), (70, 1, 16, 600)])
+def test_absorbed_far_scores(kda_pkg, B, T, H, S, dtype, a, b, bits):
+    R, P = 128, 32
+    q = torch.zeros(B, T, H, R + P, dtype=dtype, device=DEV)
+    q[..., R] = float((1 if a > 0 else -1) * 2.0 ** abs(a))
+    rows = rand(B, S, R + P, seed=96, dtype=torch.float32)
+    rows[..., R:] = 0
+    rows[..., R] = (steps((B, S), 1) * 2.0 ** b).float()
+    rows[..., 0] = 8.0                       # one latent scale: its logarithm is part of an 8-bit cache's scores
+    cache, sc = (rows.to(dtype), None) if bits == 16 else quantised(rows, R)
+    held = cache.double() if bits == 16 else dequantised(cache, sc, R)
+    got = kda_pkg.mla_absorbed(q, cache, i32([S] * B), R, 1.0, cache_scale=sc)
+    want, bound = absorbed_ref(q, held, [S] * B, R, 1.0)
+    close("o", got, want, bound)
