@@ -155,9 +155,9 @@ __device__ __forceinline__ int tokens(const int32_t* lengths, int64_t b, int64_t
     return max(0, min(n, static_cast<int>(S)));
 }
 
-// Position of sequence b's first query: starts[b] clamped to [0, S], or S - T.
+// Position of sequence b's first query: starts[b] clamped to [-T, S], beyond which no query sees a key, or S - T.
 __device__ __forceinline__ int first_position(const int32_t* starts, int64_t b, int64_t S, int64_t T) {
-    return starts ? max(0, min(starts[b], static_cast<int>(S))) : static_cast<int>(S - T);
+    return starts ? max(-static_cast<int>(T), min(starts[b], static_cast<int>(S))) : static_cast<int>(S - T);
 }
 
 }  // namespace mla

@@ -56,7 +56,7 @@ bool apart(const void* a, int64_t na, const void* b, int64_t nb) {
 }
 
 int expanded_check(const kda_mla_expanded_args& a) {
-    if (!sizes_ok(a.B, a.T, a.S, a.H)) return KDA_ERR_BAD_SHAPE;
+    if (!sizes_ok(a.B, a.T, a.S, a.H) || a.T + a.S > INT32_MAX) return KDA_ERR_BAD_SHAPE;
     if (!act(a.dtype)) return KDA_ERR_BAD_DTYPE;
     if ((a.N != 64 && a.N != 128) || a.V != a.N || !pos_ok(a.P) || !scale_ok(a.scale)) return KDA_ERR_UNSUPPORTED;
     if (a.B * a.H > kMaxGrid) return KDA_ERR_BAD_SHAPE;

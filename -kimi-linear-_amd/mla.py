@@ -112,7 +112,7 @@ def mla_expanded(q, k_nope, k_pe, v, lengths=None, starts=None, scale=None):
 
     ``lengths`` (default S) are the tokens each sequence has: rows of k and v
     from there on are never read.  ``starts`` (default S - T) is the position
-    of query 0.  A query whose position is ``lengths[b]`` or more does not
+    of query 0, of either sign.  A query whose position is ``lengths[b]`` or more does not
     exist, and one below 0 or of an empty sequence sees no key: both give zeros
     (and zero gradients).  A key or value that is not finite may reach the
     queries of up to 127 positions before its own.

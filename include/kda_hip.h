@@ -502,7 +502,7 @@ int kda_output_bwd(const kda_output_bwd_args* args, void* stream);
  *   s_tj = scale (q_t[0:N] . k_j + q_t[N:N+P] . k_pe_j)
  *   o_t  = sum_j softmax_j(s_tj) v_j   over j < lengths[b], j <= starts[b] + t
  * A query at or past position lengths[b] does not exist: its output is zero,
- * as is that of a row with no key.  Rows of k, k_pe and v at or past
+ * as is that of a row with no key (one at a position below 0, say).  Rows of k, k_pe and v at or past
  * lengths[b] are never read.  lengths NULL: S; starts NULL: S - T.
  * Products in the activation type with fp32 sums, softmax in fp32 (scores of
  * any finite size; a weight is as exact as its score, to 2^-24 of that). */
@@ -517,7 +517,7 @@ typedef struct kda_mla_expanded_args {
     const void* v;                 /* [B, S, H, V] */
     int64_t v_stride[3];
     const int32_t* lengths;        /* [B] or NULL */
-    const int32_t* starts;         /* [B], >= 0, or NULL */
+    const int32_t* starts;         /* [B], of either sign, or NULL */
     void* o;                       /* [B, T, H, V] contiguous */
     float* lse;                    /* [B, H, T] or NULL: log2 of the row's sum of exp(s), +inf for a row without keys */
     void* o_low;                   /* [B, T, H, V] contiguous, or NULL: what rounding took from o, rounded itself;

@@ -770,3 +770,38 @@ def test_absorbed_far_scores(kda_pkg, B, T, H, S, dtype, a, b, bits):
     got = kda_pkg.mla_absorbed(q, cache, i32([S] * B), R, 1.0, cache_scale=sc)
     want, bound = absorbed_ref(q, held, [S] * B, R, 1.0)
     close("o", got, want, bound)
+
+
+# ---- first queries before the first key -------------------------------------
+
+@pytest.mark.parametrize("T,S", [(40, 16), (150, 20), (700, 90), (300, 299), (1200, 1100)])
+def test_expanded_negative_starts_are_the_default(kda_pkg, T, S):
+    """starts = S - T given is starts left out, in the output and the gradients, where that is below 0."""
+    xs = [x.requires_grad_() for x in inputs(2, T, S, 2, 64, 32, BF16, seed=110)]
+    d_o = rand(2, T, 2, 64, seed=115, dtype=BF16)
+
+    def call(starts):
+        o = kda_pkg.mla_expanded(*xs, starts=starts)
+        return [o, *torch.autograd.grad(o, xs, d_o)]
+
+    want = call(None)
+    assert (want[0][:, :T - S] == 0).all() and (want[0][:, T - S:] != 0).any()
+    for given in (i32([S - T] * 2), i32([S - T] * 2).long()):
+        assert all(torch.equal(a, b) for a, b in zip(call(given), want))
+
+
+@pytest.mark.parametrize("B,T,S,lengths,starts", [(3, 40, 16, [16, 9, 0], [-24, -3, -1]), (2, 300, 200, [200, 77], [-150, -299]),
+                                                  (4, 70, 1100, [1100, 30, 1100, 5], [-1, -64, 1030, -2 ** 31])])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_expanded_negative_starts(kda_pkg, B, T, S, lengths, starts, dtype):
+    H, N, P = 2, 64, 32
+    q, kn, pe, v = inputs(B, T, S, H, N, P, dtype, seed=120)
+    d_o = rand(B, T, H, N, seed=125, dtype=dtype)
+    leaves = [x.requires_grad_() for x in (q, kn, pe, v)]
+    o = kda_pkg.mla_expanded(q, kn, pe, v, lengths=i32(lengths), starts=i32(starts))
+    grads = torch.autograd.grad(o, leaves, d_o)
+    with torch.no_grad():
+        want, bound, ref = expanded_ref(q, kn, pe, v, lengths, starts, (N + P) ** -0.5, d_o)
+    close("o", o, want, bound)
+    for m, g in zip(("q", "k_nope", "k_pe", "v"), grads):
+        close("d" + m, g, *ref[m])

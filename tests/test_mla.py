@@ -200,6 +200,12 @@ def test_negative_scale_strides(native):
         assert lib.kda_mla_cache_append(ctypes.byref(w), None) == 4
 
 
+def test_expanded_positions_stay_in_32_bits(native):
+    """A query's position may be T below 0 or S past it: together they have to fit."""
+    a = expanded(native, T=2 ** 30, S=2 ** 30, H=1)
+    assert native.load().kda_mla_expanded_fwd(ctypes.byref(a), None) == 2
+
+
 def test_wrapper_refuses_cpu_tensors(kda_pkg):
     q, k, pe = torch.zeros(1, 2, 2, 96, dtype=torch.bfloat16), torch.zeros(1, 2, 2, 64, dtype=torch.bfloat16), \
         torch.zeros(1, 2, 32, dtype=torch.bfloat16)
