@@ -19,6 +19,7 @@
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 #include <torch/extension.h>
 
@@ -573,9 +574,18 @@ bool counts_ok(const OptTensor& t, int64_t B) {
 }
 const int32_t* counts_ptr(const OptTensor& t) { return t ? static_cast<const int32_t*>(t->data_ptr()) : nullptr; }
 
+// Whether a trace is being recorded.  It would see the outputs' allocations and not the
+// kernels, and hold memory that nothing fills: such calls are refused.
+bool traced() {
+    using Mode = c10::impl::TorchDispatchModeKey;
+    const auto on = [](Mode m) { return c10::impl::TorchDispatchModeTLS::get_mode(m).has_value(); };
+    return torch::jit::tracer::isTracing() || c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::PreDispatch) ||
+           on(Mode::PROXY) || on(Mode::FUNCTIONAL) || on(Mode::FAKE);
+}
+
 bool expanded_ok(const Plain& plain, const Tensor& q, const Tensor& k, const OptTensor& k_pe, const Tensor& v,
                  const OptTensor& lengths, const OptTensor& starts) {
-    if (!plain.ok || q.dim() != 4 || k.dim() != 4 || v.dim() != 4 || !half_type(q)) return false;
+    if (!plain.ok || traced() || q.dim() != 4 || k.dim() != 4 || v.dim() != 4 || !half_type(q)) return false;
     const int64_t B = q.size(0), H = q.size(2), S = k.size(1), N = k.size(3), P = k_pe ? k_pe->size(-1) : 0;
     if (!sized(k, {B, S, H, N}) || !sized(v, {B, S, H, N}) || q.size(3) != N + P) return false;
     if (k_pe && (!sized(*k_pe, {B, S, P}) || k_pe->scalar_type() != q.scalar_type() || !wide_rows(*k_pe))) return false;
@@ -683,6 +693,10 @@ struct ExpandedFn : torch::autograd::Function<ExpandedFn> {
         {
             const at::AutoGradMode off(false);
             const py::gil_scoped_acquire gil;
+            if (traced()) {
+                PyErr_SetString(error, "mla_expanded: its backward pass cannot be traced");
+                throw py::error_already_set();
+            }
             check_capture(q.device());
             const int status = run(q.device(), [&](void* stream) -> int {
                 const auto opt = q.options().requires_grad(false);
@@ -762,7 +776,7 @@ py::object mla_absorbed(const Tensor& q, const Tensor& cache, const Tensor& leng
                         const OptTensor& cache_scale) {
     Plain plain(q);
     plain.add(cache).add(lengths).add(cache_scale);
-    if (!plain.ok || q.dim() != 4 || !half_type(q) || !wide_rows(q) || !counts_ok(lengths, q.size(0)) ||
+    if (!plain.ok || traced() || q.dim() != 4 || !half_type(q) || !wide_rows(q) || !counts_ok(lengths, q.size(0)) ||
         !cache_ok(cache, cache_scale, q.size(0), q.scalar_type()) || cache.size(2) != q.size(3))
         return py::none();
     Tensor o;
@@ -802,7 +816,7 @@ bool mla_append(const Tensor& x, const Tensor& cache, const Tensor& lengths, int
                 const OptTensor& counts, const OptTensor& weight, double eps) {
     Plain plain(x);
     plain.add(cache).add(lengths).add(cache_scale).add(counts).add(weight);
-    if (!plain.ok || x.dim() != 3 || !half_type(x) || !wide_rows(x) || !counts_ok(lengths, x.size(0)) ||
+    if (!plain.ok || traced() || x.dim() != 3 || !half_type(x) || !wide_rows(x) || !counts_ok(lengths, x.size(0)) ||
         !counts_ok(counts, x.size(0)) || !cache_ok(cache, cache_scale, x.size(0), x.scalar_type()) ||
         cache.size(2) != x.size(2) || overlaps(cache, x) || (cache_scale && overlaps(*cache_scale, x)))
         return false;
@@ -837,7 +851,7 @@ py::object mla_read(const Tensor& cache, const Tensor& cache_scale, int64_t rank
                     const OptTensor& lengths) {
     Plain plain(cache);
     plain.add(cache_scale).add(lengths);
-    if (!plain.ok || cache.dim() != 3 || (dtype != at::kHalf && dtype != at::kBFloat16) ||
+    if (!plain.ok || traced() || cache.dim() != 3 || (dtype != at::kHalf && dtype != at::kBFloat16) ||
         !cache_ok(cache, cache_scale, cache.size(0), dtype) || cache.scalar_type() == dtype ||
         !counts_ok(lengths, cache.size(0)) || count < 0 || count > cache.size(1))
         return py::none();
@@ -898,5 +912,6 @@ PYBIND11_MODULE(_kda_host, m) {
     m.def("mla_absorbed", &mla_absorbed);
     m.def("mla_append", &mla_append);
     m.def("mla_read", &mla_read);
+    m.def("traced", &traced);
     m.def("params_key", &params_key);
 }

@@ -20,7 +20,7 @@ row's latent and one for its position part.  ``lengths``, ``starts`` and
 (values out of range are clamped), so a captured graph follows them.
 
 HIP tensors only, fp16 or bf16 activations, no fallback: anything else raises
-:class:`KdaError`.  Calls are asynchronous on torch's current stream and may be
+:class:`KdaError`, as do calls under a trace, ``vmap`` or forward-mode differentiation.  Calls are asynchronous on torch's current stream and may be
 captured.  Views are read in place where their channels are contiguous and
 their rows 16-byte aligned, and copied otherwise.
 """
@@ -30,6 +30,7 @@ from __future__ import annotations
 import math
 
 import torch
+from torch.autograd import forward_ad
 from torch.utils._python_dispatch import _disable_current_modes
 
 from . import _native
@@ -88,8 +89,23 @@ def _no_grad(what, *tensors):
         raise KdaError(f"{what} is forward-only: call it under torch.no_grad() or detach the inputs")
 
 
+def _refuse_transforms(name, *tensors):
+    """A trace would record an output's memory without the kernel that fills it, and a transformed tensor or a
+    subclass that dispatches for itself has no memory that the kernels could read."""
+    if _native.host().traced():
+        raise KdaError(f"{name} cannot be traced (make_fx, torch.export, torch.jit.trace, fake tensors): "
+                       "keep the call out of the traced region")
+    for x in tensors:
+        if isinstance(x, torch.Tensor) and (torch._C._functorch.is_functorch_wrapped_tensor(x)
+                                            or type(x).__torch_dispatch__ is not torch.Tensor.__torch_dispatch__):
+            raise KdaError(f"{name} takes plain tensors: no vmap or other transform, no subclass that dispatches for itself")
+        if isinstance(x, torch.Tensor) and forward_ad._current_level >= 0 and forward_ad.unpack_dual(x).tangent is not None:
+            raise KdaError(f"{name} has no forward-mode derivative")
+
+
 def _native_call(name, *args):
-    """The native call on arguments already checked and laid out."""
+    """The native call on arguments already checked and laid out.  A dispatch mode that only looks on (one that
+    counts operations, say) does not see it."""
     with _disable_current_modes():
         got = getattr(_native.host(), name)(*args)
     if got is None or got is False:
@@ -127,6 +143,7 @@ def mla_expanded(q, k_nope, k_pe, v, lengths=None, starts=None, scale=None):
         o = None
     if o is not None:
         return o
+    _refuse_transforms("mla_expanded", q, k_nope, k_pe, v, lengths, starts)
     _activations("q", q)
     _check_tensor("k_nope", k_nope)
     _check_tensor("v", v)
@@ -208,6 +225,7 @@ def mla_absorbed(q, cache, lengths, rank, scale, cache_scale=None):
         o = None
     if o is not None:
         return o
+    _refuse_transforms("mla_absorbed", q, cache, lengths, cache_scale)
     _activations("q", q)
     if q.dim() != 4:
         raise KdaError(f"q must be [B, T, H, rank + P]; got {tuple(q.shape)}")
@@ -240,6 +258,7 @@ def mla_cache_append(x, cache, lengths, rank, cache_scale=None, counts=None, nor
             return
     except TypeError:
         pass
+    _refuse_transforms("mla_cache_append", x, cache, lengths, cache_scale, counts, norm_weight)
     _activations("x", x)
     if x.dim() != 3:
         raise KdaError(f"x must be [B, T, rank + P]; got {tuple(x.shape)}")
@@ -270,6 +289,7 @@ def mla_cache_read(cache, cache_scale, rank, dtype=torch.bfloat16, tokens=None, 
         out = None
     if out is not None:
         return out
+    _refuse_transforms("mla_cache_read", cache, cache_scale, lengths)
     _check_tensor("cache", cache)
     if dtype not in _ACT:
         raise KdaError(f"dtype must be float16 or bfloat16, got {dtype}")

@@ -805,3 +805,56 @@ def test_expanded_negative_starts(kda_pkg, B, T, S, lengths, starts, dtype):
     close("o", o, want, bound)
     for m, g in zip(("q", "k_nope", "k_pe", "v"), grads):
         close("d" + m, g, *ref[m])
+
+
+# ---- what looks on, and what would record -----------------------------------
+
+def test_traces_and_transforms_are_refused(kda_pkg):
+    """A trace would hold the outputs' memory without the kernels: every call under one raises, as do batching and
+    forward-mode transforms; a mode that only looks on changes nothing."""
+    import torch.autograd.forward_ad as fwd
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from torch.utils.flop_counter import FlopCounterMode
+    R, P = 128, 32
+    q, kn, pe, v = inputs(1, 20, 20, 2, 64, 32, BF16, seed=130)
+    qa, x, n = rand(1, 1, 2, R + P, seed=131, dtype=BF16), rand(1, 3, R + P, seed=132, dtype=BF16), i32([20])
+    cache = rand(1, 40, R + P, seed=133, dtype=BF16)
+    f8, sc = quantised(cache.float(), R)
+    calls = {"expanded": (lambda t: kda_pkg.mla_expanded(t, kn, pe, v), q),
+             "absorbed": (lambda t: kda_pkg.mla_absorbed(t, cache, n, R, 0.1), qa),
+             "append": (lambda t: kda_pkg.mla_cache_append(t, cache, n, R) or t, x),
+             "read": (lambda t: kda_pkg.mla_cache_read(t, sc, R), f8)}
+    before = cache.clone()
+    for name, (call, arg) in calls.items():
+        with pytest.raises(kda_pkg.KdaError):
+            make_fx(call)(arg)
+        with pytest.raises(kda_pkg.KdaError):
+            make_fx(call, pre_dispatch=True)(arg)
+        with pytest.raises(kda_pkg.KdaError):
+            torch.jit.trace(call, arg, check_trace=False)
+        with pytest.raises(kda_pkg.KdaError):
+            with FakeTensorMode(allow_non_fake_inputs=True):
+                call(arg)
+        with pytest.raises(kda_pkg.KdaError):
+            torch.vmap(call)(torch.stack([arg, arg]))
+        if name != "read":
+            with fwd.dual_level(), pytest.raises(kda_pkg.KdaError):
+                call(fwd.make_dual(arg, torch.ones_like(arg)))
+            with pytest.raises(kda_pkg.KdaError):
+                torch.func.grad(lambda t: call(t).float().sum())(arg)
+    assert torch.equal(cache, before)
+    leaf = q.clone().requires_grad_()
+    o = kda_pkg.mla_expanded(leaf, kn, pe, v)
+    with pytest.raises(kda_pkg.KdaError, match="traced"):
+        make_fx(lambda g: torch.autograd.grad(o, leaf, g, retain_graph=True))(torch.ones_like(o))
+    want, grad = o.detach(), torch.autograd.grad(o, leaf, torch.ones_like(o))[0]
+    with FlopCounterMode(display=False):
+        o = kda_pkg.mla_expanded(leaf, kn, pe, v)
+        assert torch.equal(o, want) and torch.equal(torch.autograd.grad(o, leaf, torch.ones_like(o))[0], grad)
+        for name in ("absorbed", "read"):
+            call, arg = calls[name]
+            got = call(arg)
+            assert torch.isfinite(got.float()).all()
+        calls["append"][0](x)
+    assert not torch.equal(cache, before)
