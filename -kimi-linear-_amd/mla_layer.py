@@ -82,8 +82,8 @@ class LatentAttention(nn.Module):
         if self._up is not None and self._up[0] == key:
             return self._up[1], self._up[2]
         H, N, R = self.num_heads, self.head_dim, self.rank
-        with torch.no_grad():
-            per_head = w.view(H, 2 * N, R)
+        with torch.inference_mode(False), torch.no_grad():      # (normal tensors, which a later call may refill)
+            per_head = w.detach().view(H, 2 * N, R)
             old = self._up
             if old is not None and old[1].dtype == w.dtype and old[1].device == w.device:
                 wk, wv = old[1], old[2]
@@ -115,12 +115,14 @@ class LatentAttention(nn.Module):
 
     # ------------------------------------------------------------ the cache
     def new_state(self, B: int, device, dtype) -> dict:
-        """An empty state for B sequences."""
+        """An empty state for B sequences; of normal tensors under inference mode too, so that a later call
+        outside it can go on with the state."""
         shape = (B, self.max_tokens, self.rank + self.position_dim)
         eight = self.cache_bits == 8
-        return {"latent": torch.empty(shape, device=device, dtype=torch.float8_e4m3fn if eight else dtype),
-                "scale": torch.empty(B, self.max_tokens, 2, device=device) if eight else None,
-                "lengths": torch.zeros(B, dtype=torch.int32, device=device), "tokens": 0}
+        with torch.inference_mode(False):
+            return {"latent": torch.empty(shape, device=device, dtype=torch.float8_e4m3fn if eight else dtype),
+                    "scale": torch.empty(B, self.max_tokens, 2, device=device) if eight else None,
+                    "lengths": torch.zeros(B, dtype=torch.int32, device=device), "tokens": 0}
 
     def _room(self, state, T):
         held, most = state["tokens"], state["latent"].shape[1]

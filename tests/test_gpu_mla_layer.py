@@ -280,3 +280,27 @@ def test_decode_step_takes_one_token(kda_pkg):
                 layer.decode_step_(bad, state)
         assert state["tokens"] == 30 and state["lengths"].tolist() == [30, 30]
         assert torch.equal(state["latent"].view(torch.int16), before)
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+def test_inference_mode_then_outside(kda_pkg, bits):
+    """A state and the absorbed form's copies made under inference mode go on outside it, with weights changed
+    in between, and the other way round."""
+    layer = make(kda_pkg, torch.float16, cache_bits=bits).eval()
+    x = torch.randn(2, 60, 256, device=DEV).half()
+    with torch.inference_mode():
+        _, state = layer(x[:, :50], use_cache=True)
+        _, state = layer(x[:, 50:51], state=state, use_cache=True)
+    with torch.no_grad():
+        layer.kv_up.weight.mul_(0.5)
+        got, state = layer(x[:, 51:52], state=state, use_cache=True)
+        layer.refresh_fused_weight()
+        fresh = copy.deepcopy(layer)
+        fresh._up = None
+        _, again = fresh(x[:, :51], use_cache=True)
+        want, again = fresh(x[:, 51:52], state=again, use_cache=True)
+        assert torch.equal(got, want)
+        layer.kv_up.weight.mul_(2)
+    with torch.inference_mode():
+        layer(x[:, 52:53], state=state, use_cache=True)
+    assert state["tokens"] == 53 and state["lengths"].tolist() == [53, 53]
