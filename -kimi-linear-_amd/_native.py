@@ -14,7 +14,7 @@ from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "libkda_hip.so"
 HOST_PATH = Path(__file__).resolve().parent / "_kda_host.so"     # csrc/host_binding.cpp
-ABI_VERSION = 17
+ABI_VERSION = 18
 
 DTYPE_F32 = 0
 DTYPE_F16 = 1
@@ -195,6 +195,7 @@ class KdaMlaAppendArgs(ctypes.Structure):
         ("cache_scale", ctypes.c_void_p), ("scale_stride", ctypes.c_int64 * 2),
         ("lengths", ctypes.c_void_p), ("counts", ctypes.c_void_p), ("norm_weight", ctypes.c_void_p),
         ("eps", ctypes.c_float), ("x_dtype", ctypes.c_int32), ("cache_dtype", ctypes.c_int32),
+        ("norm_f32", ctypes.c_int32),
     ]
 
 

@@ -820,7 +820,8 @@ bool mla_append(const Tensor& x, const Tensor& cache, const Tensor& lengths, int
         !counts_ok(counts, x.size(0)) || !cache_ok(cache, cache_scale, x.size(0), x.scalar_type()) ||
         cache.size(2) != x.size(2) || overlaps(cache, x) || (cache_scale && overlaps(*cache_scale, x)))
         return false;
-    if (weight && (weight->scalar_type() != x.scalar_type() || !sized(*weight, {rank}) || !wide_rows(*weight)))
+    if (weight && ((weight->scalar_type() != x.scalar_type() && weight->scalar_type() != at::kFloat) ||
+                   !sized(*weight, {rank}) || !wide_rows(*weight)))
         return false;
     kda_mla_append_args a{};
     a.B = x.size(0); a.T = x.size(1); a.S = cache.size(1); a.R = rank; a.P = x.size(2) - rank;
@@ -835,6 +836,7 @@ bool mla_append(const Tensor& x, const Tensor& cache, const Tensor& lengths, int
     a.lengths = static_cast<const int32_t*>(lengths.data_ptr());
     a.counts = counts_ptr(counts);
     a.norm_weight = weight ? weight->data_ptr() : nullptr;
+    a.norm_f32 = weight && weight->scalar_type() == at::kFloat;
     a.eps = static_cast<float>(eps);
     a.x_dtype = code(x);
     a.cache_dtype = cache_code(cache);

@@ -137,6 +137,7 @@ int kda_mla_cache_append(const kda_mla_append_args* a, void* stream) {
     if (a == nullptr) return KDA_ERR_NULL_POINTER;
     if (!sizes_ok(a->B, a->T, a->S, 1) || (a->T > 0 && a->B > kMaxGrid / a->T)) return KDA_ERR_BAD_SHAPE;
     if (!act(a->x_dtype) || (a->cache_dtype != a->x_dtype && a->cache_dtype != KDA_DTYPE_E4M3)) return KDA_ERR_BAD_DTYPE;
+    if (a->norm_f32 != 0 && a->norm_f32 != 1) return KDA_ERR_BAD_DTYPE;
     if ((a->R != 128 && a->R != 256 && a->R != 512) || !pos_ok(a->P)) return KDA_ERR_UNSUPPORTED;
     if (a->B == 0 || a->T == 0 || a->S == 0) return KDA_OK;
     const bool f8 = a->cache_dtype == KDA_DTYPE_E4M3;

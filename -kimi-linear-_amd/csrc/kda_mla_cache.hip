@@ -28,6 +28,12 @@ __device__ __forceinline__ void load8(const T* p, float (&x)[8]) {
     for (int i = 0; i < 8; ++i) x[i] = Elem<T>::ld(&e[i]);
 }
 
+__device__ __forceinline__ void load8(const float* p, float (&x)[8]) {
+    const f4 lo = *reinterpret_cast<const f4*>(p), hi = *reinterpret_cast<const f4*>(p + 4);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = lo[i], x[4 + i] = hi[i];
+}
+
 template <typename T>
 __device__ __forceinline__ uint4 pack8(const float (&x)[8]) {
     using A = mla::Act<T>;
@@ -86,7 +92,10 @@ __global__ __launch_bounds__(64 * kRows) void append_kernel(kda_mla_append_args 
     const int64_t held = a.lengths[b], count = a.counts ? a.counts[b] : a.T;
     if (lat) load8(xr + 8 * lane, x);
     if (pos) load8(xr + R + 8 * lane, p);
-    if (lat && a.norm_weight) load8(static_cast<const T*>(a.norm_weight) + 8 * lane, w);
+    if (lat && a.norm_weight) {
+        if (a.norm_f32) load8(static_cast<const float*>(a.norm_weight) + 8 * lane, w);
+        else load8(static_cast<const T*>(a.norm_weight) + 8 * lane, w);
+    }
     const int64_t at = held + t;
     if (t >= count || held < 0 || at >= a.S) return;
     if (a.norm_weight) {

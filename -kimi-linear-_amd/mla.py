@@ -246,8 +246,8 @@ def mla_cache_append(x, cache, lengths, rank, cache_scale=None, counts=None, nor
     would fall at or past S are dropped, every other row of the cache is left
     as it is; ``lengths`` itself does not change.
 
-    With ``norm_weight [rank]`` the latent part is RMS-normalised first, in
-    fp32.  Values are rounded once to the cache's type.  In 8 bits a row's
+    With ``norm_weight [rank]`` (x's type, or taken in fp32) the latent part is
+    RMS-normalised first, in fp32.  Values are rounded once to the cache's type.  In 8 bits a row's
     latent part and its position part each get the scale max|x| / 448 (at
     least 2^-60, written to ``cache_scale``; 1 where P = 0) and x / scale is
     rounded to the nearest e4m3 value.  A row with a value that is not finite
@@ -270,7 +270,8 @@ def mla_cache_append(x, cache, lengths, rank, cache_scale=None, counts=None, nor
         _check_tensor("norm_weight", norm_weight)
         if norm_weight.numel() != rank:
             raise KdaError(f"norm_weight must have {rank} values; got {tuple(norm_weight.shape)}")
-        norm_weight = _rows(norm_weight.detach().reshape(rank).to(x.dtype))
+        norm_weight = norm_weight.detach().reshape(rank)
+        norm_weight = _rows(norm_weight if norm_weight.dtype == x.dtype else norm_weight.float())
     lengths, counts = _counts("lengths", lengths, B, x.device), _counts("counts", counts, B, x.device)
     if lengths is None:
         raise KdaError("lengths is needed: an integer tensor [B] on the device")

@@ -131,7 +131,7 @@ class LatentAttention(nn.Module):
 
     def _append(self, x, state):
         mla_cache_append(self.kv_down(x), state["latent"], state["lengths"], self.rank, cache_scale=state["scale"],
-                         norm_weight=self.kv_norm.to(x.dtype), eps=self.eps)
+                         norm_weight=self.kv_norm, eps=self.eps)
         state["lengths"].add_(x.shape[1])
 
     # ------------------------------------------------------------ the two forms

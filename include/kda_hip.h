@@ -39,7 +39,7 @@
 extern "C" {
 #endif
 
-#define KDA_ABI_VERSION 17
+#define KDA_ABI_VERSION 18
 
 /* Element types accepted at the boundary. */
 typedef enum kda_dtype {
@@ -593,10 +593,11 @@ typedef struct kda_mla_append_args {
     int64_t scale_stride[2];
     const int32_t* lengths;        /* [B] rows held before the call */
     const int32_t* counts;         /* [B] or NULL */
-    const void* norm_weight;       /* [R] contiguous, x dtype, or NULL */
+    const void* norm_weight;       /* [R] contiguous, or NULL */
     float eps;
     int32_t x_dtype;               /* KDA_DTYPE_F16 or KDA_DTYPE_BF16 */
     int32_t cache_dtype;           /* x_dtype or KDA_DTYPE_E4M3 */
+    int32_t norm_f32;              /* norm_weight: 0 x_dtype, 1 KDA_DTYPE_F32 */
 } kda_mla_append_args;
 
 int kda_mla_cache_append(const kda_mla_append_args* args, void* stream);

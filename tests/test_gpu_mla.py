@@ -858,3 +858,29 @@ def test_traces_and_transforms_are_refused(kda_pkg):
             assert torch.isfinite(got.float()).all()
         calls["append"][0](x)
     assert not torch.equal(cache, before)
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("wtype", [torch.float32, torch.float64, BF16, F16])
+def test_append_norm_weight_types(kda_pkg, wtype, dtype, bits):
+    """A norm weight of another type than x's is not rounded to x's: fp32 arithmetic, and the cache's rounding."""
+    B, T, S, R, P = 2, 5, 9, 256, 32
+    x = rand(B, T, R + P, seed=140, dtype=dtype, std=2.0)
+    w = (1 + rand(R, seed=141, std=0.3)).to(wtype)
+    cache = torch.zeros(B, S, R + P, dtype=dtype if bits == 16 else F8, device=DEV)
+    sc = None if bits == 16 else torch.ones(B, S, 2, device=DEV)
+    kda_pkg.mla_cache_append(x, cache, i32([0, 3]), R, cache_scale=sc, norm_weight=w, eps=1e-5)
+    y = x.double()
+    y[..., :R] = y[..., :R] * torch.rsqrt(y[..., :R].square().mean(-1, keepdim=True) + 1e-5) * w.double()
+    held = cache.double() if bits == 16 else dequantised(cache, sc, R)
+    for b, at in enumerate((0, 3)):
+        got, want = held[b, at:at + T], y[b]
+        if bits == 16:          # one rounding, and fp32 arithmetic (2^-21)
+            close("row", got, want, (half_step(dtype) + 2.0 ** -21) * want.abs())
+        else:                   # half a step of e4m3, and the scale's arithmetic
+            step = sc[b, at:at + T].double() * 2.0 ** -10
+            step = torch.cat([step[:, :1].expand(T, R), step[:, 1:].expand(T, P)], -1)
+            close("row", got, want, (2.0 ** -4 + 2.0 ** -20) * want.abs() + step)
+            assert ((sc[b, at:at + T, 0].double() - want[:, :R].abs().amax(-1) / 448).abs()
+                    <= 2.0 ** -20 * sc[b, at:at + T, 0]).all()

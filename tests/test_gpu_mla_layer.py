@@ -304,3 +304,19 @@ def test_inference_mode_then_outside(kda_pkg, bits):
     with torch.inference_mode():
         layer(x[:, 52:53], state=state, use_cache=True)
     assert state["tokens"] == 53 and state["lengths"].tolist() == [53, 53]
+
+
+def test_fp32_norm_weight_is_one_layer(kda_pkg):
+    """With kv_norm in fp32 the cached rows are those of the uncached path: the weight is not rounded first."""
+    layer = make(kda_pkg, torch.bfloat16).eval()
+    layer.kv_norm = nn.Parameter(1 + 0.3 * torch.randn(128, device=DEV))
+    x = torch.randn(2, 40, 256, device=DEV).bfloat16()
+    with torch.no_grad():
+        c = layer.kv_down(x)
+        lat = c.double()[..., :128]
+        want = lat * torch.rsqrt(lat.square().mean(-1, keepdim=True) + layer.eps) * layer.kv_norm.double()
+        _, state = layer(x, use_cache=True)
+        for got in (state["latent"][:, :40, :128], layer._norm(c[..., :128])):
+            # one rounding to bf16 (7 bits behind the leading one: half a step is 2^-8), and fp32 arithmetic
+            off = (got.double() - want).abs() - (torch.finfo(torch.bfloat16).eps / 2 + 2.0 ** -20) * want.abs()
+            assert off.max().item() <= 0

@@ -200,6 +200,15 @@ def test_negative_scale_strides(native):
         assert lib.kda_mla_cache_append(ctypes.byref(w), None) == 4
 
 
+def test_append_norm_weight_code(native):
+    a = native.KdaMlaAppendArgs(B=1, T=1, S=8, R=128, P=32, x_dtype=native.DTYPE_BF16, cache_dtype=native.DTYPE_BF16,
+                                norm_f32=2)
+    for f in ("x", "cache", "lengths", "norm_weight"):
+        setattr(a, f, FAKE)
+    fill(a, {"x_stride": (160, 160), "cache_stride": (1280, 160)})
+    assert native.load().kda_mla_cache_append(ctypes.byref(a), None) == 3
+
+
 def test_expanded_positions_stay_in_32_bits(native):
     """A query's position may be T below 0 or S past it: together they have to fit."""
     a = expanded(native, T=2 ** 30, S=2 ** 30, H=1)
