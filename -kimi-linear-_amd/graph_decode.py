@@ -186,7 +186,12 @@ class KdaGraphedDecoder:
             for st, n in zip(self.static_states, held):
                 if n is not None:               # a full cache is captured too: what it has no room for is dropped
                     st["tokens"] = min(n, st["latent"].shape[1] - 1)
-            self._record()
+            if torch.is_autocast_enabled("cuda"):
+                # the casts belong into the graph: autocast's own copies of the weights end with its context
+                with torch.autocast("cuda", dtype=torch.get_autocast_dtype("cuda"), cache_enabled=False):
+                    self._record()
+            else:
+                self._record()
         finally:
             for st, n in zip(self.static_states, held):
                 if n is not None:

@@ -129,10 +129,11 @@ class LatentAttention(nn.Module):
         if held + T > most:
             raise KdaError(f"the latent cache holds {held} of at most {most} tokens a sequence; {T} more do not fit")
 
-    def _append(self, x, state):
-        mla_cache_append(self.kv_down(x), state["latent"], state["lengths"], self.rank, cache_scale=state["scale"],
+    def _append(self, c, state):
+        """Appends c, ``kv_down``'s output, whose type (x's, or autocast's) is the cache's."""
+        mla_cache_append(c, state["latent"], state["lengths"], self.rank, cache_scale=state["scale"],
                          norm_weight=self.kv_norm, eps=self.eps)
-        state["lengths"].add_(x.shape[1])
+        state["lengths"].add_(c.shape[1])
 
     # ------------------------------------------------------------ the two forms
     def _expanded(self, x, rows, lengths=None, starts=None):
@@ -171,36 +172,40 @@ class LatentAttention(nn.Module):
             if state is not None:
                 raise KdaError("a state needs use_cache=True")
             return self._whole(x)
-        if state is None:
-            state = self.new_state(x.shape[0], x.device, x.dtype)
         T = x.shape[1]
-        self._room(state, T)
-        if T == 1 and state["tokens"] > 0:
-            return self.decode_step_(x, state), state
-        self._append(x, state)
+        if state is not None:
+            self._room(state, T)
+            if T == 1 and state["tokens"] > 0:
+                return self.decode_step_(x, state), state
+        c = self.kv_down(x)
+        if state is None:
+            state = self.new_state(x.shape[0], x.device, c.dtype)
+            self._room(state, T)
+        self._append(c, state)
         state["tokens"] += T
-        return self._expanded(x, self._held(x, state, state["tokens"])), state
+        return self._expanded(x, self._held(state, state["tokens"], c.dtype)), state
 
     def _whole(self, x):
         c = self.kv_down(x)
         return self._expanded(x, torch.cat([self._norm(c[..., :self.rank]), c[..., self.rank:]], -1))
 
-    def _held(self, x, state, n):
-        """The cache's first n rows in x's type."""
+    def _held(self, state, n, dtype):
+        """The cache's first n rows in 16 bits."""
         if self.cache_bits == 8:
-            return mla_cache_read(state["latent"], state["scale"], self.rank, dtype=x.dtype, tokens=n)
+            return mla_cache_read(state["latent"], state["scale"], self.rank, dtype=dtype, tokens=n)
         return state["latent"][:, :n]
 
     def _step(self, x, state, n=None):
         """One token, unchecked: the captured part of a decode step.  ``n``: the tokens held with it, by which the
         expanded form is cut to the rows that there are; a captured step, whose count moves, expands all of the
         cache and takes the count from the device."""
-        self._append(x, state)
+        c = self.kv_down(x)
+        self._append(c, state)
         if self._absorbs(x):
             return self._absorbed(x, state)
         if n is not None:
-            return self._expanded(x, self._held(x, state, n))
-        rows = self._held(x, state, state["latent"].shape[1])
+            return self._expanded(x, self._held(state, n, c.dtype))
+        rows = self._held(state, state["latent"].shape[1], c.dtype)
         return self._expanded(x, rows, lengths=state["lengths"], starts=state["lengths"] - 1)
 
     @torch.no_grad()

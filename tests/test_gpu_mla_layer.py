@@ -320,3 +320,27 @@ def test_fp32_norm_weight_is_one_layer(kda_pkg):
             # one rounding to bf16 (7 bits behind the leading one: half a step is 2^-8), and fp32 arithmetic
             off = (got.double() - want).abs() - (torch.finfo(torch.bfloat16).eps / 2 + 2.0 ** -20) * want.abs()
             assert off.max().item() <= 0
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+def test_cached_calls_under_autocast(kda_pkg, bits):
+    """fp32 weights and x under autocast: the cache takes the type that the projections give, eager and captured."""
+    from kimi_linear_amd.graph_decode import KdaGraphedDecoder
+    layer = make(kda_pkg, torch.float32, cache_bits=bits).eval()
+    x = torch.randn(2, 60, 256, device=DEV)
+    tol = TOL[torch.bfloat16] * 10 / 8 + (0 if bits == 16 else 2 * 3.6e-2)
+    with torch.no_grad():
+        want, _ = reference(layer, x.double())
+        with torch.autocast("cuda", dtype=torch.bfloat16):
+            got, state = layer(x[:, :40], use_cache=True)
+            assert state["latent"].dtype is (torch.bfloat16 if bits == 16 else torch.float8_e4m3fn)
+            more, state = layer(x[:, 40:50], state=state, use_cache=True)
+            dec = KdaGraphedDecoder([layer], residual=False)
+            dec.prefill(x[:, :50])
+        assert rel(torch.cat([got, more], 1), want[:, :50]) <= tol
+        torch.cuda.empty_cache()             # what autocast kept is gone
+        for t in range(50, 60):
+            with torch.autocast("cuda", dtype=torch.bfloat16):
+                out, state = layer(x[:, t:t + 1], state=state, use_cache=True)
+            assert rel(out, want[:, t:t + 1]) <= tol, t
+            assert rel(dec.step(x[:, t:t + 1]), want[:, t]) <= tol, t
