@@ -668,13 +668,15 @@ void check_capture(const at::Device& dev) {
     }
 }
 
+struct Refused {};           // by the library, before any launch: the general path converts, or reports
+
 // Its node in the autograd graph: in native code, as its Python form took
 // 80 us of a small training step's 160.
 struct ExpandedFn : torch::autograd::Function<ExpandedFn> {
     static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& q, const Tensor& k, const OptTensor& k_pe,
                           const Tensor& v, const OptTensor& lengths, const OptTensor& starts, double scale) {
         Tensor o, lse, low;
-        if (!expanded_forward(q, k, k_pe, v, lengths, starts, scale, o, &lse, &low)) return Tensor();
+        if (!expanded_forward(q, k, k_pe, v, lengths, starts, scale, o, &lse, &low)) throw Refused();
         ctx->save_for_backward({q, k, or_none(k_pe), v, or_none(lengths), or_none(starts), o, lse, low});
         ctx->saved_data["scale"] = scale;
         return o;
@@ -753,9 +755,16 @@ py::object mla_expanded(const Tensor& q, const Tensor& k, const OptTensor& k_pe,
     if (at::GradMode::is_enabled())
         grad = q.requires_grad() || k.requires_grad() || v.requires_grad() || (k_pe && k_pe->requires_grad());
     Tensor o;
-    if (grad) o = ExpandedFn::apply(q, k, k_pe, v, lengths, starts, scale);
-    else if (!expanded_forward(q, k, k_pe, v, lengths, starts, scale, o)) return py::none();
-    return o.defined() ? py::cast(o) : py::object(py::none());
+    if (grad) {
+        try {
+            o = ExpandedFn::apply(q, k, k_pe, v, lengths, starts, scale);
+        } catch (const Refused&) {
+            return py::none();
+        }
+    } else if (!expanded_forward(q, k, k_pe, v, lengths, starts, scale, o)) {
+        return py::none();
+    }
+    return py::cast(o);
 }
 
 // A cache [B, S, rank + P] in 16 or 8 bits, in 8 with its scales [B, S, 2].

@@ -884,3 +884,15 @@ def test_append_norm_weight_types(kda_pkg, wtype, dtype, bits):
             close("row", got, want, (2.0 ** -4 + 2.0 ** -20) * want.abs() + step)
             assert ((sc[b, at:at + T, 0].double() - want[:, :R].abs().amax(-1) / 448).abs()
                     <= 2.0 ** -20 * sc[b, at:at + T, 0]).all()
+
+
+def test_expanded_refusals_under_grad(kda_pkg):
+    """What the library refuses is reported alike with and without inputs that require grad."""
+    for N, P, kw in ((96, 32, {}), (64, 16, {}), (64, 32, dict(scale=0.0)), (64, 32, dict(scale=float("nan")))):
+        xs = inputs(1, 6, 6, 2, N, P, BF16, seed=145)
+        said = []
+        for grad in (False, True):
+            with pytest.raises(kda_pkg.KdaError) as e:
+                kda_pkg.mla_expanded(*(x.detach().requires_grad_(grad) for x in xs), **kw)
+            said.append(str(e.value))
+        assert said[0] == said[1]
