@@ -690,7 +690,9 @@ struct ExpandedFn : torch::autograd::Function<ExpandedFn> {
         const bool again = at::GradMode::is_enabled();
         Tensor d_o = grads[0].detach();
         if (d_o.scalar_type() != q.scalar_type()) d_o = d_o.to(q.scalar_type());
-        if (!wide_rows(d_o)) d_o = d_o.clone(at::MemoryFormat::Contiguous);
+        // (tokens 2^23 elements apart are past the 32-bit offsets of a tile)
+        if (!wide_rows(d_o) || (d_o.size(1) > 1 && d_o.stride(1) >= int64_t{1} << 23))
+            d_o = d_o.clone(at::MemoryFormat::Contiguous);
         Tensor dq, dk, dpe, dv;
         {
             const at::AutoGradMode off(false);

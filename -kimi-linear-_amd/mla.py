@@ -42,11 +42,16 @@ HEAD_DIMS = (64, 128)
 _ACT = (torch.float16, torch.bfloat16)
 
 
-def _rows(x):
-    """x with contiguous channels and 16-byte aligned rows, copied if it has not."""
+_FAR = 2 ** 23          # elements between tokens from which a tile's offsets pass 32 bits
+
+
+def _rows(x, tiled=False):
+    """x with contiguous channels and 16-byte aligned rows, and tokens that are not far apart where they are
+    loaded in tiles; copied if it has not."""
     n = 16 // x.element_size()
     if (x.stride(-1) == 1 or x.shape[-1] <= 1) and x.data_ptr() % 16 == 0 and all(
-            s % n == 0 for s, m in zip(x.stride()[:-1], x.shape[:-1]) if m > 1):
+            s % n == 0 for s, m in zip(x.stride()[:-1], x.shape[:-1]) if m > 1) and not (
+            tiled and x.shape[1] > 1 and x.stride(1) >= _FAR):
         return x
     return x.clone(memory_format=torch.contiguous_format)
 
@@ -169,9 +174,9 @@ def mla_expanded(q, k_nope, k_pe, v, lengths=None, starts=None, scale=None):
             raise KdaError(f"{name} must be a floating tensor, got {x.dtype}")
     lengths, starts = _counts("lengths", lengths, B, q.device), _counts("starts", starts, B, q.device)
     scale = _positive("scale", D ** -0.5 if scale is None else scale)
-    q = _rows(q)
-    k_nope, v = _rows(k_nope.to(q.dtype)), _rows(v.to(q.dtype))
-    k_pe = None if k_pe is None else _rows(k_pe.to(q.dtype))
+    q = _rows(q, tiled=True)
+    k_nope, v = _rows(k_nope.to(q.dtype), tiled=True), _rows(v.to(q.dtype), tiled=True)
+    k_pe = None if k_pe is None else _rows(k_pe.to(q.dtype), tiled=True)
     return _native_call("mla_expanded", q, k_nope, k_pe, v, lengths, starts, scale)
 
 
@@ -218,7 +223,8 @@ def mla_absorbed(q, cache, lengths, rank, scale, cache_scale=None):
     row that sees no key (an idle slot, or ``lengths[b] < T``) gives zeros.
     ``scale`` is that of the expanded form, ``(N + P) ** -0.5``; ``cache_scale``
     of the tokens as :func:`mla_cache_append` writes it (positive, from 2^-60).
-    Ranks 128, 256, 512, P 0, 32, 64.  Forward only."""
+    Ranks 128, 256, 512, P 0, 32, 64; cache rows less than 2^23 elements apart.
+    Forward only."""
     try:
         o = _native.host().mla_absorbed(q, cache, lengths, rank, scale, cache_scale)
     except TypeError:

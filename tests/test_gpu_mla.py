@@ -896,3 +896,27 @@ def test_expanded_refusals_under_grad(kda_pkg):
                 kda_pkg.mla_expanded(*(x.detach().requires_grad_(grad) for x in xs), **kw)
             said.append(str(e.value))
         assert said[0] == said[1]
+
+
+def test_expanded_tokens_far_apart(kda_pkg):
+    """Inputs and an output gradient whose tokens are 2^23 elements apart (a time-major batch's) are copied."""
+    T, H, N, P = 5, 2, 64, 32
+    xs = inputs(1, T, T, H, N, P, BF16, seed=150)
+    d_o = rand(1, T, H, N, seed=155, dtype=BF16)
+
+    def apart(x):
+        row = x[0, 0].numel()
+        far = torch.empty(T * 2 ** 23, dtype=BF16, device=DEV).as_strided((T, row), (2 ** 23, 1))
+        far.copy_(x.reshape(T, row))
+        return far.view(x.shape)
+
+    def call(xs, d_o):
+        xs = [x.detach().requires_grad_() for x in xs]
+        o = kda_pkg.mla_expanded(*xs)
+        return [o.detach(), *torch.autograd.grad(o, xs, d_o)]
+
+    want = call(xs, d_o)
+    far = [apart(x) for x in xs]
+    assert all(f.stride(1) == 2 ** 23 for f in far)
+    assert all(torch.equal(a, b) for a, b in zip(call(far, apart(d_o)), want))
+    assert all(torch.equal(a, b) for a, b in zip(call(xs, apart(d_o)), want))
