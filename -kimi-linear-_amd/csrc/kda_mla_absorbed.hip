@@ -5,8 +5,9 @@
 //   s' = s log2(e),  M a running maximum (in fp16 less 15).
 //
 // Bound by reading the cache: 16 heads of one token make 2 (2R + P) 16 flops of
-// each row's 2 (R + P) bytes, 30 a byte.  So each row is read from memory once,
-// whole rows at a time (the score product's operand layout, a lane a row, would
+// each row's 2 (R + P) bytes, 30 a byte.  So sixteen query rows (a row tile: with up
+// to 16 heads, a token's) read each row once, and more fetch it again for each
+// sixteen of them, whole rows at a time (the score product's operand layout, a lane a row, would
 // ask for 16 cache lines an instruction: a window's loads took 6.8 k cycles to
 // issue that way, 2 k this way), and goes to LDS, from where the score product
 // reads it by rows and the value product transposed.

@@ -1,12 +1,13 @@
 // Rows written into a latent cache, and an 8-bit cache read back.
 //
 // A cache row is a token's latent (R channels) and its position channels (P).
-// Both kernels touch each row once: a wave takes a row, a lane eight channels
-// of the latent (R <= 512) and, the first P / 8 lanes, eight of the position
-// part, so the norm's sum and the two largest magnitudes are wave reductions
-// in registers.  Bound by HBM for long calls and by the launch for a decode
-// step's few rows: 64 rows of 576 in 8 bits 4 us, 6000 in 16 bits 5.2 us (2.9
-// TB/s), reading 32768 back 11.6 us (4.9 TB/s).
+// Both kernels touch each row once.  To write, a wave takes a row, a lane eight
+// channels of the latent (R <= 512) and, the first P / 8 lanes, eight of the
+// position part, so the norm's sum and the two largest magnitudes are wave
+// reductions in registers.  To read back, a lane takes sixteen channels, and the
+// lanes run on from one row into the next.  Bound by HBM for long calls and by the
+// launch for a decode step's few rows: 64 rows of 576 in 8 bits 4 us, 6000 in 16
+// bits 5.2 us (2.9 TB/s), reading 32768 back 11.6 us (4.9 TB/s).
 #include <hip/hip_runtime.h>
 
 #include "kda_launch.h"

@@ -289,9 +289,11 @@ __global__ __launch_bounds__(256) void join_kernel(kda_mla_expanded_args a, int 
 }
 
 // Workgroups that share the keys of a query tile of 64 rows: where there are too
-// few tiles for the CUs, as many as fill them with at least 512 keys each, or 256
-// in up to four.  us at T=64 H=16, parts of 512 / 256: S=1024 17.4 / 15.9, S=4096
-// 23.5 / 27.1.
+// few tiles for the CUs, as many as fill them with at least 512 keys each, or below
+// 2048 keys, where that would leave three or fewer, 256 (up to seven).  us at H=16, parts
+// of 512 / 256: T=64 S=1024 17.4 / 15.9, S=4096 23.5 / 27.1.  Between 1280 and 2047 keys
+// parts of 256 / four of them, T=1 S=1280 14.5 / 15.7, S=1792 15.7 / 17.3, S=2047 17.2 /
+// 17.2, but T=64 S=2047 21.2 / 20.2 and T=128 S=1792 21.6 / 20.9.
 int splits_of(int64_t B, int64_t T, int64_t S, int64_t H) {
     const int64_t tiles = B * H * ((T + 63) / 64);
     if (tiles == 0 || tiles > 128 || S < 1024) return 1;
