@@ -71,12 +71,13 @@ class LatentAttention(nn.Module):
         self.kv_up = nn.Linear(R, H * 2 * N, bias=False)         # per head: N key rows, then N value rows
         self.o_proj = nn.Linear(H * N, d, bias=bias)
         self.scale = (N + P) ** -0.5
-        self._up = None            # (key, W_k [H, N, R], W_v [H, R, N]) for the absorbed form
+        self._up = None            # (key, W_k [H, N, R], W_v [H, R, N], weight) for the absorbed form
 
     def _up_weights(self):
         """The up-projections as the absorbed form takes them, per head ``W_k [H, N, R]`` and ``W_v [H, R, N]``:
         copies of ``kv_up.weight``, made again (in place, so that a captured step sees them) when it changes.
-        After writes through ``.data`` call :meth:`refresh_fused_weight`."""
+        After writes through ``.data`` call :meth:`refresh_fused_weight`.  The key holds the weight's address, so
+        the weight copied from is kept too: no other can come to lie there."""
         w = self.kv_up.weight
         key = _native.host().params_key([w])
         if self._up is not None and self._up[0] == key:
@@ -91,13 +92,13 @@ class LatentAttention(nn.Module):
                 wv.copy_(per_head[:, N:].transpose(1, 2))
             else:
                 wk, wv = per_head[:, :N].clone(), per_head[:, N:].transpose(1, 2).clone(memory_format=torch.contiguous_format)
-        self._up = (key, wk.detach(), wv.detach())
+        self._up = (key, wk.detach(), wv.detach(), w.detach())
         return self._up[1], self._up[2]
 
     def refresh_fused_weight(self) -> None:
         """Make the absorbed form's copies again."""
         if self._up is not None:
-            self._up = (None, self._up[1], self._up[2])
+            self._up = (None, *self._up[1:])
         if self._absorbs():
             self._up_weights()
 

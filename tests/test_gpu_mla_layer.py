@@ -344,3 +344,22 @@ def test_cached_calls_under_autocast(kda_pkg, bits):
                 out, state = layer(x[:, t:t + 1], state=state, use_cache=True)
             assert rel(out, want[:, t:t + 1]) <= tol, t
             assert rel(dec.step(x[:, t:t + 1]), want[:, t]) <= tol, t
+
+
+def test_weight_at_the_address_of_an_earlier_one(kda_pkg):
+    """kv_up's weight replaced by one that the allocator puts where the old one was: the copies are made again."""
+    layer = make(kda_pkg, torch.float16).eval()
+    x = torch.randn(1, 9, 256, device=DEV).half()
+    shape = layer.kv_up.weight.shape
+    with torch.no_grad():
+        layer.kv_up.weight = nn.Parameter(torch.randn(shape, device=DEV, dtype=torch.float16))
+        _, state = layer(x[:, :8], use_cache=True)
+        layer(x[:, 8:], state=state, use_cache=True)
+        at, layer.kv_up.weight, tries = layer.kv_up.weight.data_ptr(), None, []
+        while len(tries) < 64 and not (tries and tries[-1].data_ptr() == at):
+            tries.append(torch.randn(shape, device=DEV, dtype=torch.float16))
+        layer.kv_up.weight = nn.Parameter(tries[-1])
+        _, state = layer(x[:, :8], use_cache=True)
+        got, _ = layer(x[:, 8:], state=state, use_cache=True)
+        # keys eleven times the usual: scores of size five, whose rounding (2^-11 of that) moves the weights by 2.4e-3 more
+        assert rel(got, reference(layer, x.double())[0][:, 8:]) <= 2 * TOL[torch.float16] * 10 / 8
