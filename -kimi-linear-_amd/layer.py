@@ -247,8 +247,8 @@ class KimiDeltaAttention(nn.Module):
         self.g_norm = HeadwiseRMSNorm(H, V, config.rms_norm_eps)
         self.o_proj = nn.Linear(H * V, d, bias=bias)
         self.fp32_recurrent_state = True
-        self._wcat = None          # (key, weight, bias) of the fused input projection
-        self._gcat = None          # (key, A_log, dt_bias) in fp32 for the gated core
+        self._wcat = None          # (key, weight, bias, parameters) of the fused input projection
+        self._gcat = None          # (key, A_log, dt_bias, parameters) in fp32 for the gated core
         self.fuse_output = None    # output epilogue in the chunk kernel: True, False, None = by shape
 
     def _input_mods(self):
@@ -268,7 +268,9 @@ class KimiDeltaAttention(nn.Module):
         the cache.  A refill of the same shape, dtype and device writes into
         the existing buffers, so a captured decode graph that reads them sees
         the new weights.  Writes through ``.data`` do not bump ``_version``:
-        call :meth:`refresh_fused_weight` after them."""
+        call :meth:`refresh_fused_weight` after them.  What was concatenated is
+        kept with the cache, so that no other parameter can come to lie at an
+        address of the key."""
         mods = self._input_mods()
         params = [m.weight for m in mods] + [m.bias for m in mods if m.bias is not None]
         key = _native.host().params_key(params)
@@ -289,7 +291,7 @@ class KimiDeltaAttention(nn.Module):
             else:
                 w = torch.cat(w_parts, 0)
                 b = torch.cat(b_parts) if b_parts is not None else None
-        self._wcat = (key, w, b)
+        self._wcat = (key, w, b, [p.detach() for p in params])
         return w, b
 
     def refresh_fused_weight(self) -> None:
@@ -298,9 +300,9 @@ class KimiDeltaAttention(nn.Module):
         unchanged).  Needed only after writes that bypass autograd's version
         counter, such as ``p.data.copy_(...)``."""
         if self._wcat is not None:
-            self._wcat = (None, self._wcat[1], self._wcat[2])
+            self._wcat = (None, *self._wcat[1:])
         if self._gcat is not None:
-            self._gcat = (None, self._gcat[1], self._gcat[2])
+            self._gcat = (None, *self._gcat[1:])
         self._input_weight()
         self._gate_params()
 
@@ -321,7 +323,7 @@ class KimiDeltaAttention(nn.Module):
             else:
                 a = self.A_log.detach().to(torch.float32).clone().contiguous()
                 d = self.dt_bias.detach().to(torch.float32).clone().contiguous()
-        self._gcat = (key, a, d)
+        self._gcat = (key, a, d, [p.detach() for p in params])
         return a, d
 
     def _fused_output_ok(self, x):

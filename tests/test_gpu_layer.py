@@ -271,3 +271,24 @@ def test_replaced_methods_are_called(kda_pkg, monkeypatch, where):
         dec.prefill(x[:, :4])
         assert seen.count("decode_step_") == 4 and seen.count("_output") == 5      # 3 warm-up steps and the capture
         assert rel(dec.step(x[:, 4:]), (x[:, 4:] + want[1])[:, 0]) <= tol
+
+
+def test_fused_weight_at_the_address_of_an_earlier_one(kda_pkg):
+    """Parameters replaced by ones that the allocator puts where the old ones were: the caches are made again."""
+    m, cfg, _ = make_layer(kda_pkg, torch.float16, seed=3)
+    x = make_x(1, 48, cfg.hidden_size, torch.float16, seed=4).to(DEV)
+    with torch.no_grad():
+        for mod, name in ((m.in_proj_v, "weight"), (m, "A_log")):
+            shape, dtype = getattr(mod, name).shape, getattr(mod, name).dtype
+            setattr(mod, name, torch.nn.Parameter(torch.randn(shape, device=DEV, dtype=dtype)))
+            m(x)                                                  # builds the caches
+            at = getattr(mod, name).data_ptr()
+            setattr(mod, name, None)
+            tries = []
+            while len(tries) < 64 and not (tries and tries[-1].data_ptr() == at):
+                tries.append(torch.randn(shape, device=DEV, dtype=dtype))
+            setattr(mod, name, torch.nn.Parameter(tries[-1]))
+            out = m(x)
+            fresh, _, _ = make_layer(kda_pkg, torch.float16, seed=3)
+            fresh.load_state_dict(m.state_dict())
+            assert torch.equal(out, fresh(x)), name
