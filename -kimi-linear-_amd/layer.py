@@ -276,7 +276,7 @@ class KimiDeltaAttention(nn.Module):
         key = _native.host().params_key(params)
         if self._wcat is not None and self._wcat[0] == key:
             return self._wcat[1], self._wcat[2]
-        with torch.no_grad():
+        with torch.inference_mode(False), torch.no_grad():      # (normal tensors, which a later call may refill)
             w_parts = [m.weight for m in mods]
             b_parts = [m.bias for m in mods] if mods[0].bias is not None else None
             n = sum(p.shape[0] for p in w_parts)
@@ -314,7 +314,7 @@ class KimiDeltaAttention(nn.Module):
         key = _native.host().params_key(params)
         if self._gcat is not None and self._gcat[0] == key:
             return self._gcat[1], self._gcat[2]
-        with torch.no_grad():
+        with torch.inference_mode(False), torch.no_grad():
             old = self._gcat
             if old is not None and old[1].shape == self.A_log.shape and old[1].device == self.A_log.device:
                 a, d = old[1], old[2]

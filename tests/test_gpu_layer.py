@@ -292,3 +292,21 @@ def test_fused_weight_at_the_address_of_an_earlier_one(kda_pkg):
             fresh, _, _ = make_layer(kda_pkg, torch.float16, seed=3)
             fresh.load_state_dict(m.state_dict())
             assert torch.equal(out, fresh(x)), name
+
+
+def test_fused_weights_made_under_inference_mode(kda_pkg):
+    """Caches first made under inference mode are refilled outside it when a parameter changes."""
+    m, cfg, _ = make_layer(kda_pkg, torch.float16, seed=3)
+    x = make_x(1, 48, cfg.hidden_size, torch.float16, seed=4).to(DEV)
+    with torch.inference_mode():
+        m(x)
+    with torch.no_grad():
+        m.in_proj_k.weight.mul_(0.5)
+        m.A_log.add_(0.25)
+        out = m(x)
+        m.refresh_fused_weight()
+        fresh, _, _ = make_layer(kda_pkg, torch.float16, seed=3)
+        fresh.load_state_dict(m.state_dict())
+        assert torch.equal(out, fresh(x))
+    with torch.inference_mode():
+        assert torch.equal(m(x), out)
