@@ -65,7 +65,8 @@ class KdaGraphedDecoder:
     gated recurrence the layer's fp32 copies of ``A_log`` and ``dt_bias``
     (``_gate_params``).  ``prefill`` refills these caches from the parameters
     (in place, so the graph keeps reading valid memory) and recaptures if a
-    buffer had to be reallocated (new dtype or shape).  After updating weights between two
+    buffer had to be reallocated (new dtype or shape) or a parameter is another
+    tensor than at the capture.  After updating weights between two
     ``step`` calls of one generation, call :meth:`refresh_weights`.
     """
 
@@ -82,7 +83,8 @@ class KdaGraphedDecoder:
         self._wbufs = None          # addresses of the fused weights the graph reads
 
     def _weight_buffers(self):
-        bufs = []
+        """Addresses of all that a captured step reads of the layers: their parameters and what is made of them."""
+        bufs = [tuple(p.data_ptr() for p in self.layers.parameters())]
         for layer in self.layers:
             if isinstance(layer, LatentAttention):
                 bufs.append(tuple(layer._weight_buffers()))
@@ -234,7 +236,7 @@ class KdaGraphedDecoder:
             self.graph = None
             self.static_states = None
         if self.graph is not None and self._weight_buffers() != self._wbufs:
-            self.graph = None           # a fused weight was reallocated: the graph would read freed memory
+            self.graph = None           # a weight was replaced: the graph would read the old one, or freed memory
         self._fill_static(states)
         if self.graph is None:
             self._B = B

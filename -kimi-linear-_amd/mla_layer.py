@@ -111,8 +111,8 @@ class LatentAttention(nn.Module):
         return _plain_weight(self.kv_up, *(() if x is None else (x,))) is not None
 
     def _weight_buffers(self):
-        """What a captured step reads of ``kv_up``."""
-        return [w.data_ptr() for w in (self._up_weights() if self._absorbs() else self.kv_up.parameters())]
+        """What a captured step reads beside the parameters."""
+        return [w.data_ptr() for w in self._up_weights()] if self._absorbs() else []
 
     # ------------------------------------------------------------ the cache
     def new_state(self, B: int, device, dtype) -> dict:

@@ -363,3 +363,31 @@ def test_weight_at_the_address_of_an_earlier_one(kda_pkg):
         got, _ = layer(x[:, 8:], state=state, use_cache=True)
         # keys eleven times the usual: scores of size five, whose rounding (2^-11 of that) moves the weights by 2.4e-3 more
         assert rel(got, reference(layer, x.double())[0][:, 8:]) <= 2 * TOL[torch.float16] * 10 / 8
+
+
+def test_decoder_follows_replaced_parameters(kda_pkg):
+    """A parameter that is another tensor than at the capture is seen by the next prompt's steps."""
+    from kimi_linear_amd.graph_decode import KdaGraphedDecoder
+    torch.manual_seed(5)
+    cfg = kda_pkg.linear_attn_config(hidden_size=256, num_heads=2, gate_low_rank=32, output_gate_low_rank=32)
+    layers = [kda_pkg.KimiDeltaAttention(cfg).to(DEV, torch.float16).eval(), make(kda_pkg, torch.float16, seed=6).eval()]
+    x = torch.randn(2, 31, 256, device=DEV).half()
+    with torch.no_grad():
+        dec = KdaGraphedDecoder(layers)
+        dec.prefill(x[:, :30])
+        captured = dec.graph
+        dec.prefill(x[:, :30])
+        assert dec.graph is captured
+        for layer, mod, name in ((0, "o_proj", "weight"), (0, "g_norm", "weight"), (1, "q_proj", "weight"), (1, "o_proj", "weight")):
+            mod = getattr(layers[layer], mod)
+            kept = getattr(mod, name)                            # (alive: nothing here reads released memory)
+            setattr(mod, name, nn.Parameter(kept * 1.5))
+            dec.prefill(x[:, :30])
+            got = dec.step(x[:, 30:]).clone()
+            fresh = KdaGraphedDecoder(layers)
+            fresh.prefill(x[:, :30])
+            assert torch.equal(got, fresh.step_eager(x[:, 30:])), (layer, mod)
+        kept = layers[1].kv_norm
+        layers[1].kv_norm = nn.Parameter(kept * 1.5)
+        dec.refresh_weights()                                    # between two steps
+        assert dec.graph is not captured
