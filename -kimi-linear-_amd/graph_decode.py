@@ -228,23 +228,25 @@ class KdaGraphedDecoder:
             raise ValueError("KdaGraphedDecoder runs on a HIP device")
         B = x.shape[0]
         h, states = self._run_stack(x, [None] * len(self.layers), use_cache=True)
-        if self.graph is not None and B != self._B:
-            self.graph = None
-            self.static_states = None
-        if self.static_states is not None and any(
-                not self._alike(st, new) for st, new in zip(self.static_states, states)):
-            self.graph = None
-            self.static_states = None
-        if self.graph is not None and self._weight_buffers() != self._wbufs:
-            self.graph = None           # a weight was replaced: the graph would read the old one, or freed memory
-        self._fill_static(states)
-        if self.graph is None:
-            self._B = B
-            self.input_static = torch.zeros(B, 1, x.shape[2], device=x.device, dtype=x.dtype)
-            self.output_static = torch.empty(B, x.shape[2], device=x.device, dtype=x.dtype)
-            self._capture()
+        with torch.inference_mode(False), torch.no_grad():       # (buffers that a step outside the mode may update)
+            if self.graph is not None and B != self._B:
+                self.graph = None
+                self.static_states = None
+            if self.static_states is not None and any(
+                    not self._alike(st, new) for st, new in zip(self.static_states, states)):
+                self.graph = None
+                self.static_states = None
+            if self.graph is not None and self._weight_buffers() != self._wbufs:
+                self.graph = None           # a weight was replaced: the graph would read the old one, or freed memory
+            self._fill_static(states)
+            if self.graph is None:
+                self._B = B
+                self.input_static = torch.zeros(B, 1, x.shape[2], device=x.device, dtype=x.dtype)
+                self.output_static = torch.empty(B, x.shape[2], device=x.device, dtype=x.dtype)
+                self._capture()
         return h[:, -1, :]
 
+    @torch.no_grad()
     def step(self, x: torch.Tensor) -> torch.Tensor:
         """Advance one token: x [B, 1, d] -> [B, d] (a view of the static output)."""
         if self.graph is None:

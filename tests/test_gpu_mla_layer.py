@@ -391,3 +391,26 @@ def test_decoder_follows_replaced_parameters(kda_pkg):
         layers[1].kv_norm = nn.Parameter(kept * 1.5)
         dec.refresh_weights()                                    # between two steps
         assert dec.graph is not captured
+
+
+def test_decoder_prefilled_under_inference_mode(kda_pkg):
+    """A prompt under inference mode, then steps and another prompt outside it, and the other way round."""
+    from kimi_linear_amd.graph_decode import KdaGraphedDecoder
+    torch.manual_seed(7)
+    cfg = kda_pkg.linear_attn_config(hidden_size=256, num_heads=2, gate_low_rank=32, output_gate_low_rank=32)
+    layers = [kda_pkg.KimiDeltaAttention(cfg).to(DEV, torch.float16).eval(), make(kda_pkg, torch.float16, seed=8).eval()]
+    x = torch.randn(2, 31, 256, device=DEV).half()
+    want = None
+    for first, then in ((torch.no_grad, torch.no_grad), (torch.inference_mode, torch.no_grad),
+                        (torch.no_grad, torch.inference_mode)):
+        dec = KdaGraphedDecoder(layers)
+        for _ in range(2):
+            with first():
+                dec.prefill(x[:, :29])
+            with then():
+                got = torch.stack([dec.step(x[:, 29:30]).clone(), dec.step_eager(x[:, 30:]).clone()])
+            want = got if want is None else want
+            assert torch.equal(got, want), (first, then)
+        with then():
+            dec.prefill(x[:, :29])
+            assert torch.equal(dec.step(x[:, 29:30]), want[0])
