@@ -30,9 +30,10 @@
 // scale again.
 //
 // At 16 heads, R=512 P=64 (a copy reaches 4.8 TB/s): B=64 of 8192 tokens 115 us
-// (5.2 TB/s), of 64 to 4096 tokens 41 us from HBM, in 8 bits 64 to 8192 44 us, with
-// 5 us of them the join; one sequence of 32768 18 us; of 200, in one workgroup,
-// 10 us: a window is 1.5 us and the way to the first one 3.
+// (5.2 TB/s), of 64 to 4096 tokens 40.5 us from HBM, in 8 bits 128 to 8192 43.5 us,
+// with 5 us of them the join; one sequence of 32768 17.8 us, in 8 bits 15.5; of 200,
+// in one workgroup, 10 us: a window is 1.5 us and the way to the first one 3.  32 heads
+// of that batch 67 us, 64 121, 128 169.
 #include <hip/hip_runtime.h>
 
 #include "kda_launch.h"
@@ -419,7 +420,8 @@ __device__ __forceinline__ int wave_scan(int x, int lane) {
 // but gives most workgroups two parts to start (1.3 us each) and more parts to join.
 // us at 16 heads, R=512 P=64, run on / cut: 64 sequences of 64 to 4096 tokens 36.6 /
 // 32.6, of 1 to 1000 23.7 / 16.8, 16 of 1900 with 4 tokens each 31 / 25, 37 of 8192
-// 74 / 73; in 8 bits 64 of 64 to 4096 29 / 24, but 52 of 8192 52 / 57.
+// 74 / 73; in 8 bits 64 of 64 to 4096 29 / 24, but 52 of 8192 52 / 57.  One rule for both
+// widths: batches whose lengths differ gain in both.
 constexpr int kLeast = 8, kCut = 64;
 template <typename T, bool F8, int R, int P>
 __global__ __launch_bounds__(kThreads, F8 ? 2 : 1) void absorbed_kernel(kda_mla_absorbed_args a, int rts, bool alone) {

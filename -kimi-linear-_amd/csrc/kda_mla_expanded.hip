@@ -5,9 +5,9 @@
 //   s' = s log2(e),  M a running maximum (in fp16 less 15).
 //
 // Bound by the matrix cores: 2 (N + P + V) flops a visible pair.  At 128 + 64
-// channels, bf16, H=16: 1110 TFLOP/s at T=16384, 930 for T=2048 over 16384 keys,
+// channels, bf16, H=16: 1110 TFLOP/s at T=16384, 920 for T=2048 over 16384 keys,
 // 850 at B=4 T=2048 (a large product reaches 1200); one prompt of 1000 tokens
-// takes 21 us, the longest tile's eight steps in a row.  A wave has 32
+// takes 21 us (23 in fp16), the longest tile's eight steps in a row.  A wave has 32
 // query rows; a workgroup's waves share 64-key tiles of K, K_pe and V in LDS,
 // two buffers, the next tile's loads in flight through the current one's
 // products.  The scores are formed transposed (keys x rows, 32x32x16), so a

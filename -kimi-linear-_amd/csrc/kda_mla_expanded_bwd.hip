@@ -86,11 +86,12 @@ __device__ __forceinline__ uint4 rest8(const f16v& x, int at) {
 }
 // FEW: p and ds go into the products with what their rounding leaves.  In variants of
 // their own: the others' registers are full (dk and dv 247 -> 277 us at 4 x 2048).
-// dq of 32 rows a wave, and delta.  196 us at B=4 T=2048 H=16, 128 + 64 channels,
+// dq of 32 rows a wave, and delta.  195 us at B=4 T=2048 H=16, 128 + 64 channels,
 // bf16: 700 TFLOP/s.  RW waves of rows times KW that share the keys of each (of
 // a step's KW kKeys keys, wave group g takes the g-th kKeys), joined at the end.
 // Four groups' tiles of 128 + 64 channels fit LDS once, and the registers do not
-// hold the next ones beside the sums: those are loaded after the products.
+// hold the next ones beside the sums: those are loaded after the products.  (The
+// variants of 128 rows spill 8 to 10 registers at 128 + 64 channels.)
 // Grid as the forward's.
 template <typename T, int N, int P, int RW, int KW, bool FEW>
 __global__ __launch_bounds__(64 * RW * KW, 2) void dq_kernel(kda_mla_expanded_bwd_args g, float* delta, int qtiles) {
@@ -285,7 +286,7 @@ __global__ __launch_bounds__(64 * RW * KW, 2) void dq_kernel(kda_mla_expanded_bw
 // sums of its keys, joined at the end.  (Four waves with K and V in registers
 // need more than 256 of them, and moving values between the two halves of the
 // register file took most of the time: 403 us at B=4 T=2048 H=16 with 128 + 64
-// channels, 268 this way, 640 TFLOP/s.)
+// channels, 273 this way, 630 TFLOP/s.)
 // Grid: (key tiles, the first have the most queries) x (batch, head), the latter inner.
 template <typename T, int N, int P, int KG>
 struct Dkv {

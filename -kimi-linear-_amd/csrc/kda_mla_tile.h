@@ -66,6 +66,8 @@ __device__ __forceinline__ uint32_t rest(float x, float y, bf16_t) {
 // leaves: of few values one rounding may be most of an output's error, and there is
 // time for it (bf16: two tokens dk 2.9e-3 off, 33 tokens 2.6e-3, by its own rounding 1.6e-3
 // and 1.7e-3, which it comes down to).  Of many the roundings average out to 2.4e-3.
+// By the tensors' sizes: the lengths are on the device, and other variants' registers are
+// full.  (So are these: the backward's at 128 channels spill 10 to 36, in kernels of 10 to 13 us.)
 inline bool few(const kda_mla_expanded_args& a) { return a.S <= 32 || (a.S <= 128 && a.B * a.H <= 64); }
 
 // Loads issued before this stay before it: the compiler otherwise sinks a

@@ -16,8 +16,14 @@ A cache is ``[B, S, rank + P]``: one row a token, latent then position
 channels.  In 16 bits it has the activations' type; in 8 bits it is
 ``torch.float8_e4m3fn`` with ``cache_scale`` fp32 ``[B, S, 2]``, a scale for a
 row's latent and one for its position part.  ``lengths``, ``starts`` and
-``counts`` are integer tensors ``[B]`` on the device; the kernels read them
-(values out of range are clamped), so a captured graph follows them.
+``counts`` are integer tensors ``[B]`` on the device; the kernels read them, so
+a captured graph follows them.  A length to read by counts as 0 below 0 and as
+S above it; rows to append that a length puts outside the cache are dropped.
+
+Softmax weights are operands of 16 bits, off by up to half a step of the type
+(2^-8 of themselves in bf16, 2^-11 in fp16); in fp16 one below 2^-29 of its row's
+largest has fewer bits, and below 2^-40 none.  Scores may be of any size that fp32 holds; a weight is as exact as
+its score, to 2^-24 of that.
 
 HIP tensors only, fp16 or bf16 activations, no fallback: anything else raises
 :class:`KdaError`, as do calls under a trace, ``vmap`` or forward-mode differentiation.  Calls are asynchronous on torch's current stream and may be
@@ -220,7 +226,8 @@ def mla_absorbed(q, cache, lengths, rank, scale, cache_scale=None):
 
     ``lengths [B]`` counts a sequence's tokens with the T new ones, which are
     its last (append them first); cache rows from there on are never read.  A
-    row that sees no key (an idle slot, or ``lengths[b] < T``) gives zeros.
+    row that sees no key (an idle slot, or ``lengths[b] < T``) gives zeros.  A
+    cached row that is not finite may reach the up to T - 1 queries before its own.
     ``scale`` is that of the expanded form, ``(N + P) ** -0.5``; ``cache_scale``
     of the tokens as :func:`mla_cache_append` writes it (positive, from 2^-60).
     Ranks 128, 256, 512, P 0, 32, 64; cache rows less than 2^23 elements apart.
@@ -249,7 +256,7 @@ def mla_absorbed(q, cache, lengths, rank, scale, cache_scale=None):
 def mla_cache_append(x, cache, lengths, rank, cache_scale=None, counts=None, norm_weight=None, eps=1e-6):
     """Write ``x [B, T, rank + P]`` into the cache, in place: row t of sequence b
     to cache row ``lengths[b] + t`` for ``t < counts[b]`` (default T).  Rows that
-    would fall at or past S are dropped, every other row of the cache is left
+    would fall below 0, at or past S are dropped, every other row of the cache is left
     as it is; ``lengths`` itself does not change.
 
     With ``norm_weight [rank]`` (x's type, or taken in fp32) the latent part is

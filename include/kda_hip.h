@@ -495,8 +495,9 @@ int kda_output_bwd(const kda_output_bwd_args* args, void* stream);
  * outputs overlap no input; asynchronous on `stream`, nothing allocated,
  * nothing read back, capturable.  Workspaces are the caller's, 16-byte
  * aligned; calls that may overlap in time need one each.  lengths, starts and
- * counts are int32 device arrays read by the kernels (lengths and counts out of
- * range are clamped, rows to append past the cache's end dropped).
+ * counts are int32 device arrays read by the kernels (a length to read by counts
+ * as 0 below 0 and as S above it; rows to append that fall outside the cache are
+ * dropped).
  *
  * Expanded form, for prompts and training:
  *   s_tj = scale (q_t[0:N] . k_j + q_t[N:N+P] . k_pe_j)
