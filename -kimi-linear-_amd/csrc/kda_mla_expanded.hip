@@ -99,7 +99,7 @@ __global__ __launch_bounds__(64 * RW * KW, RW * KW == 8 ? 2 : 1) void expanded_k
 
     if (keys > first) {
         uint4 q[D / 16];
-        const T* qr = static_cast<const T*>(a.q) + b * a.q_stride[0] + min(t, exist - 1) * a.q_stride[1] +
+        const T* qr = static_cast<const T*>(a.q) + b * a.q_stride[0] + min(max(t, -start), exist - 1) * a.q_stride[1] +
                       h * a.q_stride[2] + 8 * half;
         F tile(a, b, h);
         tile.fetch(a, first, keys);

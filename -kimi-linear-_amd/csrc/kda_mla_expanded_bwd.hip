@@ -126,7 +126,8 @@ __global__ __launch_bounds__(64 * RW * KW, 2) void dq_kernel(kda_mla_expanded_bw
     float f = kHalf<T> ? kFirst : 1.f;
 
     if (keys > 0) {
-        const int tc = min(t, at.exist - 1);
+        // a row that does not exist, or at a position below 0, takes another's data: its own is not read
+        const int tc = min(max(t, -at.start), at.exist - 1);
         const T* qr = static_cast<const T*>(a.q) + at.b * a.q_stride[0] + tc * a.q_stride[1] + at.h * a.q_stride[2] +
                       8 * half;
         const T* dor = static_cast<const T*>(g.d_o) + at.b * g.d_o_stride[0] + tc * g.d_o_stride[1] +
@@ -336,7 +337,8 @@ __global__ __launch_bounds__(512, 2) void dkv_kernel(kda_mla_expanded_bwd_args g
         for (int e = 0; e < 16; ++e) dv[i][e] = 0.f;
     float f = kHalf<T> ? kFirst : 1.f;
 
-    const int first = max(0, j0 - at.start) / kPass * kPass;         // the first queries that see a key of these
+    // the first queries that see a key of these; those before the first key are not read
+    const int first = max(max(0, j0 - at.start) / kPass * kPass, -at.start);
     if (j0 < at.len && first < at.exist) {
         const T* qb = static_cast<const T*>(a.q) + at.b * a.q_stride[0] + at.h * a.q_stride[2];
         const T* ob = static_cast<const T*>(g.d_o) + at.b * g.d_o_stride[0] + at.h * g.d_o_stride[2];

@@ -535,7 +535,8 @@ int kda_mla_expanded_fwd(const kda_mla_expanded_args* args, void* stream);
 
 /* Its gradients, from d_o and the forward's arguments, o, lse and o_low.  Every sum
  * in fp32 in a fixed order (the position part's over the heads too), rounded
- * once to the activation type.  d_o of queries that do not exist is not read. */
+ * once to the activation type.  d_o and q of queries that do not exist, or at a
+ * position below 0, are not read. */
 typedef struct kda_mla_expanded_bwd_args {
     kda_mla_expanded_args fwd;     /* o, lse and o_low as kda_mla_expanded_fwd left them */
     const void* d_o;               /* [B, T, H, V] */

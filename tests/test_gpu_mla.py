@@ -920,3 +920,32 @@ def test_expanded_tokens_far_apart(kda_pkg):
     assert all(f.stride(1) == 2 ** 23 for f in far)
     assert all(torch.equal(a, b) for a, b in zip(call(far, apart(d_o)), want))
     assert all(torch.equal(a, b) for a, b in zip(call(xs, apart(d_o)), want))
+
+
+@pytest.mark.parametrize("B,T,S,lengths,starts", [(1, 40, 16, [16], [-24]), (2, 300, 200, [200, 60], [-100, -299]),
+                                                  (4, 700, 600, [600, 600, 1, 0], [-100, 0, -500, -3]),
+                                                  (3, 130, 130, [130, 60, 5], [0, 0, -70])])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_expanded_rows_that_see_no_key_are_not_read(kda_pkg, B, T, S, lengths, starts, dtype):
+    """q and the output's gradient may hold anything in rows at positions below 0 and past the sequence's end: the
+    rows' own results are zeros and nobody else's change."""
+    H, N, P = 2, 64, 32
+    q, kn, pe, v = inputs(B, T, S, H, N, P, dtype, seed=160)
+    d_o = rand(B, T, H, N, seed=165, dtype=dtype)
+    n, st = i32(lengths), i32(starts)
+    pos = st[:, None] + torch.arange(T, device=DEV)
+    none = (pos < 0) | (pos >= n[:, None])
+
+    def call(q, d_o):
+        xs = [x.detach().clone().requires_grad_() for x in (q, kn, pe, v)]
+        o = kda_pkg.mla_expanded(*xs, lengths=n, starts=st)
+        return [o.detach(), *torch.autograd.grad(o, xs, d_o)]
+
+    want = call(q, d_o)
+    for bad in (float("nan"), float("inf")):
+        q2, d2 = q.clone(), d_o.clone()
+        q2[none], d2[none] = bad, bad
+        got = call(q2, d2)
+        assert (got[0][none] == 0).all() and (got[1][none] == 0).all()
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
