@@ -60,9 +60,9 @@ __device__ __forceinline__ float part_scale(const float (&x)[8], bool has) {
 // x / scale to the nearest e4m3 value.  The quotient is the exactly rounded one
 // (a product with 1 / scale alone would round some ties to the other side): from
 // the rounded reciprocal r, q = x r, then q + (x - q scale) r, whose remainder an
-// fma gives exactly (Markstein's theorem; a scale of 24 one bits aside, where it
-// is the quotient to one unit).  Three operations a value; the division's own
-// sequence took 10.7 us for 8192 rows of 576, three times their bytes.
+// fma gives exactly (Markstein's theorem: r is 1 / scale correctly rounded, and q
+// within a unit).  Three operations a value; the division's own sequence took 10.7
+// us for 8192 rows of 576, three times their bytes.
 __device__ __forceinline__ uint2 quantise8(const float (&x)[8], float scale) {
     const float r = 1.f / scale;
     float y[8];

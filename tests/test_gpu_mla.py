@@ -949,3 +949,18 @@ def test_expanded_rows_that_see_no_key_are_not_read(kda_pkg, B, T, S, lengths, s
         assert (got[0][none] == 0).all() and (got[1][none] == 0).all()
         for a, b in zip(got, want):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("k", [-30, -3, 0, 5])
+def test_append_8bit_scale_of_all_ones(kda_pkg, k):
+    """A scale of 24 one bits, (2 - 2^-23) 2^k, at which 2^-9 2^k over it is just past the tie below e4m3's smallest
+    value: the quotient is the exactly rounded one there too."""
+    R, P = 128, 0
+    w = torch.zeros(R, device=DEV)
+    w[0], w[1], w[2] = 895.99994 * 2.0 ** k, 2.0 ** -9 * 2.0 ** k, -2.0 ** -9 * 2.0 ** k
+    cache, sc = torch.zeros(1, 1, R, dtype=F8, device=DEV), torch.zeros(1, 1, 2, device=DEV)
+    # rows of ones: their norm is one, and what is quantised is the weight
+    kda_pkg.mla_cache_append(torch.ones(1, 1, R, dtype=BF16, device=DEV), cache, i32([0]), R, cache_scale=sc,
+                             norm_weight=w, eps=0.0)
+    assert sc[0, 0, 0].item() == (2 - 2.0 ** -23) * 2.0 ** k
+    assert cache[0, 0, :4].float().tolist() == [448.0, 2.0 ** -9, -2.0 ** -9, 0.0]
