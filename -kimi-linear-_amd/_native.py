@@ -14,12 +14,13 @@ from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "libkda_hip.so"
 HOST_PATH = Path(__file__).resolve().parent / "_kda_host.so"     # csrc/host_binding.cpp
-ABI_VERSION = 18
+ABI_VERSION = 19
 
 DTYPE_F32 = 0
 DTYPE_F16 = 1
 DTYPE_BF16 = 2
 DTYPE_E4M3 = 3
+DTYPE_E2M1 = 4
 
 STATUS_OK = 0
 STATUS_BAD_SHAPE = 2
@@ -207,6 +208,27 @@ class KdaMlaReadArgs(ctypes.Structure):
         ("cache", ctypes.c_void_p), ("cache_stride", ctypes.c_int64 * 2),
         ("cache_scale", ctypes.c_void_p), ("scale_stride", ctypes.c_int64 * 2),
         ("lengths", ctypes.c_void_p), ("out", ctypes.c_void_p), ("out_dtype", ctypes.c_int32),
+        ("cache_dtype", ctypes.c_int32),
+    ]
+
+
+class KdaMx4LinearArgs(ctypes.Structure):
+    """Mirror of ``struct kda_mx4_linear_args`` (include/kda_hip.h)."""
+
+    _fields_ = [
+        ("M", ctypes.c_int64), ("N", ctypes.c_int64), ("K", ctypes.c_int64),
+        ("x", ctypes.c_void_p), ("x_stride", ctypes.c_int64), ("w", ctypes.c_void_p), ("w_scale", ctypes.c_void_p),
+        ("bias", ctypes.c_void_p), ("residual", ctypes.c_void_p), ("residual_stride", ctypes.c_int64),
+        ("y", ctypes.c_void_p), ("dtype", ctypes.c_int32),
+    ]
+
+
+class KdaMx4ConvertArgs(ctypes.Structure):
+    """Mirror of ``struct kda_mx4_convert_args`` (include/kda_hip.h)."""
+
+    _fields_ = [
+        ("N", ctypes.c_int64), ("K", ctypes.c_int64), ("values", ctypes.c_void_p), ("value_stride", ctypes.c_int64),
+        ("data", ctypes.c_void_p), ("scale", ctypes.c_void_p), ("dtype", ctypes.c_int32),
     ]
 
 
@@ -221,7 +243,8 @@ EXPORTED_SYMBOLS = ("kda_chunkwise_fwd", "kda_recurrent_fwd", "kda_chunkwise_fwd
                     "kda_output_bwd", "kda_output_bwd_workspace_size", "kda_mla_expanded_fwd", "kda_mla_expanded_bwd",
                     "kda_mla_expanded_workspace_size",
                     "kda_mla_expanded_bwd_workspace_size", "kda_mla_absorbed_fwd", "kda_mla_absorbed_workspace_size",
-                    "kda_mla_cache_append", "kda_mla_cache_read", "kda_status_str", "kda_abi_version")
+                    "kda_mla_cache_append", "kda_mla_cache_read", "kda_mx4_linear_fwd", "kda_mx4_quantize",
+                    "kda_mx4_dequantize", "kda_status_str", "kda_abi_version")
 
 _lib = None
 _host = None
@@ -299,6 +322,10 @@ def load() -> ctypes.CDLL:
                            ("cache_read", KdaMlaReadArgs)):
             getattr(lib, f"kda_mla_{name}").argtypes = [ctypes.POINTER(args), ctypes.c_void_p]
             getattr(lib, f"kda_mla_{name}").restype = ctypes.c_int
+        for name, args in (("linear_fwd", KdaMx4LinearArgs), ("quantize", KdaMx4ConvertArgs),
+                           ("dequantize", KdaMx4ConvertArgs)):
+            getattr(lib, f"kda_mx4_{name}").argtypes = [ctypes.POINTER(args), ctypes.c_void_p]
+            getattr(lib, f"kda_mx4_{name}").restype = ctypes.c_int
         for name in ("expanded", "expanded_bwd", "absorbed"):
             getattr(lib, f"kda_mla_{name}_workspace_size").argtypes = [ctypes.c_int64] * 5
             getattr(lib, f"kda_mla_{name}_workspace_size").restype = ctypes.c_size_t

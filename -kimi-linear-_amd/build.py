@@ -22,7 +22,7 @@ HOST_PATH = PKG_DIR / "_kda_host.so"
 BUILD_DIR = PKG_DIR / "_build"
 
 SOURCES = ["kda_api.hip", "kda_recurrent.hip", "kda_chunkwise.hip", "kda_chunkwise_bwd.hip", "kda_layer_ops.hip",
-           "kda_layer_bwd.hip", "kda_long.hip", "kda_ckpt_fp32.hip", "kda_linear.hip",
+           "kda_layer_bwd.hip", "kda_long.hip", "kda_ckpt_fp32.hip", "kda_linear.hip", "kda_mx4.hip",
            "kda_mla_api.hip", "kda_mla_absorbed.hip", "kda_mla_cache.hip", "kda_mla_expanded.hip",
            "kda_mla_expanded_bwd.hip"]
 

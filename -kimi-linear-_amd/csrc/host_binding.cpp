@@ -61,6 +61,9 @@ struct Fns {
     decltype(&kda_mla_absorbed_workspace_size) mla_absorbed_ws = nullptr;
     decltype(&kda_mla_cache_append) mla_append = nullptr;
     decltype(&kda_mla_cache_read) mla_read = nullptr;
+    decltype(&kda_mx4_linear_fwd) mx4_linear = nullptr;
+    decltype(&kda_mx4_quantize) mx4_quantize = nullptr;
+    decltype(&kda_mx4_dequantize) mx4_dequantize = nullptr;
     decltype(&kda_status_str) status_str = nullptr;
 };
 Fns fn;
@@ -99,6 +102,9 @@ void bind(const py::dict& addr, const py::object& stream_fn, const py::object& e
     take(fn.mla_absorbed_ws, addr, "kda_mla_absorbed_workspace_size");
     take(fn.mla_append, addr, "kda_mla_cache_append");
     take(fn.mla_read, addr, "kda_mla_cache_read");
+    take(fn.mx4_linear, addr, "kda_mx4_linear_fwd");
+    take(fn.mx4_quantize, addr, "kda_mx4_quantize");
+    take(fn.mx4_dequantize, addr, "kda_mx4_dequantize");
     take(fn.status_str, addr, "kda_status_str");
     device_type = at::Device(device).type();
     raw_stream = stream_fn.inc_ref().ptr();
@@ -773,13 +779,23 @@ py::object mla_expanded(const Tensor& q, const Tensor& k, const OptTensor& k_pe,
 bool cache_ok(const Tensor& cache, const OptTensor& scale, int64_t B, at::ScalarType act) {
     if (cache.dim() != 3 || cache.size(0) != B || !wide_rows(cache)) return false;
     if (cache.scalar_type() == act) return !scale;
+    if (cache.scalar_type() == at::kFloat4_e2m1fn_x2)
+        return scale && scale->scalar_type() == at::kFloat8_e8m0fnu && sized(*scale, {B, cache.size(1), 8}) &&
+               scale->stride(2) == 1 && (scale->size(0) <= 1 || scale->stride(0) % 8 == 0) &&
+               (scale->size(1) <= 1 || scale->stride(1) % 8 == 0) &&
+               reinterpret_cast<uintptr_t>(scale->data_ptr()) % 8 == 0;
     return cache.scalar_type() == at::kFloat8_e4m3fn && scale && scale->scalar_type() == at::kFloat &&
            sized(*scale, {B, cache.size(1), 2}) && scale->stride(2) == 1 &&
            (scale->size(0) <= 1 || scale->stride(0) % 2 == 0) && (scale->size(1) <= 1 || scale->stride(1) % 2 == 0) &&
            reinterpret_cast<uintptr_t>(scale->data_ptr()) % 8 == 0;
 }
 int cache_code(const Tensor& cache) {
+    if (cache.scalar_type() == at::kFloat4_e2m1fn_x2) return KDA_DTYPE_E2M1;
     return cache.scalar_type() == at::kFloat8_e4m3fn ? static_cast<int>(KDA_DTYPE_E4M3) : code(cache);
+}
+// Channels of a cache row: a 4-bit cache's elements are two each.
+int64_t cache_width(const Tensor& cache) {
+    return cache.size(2) * (cache.scalar_type() == at::kFloat4_e2m1fn_x2 ? 2 : 1);
 }
 
 // mla_absorbed: o [B, T, H, rank] or None.
@@ -788,7 +804,7 @@ py::object mla_absorbed(const Tensor& q, const Tensor& cache, const Tensor& leng
     Plain plain(q);
     plain.add(cache).add(lengths).add(cache_scale);
     if (!plain.ok || traced() || q.dim() != 4 || !half_type(q) || !wide_rows(q) || !counts_ok(lengths, q.size(0)) ||
-        !cache_ok(cache, cache_scale, q.size(0), q.scalar_type()) || cache.size(2) != q.size(3))
+        !cache_ok(cache, cache_scale, q.size(0), q.scalar_type()) || cache_width(cache) != q.size(3))
         return py::none();
     Tensor o;
     const int status = run(plain.dev, [&](void* stream) -> int {
@@ -802,7 +818,7 @@ py::object mla_absorbed(const Tensor& q, const Tensor& cache, const Tensor& leng
         a.cache = cache.data_ptr();
         row_strides(a.cache_stride, cache);
         if (cache_scale) {
-            a.cache_scale = static_cast<const float*>(cache_scale->data_ptr());
+            a.cache_scale = cache_scale->data_ptr();
             row_strides(a.scale_stride, *cache_scale);
         }
         a.lengths = static_cast<const int32_t*>(lengths.data_ptr());
@@ -829,7 +845,7 @@ bool mla_append(const Tensor& x, const Tensor& cache, const Tensor& lengths, int
     plain.add(cache).add(lengths).add(cache_scale).add(counts).add(weight);
     if (!plain.ok || traced() || x.dim() != 3 || !half_type(x) || !wide_rows(x) || !counts_ok(lengths, x.size(0)) ||
         !counts_ok(counts, x.size(0)) || !cache_ok(cache, cache_scale, x.size(0), x.scalar_type()) ||
-        cache.size(2) != x.size(2) || overlaps(cache, x) || (cache_scale && overlaps(*cache_scale, x)))
+        cache_width(cache) != x.size(2) || overlaps(cache, x) || (cache_scale && overlaps(*cache_scale, x)))
         return false;
     if (weight && ((weight->scalar_type() != x.scalar_type() && weight->scalar_type() != at::kFloat) ||
                    !sized(*weight, {rank}) || !wide_rows(*weight)))
@@ -841,7 +857,7 @@ bool mla_append(const Tensor& x, const Tensor& cache, const Tensor& lengths, int
     a.cache = cache.data_ptr();
     row_strides(a.cache_stride, cache);
     if (cache_scale) {
-        a.cache_scale = static_cast<float*>(cache_scale->data_ptr());
+        a.cache_scale = cache_scale->data_ptr();
         row_strides(a.scale_stride, *cache_scale);
     }
     a.lengths = static_cast<const int32_t*>(lengths.data_ptr());
@@ -870,12 +886,13 @@ py::object mla_read(const Tensor& cache, const Tensor& cache_scale, int64_t rank
         return py::none();
     Tensor out;
     const int status = run(plain.dev, [&](void* stream) -> int {
-        out = at::empty({cache.size(0), count, cache.size(2)}, cache.options().dtype(dtype).requires_grad(false));
+        out = at::empty({cache.size(0), count, cache_width(cache)}, cache.options().dtype(dtype).requires_grad(false));
         kda_mla_read_args a{};
-        a.B = cache.size(0); a.S = count; a.R = rank; a.P = cache.size(2) - rank;
+        a.B = cache.size(0); a.S = count; a.R = rank; a.P = cache_width(cache) - rank;
         a.cache = cache.data_ptr();
         row_strides(a.cache_stride, cache);
-        a.cache_scale = static_cast<const float*>(cache_scale.data_ptr());
+        a.cache_scale = cache_scale.data_ptr();
+        a.cache_dtype = cache_code(cache);
         row_strides(a.scale_stride, cache_scale);
         a.lengths = counts_ptr(lengths);
         a.out = out.data_ptr();
@@ -883,6 +900,124 @@ py::object mla_read(const Tensor& cache, const Tensor& cache_scale, int64_t rank
         return fn.mla_read(&a, stream);
     });
     if (refused(status, "kda_mla_cache_read")) return py::none();
+    return py::cast(out);
+}
+
+// ---- matrices in 4 bits ------------------------------------------------------
+// e2m1 values, two a byte, and a byte of scale for each 32: contiguous, of these types or plain bytes.
+bool mx4_ok(const Tensor& data, const Tensor& scale) {
+    const auto d = data.scalar_type(), s = scale.scalar_type();
+    return (d == at::kFloat4_e2m1fn_x2 || d == at::kByte) && (s == at::kFloat8_e8m0fnu || s == at::kByte) && data.dim() >= 1 &&
+           data.dim() == scale.dim() && data.size(-1) == 16 * scale.size(-1) && data.size(-1) > 0 &&
+           data.sizes().slice(0, data.dim() - 1).equals(scale.sizes().slice(0, scale.dim() - 1)) && data.is_contiguous() &&
+           scale.is_contiguous() && reinterpret_cast<uintptr_t>(data.data_ptr()) % 16 == 0;
+}
+
+// The one stride between the rows [.., K] of t, or -1 where there is none.
+int64_t rows_stride(const Tensor& t) {
+    int64_t stride = -1, rows = 1;
+    for (int64_t i = t.dim() - 2; i >= 0; --i) {
+        if (t.size(i) == 1) continue;
+        if (stride < 0) stride = t.stride(i);
+        else if (t.stride(i) != stride * rows) return -1;
+        rows *= t.size(i);
+    }
+    return rows == 1 ? t.size(-1) : stride;
+}
+bool mx4_rows(const Tensor& t) {
+    const int64_t s = rows_stride(t);
+    return (t.size(-1) == 1 || t.stride(-1) == 1) && s >= 0 && s * t.element_size() % 16 == 0 &&
+           reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+}
+
+// mx4_linear: x [.., K] times w^T [N, K], [.., N]; into out, or None.
+py::object mx4_linear(const Tensor& x, const Tensor& w, const Tensor& w_scale, const OptTensor& bias, const OptTensor& residual,
+                      const OptTensor& out) {
+    Plain plain(x);
+    plain.add(w).add(w_scale).add(bias).add(residual).add(out);
+    if (!plain.ok || traced() || autocast_on() || x.dim() < 1 || w.dim() != 2 || !half_type(x) || !mx4_ok(w, w_scale) ||
+        x.size(-1) != 2 * w.size(1) || !mx4_rows(x))
+        return py::none();
+    const int64_t N = w.size(0);
+    auto shape = x.sizes().vec();
+    shape.back() = N;
+    if (bias && (bias->scalar_type() != x.scalar_type() || !sized(*bias, {N}) || !bias->is_contiguous())) return py::none();
+    if (residual && (residual->scalar_type() != x.scalar_type() || residual->sizes() != at::IntArrayRef(shape) ||
+                     (N > 1 && residual->stride(-1) != 1) || rows_stride(*residual) < 0))
+        return py::none();
+    if (out && (out->scalar_type() != x.scalar_type() || out->sizes() != at::IntArrayRef(shape) || !out->is_contiguous() ||
+                overlaps(*out, x) || overlaps(*out, w) || overlaps(*out, w_scale) || (bias && overlaps(*out, *bias)) ||
+                (residual && overlaps(*out, *residual))))
+        return py::none();
+    Tensor y;
+    const int status = run(plain.dev, [&](void* stream) -> int {
+        y = out ? *out : at::empty(shape, x.options().requires_grad(false));
+        kda_mx4_linear_args a{};
+        a.K = x.size(-1); a.N = N; a.M = x.numel() / a.K;
+        a.x = x.data_ptr();
+        a.x_stride = rows_stride(x);
+        a.w = w.data_ptr();
+        a.w_scale = w_scale.data_ptr();
+        a.bias = bias ? bias->data_ptr() : nullptr;
+        if (residual) {
+            a.residual = residual->data_ptr();
+            a.residual_stride = rows_stride(*residual);
+        }
+        a.y = y.data_ptr();
+        a.dtype = code(x);
+        return fn.mx4_linear(&a, stream);
+    });
+    if (refused(status, "kda_mx4_linear_fwd")) return py::none();
+    if (out && !out->is_inference()) out->unsafeGetTensorImpl()->bump_version();
+    return py::cast(y);
+}
+
+// mx4_quantize: (data [.., K / 2], scale [.., K / 32]) of w [.., K], or None.
+py::object mx4_quantize(const Tensor& w) {
+    Plain plain(w);
+    if (!plain.ok || traced() || w.dim() < 1 || w.size(-1) == 0 || w.size(-1) % 32 != 0 || code(w) < 0 || !mx4_rows(w))
+        return py::none();
+    Tensor data, scale;
+    const int status = run(plain.dev, [&](void* stream) -> int {
+        const auto opt = w.options().requires_grad(false);
+        auto shape = w.sizes().vec();
+        shape.back() = w.size(-1) / 2;
+        data = at::empty(shape, opt.dtype(at::kFloat4_e2m1fn_x2));
+        shape.back() = w.size(-1) / 32;
+        scale = at::empty(shape, opt.dtype(at::kFloat8_e8m0fnu));
+        kda_mx4_convert_args a{};
+        a.K = w.size(-1); a.N = w.numel() / a.K;
+        a.values = w.data_ptr();
+        a.value_stride = rows_stride(w);
+        a.data = data.data_ptr();
+        a.scale = scale.data_ptr();
+        a.dtype = code(w);
+        return fn.mx4_quantize(&a, stream);
+    });
+    if (refused(status, "kda_mx4_quantize")) return py::none();
+    return py::make_tuple(data, scale);
+}
+
+// mx4_dequantize: [.., K], or None.
+py::object mx4_dequantize(const Tensor& data, const Tensor& scale, at::ScalarType dtype) {
+    Plain plain(data);
+    plain.add(scale);
+    if (!plain.ok || traced() || (dtype != at::kHalf && dtype != at::kBFloat16) || !mx4_ok(data, scale)) return py::none();
+    Tensor out;
+    const int status = run(plain.dev, [&](void* stream) -> int {
+        auto shape = data.sizes().vec();
+        shape.back() *= 2;
+        out = at::empty(shape, data.options().dtype(dtype).requires_grad(false));
+        kda_mx4_convert_args a{};
+        a.K = shape.back(); a.N = out.numel() / a.K;
+        a.values = out.data_ptr();
+        a.value_stride = a.K;
+        a.data = data.data_ptr();
+        a.scale = scale.data_ptr();
+        a.dtype = code(out);
+        return fn.mx4_dequantize(&a, stream);
+    });
+    if (refused(status, "kda_mx4_dequantize")) return py::none();
     return py::cast(out);
 }
 
@@ -925,6 +1060,9 @@ PYBIND11_MODULE(_kda_host, m) {
     m.def("mla_absorbed", &mla_absorbed);
     m.def("mla_append", &mla_append);
     m.def("mla_read", &mla_read);
+    m.def("mx4_linear", &mx4_linear);
+    m.def("mx4_quantize", &mx4_quantize);
+    m.def("mx4_dequantize", &mx4_dequantize);
     m.def("traced", &traced);
     m.def("params_key", &params_key);
 }

@@ -289,6 +289,51 @@ int kda_linear_wgrad(const kda_linear_wgrad_args* a, void* stream) {
     return kda::linear_wgrad_launch(*a, static_cast<hipStream_t>(stream));
 }
 
+// Matrices in 4 bits: sizes that the kernels' 32-bit offsets reach.
+constexpr int64_t kMx4Depth = int64_t{1} << 22;
+
+int kda_mx4_linear_fwd(const kda_mx4_linear_args* a, void* stream) {
+    if (a == nullptr) return KDA_ERR_NULL_POINTER;
+    if (a->M < 0 || a->N < 0 || a->K <= 0 || a->K > kMx4Depth || a->M > INT32_MAX || a->N > INT32_MAX) return KDA_ERR_BAD_SHAPE;
+    if ((a->M + 127) / 128 > 65535) return KDA_ERR_BAD_SHAPE;
+    if (a->dtype != KDA_DTYPE_F16 && a->dtype != KDA_DTYPE_BF16) return KDA_ERR_BAD_DTYPE;
+    if (a->K % 32 != 0) return KDA_ERR_UNSUPPORTED;
+    if (a->M == 0 || a->N == 0) return KDA_OK;
+    if (!a->x || !a->w || !a->w_scale || !a->y) return KDA_ERR_NULL_POINTER;
+    const auto at = [](const void* p, uintptr_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; };
+    if (!at(a->x, 16) || a->x_stride < 0 || a->x_stride % 8 != 0 || a->x_stride > kMx4Depth || !at(a->w, 16) || !at(a->y, 8) ||
+        !at(a->bias, 2) || !at(a->residual, 2) || a->residual_stride < 0)
+        return KDA_ERR_UNSUPPORTED;
+    return kda::mx4_linear_launch(*a, static_cast<hipStream_t>(stream));
+}
+
+namespace {
+int mx4_convert_check(const kda_mx4_convert_args* a, bool f32) {
+    if (a == nullptr) return KDA_ERR_NULL_POINTER;
+    if (a->N < 0 || a->K <= 0 || a->K >= int64_t{1} << 32 || a->N >= (int64_t{1} << 35) / a->K) return KDA_ERR_BAD_SHAPE;
+    if (a->dtype != KDA_DTYPE_F16 && a->dtype != KDA_DTYPE_BF16 && !(f32 && a->dtype == KDA_DTYPE_F32)) return KDA_ERR_BAD_DTYPE;
+    if (a->K % 32 != 0) return KDA_ERR_UNSUPPORTED;
+    if (a->N == 0) return KDA_OK;
+    if (!a->values || !a->data || !a->scale) return KDA_ERR_NULL_POINTER;
+    const int64_t bytes = a->dtype == KDA_DTYPE_F32 ? 4 : 2;
+    if (reinterpret_cast<uintptr_t>(a->values) % 16 != 0 || a->value_stride < 0 || a->value_stride * bytes % 16 != 0 ||
+        reinterpret_cast<uintptr_t>(a->data) % 16 != 0)
+        return KDA_ERR_UNSUPPORTED;
+    return KDA_OK;
+}
+}  // namespace
+
+int kda_mx4_quantize(const kda_mx4_convert_args* a, void* stream) {
+    if (const int st = mx4_convert_check(a, true); st != KDA_OK) return st;
+    return a->N == 0 ? static_cast<int>(KDA_OK) : kda::mx4_quantize_launch(*a, static_cast<hipStream_t>(stream));
+}
+
+int kda_mx4_dequantize(const kda_mx4_convert_args* a, void* stream) {
+    if (const int st = mx4_convert_check(a, false); st != KDA_OK) return st;
+    if (a->N > 1 && a->value_stride < a->K) return KDA_ERR_UNSUPPORTED;      // rows that share memory
+    return a->N == 0 ? static_cast<int>(KDA_OK) : kda::mx4_dequantize_launch(*a, static_cast<hipStream_t>(stream));
+}
+
 const char* kda_status_str(int status) {
     switch (status) {
         case KDA_OK: return "ok";

@@ -77,6 +77,11 @@ bool linear_wgrad_supported(int64_t M, int64_t N, int64_t K);
 int64_t linear_wgrad_workspace_bytes(int64_t M, int64_t N, int64_t K);
 int linear_wgrad_launch(const kda_linear_wgrad_args& a, hipStream_t stream);
 
+// Matrices in 4 bits (kda_mx4.hip); arguments checked by the caller, no work of size zero.
+int mx4_linear_launch(const kda_mx4_linear_args& a, hipStream_t stream);
+int mx4_quantize_launch(const kda_mx4_convert_args& a, hipStream_t stream);
+int mx4_dequantize_launch(const kda_mx4_convert_args& a, hipStream_t stream);
+
 
 // Latent attention (kda_mla_*.hip); arguments checked by the caller, no work
 // of size zero.

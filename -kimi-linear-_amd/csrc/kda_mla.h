@@ -61,6 +61,11 @@ template <> struct Act<_Float16> {
     static __device__ __forceinline__ uint32_t from8(uint32_t w) {
         return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.f, HI));
     }
+    // two e2m1 values of a word (its byte BYTE) times a power of two, rounded once (255 as the exponent: NaN)
+    template <int BYTE>
+    static __device__ __forceinline__ uint32_t from4(uint32_t w, float power) {
+        return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, power, BYTE));
+    }
 };
 template <> struct Act<bf16_t> {
     static __device__ __forceinline__ f4 mma16(uint4 a, uint4 b, f4 c) {
@@ -76,6 +81,10 @@ template <> struct Act<bf16_t> {
     static __device__ __forceinline__ uint32_t from8(uint32_t w) {
         return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.f, HI));
     }
+    template <int BYTE>
+    static __device__ __forceinline__ uint32_t from4(uint32_t w, float power) {
+        return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, power, BYTE));
+    }
 };
 
 // Eight e4m3 values in the activation type.
@@ -83,6 +92,28 @@ template <typename T>
 __device__ __forceinline__ uint4 widen8(uint32_t lo, uint32_t hi) {
     return uint4{Act<T>::template from8<false>(lo), Act<T>::template from8<true>(lo),
                  Act<T>::template from8<false>(hi), Act<T>::template from8<true>(hi)};
+}
+
+// Eight e2m1 values, the low half of a byte first, times a power of two.
+template <typename T>
+__device__ __forceinline__ uint4 widen4(uint32_t w, float power = 1.f) {
+    return uint4{Act<T>::template from4<0>(w, power), Act<T>::template from4<1>(w, power),
+                 Act<T>::template from4<2>(w, power), Act<T>::template from4<3>(w, power)};
+}
+
+// The exponent + 127 of a group of e2m1 values whose largest magnitude has the bits `top`: the least
+// power that leaves at most 7, beyond which the nearest value, 6, would be further off than half
+// the format's widest step.  255 (NaN) where a value is not finite.
+__device__ __forceinline__ uint32_t group_exponent(uint32_t top, uint32_t least) {
+    return top >= 0x7f800000u ? 255u : max(static_cast<int>((top + 0x1fffffu) >> 23) - 2, static_cast<int>(least));
+}
+// Eight values divided by 2^(e - 127), which is exact, to the nearest e2m1 ones, ties to the even one.
+__device__ __forceinline__ uint32_t narrow4(const float (&x)[8], uint32_t e) {
+    const float power = __uint_as_float(e << 23);
+    uint32_t w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, x[0], x[1], power, 0);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[2], x[3], power, 1);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[4], x[5], power, 2);
+    return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[6], x[7], power, 3);
 }
 
 // Four 16-bit values of one column from a row-major LDS tile: within 16 lanes,
@@ -100,6 +131,14 @@ __device__ __forceinline__ uint2 read_tr8(const void* p) {
     typedef int i2 __attribute__((ext_vector_type(2)));
     typedef __attribute__((address_space(3))) i2* lds_i2;
     return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i2)(reinterpret_cast<const i2*>(p))));
+}
+
+// Sixteen 4-bit values of one column: within 16 lanes, lane i gets rows 0..15 of
+// column i where lane r points at row r, all sixteen columns.
+__device__ __forceinline__ uint2 read_tr4(const void* p) {
+    typedef int i2 __attribute__((ext_vector_type(2)));
+    typedef __attribute__((address_space(3))) i2* lds_i2;
+    return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr4_b64_v2i32((lds_i2)(reinterpret_cast<const i2*>(p))));
 }
 
 // Four neighbouring outputs, and where `low` is there what rounding took from each.

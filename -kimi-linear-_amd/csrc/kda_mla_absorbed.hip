@@ -46,11 +46,12 @@ using namespace mla;
 
 constexpr int kUnit = 16;         // keys of a wave's part of a window
 constexpr int kRows = 16;         // query rows of a workgroup
+constexpr int kGroup = 128;       // latent channels of a 4-bit cache's scale
 constexpr int WAVES = 4, kThreads = 64 * WAVES;
 
 // Workspace: for every slot (a workgroup's part of a row tile's sequence) the
-// rows' sums, [16][R] fp32, and their (maximum, denominator); for every row
-// tile the first and last workgroup that has a part of it.
+// rows' sums, [16][R] fp32, and their (maximum, denominator), in 4 bits for each group
+// of 128 channels; for every row tile the first and last workgroup that has a part of it.
 struct Workspace {
     float* o;
     float2* ml;
@@ -61,7 +62,7 @@ __host__ __device__ inline Workspace carve(void* p, int64_t n_slots, int64_t R) 
     Workspace w;
     w.o = static_cast<float*>(p);
     w.ml = reinterpret_cast<float2*>(w.o + n_slots * kRows * R);
-    w.span = reinterpret_cast<int2*>(w.ml + n_slots * kRows);
+    w.span = reinterpret_cast<int2*>(w.ml + n_slots * kRows * (R / kGroup));
     return w;
 }
 
@@ -121,32 +122,37 @@ __device__ __forceinline__ void landed() { asm volatile("s_waitcnt vmcnt(0)" :::
 // pieces (the score product's reads) and the rows of a transposed read (the value
 // product's) are in different banks.  8-bit values are widened after they are
 // read from LDS, by each product for itself.
-template <typename T, bool F8, int R, int P>
+template <typename T, int BITS, int R, int P>
 struct Kernel {
+    static constexpr bool F8 = BITS == 8, F4 = BITS == 4;
     static constexpr int D = R + P, kWindow = kUnit * WAVES, kSteps = D / 32, kScore = kWindow + 4;
     static constexpr int kTiles = R / 16 / WAVES;               // 16-channel tiles of a wave
-    static constexpr int ES = F8 ? 1 : 2, RB = R * ES, PB = P * ES;              // bytes
+    static constexpr int ES = BITS == 16 ? 2 : 1, RB = R * BITS / 8, PB = P * BITS / 8;   // bytes (of a stride's unit, a row)
+    static constexpr int kScales = F4 ? R / kGroup : 1;         // scales of a row's latent part
     static constexpr int kLatRows = 1024 / RB, kLat = kUnit / kLatRows;          // rows a load, loads a unit
     static constexpr int kPosRows = P == 0 || 1024 / PB > kUnit ? kUnit : 1024 / PB, kPos = P == 0 ? 0 : kUnit / kPosRows;
     static constexpr int kPosUnit = kPos * 1024;                // bytes of a unit's position parts (whole loads)
     static constexpr int kPosAt = kWindow * RB, kScaleAt = kPosAt + WAVES * kPosUnit;
-    static constexpr int kBuffer = kScaleAt + (F8 ? WAVES * 256 : 0);
+    static constexpr int kBuffer = kScaleAt + (BITS < 16 ? WAVES * 256 : 0);
     static_assert(kBuffer >= kRows * (D + 8) * 2, "the queries pass through a buffer");
 
     struct Shared {
         char buf[2][kBuffer];            // [kWindow][R], [WAVES][kPosUnit], scales
         float s[kRows][kScore];
         float inv[F8 ? kWindow : 4];
+        float e[F4 ? kScales : 1][F4 ? kWindow : 4];         // log2 of the groups' scales
     };
 
     // Where piece c of row r lies: of the latent, with r = r0 + x, r0 a multiple of the rows of a load and x
     // within one, and of the position part.
     static __device__ __forceinline__ int turn(int r) {
-        return RB >= 256 ? ((r << 1) & 14) | ((r >> 3) & 1) : (r >> 1) & 7;
+        return RB >= 256 ? ((r << 1) & 14) | ((r >> 3) & 1) : (RB == 128 ? (r >> 1) & 7 : (r >> 2) & 3);
     }
-    static __device__ __forceinline__ int turn(int r0, int x) { return turn(r0) ^ (RB >= 256 ? x << 1 : x >> 1); }
+    static __device__ __forceinline__ int turn(int r0, int x) {
+        return turn(r0) ^ (RB >= 256 ? x << 1 : (RB == 128 ? x >> 1 : x >> 2));
+    }
     static __device__ __forceinline__ int pos_piece(int r, int c) {
-        return c ^ (PB == 128 ? (r >> 1) & 7 : (PB == 64 ? (r >> 2) & 3 : (r >> 3) & 1));
+        return PB < 32 ? c : c ^ (PB == 128 ? (r >> 1) & 7 : (PB == 64 ? (r >> 2) & 3 : (r >> 3) & 1));
     }
 
     // A unit's rows, keys j.. of which those past hi - 1 repeat it, into their place in a buffer.
@@ -171,8 +177,13 @@ struct Kernel {
         }
         if constexpr (F8) {
             const int r = (lane >> 1) & 15;
-            word_to_lds(a.cache_scale + b * a.scale_stride[0] + base * a.scale_stride[1],
+            word_to_lds(static_cast<const float*>(a.cache_scale) + b * a.scale_stride[0] + base * a.scale_stride[1],
                         (min(r, last) * static_cast<int>(a.scale_stride[1]) + (lane & 1)) * 4, buf + kScaleAt + 256 * wave);
+        }
+        if constexpr (F4) {
+            const int r = (lane >> 1) & 15;
+            word_to_lds(static_cast<const uint8_t*>(a.cache_scale) + b * a.scale_stride[0] + base * a.scale_stride[1],
+                        min(r, last) * static_cast<int>(a.scale_stride[1]) + 4 * (lane & 1), buf + kScaleAt + 256 * wave);
         }
     }
 
@@ -181,13 +192,19 @@ struct Kernel {
         f4 o[kTiles];
         float top, sum;
     };
-    // Channels of step k that lane group lg has: in 8 bits a 16-byte piece is two steps'.
+    // Channels of step k that lane group lg has: in 8 bits a 16-byte piece is two steps', in 4 bits four steps'.
     static __device__ __forceinline__ int channel(int k, int lg) {
+        if constexpr (F4) return k < R / 32 ? 128 * (k / 4) + 32 * lg + 8 * (k % 4) : 32 * k + 8 * lg;
         return F8 && k < R / 32 ? 64 * (k / 2) + 16 * lg + 8 * (k % 2) : 32 * k + 8 * lg;
     }
 
-    // The scores of the wave's unit, keys 4 lg + i of row ln: times scale log2(e), plus log2 of the key's scale.
-    static __device__ __forceinline__ f4 scores(const char* buf, const State& st, float c, float* inv, int wave, int ln,
+    // A scale of a 4-bit cache, byte i of a row's word: NaN's code gives infinity.
+    static __device__ __forceinline__ float power(uint32_t w, int i) {
+        return __uint_as_float((w >> (8 * i) & 255u) << 23);
+    }
+
+    // The scores of the wave's unit, keys 4 lg + i of row ln: times scale log2(e), plus log2 of an 8-bit key's scale.
+    static __device__ __forceinline__ f4 scores(const char* buf, const State& st, float c, Shared& sh, int wave, int ln,
                                                 int lg) {
         const char* row = buf + (kUnit * wave + ln) * RB;
         const char* pos = buf + kPosAt + wave * kPosUnit + ln * PB;
@@ -195,16 +212,18 @@ struct Kernel {
         constexpr int kReads = RB / 64;
         u4 piece[kReads];                // all asked for before the first product: nothing else hides their latency
         typedef uint32_t u2 __attribute__((ext_vector_type(2)));
-        u4 tail[F8 || P == 0 ? 1 : P / 32];
+        u4 tail[BITS < 16 || P == 0 ? 1 : P / 32];
         u2 tail8[F8 && P ? P / 32 : 1];
+        uint32_t tail4[F4 && P ? P / 32 : 1];
 #pragma unroll
         for (int k = 0; k < kReads; ++k) {
-            constexpr int kLow = RB >= 256 ? 4 : 2;              // reads whose pieces are turned among themselves
+            constexpr int kLow = RB >= 256 ? 4 : RB / 64;        // reads whose pieces are turned among themselves
             piece[k] = *reinterpret_cast<const u4*>(row + 64 * kLow * (k / kLow) + 16 * ((4 * (k % kLow) + lg) ^ f));
         }
 #pragma unroll
         for (int k = 0; k < P / 32; ++k) {
-            if constexpr (F8) tail8[k] = *reinterpret_cast<const u2*>(pos + 16 * pos_piece(ln, 2 * k + (lg >> 1)) + 8 * (lg & 1));
+            if constexpr (F4) tail4[k] = *reinterpret_cast<const uint32_t*>(pos + 16 * pos_piece(ln, k) + 4 * lg);
+            else if constexpr (F8) tail8[k] = *reinterpret_cast<const u2*>(pos + 16 * pos_piece(ln, 2 * k + (lg >> 1)) + 8 * (lg & 1));
             else tail[k] = *reinterpret_cast<const u4*>(pos + 16 * pos_piece(ln, 4 * k + lg));
         }
         f4 s;
@@ -228,7 +247,32 @@ struct Kernel {
                 s[i] = fmaf((lat[i] + odd[i]) * sl[i] + far[i] * sp[i], c, __builtin_amdgcn_logf(sl[i]));
                 r[i] = __builtin_amdgcn_rcpf(sl[i]);
             }
-            if (ln == 0) *reinterpret_cast<f4*>(inv + kUnit * wave + 4 * lg) = r;
+            if (ln == 0) *reinterpret_cast<f4*>(sh.inv + kUnit * wave + 4 * lg) = r;
+        } else if constexpr (F4) {
+            // a piece is one key's 32 channels, so four products on end are of one group
+            const char* scale = buf + kScaleAt + 256 * wave;
+            const u4 w01 = *reinterpret_cast<const u4*>(scale + 32 * lg), w23 = *reinterpret_cast<const u4*>(scale + 32 * lg + 16);
+            const int byte = *reinterpret_cast<const uint8_t*>(scale + 8 * ln + (lg < kScales ? lg : 0));
+            stay();
+            f4 lat[kReads], far{};
+#pragma unroll
+            for (int k = 0; k < kReads; ++k) lat[k] = f4{};
+#pragma unroll
+            for (int n = 0; n < 4; ++n)
+#pragma unroll
+                for (int k = 0; k < kReads; ++k) lat[k] = Act<T>::mma16(widen4<T>(piece[k][n]), st.q[4 * k + n], lat[k]);
+#pragma unroll
+            for (int k = 0; k < P / 32; ++k) far = Act<T>::mma16(widen4<T>(tail4[k]), st.q[R / 32 + k], far);
+            const uint32_t w[4][2] = {{w01[0], w01[1]}, {w01[2], w01[3]}, {w23[0], w23[1]}, {w23[2], w23[3]}};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float x = P > 0 ? far[i] * power(w[i][kScales / 4], kScales % 4) : 0.f;
+#pragma unroll
+                for (int k = 0; k < kReads; ++k) x = fmaf(lat[k][i], power(w[i][0], k), x);
+                x *= c;
+                s[i] = fmaf(x, 0.f, x);          // an infinity is a scale's NaN
+            }
+            if (lg < kScales) sh.e[lg][kUnit * wave + ln] = byte == 255 ? __builtin_nanf("") : static_cast<float>(byte - 127);
         } else {
             stay();
             f4 acc{}, odd{};
@@ -246,13 +290,16 @@ struct Kernel {
         return s;
     }
 
+    // First of the eight keys of a window that lane group lg has in step k of the value product.
+    static __device__ __forceinline__ int at(int k, int lg) { return F4 ? 16 * lg + 8 * k : 32 * k + 8 * lg; }
+
     // A window at keys j0..; its rows are in `buf`, the next window's are asked for into `next`.
     static __device__ __forceinline__ void window(const kda_mla_absorbed_args& a, int64_t b, int j0, int hi, int limit,
                                                   float c, int wave, int lane, const char* buf, char* next, Shared& sh,
                                                   State& st) {
         const int ln = lane & 15, lg = lane >> 4;
         if (j0 + kWindow < hi) load(a, b, j0 + kWindow + kUnit * wave, hi, wave, lane, next);
-        f4 s = scores(buf, st, c, sh.inv, wave, ln, lg);
+        f4 s = scores(buf, st, c, sh, wave, ln, lg);
         const int key = j0 + kUnit * wave + 4 * lg;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -262,10 +309,17 @@ struct Kernel {
 
         uint4 p[kWindow / 32];
         float x[kWindow / 32][8], mx = kNoMax;
+        f4 e2[kWindow / 32][2];
 #pragma unroll
         for (int k = 0; k < kWindow / 32; ++k) {
-            const f4* from = reinterpret_cast<const f4*>(&sh.s[ln][32 * k + 8 * lg]);
-            const f4 lo4 = from[0], hi4 = from[1];
+            const f4* from = reinterpret_cast<const f4*>(&sh.s[ln][at(k, lg)]);
+            f4 lo4 = from[0], hi4 = from[1];
+            if constexpr (F4) {                  // each wave against its own channels' scales
+                const f4* more = reinterpret_cast<const f4*>(&sh.e[kScales * wave / WAVES][at(k, lg)]);
+                e2[k][0] = more[0], e2[k][1] = more[1];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) lo4[e] += e2[k][0][e], hi4[e] += e2[k][1][e];
+            }
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 x[k][e] = lo4[e];
@@ -287,7 +341,9 @@ struct Kernel {
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 x[k][e] = __builtin_amdgcn_exp2f(x[k][e] - mx);
-                part = F8 ? fmaf(x[k][e], inv[e / 4][e % 4], part) : part + x[k][e];
+                if constexpr (F8) part = fmaf(x[k][e], inv[e / 4][e % 4], part);
+                else if constexpr (F4) part += __builtin_amdgcn_ldexpf(x[k][e], -static_cast<int>(e2[k][e / 4][e % 4]));
+                else part += x[k][e];
             }
             p[k] = uint4{Act<T>::pair(x[k][0], x[k][1]), Act<T>::pair(x[k][2], x[k][3]), Act<T>::pair(x[k][4], x[k][5]),
                          Act<T>::pair(x[k][6], x[k][7])};
@@ -306,13 +362,19 @@ struct Kernel {
     static __device__ __forceinline__ void values(const char* buf, const uint4 (&p)[kWindow / 32], int wave, int ln, int lg,
                                                   State& st) {
         constexpr int kAtOnce = kTiles < 4 ? kTiles : 4;
-        constexpr int kMask = RB >= 256 ? 15 : 7;
+        constexpr int kMask = RB >= 256 ? 15 : RB / 16 - 1;
+        static_assert(!F4 || kWindow == 64, "a 4-bit transposed read gives a lane group a quarter of the window");
 #pragma unroll
         for (int i0 = 0; i0 < kTiles; i0 += kAtOnce) {
-            uint2 y[kAtOnce][kWindow / 32][F8 ? 1 : 2];
+            uint2 y[kAtOnce][F4 ? 1 : kWindow / 32][F8 || F4 ? 1 : 2];
 #pragma unroll
             for (int i = 0; i < kAtOnce; ++i) {
-                if constexpr (F8) {
+                if constexpr (F4) {
+                    // sixteen rows of sixteen channels, all of the lane group's keys: a lane points at row ln's
+                    const int tile = kTiles * wave + i0 + i, c = tile >> 1;
+                    y[i][0][0] = read_tr4(buf + (16 * lg + ln) * RB + 16 * ((c & ~kMask) | ((c & kMask) ^ turn(ln))) +
+                                          8 * (tile & 1));
+                } else if constexpr (F8) {
                     // eight rows of sixteen channels: a lane points at eight channels of row ln / 2
                     const int r = 8 * lg + (ln >> 1), at = kTiles * wave + i0 + i;
                     const char* v = buf + r * RB + 16 * ((at & ~kMask) | ((at & kMask) ^ turn(r & 15))) + 8 * (ln & 1);
@@ -336,7 +398,8 @@ struct Kernel {
 #pragma unroll
                 for (int k = 0; k < kWindow / 32; ++k) {
                     uint4 v;
-                    if constexpr (F8) v = widen8<T>(y[i][k][0].x, y[i][k][0].y);
+                    if constexpr (F4) v = widen4<T>(k == 0 ? y[i][0][0].x : y[i][0][0].y);
+                    else if constexpr (F8) v = widen8<T>(y[i][k][0].x, y[i][k][0].y);
                     else v = uint4{y[i][k][0].x, y[i][k][0].y, y[i][k][1].x, y[i][k][1].y};
                     st.o[i0 + i] = Act<T>::mma16(v, p[k], st.o[i0 + i]);
                 }
@@ -397,7 +460,9 @@ struct Kernel {
             float* out = ws.o + (slot * kRows + ln) * R + ch;
 #pragma unroll
             for (int i = 0; i < kTiles; ++i) *reinterpret_cast<f4*>(out + 16 * i) = st.o[i];
-            if (wave == 0 && lg == 0) ws.ml[slot * kRows + ln] = float2{st.top, den};
+            constexpr int kPerGroup = WAVES / kScales;
+            if (wave % kPerGroup == 0 && lg == 0)
+                ws.ml[(slot * kScales + wave / kPerGroup) * kRows + ln] = float2{st.top, den};
         }
     }
 };
@@ -423,9 +488,9 @@ __device__ __forceinline__ int wave_scan(int x, int lane) {
 // 74 / 73; in 8 bits 64 of 64 to 4096 29 / 24, but 52 of 8192 52 / 57.  One rule for both
 // widths: batches whose lengths differ gain in both.
 constexpr int kLeast = 8, kCut = 64;
-template <typename T, bool F8, int R, int P>
-__global__ __launch_bounds__(kThreads, F8 ? 2 : 1) void absorbed_kernel(kda_mla_absorbed_args a, int rts, bool alone) {
-    using K = Kernel<T, F8, R, P>;
+template <typename T, int BITS, int R, int P>
+__global__ __launch_bounds__(kThreads, BITS < 16 ? 2 : 1) void absorbed_kernel(kda_mla_absorbed_args a, int rts, bool alone) {
+    using K = Kernel<T, BITS, R, P>;
     __shared__ __align__(16) typename K::Shared sh;
     const int lane = threadIdx.x & 63, nv = static_cast<int>(a.B) * rts, group = static_cast<int>(blockIdx.x);
     if (alone) {
@@ -513,8 +578,9 @@ __global__ __launch_bounds__(kThreads, F8 ? 2 : 1) void absorbed_kernel(kda_mla_
 // The parts of one row's sequence joined: grid (row tiles, their rows, R / 4 /
 // LANES), LANES lanes on 4 channels each and 256 / LANES groups of them on every
 // so-manieth part, whose sums meet in LDS, in an order that the lengths alone decide.
+// scales: the channel groups that have a maximum and a denominator of their own.
 template <typename T, int LANES>
-__global__ __launch_bounds__(256) void join_kernel(kda_mla_absorbed_args a, int rts, int groups) {
+__global__ __launch_bounds__(256) void join_kernel(kda_mla_absorbed_args a, int rts, int groups, int scales) {
     const int64_t v = blockIdx.x, b = v / rts, nv = a.B * rts;
     const int rows = static_cast<int>(a.T * a.H), m = static_cast<int>(v - b * rts) * kRows + blockIdx.y;
     if (m >= rows) return;
@@ -524,7 +590,8 @@ __global__ __launch_bounds__(256) void join_kernel(kda_mla_absorbed_args a, int 
     int2 span = ws.span[v];                      // (asked for with the length; unwritten where that is zero)
     if (tokens(a.lengths, b, a.S) == 0) span = int2{0, -1};
     if (span.x == span.y) return;                // one workgroup had it all, and wrote the result
-    const float2* ml = ws.ml + v * kRows + blockIdx.y;
+    const int per = kRows * scales, own = scales > 1 ? c / kGroup : 0;
+    const float2* ml = ws.ml + v * per + own * kRows + blockIdx.y;
     const float* o = ws.o + (v * kRows + blockIdx.y) * a.R + c;
     float top = kNoMax, den = 0.f;
     f4 r{};
@@ -536,7 +603,7 @@ __global__ __launch_bounds__(256) void join_kernel(kda_mla_absorbed_args a, int 
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) {
             const int at_g = min(g + i * kJoinGroups, span.y);
-            x[i] = ml[at_g * kRows];
+            x[i] = ml[at_g * per];
             y[i] = *reinterpret_cast<const f4*>(o + static_cast<int64_t>(at_g) * kRows * a.R);
         }
         float now = top;
@@ -559,18 +626,19 @@ __global__ __launch_bounds__(256) void join_kernel(kda_mla_absorbed_args a, int 
         }
     }
     __shared__ f4 sums[kJoinGroups][LANES];
-    __shared__ float2 stats[kJoinGroups];
+    constexpr int kStats = LANES > 32 ? LANES / 32 : 1;          // channel groups of the lanes
+    __shared__ float2 stats[kJoinGroups][kStats];
     sums[group][at] = r;
-    if (at == 0) stats[group] = float2{top, den};
+    if (at % 32 == 0) stats[group][at / 32] = float2{top, den};
     __syncthreads();
     if (group != 0) return;
     const int n = min(kJoinGroups, span.y - span.x + 1);
-    for (int g = 0; g < n; ++g) top = fmaxf(top, stats[g].x);
+    for (int g = 0; g < n; ++g) top = fmaxf(top, stats[g][at / 32].x);
     den = 0.f;
     r = f4{};
     for (int g = 0; g < n; ++g) {
-        const float w = __builtin_amdgcn_exp2f(stats[g].x - top);
-        den = fmaf(w, stats[g].y, den);
+        const float w = __builtin_amdgcn_exp2f(stats[g][at / 32].x - top);
+        den = fmaf(w, stats[g][at / 32].y, den);
         const f4 y = sums[g][at];
 #pragma unroll
         for (int e = 0; e < 4; ++e) r[e] = fmaf(w, y[e], r[e]);
@@ -594,39 +662,40 @@ static_assert(kGroups > kCut);
 // 183, up to 1024 46 / 44; 600 up to 1024 104 / 97, in 8 bits 71 / 57.
 bool shared_form(int64_t nv, int64_t S) { return nv < 512 && S > 512; }
 
-template <typename T, bool F8, int R, int P>
+template <typename T, int BITS, int R, int P>
 int launch(const kda_mla_absorbed_args& a, hipStream_t stream) {
     const int rts = row_tiles(a.T, a.H);
     const int64_t nv = a.B * rts;
     if (!shared_form(nv, a.S)) {
-        absorbed_kernel<T, F8, R, P><<<static_cast<unsigned>(nv), kThreads, 0, stream>>>(a, rts, true);
+        absorbed_kernel<T, BITS, R, P><<<static_cast<unsigned>(nv), kThreads, 0, stream>>>(a, rts, true);
     } else {
         constexpr int groups = static_cast<int>(kGroups);
-        absorbed_kernel<T, F8, R, P><<<groups, kThreads, 0, stream>>>(a, rts, false);
+        absorbed_kernel<T, BITS, R, P><<<groups, kThreads, 0, stream>>>(a, rts, false);
         // many rows have few parts each, and few rows may have many
         const dim3 grid(static_cast<unsigned>(nv), kRows);
+        constexpr int scales = Kernel<T, BITS, R, P>::kScales;
         if (nv >= 32)
-            join_kernel<T, R / 4><<<grid, 256, 0, stream>>>(a, rts, groups);
+            join_kernel<T, R / 4><<<grid, 256, 0, stream>>>(a, rts, groups, scales);
         else
-            join_kernel<T, 16><<<dim3(grid.x, grid.y, R / 64), 256, 0, stream>>>(a, rts, groups);
+            join_kernel<T, 16><<<dim3(grid.x, grid.y, R / 64), 256, 0, stream>>>(a, rts, groups, scales);
     }
     return hipGetLastError() == hipSuccess ? KDA_OK : KDA_ERR_LAUNCH;
 }
 
-template <typename T, bool F8, int R>
+template <typename T, int BITS, int R>
 int launch_pos(const kda_mla_absorbed_args& a, hipStream_t stream) {
     switch (a.P) {
-        case 64: return launch<T, F8, R, 64>(a, stream);
-        case 32: return launch<T, F8, R, 32>(a, stream);
-        default: return launch<T, F8, R, 0>(a, stream);
+        case 64: return launch<T, BITS, R, 64>(a, stream);
+        case 32: return launch<T, BITS, R, 32>(a, stream);
+        default: return launch<T, BITS, R, 0>(a, stream);
     }
 }
-template <typename T, bool F8>
+template <typename T, int BITS>
 int launch_rank(const kda_mla_absorbed_args& a, hipStream_t stream) {
     switch (a.R) {
-        case 512: return launch_pos<T, F8, 512>(a, stream);
-        case 256: return launch_pos<T, F8, 256>(a, stream);
-        default: return launch_pos<T, F8, 128>(a, stream);
+        case 512: return launch_pos<T, BITS, 512>(a, stream);
+        case 256: return launch_pos<T, BITS, 256>(a, stream);
+        default: return launch_pos<T, BITS, 128>(a, stream);
     }
 }
 
@@ -635,13 +704,16 @@ int launch_rank(const kda_mla_absorbed_args& a, hipStream_t stream) {
 int64_t mla_absorbed_workspace_bytes(int64_t B, int64_t T, int64_t H, int64_t S, int64_t R) {
     const int64_t nv = B * row_tiles(T, H);
     if (nv == 0 || !shared_form(nv, S)) return 0;
-    return slots(kGroups, nv) * kRows * (R * 4 + 8) + nv * 8;
+    return slots(kGroups, nv) * kRows * (R * 4 + 8 * (R / kGroup)) + nv * 8;
 }
 
 int mla_absorbed_launch(const kda_mla_absorbed_args& a, hipStream_t stream) {
-    if (a.cache_dtype == KDA_DTYPE_E4M3)
-        return a.dtype == KDA_DTYPE_F16 ? launch_rank<_Float16, true>(a, stream) : launch_rank<bf16_t, true>(a, stream);
-    return a.dtype == KDA_DTYPE_F16 ? launch_rank<_Float16, false>(a, stream) : launch_rank<bf16_t, false>(a, stream);
+    const bool half = a.dtype == KDA_DTYPE_F16;
+    switch (a.cache_dtype) {
+        case KDA_DTYPE_E2M1: return half ? launch_rank<_Float16, 4>(a, stream) : launch_rank<bf16_t, 4>(a, stream);
+        case KDA_DTYPE_E4M3: return half ? launch_rank<_Float16, 8>(a, stream) : launch_rank<bf16_t, 8>(a, stream);
+        default: return half ? launch_rank<_Float16, 16>(a, stream) : launch_rank<bf16_t, 16>(a, stream);
+    }
 }
 
 }  // namespace kda

@@ -42,6 +42,17 @@ bool sizes_ok(int64_t B, int64_t T, int64_t S, int64_t H) {
     return B >= 0 && T >= 0 && S >= 0 && H >= 0 && T <= kMaxTokens && S <= kMaxTokens && B <= kMaxGrid && H <= kMaxGrid;
 }
 
+// 16 bits a channel as the activations, or 8 or 4.
+bool cache_type(int32_t d, int32_t act_dtype) { return d == act_dtype || d == KDA_DTYPE_E4M3 || d == KDA_DTYPE_E2M1; }
+bool scaled(int32_t d) { return d == KDA_DTYPE_E4M3 || d == KDA_DTYPE_E2M1; }
+// A cache row's width in the units of its strides: elements, or of a 4-bit cache bytes.
+int64_t width(int32_t d, int64_t D) { return d == KDA_DTYPE_E2M1 ? D / 2 : D; }
+// Its scales' rows: 4 bits, eight bytes with byte strides.
+bool scales_ok(int32_t d, const void* p, const int64_t (&stride)[2]) {
+    if (d != KDA_DTYPE_E2M1) return scale_rows_ok(p, stride);
+    return reinterpret_cast<uintptr_t>(p) % 8 == 0 && stride[0] >= 0 && stride[1] >= 0 && stride[0] % 8 == 0 && stride[1] % 8 == 0;
+}
+
 // [n0, n1] rows of `width` elements of which no two share any, by strides that nest.
 bool distinct(const int64_t (&stride)[2], int64_t n0, int64_t n1, int64_t width) {
     const int64_t s0 = n0 > 1 ? stride[0] : 0, s1 = n1 > 1 ? stride[1] : 0;
@@ -116,19 +127,19 @@ size_t kda_mla_absorbed_workspace_size(int64_t B, int64_t T, int64_t H, int64_t 
 int kda_mla_absorbed_fwd(const kda_mla_absorbed_args* a, void* stream) {
     if (a == nullptr) return KDA_ERR_NULL_POINTER;
     if (!sizes_ok(a->B, a->T, a->S, a->H)) return KDA_ERR_BAD_SHAPE;
-    if (!act(a->dtype) || (a->cache_dtype != a->dtype && a->cache_dtype != KDA_DTYPE_E4M3)) return KDA_ERR_BAD_DTYPE;
+    if (!act(a->dtype) || !cache_type(a->cache_dtype, a->dtype)) return KDA_ERR_BAD_DTYPE;
     if ((a->R != 128 && a->R != 256 && a->R != 512) || !pos_ok(a->P) || !scale_ok(a->scale)) return KDA_ERR_UNSUPPORTED;
     if (a->H > 0 && a->T > kMaxGrid / 16 / a->H) return KDA_ERR_BAD_SHAPE;
     if (a->B * ((a->T * a->H + 15) / 16) > kMaxGrid) return KDA_ERR_BAD_SHAPE;
     if (a->B == 0 || a->H == 0 || a->T == 0) return KDA_OK;
-    const bool f8 = a->cache_dtype == KDA_DTYPE_E4M3;
+    const bool few = scaled(a->cache_dtype);
     if (!a->q || !a->o || !a->lengths) return KDA_ERR_NULL_POINTER;
-    if (a->S > 0 && (!a->cache || (f8 && !a->cache_scale))) return KDA_ERR_NULL_POINTER;
+    if (a->S > 0 && (!a->cache || (few && !a->cache_scale))) return KDA_ERR_NULL_POINTER;
     if (!a->workspace && kda::mla_absorbed_workspace_bytes(a->B, a->T, a->H, a->S, a->R) > 0) return KDA_ERR_NULL_POINTER;
-    if (!rows_ok(a->q, a->q_stride, 3, 2) || !rows_ok(a->cache, a->cache_stride, 2, f8 ? 1 : 2) || !at16(a->o) ||
+    if (!rows_ok(a->q, a->q_stride, 3, 2) || !rows_ok(a->cache, a->cache_stride, 2, few ? 1 : 2) || !at16(a->o) ||
         !at16(a->workspace) || !near(a->cache_stride[1]))
         return KDA_ERR_UNSUPPORTED;
-    if (f8 && (!scale_rows_ok(a->cache_scale, a->scale_stride) || !near(a->scale_stride[1])))
+    if (few && (!scales_ok(a->cache_dtype, a->cache_scale, a->scale_stride) || !near(a->scale_stride[1])))
         return KDA_ERR_UNSUPPORTED;
     return kda::mla_absorbed_launch(*a, static_cast<hipStream_t>(stream));
 }
@@ -136,17 +147,18 @@ int kda_mla_absorbed_fwd(const kda_mla_absorbed_args* a, void* stream) {
 int kda_mla_cache_append(const kda_mla_append_args* a, void* stream) {
     if (a == nullptr) return KDA_ERR_NULL_POINTER;
     if (!sizes_ok(a->B, a->T, a->S, 1) || (a->T > 0 && a->B > kMaxGrid / a->T)) return KDA_ERR_BAD_SHAPE;
-    if (!act(a->x_dtype) || (a->cache_dtype != a->x_dtype && a->cache_dtype != KDA_DTYPE_E4M3)) return KDA_ERR_BAD_DTYPE;
+    if (!act(a->x_dtype) || !cache_type(a->cache_dtype, a->x_dtype)) return KDA_ERR_BAD_DTYPE;
     if (a->norm_f32 != 0 && a->norm_f32 != 1) return KDA_ERR_BAD_DTYPE;
     if ((a->R != 128 && a->R != 256 && a->R != 512) || !pos_ok(a->P)) return KDA_ERR_UNSUPPORTED;
     if (a->B == 0 || a->T == 0 || a->S == 0) return KDA_OK;
-    const bool f8 = a->cache_dtype == KDA_DTYPE_E4M3;
-    if (!a->x || !a->cache || !a->lengths || (f8 && !a->cache_scale)) return KDA_ERR_NULL_POINTER;
-    if (!rows_ok(a->x, a->x_stride, 2, 2) || !rows_ok(a->cache, a->cache_stride, 2, f8 ? 1 : 2) || !at16(a->norm_weight))
+    const bool few = scaled(a->cache_dtype);
+    if (!a->x || !a->cache || !a->lengths || (few && !a->cache_scale)) return KDA_ERR_NULL_POINTER;
+    if (!rows_ok(a->x, a->x_stride, 2, 2) || !rows_ok(a->cache, a->cache_stride, 2, few ? 1 : 2) || !at16(a->norm_weight))
         return KDA_ERR_UNSUPPORTED;
     // distinct rows of the cache, so that no two waves write one
-    if (!distinct(a->cache_stride, a->B, a->S, a->R + a->P)) return KDA_ERR_UNSUPPORTED;
-    if (f8 && (!scale_rows_ok(a->cache_scale, a->scale_stride) || !distinct(a->scale_stride, a->B, a->S, 2)))
+    if (!distinct(a->cache_stride, a->B, a->S, width(a->cache_dtype, a->R + a->P))) return KDA_ERR_UNSUPPORTED;
+    if (few && (!scales_ok(a->cache_dtype, a->cache_scale, a->scale_stride) ||
+                !distinct(a->scale_stride, a->B, a->S, a->cache_dtype == KDA_DTYPE_E2M1 ? 8 : 2)))
         return KDA_ERR_UNSUPPORTED;
     return kda::mla_append_launch(*a, static_cast<hipStream_t>(stream));
 }
@@ -154,14 +166,15 @@ int kda_mla_cache_append(const kda_mla_append_args* a, void* stream) {
 int kda_mla_cache_read(const kda_mla_read_args* a, void* stream) {
     if (a == nullptr) return KDA_ERR_NULL_POINTER;
     if (!sizes_ok(a->B, 0, a->S, 1) || a->B * (a->S / 7 + 1) > kMaxGrid) return KDA_ERR_BAD_SHAPE;
-    if (!act(a->out_dtype)) return KDA_ERR_BAD_DTYPE;
+    if (!act(a->out_dtype) || (a->cache_dtype != 0 && !scaled(a->cache_dtype))) return KDA_ERR_BAD_DTYPE;
     if ((a->R != 128 && a->R != 256 && a->R != 512) || !pos_ok(a->P)) return KDA_ERR_UNSUPPORTED;
     if (a->B == 0 || a->S == 0) return KDA_OK;
     if (!a->cache || !a->cache_scale || !a->out) return KDA_ERR_NULL_POINTER;
-    if (!rows_ok(a->cache, a->cache_stride, 2, 1) || !at16(a->out) || !scale_rows_ok(a->cache_scale, a->scale_stride))
+    if (!rows_ok(a->cache, a->cache_stride, 2, 1) || !at16(a->out) || !scales_ok(a->cache_dtype, a->cache_scale, a->scale_stride))
         return KDA_ERR_UNSUPPORTED;
     const int64_t D = a->R + a->P;
-    if (!apart(a->out, a->B * a->S * D * 2, a->cache, (a->B - 1) * a->cache_stride[0] + (a->S - 1) * a->cache_stride[1] + D))
+    if (!apart(a->out, a->B * a->S * D * 2, a->cache,
+               (a->B - 1) * a->cache_stride[0] + (a->S - 1) * a->cache_stride[1] + width(a->cache_dtype, D)))
         return KDA_ERR_ALIAS;
     return kda::mla_read_launch(*a, static_cast<hipStream_t>(stream));
 }

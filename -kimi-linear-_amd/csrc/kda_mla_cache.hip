@@ -79,7 +79,31 @@ __device__ __forceinline__ uint2 quantise8(const float (&x)[8], float scale) {
     return uint2{static_cast<uint32_t>(lo), static_cast<uint32_t>(hi)};
 }
 
-template <typename T, bool F8>
+constexpr uint32_t kLeast4 = 67;        // 2^-60 here too
+constexpr int kGroup = 128;             // latent channels of a scale
+
+// Largest bits (of magnitudes: numbers, then infinity, then NaN) over 16 lanes.
+__device__ __forceinline__ uint32_t row_max(uint32_t x) {
+    x = max(x, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(x), 0x128, 0xf, 0xf, false)));   // row_ror:8, 4, 2, 1
+    x = max(x, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(x), 0x124, 0xf, 0xf, false)));
+    x = max(x, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(x), 0x122, 0xf, 0xf, false)));
+    return max(x, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(x), 0x121, 0xf, 0xf, false)));
+}
+__device__ __forceinline__ uint32_t largest(const float (&x)[8]) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(x[i]) & 0x7fffffffu);
+    return m;
+}
+// The sum over a wave in 64 bits, which leaves the row's norm, and with it a value
+// next to a border of the format, to no order of sums.
+__device__ __forceinline__ double wave_sum64(double x) {
+#pragma unroll
+    for (int d = 32; d > 0; d /= 2) x += __shfl_xor(x, d);
+    return x;
+}
+
+template <typename T, int BITS>
 __global__ __launch_bounds__(64 * kRows) void append_kernel(kda_mla_append_args a) {
     const int lane = threadIdx.x & 63;
     const uint32_t T_ = static_cast<uint32_t>(a.T), row = blockIdx.x * kRows + (threadIdx.x >> 6);
@@ -99,7 +123,18 @@ __global__ __launch_bounds__(64 * kRows) void append_kernel(kda_mla_append_args 
     }
     const int64_t at = held + t;
     if (t >= count || held < 0 || at >= a.S) return;
-    if (a.norm_weight) {
+    if (BITS == 4 && a.norm_weight) {
+        double ss = 0.;
+        if (lat) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) ss = fma(static_cast<double>(x[i]), static_cast<double>(x[i]), ss);
+        }
+        const float rstd = static_cast<float>(rsqrt(wave_sum64(ss) / R + static_cast<double>(a.eps)));
+        if (lat) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = x[i] * rstd * w[i];
+        }
+    } else if (a.norm_weight) {
         float ss = 0.f;
         if (lat) {
 #pragma unroll
@@ -111,13 +146,29 @@ __global__ __launch_bounds__(64 * kRows) void append_kernel(kda_mla_append_args 
             for (int i = 0; i < 8; ++i) x[i] = x[i] * rstd * w[i];
         }
     }
-    if constexpr (F8) {
+    if constexpr (BITS == 4) {
+        uint8_t* out = static_cast<uint8_t*>(a.cache) + b * a.cache_stride[0] + at * a.cache_stride[1];
+        // a scale's 128 channels are 16 lanes'; the position part lies in the first 16
+        const uint32_t e0 = mla::group_exponent(row_max(lat ? largest(x) : 0u), kLeast4);
+        const uint32_t e1 = mla::group_exponent(row_max(pos ? largest(p) : 0u), kLeast4);
+        if (lat) *reinterpret_cast<uint32_t*>(out + 4 * lane) = mla::narrow4(x, e0);
+        if (pos) *reinterpret_cast<uint32_t*>(out + R / 2 + 4 * lane) = mla::narrow4(p, e1);
+        const uint64_t one = 0x7f7f7f7f7f7f7f7full;
+        const int groups = R / kGroup;
+        uint64_t s = P ? static_cast<uint64_t>(__builtin_amdgcn_readlane(e1, 0)) << (8 * groups) | one << 8 << (8 * groups)
+                       : one << (8 * groups);
+        for (int g = 0; g < groups; ++g) s |= static_cast<uint64_t>(__builtin_amdgcn_readlane(e0, 16 * g)) << (8 * g);
+        if (lane == 0)
+            *reinterpret_cast<uint64_t*>(static_cast<uint8_t*>(a.cache_scale) + b * a.scale_stride[0] +
+                                         at * a.scale_stride[1]) = s;
+    } else if constexpr (BITS == 8) {
         uint8_t* out = static_cast<uint8_t*>(a.cache) + b * a.cache_stride[0] + at * a.cache_stride[1];
         const float s0 = part_scale(x, lat), s1 = P ? part_scale(p, pos) : 1.f;
         if (lat) *reinterpret_cast<uint2*>(out + 8 * lane) = quantise8(x, s0);
         if (pos) *reinterpret_cast<uint2*>(out + R + 8 * lane) = quantise8(p, s1);
         if (lane == 0)
-            *reinterpret_cast<float2*>(a.cache_scale + b * a.scale_stride[0] + at * a.scale_stride[1]) = float2{s0, s1};
+            *reinterpret_cast<float2*>(static_cast<float*>(a.cache_scale) + b * a.scale_stride[0] + at * a.scale_stride[1]) =
+                float2{s0, s1};
     } else {
         T* out = static_cast<T*>(a.cache) + b * a.cache_stride[0] + at * a.cache_stride[1];
         if (lat) *reinterpret_cast<uint4*>(out + 8 * lane) = pack8<T>(x);
@@ -125,8 +176,8 @@ __global__ __launch_bounds__(64 * kRows) void append_kernel(kda_mla_append_args 
     }
 }
 
-// 16 channels a lane: 16 bytes read, 32 written.
-template <typename T>
+// 16 channels a lane: 16 bytes read (8 in 4 bits), 32 written.
+template <typename T, int BITS>
 __global__ __launch_bounds__(256) void read_kernel(kda_mla_read_args a) {
     const int per = static_cast<int>(a.R + a.P) / 16;       // lanes a row
     const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
@@ -136,9 +187,17 @@ __global__ __launch_bounds__(256) void read_kernel(kda_mla_read_args a) {
     const int64_t b = row / a.S, j = row - b * a.S;
     uint4 out[2] = {};
     if (j < mla::tokens(a.lengths, b, a.S)) {
+      if constexpr (BITS == 4) {
+        const uint2 raw = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.cache) + b * a.cache_stride[0] +
+                                                          j * a.cache_stride[1] + c / 2);
+        const uint32_t e = static_cast<const uint8_t*>(a.cache_scale)[b * a.scale_stride[0] + j * a.scale_stride[1] +
+                                                                      (c < a.R ? c : static_cast<int>(a.R)) / kGroup];
+        out[0] = mla::widen4<T>(raw.x, __uint_as_float(e << 23));
+        out[1] = mla::widen4<T>(raw.y, __uint_as_float(e << 23));
+      } else {
         const uint4 raw = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(a.cache) +
                                                           b * a.cache_stride[0] + j * a.cache_stride[1] + c);
-        const float s = a.cache_scale[b * a.scale_stride[0] + j * a.scale_stride[1] + (c < a.R ? 0 : 1)];
+        const float s = static_cast<const float*>(a.cache_scale)[b * a.scale_stride[0] + j * a.scale_stride[1] + (c < a.R ? 0 : 1)];
         const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
         float x[2][8];
 #pragma unroll
@@ -150,6 +209,7 @@ __global__ __launch_bounds__(256) void read_kernel(kda_mla_read_args a) {
         }
         out[0] = pack8<T>(x[0]);
         out[1] = pack8<T>(x[1]);
+      }
     }
     uint4* to = reinterpret_cast<uint4*>(static_cast<T*>(a.out) + row * (a.R + a.P) + c);
     to[0] = out[0];
@@ -158,24 +218,32 @@ __global__ __launch_bounds__(256) void read_kernel(kda_mla_read_args a) {
 
 }  // namespace
 
+namespace {
+template <typename T>
+void append_type(const kda_mla_append_args& a, dim3 grid, hipStream_t stream) {
+    if (a.cache_dtype == KDA_DTYPE_E2M1) append_kernel<T, 4><<<grid, 64 * kRows, 0, stream>>>(a);
+    else if (a.cache_dtype == KDA_DTYPE_E4M3) append_kernel<T, 8><<<grid, 64 * kRows, 0, stream>>>(a);
+    else append_kernel<T, 16><<<grid, 64 * kRows, 0, stream>>>(a);
+}
+template <typename T>
+void read_type(const kda_mla_read_args& a, dim3 grid, hipStream_t stream) {
+    if (a.cache_dtype == KDA_DTYPE_E2M1) read_kernel<T, 4><<<grid, 256, 0, stream>>>(a);
+    else read_kernel<T, 8><<<grid, 256, 0, stream>>>(a);
+}
+}  // namespace
+
 int mla_append_launch(const kda_mla_append_args& a, hipStream_t stream) {
     const dim3 grid(static_cast<unsigned>((a.B * a.T + kRows - 1) / kRows));
-    const bool f8 = a.cache_dtype == KDA_DTYPE_E4M3;
-    if (a.x_dtype == KDA_DTYPE_F16) {
-        if (f8) append_kernel<_Float16, true><<<grid, 64 * kRows, 0, stream>>>(a);
-        else append_kernel<_Float16, false><<<grid, 64 * kRows, 0, stream>>>(a);
-    } else {
-        if (f8) append_kernel<bf16_t, true><<<grid, 64 * kRows, 0, stream>>>(a);
-        else append_kernel<bf16_t, false><<<grid, 64 * kRows, 0, stream>>>(a);
-    }
+    if (a.x_dtype == KDA_DTYPE_F16) append_type<_Float16>(a, grid, stream);
+    else append_type<bf16_t>(a, grid, stream);
     return hipGetLastError() == hipSuccess ? KDA_OK : KDA_ERR_LAUNCH;
 }
 
 int mla_read_launch(const kda_mla_read_args& a, hipStream_t stream) {
     const int64_t lanes = a.B * a.S * ((a.R + a.P) / 16);
     const dim3 grid(static_cast<unsigned>((lanes + 255) / 256));
-    if (a.out_dtype == KDA_DTYPE_F16) read_kernel<_Float16><<<grid, 256, 0, stream>>>(a);
-    else read_kernel<bf16_t><<<grid, 256, 0, stream>>>(a);
+    if (a.out_dtype == KDA_DTYPE_F16) read_type<_Float16>(a, grid, stream);
+    else read_type<bf16_t>(a, grid, stream);
     return hipGetLastError() == hipSuccess ? KDA_OK : KDA_ERR_LAUNCH;
 }
 

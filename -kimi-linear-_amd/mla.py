@@ -9,13 +9,16 @@ a few position channels that all heads share.
 * :func:`mla_absorbed` -- in the latent space over the cache itself, for
   decoding: single tokens, or a few at once;
 * :func:`mla_cache_append` -- new rows written behind the cached ones, the
-  latent part RMS-normalised on the way if asked, in 16 bits or 8;
-* :func:`mla_cache_read` -- an 8-bit cache back in 16 bits.
+  latent part RMS-normalised on the way if asked, in 16 bits, 8 or 4;
+* :func:`mla_cache_read` -- an 8- or 4-bit cache back in 16 bits.
 
 A cache is ``[B, S, rank + P]``: one row a token, latent then position
 channels.  In 16 bits it has the activations' type; in 8 bits it is
 ``torch.float8_e4m3fn`` with ``cache_scale`` fp32 ``[B, S, 2]``, a scale for a
-row's latent and one for its position part.  ``lengths``, ``starts`` and
+row's latent and one for its position part; in 4 bits ``torch.float4_e2m1fn_x2
+[B, S, (rank + P) / 2]``, two channels a byte, with ``cache_scale``
+``torch.float8_e8m0fnu [B, S, 8]``: a power of two for each 128 latent channels,
+then one for the position part (bytes beyond it are not read).  ``lengths``, ``starts`` and
 ``counts`` are integer tensors ``[B]`` on the device; the kernels read them, so
 a captured graph follows them.  A length to read by counts as 0 below 0 and as
 S above it; rows to append that a length puts outside the cache are dropped.
@@ -46,6 +49,7 @@ RANKS = (128, 256, 512)
 POSITION_DIMS = (0, 32, 64)
 HEAD_DIMS = (64, 128)
 _ACT = (torch.float16, torch.bfloat16)
+_FOUR = torch.float4_e2m1fn_x2
 
 
 _FAR = 2 ** 23          # elements between tokens from which a tile's offsets pass 32 bits
@@ -193,25 +197,32 @@ def _check_cache(cache, cache_scale, rank, B, D, act):
     if rank not in RANKS or D - rank not in POSITION_DIMS:
         raise KdaError(f"no kernel for rank {rank} and position dimension {D - rank} "
                        f"(rank in {RANKS}, position dimension in {POSITION_DIMS})")
-    if cache.dim() != 3 or cache.shape[0] != B or cache.shape[2] != D:
-        raise KdaError(f"cache must be [B, S, rank + P] = [{B}, S, {D}]; got {tuple(cache.shape)}")
-    if cache.dtype == torch.float8_e4m3fn:
+    width = D // 2 if cache.dtype == _FOUR else D
+    if cache.dim() != 3 or cache.shape[0] != B or cache.shape[2] != width:
+        raise KdaError(f"cache must be [B, S, rank + P{' over 2' if width != D else ''}] = [{B}, S, {width}]; got {tuple(cache.shape)}")
+    if cache.dtype == _FOUR:
+        if not isinstance(cache_scale, torch.Tensor) or cache_scale.dtype != torch.float8_e8m0fnu or tuple(
+                cache_scale.shape) != (B, cache.shape[1], 8):
+            raise KdaError(f"a 4-bit cache needs cache_scale, float8_e8m0fnu [B, S, 8] = [{B}, {cache.shape[1]}, 8]")
+    elif cache.dtype == torch.float8_e4m3fn:
         if not isinstance(cache_scale, torch.Tensor) or cache_scale.dtype != torch.float32 or tuple(
                 cache_scale.shape) != (B, cache.shape[1], 2):
             raise KdaError(f"an 8-bit cache needs cache_scale, float32 [B, S, 2] = [{B}, {cache.shape[1]}, 2]")
     elif cache.dtype != act:
-        raise KdaError(f"cache must be {act} (the activations' type) or float8_e4m3fn, got {cache.dtype}")
+        raise KdaError(f"cache must be {act} (the activations' type), float8_e4m3fn or float4_e2m1fn_x2, got {cache.dtype}")
     elif cache_scale is not None:
-        raise KdaError("cache_scale belongs to an 8-bit cache only")
+        raise KdaError("cache_scale belongs to an 8- or 4-bit cache only")
 
 
 def _check_layout(**tensors):
     """The cache and its scales are used in place, so their layout has to fit as it is."""
     for name, x in tensors.items():
-        n = 2 if x is not None and x.dtype == torch.float32 else 16
-        if x is not None and (x.stride(-1) != 1 or x.data_ptr() % (n * x.element_size() if n == 2 else n) != 0 or any(
-                s * (1 if n == 2 else x.element_size()) % n != 0 for s, m in zip(x.stride()[:-1], x.shape[:-1]) if m > 1)):
-            raise KdaError(f"{name} needs contiguous channels and aligned rows (16 bytes; a scale pair 8); "
+        if x is None:
+            continue
+        n = 8 if x.dtype in (torch.float32, torch.float8_e8m0fnu) else 16          # bytes
+        if x.stride(-1) != 1 or x.data_ptr() % n != 0 or any(
+                s * x.element_size() % n != 0 for s, m in zip(x.stride()[:-1], x.shape[:-1]) if m > 1):
+            raise KdaError(f"{name} needs contiguous channels and aligned rows (16 bytes; a row's scales 8); "
                            f"got strides {x.stride()}")
 
 
@@ -263,7 +274,11 @@ def mla_cache_append(x, cache, lengths, rank, cache_scale=None, counts=None, nor
     RMS-normalised first, in fp32.  Values are rounded once to the cache's type.  In 8 bits a row's
     latent part and its position part each get the scale max|x| / 448 (at
     least 2^-60, written to ``cache_scale``; 1 where P = 0) and x / scale is
-    rounded to the nearest e4m3 value.  A row with a value that is not finite
+    rounded to the nearest e4m3 value.  In 4 bits each 128 channels of the latent
+    part, and the position part, get the least power of two (at least 2^-60) that
+    leaves their largest magnitude at most 7, the quotients, which are exact, go
+    to the nearest e2m1 value, ties to the even one, above 6 to 6, and the norm's
+    mean is summed in 64 bits.  A row with a value that is not finite
     reads back as not finite.  x must not overlap the cache, nor rows of the
     cache each other.  Forward only."""
     try:
@@ -293,7 +308,7 @@ def mla_cache_append(x, cache, lengths, rank, cache_scale=None, counts=None, nor
 
 
 def mla_cache_read(cache, cache_scale, rank, dtype=torch.bfloat16, tokens=None, lengths=None):
-    """The first ``tokens`` (default all) rows of an 8-bit cache in 16 bits:
+    """The first ``tokens`` (default all) rows of an 8- or 4-bit cache in 16 bits:
     ``[B, tokens, rank + P]`` of value x scale, rounded once.  Rows at or past
     ``lengths[b]`` are zeros, and not read.  Forward only."""
     try:
@@ -309,9 +324,10 @@ def mla_cache_read(cache, cache_scale, rank, dtype=torch.bfloat16, tokens=None, 
         raise KdaError(f"dtype must be float16 or bfloat16, got {dtype}")
     if cache.device.type != "cuda":
         raise KdaError(f"the latent-attention kernels need HIP tensors (got cache on {cache.device}); there is no CPU path")
-    if cache.dtype != torch.float8_e4m3fn or cache.dim() != 3:
-        raise KdaError(f"cache must be float8_e4m3fn [B, S, rank + P]; got {cache.dtype} {tuple(cache.shape)}")
-    _check_cache(cache, cache_scale, rank, cache.shape[0], cache.shape[2], dtype)
+    if cache.dtype not in (torch.float8_e4m3fn, _FOUR) or cache.dim() != 3:
+        raise KdaError(f"cache must be float8_e4m3fn [B, S, rank + P] or float4_e2m1fn_x2 [B, S, (rank + P) / 2]; "
+                       f"got {cache.dtype} {tuple(cache.shape)}")
+    _check_cache(cache, cache_scale, rank, cache.shape[0], cache.shape[2] * (2 if cache.dtype == _FOUR else 1), dtype)
     _on_device(cache.device, cache_scale=cache_scale)
     n = cache.shape[1] if tokens is None else int(tokens)
     if not 0 <= n <= cache.shape[1]:

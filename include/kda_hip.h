@@ -39,14 +39,15 @@
 extern "C" {
 #endif
 
-#define KDA_ABI_VERSION 18
+#define KDA_ABI_VERSION 19
 
 /* Element types accepted at the boundary. */
 typedef enum kda_dtype {
     KDA_DTYPE_F32 = 0,
     KDA_DTYPE_F16 = 1,
     KDA_DTYPE_BF16 = 2,
-    KDA_DTYPE_E4M3 = 3             /* 8 bits, of a latent cache only (kda_mla_*) */
+    KDA_DTYPE_E4M3 = 3,            /* 8 bits, of a latent cache only (kda_mla_*) */
+    KDA_DTYPE_E2M1 = 4             /* 4 bits, of a latent cache only; two a byte */
 } kda_dtype;
 
 typedef enum kda_status {
@@ -558,20 +559,24 @@ int kda_mla_expanded_bwd(const kda_mla_expanded_bwd_args* args, void* stream);
  * over j <= lengths[b] - T + t: the T queries are the last of the sequence's
  * lengths[b] tokens.  A row without keys is zero.  Cache rows at or past
  * lengths[b] are never read.  A KDA_DTYPE_E4M3 cache stands for
- * cache[j] * cache_scale[j][0 (latent) or 1 (position)], scales at least 2^-60. */
+ * cache[j] * cache_scale[j][0 (latent) or 1 (position)], scales at least 2^-60.
+ * A KDA_DTYPE_E2M1 cache holds two channels a byte, the lower half first, and has
+ * eight bytes of scales a row: byte g is the exponent + 127 (at least 67; 255: NaN) of the
+ * power of two for latent channels 128 g to 128 g + 127, byte R / 128 that for
+ * the position part.  Its strides and its scales' are in bytes. */
 typedef struct kda_mla_absorbed_args {
     int64_t B, T, H, S, R, P;      /* R in {128, 256, 512}; P in {0, 32, 64} */
     const void* q;                 /* [B, T, H, R+P] */
     int64_t q_stride[3];
     const void* cache;             /* [B, S, R+P] */
     int64_t cache_stride[2];       /* (batch, token) */
-    const float* cache_scale;      /* [B, S, 2], 8-bit caches only */
-    int64_t scale_stride[2];       /* (batch, token), even */
+    const void* cache_scale;       /* 8-bit caches: fp32 [B, S, 2]; 4-bit: [B, S, 8] bytes */
+    int64_t scale_stride[2];       /* (batch, token), even; 4-bit: multiples of 8 */
     const int32_t* lengths;        /* [B] */
     void* o;                       /* [B, T, H, R] contiguous */
     float scale;
     int32_t dtype;                 /* of q and o: KDA_DTYPE_F16 or KDA_DTYPE_BF16 */
-    int32_t cache_dtype;           /* dtype, or KDA_DTYPE_E4M3 */
+    int32_t cache_dtype;           /* dtype, KDA_DTYPE_E4M3 or KDA_DTYPE_E2M1 */
     void* workspace;               /* kda_mla_absorbed_workspace_size() bytes */
 } kda_mla_absorbed_args;
 
@@ -584,40 +589,85 @@ int kda_mla_absorbed_fwd(const kda_mla_absorbed_args* args, void* stream);
  * (x rsqrt(mean x^2 + eps) weight, in fp32).  Rounded once to the cache's type;
  * in 8 bits x / scale to the nearest e4m3 value, with scale = max|x| / 448 (at
  * least 2^-60) of the row's latent part and, separately, of its position part
- * (1 if P = 0).  A row with a value that is not finite gets scales that are not. */
+ * (1 if P = 0).  A row with a value that is not finite gets scales that are not.
+ * In 4 bits the values are x / 2^e to the nearest e2m1 one, ties to the even
+ * one, e the least exponent (at least -60) that leaves the group's largest
+ * magnitude at most 7 (a larger one than 6 is taken as 6); the mean is summed in
+ * 64 bits, and scale bytes without a group are 127. */
 typedef struct kda_mla_append_args {
     int64_t B, T, S, R, P;
     const void* x;                 /* [B, T, R+P] */
     int64_t x_stride[2];           /* (batch, token) */
     void* cache;                   /* [B, S, R+P] */
     int64_t cache_stride[2];
-    float* cache_scale;            /* [B, S, 2], 8-bit caches only */
+    void* cache_scale;             /* 8-bit caches: fp32 [B, S, 2]; 4-bit: [B, S, 8] bytes */
     int64_t scale_stride[2];
     const int32_t* lengths;        /* [B] rows held before the call */
     const int32_t* counts;         /* [B] or NULL */
     const void* norm_weight;       /* [R] contiguous, or NULL */
     float eps;
     int32_t x_dtype;               /* KDA_DTYPE_F16 or KDA_DTYPE_BF16 */
-    int32_t cache_dtype;           /* x_dtype or KDA_DTYPE_E4M3 */
+    int32_t cache_dtype;           /* x_dtype, KDA_DTYPE_E4M3 or KDA_DTYPE_E2M1 */
     int32_t norm_f32;              /* norm_weight: 0 x_dtype, 1 KDA_DTYPE_F32 */
 } kda_mla_append_args;
 
 int kda_mla_cache_append(const kda_mla_append_args* args, void* stream);
 
-/* An 8-bit cache's first S rows back in 16 bits: out = value * scale rounded
+/* An 8- or 4-bit cache's first S rows back in 16 bits: out = value * scale rounded
  * once; zeros in rows at or past lengths[b] (NULL: S). */
 typedef struct kda_mla_read_args {
     int64_t B, S, R, P;
-    const void* cache;             /* [B, >= S, R+P] e4m3 */
+    const void* cache;             /* [B, >= S, R+P] */
     int64_t cache_stride[2];
-    const float* cache_scale;      /* [B, >= S, 2] */
+    const void* cache_scale;       /* fp32 [B, >= S, 2]; 4-bit: [B, >= S, 8] bytes */
     int64_t scale_stride[2];
     const int32_t* lengths;        /* [B] or NULL */
     void* out;                     /* [B, S, R+P] contiguous */
     int32_t out_dtype;             /* KDA_DTYPE_F16 or KDA_DTYPE_BF16 */
+    int32_t cache_dtype;           /* KDA_DTYPE_E2M1: 4 bits; 0 or KDA_DTYPE_E4M3: 8 bits */
 } kda_mla_read_args;
 
 int kda_mla_cache_read(const kda_mla_read_args* args, void* stream);
+
+/* Matrices in 4 bits: e2m1 values, two a byte, the lower half first, and for
+ * each 32 along a row a power of two, stored as its exponent + 127 (255: NaN).
+ *
+ * y = x W^T (+ bias) for any number of rows: sums in fp32, W's values taken in the
+ * activation type (exact in bf16, and in fp16 for powers from 2^-23 to 2^13;
+ * others are rounded), the result rounded once.  residual: y = residual + that
+ * rounded result.  K a multiple of 32; x rows and w 16-byte aligned; other calls
+ * return KDA_ERR_UNSUPPORTED.  y overlaps no input. */
+typedef struct kda_mx4_linear_args {
+    int64_t M, N, K;
+    const void* x;                 /* [M, K] */
+    int64_t x_stride;              /* row strides in elements */
+    const void* w;                 /* [N, K / 2] bytes, contiguous */
+    const void* w_scale;           /* [N, K / 32] bytes, contiguous */
+    const void* bias;              /* [N] contiguous, or NULL */
+    const void* residual;          /* [M, N], or NULL */
+    int64_t residual_stride;
+    void* y;                       /* [M, N] contiguous */
+    int32_t dtype;                 /* KDA_DTYPE_F16 or KDA_DTYPE_BF16, of x, bias, residual and y */
+} kda_mx4_linear_args;
+
+int kda_mx4_linear_fwd(const kda_mx4_linear_args* args, void* stream);
+
+/* Rows of a matrix to that form and back.  To it: x / 2^e to the nearest e2m1
+ * value, ties to the even one, e the least exponent (at least -126) that leaves
+ * the group's largest magnitude at most 7 (a larger one than 6 is taken as 6);
+ * 255 where a value is not finite.  From it: value times power, rounded once.
+ * K a multiple of 32; values and data rows 16-byte aligned. */
+typedef struct kda_mx4_convert_args {
+    int64_t N, K;
+    void* values;                  /* [N, K] */
+    int64_t value_stride;          /* row stride in elements */
+    void* data;                    /* [N, K / 2] bytes, contiguous */
+    void* scale;                   /* [N, K / 32] bytes, contiguous */
+    int32_t dtype;                 /* of the values: KDA_DTYPE_F16 or KDA_DTYPE_BF16, kda_mx4_quantize also KDA_DTYPE_F32 */
+} kda_mx4_convert_args;
+
+int kda_mx4_quantize(const kda_mx4_convert_args* args, void* stream);
+int kda_mx4_dequantize(const kda_mx4_convert_args* args, void* stream);
 
 /* Human-readable name of a kda_status code (static storage). */
 const char* kda_status_str(int status);
