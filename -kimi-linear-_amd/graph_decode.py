@@ -46,6 +46,11 @@ from .layer import KimiDeltaAttention
 from .mla_layer import LatentAttention
 
 
+def _bytes(t):
+    """A cache in 4 bits as bytes to copy."""
+    return t.view(torch.uint8) if t.dtype in (torch.float4_e2m1fn_x2, torch.float8_e8m0fnu) else t
+
+
 class KdaGraphedDecoder:
     """Graph-replayed incremental decoding of a stack of KDA and latent-attention layers.
 
@@ -83,15 +88,18 @@ class KdaGraphedDecoder:
         self._wbufs = None          # addresses of the fused weights the graph reads
 
     def _weight_buffers(self):
-        """Addresses of all that a captured step reads of the layers: their parameters and what is made of them."""
-        bufs = [tuple(p.data_ptr() for p in self.layers.parameters())]
+        """Addresses of all that a captured step reads of the layers: their parameters, weights in 4 bits, and what is
+        made of them."""
+        bufs = [tuple(p.data_ptr() for p in self.layers.parameters()), tuple(p.data_ptr() for p in self.layers.buffers())]
         for layer in self.layers:
             if isinstance(layer, LatentAttention):
                 bufs.append(tuple(layer._weight_buffers()))
                 continue
             w, b = layer._input_weight()
             a_log, dt_bias = layer._gate_params()
-            bufs.append((w.data_ptr(), b.data_ptr() if b is not None else 0, a_log.data_ptr(), dt_bias.data_ptr()))
+            four = layer._input_weight4() if layer._in_mx4() else ()
+            bufs.append((w.data_ptr(), b.data_ptr() if b is not None else 0, a_log.data_ptr(), dt_bias.data_ptr(),
+                         *(t.data_ptr() for t in four if t is not None)))
         return bufs
 
     @torch.no_grad()
@@ -160,9 +168,9 @@ class KdaGraphedDecoder:
         for st, new in zip(self.static_states, states):
             if "latent" in st:
                 n = st["tokens"] = new["tokens"]
-                st["latent"][:, :n].copy_(new["latent"][:, :n])
+                _bytes(st["latent"])[:, :n].copy_(_bytes(new["latent"])[:, :n])
                 if st["scale"] is not None:
-                    st["scale"][:, :n].copy_(new["scale"][:, :n])
+                    _bytes(st["scale"])[:, :n].copy_(_bytes(new["scale"])[:, :n])
         self._restore(states)
 
     @staticmethod

@@ -59,6 +59,7 @@ from . import _native
 from .kda import (KdaError, kda_chunkwise, kda_chunkwise_fused, kda_chunkwise_gated, kda_recurrent,
                   kda_recurrent_gated, long_segments)
 from .layer_ops import kda_output, kda_output_train, kda_prep, kda_prep_train, split_joined
+from .mx4 import Mx4Linear, _linear, _plain_mx4
 
 
 def l2norm(x, eps: float):
@@ -200,7 +201,9 @@ def _few_rows(rows: int, k: int, n: int) -> bool:
 
 def _project(mod, x, residual=None, out=None):
     """``mod(x)``, plus ``residual``, into ``out``: in the few-row kernel
-    (``kda_linear_fwd``) where it applies, else as written."""
+    (``kda_linear_fwd``) where it applies, in the 4-bit one where the module is of that kind, else as written."""
+    if _plain_mx4(mod) and not has_torch_function((x,)):
+        return _linear(x, mod.weight, mod.weight_scale, mod.bias, residual, out)
     B, T, k = x.shape
     w = _plain_weight(mod, x) if B * T <= 64 else None
     if w is not None and not _few_rows(B * T, k, w.shape[0]):
@@ -248,12 +251,61 @@ class KimiDeltaAttention(nn.Module):
         self.o_proj = nn.Linear(H * V, d, bias=bias)
         self.fp32_recurrent_state = True
         self._wcat = None          # (key, weight, bias, parameters) of the fused input projection
+        self._w4cat = None         # (key, data, scale, bias, buffers) of the q, k and v projections in 4 bits
         self._gcat = None          # (key, A_log, dt_bias, parameters) in fp32 for the gated core
         self.fuse_output = None    # output epilogue in the chunk kernel: True, False, None = by shape
 
     def _input_mods(self):
         return (self.in_proj_q, self.in_proj_k, self.in_proj_v, self.beta_proj, next(iter(self.gk_proj)),
                 next(iter(self.og_proj)))
+
+    def quantize_mx4_(self):
+        """Turn the wide projections -- q, k, v and the output's -- into :class:`Mx4Linear`, in place, for serving: a
+        decode step reads about a quarter of their bytes.  The small ones (beta, the gates) stay as they are.
+        The layer must be on a HIP device, its ``hidden_size`` and H V multiples of 32; it no longer trains.  A graph captured before has to be
+        made again (``KdaGraphedDecoder.prefill`` or ``refresh_weights`` notice)."""
+        names = ("in_proj_q", "in_proj_k", "in_proj_v", "o_proj")
+        new = {n: m if isinstance(m, Mx4Linear) else Mx4Linear.from_linear(m) for n, m in ((n, getattr(self, n)) for n in names)}
+        for n, m in new.items():
+            setattr(self, n, m)
+        self._wcat = self._w4cat = None
+        return self
+
+    def _in_mx4(self):
+        """Whether the q, k and v projections are in 4 bits; the other projections of x never are."""
+        mods = self._input_mods()
+        four = [isinstance(m, Mx4Linear) for m in mods]
+        if not any(four):
+            return False
+        if four != [True, True, True, False, False, False]:
+            raise KdaError("in_proj_q, in_proj_k and in_proj_v are all Mx4Linear or none of them, and beta_proj and the "
+                           "gates' first projections are not")
+        return True
+
+    def _input_weight4(self):
+        """The q, k and v projections in 4 bits as one: ``(data, scale, bias or None)``, cached and refilled like
+        :meth:`_input_weight`."""
+        mods = self._input_mods()[:3]
+        bufs = [m.weight for m in mods] + [m.weight_scale for m in mods] + [m.bias for m in mods if m.bias is not None]
+        key = _native.host().params_key(bufs)
+        old = self._w4cat
+        if old is not None and old[0] == key:
+            return old[1:4]
+        with torch.inference_mode(False), torch.no_grad():
+            parts = [[m.weight for m in mods], [m.weight_scale for m in mods],
+                     None if mods[0].bias is None else [m.bias for m in mods]]
+            new = []
+            for i, ps in enumerate(parts):
+                had = None if old is None else old[1 + i]
+                if ps is None:
+                    new.append(None)
+                elif (had is not None and had.shape == (sum(p.shape[0] for p in ps), *ps[0].shape[1:])
+                        and had.dtype == ps[0].dtype and had.device == ps[0].device):
+                    new.append(torch.cat(ps, 0, out=had))
+                else:
+                    new.append(torch.cat(ps, 0))
+        self._w4cat = (key, *new, [b.detach() for b in bufs])
+        return tuple(new)
 
     def _input_weight(self):
         """The six projections of x -- q, k, v, beta and the down-projections
@@ -270,8 +322,8 @@ class KimiDeltaAttention(nn.Module):
         the new weights.  Writes through ``.data`` do not bump ``_version``:
         call :meth:`refresh_fused_weight` after them.  What was concatenated is
         kept with the cache, so that no other parameter can come to lie at an
-        address of the key."""
-        mods = self._input_mods()
+        address of the key.  With q, k and v in 4 bits it is of the other three."""
+        mods = self._input_mods()[3 if self._in_mx4() else 0:]
         params = [m.weight for m in mods] + [m.bias for m in mods if m.bias is not None]
         key = _native.host().params_key(params)
         if self._wcat is not None and self._wcat[0] == key:
@@ -301,9 +353,13 @@ class KimiDeltaAttention(nn.Module):
         counter, such as ``p.data.copy_(...)``."""
         if self._wcat is not None:
             self._wcat = (None, *self._wcat[1:])
+        if self._w4cat is not None:
+            self._w4cat = (None, *self._w4cat[1:])
         if self._gcat is not None:
             self._gcat = (None, *self._gcat[1:])
         self._input_weight()
+        if self._in_mx4():
+            self._input_weight4()
         self._gate_params()
 
     def _gate_params(self):
@@ -386,14 +442,19 @@ class KimiDeltaAttention(nn.Module):
         B, T, d = x.shape
         rows = B * T
         few = rows <= 64 and not has_torch_function((x,))
+        four = _linear(x, *self._input_weight4(), None, None) if self._in_mx4() else None      # q, k and v
         y = None
         if few and b is None and _few_rows(rows, d, w.shape[0]):
             y = _native.host().linear(x, w, None, None)
         if y is None:
             y = torch.nn.functional.linear(x, w, b)
         (gk_down, gk_up, *_), (og_down, og_up, *_) = self.gk_proj, self.og_proj
-        q_in, k_in, v_in, beta_logit, gk_low, og_low = torch.split(
-            y, (H * K, H * K, H * V, H, gk_down.out_features, og_down.out_features), dim=-1)
+        wide, small = (H * K, H * K, H * V), (H, gk_down.out_features, og_down.out_features)
+        if four is not None:
+            q_in, k_in, v_in = torch.split(four, wide, dim=-1)
+            beta_logit, gk_low, og_low = torch.split(y, small, dim=-1)
+        else:
+            q_in, k_in, v_in, beta_logit, gk_low, og_low = torch.split(y, wide + small, dim=-1)
         gk = gate = None
         if few and output_gate:       # both up-projections in one launch
             w_gk, w_og = _plain_weight(gk_up), _plain_weight(og_up)
@@ -476,6 +537,8 @@ class KimiDeltaAttention(nn.Module):
         so the reference's chunkwise body plus recurrent tail is the same
         function), the output epilogue (:func:`kda_output_train`) and o_proj.
         Every step has a native backward; no cache, no state."""
+        if any(isinstance(m, Mx4Linear) for m in self.modules()):
+            raise KdaError("a layer with projections in 4 bits does not train: run it under torch.no_grad()")
         H, K, V = self.num_heads, self.head_dim, self.value_head_dim
         if K not in (64, 128) or V not in (64, 128):
             # the pre-processing backward (kda_prep_bwd) takes head dims 64 and 128:

@@ -15,7 +15,7 @@ protocol of ``KimiDeltaAttention``, so the two mix in one stack and in
   differentiable, without a cache or state;
 * ``layer(x, use_cache=True)``: the same, with the state
   ``{"latent", "scale", "lengths", "tokens"}``: the cache ``[B, max_tokens,
-  rank + P]`` in 16 or 8 bits and its scales, the tokens held per sequence on
+  rank + P]`` in 16, 8 or 4 bits and its scales, the tokens held per sequence on
   the device and, as all sequences grow together, on the host;
 * ``layer(x, state=state, use_cache=True)``: continues it, in place: one token
   through the absorbed form (the key and value up-projections applied to q and
@@ -39,16 +39,22 @@ from . import _native
 from .kda import KdaError
 from .layer import _plain_weight
 from .mla import mla_absorbed, mla_cache_append, mla_cache_read, mla_expanded
+from .mx4 import Mx4Linear
 
 
 def latent_attn_config(**kw) -> SimpleNamespace:
     """A config object with the fields :class:`LatentAttention` reads; keyword
-    overrides go into ``latent_attn_config`` except ``hidden_size`` and ``rms_norm_eps``."""
-    la = dict(num_heads=16, head_dim=128, position_dim=64, rank=512, cache_bits=16, max_tokens=4096, proj_bias=False)
+    overrides go into ``latent_attn_config`` except ``hidden_size`` and ``rms_norm_eps``.  ``cache_bits`` is 16 or 8;
+    ``cache_dtype=torch.float4_e2m1fn_x2`` (or ``torch.float8_e4m3fn``) names the cache's type instead."""
+    la = dict(num_heads=16, head_dim=128, position_dim=64, rank=512, cache_bits=16, max_tokens=4096, proj_bias=False,
+              cache_dtype=None)
     top = dict(hidden_size=2048, rms_norm_eps=1e-6)
     for k, v in kw.items():
         (top if k in top else la)[k] = v
     return SimpleNamespace(latent_attn_config=la, **top)
+
+
+_CACHE_BITS = {torch.float4_e2m1fn_x2: 4, torch.float8_e4m3fn: 8}
 
 
 class LatentAttention(nn.Module):
@@ -62,6 +68,10 @@ class LatentAttention(nn.Module):
         self.cache_bits, self.max_tokens = la["cache_bits"], la["max_tokens"]
         if self.cache_bits not in (8, 16):
             raise KdaError(f"cache_bits must be 8 or 16, got {self.cache_bits}")
+        if la.get("cache_dtype") is not None:
+            if la["cache_dtype"] not in _CACHE_BITS:
+                raise KdaError(f"cache_dtype must be None or one of {list(_CACHE_BITS)}, got {la['cache_dtype']}")
+            self.cache_bits = _CACHE_BITS[la["cache_dtype"]]
         self.eps = config.rms_norm_eps
         H, N, P, R = self.num_heads, self.head_dim, self.position_dim, self.rank
         bias = la.get("proj_bias", False)
@@ -72,6 +82,17 @@ class LatentAttention(nn.Module):
         self.o_proj = nn.Linear(H * N, d, bias=bias)
         self.scale = (N + P) ** -0.5
         self._up = None            # (key, W_k [H, N, R], W_v [H, R, N], weight) for the absorbed form
+
+    def quantize_mx4_(self):
+        """Turn ``q_proj``, ``kv_down`` and ``o_proj`` into :class:`Mx4Linear`, in place, for serving.  ``kv_up``, which the
+        absorbed form splits, stays as it is.  The layer must be on a HIP device, ``hidden_size`` and H N multiples
+        of 32; it no longer trains.  A graph captured before has to be made again (``KdaGraphedDecoder.prefill`` or
+        ``refresh_weights`` notice)."""
+        names = ("q_proj", "kv_down", "o_proj")
+        new = {n: m if isinstance(m, Mx4Linear) else Mx4Linear.from_linear(m) for n, m in ((n, getattr(self, n)) for n in names)}
+        for n, m in new.items():
+            setattr(self, n, m)
+        return self
 
     def _up_weights(self):
         """The up-projections as the absorbed form takes them, per head ``W_k [H, N, R]`` and ``W_v [H, R, N]``:
@@ -118,11 +139,13 @@ class LatentAttention(nn.Module):
     def new_state(self, B: int, device, dtype) -> dict:
         """An empty state for B sequences; of normal tensors under inference mode too, so that a later call
         outside it can go on with the state."""
-        shape = (B, self.max_tokens, self.rank + self.position_dim)
-        eight = self.cache_bits == 8
+        D, bits = self.rank + self.position_dim, self.cache_bits
+        kept, scales = {16: (dtype, None), 8: (torch.float8_e4m3fn, (2, torch.float32)),
+                        4: (torch.float4_e2m1fn_x2, (8, torch.float8_e8m0fnu))}[bits]
         with torch.inference_mode(False):
-            return {"latent": torch.empty(shape, device=device, dtype=torch.float8_e4m3fn if eight else dtype),
-                    "scale": torch.empty(B, self.max_tokens, 2, device=device) if eight else None,
+            return {"latent": torch.empty(B, self.max_tokens, D // 2 if bits == 4 else D, device=device, dtype=kept),
+                    "scale": None if scales is None else torch.empty(B, self.max_tokens, scales[0], device=device,
+                                                                     dtype=scales[1]),
                     "lengths": torch.zeros(B, dtype=torch.int32, device=device), "tokens": 0}
 
     def _room(self, state, T):
@@ -192,7 +215,7 @@ class LatentAttention(nn.Module):
 
     def _held(self, state, n, dtype):
         """The cache's first n rows in 16 bits."""
-        if self.cache_bits == 8:
+        if self.cache_bits < 16:
             return mla_cache_read(state["latent"], state["scale"], self.rank, dtype=dtype, tokens=n)
         return state["latent"][:, :n]
 

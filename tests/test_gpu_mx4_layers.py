@@ -1,0 +1,246 @@
+"""The layers with projections and caches in 4 bits.
+
+A layer whose projections are in 4 bits is the layer with the weights that they
+stand for (exact in bf16 and, at these sizes, in fp16), summed in another order:
+the tolerances are those of the 16-bit layers against their restatements, relative
+L2 norms.  The two forms of latent attention over one 4-bit cache see the same rows.
+"""
+
+from __future__ import annotations
+
+import copy
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda:0"
+BF16, F16 = torch.bfloat16, torch.float16
+FOUR = torch.float4_e2m1fn_x2
+TOL = {BF16: 2e-2, F16: 5e-3}
+
+
+def rel(a, b):
+    a, b = a.detach().double(), b.detach().double()
+    return ((a - b).norm() / b.norm()).item()
+
+
+def kda_layer(kda_pkg, dtype, seed=0, **kw):
+    torch.manual_seed(seed)
+    cfg = kda_pkg.linear_attn_config(**{**dict(hidden_size=256, num_heads=2, gate_low_rank=32, output_gate_low_rank=32), **kw})
+    return kda_pkg.KimiDeltaAttention(cfg).to(DEV, dtype).eval()
+
+
+def latent_layer(kda_pkg, dtype, seed=0, **kw):
+    torch.manual_seed(seed)
+    cfg = kda_pkg.latent_attn_config(**{**dict(hidden_size=256, num_heads=4, head_dim=64, position_dim=32, rank=128,
+                                               max_tokens=96), **kw})
+    return kda_pkg.LatentAttention(cfg).to(DEV, dtype).eval()
+
+
+def stands_for(kda_pkg, layer):
+    """The layer in 16 bits with the weights of its 4-bit projections."""
+    new = copy.deepcopy(layer)
+    for name, m in layer.named_children():
+        if isinstance(m, kda_pkg.Mx4Linear):
+            lin = torch.nn.Linear(m.in_features, m.out_features, bias=m.bias is not None, device=DEV, dtype=layer.beta_proj.weight.dtype
+                                  if hasattr(layer, "beta_proj") else layer.kv_up.weight.dtype)
+            with torch.no_grad():
+                lin.weight.copy_(kda_pkg.mx4_dequantize(m.weight, m.weight_scale, dtype=lin.weight.dtype))
+                if m.bias is not None:
+                    lin.bias.copy_(m.bias)
+            setattr(new, name, lin)
+    new._wcat = None
+    return new
+
+
+def cached(layer, x, pieces):
+    out, state, at = [], None, 0
+    for n in pieces:
+        y, state = layer(x[:, at:at + n], state=state, use_cache=True)
+        out.append(y)
+        at += n
+    return torch.cat(out, 1), state
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("kw", [{}, dict(proj_bias=True), dict(num_heads=4, head_dim=64, value_head_dim=128)], ids=str)
+@torch.no_grad()
+def test_kda_layer(kda_pkg, dtype, kw):
+    layer = kda_layer(kda_pkg, dtype, **kw)
+    before = layer(torch.ones(1, 3, 256, device=DEV, dtype=dtype))
+    assert layer.quantize_mx4_() is layer and layer.quantize_mx4_() is layer
+    same = stands_for(kda_pkg, layer)
+    assert not torch.equal(layer(torch.ones(1, 3, 256, device=DEV, dtype=dtype)), before)
+    x = torch.randn(3, 130, 256, device=DEV).to(dtype)
+    assert rel(layer(x), same(x)) <= TOL[dtype]
+    got, state = cached(layer, x, (70, 5, *[1] * 6))
+    want, wstate = cached(same, x, (70, 5, *[1] * 6))
+    assert rel(got, want) <= TOL[dtype] and rel(state["recurrent"], wstate["recurrent"]) <= TOL[dtype]
+    y = layer.decode_step_(x[:, 81:82], state)
+    assert rel(y, same.decode_step_(x[:, 81:82], wstate)) <= TOL[dtype]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("kw", [{}, dict(proj_bias=True), dict(rank=256, position_dim=0)], ids=str)
+@pytest.mark.parametrize("cache_dtype", [None, FOUR])
+@torch.no_grad()
+def test_latent_layer(kda_pkg, dtype, kw, cache_dtype):
+    layer = latent_layer(kda_pkg, dtype, cache_dtype=cache_dtype, **kw)
+    layer.quantize_mx4_()
+    same = stands_for(kda_pkg, layer)
+    x = torch.randn(2, 80, 256, device=DEV).to(dtype)
+    assert rel(layer(x), same(x)) <= TOL[dtype]
+    if cache_dtype is None:          # (over a 4-bit cache a row of a sum next to a border moves by a whole step)
+        assert rel(cached(layer, x, (50, 20, 1, 1, 1))[0], cached(same, x, (50, 20, 1, 1, 1))[0]) <= TOL[dtype]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("mx4", [False, True])
+@torch.no_grad()
+def test_latent_cache(kda_pkg, dtype, mx4):
+    """Single tokens through the absorbed form give what the expanded form gives over the rows read back; a cache
+    that is full is refused before anything is written."""
+    layer = latent_layer(kda_pkg, dtype, cache_dtype=FOUR)
+    if mx4:
+        layer.quantize_mx4_()
+    x = torch.randn(2, 96, 256, device=DEV).to(dtype)
+    out, state = layer(x[:, :50], use_cache=True)
+    assert state["latent"].dtype == FOUR and state["latent"].shape == (2, 96, 80)
+    assert state["scale"].dtype == torch.float8_e8m0fnu and state["scale"].shape == (2, 96, 8)
+    out, state = layer(x[:, 50:83], state=state, use_cache=True)
+    rows = layer._held(state, 83, dtype)
+    assert torch.equal(out, layer._expanded(x[:, 50:83], rows))
+    for t in range(83, 96):
+        out, state = layer(x[:, t:t + 1], state=state, use_cache=True)
+        assert rel(out, layer._expanded(x[:, t:t + 1], layer._held(state, t + 1, dtype))) <= TOL[dtype]
+    assert state["tokens"] == 96 and state["lengths"].tolist() == [96, 96]
+    held = state["latent"].view(torch.uint8).clone()
+    for call in (lambda: layer(x[:, :1], state=state, use_cache=True), lambda: layer.decode_step_(x[:, :1], state),
+                 lambda: layer(x[:, :5], state=state, use_cache=True)):
+        with pytest.raises(kda_pkg.KdaError, match="96"):
+            call()
+    assert torch.equal(state["latent"].view(torch.uint8), held)
+
+
+def stack(kda_pkg, dtype):
+    layers = [kda_layer(kda_pkg, dtype, seed=3), latent_layer(kda_pkg, dtype, seed=4, cache_dtype=FOUR),
+              kda_layer(kda_pkg, dtype, seed=5, proj_bias=True)]
+    return [m.quantize_mx4_() for m in layers]
+
+
+@pytest.mark.parametrize("residual", [True, False])
+@torch.no_grad()
+def test_stack_captured(kda_pkg, residual):
+    """Every replayed step is the eager layers', bit for bit, with prompts that reuse the capture."""
+    from kimi_linear_amd.graph_decode import KdaGraphedDecoder
+    layers = stack(kda_pkg, F16)
+    x = torch.randn(2, 90, 256, device=DEV).half()
+    dec = KdaGraphedDecoder(layers, residual=residual)
+    graph = None
+    for n, steps in ((40, 9), (61, 12), (5, 3)):
+        h = dec.prefill(x[:, :n])
+        assert graph is None or dec.graph is graph
+        graph = dec.graph
+        states, y = [None] * 3, x[:, :n]
+        for i, layer in enumerate(layers):
+            out, states[i] = layer(y, use_cache=True)
+            y = y + out if residual else out
+        assert torch.equal(h, y[:, -1])
+        for t in range(n, n + steps):
+            got = dec.step(x[:, t:t + 1]).clone()
+            y = x[:, t:t + 1]
+            for i, layer in enumerate(layers):
+                out, states[i] = layer(y, state=states[i], use_cache=True)
+                y = y + out if residual else out
+            torch.cuda.synchronize()
+            assert torch.equal(got, y[:, 0]), (n, t)
+
+
+@torch.no_grad()
+def test_weights_change(kda_pkg):
+    """Other weights loaded in place, and layers turned to 4 bits after a capture, are what the next step runs."""
+    from kimi_linear_amd.graph_decode import KdaGraphedDecoder
+    x = torch.randn(1, 20, 256, device=DEV).half()
+
+    def step(layers, dec=None):
+        dec = dec or KdaGraphedDecoder(layers)
+        dec.prefill(x[:, :19])
+        return dec.step(x[:, 19:]).clone(), dec
+
+    layers = stack(kda_pkg, F16)
+    a, dec = step(layers)
+    other = kda_layer(kda_pkg, F16, seed=9).quantize_mx4_()
+    layers[0].load_state_dict(other.state_dict())
+    b, _ = step(layers, dec)
+    assert not torch.equal(a, b) and torch.equal(b, step(layers)[0])
+    assert torch.equal(layers[0](x), other(x))
+    plain = [kda_layer(kda_pkg, F16, seed=3), latent_layer(kda_pkg, F16, seed=4)]
+    a, dec = step(plain)
+    for m in plain:
+        m.quantize_mx4_()
+    b, _ = step(plain, dec)
+    assert not torch.equal(a, b) and torch.equal(b, step(plain)[0])
+    plain[0].in_proj_q.weight.data.random_(0, 255)                 # unseen by the version counter
+    dec.refresh_weights()
+    dec.prefill(x[:, :19])
+    assert torch.equal(dec.step(x[:, 19:]), step(plain)[0])
+
+
+def test_refusals(kda_pkg):
+    err = kda_pkg.KdaError
+    layer = kda_layer(kda_pkg, F16)
+    x = torch.randn(1, 70, 256, device=DEV).half()
+    mixed = copy.deepcopy(layer)
+    mixed.in_proj_k = kda_pkg.Mx4Linear.from_linear(mixed.in_proj_k)
+    small = copy.deepcopy(layer).quantize_mx4_()
+    small.beta_proj = kda_pkg.Mx4Linear.from_linear(small.beta_proj)
+    with torch.no_grad():
+        for m in (mixed, small):
+            with pytest.raises(err, match="Mx4Linear"):
+                m(x)
+    layer.quantize_mx4_()
+    with pytest.raises(err, match="train"):
+        layer(x)
+    only_out = kda_layer(kda_pkg, F16)
+    only_out.o_proj = kda_pkg.Mx4Linear.from_linear(only_out.o_proj)
+    with pytest.raises(err, match="train"):
+        only_out(x)
+    with torch.no_grad():
+        assert torch.isfinite(only_out(x)).all()
+    with pytest.raises(err):
+        latent_layer(kda_pkg, F16).quantize_mx4_()(x)              # under grad mode
+    with pytest.raises(err):
+        kda_layer(kda_pkg, F16).cpu().quantize_mx4_()
+    with pytest.raises(err), torch.no_grad():
+        layer(x.float())
+    for bad in (torch.int8, torch.uint8, torch.float16, 4):
+        with pytest.raises(err, match="cache_dtype"):
+            latent_layer(kda_pkg, F16, cache_dtype=bad)
+    assert latent_layer(kda_pkg, F16, cache_dtype=torch.float8_e4m3fn).cache_bits == 8
+
+
+@torch.no_grad()
+def test_inference_mode_and_autocast(kda_pkg):
+    """Quantised and run under inference mode, then outside it; in fp32 modules under autocast."""
+    x = torch.randn(2, 40, 256, device=DEV)
+    layers = [kda_layer(kda_pkg, F16, seed=6), latent_layer(kda_pkg, F16, seed=7, cache_dtype=FOUR)]
+    with torch.inference_mode():
+        for m in layers:
+            m.quantize_mx4_()
+            _, state = m(x[:, :30].half(), use_cache=True)
+            a, _ = m(x[:, 30:31].half(), state=state, use_cache=True)
+    for m in layers:
+        _, state = m(x[:, :30].half(), use_cache=True)
+        assert torch.equal(m(x[:, 30:31].half(), state=state, use_cache=True)[0].isfinite().all(), torch.tensor(True, device=DEV))
+    assert torch.equal(a, m(x[:, 30:31].half(), state=m(x[:, :30].half(), use_cache=True)[1], use_cache=True)[0])
+    layer = latent_layer(kda_pkg, torch.float32, seed=8).quantize_mx4_()
+    with torch.autocast("cuda", dtype=BF16):
+        y = layer(x)
+    assert y.dtype == BF16 and rel(y, latent_like(kda_pkg, layer)(x.to(BF16))) <= TOL[BF16]
+
+
+def latent_like(kda_pkg, layer):
+    """The fp32 layer's bf16 form."""
+    return stands_for(kda_pkg, copy.deepcopy(layer).to(BF16))
