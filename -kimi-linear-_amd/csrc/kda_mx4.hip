@@ -16,7 +16,7 @@ namespace {
 
 using mla::Act;
 
-// Dword i of lane group lg to dword lg of lane group i.
+// b's lower half (16 lanes: even ones) in place of a's upper (odd) and the other way round.
 __device__ __forceinline__ void swap32(uint32_t& a, uint32_t& b) {
     const auto r = __builtin_amdgcn_permlane32_swap(a, b, false, false);
     a = r[0], b = r[1];
@@ -25,15 +25,37 @@ __device__ __forceinline__ void swap16(uint32_t& a, uint32_t& b) {
     const auto r = __builtin_amdgcn_permlane16_swap(a, b, false, false);
     a = r[0], b = r[1];
 }
-__device__ __forceinline__ uint4 turned(uint4 w) {
-    swap32(w.x, w.z);
-    swap32(w.y, w.w);
-    swap16(w.x, w.y);
-    swap16(w.z, w.w);
-    return w;
-}
 __device__ __forceinline__ uint32_t word(const uint4& w, int i) { return i == 0 ? w.x : i == 1 ? w.y : i == 2 ? w.z : w.w; }
-__device__ __forceinline__ float power(uint32_t bytes, int i) { return __uint_as_float((bytes >> (8 * i) & 255u) << 23); }
+
+__device__ __forceinline__ uint32_t lds_address(void* p) {
+    return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) void*)(p)));
+}
+// 64 lanes' 16 bytes each, from base + offset bytes, on end to LDS; the reader waits for them.
+__device__ __forceinline__ void to_lds(const void* base, int offset, char* lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+                 :
+                 : "s"(lds_address(lds)), "v"(offset), "s"(base)
+                 : "memory");
+}
+// All but the wave's last N loads are there.
+template <int N>
+__device__ __forceinline__ void landed() { asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory"); }
+
+// A span's scales, a lane group a chunk's, handed around: e[j] of chunk j.
+template <int SPAN>
+__device__ __forceinline__ void hand_around(uint32_t held, uint32_t (&e)[SPAN]) {
+    if constexpr (SPAN == 4) {
+        e[0] = e[2] = held;
+        swap32(e[0], e[2]);
+        e[1] = e[0];
+        e[3] = e[2];
+        swap16(e[0], e[1]);
+        swap16(e[2], e[3]);
+    } else {
+        e[0] = e[1] = held;
+        swap16(e[0], e[1]);
+    }
+}
 
 // What goes to four neighbouring outputs n.. of a row beside the product, asked for ahead of it.
 template <typename T>
@@ -79,310 +101,365 @@ __device__ __forceinline__ void put(const kda_mx4_linear_args& a, int64_t row, i
     }
 }
 
-// ---- few rows of x ----------------------------------------------------------
-// Grid ceil(N / (16 NT)), 64 SPLIT threads.  MT 16-row tiles of x, NT of W; the
-// waves take the spans of four chunks of 128 channels in turn, D chunks at a time, the
-// next D under way.  A span's scales are one load, a lane group a chunk's, and are handed
-// around in registers: a load for each chunk took as long as the weight's own
-// (28672 x 8192 from HBM, one row: 41 us, without any scales 29).
-// All loads go through descriptors that end with the workgroup's rows: what does not exist
-// (rows, groups past K, chunks past a wave's last) is an offset past the end, which reads as
-// zero without a branch, and asks memory for nothing.
-template <typename T, int MT, int NT, int SPLIT, int D, bool WORDS>
-struct Few {
-    static constexpr int kNone = 0x7f000000;         // past every descriptor's end
-    static constexpr int kSpan = 4;
-    __amdgpu_buffer_rsrc_t w, scale, x;
-    int w_at[NT], e_at[NT], x_at[MT];                // the lane's rows, in bytes
-    int groups, lg;
-    f4 acc[NT][MT];
-
-    struct Set {
-        uint4 p[D][NT], x[D][MT][4];
+// ---- few outputs ------------------------------------------------------------
+// Grid (ceil(N / (16 NT)), ceil(M / (16 MT))), 64 SPLIT threads.  MT 16-row tiles of x, NT of
+// W; the waves take spans of SPAN chunks of 128 channels in turn, and their sums meet in LDS.
+//
+// Bound by the way to memory.  Three things carry it.  A span's scales are one load, a lane
+// group a chunk's, handed around in registers: a load for each chunk took as long as W's own (one
+// row by 28672 x 8192 41 us, without any scales 29).  x goes through LDS, a buffer a wave, where
+// a row's 256 bytes come as one piece; read as operands they come as 64 from each of
+// sixteen rows (53 rows by 6160 x 4096 18.9 us, this way 12.3).  And W and the scales come
+// through descriptors that end with the workgroup's rows, so that what does not exist is an
+// offset past the end, which reads as zero without a branch and asks memory for nothing.
+//
+// x's 16-byte piece c of row r lies at c turned by r, so that sixteen rows' pieces are in
+// different banks.  A lane has the same group of x and W, channels 32 lg + 8 i of a chunk in step
+// i.  Rows of x past the last leave what LDS holds, in columns of the product that go nowhere.
+template <typename T, int MT, int NT, int SPLIT, int SPAN, bool WORDS>
+__global__ __launch_bounds__(64 * SPLIT) void rows_kernel(kda_mx4_linear_args a) {
+    constexpr int kTiles = NT * MT, kOwn = (kTiles + SPLIT - 1) / SPLIT, kNone = 0x7f000000;
+    constexpr int kLoads = 4 * MT;                           // of a chunk of x, four rows each
+    __shared__ __align__(16) char buf[SPLIT][1024 * (kLoads > kTiles ? kLoads : kTiles)];
+    const int lane = threadIdx.x & 63, ln = lane & 15, lg = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t n0 = static_cast<int64_t>(blockIdx.x) * (16 * NT), m0 = static_cast<int64_t>(blockIdx.y) * (16 * MT);
+    const int groups = static_cast<int>(a.K / 32), chunks = (groups + 3) / 4;
+    const uint32_t rows = static_cast<uint32_t>(min(a.N - n0, static_cast<int64_t>(16 * NT)));
+    const auto w = make_rsrc(static_cast<const uint8_t*>(a.w) + n0 * groups * 16, rows * groups * 16);
+    const auto scale = make_rsrc(static_cast<const uint8_t*>(a.w_scale) + n0 * groups, rows * groups);
+    int w_at[NT], e_at[NT], x_at[kLoads];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        e_at[t] = (16 * t + ln) * groups;
+        w_at[t] = 16 * (e_at[t] + lg);
+    }
+    const int last = static_cast<int>(min(a.M - 1 - m0, static_cast<int64_t>(16 * MT - 1)));
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+        const int r = 4 * i + lg;
+        x_at[i] = min(r, last) * static_cast<int>(a.x_stride) * 2 + 16 * (ln ^ (r & 15));
+    }
+    const T* xb = static_cast<const T*>(a.x) + m0 * a.x_stride;
+    char* mine = buf[wave];
+    const auto load_x = [&](int c) {
+        if (4 * c + 4 <= groups) {
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i)
+                if (4 * i <= last) to_lds(xb + 128 * c, x_at[i], mine + 1024 * i);
+        } else {                                             // pieces past the last are read as it
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) {
+                if (4 * i > last) continue;
+                const int piece = ln ^ ((4 * i + lg) & 15);
+                to_lds(xb + 128 * c, x_at[i] - 16 * max(piece - (4 * (groups - 4 * c) - 1), 0), mine + 1024 * i);
+            }
+        }
     };
-    struct Scales {
-        uint32_t e[NT];                              // of the span's chunk lg
+    const auto load_w = [&](int c, uint4 (&p)[NT]) {
+        const bool there = 4 * c + lg < groups;
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+            p[t] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(w, there ? w_at[t] + 64 * c : kNone, 0, 0));
     };
-    __device__ __forceinline__ void load(Scales& s, int c) const {
-        const int g = 4 * (c + lg);
+    const auto load_scales = [&](int c, uint32_t (&e)[NT]) {
+        const int g = 4 * (c + lg % SPAN);
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
             if constexpr (WORDS) {
-                s.e[t] = __builtin_amdgcn_raw_buffer_load_b32(scale, g < groups ? e_at[t] + g : kNone, 0, 0);
+                e[t] = __builtin_amdgcn_raw_buffer_load_b32(scale, g < groups ? e_at[t] + g : kNone, 0, 0);
             } else {
-                s.e[t] = 0;
+                e[t] = 0;
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    s.e[t] |= static_cast<uint32_t>(
+                    e[t] |= static_cast<uint32_t>(
                         __builtin_amdgcn_raw_buffer_load_b8(scale, g + i < groups ? e_at[t] + g + i : kNone, 0, 0)) << (8 * i);
             }
         }
-    }
-    __device__ __forceinline__ void load(Set& s, int c0) const {
+    };
+    f4 acc[NT][MT];
 #pragma unroll
-        for (int d = 0; d < D; ++d) {
-            const int g = 4 * (c0 + d);
-            const bool mine = g + lg < groups;
+    for (int t = 0; t < NT; ++t)
 #pragma unroll
-            for (int t = 0; t < NT; ++t)
-                s.p[d][t] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(w, mine ? w_at[t] + 16 * g : kNone, 0, 0));
-#pragma unroll
-            for (int m = 0; m < MT; ++m)
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    s.x[d][m][i] = __builtin_bit_cast(
-                        uint4, __builtin_amdgcn_raw_buffer_load_b128(x, x_at[m], g + i < groups ? 64 * (g + i) : kNone, 0));
-        }
-    }
-    // Chunks j.. of a span, e[j][t] their scales.
-    __device__ __forceinline__ void add(Set& s, const uint32_t (&e)[kSpan][NT], int j) {
-#pragma unroll
-        for (int d = 0; d < D; ++d) {
-#pragma unroll
-            for (int t = 0; t < NT; ++t) s.p[d][t] = turned(s.p[d][t]);
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int t = 0; t < NT; ++t) {
-                    const uint4 wide = mla::widen4<T>(word(s.p[d][t], i), power(e[j + d][t], i));
-#pragma unroll
-                    for (int m = 0; m < MT; ++m) acc[t][m] = Act<T>::mma16(wide, s.x[d][m][i], acc[t][m]);
-                }
-        }
-    }
-};
-
-template <typename T, int MT, int NT, int SPLIT, int D, bool WORDS>
-__global__ __launch_bounds__(64 * SPLIT) void few_kernel(kda_mx4_linear_args a) {
-    using F = Few<T, MT, NT, SPLIT, D, WORDS>;
-    constexpr int kTiles = NT * MT, kOwn = (kTiles + SPLIT - 1) / SPLIT;
-    const int lane = threadIdx.x & 63, ln = lane & 15, lg = lane >> 4;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int64_t n0 = static_cast<int64_t>(blockIdx.x) * (16 * NT);
-    F f;
-    f.groups = static_cast<int>(a.K / 32);
-    f.lg = lg;
-    const uint32_t rows = static_cast<uint32_t>(min(a.N - n0, static_cast<int64_t>(16 * NT)));
-    f.w = make_rsrc(static_cast<const uint8_t*>(a.w) + n0 * f.groups * 16, rows * f.groups * 16);
-    f.scale = make_rsrc(static_cast<const uint8_t*>(a.w_scale) + n0 * f.groups, rows * f.groups);
-    f.x = make_rsrc(a.x, static_cast<uint32_t>(2 * ((a.M - 1) * a.x_stride + a.K)));
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-        f.e_at[t] = (16 * t + ln) * f.groups;
-        f.w_at[t] = 16 * (f.e_at[t] + lg);
-    }
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-        f.x_at[m] = 16 * m + ln < a.M ? 2 * (16 * m + ln) * static_cast<int>(a.x_stride) + 16 * lg : F::kNone;
-    typename F::Set s[2];
-    typename F::Scales next;
-    const int chunks = (f.groups + 3) / 4;
-    f.load(next, F::kSpan * wave);
-    f.load(s[0], F::kSpan * wave);
+        for (int m = 0; m < MT; ++m) acc[t][m] = f4{0.f, 0.f, 0.f, 0.f};
     // tile i's outputs of this lane, i one of the wave's in the end
-    const auto row = [&](int i) { return static_cast<int64_t>(16 * (i % MT) + ln); };
+    const auto row = [&](int i) { return m0 + 16 * (i % MT) + ln; };
     const auto col = [&](int i) { return n0 + 16 * (i / MT) + 4 * lg; };
     Beside<T> beside[kOwn];
 #pragma unroll
     for (int o = 0; o < kOwn; ++o)
         if (wave + o * SPLIT < kTiles) beside[o].load(a, row(wave + o * SPLIT), col(wave + o * SPLIT));
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int m = 0; m < MT; ++m) f.acc[t][m] = f4{0.f, 0.f, 0.f, 0.f};
-    for (int c = F::kSpan * wave; c < chunks; c += F::kSpan * SPLIT) {
-        uint32_t e[F::kSpan][NT];
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            e[0][t] = e[2][t] = next.e[t];
-            swap32(e[0][t], e[2][t]);
-            e[1][t] = e[0][t];
-            e[3][t] = e[2][t];
-            swap16(e[0][t], e[1][t]);
-            swap16(e[2][t], e[3][t]);
-        }
-        f.load(next, c + F::kSpan * SPLIT);
-#pragma unroll
-        for (int j = 0; j < F::kSpan; j += D) {
-            const bool more = j + D < F::kSpan;
-            f.load(s[(j / D + 1) & 1], more ? c + j + D : c + F::kSpan * SPLIT);
-            f.add(s[(j / D) & 1], e, j);
-        }
-    }
 
-    __shared__ f4 part[SPLIT == 1 ? 1 : SPLIT * kTiles * 64];
-    if constexpr (SPLIT > 1) {
+    uint32_t next[NT];
+    uint4 p[2][NT];
+    load_scales(SPAN * wave, next);
+    load_w(SPAN * wave, p[0]);
+    for (int c0 = SPAN * wave; c0 < chunks; c0 += SPAN * SPLIT) {
+        uint32_t e[NT][SPAN];
 #pragma unroll
-        for (int i = 0; i < kTiles; ++i) part[(wave * kTiles + i) * 64 + lane] = f.acc[i / MT][i % MT];
-        __syncthreads();
+        for (int t = 0; t < NT; ++t) hand_around<SPAN>(next[t], e[t]);
+        load_scales(c0 + SPAN * SPLIT, next);
+#pragma unroll
+        for (int j = 0; j < SPAN; ++j) {
+            const int c = c0 + j;
+            if (c >= chunks) break;
+            uint4 x[4][MT];
+            load_x(c);
+            load_w(j + 1 < SPAN ? c + 1 : c0 + SPAN * SPLIT, p[(j + 1) % 2]);
+            landed<NT>();                                        // all but the next chunk's W
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int m = 0; m < MT; ++m)
+                    x[i][m] = *reinterpret_cast<const uint4*>(mine + 4096 * m + 256 * ln + 16 * ((4 * lg + i) ^ ln));
+            if (4 * c + 4 > groups && 4 * c + lg >= groups) {    // (W's are zero already)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int m = 0; m < MT; ++m) x[i][m] = uint4{0, 0, 0, 0};
+            }
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                const float pw = __uint_as_float((e[t][j] >> (8 * lg) & 255u) << 23);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint4 wide = mla::widen4<T>(word(p[j % 2][t], i), pw);
+#pragma unroll
+                    for (int m = 0; m < MT; ++m) acc[t][m] = Act<T>::mma16(wide, x[i][m], acc[t][m]);
+                }
+            }
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the chunk has been read: the next may lie there
+        }
     }
+    landed<0>();                                                 // (the scales asked for last)
+    f4* part = reinterpret_cast<f4*>(buf);
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kTiles; ++i) part[(wave * kTiles + i) * 64 + lane] = acc[i / MT][i % MT];
+    __syncthreads();
 #pragma unroll
     for (int o = 0; o < kOwn; ++o) {
         const int i = wave + o * SPLIT;
         if (i >= kTiles) break;
-        f4 r;
-        if constexpr (SPLIT == 1) {
-            r = f.acc[o / MT][o % MT];
-        } else {
-            r = part[i * 64 + lane];
+        f4 r = part[i * 64 + lane];
 #pragma unroll
-            for (int v = 1; v < SPLIT; ++v) {
-                const f4 p = part[(v * kTiles + i) * 64 + lane];
+        for (int v = 1; v < SPLIT; ++v) {
+            const f4 q = part[(v * kTiles + i) * 64 + lane];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) r[j] += p[j];
-            }
+            for (int k = 0; k < 4; ++k) r[k] += q[k];
         }
         put<T>(a, row(i), col(i), r, beside[o]);
     }
 }
 
-// ---- many rows of x ---------------------------------------------------------
-// 128 rows of x and 128 of W a workgroup, 64 and 64 a wave.  x goes to LDS 128 channels
-// at a time, two buffers; its 16-byte piece c of row r lies at c turned by r, so that
-// sixteen rows' pieces are in different banks.  W goes to registers as it is, the next
-// chunk's under way, and is widened there.
-constexpr int kTile = 128, kChunk = 128;
+// ---- many outputs -----------------------------------------------------------
+// 64 WM rows of x and 16 NT WN of W a workgroup, 64 and 16 NT a wave.  Both go to LDS 128
+// channels at a time, asynchronously, STAGES buffers.  x's 16-byte piece c of row r lies at c
+// turned by r, W's by bits of r, so that sixteen rows' pieces are in different banks; W is widened
+// after it is read.  A lane has the same group of x and W, channels 32 lg + 8 i of a chunk in step i.
+constexpr int kChunk = 128;
 
-__device__ __forceinline__ uint32_t lds_address(void* p) {
-    return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) void*)(p)));
-}
-__device__ __forceinline__ void to_lds(const void* base, int offset, char* lds) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
-                 :
-                 : "s"(lds_address(lds)), "v"(offset), "s"(base)
-                 : "memory");
-}
+template <typename T, int WM, int WN, int NT, int STAGES, bool WORDS>
+struct Tile {
+    static constexpr int kWaves = WM * WN, kThreads = 64 * kWaves, kM = 64 * WM, kN = 16 * NT * WN;
+    static constexpr int kX = kM * 2 * kChunk, kW = kN * kChunk / 2;             // bytes of a stage
+    static constexpr int kXLoads = kX / 1024 / kWaves, kWLoads = kW / 1024 / kWaves;
+    static_assert(kXLoads * kWaves * 1024 == kX && kWLoads * kWaves * 1024 == kW, "whole loads, as many each wave");
+};
 
-template <typename T>
-__global__ __launch_bounds__(256, 2) void many_kernel(kda_mx4_linear_args a) {
-    __shared__ __align__(16) char buf[2][kTile * kChunk * 2];
+template <typename T, int WM, int WN, int NT, int STAGES, bool WORDS>
+__global__ __launch_bounds__(64 * WM * WN) void tile_kernel(kda_mx4_linear_args a) {
+    using K = Tile<T, WM, WN, NT, STAGES, WORDS>;
+    __shared__ __align__(16) char buf[STAGES][K::kX + K::kW];
     const int lane = threadIdx.x & 63, ln = lane & 15, lg = lane >> 4;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wn = wave & 1, wm = wave >> 1;
-    const int64_t n0 = static_cast<int64_t>(blockIdx.x) * kTile, m0 = static_cast<int64_t>(blockIdx.y) * kTile;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wn = wave % WN, wm = wave / WN;
+    const int64_t n0 = static_cast<int64_t>(blockIdx.x) * K::kN, m0 = static_cast<int64_t>(blockIdx.y) * K::kM;
     const int groups = static_cast<int>(a.K / 32), chunks = (groups + 3) / 4;
-    const int last = static_cast<int>(min(a.M - 1 - m0, static_cast<int64_t>(kTile - 1)));
+    const int last_m = static_cast<int>(min(a.M - 1 - m0, static_cast<int64_t>(K::kM - 1)));
+    const int last_n = static_cast<int>(min(a.N - 1 - n0, static_cast<int64_t>(K::kN - 1)));
     const T* xb = static_cast<const T*>(a.x) + m0 * a.x_stride;
-    const uint8_t *w[4], *scale[4];
+    const uint8_t* wb = static_cast<const uint8_t*>(a.w) + n0 * groups * 16;
+    const uint8_t* scale[NT];
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-        const int64_t n = min(n0 + 64 * wn + 16 * t + ln, a.N - 1) * groups;
-        w[t] = static_cast<const uint8_t*>(a.w) + 16 * n;
-        scale[t] = static_cast<const uint8_t*>(a.w_scale) + n;
+    for (int t = 0; t < NT; ++t)
+        scale[t] = static_cast<const uint8_t*>(a.w_scale) + min(n0 + 16 * (NT * wn + t) + ln, a.N - 1) * groups;
+    // a lane's rows of a stage, and its piece of each: constant from chunk to chunk
+    int x_at[K::kXLoads], w_at[K::kWLoads];
+#pragma unroll
+    for (int i = 0; i < K::kXLoads; ++i) {               // four rows a load
+        const int r = 4 * (K::kXLoads * wave + i) + lg;
+        x_at[i] = min(r, last_m) * static_cast<int>(a.x_stride) * 2 + 16 * (ln ^ (r & 15));
     }
-    const int pieces = 4 * groups;               // of 8 channels, in a row of x
-    const auto load_x = [&](int c, char* to) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {            // four rows a load
-            const int r = 32 * wave + 4 * i + lg;
-            const int piece = min(16 * c + (ln ^ (r & 15)), pieces - 1);
-            to_lds(xb, (min(r, last) * static_cast<int>(a.x_stride) + 8 * piece) * 2, to + (32 * wave + 4 * i) * (2 * kChunk));
+    for (int i = 0; i < K::kWLoads; ++i) {               // sixteen
+        const int r = 16 * (K::kWLoads * wave + i) + (lane >> 2);
+        w_at[i] = 16 * (min(r, last_n) * groups + ((lane & 3) ^ ((r >> 2) & 3)));
+    }
+    const auto load = [&](int c, char* stage) {
+        char* xs = stage + 1024 * K::kXLoads * wave;
+        char* ws = stage + K::kX + 1024 * K::kWLoads * wave;
+        if (4 * c + 4 <= groups) {
+#pragma unroll
+            for (int i = 0; i < K::kXLoads; ++i) to_lds(xb + kChunk * static_cast<int64_t>(c), x_at[i], xs + 1024 * i);
+#pragma unroll
+            for (int i = 0; i < K::kWLoads; ++i) to_lds(wb + 64 * static_cast<int64_t>(c), w_at[i], ws + 1024 * i);
+        } else {                                         // pieces past the last are read as it
+            const int held = groups - 4 * c;
+#pragma unroll
+            for (int i = 0; i < K::kXLoads; ++i) {
+                const int piece = ln ^ ((4 * (K::kXLoads * wave + i) + lg) & 15);
+                to_lds(xb + kChunk * static_cast<int64_t>(c), x_at[i] - 16 * max(piece - (4 * held - 1), 0), xs + 1024 * i);
+            }
+#pragma unroll
+            for (int i = 0; i < K::kWLoads; ++i) {
+                const int piece = (lane & 3) ^ (((16 * (K::kWLoads * wave + i) + (lane >> 2)) >> 2) & 3);
+                to_lds(wb + 64 * static_cast<int64_t>(c), w_at[i] - 16 * max(piece - (held - 1), 0), ws + 1024 * i);
+            }
         }
     };
-    const auto load_w = [&](int c, uint4 (&p)[4], uint32_t (&e)[4]) {
-        const int g = min(4 * c + lg, groups - 1);
+    // the scales of four chunks from c on: a lane group a chunk's
+    const auto load_scales = [&](int c, uint32_t (&e)[NT]) {
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-            p[t] = *reinterpret_cast<const uint4*>(w[t] + 16 * g);
-            e[t] = scale[t][g];
+        for (int t = 0; t < NT; ++t) {
+            if constexpr (WORDS) {
+                e[t] = *reinterpret_cast<const uint32_t*>(scale[t] + min(4 * (c + lg), groups - 4));
+            } else {
+                e[t] = 0;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) e[t] |= static_cast<uint32_t>(scale[t][min(4 * (c + lg) + i, groups - 1)]) << (8 * i);
+            }
         }
     };
-    f4 acc[4][4];
+    f4 acc[NT][4];
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
+    for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int m = 0; m < 4; ++m) acc[t][m] = f4{0.f, 0.f, 0.f, 0.f};
-    uint4 p[4], next[4];
-    uint32_t e[4], next_e[4];
-    load_w(0, p, e);
-    load_x(0, buf[0]);
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    for (int c = 0; c < chunks; ++c) {
-        if (c + 1 < chunks) {
-            load_w(c + 1, next, next_e);
-            load_x(c + 1, buf[(c + 1) & 1]);
-        }
-        const char* from = buf[c & 1] + (64 * wm + ln) * (2 * kChunk);
-        const bool past = 4 * c + lg >= groups;          // no channels of the lane's: zero, on both sides
-        if (past) {
+    uint32_t next[NT];
+    load_scales(0, next);
 #pragma unroll
-            for (int t = 0; t < 4; ++t) p[t] = uint4{0, 0, 0, 0};
-        }
+    for (int i = 0; i < STAGES - 1; ++i) load(min(i, chunks - 1), buf[i]);
+    int at = 0;                                          // the stage of chunk c
+    for (int c0 = 0; c0 < chunks; c0 += 4) {
+        uint32_t e[NT][4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            uint4 x[4];
+        for (int t = 0; t < NT; ++t) hand_around<4>(next[t], e[t]);
+        load_scales(min(c0 + 4, chunks - 1), next);
 #pragma unroll
-            for (int m = 0; m < 4; ++m) {
-                x[m] = *reinterpret_cast<const uint4*>(from + 16 * m * (2 * kChunk) + 16 * ((4 * lg + i) ^ ln));
-                if (past) x[m] = uint4{0, 0, 0, 0};
+        for (int j = 0; j < 4; ++j) {
+            const int c = c0 + j;
+            if (c >= chunks) break;
+            // chunk c is there, in every wave; the stage of chunk c - 1 is free
+            landed<(STAGES - 2) * (K::kXLoads + K::kWLoads)>();
+            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            load(min(c + STAGES - 1, chunks - 1), buf[at == 0 ? STAGES - 1 : at - 1]);
+            const char* xs = buf[at] + (64 * wm + ln) * (2 * kChunk);
+            const char* ws = buf[at] + K::kX + (16 * NT * wn + ln) * (kChunk / 2) + 16 * (lg ^ ((ln >> 2) & 3));
+            uint4 p[NT], x[4][4];
+#pragma unroll
+            for (int t = 0; t < NT; ++t) p[t] = *reinterpret_cast<const uint4*>(ws + 16 * t * (kChunk / 2));
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int m = 0; m < 4; ++m)
+                    x[i][m] = *reinterpret_cast<const uint4*>(xs + 16 * m * (2 * kChunk) + 16 * ((4 * lg + i) ^ ln));
+            asm volatile("" ::: "memory");              // all asked for before the first product
+            float power[NT];
+#pragma unroll
+            for (int t = 0; t < NT; ++t) power[t] = __uint_as_float((e[t][j] >> (8 * lg) & 255u) << 23);
+            if (4 * c + 4 > groups && 4 * c + lg >= groups) {       // no channels of the lane's: zero, on both sides
+#pragma unroll
+                for (int t = 0; t < NT; ++t) p[t] = uint4{0, 0, 0, 0}, power[t] = 0.f;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int m = 0; m < 4; ++m) x[i][m] = uint4{0, 0, 0, 0};
             }
 #pragma unroll
-            for (int t = 0; t < 4; ++t) {
-                const uint4 wide = mla::widen4<T>(word(p[t], i), power(e[t], 0));
+            for (int i = 0; i < 4; ++i)
 #pragma unroll
-                for (int m = 0; m < 4; ++m) acc[t][m] = Act<T>::mma16(wide, x[m], acc[t][m]);
-            }
+                for (int t = 0; t < NT; ++t) {
+                    const uint4 wide = mla::widen4<T>(word(p[t], i), power[t]);
+#pragma unroll
+                    for (int m = 0; m < 4; ++m) acc[t][m] = Act<T>::mma16(wide, x[i][m], acc[t][m]);
+                }
+            at = at + 1 == STAGES ? 0 : at + 1;
         }
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();
-#pragma unroll
-        for (int t = 0; t < 4; ++t) p[t] = next[t], e[t] = next_e[t];
     }
+    landed<0>();                                         // no load is under way when the workgroup's LDS goes to another
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
+    for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
-            const int64_t row = m0 + 64 * wm + 16 * m + ln, n = n0 + 64 * wn + 16 * t + 4 * lg;
+            const int64_t row = m0 + 64 * wm + 16 * m + ln, n = n0 + 16 * (NT * wn + t) + 4 * lg;
             Beside<T> beside;
             beside.load(a, row, n);
             put<T>(a, row, n, acc[t][m], beside);
         }
 }
 
-#include <cstdlib>
-static int tune(const char* n, int d) { const char* s = getenv(n); return s ? atoi(s) : d; }
-template <typename T, int MT, int NT, int SPLIT, int D>
-void launch_few(const kda_mx4_linear_args& a, hipStream_t stream) {
-    const unsigned grid = static_cast<unsigned>((a.N + 16 * NT - 1) / (16 * NT));
+template <typename T, int MT, int NT, int SPLIT, int SPAN>
+void launch_rows(const kda_mx4_linear_args& a, hipStream_t stream) {
+    const dim3 grid(static_cast<unsigned>((a.N + 16 * NT - 1) / (16 * NT)), static_cast<unsigned>((a.M + 16 * MT - 1) / (16 * MT)));
     if (a.K % 128 == 0 && reinterpret_cast<uintptr_t>(a.w_scale) % 4 == 0)
-        few_kernel<T, MT, NT, SPLIT, D, true><<<grid, 64 * SPLIT, 0, stream>>>(a);
+        rows_kernel<T, MT, NT, SPLIT, SPAN, true><<<grid, 64 * SPLIT, 0, stream>>>(a);
     else
-        few_kernel<T, MT, NT, SPLIT, D, false><<<grid, 64 * SPLIT, 0, stream>>>(a);
-}
-template <typename T, int MT, int NT, int SPLIT>
-void launch_d(const kda_mx4_linear_args& a, hipStream_t stream) {
-    const int d = tune("TD", MT == 1 ? 2 : 1);
-    if (d == 1 || MT == 4) launch_few<T, MT, NT, SPLIT, 1>(a, stream);
-    else launch_few<T, MT, NT, SPLIT, MT == 4 ? 1 : 2>(a, stream);
-}
-template <typename T, int MT, int NT>
-void launch_split(const kda_mx4_linear_args& a, hipStream_t stream) {
-    const int64_t spans = (a.K + 511) / 512;
-    const int sp = tune("TS", spans >= 8 ? 8 : spans >= 3 ? 4 : spans);
-    if (sp == 8) launch_d<T, MT, NT, 8>(a, stream);
-    else if (sp == 4) launch_d<T, MT, NT, 4>(a, stream);
-    else if (sp == 2) launch_d<T, MT, NT, 2>(a, stream);
-    else launch_d<T, MT, NT, 1>(a, stream);
+        rows_kernel<T, MT, NT, SPLIT, SPAN, false><<<grid, 64 * SPLIT, 0, stream>>>(a);
 }
 
+template <typename T, int WM, int WN, int NT, int STAGES>
+void launch_tile(const kda_mx4_linear_args& a, hipStream_t stream) {
+    using K = Tile<T, WM, WN, NT, STAGES, true>;
+    const dim3 grid(static_cast<unsigned>((a.N + K::kN - 1) / K::kN), static_cast<unsigned>((a.M + K::kM - 1) / K::kM));
+    if (a.K % 128 == 0 && reinterpret_cast<uintptr_t>(a.w_scale) % 4 == 0)
+        tile_kernel<T, WM, WN, NT, STAGES, true><<<grid, K::kThreads, 0, stream>>>(a);
+    else
+        tile_kernel<T, WM, WN, NT, STAGES, false><<<grid, K::kThreads, 0, stream>>>(a);
+}
+
+// The smallest tiles of outputs that are at most a workgroup a CU, since a workgroup's way to its
+// first product is most of a small call, and larger ones of larger calls, whose operands come
+// less often.  us in a graph of 24 over weights that rotate through 600 MB, fp16 (M, N, K):
+//   M x N of a tile     16x16  16x32  16x64
+//   1, 2048, 2048         3.7    4.6    6.0
+//   1, 8192, 8192        12.5   12.6   17.4
+//   16, 6144, 2048        5.7    5.2    6.4
+//   16, 28672, 8192      53.1   46.9   39.6      (one row 38.9, 37.4, 34.3)
+//                       32x32  32x64  64x32  64x64  64x128  128x128
+//   32, 2048, 2048        5.6    7.5    6.0    8.6
+//   32, 28672, 8192      56.8   46.5   64.3   53.6    55.5
+//   53, 6160, 4096       14.7   13.5   12.3   16.3    28.3
+//   64, 28672, 8192      87.5   73.7   82.6   61.8    57.4
+//   128, 6144, 2048      12.0   11.7   13.2   10.3    16.3     27.7
+//   128, 16384, 4096     48.4   38.7   43.7   35.3    29.3     51.9
+// 64x128 with eight waves of 64x16, and with four of 64x32, and 128x128 with four of 64x64 (bf16
+// for the last two):
+//   300, 6144, 2048      17.7   18.7   28.4
+//   1500, 6144, 2048     59.6   49.6   59.5
+//   4000, 6144, 2048    125.6  107.4  105.0
+//   8192, 8192, 8192     1207    978    911
 template <typename T>
 int launch_linear(const kda_mx4_linear_args& a, hipStream_t stream) {
-    const int nt = tune("TN", a.N > 8192 ? 2 : 1);
-    if (a.M > 64) {
-        const dim3 grid(static_cast<unsigned>((a.N + kTile - 1) / kTile), static_cast<unsigned>((a.M + kTile - 1) / kTile));
-        many_kernel<T><<<grid, 256, 0, stream>>>(a);
-    } else if (a.M > 32) {
-        if (nt == 1) launch_split<T, 4, 1>(a, stream);
-        else if (nt == 2) launch_split<T, 4, 2>(a, stream);
-        else launch_split<T, 4, 4>(a, stream);
-    } else if (a.M > 16) {
-        if (nt == 1) launch_split<T, 2, 1>(a, stream);
-        else if (nt == 2) launch_split<T, 2, 2>(a, stream);
-        else launch_split<T, 2, 4>(a, stream);
+    const auto tiles = [&](int64_t m, int64_t n) { return ((a.M + m - 1) / m) * ((a.N + n - 1) / n); };
+    constexpr int64_t kCus = 256;
+    if (a.M <= 16) {
+        if (tiles(16, 16) <= kCus) launch_rows<T, 1, 1, 8, 2>(a, stream);
+        else if (tiles(16, 32) <= kCus) launch_rows<T, 1, 2, 8, 2>(a, stream);
+        else launch_rows<T, 1, 4, 4, 4>(a, stream);
+    } else if (tiles(32, 32) <= kCus) {
+        launch_rows<T, 2, 2, 8, 2>(a, stream);
+    } else if (a.M <= 32) {
+        launch_rows<T, 2, 4, 4, 4>(a, stream);
+    } else if (tiles(64, 32) <= kCus) {
+        launch_rows<T, 4, 2, 8, 2>(a, stream);
+    } else if (tiles(64, 64) <= kCus) {
+        launch_rows<T, 4, 4, 8, 2>(a, stream);
+    } else if (tiles(64, 128) <= kCus) {
+        launch_tile<T, 1, 8, 1, 3>(a, stream);
+    } else if (tiles(128, 128) < 6 * kCus) {             // three rounds of two a CU
+        launch_tile<T, 1, 4, 2, 2>(a, stream);
     } else {
-        if (nt == 1) launch_split<T, 1, 1>(a, stream);
-        else if (nt == 2) launch_split<T, 1, 2>(a, stream);
-        else launch_split<T, 1, 4>(a, stream);
+        launch_tile<T, 2, 2, 4, 2>(a, stream);
     }
     return hipGetLastError() == hipSuccess ? KDA_OK : KDA_ERR_LAUNCH;
 }
