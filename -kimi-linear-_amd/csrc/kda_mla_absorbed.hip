@@ -29,11 +29,22 @@
 // largest of the sums, and the terms of the softmax's denominator are divided by the
 // scale again.
 //
+// In 4 bits (e2m1) each 128 channels have a power of two.  The score product's pieces
+// are 32 channels of a key, so a scale is one operand of the conversion that widens them (in fp16,
+// which holds fewer powers, it multiplies the group's products instead).  In the value product a
+// wave's channels are of one group, so as in 8 bits the scale enters through the exponent, each
+// wave for its own: a wave has its own maximum and denominator, and so has a part of a sequence
+// for each group.  A transposed read gives a lane sixteen keys of a channel, the window's
+// quarter of its lane group.  The maximum may lag, as the arithmetic, and not the bytes, is
+// most of a window: 386 vector operations before the scales went into the conversions, the lag, the
+// constant load offsets and the masks only where there is one to apply, about 290 after.
+//
 // At 16 heads, R=512 P=64 (a copy reaches 4.8 TB/s): B=64 of 8192 tokens 115 us
 // (5.2 TB/s), of 64 to 4096 tokens 40.5 us from HBM, in 8 bits 128 to 8192 43.5 us,
 // with 5 us of them the join; one sequence of 32768 17.8 us, in 8 bits 15.5; of 200,
 // in one workgroup, 10 us: a window is 1.5 us and the way to the first one 3.  32 heads
-// of that batch 67 us, 64 121, 128 169.
+// of that batch 67 us, 64 121, 128 169.  In 4 bits B=64 of 8192 tokens 54 us, of 128 to 8192
+// 35, one of 65536 20, of 200 8.6.
 #include <hip/hip_runtime.h>
 
 #include "kda_launch.h"
@@ -129,6 +140,8 @@ struct Kernel {
     static constexpr int kTiles = R / 16 / WAVES;               // 16-channel tiles of a wave
     static constexpr int ES = BITS == 16 ? 2 : 1, RB = R * BITS / 8, PB = P * BITS / 8;   // bytes (of a stride's unit, a row)
     static constexpr int kScales = F4 ? R / kGroup : 1;         // scales of a row's latent part
+    // bf16 holds every value times its scale: the conversion of a 4-bit row's values takes it in.
+    static constexpr bool kWide = Elem<T>::code == KDA_DTYPE_BF16;
     static constexpr int kLatRows = 1024 / RB, kLat = kUnit / kLatRows;          // rows a load, loads a unit
     static constexpr int kPosRows = P == 0 || 1024 / PB > kUnit ? kUnit : 1024 / PB, kPos = P == 0 ? 0 : kUnit / kPosRows;
     static constexpr int kPosUnit = kPos * 1024;                // bytes of a unit's position parts (whole loads)
@@ -140,7 +153,7 @@ struct Kernel {
         char buf[2][kBuffer];            // [kWindow][R], [WAVES][kPosUnit], scales
         float s[kRows][kScore];
         float inv[F8 ? kWindow : 4];
-        float e[F4 ? kScales : 1][F4 ? kWindow : 4];         // log2 of the groups' scales
+        float e[F4 ? kScales : 1][F4 ? kWindow : 4], e_inv[F4 ? kScales : 1][F4 ? kWindow : 4];    // log2 of the groups' scales, and 1 / scale
     };
 
     // Where piece c of row r lies: of the latent, with r = r0 + x, r0 a multiple of the rows of a load and x
@@ -153,6 +166,34 @@ struct Kernel {
     }
     static __device__ __forceinline__ int pos_piece(int r, int c) {
         return PB < 32 ? c : c ^ (PB == 128 ? (r >> 1) & 7 : (PB == 64 ? (r >> 2) & 3 : (r >> 3) & 1));
+    }
+
+    // Offsets of what a lane loads of a 4-bit unit's rows: the same for every unit whose rows all exist.
+    struct Offsets {
+        int lat[F4 ? kLat : 1], pos, scale;
+    };
+    static __device__ __forceinline__ Offsets offsets(const kda_mla_absorbed_args& a, int lane) {
+        Offsets o{};
+        if constexpr (F4) {
+            const int stride = static_cast<int>(a.cache_stride[1]), x = lane / (RB / 16), c = lane % (RB / 16);
+#pragma unroll
+            for (int i = 0; i < kLat; ++i) o.lat[i] = (kLatRows * i + x) * stride + 16 * (c ^ turn(kLatRows * i, x));
+            if constexpr (P > 0) {
+                const int r = lane / (PB / 16) % kUnit;
+                o.pos = r * stride + RB + 16 * pos_piece(r, lane % (PB / 16));
+            }
+            o.scale = ((lane >> 1) & 15) * static_cast<int>(a.scale_stride[1]) + 4 * (lane & 1);
+        }
+        return o;
+    }
+    static __device__ __forceinline__ void load_whole(const kda_mla_absorbed_args& a, int64_t b, int j, int wave, const Offsets& o,
+                                                      char* buf) {
+        const char* rows = static_cast<const char*>(a.cache) + (b * a.cache_stride[0] + j * a.cache_stride[1]);
+        const char* scales = static_cast<const char*>(a.cache_scale) + (b * a.scale_stride[0] + j * a.scale_stride[1]);
+#pragma unroll
+        for (int i = 0; i < kLat; ++i) to_lds(rows, o.lat[i], buf + (kUnit * wave + kLatRows * i) * RB);
+        if constexpr (P > 0) to_lds(rows, o.pos, buf + kPosAt + wave * kPosUnit);
+        word_to_lds(scales, o.scale, buf + kScaleAt + 256 * wave);
     }
 
     // A unit's rows, keys j.. of which those past hi - 1 repeat it, into their place in a buffer.
@@ -250,9 +291,13 @@ struct Kernel {
             if (ln == 0) *reinterpret_cast<f4*>(sh.inv + kUnit * wave + 4 * lg) = r;
         } else if constexpr (F4) {
             // a piece is one key's 32 channels, so four products on end are of one group
-            const char* scale = buf + kScaleAt + 256 * wave;
-            const u4 w01 = *reinterpret_cast<const u4*>(scale + 32 * lg), w23 = *reinterpret_cast<const u4*>(scale + 32 * lg + 16);
-            const int byte = *reinterpret_cast<const uint8_t*>(scale + 8 * ln + (lg < kScales ? lg : 0));
+            const uint2 own = *reinterpret_cast<const uint2*>(buf + kScaleAt + 256 * wave + 8 * ln);    // key ln's scales
+            u4 w01{}, w23{};
+            if constexpr (!kWide) {
+                w01 = *reinterpret_cast<const u4*>(buf + kScaleAt + 256 * wave + 32 * lg);              // keys 4 lg + i's
+                w23 = *reinterpret_cast<const u4*>(buf + kScaleAt + 256 * wave + 32 * lg + 16);
+            }
+            const int byte = static_cast<int>(own.x >> (8 * (lg < kScales ? lg : 0)) & 255u);
             stay();
             f4 lat[kReads], far{};
 #pragma unroll
@@ -260,19 +305,32 @@ struct Kernel {
 #pragma unroll
             for (int n = 0; n < 4; ++n)
 #pragma unroll
-                for (int k = 0; k < kReads; ++k) lat[k] = Act<T>::mma16(widen4<T>(piece[k][n]), st.q[4 * k + n], lat[k]);
+                for (int k = 0; k < kReads; ++k)
+                    lat[k] = Act<T>::mma16(widen4<T>(piece[k][n], kWide ? power(own.x, k) : 1.f), st.q[4 * k + n], lat[k]);
 #pragma unroll
-            for (int k = 0; k < P / 32; ++k) far = Act<T>::mma16(widen4<T>(tail4[k]), st.q[R / 32 + k], far);
-            const uint32_t w[4][2] = {{w01[0], w01[1]}, {w01[2], w01[3]}, {w23[0], w23[1]}, {w23[2], w23[3]}};
+            for (int k = 0; k < P / 32; ++k)
+                far = Act<T>::mma16(widen4<T>(tail4[k], kWide ? power(kScales == 4 ? own.y : own.x, kScales % 4) : 1.f),
+                                    st.q[R / 32 + k], far);
+            if constexpr (kWide) {               // (a scale's NaN has made its key's products NaN)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                float x = P > 0 ? far[i] * power(w[i][kScales / 4], kScales % 4) : 0.f;
+                for (int k = 0; k < kReads; ++k) far += lat[k];
 #pragma unroll
-                for (int k = 0; k < kReads; ++k) x = fmaf(lat[k][i], power(w[i][0], k), x);
-                x *= c;
-                s[i] = fmaf(x, 0.f, x);          // an infinity is a scale's NaN
+                for (int i = 0; i < 4; ++i) s[i] = far[i] * c;
+            } else {
+                const uint32_t w[4][2] = {{w01[0], w01[1]}, {w01[2], w01[3]}, {w23[0], w23[1]}, {w23[2], w23[3]}};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float x = P > 0 ? far[i] * power(w[i][kScales / 4], kScales % 4) : 0.f;
+#pragma unroll
+                    for (int k = 0; k < kReads; ++k) x = fmaf(lat[k][i], power(w[i][0], k), x);
+                    x *= c;
+                    s[i] = fmaf(x, 0.f, x);      // an infinity is a scale's NaN
+                }
             }
-            if (lg < kScales) sh.e[lg][kUnit * wave + ln] = byte == 255 ? __builtin_nanf("") : static_cast<float>(byte - 127);
+            if (lg < kScales) {
+                sh.e[lg][kUnit * wave + ln] = byte == 255 ? __builtin_nanf("") : static_cast<float>(byte - 127);
+                sh.e_inv[lg][kUnit * wave + ln] = __uint_as_float(static_cast<uint32_t>(254 - byte) << 23);
+            }
         } else {
             stay();
             f4 acc{}, odd{};
@@ -293,32 +351,45 @@ struct Kernel {
     // First of the eight keys of a window that lane group lg has in step k of the value product.
     static __device__ __forceinline__ int at(int k, int lg) { return F4 ? 16 * lg + 8 * k : 32 * k + 8 * lg; }
 
+    static __device__ __forceinline__ void rescale(State& st, float alpha) {
+        st.sum *= alpha;
+#pragma unroll
+        for (int i = 0; i < kTiles; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) st.o[i][e] *= alpha;
+    }
+
     // A window at keys j0..; its rows are in `buf`, the next window's are asked for into `next`.
     static __device__ __forceinline__ void window(const kda_mla_absorbed_args& a, int64_t b, int j0, int hi, int limit,
-                                                  float c, int wave, int lane, const char* buf, char* next, Shared& sh,
-                                                  State& st) {
+                                                  float c, int wave, int lane, const Offsets& offs, const char* buf, char* next,
+                                                  Shared& sh, State& st) {
         const int ln = lane & 15, lg = lane >> 4;
-        if (j0 + kWindow < hi) load(a, b, j0 + kWindow + kUnit * wave, hi, wave, lane, next);
+        if (j0 + kWindow < hi) {
+            const int j = j0 + kWindow + kUnit * wave;
+            if (F4 && j + kUnit <= hi) load_whole(a, b, j, wave, offs, next);
+            else load(a, b, j, hi, wave, lane, next);
+        }
         f4 s = scores(buf, st, c, sh, wave, ln, lg);
         const int key = j0 + kUnit * wave + 4 * lg;
+        if (!F4 || __any(key + 3 > limit)) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (key + i > limit) s[i] = -INFINITY;
+            for (int i = 0; i < 4; ++i)
+                if (key + i > limit) s[i] = -INFINITY;
+        }
         *reinterpret_cast<f4*>(&sh.s[ln][kUnit * wave + 4 * lg]) = s;
         lds_barrier();
 
         uint4 p[kWindow / 32];
         float x[kWindow / 32][8], mx = kNoMax;
-        f4 e2[kWindow / 32][2];
 #pragma unroll
         for (int k = 0; k < kWindow / 32; ++k) {
             const f4* from = reinterpret_cast<const f4*>(&sh.s[ln][at(k, lg)]);
             f4 lo4 = from[0], hi4 = from[1];
             if constexpr (F4) {                  // each wave against its own channels' scales
                 const f4* more = reinterpret_cast<const f4*>(&sh.e[kScales * wave / WAVES][at(k, lg)]);
-                e2[k][0] = more[0], e2[k][1] = more[1];
+                const f4 e0 = more[0], e1 = more[1];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) lo4[e] += e2[k][0][e], hi4[e] += e2[k][1][e];
+                for (int e = 0; e < 4; ++e) lo4[e] += e0[e], hi4[e] += e1[e];
             }
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
@@ -327,32 +398,48 @@ struct Kernel {
                 mx = fmaxf(mx, fmaxf(lo4[e], hi4[e]));
             }
         }
-        mx = fmaxf(st.top, reference<T>(lanegroup4_max(mx)));
-        const float alpha = __builtin_amdgcn_exp2f(st.top - mx);
-        st.top = mx;
+        float alpha = 1.f;
+        if constexpr (F4) {
+            // the maximum may lag: in bf16, which has the range, by 2^8.  Most windows then leave the sums as they are.
+            constexpr float kLag = Elem<T>::code == KDA_DTYPE_F16 ? 0.f : 8.f;
+            mx = reference<T>(lanegroup4_max(mx));
+            if (__any(mx > st.top + kLag)) {
+                mx = fmaxf(st.top, mx);
+                rescale(st, __builtin_amdgcn_exp2f(st.top - mx));
+                st.top = mx;
+            }
+            mx = st.top;
+        } else {
+            mx = fmaxf(st.top, reference<T>(lanegroup4_max(mx)));
+            alpha = __builtin_amdgcn_exp2f(st.top - mx);
+            st.top = mx;
+        }
         float part = 0.f;
 #pragma unroll
         for (int k = 0; k < kWindow / 32; ++k) {
             f4 inv[2];
-            if constexpr (F8) {
-                inv[0] = *reinterpret_cast<const f4*>(&sh.inv[32 * k + 8 * lg]);
-                inv[1] = *reinterpret_cast<const f4*>(&sh.inv[32 * k + 8 * lg + 4]);
+            if constexpr (F8 || F4) {
+                const f4* from = reinterpret_cast<const f4*>(F4 ? &sh.e_inv[kScales * wave / WAVES][at(k, lg)] : &sh.inv[at(k, lg)]);
+                inv[0] = from[0];
+                inv[1] = from[1];
             }
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 x[k][e] = __builtin_amdgcn_exp2f(x[k][e] - mx);
-                if constexpr (F8) part = fmaf(x[k][e], inv[e / 4][e % 4], part);
-                else if constexpr (F4) part += __builtin_amdgcn_ldexpf(x[k][e], -static_cast<int>(e2[k][e / 4][e % 4]));
-                else part += x[k][e];
+                part = F8 || F4 ? fmaf(x[k][e], inv[e / 4][e % 4], part) : part + x[k][e];
             }
             p[k] = uint4{Act<T>::pair(x[k][0], x[k][1]), Act<T>::pair(x[k][2], x[k][3]), Act<T>::pair(x[k][4], x[k][5]),
                          Act<T>::pair(x[k][6], x[k][7])};
         }
-        st.sum = fmaf(st.sum, alpha, part);
+        if constexpr (F4) {
+            st.sum += part;
+        } else {
+            st.sum = fmaf(st.sum, alpha, part);
 #pragma unroll
-        for (int i = 0; i < kTiles; ++i)
+            for (int i = 0; i < kTiles; ++i)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) st.o[i][e] *= alpha;
+                for (int e = 0; e < 4; ++e) st.o[i][e] *= alpha;
+        }
         values(buf, p, wave, ln, lg, st);
         landed();                        // the next window's
         lds_barrier();
@@ -415,6 +502,7 @@ struct Kernel {
         const int rows = static_cast<int>(a.T * a.H), m0 = rt * kRows;
         const float c = a.scale * kLog2E;
         load(a, b, lo + kUnit * wave, hi, wave, lane, sh.buf[0]);
+        const Offsets offs = offsets(a, lane);
         // the queries through the other buffer: each piece is read from memory once
         const Queries rq(a, m0);
         constexpr int kQStride = D + 8, kPieces = kRows * (D / 8), kPer = (kPieces + kThreads - 1) / kThreads;
@@ -444,8 +532,9 @@ struct Kernel {
         landed();
         lds_barrier();
         for (int j0 = lo; j0 < hi; j0 += 2 * kWindow) {
-            window(a, b, j0, hi, limit, c, wave, lane, sh.buf[0], sh.buf[1], sh, st);
-            if (j0 + kWindow < hi) window(a, b, j0 + kWindow, hi, limit, c, wave, lane, sh.buf[1], sh.buf[0], sh, st);
+            window(a, b, j0, hi, limit, c, wave, lane, offs, sh.buf[0], sh.buf[1], sh, st);
+            if (j0 + kWindow < hi)
+                window(a, b, j0 + kWindow, hi, limit, c, wave, lane, offs, sh.buf[1], sh.buf[0], sh, st);
         }
         const float den = lanegroup4_sum(st.sum), norm = den == 0.f ? 0.f : 1.f / den;
         const int ch = 16 * kTiles * wave + 4 * lg;
@@ -653,9 +742,12 @@ int row_tiles(int64_t T, int64_t H) { return static_cast<int>((T * H + kRows - 1
 // Workgroups of the shared form: one a CU.  Two leave twice the parts to join
 // and are no faster in between; us at 16 heads, 256 / 512 workgroups: B=64 of 64
 // to 4096 tokens 36.8 / 44.4, in 8 bits 29.7 / 29.6; B=16 of 8192 34.1 / 40.2, in 8
-// bits 23.9 / 25.8.
+// bits 23.9 / 25.8.  In 4 bits a window is mostly arithmetic, which two workgroups hide for each
+// other where there are four windows for each: 64 of 128 to 8192 36.2 / 35.0, 200 of 10 to 2000
+// 59.5 / 47.6, 16 of 8192 at 64 heads 34.7 / 32.3, but 64 of 16 to 1024 15.7 / 17.4, one of 65536 20.3 / 23.7.
 constexpr int64_t kGroups = 256;
 static_assert(kGroups > kCut);
+int64_t most_groups(int64_t nv, int64_t S) { return nv * ((S + 63) / 64) >= 8 * kGroups ? 2 * kGroups : kGroups; }
 // Whether the units are shared among the workgroups: where one workgroup a row
 // tile would leave CUs idle or wait for the longest sequence.  us, shared /
 // one a row tile, lengths spread evenly: 300 sequences up to 4096 tokens 158 /
@@ -669,7 +761,7 @@ int launch(const kda_mla_absorbed_args& a, hipStream_t stream) {
     if (!shared_form(nv, a.S)) {
         absorbed_kernel<T, BITS, R, P><<<static_cast<unsigned>(nv), kThreads, 0, stream>>>(a, rts, true);
     } else {
-        constexpr int groups = static_cast<int>(kGroups);
+        const int groups = static_cast<int>(BITS == 4 ? most_groups(nv, a.S) : kGroups);
         absorbed_kernel<T, BITS, R, P><<<groups, kThreads, 0, stream>>>(a, rts, false);
         // many rows have few parts each, and few rows may have many
         const dim3 grid(static_cast<unsigned>(nv), kRows);
@@ -704,7 +796,7 @@ int launch_rank(const kda_mla_absorbed_args& a, hipStream_t stream) {
 int64_t mla_absorbed_workspace_bytes(int64_t B, int64_t T, int64_t H, int64_t S, int64_t R) {
     const int64_t nv = B * row_tiles(T, H);
     if (nv == 0 || !shared_form(nv, S)) return 0;
-    return slots(kGroups, nv) * kRows * (R * 4 + 8 * (R / kGroup)) + nv * 8;
+    return slots(most_groups(nv, S), nv) * kRows * (R * 4 + 8 * (R / kGroup)) + nv * 8;
 }
 
 int mla_absorbed_launch(const kda_mla_absorbed_args& a, hipStream_t stream) {
