@@ -77,11 +77,9 @@ struct Beside {
         }
     }
 };
-// The outputs: bias, rounding, residual.
+// Four outputs: bias, rounding, residual.
 template <typename T>
-__device__ __forceinline__ void put(const kda_mx4_linear_args& a, int64_t row, int64_t n, f4 r, const Beside<T>& s) {
-    if (row >= a.M || n >= a.N) return;
-    T* y = static_cast<T*>(a.y) + row * a.N + n;
+__device__ __forceinline__ uint2 outputs(const kda_mx4_linear_args& a, f4 r, const Beside<T>& s) {
     T out[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -90,11 +88,21 @@ __device__ __forceinline__ void put(const kda_mx4_linear_args& a, int64_t row, i
         if (a.residual) v = Elem<T>::ld(&s.res[j]) + round_elem<T>(v);
         Elem<T>::st(&out[j], v);
     }
+    uint2 raw;
+    __builtin_memcpy(&raw, out, 8);
+    return raw;
+}
+// To their place, n.. of a row.
+template <typename T>
+__device__ __forceinline__ void put(const kda_mx4_linear_args& a, int64_t row, int64_t n, f4 r, const Beside<T>& s) {
+    if (row >= a.M || n >= a.N) return;
+    T* y = static_cast<T*>(a.y) + row * a.N + n;
+    const uint2 raw = outputs<T>(a, r, s);
     if (a.N % 4 == 0) {          // (y is 8-byte aligned)
-        uint2 raw;
-        __builtin_memcpy(&raw, out, 8);
         *reinterpret_cast<uint2*>(y) = raw;
     } else {
+        T out[4];
+        __builtin_memcpy(out, &raw, 8);
 #pragma unroll
         for (int j = 0; j < 4; ++j)
             if (n + j < a.N) y[j] = out[j];
@@ -257,6 +265,12 @@ __global__ __launch_bounds__(64 * SPLIT) void rows_kernel(kda_mx4_linear_args a)
 // channels at a time, asynchronously, STAGES buffers.  x's 16-byte piece c of row r lies at c
 // turned by r, W's by bits of r, so that sixteen rows' pieces are in different banks; W is widened
 // after it is read.  A lane has the same group of x and W, channels 32 lg + 8 i of a chunk in step i.
+//
+// Bound by the matrix cores and what stands beside them: at 8192^3 (1.22 PFLOP/s) 711 us
+// without the loads, 643 without the barriers too, 631 without the conversions and LDS reads
+// as well; over 2048 channels a tile's way in and out is about a fifth of it.  So the W rows of
+// a wave's tiles are dealt in fours, which gives a lane 8 NT bytes of a row of outputs on end
+// (4000 rows by 6144 x 2048 107 -> 101 us).
 constexpr int kChunk = 128;
 
 template <typename T, int WM, int WN, int NT, int STAGES, bool WORDS>
@@ -265,6 +279,11 @@ struct Tile {
     static constexpr int kX = kM * 2 * kChunk, kW = kN * kChunk / 2;             // bytes of a stage
     static constexpr int kXLoads = kX / 1024 / kWaves, kWLoads = kW / 1024 / kWaves;
     static_assert(kXLoads * kWaves * 1024 == kX && kWLoads * kWaves * 1024 == kW, "whole loads, as many each wave");
+    // Row r of tile t is W's 4 NT (r / 4) + 4 t + r % 4 of the wave's, so that a lane's outputs of one row of x, four a
+    // tile, lie on end.
+    static __device__ __forceinline__ int w_row(int t, int r) { return 4 * NT * (r >> 2) + 4 * t + (r & 3); }
+    // What W's row r turns its pieces by: the sixteen rows of a read are in different banks.
+    static __device__ __forceinline__ int turn(int r) { return r / (4 * NT) & 3; }
 };
 
 template <typename T, int WM, int WN, int NT, int STAGES, bool WORDS>
@@ -282,7 +301,7 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(kda_mx4_linear_args 
     const uint8_t* scale[NT];
 #pragma unroll
     for (int t = 0; t < NT; ++t)
-        scale[t] = static_cast<const uint8_t*>(a.w_scale) + min(n0 + 16 * (NT * wn + t) + ln, a.N - 1) * groups;
+        scale[t] = static_cast<const uint8_t*>(a.w_scale) + min(n0 + 16 * NT * wn + K::w_row(t, ln), a.N - 1) * groups;
     // a lane's rows of a stage, and its piece of each: constant from chunk to chunk
     int x_at[K::kXLoads], w_at[K::kWLoads];
 #pragma unroll
@@ -293,7 +312,7 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(kda_mx4_linear_args 
 #pragma unroll
     for (int i = 0; i < K::kWLoads; ++i) {               // sixteen
         const int r = 16 * (K::kWLoads * wave + i) + (lane >> 2);
-        w_at[i] = 16 * (min(r, last_n) * groups + ((lane & 3) ^ ((r >> 2) & 3)));
+        w_at[i] = 16 * (min(r, last_n) * groups + ((lane & 3) ^ K::turn(r)));
     }
     const auto load = [&](int c, char* stage) {
         char* xs = stage + 1024 * K::kXLoads * wave;
@@ -312,7 +331,7 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(kda_mx4_linear_args 
             }
 #pragma unroll
             for (int i = 0; i < K::kWLoads; ++i) {
-                const int piece = (lane & 3) ^ (((16 * (K::kWLoads * wave + i) + (lane >> 2)) >> 2) & 3);
+                const int piece = (lane & 3) ^ K::turn(16 * (K::kWLoads * wave + i) + (lane >> 2));
                 to_lds(wb + 64 * static_cast<int64_t>(c), w_at[i] - 16 * max(piece - (held - 1), 0), ws + 1024 * i);
             }
         }
@@ -354,10 +373,10 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(kda_mx4_linear_args 
             asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
             load(min(c + STAGES - 1, chunks - 1), buf[at == 0 ? STAGES - 1 : at - 1]);
             const char* xs = buf[at] + (64 * wm + ln) * (2 * kChunk);
-            const char* ws = buf[at] + K::kX + (16 * NT * wn + ln) * (kChunk / 2) + 16 * (lg ^ ((ln >> 2) & 3));
+            const char* ws = buf[at] + K::kX + (16 * NT * wn + K::w_row(0, ln)) * (kChunk / 2) + 16 * (lg ^ (ln >> 2));
             uint4 p[NT], x[4][4];
 #pragma unroll
-            for (int t = 0; t < NT; ++t) p[t] = *reinterpret_cast<const uint4*>(ws + 16 * t * (kChunk / 2));
+            for (int t = 0; t < NT; ++t) p[t] = *reinterpret_cast<const uint4*>(ws + 4 * t * (kChunk / 2));
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -388,14 +407,24 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(kda_mx4_linear_args 
     }
     landed<0>();                                         // no load is under way when the workgroup's LDS goes to another
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
+    for (int m = 0; m < 4; ++m) {
+        const int64_t row = m0 + 64 * wm + 16 * m + ln, n = n0 + 16 * NT * wn + 4 * NT * lg;
+        Beside<T> beside[NT];
 #pragma unroll
-        for (int m = 0; m < 4; ++m) {
-            const int64_t row = m0 + 64 * wm + 16 * m + ln, n = n0 + 16 * (NT * wn + t) + 4 * lg;
-            Beside<T> beside;
-            beside.load(a, row, n);
-            put<T>(a, row, n, acc[t][m], beside);
+        for (int t = 0; t < NT; ++t) beside[t].load(a, row, n + 4 * t);
+        if (NT % 2 == 0 && a.N % 8 == 0 && reinterpret_cast<uintptr_t>(a.y) % 16 == 0) {
+            if (row >= a.M) continue;
+#pragma unroll
+            for (int t = 0; t + 1 < NT; t += 2) {
+                if (n + 4 * t >= a.N) break;
+                const uint2 lo = outputs<T>(a, acc[t][m], beside[t]), hi = outputs<T>(a, acc[t + 1][m], beside[t + 1]);
+                *reinterpret_cast<uint4*>(static_cast<T*>(a.y) + row * a.N + n + 4 * t) = uint4{lo.x, lo.y, hi.x, hi.y};
+            }
+        } else {
+#pragma unroll
+            for (int t = 0; t < NT; ++t) put<T>(a, row, n + 4 * t, acc[t][m], beside[t]);
         }
+    }
 }
 
 template <typename T, int MT, int NT, int SPLIT, int SPAN>
@@ -435,9 +464,9 @@ void launch_tile(const kda_mx4_linear_args& a, hipStream_t stream) {
 // 64x128 with eight waves of 64x16, and with four of 64x32, and 128x128 with four of 64x64 (bf16
 // for the last two):
 //   300, 6144, 2048      17.7   18.7   28.4
-//   1500, 6144, 2048     59.6   49.6   59.5
-//   4000, 6144, 2048    125.6  107.4  105.0
-//   8192, 8192, 8192     1207    978    911
+//   1500, 6144, 2048     61.8   48.7   55.4
+//   4000, 6144, 2048    132.0  106.6  101.4     (the library's product of 16-bit operands 98)
+//   8192, 8192, 8192     1238    973    899     (771)
 template <typename T>
 int launch_linear(const kda_mx4_linear_args& a, hipStream_t stream) {
     const auto tiles = [&](int64_t m, int64_t n) { return ((a.M + m - 1) / m) * ((a.N + n - 1) / n); };

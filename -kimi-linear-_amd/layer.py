@@ -280,6 +280,8 @@ class KimiDeltaAttention(nn.Module):
         if four != [True, True, True, False, False, False]:
             raise KdaError("in_proj_q, in_proj_k and in_proj_v are all Mx4Linear or none of them, and beta_proj and the "
                            "gates' first projections are not")
+        if len({m.bias is None for m in mods[:3]}) > 1:
+            raise KdaError("in_proj_q, in_proj_k and in_proj_v all have a bias or none of them")
         return True
 
     def _input_weight4(self):

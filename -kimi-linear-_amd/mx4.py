@@ -178,7 +178,11 @@ class Mx4Linear(nn.Module):
     @classmethod
     @torch.no_grad()
     def from_linear(cls, linear):
-        """The 4-bit form of an ``nn.Linear`` on a HIP device."""
+        """The 4-bit form of an ``nn.Linear`` on a HIP device.  A module that does more than the product with its
+        weight and the bias (an adapter, a hook, a forward of its own) is refused: it would lose that."""
+        if (type(linear) is not nn.Linear or linear._forward_hooks or linear._forward_pre_hooks or "forward" in linear.__dict__):
+            raise KdaError(f"only a plain nn.Linear has a 4-bit form; got {type(linear).__name__} with hooks, a forward of its "
+                           "own or another type")
         w = linear.weight
         data, scale = mx4_quantize(w)
         with torch.inference_mode(False), torch.no_grad():

@@ -244,3 +244,42 @@ def test_inference_mode_and_autocast(kda_pkg):
 def latent_like(kda_pkg, layer):
     """The fp32 layer's bf16 form."""
     return stands_for(kda_pkg, copy.deepcopy(layer).to(BF16))
+
+
+def test_only_plain_projections_are_quantised(kda_pkg):
+    """A projection that does more than its product is refused, and the layer stays as it was."""
+    class Scaled(torch.nn.Linear):
+        def forward(self, x):
+            return 2 * super().forward(x)
+
+    def wrap(kind, lin):
+        if kind == "type":
+            new = Scaled(lin.in_features, lin.out_features, bias=False, device=DEV, dtype=F16)
+            return new
+        if kind == "hook":
+            lin.register_forward_hook(lambda m, a, out: 2 * out)
+        else:
+            lin.forward = lambda x: x
+        return lin
+
+    for kind in ("type", "hook", "forward"):
+        for make, name in ((kda_layer, "o_proj"), (latent_layer, "q_proj")):
+            layer = make(kda_pkg, F16)
+            setattr(layer, name, wrap(kind, getattr(layer, name)))
+            with pytest.raises(kda_pkg.KdaError, match="plain"):
+                layer.quantize_mx4_()
+            assert not any(isinstance(m, kda_pkg.Mx4Linear) for m in layer.modules())
+    layer = kda_layer(kda_pkg, F16, proj_bias=True).quantize_mx4_()
+    layer.in_proj_k.bias = None
+    with pytest.raises(kda_pkg.KdaError, match="bias"), torch.no_grad():
+        layer(torch.randn(1, 5, 256, device=DEV).half())
+
+
+@torch.no_grad()
+def test_hooks_on_quantised_projections(kda_pkg):
+    """A hook on an output projection in 4 bits is called: it is a module like another."""
+    layer = kda_layer(kda_pkg, F16).quantize_mx4_()
+    x = torch.randn(2, 9, 256, device=DEV).half()
+    want = layer(x)
+    layer.o_proj.register_forward_hook(lambda m, a, out: 2 * out)
+    assert torch.equal(layer(x), 2 * want)
