@@ -329,7 +329,7 @@ struct Kernel {
             }
             if (lg < kScales) {
                 sh.e[lg][kUnit * wave + ln] = byte == 255 ? __builtin_nanf("") : static_cast<float>(byte - 127);
-                sh.e_inv[lg][kUnit * wave + ln] = __uint_as_float(static_cast<uint32_t>(254 - byte) << 23);
+                sh.e_inv[lg][kUnit * wave + ln] = __uint_as_float(byte == 254 ? 0x400000u : static_cast<uint32_t>(254 - byte) << 23);   // (2^-127)
             }
         } else {
             stay();

@@ -111,6 +111,23 @@ def test_absorbed_small_groups_in_bf16(kda_pkg):
     close("o", got, want, bound)
 
 
+@pytest.mark.parametrize("S", [40, 3000])
+def test_absorbed_largest_scales(kda_pkg, S):
+    """The largest power there is, 2^127, beside others: its group's denominator is 2^-127 of its sums, a number
+    below the normal ones, which is no zero.  (Queries of zeros: every weight is alike.)"""
+    R, P = 512, 64
+    cache, scale = quantised(rand(2, S, R + P, seed=12, dtype=torch.float32), R)
+    raw(cache).bitwise_and_(0x99)                        # 0 and 0.5, of either sign
+    raw(scale)[..., 0], raw(scale)[..., 1], raw(scale)[..., 2] = 254, 253, 0
+    q = torch.zeros(2, 1, 16, R + P, dtype=BF16, device=DEV)
+    got = kda_pkg.mla_absorbed(q, cache, i32([S, S - 3]), R, 0.1, cache_scale=scale)
+    held = dequantised(cache, scale, R)[..., :R]
+    want = torch.stack([held[0].mean(0), held[1, :S - 3].mean(0)])[:, None, None]
+    # one rounding of the output; the weights are 1, the sums of halves exact, and the denominator has the 22 bits
+    # of a number of that size, as 1 / it and their product have 24 or more
+    close("o", got, want.expand(2, 1, 16, R), half_step(BF16) * (1 + 2.0 ** -8) * want.abs().expand(2, 1, 16, R))
+
+
 @pytest.mark.parametrize("S", [100, 2000])
 def test_absorbed_not_finite(kda_pkg, S):
     """A NaN scale reaches every channel of the queries that see its row, and no other sequence; behind the
