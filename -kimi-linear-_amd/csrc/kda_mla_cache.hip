@@ -1,4 +1,4 @@
-// Rows written into a latent cache, and an 8-bit cache read back.
+// Rows written into a latent cache, and an 8- or 4-bit cache read back.
 //
 // A cache row is a token's latent (R channels) and its position channels (P).
 // Both kernels touch each row once.  To write, a wave takes a row, a lane eight
@@ -7,7 +7,9 @@
 // reductions in registers.  To read back, a lane takes sixteen channels, and the
 // lanes run on from one row into the next.  Bound by HBM for long calls and by the
 // launch for a decode step's few rows: 64 rows of 576 in 8 bits 4 us, 6000 in 16
-// bits 5.2 us (2.9 TB/s), reading 32768 back 11.6 us (4.9 TB/s).
+// bits 5.2 us (2.9 TB/s), reading 32768 back 11.6 us (4.9 TB/s).  In 4 bits 64 rows 4.0
+// us, 8192 7.2, reading 32768 back 11.2; a row's magnitudes are compared as bits and over
+// 16 lanes in the vector unit, without LDS.
 #include <hip/hip_runtime.h>
 
 #include "kda_launch.h"
@@ -96,11 +98,34 @@ __device__ __forceinline__ uint32_t largest(const float (&x)[8]) {
     return m;
 }
 // The sum over a wave in 64 bits, which leaves the row's norm, and with it a value
-// next to a border of the format, to no order of sums.
-__device__ __forceinline__ double wave_sum64(double x) {
-#pragma unroll
-    for (int d = 32; d > 0; d /= 2) x += __shfl_xor(x, d);
+// next to a border of the format, to no order of sums.  (By shuffles through LDS 64 rows
+// took 4.7 us.)
+template <int CTRL>
+__device__ __forceinline__ double turned(double x) {         // within 16 lanes
+    int w[2];
+    __builtin_memcpy(w, &x, 8);
+    w[0] = __builtin_amdgcn_update_dpp(0, w[0], CTRL, 0xf, 0xf, false);
+    w[1] = __builtin_amdgcn_update_dpp(0, w[1], CTRL, 0xf, 0xf, false);
+    __builtin_memcpy(&x, w, 8);
     return x;
+}
+__device__ __forceinline__ double joined(uint32_t lo, uint32_t hi) {
+    const uint64_t w = static_cast<uint64_t>(hi) << 32 | lo;
+    return __builtin_bit_cast(double, w);
+}
+__device__ __forceinline__ double wave_sum64(double x) {
+    x += turned<0x128>(x);                                   // row_ror:8, 4, 2, 1
+    x += turned<0x124>(x);
+    x += turned<0x122>(x);
+    x += turned<0x121>(x);
+    uint64_t w = __builtin_bit_cast(uint64_t, x);
+    const auto l16 = __builtin_amdgcn_permlane16_swap(static_cast<uint32_t>(w), static_cast<uint32_t>(w), false, false);
+    const auto h16 = __builtin_amdgcn_permlane16_swap(static_cast<uint32_t>(w >> 32), static_cast<uint32_t>(w >> 32), false, false);
+    x = joined(l16[0], h16[0]) + joined(l16[1], h16[1]);
+    w = __builtin_bit_cast(uint64_t, x);
+    const auto l32 = __builtin_amdgcn_permlane32_swap(static_cast<uint32_t>(w), static_cast<uint32_t>(w), false, false);
+    const auto h32 = __builtin_amdgcn_permlane32_swap(static_cast<uint32_t>(w >> 32), static_cast<uint32_t>(w >> 32), false, false);
+    return joined(l32[0], h32[0]) + joined(l32[1], h32[1]);
 }
 
 template <typename T, int BITS>
@@ -129,7 +154,7 @@ __global__ __launch_bounds__(64 * kRows) void append_kernel(kda_mla_append_args 
 #pragma unroll
             for (int i = 0; i < 8; ++i) ss = fma(static_cast<double>(x[i]), static_cast<double>(x[i]), ss);
         }
-        const float rstd = static_cast<float>(rsqrt(wave_sum64(ss) / R + static_cast<double>(a.eps)));
+        const float rstd = static_cast<float>(rsqrt(wave_sum64(ss) * (1.f / static_cast<float>(R)) + static_cast<double>(a.eps)));
         if (lat) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) x[i] = x[i] * rstd * w[i];
