@@ -41,20 +41,22 @@ __device__ __forceinline__ void to_lds(const void* base, int offset, char* lds) 
 template <int N>
 __device__ __forceinline__ void landed() { asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory"); }
 
-// A span's scales, a lane group a chunk's, handed around: e[j] of chunk j.
-template <int SPAN>
-__device__ __forceinline__ void hand_around(uint32_t held, uint32_t (&e)[SPAN]) {
-    if constexpr (SPAN == 4) {
-        e[0] = e[2] = held;
-        swap32(e[0], e[2]);
-        e[1] = e[0];
-        e[3] = e[2];
-        swap16(e[0], e[1]);
-        swap16(e[2], e[3]);
-    } else {
-        e[0] = e[1] = held;
-        swap16(e[0], e[1]);
-    }
+// The same, which the compiler takes into account: what came before those it does not wait for again.
+template <int N>
+__device__ __forceinline__ void known_landed() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt((N & 15) | (N >> 4) << 14 | 0xf70);
+    asm volatile("" ::: "memory");
+}
+
+// The scales of four chunks, a lane group a chunk's, handed around: e[j] of chunk j.
+__device__ __forceinline__ void hand_around(uint32_t held, uint32_t (&e)[4]) {
+    e[0] = e[2] = held;
+    swap32(e[0], e[2]);
+    e[1] = e[0];
+    e[3] = e[2];
+    swap16(e[0], e[1]);
+    swap16(e[2], e[3]);
 }
 
 // What goes to four neighbouring outputs n.. of a row beside the product, asked for ahead of it.
@@ -111,20 +113,23 @@ __device__ __forceinline__ void put(const kda_mx4_linear_args& a, int64_t row, i
 
 // ---- few outputs ------------------------------------------------------------
 // Grid (ceil(N / (16 NT)), ceil(M / (16 MT))), 64 SPLIT threads.  MT 16-row tiles of x, NT of
-// W; the waves take spans of SPAN chunks of 128 channels in turn, and their sums meet in LDS.
+// W; the waves take chunks of 128 channels in turn, and their sums meet in LDS.
 //
-// Bound by the way to memory.  Three things carry it.  A span's scales are one load, a lane
+// Bound by the way to memory.  Five things carry it.  Four chunks' scales are one load, a lane
 // group a chunk's, handed around in registers: a load for each chunk took as long as W's own (one
 // row by 28672 x 8192 41 us, without any scales 29).  x goes through LDS, a buffer a wave, where
 // a row's 256 bytes come as one piece; read as operands they come as 64 from each of
-// sixteen rows (53 rows by 6160 x 4096 18.9 us, this way 12.3).  And W and the scales come
+// sixteen rows (53 rows by 6160 x 4096 18.9 us, this way 12.3).  W and the scales come
 // through descriptors that end with the workgroup's rows, so that what does not exist is an
-// offset past the end, which reads as zero without a branch and asks memory for nothing.
+// offset past the end, which reads as zero without a branch and asks memory for nothing.  A chunk's
+// loads are under way while the one before is used, W's a chunk earlier still (the one row 35.2 ->
+// 34.2 us).  And neighbouring waves have neighbouring chunks, which share W's lines of 128 bytes
+// and make 2 KB pieces of x's rows (with two or four chunks on end a wave 34.2, in turn 31.3; the 53 rows 11.7).
 //
 // x's 16-byte piece c of row r lies at c turned by r, so that sixteen rows' pieces are in
 // different banks.  A lane has the same group of x and W, channels 32 lg + 8 i of a chunk in step
 // i.  Rows of x past the last leave what LDS holds, in columns of the product that go nowhere.
-template <typename T, int MT, int NT, int SPLIT, int SPAN, bool WORDS>
+template <typename T, int MT, int NT, int SPLIT, bool WORDS>
 __global__ __launch_bounds__(64 * SPLIT) void rows_kernel(kda_mx4_linear_args a) {
     constexpr int kTiles = NT * MT, kOwn = (kTiles + SPLIT - 1) / SPLIT, kNone = 0x7f000000;
     constexpr int kLoads = 4 * MT;                           // of a chunk of x, four rows each
@@ -171,7 +176,7 @@ __global__ __launch_bounds__(64 * SPLIT) void rows_kernel(kda_mx4_linear_args a)
             p[t] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(w, there ? w_at[t] + 64 * c : kNone, 0, 0));
     };
     const auto load_scales = [&](int c, uint32_t (&e)[NT]) {
-        const int g = 4 * (c + lg % SPAN);
+        const int g = 4 * (c + SPLIT * lg);
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
             if constexpr (WORDS) {
@@ -198,23 +203,26 @@ __global__ __launch_bounds__(64 * SPLIT) void rows_kernel(kda_mx4_linear_args a)
     for (int o = 0; o < kOwn; ++o)
         if (wave + o * SPLIT < kTiles) beside[o].load(a, row(wave + o * SPLIT), col(wave + o * SPLIT));
 
+    // Under way at the top of a chunk: its W and x, then the next chunk's W.  As soon as x is in registers its
+    // buffer takes the next chunk's, as soon as W's words are used their registers take the chunk's after that.
     uint32_t next[NT];
     uint4 p[2][NT];
-    load_scales(SPAN * wave, next);
-    load_w(SPAN * wave, p[0]);
-    for (int c0 = SPAN * wave; c0 < chunks; c0 += SPAN * SPLIT) {
-        uint32_t e[NT][SPAN];
+    load_scales(wave, next);
+    load_w(wave, p[0]);
+    if (wave < chunks) load_x(wave);
+    load_w(wave + SPLIT, p[1]);
+    for (int c0 = wave; c0 < chunks; c0 += 4 * SPLIT) {
+        uint32_t e[NT][4];
 #pragma unroll
-        for (int t = 0; t < NT; ++t) hand_around<SPAN>(next[t], e[t]);
-        load_scales(c0 + SPAN * SPLIT, next);
-#pragma unroll
-        for (int j = 0; j < SPAN; ++j) {
-            const int c = c0 + j;
+        for (int j = 0; j < 4; ++j) {
+            const int c = c0 + j * SPLIT;
             if (c >= chunks) break;
             uint4 x[4][MT];
-            load_x(c);
-            load_w(j + 1 < SPAN ? c + 1 : c0 + SPAN * SPLIT, p[(j + 1) % 2]);
-            landed<NT>();                                        // all but the next chunk's W
+            known_landed<NT>();
+            if (j == 0) {
+#pragma unroll
+                for (int t = 0; t < NT; ++t) hand_around(next[t], e[t]);
+            }
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -226,6 +234,10 @@ __global__ __launch_bounds__(64 * SPLIT) void rows_kernel(kda_mx4_linear_args a)
 #pragma unroll
                     for (int m = 0; m < MT; ++m) x[i][m] = uint4{0, 0, 0, 0};
             }
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the chunk has been read: the next may lie there
+            const int after = c + SPLIT;
+            if (j == 0) load_scales(c0 + 4 * SPLIT, next);
+            if (after < chunks) load_x(after);
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
                 const float pw = __uint_as_float((e[t][j] >> (8 * lg) & 255u) << 23);
@@ -236,7 +248,7 @@ __global__ __launch_bounds__(64 * SPLIT) void rows_kernel(kda_mx4_linear_args a)
                     for (int m = 0; m < MT; ++m) acc[t][m] = Act<T>::mma16(wide, x[i][m], acc[t][m]);
                 }
             }
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the chunk has been read: the next may lie there
+            load_w(c + 2 * SPLIT, p[j % 2]);
         }
     }
     landed<0>();                                                 // (the scales asked for last)
@@ -362,7 +374,7 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(kda_mx4_linear_args 
     for (int c0 = 0; c0 < chunks; c0 += 4) {
         uint32_t e[NT][4];
 #pragma unroll
-        for (int t = 0; t < NT; ++t) hand_around<4>(next[t], e[t]);
+        for (int t = 0; t < NT; ++t) hand_around(next[t], e[t]);
         load_scales(min(c0 + 4, chunks - 1), next);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -427,13 +439,13 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(kda_mx4_linear_args 
     }
 }
 
-template <typename T, int MT, int NT, int SPLIT, int SPAN>
+template <typename T, int MT, int NT, int SPLIT>
 void launch_rows(const kda_mx4_linear_args& a, hipStream_t stream) {
     const dim3 grid(static_cast<unsigned>((a.N + 16 * NT - 1) / (16 * NT)), static_cast<unsigned>((a.M + 16 * MT - 1) / (16 * MT)));
     if (a.K % 128 == 0 && reinterpret_cast<uintptr_t>(a.w_scale) % 4 == 0)
-        rows_kernel<T, MT, NT, SPLIT, SPAN, true><<<grid, 64 * SPLIT, 0, stream>>>(a);
+        rows_kernel<T, MT, NT, SPLIT, true><<<grid, 64 * SPLIT, 0, stream>>>(a);
     else
-        rows_kernel<T, MT, NT, SPLIT, SPAN, false><<<grid, 64 * SPLIT, 0, stream>>>(a);
+        rows_kernel<T, MT, NT, SPLIT, false><<<grid, 64 * SPLIT, 0, stream>>>(a);
 }
 
 template <typename T, int WM, int WN, int NT, int STAGES>
@@ -450,15 +462,22 @@ void launch_tile(const kda_mx4_linear_args& a, hipStream_t stream) {
 // first product is most of a small call, and larger ones of larger calls, whose operands come
 // less often.  us in a graph of 24 over weights that rotate through 600 MB, fp16 (M, N, K):
 //   M x N of a tile     16x16  16x32  16x64
-//   1, 2048, 2048         3.7    4.6    6.0
-//   1, 8192, 8192        12.5   12.6   17.4
-//   16, 6144, 2048        5.7    5.2    6.4
-//   16, 28672, 8192      53.1   46.9   39.6      (one row 38.9, 37.4, 34.3)
+//   1, 2048, 2048         3.6    4.3    5.8
+//   1, 8192, 8192        11.1   11.1   16.0
+//   16, 6144, 2048        5.4    4.8    6.2
+//   16, 28672, 8192      49.5   42.2   37.4      (one row 32.9, 31.4, 30.9)
+// Up to four rows of x are one load a chunk, so small tiles cost little: the smallest as long as all workgroups are
+// under way at once (three a CU), then up to two a CU.
+//   1, 11008, 4096        8.2    9.2   10.1      (four rows 8.5, 9.8, 10.2, eight 10.3, 10.7, 10.6)
+//   1, 12288, 2048        6.1    6.6    6.8
+//   1, 14336, 4096       10.8    9.4   10.2
+//   4, 14336, 2048        7.5    6.9    7.0
+//   4, 32768, 4096       21.1   19.5   17.6
 //                       32x32  32x64  64x32  64x64  64x128  128x128
-//   32, 2048, 2048        5.6    7.5    6.0    8.6
-//   32, 28672, 8192      56.8   46.5   64.3   53.6    55.5
-//   53, 6160, 4096       14.7   13.5   12.3   16.3    28.3
-//   64, 28672, 8192      87.5   73.7   82.6   61.8    57.4
+//   32, 2048, 2048        5.5    7.2    6.0    8.6
+//   32, 28672, 8192      54.0   43.6   64.3   53.6    55.5
+//   53, 6160, 4096       13.8   12.8   11.8   16.3    28.3
+//   64, 28672, 8192      78.9   73.7   74.3   56.7    57.4
 //   128, 6144, 2048      12.0   11.7   13.2   10.3    16.3     27.7
 //   128, 16384, 4096     48.4   38.7   43.7   35.3    29.3     51.9
 // 64x128 with eight waves of 64x16, and with four of 64x32, and 128x128 with four of 64x64 (bf16
@@ -472,17 +491,20 @@ int launch_linear(const kda_mx4_linear_args& a, hipStream_t stream) {
     const auto tiles = [&](int64_t m, int64_t n) { return ((a.M + m - 1) / m) * ((a.N + n - 1) / n); };
     constexpr int64_t kCus = 256;
     if (a.M <= 16) {
-        if (tiles(16, 16) <= kCus) launch_rows<T, 1, 1, 8, 2>(a, stream);
-        else if (tiles(16, 32) <= kCus) launch_rows<T, 1, 2, 8, 2>(a, stream);
-        else launch_rows<T, 1, 4, 4, 4>(a, stream);
+        const bool few = a.M <= 4;
+        if (tiles(16, 16) <= kCus) launch_rows<T, 1, 1, 8>(a, stream);
+        else if (tiles(16, 32) <= kCus) launch_rows<T, 1, 2, 8>(a, stream);
+        else if (few && tiles(16, 16) <= 3 * kCus) launch_rows<T, 1, 1, 8>(a, stream);
+        else if (few && tiles(16, 32) <= 2 * kCus) launch_rows<T, 1, 2, 8>(a, stream);
+        else launch_rows<T, 1, 4, 4>(a, stream);
     } else if (tiles(32, 32) <= kCus) {
-        launch_rows<T, 2, 2, 8, 2>(a, stream);
+        launch_rows<T, 2, 2, 8>(a, stream);
     } else if (a.M <= 32) {
-        launch_rows<T, 2, 4, 4, 4>(a, stream);
+        launch_rows<T, 2, 4, 4>(a, stream);
     } else if (tiles(64, 32) <= kCus) {
-        launch_rows<T, 4, 2, 8, 2>(a, stream);
+        launch_rows<T, 4, 2, 8>(a, stream);
     } else if (tiles(64, 64) <= kCus) {
-        launch_rows<T, 4, 4, 8, 2>(a, stream);
+        launch_rows<T, 4, 4, 8>(a, stream);
     } else if (tiles(64, 128) <= kCus) {
         launch_tile<T, 1, 8, 1, 3>(a, stream);
     } else if (tiles(128, 128) < 6 * kCus) {             // three rounds of two a CU

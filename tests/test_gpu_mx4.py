@@ -167,6 +167,20 @@ def test_linear(kda_pkg, M, K, N, dtype):
     assert torch.equal(kda_pkg.mx4_linear(x, data, scale, bias=bias, residual=res), res + z)
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("M,N,K", [
+    (1, 600, 9248), (16, 5000, 9248), (3, 11000, 4640), (2, 14000, 4640), (9, 14000, 4640), (4, 33000, 2080),      # up to 16 rows
+    (20, 300, 9248), (20, 9000, 4640), (50, 300, 9248), (50, 5000, 9248), (50, 9000, 4640), (50, 30000, 1056)], ids=str)
+def test_linear_deep_and_wide(kda_pkg, M, N, K, dtype):
+    """Every tile of few rows at a depth at which each wave comes round again, and a last chunk of one group."""
+    data, scale, w = weight(kda_pkg, N, K, seed=8)
+    x = rand(M, K, seed=9, dtype=dtype)
+    y = kda_pkg.mx4_linear(x, data, scale)
+    check(y, x, w)
+    for _ in range(2):
+        assert torch.equal(y, kda_pkg.mx4_linear(x, data, scale))
+
+
 @pytest.mark.parametrize("M", [1, 20, 50, 130, 700])
 @pytest.mark.parametrize("K", [64, 288, 4096])
 def test_not_finite(kda_pkg, M, K):
