@@ -289,6 +289,7 @@ template <typename T, int WM, int WN, int NT, int STAGES, bool WORDS>
 struct Tile {
     static constexpr int kWaves = WM * WN, kThreads = 64 * kWaves, kM = 64 * WM, kN = 16 * NT * WN;
     static constexpr int kX = kM * 2 * kChunk, kW = kN * kChunk / 2;             // bytes of a stage
+    static constexpr int kBytes = STAGES * (kX + kW), kAcross = WN;
     static constexpr int kXLoads = kX / 1024 / kWaves, kWLoads = kW / 1024 / kWaves;
     static_assert(kXLoads * kWaves * 1024 == kX && kWLoads * kWaves * 1024 == kW, "whole loads, as many each wave");
     // Row r of tile t is W's 4 NT (r / 4) + 4 t + r % 4 of the wave's, so that a lane's outputs of one row of x, four a
@@ -297,6 +298,75 @@ struct Tile {
     // What W's row r turns its pieces by: the sixteen rows of a read are in different banks.
     static __device__ __forceinline__ int turn(int r) { return r / (4 * NT) & 3; }
 };
+
+// A tile's outputs where rows of y begin at no multiple of 8 bytes: gathered in LDS, and written from there a row's pairs on
+// end.  (3483 rows by 7693 x 224 56 us, with a store for each of a lane's values 98; a width of 7696 38.)
+template <typename T, typename K, int NT>
+__device__ __forceinline__ void through_lds(const kda_mx4_linear_args& a, const f4 (&acc)[NT][4], T* tile, int64_t m0, int64_t n0,
+                                            int rows, int cols) {
+    constexpr int kStride = K::kN + 4, kPairs = K::kN / 2 + 1;
+    static_assert(K::kM * kStride * 2 <= K::kBytes, "the tile fits where its operands were");
+    const int lane = threadIdx.x & 63, ln = lane & 15, lg = lane >> 4, wave = threadIdx.x >> 6;
+    const int row = 64 * (wave / K::kAcross) + ln, col = 16 * NT * (wave % K::kAcross) + 4 * NT * lg;
+    __syncthreads();                                     // all waves have read their last operands
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        T bias[4] = {};
+        if (a.bias && col + 4 * t < cols) Beside<T>::four(static_cast<const T*>(a.bias) + n0 + col + 4 * t, min(cols - col - 4 * t, 4), bias);
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+            T out[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) Elem<T>::st(&out[j], a.bias ? acc[t][m][j] + Elem<T>::ld(&bias[j]) : acc[t][m][j]);
+            __builtin_memcpy(tile + (row + 16 * m) * kStride + col + 4 * t, out, 8);
+        }
+    }
+    __syncthreads();
+    constexpr int kAtOnce = 8;                           // read before any is written
+    T* y = static_cast<T*>(a.y) + m0 * a.N + n0;
+    const T* res = static_cast<const T*>(a.residual) + (a.residual ? m0 * a.residual_stride + n0 : 0);
+    const uint32_t odd = a.N & 1, base = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(y) >> 1 & 1);
+    for (int i0 = threadIdx.x; i0 < rows * kPairs; i0 += kAtOnce * K::kThreads) {
+        T out[kAtOnce][2];
+        int row_of[kAtOnce], col_of[kAtOnce];            // c: a multiple of 4 bytes in y, from -1 on
+#pragma unroll
+        for (int u = 0; u < kAtOnce; ++u) {
+            const int i = i0 + u * K::kThreads, r = i / kPairs, c = 2 * (i - r * kPairs) - static_cast<int>((base + r * odd) & 1);
+            row_of[u] = min(r, K::kM - 1);
+            col_of[u] = r < rows ? c : cols;
+            const T* from = tile + row_of[u] * kStride;
+            out[u][0] = from[max(c, 0)];
+            out[u][1] = from[c + 1];
+        }
+        if (a.residual) {
+            T held[kAtOnce][2];
+#pragma unroll
+            for (int u = 0; u < kAtOnce; ++u) {
+                const T* from = res + row_of[u] * a.residual_stride;
+                if (col_of[u] >= 0 && col_of[u] < cols) held[u][0] = from[col_of[u]];
+                if (col_of[u] + 1 < cols) held[u][1] = from[col_of[u] + 1];
+            }
+#pragma unroll
+            for (int u = 0; u < kAtOnce; ++u)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) Elem<T>::st(&out[u][j], Elem<T>::ld(&held[u][j]) + Elem<T>::ld(&out[u][j]));
+        }
+#pragma unroll
+        for (int u = 0; u < kAtOnce; ++u) {
+            T* to = y + row_of[u] * a.N;
+            const int c = col_of[u];
+            if (c >= 0 && c + 1 < cols) {
+                uint32_t raw;
+                __builtin_memcpy(&raw, out[u], 4);
+                *reinterpret_cast<uint32_t*>(to + c) = raw;
+            } else if (c >= 0 && c < cols) {
+                to[c] = out[u][0];
+            } else if (c + 1 < cols) {
+                to[c + 1] = out[u][1];
+            }
+        }
+    }
+}
 
 template <typename T, int WM, int WN, int NT, int STAGES, bool WORDS>
 __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(kda_mx4_linear_args a) {
@@ -418,6 +488,10 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(kda_mx4_linear_args 
         }
     }
     landed<0>();                                         // no load is under way when the workgroup's LDS goes to another
+    if (a.N % 4 != 0) {
+        through_lds<T, K>(a, acc, reinterpret_cast<T*>(buf), m0, n0, last_m + 1, last_n + 1);
+        return;
+    }
 #pragma unroll
     for (int m = 0; m < 4; ++m) {
         const int64_t row = m0 + 64 * wm + 16 * m + ln, n = n0 + 16 * NT * wn + 4 * NT * lg;

@@ -181,6 +181,21 @@ def test_linear_deep_and_wide(kda_pkg, M, N, K, dtype):
         assert torch.equal(y, kda_pkg.mx4_linear(x, data, scale))
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("M,N,K", [(5000, 5003, 96), (4999, 5002, 64), (700, 2001, 160), (129, 6405, 288), (65, 8198, 32)], ids=str)
+def test_linear_odd_widths(kda_pkg, M, N, K, dtype):
+    """Rows of outputs that begin at any multiple of two bytes, in every tile of many rows."""
+    data, scale, w = weight(kda_pkg, N, K, seed=50)
+    x, bias = rand(M, K, seed=51, dtype=dtype), rand(N, seed=52, dtype=dtype)
+    res = rand(M, N + 3, seed=53, dtype=dtype, std=3.0)[:, 1:N + 1]
+    y = kda_pkg.mx4_linear(x, data, scale)
+    check(y, x, w)
+    z = kda_pkg.mx4_linear(x, data, scale, bias=bias)
+    check(z, x, w, bias)
+    assert torch.equal(kda_pkg.mx4_linear(x, data, scale, residual=res), res + y)
+    assert torch.equal(kda_pkg.mx4_linear(x, data, scale, bias=bias, residual=res), res + z)
+
+
 @pytest.mark.parametrize("M", [1, 20, 50, 130, 700])
 @pytest.mark.parametrize("K", [64, 288, 4096])
 def test_not_finite(kda_pkg, M, K):
