@@ -346,6 +346,25 @@ def test_autocast(kda_pkg):
     assert y.dtype == BF16 and torch.equal(y, kda_pkg.mx4_linear(x.to(BF16), data, scale))
 
 
+def test_outputs_are_ordinary_tensors(kda_pkg):
+    """Of torch's own memory: counted, freed, resizable, usable by autograd unless made under inference mode."""
+    data, scale, _ = weight(kda_pkg, 64, 256, seed=60)
+    x = rand(3000, 256, seed=61, dtype=F16)
+    held = torch.cuda.memory_allocated()
+    made = [kda_pkg.mx4_linear(x, data, scale), kda_pkg.mx4_dequantize(data, scale, dtype=F16), *kda_pkg.mx4_quantize(x)]
+    assert torch.cuda.memory_allocated() >= held + sum(t.numel() * t.element_size() for t in made)
+    for t in made:
+        assert t.device == x.device == t.untyped_storage().device and t.is_contiguous() and t._version == 0
+        assert not t.requires_grad and not t.is_inference() and t.untyped_storage().resizable()
+    w = made[0].detach().requires_grad_()
+    w.float().sum().backward()
+    assert torch.equal(w.grad, torch.ones_like(w))
+    with torch.inference_mode():
+        assert kda_pkg.mx4_linear(x, data, scale).is_inference()
+    del made, t, w
+    assert torch.cuda.memory_allocated() == held
+
+
 @pytest.mark.parametrize("bias", [False, True])
 def test_module(kda_pkg, bias):
     lin = torch.nn.Linear(256, 70, bias=bias).to(DEV, F16)
