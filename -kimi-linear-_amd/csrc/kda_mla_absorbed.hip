@@ -33,9 +33,12 @@
 // are 32 channels of a key, so a scale is one operand of the conversion that widens them (in fp16,
 // which holds fewer powers, it multiplies the group's products instead).  In the value product a
 // wave's channels are of one group, so as in 8 bits the scale enters through the exponent, each
-// wave for its own: a wave has its own maximum and denominator, and so has a part of a sequence
-// for each group.  A transposed read gives a lane sixteen keys of a channel, the window's
-// quarter of its lane group.  The arithmetic, and not the bytes, is most of a window: 386 vector
+// wave for its own: a wave has its own maximum M of the sums s' + log2 scale.  The denominator
+// knows no scales, which may lie 2^187 apart: a lane sums 2^s' of the keys whose scores it
+// forms, and a segment ends with its output, 2^M / denominator times what was summed.  Where a
+// row's largest score D is far from zero, fp32 holds no such sums and a score no scale's exponent beside
+// it: then the segment is gone over again with scores less D.  A transposed read gives a lane sixteen
+// keys of a channel, the window's quarter of its lane group.  The arithmetic, and not the bytes, is most of a window: 386 vector
 // operations before the scales went into the conversions, sums were rescaled only where there is a new
 // maximum, load offsets became constants and masks were only applied where there is one, about 290 after.
 //
@@ -61,19 +64,25 @@ constexpr int kGroup = 128;       // latent channels of a 4-bit cache's scale
 constexpr int WAVES = 4, kThreads = 64 * WAVES;
 
 // Workspace: for every slot (a workgroup's part of a row tile's sequence) the
-// rows' sums, [16][R] fp32, and their (maximum, denominator), in 4 bits for each group
-// of 128 channels; for every row tile the first and last workgroup that has a part of it.
+// rows' sums, [16][R] fp32, and their (maximum, denominator), in 4 bits the rows' outputs in
+// place of the sums, times kOutRoom and kDenRoom; for every row tile the first and last workgroup that has a part of it.
 struct Workspace {
     float* o;
     float2* ml;
     int2* span;
 };
+// A row's output is below 2^130 and its denominator, against its largest score, at most 2^30: with this off both, no sum of
+// their products overflows.
+constexpr float kOutRoom = 0x1p-4f, kDenRoom = 0x1p-30f;
+// Rows whose largest score is further from zero count from that: 2^96 2^30 is still a number, and what ends below
+// 2^-126 is 2^-30 of the largest.
+constexpr float kAway = 96.f;
 __host__ __device__ inline int64_t slots(int64_t groups, int64_t tiles) { return groups + tiles; }
 __host__ __device__ inline Workspace carve(void* p, int64_t n_slots, int64_t R) {
     Workspace w;
     w.o = static_cast<float*>(p);
     w.ml = reinterpret_cast<float2*>(w.o + n_slots * kRows * R);
-    w.span = reinterpret_cast<int2*>(w.ml + n_slots * kRows * (R / kGroup));
+    w.span = reinterpret_cast<int2*>(w.ml + n_slots * kRows);
     return w;
 }
 
@@ -136,6 +145,7 @@ __device__ __forceinline__ void landed() { asm volatile("s_waitcnt vmcnt(0)" :::
 template <typename T, int BITS, int R, int P>
 struct Kernel {
     static constexpr bool F8 = BITS == 8, F4 = BITS == 4;
+    static constexpr bool kApart = F4;                          // the denominator apart from the scales
     static constexpr int D = R + P, kWindow = kUnit * WAVES, kSteps = D / 32, kScore = kWindow + 4;
     static constexpr int kTiles = R / 16 / WAVES;               // 16-channel tiles of a wave
     static constexpr int ES = BITS == 16 ? 2 : 1, RB = R * BITS / 8, PB = P * BITS / 8;   // bytes (of a stride's unit, a row)
@@ -153,7 +163,8 @@ struct Kernel {
         char buf[2][kBuffer];            // [kWindow][R], [WAVES][kPosUnit], scales
         float s[kRows][kScore];
         float inv[F8 ? kWindow : 4];
-        float e[F4 ? kScales : 1][F4 ? kWindow : 4], e_inv[F4 ? kScales : 1][F4 ? kWindow : 4];    // log2 of the groups' scales, and 1 / scale
+        float e[kApart ? kScales : 1][kApart ? kWindow : 4];     // log2 of the groups' scales
+        float2 den[kApart ? WAVES : 1][kRows];                   // each wave's keys: largest score, and their sum
     };
 
     // Where piece c of row r lies: of the latent, with r = r0 + x, r0 a multiple of the rows of a load and x
@@ -232,6 +243,7 @@ struct Kernel {
         uint4 q[kSteps];
         f4 o[kTiles];
         float top, sum;
+        float most, from;        // apart: the largest score less what they count from, 0 or D
     };
     // Channels of step k that lane group lg has: in 8 bits a 16-byte piece is two steps', in 4 bits four steps'.
     static __device__ __forceinline__ int channel(int k, int lg) {
@@ -327,10 +339,7 @@ struct Kernel {
                     s[i] = fmaf(x, 0.f, x);      // an infinity is a scale's NaN
                 }
             }
-            if (lg < kScales) {
-                sh.e[lg][kUnit * wave + ln] = byte == 255 ? __builtin_nanf("") : static_cast<float>(byte - 127);
-                sh.e_inv[lg][kUnit * wave + ln] = __uint_as_float(byte == 254 ? 0x400000u : static_cast<uint32_t>(254 - byte) << 23);   // (2^-127)
-            }
+            if (lg < kScales) sh.e[lg][kUnit * wave + ln] = byte == 255 ? __builtin_nanf("") : static_cast<float>(byte - 127);
         } else {
             stay();
             f4 acc{}, odd{};
@@ -352,11 +361,35 @@ struct Kernel {
     static __device__ __forceinline__ int at(int k, int lg) { return F4 ? 16 * lg + 8 * k : 32 * k + 8 * lg; }
 
     static __device__ __forceinline__ void rescale(State& st, float alpha) {
-        st.sum *= alpha;
 #pragma unroll
         for (int i = 0; i < kTiles; ++i)
 #pragma unroll
             for (int e = 0; e < 4; ++e) st.o[i][e] *= alpha;
+    }
+
+    // What the lane's own scores add to the denominator.
+    static __device__ __forceinline__ void count(State& st, const f4& s) {
+        st.most = fmaxf(st.most, fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) st.sum += __builtin_amdgcn_exp2f(s[i]);
+    }
+
+    // A window's scores plus log2 of the scales of the wave's channels, and the largest of a lane's.
+    static __device__ __forceinline__ float scaled(const Shared& sh, int wave, int ln, int lg,
+                                                   float (&x)[kWindow / 32][8]) {
+        float mx = kNoMax;
+#pragma unroll
+        for (int k = 0; k < kWindow / 32; ++k) {
+            const f4* from = reinterpret_cast<const f4*>(&sh.s[ln][at(k, lg)]);
+            const f4* more = reinterpret_cast<const f4*>(&sh.e[kScales * wave / WAVES][at(k, lg)]);
+            const f4 s[2] = {from[0], from[1]}, e[2] = {more[0], more[1]};
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                x[k][i] = s[i / 4][i % 4] + e[i / 4][i % 4];
+                mx = fmaxf(mx, x[k][i]);
+            }
+        }
+        return mx;
     }
 
     // A window at keys j0..; its rows are in `buf`, the next window's are asked for into `next`.
@@ -376,34 +409,36 @@ struct Kernel {
             for (int i = 0; i < 4; ++i)
                 if (key + i > limit) s[i] = -INFINITY;
         }
+        if constexpr (kApart) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[i] -= st.from;
+        }
         *reinterpret_cast<f4*>(&sh.s[ln][kUnit * wave + 4 * lg]) = s;
         lds_barrier();
 
         uint4 p[kWindow / 32];
         float x[kWindow / 32][8], mx = kNoMax;
+        if constexpr (kApart) {
+            count(st, s);
+        } else {
 #pragma unroll
-        for (int k = 0; k < kWindow / 32; ++k) {
-            const f4* from = reinterpret_cast<const f4*>(&sh.s[ln][at(k, lg)]);
-            f4 lo4 = from[0], hi4 = from[1];
-            if constexpr (F4) {                  // each wave against its own channels' scales
-                const f4* more = reinterpret_cast<const f4*>(&sh.e[kScales * wave / WAVES][at(k, lg)]);
-                const f4 e0 = more[0], e1 = more[1];
+            for (int k = 0; k < kWindow / 32; ++k) {
+                const f4* from = reinterpret_cast<const f4*>(&sh.s[ln][at(k, lg)]);
+                const f4 lo4 = from[0], hi4 = from[1];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) lo4[e] += e0[e], hi4[e] += e1[e];
-            }
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                x[k][e] = lo4[e];
-                x[k][4 + e] = hi4[e];
-                mx = fmaxf(mx, fmaxf(lo4[e], hi4[e]));
+                for (int e = 0; e < 4; ++e) {
+                    x[k][e] = lo4[e];
+                    x[k][4 + e] = hi4[e];
+                    mx = fmaxf(mx, fmaxf(lo4[e], hi4[e]));
+                }
             }
         }
         float alpha = 1.f;
-        if constexpr (F4) {
+        if constexpr (kApart) {
             // Later windows mostly hold no new maximum, and leave the sums as they are.  (In bf16 the maximum might lag
             // by 2^8 as well, but a largest weight of 1 has no rounding, and where it is most of the softmax that
             // shows: 64 sequences of up to 8192 tokens 1.8e-3 off, with the lag 2.1e-3, in the same time.)
-            mx = reference<T>(lanegroup4_max(mx));
+            mx = reference<T>(lanegroup4_max(scaled(sh, wave, ln, lg, x)));
             if (__any(mx > st.top)) {
                 mx = fmaxf(st.top, mx);
                 rescale(st, __builtin_amdgcn_exp2f(st.top - mx));
@@ -419,22 +454,20 @@ struct Kernel {
 #pragma unroll
         for (int k = 0; k < kWindow / 32; ++k) {
             f4 inv[2];
-            if constexpr (F8 || F4) {
-                const f4* from = reinterpret_cast<const f4*>(F4 ? &sh.e_inv[kScales * wave / WAVES][at(k, lg)] : &sh.inv[at(k, lg)]);
+            if constexpr (F8) {
+                const f4* from = reinterpret_cast<const f4*>(&sh.inv[at(k, lg)]);
                 inv[0] = from[0];
                 inv[1] = from[1];
             }
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 x[k][e] = __builtin_amdgcn_exp2f(x[k][e] - mx);
-                part = F8 || F4 ? fmaf(x[k][e], inv[e / 4][e % 4], part) : part + x[k][e];
+                if constexpr (!kApart) part = F8 ? fmaf(x[k][e], inv[e / 4][e % 4], part) : part + x[k][e];
             }
             p[k] = uint4{Act<T>::pair(x[k][0], x[k][1]), Act<T>::pair(x[k][2], x[k][3]), Act<T>::pair(x[k][4], x[k][5]),
                          Act<T>::pair(x[k][6], x[k][7])};
         }
-        if constexpr (F4) {
-            st.sum += part;
-        } else {
+        if constexpr (!kApart) {
             st.sum = fmaf(st.sum, alpha, part);
 #pragma unroll
             for (int i = 0; i < kTiles; ++i)
@@ -526,18 +559,48 @@ struct Kernel {
         State st;
 #pragma unroll
         for (int k = 0; k < kSteps; ++k) st.q[k] = *reinterpret_cast<const uint4*>(qs + ln * kQStride + channel(k, lg));
+        st.from = 0.f;
+        float den, norm;
+        for (bool again = false;; again = true) {
 #pragma unroll
-        for (int i = 0; i < kTiles; ++i) st.o[i] = f4{0.f, 0.f, 0.f, 0.f};
-        st.top = kNoMax;
-        st.sum = 0.f;
-        landed();
-        lds_barrier();
-        for (int j0 = lo; j0 < hi; j0 += 2 * kWindow) {
-            window(a, b, j0, hi, limit, c, wave, lane, offs, sh.buf[0], sh.buf[1], sh, st);
-            if (j0 + kWindow < hi)
-                window(a, b, j0 + kWindow, hi, limit, c, wave, lane, offs, sh.buf[1], sh.buf[0], sh, st);
+            for (int i = 0; i < kTiles; ++i) st.o[i] = f4{0.f, 0.f, 0.f, 0.f};
+            st.top = st.most = kNoMax;
+            st.sum = 0.f;
+            landed();
+            lds_barrier();
+            for (int j0 = lo; j0 < hi; j0 += 2 * kWindow) {
+                window(a, b, j0, hi, limit, c, wave, lane, offs, sh.buf[0], sh.buf[1], sh, st);
+                if (j0 + kWindow < hi)
+                    window(a, b, j0 + kWindow, hi, limit, c, wave, lane, offs, sh.buf[1], sh.buf[0], sh, st);
+            }
+            if constexpr (kApart) {
+                const float most = lanegroup4_max(st.most), sum = lanegroup4_sum(st.sum);
+                if (lg == 0) sh.den[wave][ln] = float2{most, sum};
+                lds_barrier();
+                float all = kNoMax;
+                den = 0.f;
+#pragma unroll
+                for (int w = 0; w < WAVES; ++w) {
+                    const float2 part = sh.den[w][ln];
+                    all = fmaxf(all, part.x);
+                    den += part.y;
+                }
+                if (!again && __any(fabsf(all) > kAway && all > kNoMax)) {       // the same in every wave
+                    st.from = fabsf(all) > kAway ? all : 0.f;
+                    load(a, b, lo + kUnit * wave, hi, wave, lane, sh.buf[0]);
+                    continue;
+                }
+                const bool none = all == kNoMax;
+                den = none ? 0.f : den * __builtin_amdgcn_exp2f(-all);           // against the largest score
+                norm = none ? 0.f : (whole ? 1.f : kOutRoom) * __builtin_amdgcn_exp2f(st.top - all) / den;
+                st.top = none ? kNoMax : st.from + all;
+                den *= kDenRoom;
+            } else {
+                den = lanegroup4_sum(st.sum);
+                norm = den == 0.f ? 0.f : 1.f / den;
+            }
+            break;
         }
-        const float den = lanegroup4_sum(st.sum), norm = den == 0.f ? 0.f : 1.f / den;
         const int ch = 16 * kTiles * wave + 4 * lg;
         if (whole) {
             if (m0 + ln >= rows) return;
@@ -549,10 +612,14 @@ struct Kernel {
         } else {
             float* out = ws.o + (slot * kRows + ln) * R + ch;
 #pragma unroll
-            for (int i = 0; i < kTiles; ++i) *reinterpret_cast<f4*>(out + 16 * i) = st.o[i];
-            constexpr int kPerGroup = WAVES / kScales;
-            if (wave % kPerGroup == 0 && lg == 0)
-                ws.ml[(slot * kScales + wave / kPerGroup) * kRows + ln] = float2{st.top, den};
+            for (int i = 0; i < kTiles; ++i) {
+                if constexpr (kApart) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) st.o[i][e] *= norm;
+                }
+                *reinterpret_cast<f4*>(out + 16 * i) = st.o[i];
+            }
+            if (wave == 0 && lg == 0) ws.ml[slot * kRows + ln] = float2{st.top, den};
         }
     }
 };
@@ -668,9 +735,9 @@ __global__ __launch_bounds__(kThreads, BITS < 16 ? 2 : 1) void absorbed_kernel(k
 // The parts of one row's sequence joined: grid (row tiles, their rows, R / 4 /
 // LANES), LANES lanes on 4 channels each and 256 / LANES groups of them on every
 // so-manieth part, whose sums meet in LDS, in an order that the lengths alone decide.
-// scales: the channel groups that have a maximum and a denominator of their own.
-template <typename T, int LANES>
-__global__ __launch_bounds__(256) void join_kernel(kda_mla_absorbed_args a, int rts, int groups, int scales) {
+// APART: the parts are outputs, to be weighted with their denominators.
+template <typename T, int LANES, bool APART>
+__global__ __launch_bounds__(256) void join_kernel(kda_mla_absorbed_args a, int rts, int groups) {
     const int64_t v = blockIdx.x, b = v / rts, nv = a.B * rts;
     const int rows = static_cast<int>(a.T * a.H), m = static_cast<int>(v - b * rts) * kRows + blockIdx.y;
     if (m >= rows) return;
@@ -680,8 +747,7 @@ __global__ __launch_bounds__(256) void join_kernel(kda_mla_absorbed_args a, int 
     int2 span = ws.span[v];                      // (asked for with the length; unwritten where that is zero)
     if (tokens(a.lengths, b, a.S) == 0) span = int2{0, -1};
     if (span.x == span.y) return;                // one workgroup had it all, and wrote the result
-    const int per = kRows * scales, own = scales > 1 ? c / kGroup : 0;
-    const float2* ml = ws.ml + v * per + own * kRows + blockIdx.y;
+    const float2* ml = ws.ml + v * kRows + blockIdx.y;
     const float* o = ws.o + (v * kRows + blockIdx.y) * a.R + c;
     float top = kNoMax, den = 0.f;
     f4 r{};
@@ -693,7 +759,7 @@ __global__ __launch_bounds__(256) void join_kernel(kda_mla_absorbed_args a, int 
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) {
             const int at_g = min(g + i * kJoinGroups, span.y);
-            x[i] = ml[at_g * per];
+            x[i] = ml[at_g * kRows];
             y[i] = *reinterpret_cast<const f4*>(o + static_cast<int64_t>(at_g) * kRows * a.R);
         }
         float now = top;
@@ -709,31 +775,31 @@ __global__ __launch_bounds__(256) void join_kernel(kda_mla_absorbed_args a, int 
         for (int e = 0; e < 4; ++e) r[e] *= f0;
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) {
-            const float f = x[i].y == 0.f ? 0.f : __builtin_amdgcn_exp2f(x[i].x - now);
+            float f = x[i].y == 0.f ? 0.f : __builtin_amdgcn_exp2f(x[i].x - now);
             den = fmaf(f, x[i].y, den);
+            if constexpr (APART) f *= x[i].y;
 #pragma unroll
             for (int e = 0; e < 4; ++e) r[e] = fmaf(f, y[i][e], r[e]);
         }
     }
     __shared__ f4 sums[kJoinGroups][LANES];
-    constexpr int kStats = LANES > 32 ? LANES / 32 : 1;          // channel groups of the lanes
-    __shared__ float2 stats[kJoinGroups][kStats];
+    __shared__ float2 stats[kJoinGroups];
     sums[group][at] = r;
-    if (at % 32 == 0) stats[group][at / 32] = float2{top, den};
+    if (at == 0) stats[group] = float2{top, den};
     __syncthreads();
     if (group != 0) return;
     const int n = min(kJoinGroups, span.y - span.x + 1);
-    for (int g = 0; g < n; ++g) top = fmaxf(top, stats[g][at / 32].x);
+    for (int g = 0; g < n; ++g) top = fmaxf(top, stats[g].x);
     den = 0.f;
     r = f4{};
     for (int g = 0; g < n; ++g) {
-        const float w = __builtin_amdgcn_exp2f(stats[g][at / 32].x - top);
-        den = fmaf(w, stats[g][at / 32].y, den);
+        const float w = __builtin_amdgcn_exp2f(stats[g].x - top);
+        den = fmaf(w, stats[g].y, den);
         const f4 y = sums[g][at];
 #pragma unroll
         for (int e = 0; e < 4; ++e) r[e] = fmaf(w, y[e], r[e]);
     }
-    const float norm = den == 0.f ? 0.f : 1.f / den;
+    const float norm = den == 0.f ? 0.f : (APART ? 1.f / kOutRoom : 1.f) / den;
     *reinterpret_cast<uint2*>(static_cast<T*>(a.o) + (b * rows + m) * a.R + c) =
         uint2{Act<T>::pair(r[0] * norm, r[1] * norm), Act<T>::pair(r[2] * norm, r[3] * norm)};
 }
@@ -766,11 +832,11 @@ int launch(const kda_mla_absorbed_args& a, hipStream_t stream) {
         absorbed_kernel<T, BITS, R, P><<<groups, kThreads, 0, stream>>>(a, rts, false);
         // many rows have few parts each, and few rows may have many
         const dim3 grid(static_cast<unsigned>(nv), kRows);
-        constexpr int scales = Kernel<T, BITS, R, P>::kScales;
+        constexpr bool apart = Kernel<T, BITS, R, P>::kApart;
         if (nv >= 32)
-            join_kernel<T, R / 4><<<grid, 256, 0, stream>>>(a, rts, groups, scales);
+            join_kernel<T, R / 4, apart><<<grid, 256, 0, stream>>>(a, rts, groups);
         else
-            join_kernel<T, 16><<<dim3(grid.x, grid.y, R / 64), 256, 0, stream>>>(a, rts, groups, scales);
+            join_kernel<T, 16, apart><<<dim3(grid.x, grid.y, R / 64), 256, 0, stream>>>(a, rts, groups);
     }
     return hipGetLastError() == hipSuccess ? KDA_OK : KDA_ERR_LAUNCH;
 }
@@ -797,7 +863,7 @@ int launch_rank(const kda_mla_absorbed_args& a, hipStream_t stream) {
 int64_t mla_absorbed_workspace_bytes(int64_t B, int64_t T, int64_t H, int64_t S, int64_t R) {
     const int64_t nv = B * row_tiles(T, H);
     if (nv == 0 || !shared_form(nv, S)) return 0;
-    return slots(most_groups(nv, S), nv) * kRows * (R * 4 + 8 * (R / kGroup)) + nv * 8;
+    return slots(most_groups(nv, S), nv) * kRows * (R * 4 + 8) + nv * 8;
 }
 
 int mla_absorbed_launch(const kda_mla_absorbed_args& a, hipStream_t stream) {

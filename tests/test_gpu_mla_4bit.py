@@ -342,3 +342,58 @@ def test_refusals(kda_pkg):
             call()
             pytest.fail(f"call {i} was answered")
     assert torch.equal(raw(cache), before)
+
+
+@pytest.mark.parametrize("top", [66, 67, 100, 125])
+@pytest.mark.parametrize("B,T,H,S,R,P", [(1, 1, 16, 2, 512, 64), (2, 3, 5, 130, 128, 32), (3, 1, 16, 3000, 512, 64), (40, 1, 16, 700, 256, 0)])
+def test_absorbed_scales_far_apart(kda_pkg, B, T, H, S, R, P, top):
+    """Powers of one group from 2^-60, which rows of zeros have, to 2^125: the softmax's denominator goes by the scores
+    alone.  (Queries of zeros but where the powers are ordinary, so that scores are of like size.)"""
+    g = torch.Generator(device=DEV).manual_seed(100 + S)
+    cache, scale = quantised(rand(B, S, R + P, seed=101, dtype=torch.float32), R)
+    any_of = torch.tensor([67, 67, 127, top + 127], dtype=torch.uint8, device=DEV)
+    raw(scale)[..., :R // 128] = any_of[torch.randint(0, 4, (B, S, R // 128), generator=g, device=DEV)]
+    raw(scale)[:, :2, 0] = torch.tensor([67, top + 127], dtype=torch.uint8, device=DEV)
+    q = rand(B, T, H, R + P, seed=102, dtype=BF16, std=0.5)
+    q[..., :R] = 0
+    lengths = [max(S - 7 * b, 0) for b in range(B)]
+    held = dequantised(cache, scale, R)
+    got = kda_pkg.mla_absorbed(q, cache, i32(lengths), R, 0.1, cache_scale=scale)
+    close("o", got, *absorbed_ref(q, held, lengths, R, 0.1))
+
+
+@pytest.mark.parametrize("S", [2, 90, 2500])
+def test_absorbed_zeros_beside_large_rows(kda_pkg, S):
+    """Rows as they are appended, half of them zeros: of equal weights the output is half of the others' mean."""
+    R, P = 256, 32
+    x = rand(1, S, R + P, seed=103, dtype=BF16) * 2.0 ** 90
+    x[:, ::2] = 0
+    cache = torch.zeros(1, S, (R + P) // 2, dtype=torch.uint8, device=DEV).view(FOUR)
+    scale = torch.zeros(1, S, 8, dtype=torch.uint8, device=DEV).view(E8M0)
+    kda_pkg.mla_cache_append(x, cache, i32([0]), R, cache_scale=scale)
+    q = torch.zeros(1, 1, 4, R + P, dtype=BF16, device=DEV)
+    got = kda_pkg.mla_absorbed(q, cache, i32([S]), R, 1.0, cache_scale=scale)
+    close("o", got, *absorbed_ref(q, dequantised(cache, scale, R), [S], R, 1.0))
+
+
+@pytest.mark.parametrize("late", [False, True])
+@pytest.mark.parametrize("dtype,a,b", [(BF16, 60, 43), (BF16, -60, 43), (BF16, 60, 65), (BF16, -60, 65), (BF16, 20, 7), (BF16, 17, 0),
+                                       (BF16, -17, 0), (F16, 15, 14), (F16, -15, 14), (F16, 12, 10)], ids=str)
+@pytest.mark.parametrize("B,T,H,S", [(1, 1, 16, 100), (2, 3, 4, 1000), (70, 1, 16, 600)])
+def test_absorbed_far_scores_and_scales(kda_pkg, B, T, H, S, dtype, a, b, late):
+    """Scores of up to 2^126 in size over rows of different powers: the keys that share the largest share the weight,
+    whatever their powers.  late: the far scores come behind keys whose scores are zero."""
+    R, P = 128, 32
+    g = torch.Generator(device=DEV).manual_seed(104)
+    cache, scale = quantised(rand(B, S, R + P, seed=105, dtype=torch.float32), R)
+    lo, hi = (-10, 10) if dtype == F16 else (-50, 50)
+    raw(scale)[..., 0] = (torch.randint(lo, hi, (B, S), generator=g, device=DEV) + 127).to(torch.uint8)
+    raw(scale)[..., 1] = b + 127
+    raw(cache)[..., R // 2:] = 0
+    raw(cache)[..., R // 2] = torch.randint(2, 8, (B, S), generator=g, device=DEV, dtype=torch.uint8)       # 1 to 6
+    if late:
+        raw(cache)[:, :S // 2, R // 2] = 0
+    q = torch.zeros(B, T, H, R + P, dtype=dtype, device=DEV)
+    q[..., R] = float((1 if a > 0 else -1) * 2.0 ** abs(a))
+    got = kda_pkg.mla_absorbed(q, cache, i32([S] * B), R, 0.125, cache_scale=scale)
+    close("o", got, *absorbed_ref(q, dequantised(cache, scale, R), [S] * B, R, 0.125))
