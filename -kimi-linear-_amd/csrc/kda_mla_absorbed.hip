@@ -26,18 +26,16 @@
 // multiplies its score, and enters the value product through the exponent,
 // 2^(s' + log2 scale - M), so that P keeps its full precision in 16 bits whatever
 // the scales' size (in fp16 down to 2^-29 of the largest: reference).  M is then the
-// largest of the sums, and the terms of the softmax's denominator are divided by the
-// scale again.
+// largest of those sums.  The denominator knows no scales, which may lie 2^187 apart: a lane
+// sums 2^s' of the keys whose scores it forms, and a segment ends with its output, 2^M / denominator
+// times what was summed.  Where a row's largest score D is far from zero, fp32 holds no such sums
+// and a score no scale's exponent beside it: then the segment is gone over again with scores less D.
 //
 // In 4 bits (e2m1) each 128 channels have a power of two.  The score product's pieces
 // are 32 channels of a key, so a scale is one operand of the conversion that widens them (in fp16,
 // which holds fewer powers, it multiplies the group's products instead).  In the value product a
 // wave's channels are of one group, so as in 8 bits the scale enters through the exponent, each
-// wave for its own: a wave has its own maximum M of the sums s' + log2 scale.  The denominator
-// knows no scales, which may lie 2^187 apart: a lane sums 2^s' of the keys whose scores it
-// forms, and a segment ends with its output, 2^M / denominator times what was summed.  Where a
-// row's largest score D is far from zero, fp32 holds no such sums and a score no scale's exponent beside
-// it: then the segment is gone over again with scores less D.  A transposed read gives a lane sixteen
+// wave for its own: a wave has its own maximum M.  A transposed read gives a lane sixteen
 // keys of a channel, the window's quarter of its lane group.  The arithmetic, and not the bytes, is most of a window: 386 vector
 // operations before the scales went into the conversions, sums were rescaled only where there is a new
 // maximum, load offsets became constants and masks were only applied where there is one, about 290 after.
@@ -64,7 +62,7 @@ constexpr int kGroup = 128;       // latent channels of a 4-bit cache's scale
 constexpr int WAVES = 4, kThreads = 64 * WAVES;
 
 // Workspace: for every slot (a workgroup's part of a row tile's sequence) the
-// rows' sums, [16][R] fp32, and their (maximum, denominator), in 4 bits the rows' outputs in
+// rows' sums, [16][R] fp32, and their (maximum, denominator), in 8 and 4 bits the rows' outputs in
 // place of the sums, times kOutRoom and kDenRoom; for every row tile the first and last workgroup that has a part of it.
 struct Workspace {
     float* o;
@@ -145,7 +143,7 @@ __device__ __forceinline__ void landed() { asm volatile("s_waitcnt vmcnt(0)" :::
 template <typename T, int BITS, int R, int P>
 struct Kernel {
     static constexpr bool F8 = BITS == 8, F4 = BITS == 4;
-    static constexpr bool kApart = F4;                          // the denominator apart from the scales
+    static constexpr bool kApart = BITS < 16;                   // the denominator apart from the scales
     static constexpr int D = R + P, kWindow = kUnit * WAVES, kSteps = D / 32, kScore = kWindow + 4;
     static constexpr int kTiles = R / 16 / WAVES;               // 16-channel tiles of a wave
     static constexpr int ES = BITS == 16 ? 2 : 1, RB = R * BITS / 8, PB = P * BITS / 8;   // bytes (of a stride's unit, a row)
@@ -162,8 +160,7 @@ struct Kernel {
     struct Shared {
         char buf[2][kBuffer];            // [kWindow][R], [WAVES][kPosUnit], scales
         float s[kRows][kScore];
-        float inv[F8 ? kWindow : 4];
-        float e[kApart ? kScales : 1][kApart ? kWindow : 4];     // log2 of the groups' scales
+        float e[kApart ? kScales : 1][kApart ? kWindow : 4];     // log2 of the scales
         float2 den[kApart ? WAVES : 1][kRows];                   // each wave's keys: largest score, and their sum
     };
 
@@ -256,7 +253,7 @@ struct Kernel {
         return __uint_as_float((w >> (8 * i) & 255u) << 23);
     }
 
-    // The scores of the wave's unit, keys 4 lg + i of row ln: times scale log2(e), plus log2 of an 8-bit key's scale.
+    // The scores of the wave's unit, keys 4 lg + i of row ln: times scale log2(e).
     static __device__ __forceinline__ f4 scores(const char* buf, const State& st, float c, Shared& sh, int wave, int ln,
                                                 int lg) {
         const char* row = buf + (kUnit * wave + ln) * RB;
@@ -294,13 +291,13 @@ struct Kernel {
             for (int k = 0; k < P / 32; ++k)
                 far = Act<T>::mma16(widen8<T>(tail8[k][0], tail8[k][1]), st.q[R / 32 + k], far);
             const float sl[4] = {s01[0], s01[2], s23[0], s23[2]}, sp[4] = {s01[1], s01[3], s23[1], s23[3]};
-            f4 r;
+            f4 e;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                s[i] = fmaf((lat[i] + odd[i]) * sl[i] + far[i] * sp[i], c, __builtin_amdgcn_logf(sl[i]));
-                r[i] = __builtin_amdgcn_rcpf(sl[i]);
+                s[i] = ((lat[i] + odd[i]) * sl[i] + far[i] * sp[i]) * c;
+                e[i] = __builtin_amdgcn_logf(sl[i]);
             }
-            if (ln == 0) *reinterpret_cast<f4*>(sh.inv + kUnit * wave + 4 * lg) = r;
+            if (ln == 0) *reinterpret_cast<f4*>(&sh.e[0][kUnit * wave + 4 * lg]) = e;
         } else if constexpr (F4) {
             // a piece is one key's 32 channels, so four products on end are of one group
             const uint2 own = *reinterpret_cast<const uint2*>(buf + kScaleAt + 256 * wave + 8 * ln);    // key ln's scales
@@ -437,9 +434,10 @@ struct Kernel {
         if constexpr (kApart) {
             // Later windows mostly hold no new maximum, and leave the sums as they are.  (In bf16 the maximum might lag
             // by 2^8 as well, but a largest weight of 1 has no rounding, and where it is most of the softmax that
-            // shows: 64 sequences of up to 8192 tokens 1.8e-3 off, with the lag 2.1e-3, in the same time.)
+            // shows: 64 sequences of up to 8192 tokens 1.8e-3 off, with the lag 2.1e-3, in the same time.)  In 8 bits, where
+            // a window has less to do beside, the question costs what it saves: 600 of up to 1024 44.5 us with it, 43.3.
             mx = reference<T>(lanegroup4_max(scaled(sh, wave, ln, lg, x)));
-            if (__any(mx > st.top)) {
+            if (F8 || __any(mx > st.top)) {
                 mx = fmaxf(st.top, mx);
                 rescale(st, __builtin_amdgcn_exp2f(st.top - mx));
                 st.top = mx;
@@ -453,16 +451,10 @@ struct Kernel {
         float part = 0.f;
 #pragma unroll
         for (int k = 0; k < kWindow / 32; ++k) {
-            f4 inv[2];
-            if constexpr (F8) {
-                const f4* from = reinterpret_cast<const f4*>(&sh.inv[at(k, lg)]);
-                inv[0] = from[0];
-                inv[1] = from[1];
-            }
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 x[k][e] = __builtin_amdgcn_exp2f(x[k][e] - mx);
-                if constexpr (!kApart) part = F8 ? fmaf(x[k][e], inv[e / 4][e % 4], part) : part + x[k][e];
+                if constexpr (!kApart) part += x[k][e];
             }
             p[k] = uint4{Act<T>::pair(x[k][0], x[k][1]), Act<T>::pair(x[k][2], x[k][3]), Act<T>::pair(x[k][4], x[k][5]),
                          Act<T>::pair(x[k][6], x[k][7])};
@@ -587,7 +579,10 @@ struct Kernel {
                 }
                 if (!again && __any(fabsf(all) > kAway && all > kNoMax)) {       // the same in every wave
                     st.from = fabsf(all) > kAway ? all : 0.f;
-                    load(a, b, lo + kUnit * wave, hi, wave, lane, sh.buf[0]);
+                    // (unknown to be the first load's: its addresses would be kept for this, in 14 registers more than there are)
+                    int first = lo, own = lane;
+                    asm volatile("" : "+v"(first), "+v"(own));
+                    load(a, b, __builtin_amdgcn_readfirstlane(first) + kUnit * wave, hi, wave, own, sh.buf[0]);
                     continue;
                 }
                 const bool none = all == kNoMax;

@@ -966,3 +966,43 @@ def test_append_8bit_scale_of_all_ones(kda_pkg, k):
                              norm_weight=w, eps=0.0)
     assert sc[0, 0, 0].item() == (2 - 2.0 ** -23) * 2.0 ** k
     assert cache[0, 0, :4].float().tolist() == [448.0, 2.0 ** -9, -2.0 ** -9, 0.0]
+
+
+# ---- an 8-bit cache's scales ------------------------------------------------
+
+@pytest.mark.parametrize("top", [66, 70, 100, 115])
+@pytest.mark.parametrize("B,T,H,S,R,P", [(1, 1, 16, 2, 512, 64), (2, 3, 5, 130, 128, 32), (3, 1, 16, 3000, 512, 64), (40, 1, 16, 700, 256, 64)])
+def test_absorbed_8bit_scales_far_apart(kda_pkg, B, T, H, S, R, P, top):
+    """Scales from 2^-60, which rows of zeros have, to 2^115: the softmax's denominator goes by the scores alone."""
+    g = torch.Generator(device=DEV).manual_seed(110 + S)
+    rows = rand(B, S, R + P, seed=111, dtype=torch.float32)
+    size = torch.tensor([0.0, 0.0, 1.0, 2.0 ** (top + 7)], device=DEV)[torch.randint(0, 4, (B, S), generator=g, device=DEV)]
+    size[:, 0], size[:, 1] = 0.0, 2.0 ** (top + 7)
+    rows[..., :R] *= size[..., None]
+    cache, scale = quantised(rows, R)
+    q = rand(B, T, H, R + P, seed=112, dtype=BF16, std=0.5)
+    q[..., :R] = 0
+    lengths = [max(S - 7 * b, 0) for b in range(B)]
+    got = kda_pkg.mla_absorbed(q, cache, i32(lengths), R, 0.1, cache_scale=scale)
+    close("o", got, *absorbed_ref(q, dequantised(cache, scale, R), lengths, R, 0.1))
+
+
+@pytest.mark.parametrize("late", [False, True])
+@pytest.mark.parametrize("dtype,a,b", FAR, ids=lambda x: str(x)[6:] if isinstance(x, torch.dtype) else str(x))
+@pytest.mark.parametrize("B,T,H,S", [(1, 1, 16, 100), (2, 3, 4, 1000), (70, 1, 16, 600)])
+def test_absorbed_8bit_far_scores_and_scales(kda_pkg, B, T, H, S, dtype, a, b, late):
+    """Scores of up to 2^126 in size over rows of different latent scales: the keys that share the largest share the
+    weight, whatever their scales.  late: the far scores come behind keys whose scores are zero."""
+    R, P = 128, 32
+    q = torch.zeros(B, T, H, R + P, dtype=dtype, device=DEV)
+    q[..., R] = float((1 if a > 0 else -1) * 2.0 ** abs(a))
+    rows = rand(B, S, R + P, seed=113, dtype=torch.float32)
+    span = 6 if dtype == F16 else 40
+    rows[..., :R] *= torch.exp2(rand(B, S, 1, seed=114, dtype=torch.float32).clamp(-1, 1) * span)
+    rows[..., R:] = 0
+    rows[..., R] = (steps((B, S), 1) * 2.0 ** b).float()
+    if late:
+        rows[:, :S // 2, R] = 0
+    cache, scale = quantised(rows, R)
+    got = kda_pkg.mla_absorbed(q, cache, i32([S] * B), R, 1.0, cache_scale=scale)
+    close("o", got, *absorbed_ref(q, dequantised(cache, scale, R), [S] * B, R, 1.0))
