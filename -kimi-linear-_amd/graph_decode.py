@@ -72,7 +72,10 @@ class KdaGraphedDecoder:
     (in place, so the graph keeps reading valid memory) and recaptures if a
     buffer had to be reallocated (new dtype or shape) or a parameter is another
     tensor than at the capture.  After updating weights between two
-    ``step`` calls of one generation, call :meth:`refresh_weights`.
+    ``step`` calls of one generation, call :meth:`refresh_weights`.  Until one
+    of the two, ``step`` runs with the tensors of the capture, which the decoder
+    keeps: replacing a layer's weights (``quantize_mx4_``, say) frees the old ones
+    with the next capture.
     """
 
     def __init__(self, layers: Sequence[KimiDeltaAttention | LatentAttention], residual: bool = True, warmup_iters: int = 3):
@@ -85,22 +88,25 @@ class KdaGraphedDecoder:
         self.graph: torch.cuda.CUDAGraph | None = None
         self.static_states: list[dict] | None = None
         self._B = None
-        self._wbufs = None          # addresses of the fused weights the graph reads
+        self._wbufs = None          # addresses of the weights the graph reads
+        self._kept = None           # and the weights, which a layer may let go of before the next capture
 
-    def _weight_buffers(self):
-        """Addresses of all that a captured step reads of the layers: their parameters, weights in 4 bits, and what is
-        made of them."""
-        bufs = [tuple(p.data_ptr() for p in self.layers.parameters()), tuple(p.data_ptr() for p in self.layers.buffers())]
+    def _weights(self):
+        """All that a captured step reads of the layers: their parameters, weights in 4 bits, and what is made of them."""
+        groups = [list(self.layers.parameters()), list(self.layers.buffers())]
         for layer in self.layers:
             if isinstance(layer, LatentAttention):
-                bufs.append(tuple(layer._weight_buffers()))
+                groups.append(list(layer._up_weights()) if layer._absorbs() else [])
                 continue
-            w, b = layer._input_weight()
-            a_log, dt_bias = layer._gate_params()
-            four = layer._input_weight4() if layer._in_mx4() else ()
-            bufs.append((w.data_ptr(), b.data_ptr() if b is not None else 0, a_log.data_ptr(), dt_bias.data_ptr(),
-                         *(t.data_ptr() for t in four if t is not None)))
-        return bufs
+            groups.append([*layer._input_weight(), *layer._gate_params(), *(layer._input_weight4() if layer._in_mx4() else ())])
+        return [[t.detach() for t in g if t is not None] for g in groups]
+
+    @staticmethod
+    def _addresses(groups):
+        return [tuple(t.data_ptr() for t in g) for g in groups]
+
+    def _weight_buffers(self):
+        return self._addresses(self._weights())
 
     @torch.no_grad()
     def refresh_weights(self) -> None:
@@ -223,7 +229,8 @@ class KdaGraphedDecoder:
             self._step()
         self._restore(snap)
         torch.cuda.synchronize()
-        self._wbufs = self._weight_buffers()
+        self._kept = self._weights()
+        self._wbufs = self._addresses(self._kept)
 
     # ------------------------------------------------------------ public API
     @torch.no_grad()

@@ -131,10 +131,6 @@ class LatentAttention(nn.Module):
         """Whether ``kv_up`` is just the product with its weight, which the absorbed form splits."""
         return _plain_weight(self.kv_up, *(() if x is None else (x,))) is not None
 
-    def _weight_buffers(self):
-        """What a captured step reads beside the parameters."""
-        return [w.data_ptr() for w in self._up_weights()] if self._absorbs() else []
-
     # ------------------------------------------------------------ the cache
     def new_state(self, B: int, device, dtype) -> dict:
         """An empty state for B sequences; of normal tensors under inference mode too, so that a later call

@@ -283,3 +283,33 @@ def test_hooks_on_quantised_projections(kda_pkg):
     want = layer(x)
     layer.o_proj.register_forward_hook(lambda m, a, out: 2 * out)
     assert torch.equal(layer(x), 2 * want)
+
+
+@torch.no_grad()
+def test_a_capture_keeps_its_weights(kda_pkg):
+    """Layers turned to 4 bits, or given other parameters, after a capture: until the next one a step runs with what was
+    captured, whose memory nothing else gets."""
+    from kimi_linear_amd.graph_decode import KdaGraphedDecoder
+    x = torch.randn(1, 20, 256, device=DEV).half()
+    layers = [kda_layer(kda_pkg, F16, seed=3), latent_layer(kda_pkg, F16, seed=4), kda_layer(kda_pkg, F16, seed=5)]
+    dec, same = KdaGraphedDecoder(layers), KdaGraphedDecoder([copy.deepcopy(m) for m in layers])
+    for d in (dec, same):
+        d.prefill(x[:, :10])
+    assert torch.equal(dec.step(x[:, 10:11]), same.step(x[:, 10:11]))
+    sizes = {t.untyped_storage().nbytes() for m in layers for t in m.parameters()}
+    layers[0].quantize_mx4_()
+    layers[1].quantize_mx4_()
+    layers[1].kv_up.weight = torch.nn.Parameter(torch.randn_like(layers[1].kv_up.weight))
+    layers[2].o_proj = torch.nn.Linear(256, 256, bias=False, device=DEV, dtype=F16)
+    for m in layers[::2]:
+        m.refresh_fused_weight()
+    torch.cuda.synchronize()
+    others = [torch.full((n // 2,), float("nan"), dtype=F16, device=DEV) for n in sizes for _ in range(40)]
+    for t in range(11, 15):
+        assert torch.equal(dec.step(x[:, t:t + 1]), same.step(x[:, t:t + 1]))
+    fresh = KdaGraphedDecoder(layers)
+    for d in (dec, fresh):
+        d.prefill(x[:, :15])
+    for t in range(15, 20):
+        assert torch.equal(dec.step(x[:, t:t + 1]), fresh.step(x[:, t:t + 1]))
+    assert len(others) > 0
