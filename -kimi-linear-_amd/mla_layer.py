@@ -135,14 +135,16 @@ class LatentAttention(nn.Module):
     def new_state(self, B: int, device, dtype) -> dict:
         """An empty state for B sequences; of normal tensors under inference mode too, so that a later call
         outside it can go on with the state."""
-        D, bits = self.rank + self.position_dim, self.cache_bits
-        kept, scales = {16: (dtype, None), 8: (torch.float8_e4m3fn, (2, torch.float32)),
-                        4: (torch.float4_e2m1fn_x2, (8, torch.float8_e8m0fnu))}[bits]
+        D, S = self.rank + self.position_dim, self.max_tokens
         with torch.inference_mode(False):
-            return {"latent": torch.empty(B, self.max_tokens, D // 2 if bits == 4 else D, device=device, dtype=kept),
-                    "scale": None if scales is None else torch.empty(B, self.max_tokens, scales[0], device=device,
-                                                                     dtype=scales[1]),
-                    "lengths": torch.zeros(B, dtype=torch.int32, device=device), "tokens": 0}
+            if self.cache_bits == 4:         # (allocated as bytes: in torch's deterministic mode these types have no fill)
+                latent = torch.empty(B, S, D // 2, device=device, dtype=torch.uint8).view(torch.float4_e2m1fn_x2)
+                scale = torch.empty(B, S, 8, device=device, dtype=torch.uint8).view(torch.float8_e8m0fnu)
+            else:
+                eight = self.cache_bits == 8
+                latent = torch.empty(B, S, D, device=device, dtype=torch.float8_e4m3fn if eight else dtype)
+                scale = torch.empty(B, S, 2, device=device, dtype=torch.float32) if eight else None
+            return {"latent": latent, "scale": scale, "lengths": torch.zeros(B, dtype=torch.int32, device=device), "tokens": 0}
 
     def _room(self, state, T):
         held, most = state["tokens"], state["latent"].shape[1]

@@ -313,3 +313,27 @@ def test_a_capture_keeps_its_weights(kda_pkg):
     for t in range(15, 20):
         assert torch.equal(dec.step(x[:, t:t + 1]), fresh.step(x[:, t:t + 1]))
     assert len(others) > 0
+
+
+@torch.no_grad()
+def test_deterministic_mode(kda_pkg):
+    """Where torch fills new memory: prompts, steps and captures are what they are without."""
+    from kimi_linear_amd.graph_decode import KdaGraphedDecoder
+    x = torch.randn(2, 24, 256, device=DEV).half()
+    layers = stack(kda_pkg, F16)
+
+    def run():
+        dec = KdaGraphedDecoder(layers)
+        out = [dec.prefill(x[:, :20]).clone()]
+        out += [dec.step(x[:, t:t + 1]).clone() for t in range(20, 24)]
+        data, scale = kda_pkg.mx4_quantize(x)
+        return [*out, kda_pkg.mx4_dequantize(data, scale, dtype=F16), layers[1](x, use_cache=True)[0]]
+
+    want = run()
+    was = torch.are_deterministic_algorithms_enabled(), torch.is_deterministic_algorithms_warn_only_enabled()
+    torch.use_deterministic_algorithms(True, warn_only=True)         # (a library's product may have no such form)
+    try:
+        got = run()
+    finally:
+        torch.use_deterministic_algorithms(was[0], warn_only=was[1])
+    assert all(torch.equal(a, b) for a, b in zip(got, want))

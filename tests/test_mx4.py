@@ -161,3 +161,21 @@ def test_module(kda_pkg):
     half = other.to(torch.bfloat16)                       # the packed weight is no number to convert
     assert torch.equal(half.weight, mod.weight) and half.bias.dtype == torch.bfloat16
     assert "in_features=64" in repr(mod)
+
+
+@pytest.mark.parametrize("cache_dtype", [None, torch.float8_e4m3fn, FOUR])
+def test_new_state_in_deterministic_mode(kda_pkg, cache_dtype):
+    """In torch's deterministic mode new memory is filled, which is not there for every type."""
+    layer = kda_pkg.LatentAttention(kda_pkg.latent_attn_config(hidden_size=64, num_heads=1, head_dim=64, position_dim=32, rank=128,
+                                                               max_tokens=6, cache_dtype=cache_dtype))
+    was = torch.are_deterministic_algorithms_enabled()
+    torch.use_deterministic_algorithms(True)
+    try:
+        state = layer.new_state(2, "cpu", torch.float16)
+    finally:
+        torch.use_deterministic_algorithms(was)
+    other = layer.new_state(2, "cpu", torch.float16)
+    for name in ("latent", "scale", "lengths"):
+        a, b = state[name], other[name]
+        assert (a is None and b is None) or (a.shape == b.shape and a.dtype == b.dtype and a.is_contiguous()), name
+    assert state["latent"].dtype == (cache_dtype or torch.float16) and state["latent"].shape == (2, 6, 80 if cache_dtype == FOUR else 160)
