@@ -286,7 +286,8 @@ class KimiDeltaAttention(nn.Module):
 
     def _input_weight4(self):
         """The q, k and v projections in 4 bits as one: ``(data, scale, bias or None)``, cached and refilled like
-        :meth:`_input_weight`."""
+        :meth:`_input_weight`.  For modules as they are made: with a hook, a forward of their own or a subclass
+        among them the modules are called."""
         mods = self._input_mods()[:3]
         bufs = [m.weight for m in mods] + [m.weight_scale for m in mods] + [m.bias for m in mods if m.bias is not None]
         key = _native.host().params_key(bufs)
@@ -444,7 +445,13 @@ class KimiDeltaAttention(nn.Module):
         B, T, d = x.shape
         rows = B * T
         few = rows <= 64 and not has_torch_function((x,))
-        four = _linear(x, *self._input_weight4(), None, None) if self._in_mx4() else None      # q, k and v
+        four = None                  # q, k and v where they are in 4 bits: joined, unless a module does more than its product
+        if self._in_mx4():
+            mods = self._input_mods()[:3]
+            if all(map(_plain_mx4, mods)) and not has_torch_function((x,)):
+                four = torch.split(_linear(x, *self._input_weight4(), None, None), [m.out_features for m in mods], dim=-1)
+            else:
+                four = [m(x) for m in mods]
         y = None
         if few and b is None and _few_rows(rows, d, w.shape[0]):
             y = _native.host().linear(x, w, None, None)
@@ -453,7 +460,7 @@ class KimiDeltaAttention(nn.Module):
         (gk_down, gk_up, *_), (og_down, og_up, *_) = self.gk_proj, self.og_proj
         wide, small = (H * K, H * K, H * V), (H, gk_down.out_features, og_down.out_features)
         if four is not None:
-            q_in, k_in, v_in = torch.split(four, wide, dim=-1)
+            q_in, k_in, v_in = four
             beta_logit, gk_low, og_low = torch.split(y, small, dim=-1)
         else:
             q_in, k_in, v_in, beta_logit, gk_low, og_low = torch.split(y, wide + small, dim=-1)

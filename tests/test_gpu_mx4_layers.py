@@ -337,3 +337,42 @@ def test_deterministic_mode(kda_pkg):
     finally:
         torch.use_deterministic_algorithms(was[0], warn_only=was[1])
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@torch.no_grad()
+def test_hooks_on_quantised_inputs(kda_pkg):
+    """A hook, another forward or a subclass in the place of a q, k or v projection in 4 bits is called too."""
+    from kimi_linear_amd.graph_decode import KdaGraphedDecoder
+
+    class Doubled(kda_pkg.Mx4Linear):
+        def forward(self, x):
+            return 2 * super().forward(x)
+
+    def subclass(layer, name):
+        old = getattr(layer, name)
+        new = Doubled(old.in_features, old.out_features, old.bias is not None, device=DEV, dtype=F16)
+        new.load_state_dict(old.state_dict())
+        setattr(layer, name, new)
+
+    def forward(layer, name):
+        m = getattr(layer, name)
+        m.forward = lambda x: 2 * type(m).forward(m, x)
+
+    kinds = [lambda layer, name: getattr(layer, name).register_forward_hook(lambda m, a, out: 2 * out),
+             lambda layer, name: getattr(layer, name).register_forward_pre_hook(lambda m, a: (2 * a[0],)), forward, subclass]
+    x = torch.randn(2, 80, 256, device=DEV).half()
+    for i, change in enumerate(kinds):
+        layer = kda_layer(kda_pkg, F16, seed=20, proj_bias=i == 2, conv_bias=i != 1).quantize_mx4_()
+        want = copy.deepcopy(layer)
+        plain = layer(x)
+        change(layer, "in_proj_v")
+        want.in_proj_v.weight_scale.add_(1)                  # the same as a product twice as large
+        if want.in_proj_v.bias is not None:
+            want.in_proj_v.bias.mul_(2)
+        assert torch.equal(layer(x), want(x)) and not torch.equal(layer(x), plain)
+        got, ref = cached(layer, x, (70, 1, 1))[0], cached(want, x, (70, 1, 1))[0]
+        assert torch.equal(got, ref)
+        decs = [KdaGraphedDecoder([m]) for m in (layer, want)]
+        for d in decs:
+            d.prefill(x[:, :9])
+        assert torch.equal(decs[0].step(x[:, 9:10]), decs[1].step(x[:, 9:10]))
