@@ -376,3 +376,27 @@ def test_hooks_on_quantised_inputs(kda_pkg):
         for d in decs:
             d.prefill(x[:, :9])
         assert torch.equal(decs[0].step(x[:, 9:10]), decs[1].step(x[:, 9:10]))
+
+
+@torch.no_grad()
+def test_refreshed_joined_weights(kda_pkg):
+    """Bytes, scales and biases written past the version counters are what a layer runs with after a refresh: the
+    same as a layer that has joined nothing yet."""
+    from kimi_linear_amd.graph_decode import KdaGraphedDecoder
+    x = torch.randn(2, 12, 256, device=DEV).half()
+    for i, name in enumerate(("weight", "weight_scale", "bias")):
+        layer = kda_layer(kda_pkg, F16, seed=30 + i, proj_bias=True).quantize_mx4_()
+        dec = KdaGraphedDecoder([layer])
+        dec.prefill(x[:, :10])
+        before, stepped = layer(x), dec.step_eager(x[:, 10:11]).clone()
+        t = getattr(layer.in_proj_k, name).data
+        t.copy_(torch.randint(0, 256, t.shape, device=DEV, dtype=torch.uint8) if name == "weight" else t + 1)
+        new = copy.deepcopy(layer)
+        new._w4cat = None
+        dec.refresh_weights()
+        assert torch.equal(layer(x), new(x)) and not torch.equal(layer(x), before), name
+        assert layer._w4cat[1].data_ptr() in dec._wbufs[2]                          # refilled in place, as captured
+        other = KdaGraphedDecoder([new])
+        for d in (dec, other):
+            d.prefill(x[:, :10])
+        assert torch.equal(dec.step(x[:, 10:11]), other.step(x[:, 10:11])) and not torch.equal(dec.output_static, stepped)
