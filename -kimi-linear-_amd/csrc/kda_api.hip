@@ -295,7 +295,6 @@ constexpr int64_t kMx4Depth = int64_t{1} << 22;
 int kda_mx4_linear_fwd(const kda_mx4_linear_args* a, void* stream) {
     if (a == nullptr) return KDA_ERR_NULL_POINTER;
     if (a->M < 0 || a->N < 0 || a->K <= 0 || a->K > kMx4Depth || a->M > INT32_MAX || a->N > INT32_MAX) return KDA_ERR_BAD_SHAPE;
-    if ((a->M + 63) / 64 > 65535) return KDA_ERR_BAD_SHAPE;
     if (a->dtype != KDA_DTYPE_F16 && a->dtype != KDA_DTYPE_BF16) return KDA_ERR_BAD_DTYPE;
     if (a->K % 32 != 0) return KDA_ERR_UNSUPPORTED;
     if (a->M == 0 || a->N == 0) return KDA_OK;

@@ -642,7 +642,18 @@ __global__ __launch_bounds__(256) void dequantize_kernel(kda_mx4_convert_args a,
 }  // namespace
 
 int mx4_linear_launch(const kda_mx4_linear_args& a, hipStream_t stream) {
-    return a.dtype == KDA_DTYPE_F16 ? launch_linear<_Float16>(a, stream) : launch_linear<bf16_t>(a, stream);
+    // rows in pieces that a grid's second dimension (65535) reaches with the smallest tiles of many rows
+    constexpr int64_t kMost = int64_t{65535} * 64;
+    for (int64_t m = 0; m < a.M; m += kMost) {
+        kda_mx4_linear_args p = a;
+        p.M = min(a.M - m, kMost);
+        p.x = static_cast<const char*>(a.x) + 2 * m * a.x_stride;
+        p.y = static_cast<char*>(a.y) + 2 * m * a.N;
+        if (a.residual) p.residual = static_cast<const char*>(a.residual) + 2 * m * a.residual_stride;
+        const int status = a.dtype == KDA_DTYPE_F16 ? launch_linear<_Float16>(p, stream) : launch_linear<bf16_t>(p, stream);
+        if (status != KDA_OK) return status;
+    }
+    return KDA_OK;
 }
 
 int mx4_quantize_launch(const kda_mx4_convert_args& a, hipStream_t stream) {

@@ -376,3 +376,23 @@ def test_module(kda_pkg, bias):
     with torch.inference_mode():
         made = kda_pkg.Mx4Linear.from_linear(lin)
     assert torch.equal(made(x), mod(x)) and not made.weight.is_inference()
+
+
+@pytest.mark.parametrize("K,N,dtype", [(32, 8, BF16), (64, 5, F16)])
+def test_linear_most_rows(kda_pkg, K, N, dtype):
+    """More rows than one launch's grid reaches in its second dimension, and the rows about that border."""
+    data, scale, w = weight(kda_pkg, N, K, seed=70)
+    border = 65535 * 64
+    M = border + 200
+    x = rand(1, K, seed=71, dtype=dtype).expand(M, K).contiguous()
+    at = torch.tensor([0, 1, 5000, border - 1, border, border + 1, border + 130, M - 1], device=DEV)
+    x[at] = rand(len(at), K, seed=72, dtype=dtype)
+    res, bias = torch.ones(M, N + 3, dtype=dtype, device=DEV)[:, :N], rand(N, seed=73, dtype=dtype)
+    y = kda_pkg.mx4_linear(x, data, scale, bias=bias, residual=res)
+    z = kda_pkg.mx4_linear(x[at], data, scale, bias=bias)
+    check(z, x[at], w, bias)
+    assert torch.equal(y[at], res[at] + z)
+    rest = torch.ones(M, dtype=torch.bool, device=DEV)
+    rest[at] = False
+    same = kda_pkg.mx4_linear(x[2:3], data, scale, bias=bias) + 1
+    assert torch.equal(y[rest], same.expand(M - len(at), N))
