@@ -238,7 +238,8 @@ def mla_absorbed(q, cache, lengths, rank, scale, cache_scale=None):
 
     ``lengths [B]`` counts a sequence's tokens with the T new ones, which are
     its last (append them first); cache rows from there on are never read.  A
-    row that sees no key (an idle slot, or ``lengths[b] < T``) gives zeros.  A
+    row that sees no key (an idle slot, or ``lengths[b] < T``) gives zeros.  A value of a 4-bit cache is taken in q's
+    type by a score in bf16, where one past the type's range (scales of 2^126 and 2^127) is infinity.  A
     cached row that is not finite may reach the up to T - 1 queries before its own.
     ``scale`` is that of the expanded form, ``(N + P) ** -0.5``; ``cache_scale``
     of the tokens as :func:`mla_cache_append` writes it (positive, from 2^-60).

@@ -93,7 +93,8 @@ def mx4_quantize(w):
 
 def mx4_dequantize(data, scale, dtype=torch.bfloat16):
     """The matrix ``[.., K]`` that ``data`` and ``scale`` stand for, each value rounded once to ``dtype`` (fp16 or
-    bf16; exact in bf16 for scales from 2^-125, in fp16 from 2^-23 to 2^13)."""
+    bf16; exact in bf16 for scales from 2^-125 to 2^125, in fp16 from 2^-23 to 2^13).  Past ``dtype``'s range that is
+    infinity, which :func:`mx4_quantize` makes of finite values beyond 1.75 2^127 (fp16: 1.75 2^15): taken as 2^128 (2^16)."""
     try:
         out = _native.host().mx4_dequantize(data, scale, dtype)
     except (TypeError, AttributeError):
@@ -113,8 +114,8 @@ def mx4_dequantize(data, scale, dtype=torch.bfloat16):
 def mx4_linear(x, weight, weight_scale, bias=None, residual=None):
     """``x [.., K]`` times the transpose of a weight ``[N, K]`` in 4 bits, ``[.., N]`` in x's type.
 
-    Sums are fp32, with the weight's values in x's type (exact in bf16; in fp16
-    for scales from 2^-23 to 2^13, others are rounded, which beyond fp16's range is infinity); ``bias [N]`` is
+    Sums are fp32, with the weight's values in x's type (exact in bf16 for
+    scales from 2^-125 to 2^125, in fp16 from 2^-23 to 2^13; others are rounded, which beyond the type's range is infinity); ``bias [N]`` is
     added before the one rounding.  ``residual [.., N]``: the sum of it and the
     rounded product, as a residual stream adds it.  x may have any strides;
     rows that are not 16-byte aligned are copied.  Forward only."""

@@ -633,8 +633,8 @@ int kda_mla_cache_read(const kda_mla_read_args* args, void* stream);
  * each 32 along a row a power of two, stored as its exponent + 127 (255: NaN).
  *
  * y = x W^T (+ bias) for any number of rows: sums in fp32, W's values taken in the
- * activation type (exact in bf16, and in fp16 for powers from 2^-23 to 2^13;
- * others are rounded), the result rounded once.  residual: y = residual + that
+ * activation type (exact in bf16 for powers from 2^-125 to 2^125, in fp16 from 2^-23
+ * to 2^13; others are rounded, beyond the type's range to infinity), the result rounded once.  residual: y = residual + that
  * rounded result.  K a multiple of 32; x rows and w 16-byte aligned; other calls
  * return KDA_ERR_UNSUPPORTED.  y overlaps no input. */
 typedef struct kda_mx4_linear_args {

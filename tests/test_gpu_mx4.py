@@ -396,3 +396,24 @@ def test_linear_most_rows(kda_pkg, K, N, dtype):
     rest[at] = False
     same = kda_pkg.mx4_linear(x[2:3], data, scale, bias=bias) + 1
     assert torch.equal(y[rest], same.expand(M - len(at), N))
+
+
+@pytest.mark.parametrize("dtype,top", [(BF16, 125), (F16, 13)])
+def test_exact_scales(kda_pkg, dtype, top):
+    """Where a value times its scale is exact, and what is beyond: from the largest values whose group's power
+    passes that, infinity."""
+    least = -125 if dtype == BF16 else -23
+    scale = (torch.arange(least, top + 1, device=DEV) + 127).to(torch.uint8)[:, None]
+    data = torch.arange(16, dtype=torch.uint8, device=DEV).mul(17).expand(scale.shape[0], 16).contiguous()
+    back = kda_pkg.mx4_dequantize(data, scale, dtype=dtype)
+    assert torch.equal(back.double(), values(data, scale))
+    w = torch.full((2, 32), torch.finfo(dtype).max, dtype=dtype, device=DEV)
+    w[1] = 1.75 * 2.0 ** (top + 2)                           # 7 of the largest such power: taken as 6
+    data, scale = kda_pkg.mx4_quantize(w)
+    assert raw(scale).flatten().tolist() == [top + 1 + 127, top + 127]
+    back = kda_pkg.mx4_dequantize(data, scale, dtype=dtype)
+    assert (back[0] == float("inf")).all() and (back[1].double() == 6 * 2.0 ** top).all()
+    x = torch.zeros(1, 32, dtype=dtype, device=DEV)
+    x[0, 0] = 2.0 ** -10
+    y = kda_pkg.mx4_linear(x, data, scale)[0]
+    assert y[0].isnan() and y[1].item() == 6 * 2.0 ** (top - 10)         # (x's zeros times infinity; one product)
