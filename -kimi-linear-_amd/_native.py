@@ -14,7 +14,7 @@ from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "libkda_hip.so"
 HOST_PATH = Path(__file__).resolve().parent / "_kda_host.so"     # csrc/host_binding.cpp
-ABI_VERSION = 19
+ABI_VERSION = 20
 
 DTYPE_F32 = 0
 DTYPE_F16 = 1
@@ -243,6 +243,7 @@ EXPORTED_SYMBOLS = ("kda_chunkwise_fwd", "kda_recurrent_fwd", "kda_chunkwise_fwd
                     "kda_output_bwd", "kda_output_bwd_workspace_size", "kda_mla_expanded_fwd", "kda_mla_expanded_bwd",
                     "kda_mla_expanded_workspace_size",
                     "kda_mla_expanded_bwd_workspace_size", "kda_mla_absorbed_fwd", "kda_mla_absorbed_workspace_size",
+                    "kda_mla_absorbed_cache_workspace_size",
                     "kda_mla_cache_append", "kda_mla_cache_read", "kda_mx4_linear_fwd", "kda_mx4_quantize",
                     "kda_mx4_dequantize", "kda_status_str", "kda_abi_version")
 
@@ -329,6 +330,8 @@ def load() -> ctypes.CDLL:
         for name in ("expanded", "expanded_bwd", "absorbed"):
             getattr(lib, f"kda_mla_{name}_workspace_size").argtypes = [ctypes.c_int64] * 5
             getattr(lib, f"kda_mla_{name}_workspace_size").restype = ctypes.c_size_t
+        lib.kda_mla_absorbed_cache_workspace_size.argtypes = [ctypes.c_int64] * 5 + [ctypes.c_int32]
+        lib.kda_mla_absorbed_cache_workspace_size.restype = ctypes.c_size_t
         lib.kda_status_str.argtypes = [ctypes.c_int]
         lib.kda_status_str.restype = ctypes.c_char_p
         lib.kda_abi_version.argtypes = []

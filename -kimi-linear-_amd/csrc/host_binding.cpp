@@ -60,7 +60,7 @@ struct Fns {
     decltype(&kda_mla_expanded_bwd) mla_expanded_bwd = nullptr;
     decltype(&kda_mla_expanded_bwd_workspace_size) mla_expanded_bwd_ws = nullptr;
     decltype(&kda_mla_absorbed_fwd) mla_absorbed = nullptr;
-    decltype(&kda_mla_absorbed_workspace_size) mla_absorbed_ws = nullptr;
+    decltype(&kda_mla_absorbed_cache_workspace_size) mla_absorbed_ws = nullptr;
     decltype(&kda_mla_cache_append) mla_append = nullptr;
     decltype(&kda_mla_cache_read) mla_read = nullptr;
     decltype(&kda_mx4_linear_fwd) mx4_linear = nullptr;
@@ -101,7 +101,7 @@ void bind(const py::dict& addr, const py::object& stream_fn, const py::object& e
     take(fn.mla_expanded_bwd, addr, "kda_mla_expanded_bwd");
     take(fn.mla_expanded_bwd_ws, addr, "kda_mla_expanded_bwd_workspace_size");
     take(fn.mla_absorbed, addr, "kda_mla_absorbed_fwd");
-    take(fn.mla_absorbed_ws, addr, "kda_mla_absorbed_workspace_size");
+    take(fn.mla_absorbed_ws, addr, "kda_mla_absorbed_cache_workspace_size");
     take(fn.mla_append, addr, "kda_mla_cache_append");
     take(fn.mla_read, addr, "kda_mla_cache_read");
     take(fn.mx4_linear, addr, "kda_mx4_linear_fwd");
@@ -835,7 +835,7 @@ py::object mla_absorbed(const Tensor& q, const Tensor& cache, const Tensor& leng
         a.scale = static_cast<float>(scale);
         a.dtype = code(q);
         a.cache_dtype = cache_code(cache);
-        const size_t bytes = fn.mla_absorbed_ws(a.B, a.T, a.H, a.S, a.R);
+        const size_t bytes = fn.mla_absorbed_ws(a.B, a.T, a.H, a.S, a.R, a.cache_dtype);
         Tensor ws;
         if (bytes > 0) {
             ws = fresh({static_cast<int64_t>(bytes)}, at::kByte, q);

@@ -89,7 +89,7 @@ int64_t mla_expanded_workspace_bytes(int64_t B, int64_t T, int64_t S, int64_t H,
 int mla_expanded_launch(const kda_mla_expanded_args& a, hipStream_t stream);
 int64_t mla_expanded_bwd_workspace_bytes(int64_t B, int64_t T, int64_t S, int64_t H, int64_t P);
 int mla_expanded_bwd_launch(const kda_mla_expanded_bwd_args& a, hipStream_t stream);
-int64_t mla_absorbed_workspace_bytes(int64_t B, int64_t T, int64_t H, int64_t S, int64_t R);
+int64_t mla_absorbed_workspace_bytes(int64_t B, int64_t T, int64_t H, int64_t S, int64_t R, int32_t cache_dtype);
 int mla_absorbed_launch(const kda_mla_absorbed_args& a, hipStream_t stream);
 int mla_append_launch(const kda_mla_append_args& a, hipStream_t stream);
 int mla_read_launch(const kda_mla_read_args& a, hipStream_t stream);

@@ -809,7 +809,9 @@ int row_tiles(int64_t T, int64_t H) { return static_cast<int>((T * H + kRows - 1
 // 59.5 / 47.6, 16 of 8192 at 64 heads 34.7 / 32.3, but 64 of 16 to 1024 15.7 / 17.4, one of 65536 20.3 / 23.7.
 constexpr int64_t kGroups = 256;
 static_assert(kGroups > kCut);
-int64_t most_groups(int64_t nv, int64_t S) { return nv * ((S + 63) / 64) >= 8 * kGroups ? 2 * kGroups : kGroups; }
+int64_t most_groups(int64_t nv, int64_t S, bool four) {
+    return four && nv * ((S + 63) / 64) >= 8 * kGroups ? 2 * kGroups : kGroups;
+}
 // Whether the units are shared among the workgroups: where one workgroup a row
 // tile would leave CUs idle or wait for the longest sequence.  us, shared /
 // one a row tile, lengths spread evenly: 300 sequences up to 4096 tokens 158 /
@@ -823,7 +825,7 @@ int launch(const kda_mla_absorbed_args& a, hipStream_t stream) {
     if (!shared_form(nv, a.S)) {
         absorbed_kernel<T, BITS, R, P><<<static_cast<unsigned>(nv), kThreads, 0, stream>>>(a, rts, true);
     } else {
-        const int groups = static_cast<int>(BITS == 4 ? most_groups(nv, a.S) : kGroups);
+        const int groups = static_cast<int>(most_groups(nv, a.S, BITS == 4));
         absorbed_kernel<T, BITS, R, P><<<groups, kThreads, 0, stream>>>(a, rts, false);
         // many rows have few parts each, and few rows may have many
         const dim3 grid(static_cast<unsigned>(nv), kRows);
@@ -855,10 +857,10 @@ int launch_rank(const kda_mla_absorbed_args& a, hipStream_t stream) {
 
 }  // namespace
 
-int64_t mla_absorbed_workspace_bytes(int64_t B, int64_t T, int64_t H, int64_t S, int64_t R) {
+int64_t mla_absorbed_workspace_bytes(int64_t B, int64_t T, int64_t H, int64_t S, int64_t R, int32_t cache_dtype) {
     const int64_t nv = B * row_tiles(T, H);
     if (nv == 0 || !shared_form(nv, S)) return 0;
-    return slots(most_groups(nv, S), nv) * kRows * (R * 4 + 8) + nv * 8;
+    return slots(most_groups(nv, S, cache_dtype == KDA_DTYPE_E2M1), nv) * kRows * (R * 4 + 8) + nv * 8;
 }
 
 int mla_absorbed_launch(const kda_mla_absorbed_args& a, hipStream_t stream) {

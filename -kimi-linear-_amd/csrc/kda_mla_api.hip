@@ -121,7 +121,12 @@ int kda_mla_expanded_bwd(const kda_mla_expanded_bwd_args* g, void* stream) {
 
 size_t kda_mla_absorbed_workspace_size(int64_t B, int64_t T, int64_t H, int64_t S, int64_t R) {
     if (!sizes_ok(B, T, S, H) || (R != 128 && R != 256 && R != 512)) return 0;
-    return static_cast<size_t>(kda::mla_absorbed_workspace_bytes(B, T, H, S, R));
+    return static_cast<size_t>(kda::mla_absorbed_workspace_bytes(B, T, H, S, R, KDA_DTYPE_E2M1));
+}
+
+size_t kda_mla_absorbed_cache_workspace_size(int64_t B, int64_t T, int64_t H, int64_t S, int64_t R, int32_t cache_dtype) {
+    if (!sizes_ok(B, T, S, H) || (R != 128 && R != 256 && R != 512) || !(act(cache_dtype) || scaled(cache_dtype))) return 0;
+    return static_cast<size_t>(kda::mla_absorbed_workspace_bytes(B, T, H, S, R, cache_dtype));
 }
 
 int kda_mla_absorbed_fwd(const kda_mla_absorbed_args* a, void* stream) {
@@ -135,7 +140,7 @@ int kda_mla_absorbed_fwd(const kda_mla_absorbed_args* a, void* stream) {
     const bool few = scaled(a->cache_dtype);
     if (!a->q || !a->o || !a->lengths) return KDA_ERR_NULL_POINTER;
     if (a->S > 0 && (!a->cache || (few && !a->cache_scale))) return KDA_ERR_NULL_POINTER;
-    if (!a->workspace && kda::mla_absorbed_workspace_bytes(a->B, a->T, a->H, a->S, a->R) > 0) return KDA_ERR_NULL_POINTER;
+    if (!a->workspace && kda::mla_absorbed_workspace_bytes(a->B, a->T, a->H, a->S, a->R, a->cache_dtype) > 0) return KDA_ERR_NULL_POINTER;
     if (!rows_ok(a->q, a->q_stride, 3, 2) || !rows_ok(a->cache, a->cache_stride, 2, few ? 1 : 2) || !at16(a->o) ||
         !at16(a->workspace) || !near(a->cache_stride[1]))
         return KDA_ERR_UNSUPPORTED;

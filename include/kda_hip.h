@@ -39,7 +39,7 @@
 extern "C" {
 #endif
 
-#define KDA_ABI_VERSION 19
+#define KDA_ABI_VERSION 20
 
 /* Element types accepted at the boundary. */
 typedef enum kda_dtype {
@@ -577,10 +577,12 @@ typedef struct kda_mla_absorbed_args {
     float scale;
     int32_t dtype;                 /* of q and o: KDA_DTYPE_F16 or KDA_DTYPE_BF16 */
     int32_t cache_dtype;           /* dtype, KDA_DTYPE_E4M3 or KDA_DTYPE_E2M1 */
-    void* workspace;               /* kda_mla_absorbed_workspace_size() bytes */
+    void* workspace;               /* kda_mla_absorbed_cache_workspace_size() bytes */
 } kda_mla_absorbed_args;
 
+/* Enough for a cache of any type, or for one of cache_dtype (a 4-bit one may take about twice the others'). */
 size_t kda_mla_absorbed_workspace_size(int64_t B, int64_t T, int64_t H, int64_t S, int64_t R);
+size_t kda_mla_absorbed_cache_workspace_size(int64_t B, int64_t T, int64_t H, int64_t S, int64_t R, int32_t cache_dtype);
 int kda_mla_absorbed_fwd(const kda_mla_absorbed_args* args, void* stream);
 
 /* New rows behind the cached ones: x[b, t] goes to cache row lengths[b] + t for

@@ -179,3 +179,24 @@ def test_new_state_in_deterministic_mode(kda_pkg, cache_dtype):
         a, b = state[name], other[name]
         assert (a is None and b is None) or (a.shape == b.shape and a.dtype == b.dtype and a.is_contiguous()), name
     assert state["latent"].dtype == (cache_dtype or torch.float16) and state["latent"].shape == (2, 6, 80 if cache_dtype == FOUR else 160)
+
+
+def test_absorbed_workspace_by_cache_type(native):
+    """A cache in 16 or 8 bits asks for 256 workgroups' parts at any length, one in 4 bits for 512 where it is cut into as many."""
+    size, most = native.load().kda_mla_absorbed_cache_workspace_size, native.load().kda_mla_absorbed_workspace_size
+    wide = (native.DTYPE_F16, native.DTYPE_BF16, native.DTYPE_E4M3)
+
+    def parts(groups, tiles, R):                 # rows of sums, their maximum and denominator, and the tiles' spans
+        return (groups + tiles) * 16 * (4 * R + 8) + 8 * tiles
+
+    for B, T, H, S, R in ((64, 1, 16, 8192, 512), (200, 1, 16, 4096, 256), (1, 1, 16, 600, 128), (8, 5, 20, 1501, 256), (1, 1, 16, 400, 512),
+                          (600, 1, 16, 8192, 512)):
+        tiles = B * -(-T * H // 16)
+        shared = tiles < 512 and S > 512
+        long = tiles * -(-S // 64) >= 2048
+        for t in wide:
+            assert size(B, T, H, S, R, t) == (parts(256, tiles, R) if shared else 0)
+        four = size(B, T, H, S, R, native.DTYPE_E2M1)
+        assert four == (parts(512 if long else 256, tiles, R) if shared else 0) == most(B, T, H, S, R)
+    assert size(1, 1, 16, 10000, 512, native.DTYPE_F32) == 0 and size(1, 1, 16, 10000, 512, 9) == 0
+    assert size(1, 1, 16, 10000, 500, native.DTYPE_E2M1) == 0 and size(-1, 1, 16, 10000, 512, native.DTYPE_E2M1) == 0
