@@ -300,7 +300,8 @@ struct Tile {
 };
 
 // A tile's outputs where rows of y begin at no multiple of 8 bytes: gathered in LDS, and written from there a row's pairs on
-// end.  (3483 rows by 7693 x 224 56 us, with a store for each of a lane's values 98; a width of 7696 38.)
+// end.  (3483 rows by 7693 x 224 in the largest tile 56 us, with a store for each of a lane's values 98; a width of 7696
+// 38.  In the one that it gets 45 and 32.)
 template <typename T, typename K, int NT>
 __device__ __forceinline__ void through_lds(const kda_mx4_linear_args& a, const f4 (&acc)[NT][4], T* tile, int64_t m0, int64_t n0,
                                             int rows, int cols) {
@@ -554,12 +555,24 @@ void launch_tile(const kda_mx4_linear_args& a, hipStream_t stream) {
 //   64, 28672, 8192      78.9   73.7   74.3   56.7    57.4
 //   128, 6144, 2048      12.0   11.7   13.2   10.3    16.3     27.7
 //   128, 16384, 4096     48.4   38.7   43.7   35.3    29.3     51.9
-// 64x128 with eight waves of 64x16, and with four of 64x32, and 128x128 with four of 64x64 (bf16
-// for the last two):
+// 64x128 with eight waves of 64x16, and with four of 64x32, and 128x128 with four of 64x64 (fp16):
 //   300, 6144, 2048      17.7   18.7   28.4
-//   1500, 6144, 2048     61.8   48.7   55.4
-//   4000, 6144, 2048    132.0  106.6  101.4     (the library's product of 16-bit operands 98)
-//   8192, 8192, 8192     1238    973    899     (771)
+//   1250, 6144, 2048            43.3   39.2
+//   1400, 6144, 2048            46.0   55.7
+//   2000, 6144, 2048            59.8   60.8
+//   2560, 6144, 2048            72.3   68.1
+//   2700, 6144, 2048            78.0   81.6
+//   4000, 6144, 2048     132   106.5   99.5     (the library's product of 16-bit operands 98)
+//   4200, 6144, 2048           111.5  112.3
+//   5000, 4096, 4096           167.6  159.4
+//   1000, 8192, 8192           148.4  127.8
+//   8192, 8192, 8192    1238    1021    949     (771)
+//   12000, 7696, 1024          236.0  231.1
+//   12000, 7696, 448           147.6  153.0
+//   7000, 7696, 224             61.7   67.7
+// The largest, two a CU, are faster where their rounds of 512 are full to 5/6 or more (480 and 512 tiles, 960, 1280, 1536; not
+// 528, 768, 1056 and 1584) and a tile is deep enough for its way in and out; bf16 is within 5 %.
+constexpr int64_t kDeep = 1024;
 template <typename T>
 int launch_linear(const kda_mx4_linear_args& a, hipStream_t stream) {
     const auto tiles = [&](int64_t m, int64_t n) { return ((a.M + m - 1) / m) * ((a.N + n - 1) / n); };
@@ -581,10 +594,10 @@ int launch_linear(const kda_mx4_linear_args& a, hipStream_t stream) {
         launch_rows<T, 4, 4, 8>(a, stream);
     } else if (tiles(64, 128) <= kCus) {
         launch_tile<T, 1, 8, 1, 3>(a, stream);
-    } else if (tiles(128, 128) < 6 * kCus) {             // three rounds of two a CU
-        launch_tile<T, 1, 4, 2, 2>(a, stream);
     } else {
-        launch_tile<T, 2, 2, 4, 2>(a, stream);
+        const int64_t large = tiles(128, 128), round = 2 * kCus, rounds = (large + round - 1) / round;
+        if (a.K >= kDeep && 6 * large >= 5 * round * rounds) launch_tile<T, 2, 2, 4, 2>(a, stream);
+        else launch_tile<T, 1, 4, 2, 2>(a, stream);
     }
     return hipGetLastError() == hipSuccess ? KDA_OK : KDA_ERR_LAUNCH;
 }

@@ -417,3 +417,22 @@ def test_exact_scales(kda_pkg, dtype, top):
     x[0, 0] = 2.0 ** -10
     y = kda_pkg.mx4_linear(x, data, scale)[0]
     assert y[0].isnan() and y[1].item() == 6 * 2.0 ** (top - 10)         # (x's zeros times infinity; one product)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("M,N,K", [(1400, 5003, 1056), (1401, 5002, 1024), (1399, 5016, 1152), (1281, 5441, 1024), (2500, 5121, 1088),
+                                   (2700, 6144, 1024), (1400, 5003, 992)], ids=str)
+def test_linear_large_tiles(kda_pkg, M, N, K, dtype):
+    """Products deep enough for the largest tiles, whose rounds are full (and one each that is not, and not deep enough),
+    at widths of every alignment."""
+    data, scale, w = weight(kda_pkg, N, K, seed=80)
+    x, bias = rand(M, K, seed=81, dtype=dtype), rand(N, seed=82, dtype=dtype)
+    res = rand(M, N + 3, seed=83, dtype=dtype, std=3.0)[:, 1:N + 1]
+    y = kda_pkg.mx4_linear(x, data, scale)
+    check(y, x, w)
+    z = kda_pkg.mx4_linear(x, data, scale, bias=bias)
+    check(z, x, w, bias)
+    assert torch.equal(kda_pkg.mx4_linear(x, data, scale, residual=res), res + y)
+    assert torch.equal(kda_pkg.mx4_linear(x, data, scale, bias=bias, residual=res), res + z)
+    few = kda_pkg.mx4_linear(x[-70:], data, scale)
+    check(few, x[-70:], w)
