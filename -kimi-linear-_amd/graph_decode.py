@@ -93,17 +93,23 @@ class KdaGraphedDecoder:
 
     def _weights(self):
         """All that a captured step reads of the layers: their parameters, weights in 4 bits, and what is made of them."""
-        groups = [list(self.layers.parameters()), list(self.layers.buffers())]
+        params, bufs = [], []
+        for m in self.layers.modules():
+            params.extend(m._parameters.values())
+            bufs.extend(m._buffers.values())
+        groups = [params, bufs]
         for layer in self.layers:
             if isinstance(layer, LatentAttention):
-                groups.append(list(layer._up_weights()) if layer._absorbs() else [])
+                groups.append(layer._up_weights() if layer._absorbs() else ())
                 continue
-            groups.append([*layer._input_weight(), *layer._gate_params(), *(layer._input_weight4() if layer._in_mx4() else ())])
-        return [[t.detach() for t in g if t is not None] for g in groups]
+            mods = layer._input_mods()
+            groups.append((*layer._input_weight(mods), *layer._gate_params(),
+                           *(layer._input_weight4(mods) if layer._in_mx4(mods) else ())))
+        return groups
 
     @staticmethod
     def _addresses(groups):
-        return [tuple(t.data_ptr() for t in g) for g in groups]
+        return [[0 if t is None else t.data_ptr() for t in g] for g in groups]
 
     def _weight_buffers(self):
         return self._addresses(self._weights())
@@ -229,8 +235,9 @@ class KdaGraphedDecoder:
             self._step()
         self._restore(snap)
         torch.cuda.synchronize()
-        self._kept = self._weights()
-        self._wbufs = self._addresses(self._kept)
+        weights = self._weights()
+        self._wbufs = self._addresses(weights)
+        self._kept = [t.detach() for g in weights for t in g if t is not None]
 
     # ------------------------------------------------------------ public API
     @torch.no_grad()

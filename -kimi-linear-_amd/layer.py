@@ -271,11 +271,12 @@ class KimiDeltaAttention(nn.Module):
         self._wcat = self._w4cat = None
         return self
 
-    def _in_mx4(self):
-        """Whether the q, k and v projections are in 4 bits; the other projections of x never are."""
-        mods = self._input_mods()
+    def _in_mx4(self, mods=None):
+        """Whether the q, k and v projections (of ``mods``, :meth:`_input_mods`) are in 4 bits; the other projections of x
+        never are."""
+        mods = self._input_mods() if mods is None else mods
         four = [isinstance(m, Mx4Linear) for m in mods]
-        if not any(four):
+        if True not in four:
             return False
         if four != [True, True, True, False, False, False]:
             raise KdaError("in_proj_q, in_proj_k and in_proj_v are all Mx4Linear or none of them, and beta_proj and the "
@@ -284,11 +285,11 @@ class KimiDeltaAttention(nn.Module):
             raise KdaError("in_proj_q, in_proj_k and in_proj_v all have a bias or none of them")
         return True
 
-    def _input_weight4(self):
+    def _input_weight4(self, mods=None):
         """The q, k and v projections in 4 bits as one: ``(data, scale, bias or None)``, cached and refilled like
         :meth:`_input_weight`.  For modules as they are made: with a hook, a forward of their own or a subclass
         among them the modules are called."""
-        mods = self._input_mods()[:3]
+        mods = (self._input_mods() if mods is None else mods)[:3]
         bufs = [m.weight for m in mods] + [m.weight_scale for m in mods] + [m.bias for m in mods if m.bias is not None]
         key = _native.host().params_key(bufs)
         old = self._w4cat
@@ -310,7 +311,7 @@ class KimiDeltaAttention(nn.Module):
         self._w4cat = (key, *new, [b.detach() for b in bufs])
         return tuple(new)
 
-    def _input_weight(self):
+    def _input_weight(self, mods=None):
         """The six projections of x -- q, k, v, beta and the down-projections
         of the forget gate and the output gate -- as one ``[N, d]`` weight (and
         bias), so that a step runs one GEMM over x instead of six small ones.
@@ -326,7 +327,8 @@ class KimiDeltaAttention(nn.Module):
         call :meth:`refresh_fused_weight` after them.  What was concatenated is
         kept with the cache, so that no other parameter can come to lie at an
         address of the key.  With q, k and v in 4 bits it is of the other three."""
-        mods = self._input_mods()[3 if self._in_mx4() else 0:]
+        mods = self._input_mods() if mods is None else mods
+        mods = mods[3 if self._in_mx4(mods) else 0:]
         params = [m.weight for m in mods] + [m.bias for m in mods if m.bias is not None]
         key = _native.host().params_key(params)
         if self._wcat is not None and self._wcat[0] == key:
@@ -441,17 +443,18 @@ class KimiDeltaAttention(nn.Module):
         hist = conv_cache if (use_cache and conv_cache is not None and keep > 0) else None
         convs = (self.conv_q.conv, self.conv_k.conv, self.conv_v.conv)
         H, K, V = self.num_heads, self.head_dim, self.value_head_dim
-        w, b = self._input_weight()
+        mods = self._input_mods()        # (looked up once: 2 us of an eager step's 120)
+        w, b = self._input_weight(mods)
         B, T, d = x.shape
         rows = B * T
         few = rows <= 64 and not has_torch_function((x,))
         four = None                  # q, k and v where they are in 4 bits: joined, unless a module does more than its product
-        if self._in_mx4():
-            mods = self._input_mods()[:3]
-            if all(map(_plain_mx4, mods)) and not has_torch_function((x,)):
-                four = torch.split(_linear(x, *self._input_weight4(), None, None), [m.out_features for m in mods], dim=-1)
+        if isinstance(mods[0], Mx4Linear):
+            qkv = mods[:3]
+            if all(map(_plain_mx4, qkv)) and not has_torch_function((x,)):
+                four = torch.split(_linear(x, *self._input_weight4(mods), None, None), [m.out_features for m in qkv], dim=-1)
             else:
-                four = [m(x) for m in mods]
+                four = [m(x) for m in qkv]
         y = None
         if few and b is None and _few_rows(rows, d, w.shape[0]):
             y = _native.host().linear(x, w, None, None)

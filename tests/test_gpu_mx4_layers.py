@@ -400,3 +400,25 @@ def test_refreshed_joined_weights(kda_pkg):
         for d in (dec, other):
             d.prefill(x[:, :10])
         assert torch.equal(dec.step(x[:, 10:11]), other.step(x[:, 10:11])) and not torch.equal(dec.output_static, stepped)
+
+
+@pytest.mark.parametrize("mx4", [False, True])
+@torch.no_grad()
+def test_a_step_looks_its_projections_up_once(kda_pkg, mx4):
+    """Which projections are in 4 bits is asked of modules looked up once a call, which an eager step of 120 us notices."""
+    layer = kda_layer(kda_pkg, F16)
+    if mx4:
+        layer.quantize_mx4_()
+    x = torch.randn(1, 9, 256, device=DEV).half()
+    _, state = layer(x, use_cache=True)
+    looked, made = [], layer._input_mods
+
+    def input_mods():
+        looked.append(1)
+        return made()
+
+    layer._input_mods = input_mods
+    layer.decode_step_(x[:, :1], state)
+    layer(x[:, :1], state=state, use_cache=True)
+    layer(x)
+    assert len(looked) == 3
