@@ -141,6 +141,29 @@ __device__ __forceinline__ uint2 read_tr4(const void* p) {
     return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr4_b64_v2i32((lds_i2)(reinterpret_cast<const i2*>(p))));
 }
 
+// 64 lanes' 16 (or 4) bytes each, from base + offset bytes, on end to LDS; waited
+// for by the reader (landed).  In assembly for the compiler not to wait: it takes
+// a transposed LDS read for one that may be of any load's place.  (m0 is
+// reserved: the compiler keeps nothing in it.)
+__device__ __forceinline__ uint32_t lds_address(void* p) {
+    return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) void*)(p)));
+}
+__device__ __forceinline__ void to_lds(const void* base, int offset, char* lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+                 :
+                 : "s"(lds_address(lds)), "v"(offset), "s"(base)
+                 : "memory");
+}
+__device__ __forceinline__ void word_to_lds(const void* base, int offset, char* lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2"
+                 :
+                 : "s"(lds_address(lds)), "v"(offset), "s"(base)
+                 : "memory");
+}
+// All but the wave's last N loads are there.
+template <int N>
+__device__ __forceinline__ void landed() { asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory"); }
+
 // Four neighbouring outputs, and where `low` is there what rounding took from each.
 template <typename T>
 __device__ __forceinline__ void store_out(T* out, T* low, f4 x) {

@@ -111,28 +111,6 @@ __device__ __forceinline__ void stay() { asm volatile("" ::: "memory"); }
 // A barrier for what the waves leave each other in LDS, that does not wait for loads under way as __syncthreads does.
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
-// 64 lanes' 16 (or 4) bytes each, from base + offset bytes, on end to LDS; waited
-// for by the reader (landed).  In assembly for the compiler not to wait: it takes
-// a transposed LDS read for one that may be of any load's place.  (m0 is
-// reserved: the compiler keeps nothing in it.)
-__device__ __forceinline__ uint32_t lds_address(void* p) {
-    return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) void*)(p)));
-}
-__device__ __forceinline__ void to_lds(const void* base, int offset, char* lds) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
-                 :
-                 : "s"(lds_address(lds)), "v"(offset), "s"(base)
-                 : "memory");
-}
-__device__ __forceinline__ void word_to_lds(const void* base, int offset, char* lds) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2"
-                 :
-                 : "s"(lds_address(lds)), "v"(offset), "s"(base)
-                 : "memory");
-}
-// This wave's loads into LDS are there.
-__device__ __forceinline__ void landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
-
 // Rows go straight to LDS as they are in the cache, asynchronously: two buffers,
 // the next window's rows under way while this one is worked on, none in
 // registers.  LDS rows have no padding (a load fills 1 KB on end); instead the
@@ -467,7 +445,7 @@ struct Kernel {
                 for (int e = 0; e < 4; ++e) st.o[i][e] *= alpha;
         }
         values(buf, p, wave, ln, lg, st);
-        landed();                        // the next window's
+        landed<0>();                        // the next window's
         lds_barrier();
     }
 
@@ -558,7 +536,7 @@ struct Kernel {
             for (int i = 0; i < kTiles; ++i) st.o[i] = f4{0.f, 0.f, 0.f, 0.f};
             st.top = st.most = kNoMax;
             st.sum = 0.f;
-            landed();
+            landed<0>();
             lds_barrier();
             for (int j0 = lo; j0 < hi; j0 += 2 * kWindow) {
                 window(a, b, j0, hi, limit, c, wave, lane, offs, sh.buf[0], sh.buf[1], sh, st);

@@ -15,6 +15,8 @@ namespace kda {
 namespace {
 
 using mla::Act;
+using mla::landed;
+using mla::to_lds;
 
 // b's lower half (16 lanes: even ones) in place of a's upper (odd) and the other way round.
 __device__ __forceinline__ void swap32(uint32_t& a, uint32_t& b) {
@@ -27,21 +29,7 @@ __device__ __forceinline__ void swap16(uint32_t& a, uint32_t& b) {
 }
 __device__ __forceinline__ uint32_t word(const uint4& w, int i) { return i == 0 ? w.x : i == 1 ? w.y : i == 2 ? w.z : w.w; }
 
-__device__ __forceinline__ uint32_t lds_address(void* p) {
-    return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) void*)(p)));
-}
-// 64 lanes' 16 bytes each, from base + offset bytes, on end to LDS; the reader waits for them.
-__device__ __forceinline__ void to_lds(const void* base, int offset, char* lds) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
-                 :
-                 : "s"(lds_address(lds)), "v"(offset), "s"(base)
-                 : "memory");
-}
-// All but the wave's last N loads are there.
-template <int N>
-__device__ __forceinline__ void landed() { asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory"); }
-
-// The same, which the compiler takes into account: what came before those it does not wait for again.
+// landed<N>(), which the compiler takes into account: what came before those it does not wait for again.
 template <int N>
 __device__ __forceinline__ void known_landed() {
     asm volatile("" ::: "memory");
