@@ -41,11 +41,11 @@
 // maximum, load offsets became constants and masks were only applied where there is one, about 290 after.
 //
 // At 16 heads, R=512 P=64 (a copy reaches 4.8 TB/s): B=64 of 8192 tokens 115 us
-// (5.2 TB/s), of 64 to 4096 tokens 40.5 us from HBM, in 8 bits 128 to 8192 43.5 us,
+// (5.2 TB/s), of 64 to 4096 tokens 40.6 us from HBM, in 8 bits 128 to 8192 43.8 us,
 // with 5 us of them the join; one sequence of 32768 17.8 us, in 8 bits 15.5; of 200,
 // in one workgroup, 10 us: a window is 1.5 us and the way to the first one 3.  32 heads
-// of that batch 67 us, 64 121, 128 169.  In 4 bits B=64 of 8192 tokens 54 us, of 128 to 8192
-// 35, one of 65536 20, of 200 8.6.
+// of that batch 67 us, 64 121, 128 169.  In 4 bits B=64 of 8192 tokens 48 us, of 128 to 8192
+// 33, one of 65536 20, of 200 8.7.
 #include <hip/hip_runtime.h>
 
 #include "kda_launch.h"
