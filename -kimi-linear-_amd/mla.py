@@ -27,7 +27,8 @@ Softmax weights are operands of 16 bits, off by up to half a step of the type
 (2^-8 of themselves in bf16, 2^-11 in fp16); in fp16 one below 2^-29 of its row's
 largest has fewer bits, and below 2^-40 none.  (Over an 8-bit cache that goes for a weight times its row's scale,
 in 4 bits its group's, and in bf16 nothing is left below 2^-126 of the largest.)  Scores may be of any size that fp32 holds; a
-weight is as exact as its score, to 2^-24 of that.
+weight is as exact as its score, to 2^-24 of that.  (Over 8 and 4 bits, what a workgroup has of a sequence is gone over
+twice where a row's largest score there is past 66.)
 
 HIP tensors only, fp16 or bf16 activations, no fallback: anything else raises
 :class:`KdaError`, as do calls under a trace, ``vmap`` or forward-mode differentiation.  Calls are asynchronous on torch's current stream and may be

@@ -11,6 +11,7 @@ from __future__ import annotations
 import pytest
 import torch
 from test_gpu_mla import ABSORBED, BF16, CACHE, F16, SHARED, absorbed_ref, close, half_step, i32, rand
+from test_gpu_mla import dequantised as dequantised8, quantised as quantised8
 from test_gpu_mx4 import definition, raw
 
 pytestmark = pytest.mark.gpu
@@ -397,3 +398,30 @@ def test_absorbed_far_scores_and_scales(kda_pkg, B, T, H, S, dtype, a, b, late):
     q[..., R] = float((1 if a > 0 else -1) * 2.0 ** abs(a))
     got = kda_pkg.mla_absorbed(q, cache, i32([S] * B), R, 0.125, cache_scale=scale)
     close("o", got, *absorbed_ref(q, dequantised(cache, scale, R), [S] * B, R, 0.125))
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("B,T,H,S", [(1, 1, 16, 100), (2, 3, 20, 700), (70, 1, 16, 600), (1, 2, 16, 20000), (600, 1, 4, 130)])
+def test_absorbed_scores_of_all_sizes_in_a_tile(kda_pkg, B, T, H, S, dtype, bits):
+    """Heads of one row tile whose scores are small, large and of either sign, over parts of a sequence whose scores
+    are near zero, past 66 and past 200, and powers that differ.  One channel makes the scores: products are exact."""
+    R, P = 128, 32
+    g = torch.Generator(device=DEV).manual_seed(120 + S)
+    size = torch.tensor([0.0, 1.0, -1.0, 5.0, -5.0, 10.0, -10.0, 20.0, 30.0, -40.0], dtype=torch.float64, device=DEV)
+    q = torch.zeros(B, T, H, R + P, dtype=dtype, device=DEV)
+    q[..., R] = size[torch.randint(0, len(size), (B, T, H), generator=g, device=DEV)].to(dtype)
+    rows = rand(B, S, R + P, seed=121, dtype=torch.float32) * torch.exp2(torch.randint(-8, 5, (B, S, 1), generator=g, device=DEV).float())
+    rows[..., R:] = 0
+    step = torch.tensor([1.0, 1.5, 2.0, 3.0, 4.0, 6.0], device=DEV)[torch.randint(0, 6, (B, S), generator=g, device=DEV)]
+    at = torch.arange(S, device=DEV) * 5 // S                        # fifths: far, near zero, far the other way, further, near zero
+    rows[..., R] = step * torch.tensor([1.0, 2.0 ** -6, -1.0, 2.0, 0.0], device=DEV)[at]
+    if bits == 4:
+        cache, scale = quantised(rows, R)
+        held = dequantised(cache, scale, R)
+    else:
+        cache, scale = quantised8(rows, R)
+        held = dequantised8(cache, scale, R)
+    lengths = [max(S - 3 * (b % 40), 0) for b in range(B)]
+    got = kda_pkg.mla_absorbed(q, cache, i32(lengths), R, 1.0, cache_scale=scale)
+    close("o", got, *absorbed_ref(q, held, lengths, R, 1.0))
