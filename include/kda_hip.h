@@ -563,7 +563,9 @@ int kda_mla_expanded_bwd(const kda_mla_expanded_bwd_args* args, void* stream);
  * A KDA_DTYPE_E2M1 cache holds two channels a byte, the lower half first, and has
  * eight bytes of scales a row: byte g is the exponent + 127 (at least 67; 255: NaN) of the
  * power of two for latent channels 128 g to 128 g + 127, byte R / 128 that for
- * the position part.  Its strides and its scales' are in bytes. */
+ * the position part.  Its strides and its scales' are in bytes.  Over either, a
+ * weight times its scale is an operand of 16 bits: below 2^-126 (fp16: 2^-40) of its
+ * row's (in 4 bits its group's) largest it counts in the denominator only. */
 typedef struct kda_mla_absorbed_args {
     int64_t B, T, H, S, R, P;      /* R in {128, 256, 512}; P in {0, 32, 64} */
     const void* q;                 /* [B, T, H, R+P] */
